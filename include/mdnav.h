@@ -401,6 +401,50 @@ int mdn_sim_validate_rollout(MdnSim* sim);
 int mdn_checkpoint_read_params(const char* path, MdnCheckpointHeader* header, float* actor, uint64_t actor_count,
                                float* critic, uint64_t critic_count);
 
+/* ---- Operators of recurrent policies.  No counterpart in the reference,
+ * whose policies are feed-forward.  They work on device memory of the current
+ * device, are enqueued on `stream` (a hipStream_t; NULL for the default
+ * stream) and not waited for, allocate nothing and keep nothing between
+ * calls; workspaces are the caller's.  Arguments are checked before anything
+ * is launched (MDN_E_ARG).
+ *
+ * Rows are time-major like the rollout buffers.  An MdnRows names an array
+ * [ticks][envs][heads][width] by its strides in elements (0 broadcasts an
+ * input); the width is contiguous. */
+#define MDN_F32 0u
+#define MDN_BF16 1u
+typedef struct MdnRows {
+    void* data;
+    int64_t tick, env, head;
+} MdnRows;
+
+/* The gated delta rule: per env and head a state S[k_dim][v_dim] in fp32 and
+ * per tick
+ *     S <- 0 where reset != 0
+ *     S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
+ * g is the logarithm of the decay (-inf allowed) and beta the strength of the
+ * write.  qk_heads divides heads: value head h reads query and key head
+ * h / (heads / qk_heads).  k_dim and v_dim are 1..128, ticks and envs may be
+ * 0 (the state then passes through). */
+typedef struct MdnDeltaRule {
+    uint32_t ticks, envs, qk_heads, heads, k_dim, v_dim;
+    uint32_t dtype;       /* of q, k, v and o: MDN_F32 or MDN_BF16 */
+    uint32_t gate_dtype;  /* of g and beta: MDN_F32 or dtype */
+    float scale;
+    MdnRows q, k, v, g, beta, o;      /* g and beta have width 1 */
+    const uint8_t* reset;             /* [ticks][envs] with the strides below, or NULL */
+    int64_t reset_tick, reset_env;
+    const float* state;               /* [envs][heads][k_dim][v_dim] before the first tick, or NULL (zeros) */
+    float* state_out;                 /* the same after the last tick, or NULL; may be `state` itself */
+} MdnDeltaRule;
+
+/* All ticks of a rollout.  `keep` (mdn_op_delta_rule_keep_bytes of it, or
+ * NULL) receives what the backward pass reads besides the inputs. */
+int mdn_op_delta_rule_forward(const MdnDeltaRule* rule, void* keep, uint64_t keep_bytes, void* workspace,
+                              uint64_t workspace_bytes, void* stream);
+int mdn_op_delta_rule_keep_bytes(const MdnDeltaRule* rule, uint64_t* bytes);
+int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backward, uint64_t* bytes);
+
 /* Test support, no counterpart in the reference: the kernels divide by
  * constants (plant mass and rotor time constants, the RK4 weight 6, the
  * observation scales) as (float)((double)x * (1.0 / (double)b)).  For each

@@ -16,6 +16,7 @@
 #include <string>
 #include <vector>
 
+#include "delta_rule.h"
 #include "kernel_args.h"
 #include "mdnav.h"
 #include "mdnav_host.h"
@@ -2184,6 +2185,99 @@ int mdn_navwid_write(const char* path, const MdnNavPolicyMeta* meta, const MdnSe
         std::remove(temp.c_str());
         return fail(MDN_E_ARG, std::string("cannot replace wide policy: ") + path);
     }
+    return MDN_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- operators of recurrent policies
+namespace {
+
+constexpr uint64_t kMostBlocks = 0x7fffffffull;  // of a grid
+
+uint32_t size_of(uint32_t dtype) { return dtype == MDN_BF16 ? 2u : 4u; }
+
+// Rows for a kernel; `ticks`, `envs` and `heads` bound the strides that matter.
+delta::Rows device_rows(const MdnRows& r, uint32_t size, uint32_t ticks, uint32_t envs, uint32_t heads) {
+    delta::Rows out{static_cast<char*>(r.data), r.tick, r.env, r.head, 0u};
+    const auto words = [&](int64_t stride, uint32_t count) { return count <= 1 || (stride * int64_t(size)) % 16 == 0; };
+    out.wide = reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && words(r.tick, ticks) && words(r.env, envs) && words(r.head, heads);
+    return out;
+}
+
+int delta_args(const char* name, const MdnDeltaRule* d, delta::Args* out) {
+    const std::string who = std::string(name) + ": ";
+    if (!d) return fail(MDN_E_ARG, who + "null");
+    if (d->dtype > MDN_BF16) return fail(MDN_E_ARG, who + "dtype must be MDN_F32 or MDN_BF16");
+    if (d->gate_dtype != MDN_F32 && d->gate_dtype != d->dtype) return fail(MDN_E_ARG, who + "gate_dtype must be MDN_F32 or dtype");
+    if (d->k_dim < 1 || d->k_dim > delta::MAX_DIM || d->v_dim < 1 || d->v_dim > delta::MAX_DIM)
+        return fail(MDN_E_ARG, who + "k_dim and v_dim must be 1..128");
+    if (d->heads < 1 || d->qk_heads < 1 || d->heads % d->qk_heads != 0)
+        return fail(MDN_E_ARG, who + "qk_heads must divide heads");
+    if (uint64_t(d->envs) * d->heads > kMostBlocks / 16) return fail(MDN_E_ARG, who + "too many states");
+    if (d->ticks > 0x7fffff00u) return fail(MDN_E_ARG, who + "too many ticks");
+    const bool any = d->ticks && d->envs;
+    if (any && (!d->q.data || !d->k.data || !d->v.data || !d->g.data || !d->beta.data))
+        return fail(MDN_E_ARG, who + "null rows");
+    const uint32_t size = size_of(d->dtype), T = d->ticks, N = d->envs, H = d->heads, Q = d->qk_heads;
+    delta::Args a{};
+    a.ticks = T; a.envs = N; a.qk_heads = Q; a.heads = H; a.k_dim = d->k_dim; a.v_dim = d->v_dim;
+    a.gate_f32 = d->gate_dtype == MDN_F32;
+    a.scale = d->scale;
+    a.q = device_rows(d->q, size, T, N, Q);
+    a.k = device_rows(d->k, size, T, N, Q);
+    a.v = device_rows(d->v, size, T, N, H);
+    a.o = device_rows(d->o, size, T, N, H);
+    a.g = device_rows(d->g, size, T, N, H);
+    a.beta = device_rows(d->beta, size, T, N, H);
+    a.reset = d->reset; a.reset_tick = d->reset_tick; a.reset_env = d->reset_env;
+    a.state = d->state; a.state_out = d->state_out;
+    *out = a;
+    return MDN_OK;
+}
+
+uint64_t delta_keep_bytes(const delta::Args& a) {
+    const uint64_t chunks = (uint64_t(a.ticks) + delta::CHUNK - 1) / delta::CHUNK;
+    return chunks > 1 ? (chunks - 1) * a.envs * a.heads * delta::state_tile_words(a) * sizeof(float) : 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mdn_op_delta_rule_keep_bytes(const MdnDeltaRule* rule, uint64_t* bytes) {
+    delta::Args a;
+    if (int rc = delta_args("mdn_op_delta_rule_keep_bytes", rule, &a)) return rc;
+    if (!bytes) return fail(MDN_E_ARG, "mdn_op_delta_rule_keep_bytes: null");
+    *bytes = delta_keep_bytes(a);
+    return MDN_OK;
+}
+
+int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backward, uint64_t* bytes) {
+    delta::Args a;
+    if (int rc = delta_args("mdn_op_delta_rule_workspace_bytes", rule, &a)) return rc;
+    if (!bytes) return fail(MDN_E_ARG, "mdn_op_delta_rule_workspace_bytes: null");
+    (void)backward;
+    *bytes = 0;
+    return MDN_OK;
+}
+
+int mdn_op_delta_rule_forward(const MdnDeltaRule* rule, void* keep, uint64_t keep_bytes, void* workspace,
+                              uint64_t workspace_bytes, void* stream) {
+    delta::Args a;
+    if (int rc = delta_args("mdn_op_delta_rule_forward", rule, &a)) return rc;
+    (void)workspace;
+    (void)workspace_bytes;
+    if (a.envs == 0) return MDN_OK;
+    if (a.ticks && !a.o.p) return fail(MDN_E_ARG, "mdn_op_delta_rule_forward: null rows");
+    if (keep && keep_bytes < delta_keep_bytes(a)) return fail(MDN_E_ARG, "mdn_op_delta_rule_forward: keep is too small");
+    a.chunk_states = keep && delta_keep_bytes(a) ? static_cast<float*>(keep) : nullptr;
+    const bool bf = rule->dtype == MDN_BF16;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.ticks <= 1 && !a.chunk_states)
+        HIP_TRY(delta::launch_recurrent(a, bf, st));
+    else
+        HIP_TRY(delta::launch_forward(a, bf, st));
     return MDN_OK;
 }
 

@@ -1,0 +1,268 @@
+// delta_chunk.h — what the forward and the backward pass of a chunk share:
+// its rows in LDS, its decays, and the triangular system of its ticks.
+//
+// With gamma_i = exp(g_1 + .. + g_i) inside the chunk, D_ij = gamma_i / gamma_j
+// and S the state before the chunk, the rows u_i = beta_i (v_i - S_{i-1}^T k_i)
+// that the ticks add to the state solve
+//     (1 + A) U = beta (V - gamma (K S)),   A_ij = beta_i D_ij (k_i k_j), j < i
+// and  O = scale (gamma (Q S) + (D Q K^T) U),  S' = gamma_C S + sum_j (gamma_C / gamma_j) k_j u_j^T.
+// A tick flagged as an episode's first sees none of what is before it: D is 0
+// between ticks of different episodes, gamma 0 after the first flag and
+// gamma_C / gamma_j 0 before the last.
+#ifndef MDNAV_DELTA_CHUNK_H
+#define MDNAV_DELTA_CHUNK_H
+
+#include "delta_rule.h"
+#include "delta_tiles.h"
+
+namespace delta {
+
+constexpr int C = int(CHUNK);
+constexpr int CP = C + 8;  // row of a chunk x chunk matrix in LDS
+
+// A decay this low is exp(g) = 0 in fp32; taken as the flag is, so that sums
+// of decays stay finite (-inf included).
+constexpr float NO_DECAY = -104.0f;
+
+template <class E>
+__device__ __forceinline__ float load_one(const char* p, int64_t i) {
+    return float(reinterpret_cast<const E*>(p)[i]);
+}
+__device__ __forceinline__ float load_gate(const Args& a, const Rows& r, int64_t i, bool bf) {
+    if (a.gate_f32 || !bf) return reinterpret_cast<const float*>(r.p)[i];
+    return float(reinterpret_cast<const bf16*>(r.p)[i]);
+}
+
+// Wavefront `wave`'s tiles of the state before chunk `c` >= 1.
+__device__ __forceinline__ f32x4* state_tiles(const Args& a, uint64_t seq, uint32_t c, int wave) {
+    const uint64_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
+    return reinterpret_cast<f32x4*>(a.chunk_states + (seq * (chunks - 1) + c - 1) * state_tile_words(a)) +
+           wave * ((a.k_dim + 15) / 16) * 64;
+}
+
+// ---- eight elements of a row, in registers.  WIDE: rows start at multiples
+// of 16 bytes and widths are multiples of eight elements; a piece is then
+// wholly inside its row or wholly past it, and moves in 16-byte words.
+template <class E> struct Piece { uint4 w[sizeof(E) / 2]; };
+
+// What is past the row's end or the last tick reads as 0 (`base` is then
+// some other row of the array).
+template <class E, bool WIDE>
+__device__ __forceinline__ Piece<E> load_piece(const Rows& r, int64_t base, uint32_t dim, uint32_t col, bool row_in) {
+    constexpr int W = sizeof(E) / 2;
+    Piece<E> out;
+    const E* p = reinterpret_cast<const E*>(r.p) + base;
+    if (WIDE) {
+        const bool in = row_in && col < dim;
+        const uint4* q = reinterpret_cast<const uint4*>(p + (col < dim ? col : 0u));
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            const uint4 x = q[i];
+            out.w[i] = uint4{in ? x.x : 0u, in ? x.y : 0u, in ? x.z : 0u, in ? x.w : 0u};
+        }
+    } else {
+        uint32_t word[4 * W];
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * W; i++) {
+            if (sizeof(E) == 4) {
+                const uint32_t c = col + i;
+                const uint32_t x = reinterpret_cast<const uint32_t*>(p)[c < dim ? c : 0u];
+                word[i] = row_in && c < dim ? x : 0u;
+            } else {
+                const uint32_t c = col + 2 * i;
+                const uint32_t lo = reinterpret_cast<const uint16_t*>(p)[c < dim ? c : 0u];
+                const uint32_t hi = reinterpret_cast<const uint16_t*>(p)[c + 1 < dim ? c + 1 : 0u];
+                word[i] = (row_in && c < dim ? lo : 0u) | (row_in && c + 1 < dim ? hi << 16 : 0u);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W; i++) out.w[i] = uint4{word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]};
+    }
+    return out;
+}
+template <class E, bool WIDE>
+__device__ __forceinline__ void store_piece(const Rows& r, int64_t base, uint32_t dim, uint32_t col, const Piece<E>& in) {
+    constexpr int W = sizeof(E) / 2;
+    E* p = reinterpret_cast<E*>(r.p) + base + col;
+    if (WIDE) {
+        if (col < dim)
+#pragma unroll
+            for (int i = 0; i < W; i++) reinterpret_cast<uint4*>(p)[i] = in.w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            const uint32_t word[4] = {in.w[i].x, in.w[i].y, in.w[i].z, in.w[i].w};
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                if (sizeof(E) == 4) {
+                    if (col + 4 * i + e < dim) reinterpret_cast<uint32_t*>(p)[4 * i + e] = word[e];
+                } else {
+                    const uint32_t at = 2 * (4 * i + e);
+                    if (col + at < dim) reinterpret_cast<uint16_t*>(p)[at] = uint16_t(word[e]);
+                    if (col + at + 1 < dim) reinterpret_cast<uint16_t*>(p)[at + 1] = uint16_t(word[e] >> 16);
+                }
+            }
+        }
+    }
+}
+// To a row in the order of place(); `m` is the row's start.
+__device__ __forceinline__ void piece_to_ordered(bf16* m, uint32_t col, const Piece<bf16>& in) {
+    *reinterpret_cast<uint2*>(m + place(int(col))) = uint2{in.w[0].x, in.w[0].y};
+    *reinterpret_cast<uint2*>(m + place(int(col)) + 8) = uint2{in.w[0].z, in.w[0].w};
+}
+__device__ __forceinline__ void piece_to_ordered(float* m, uint32_t col, const Piece<float>& in) {
+    *reinterpret_cast<uint4*>(m + place(int(col))) = in.w[0];
+    *reinterpret_cast<uint4*>(m + place(int(col)) + 8) = in.w[1];
+}
+template <class E>
+__device__ __forceinline__ void piece_to_lds(E* m, const Piece<E>& in) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(E) / 2); i++) reinterpret_cast<uint4*>(m)[i] = in.w[i];
+}
+template <class E>
+__device__ __forceinline__ Piece<E> piece_from_lds(const E* m) {
+    Piece<E> out;
+#pragma unroll
+    for (int i = 0; i < int(sizeof(E) / 2); i++) out.w[i] = reinterpret_cast<const uint4*>(m)[i];
+    return out;
+}
+
+// ---- decays of a chunk, in LDS
+struct Gates {
+    double sum[C];     // g_1 + .. + g_i, in 64 bits: differences of nearby sums keep their digits
+    float beta[C];
+    float before[C];   // gamma_i, 0 after a flag
+    float after[C];    // gamma_C / gamma_i, 0 before the last flag
+    int episode[C];    // flags up to and with tick i
+};
+
+struct GateRegs { float g, beta; uint32_t flag; };
+
+// Tick `t` of lane t - t0; a tick past the end adds nothing and decays nothing.
+__device__ __forceinline__ GateRegs load_gates(const Args& a, bool bf, uint32_t n, uint32_t h, int64_t t, bool in) {
+    GateRegs r{0.0f, 0.0f, 0u};
+    if (in) {
+        r.g = load_gate(a, a.g, t * a.g.tick + n * a.g.env + h * a.g.head, bf);
+        r.beta = load_gate(a, a.beta, t * a.beta.tick + n * a.beta.env + h * a.beta.head, bf);
+        r.flag = a.reset ? a.reset[t * a.reset_tick + n * a.reset_env] != 0 : 0u;
+        if (r.g < NO_DECAY) r.flag = 1u;
+    }
+    return r;
+}
+// By one wavefront, lanes 0..31 its ticks (the others are given zeros).
+__device__ __forceinline__ void put_gates(Gates& s, const GateRegs& r) {
+    const int l = int(threadIdx.x) & 63;
+    const uint32_t flags = uint32_t(__ballot(r.flag != 0));
+    const int i = l & 31;
+    const int episode = __popc(flags & (0xffffffffu >> (31 - i)));
+    const int last = __popc(flags);
+    double sum = r.flag ? 0.0 : double(r.g);
+#pragma unroll
+    for (int d = 1; d < C; d <<= 1) {
+        const double up = __shfl_up(sum, d, C);
+        if (i >= d) sum += up;
+    }
+    const double total = __shfl(sum, C - 1, C);
+    if (l < C) {
+        s.sum[i] = sum;
+        s.beta[i] = r.beta;
+        s.episode[i] = episode;
+        s.before[i] = episode == 0 ? __expf(float(sum)) : 0.0f;
+        s.after[i] = episode == last ? __expf(float(total - sum)) : 0.0f;
+    }
+}
+
+// D of a tile's entries: rows i0 + 4 (l / 16) + r, column j0 + l % 16; 0 above the diagonal.
+__device__ __forceinline__ f32x4 decay_tile(Lane l, const Gates& s, int i0, int j0) {
+    const int j = j0 + l.col;
+    const double sj = s.sum[j];
+    const int ej = s.episode[j];
+    f32x4 d;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int i = i0 + 4 * l.quad + r;
+        d[r] = (i >= j && s.episode[i] == ej) ? __expf(float(s.sum[i] - sj)) : 0.0f;
+    }
+    return d;
+}
+
+// ---- the triangular system.  X = the inverse of 1 + A for a diagonal block,
+// by substitution: lane c of each 16 has column c, rows leave in order and
+// subtract themselves from the rows below (A's column j from LDS, the same
+// address in all lanes).  `at` holds the block of A transposed, [j][i].
+__device__ __forceinline__ void invert_block(Lane l, const float* at, int stride, f32x4 x[4]) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = i == l.col ? 1.0f : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 15; j++) {
+#pragma unroll
+        for (int q = (j + 1) / 4; q < 4; q++) {
+            const f32x4 col = *reinterpret_cast<const f32x4*>(at + j * stride + 4 * q);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (4 * q + r > j) v[4 * q + r] -= col[r] * v[j];
+        }
+        if (j % 4 == 3) asm volatile("" ::: "memory");  // else all of A's block is loaded first, 160 registers
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) x[q] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+}
+
+// The chunk's small matrices in LDS.  All are stored transposed, [j][i]:
+// read across rows they are the operand with rows i, along a row the one with
+// rows j.
+template <class E> struct System {
+    static constexpr int N = Kind<E>::MID;
+    static constexpr int PLANE = C * CP;
+    float at[2][16 * 20];      // the diagonal blocks of A
+    E inv[N * PLANE];          // [j][i]: the diagonal blocks' inverses; A_10 at [j][16 + i]
+    E scores[N * PLANE];       // scale D (q_i k_j)
+};
+
+// The wavefront that holds a diagonal block of A in a result tile inverts it
+// and stores the inverse.
+template <class E>
+__device__ __forceinline__ void solve_diagonal(Lane l, System<E>& s, int block, f32x4 a) {
+    float* at = s.at[block];
+    *reinterpret_cast<f32x4*>(at + l.col * 20 + 4 * l.quad) = a;
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wavefront's own writes
+    f32x4 x[4];
+    invert_block(l, at, 20, x);
+    // all four quads hold the same columns; quad q stores rows 4 q .. 4 q + 3
+    f32x4 mine = x[0];
+    if (l.quad == 1) mine = x[1];
+    if (l.quad == 2) mine = x[2];
+    if (l.quad == 3) mine = x[3];
+    put_tile(l, s.inv, CP, System<E>::PLANE, 16 * block, 16 * block, mine);
+}
+
+// U = (1 + A)^-1 R for 16 columns of R, as two result tiles.
+template <class E>
+__device__ __forceinline__ void solve(Lane l, const System<E>& s, const f32x4 r[2], f32x4 u[2]) {
+    constexpr int N = Kind<E>::MID, P = System<E>::PLANE;
+    const f32x4 zero{0, 0, 0, 0};
+    u[0] = zero;
+    mma(u[0], col_half<N>(l, s.inv, CP, P, 0, 0), half_of<E>(r[0]));
+    f32x4 below = zero;
+    mma(below, col_half<N>(l, s.inv, CP, P, 0, 16), half_of<E>(u[0]));
+    u[1] = zero;
+    mma(u[1], col_half<N>(l, s.inv, CP, P, 16, 16), half_of<E>(r[1] - below));
+}
+// R = (1 + A)^-T U.
+template <class E>
+__device__ __forceinline__ void solve_transposed(Lane l, const System<E>& s, const f32x4 u[2], f32x4 r[2]) {
+    constexpr int N = Kind<E>::MID, P = System<E>::PLANE;
+    const f32x4 zero{0, 0, 0, 0};
+    r[1] = zero;
+    mma(r[1], row_half<N>(l, s.inv, CP, P, 16, 16), half_of<E>(u[1]));
+    f32x4 above = zero;
+    mma(above, row_half<N>(l, s.inv, CP, P, 0, 16), half_of<E>(r[1]));
+    r[0] = zero;
+    mma(r[0], row_half<N>(l, s.inv, CP, P, 0, 0), half_of<E>(u[0] - above));
+}
+
+}  // namespace delta
+
+#endif

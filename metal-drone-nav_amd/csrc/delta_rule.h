@@ -1,0 +1,46 @@
+// delta_rule.h — arguments and launchers of the gated delta rule kernels
+// (delta_rule.hip, delta_rule_backward.hip).
+#ifndef MDNAV_DELTA_RULE_H
+#define MDNAV_DELTA_RULE_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mdnav.h"
+
+namespace delta {
+
+constexpr uint32_t CHUNK = 32;    // ticks of a chunk
+constexpr uint32_t MAX_DIM = 128; // widest head
+
+// One strided [ticks][envs][heads][width] array; the width is contiguous.
+struct Rows {
+    char* p;
+    int64_t tick, env, head;  // strides in elements
+    uint32_t wide;            // base and strides are multiples of 16 bytes
+};
+
+struct Args {
+    uint32_t ticks, envs, qk_heads, heads, k_dim, v_dim;
+    uint32_t gate_f32;        // g and beta are fp32 (else the type of q)
+    float scale;
+    Rows q, k, v, o, g, beta; // g and beta have width 1
+    const uint8_t* reset;     // [ticks][envs] with the strides below, or null
+    int64_t reset_tick, reset_env;
+    const float* state;       // [envs][heads][k][v] or null (zeros)
+    float* state_out;         // the same, or null
+    float* chunk_states;      // the states before chunks 1.. for the backward pass, or null
+};
+
+// chunk_states keeps result tiles as they are in registers: of each state and
+// chunk, [v / 16][k / 16] tiles of 64 lanes x 4 values.
+inline __host__ __device__ uint64_t state_tile_words(const Args& a) {
+    return uint64_t((a.k_dim + 15) / 16) * ((a.v_dim + 15) / 16) * 256;
+}
+
+hipError_t launch_recurrent(const Args& a, bool bf16, hipStream_t stream);
+hipError_t launch_forward(const Args& a, bool bf16, hipStream_t stream);
+
+}  // namespace delta
+
+#endif

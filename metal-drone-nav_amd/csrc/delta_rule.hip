@@ -1,0 +1,324 @@
+// delta_rule.hip — the gated delta rule forward: single ticks and chunks.
+#include "delta_rule.h"
+
+#include "delta_chunk.h"
+#include "delta_tiles.h"
+
+namespace delta {
+namespace {
+
+// ---------------------------------------------------------------- recurrent
+// One wavefront has all K rows of 4 CG columns of a state in registers for
+// the whole call: lane l the four columns 4 (l % CG) of rows l / CG, + 64 / CG, ..
+// Columns of a state do not meet in a tick (u_c needs column c of S only), so
+// wavefronts need no exchange; a tick's two sums over K are made in the lane,
+// then over the 64 / CG lanes of a column.
+template <class E, int CG, int ROWS>
+__global__ void __launch_bounds__(256, 4) recurrent_kernel(Args a) {
+    constexpr int RG = 64 / CG;  // rows of a step of the loop over K
+    const int lane = int(threadIdx.x) & 63;
+    const uint32_t slices = (a.v_dim + 4 * CG - 1) / (4 * CG);
+    const uint64_t wave = uint64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave >= uint64_t(a.envs) * a.heads * slices) return;
+    const uint32_t slice = uint32_t(wave % slices);
+    const uint64_t seq = wave / slices;
+    const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
+    const uint32_t hq = h / (a.heads / a.qk_heads);
+    const uint32_t col = slice * 4 * CG + 4 * (lane % CG), row0 = lane / CG;
+    const uint32_t kd = a.k_dim, vd = a.v_dim;
+    const bool wide = (vd & 3u) == 0 && col < vd;
+    const uint64_t base = seq * kd * vd;
+    f32x4 s[ROWS];
+    const bool cleared = a.reset && a.ticks && a.reset[n * a.reset_env] != 0;  // the first tick reads no state
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const uint32_t row = row0 + i * RG;
+        s[i] = f32x4{0, 0, 0, 0};
+        if (a.state && !cleared && row < kd) {
+            const float* p = a.state + base + (row * vd + col);
+            if (wide) {
+                s[i] = *reinterpret_cast<const f32x4*>(p);
+            } else {
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++)
+                    if (col + c < vd) s[i][c] = p[c];
+            }
+        }
+    }
+    constexpr bool bf = sizeof(E) == 2;
+    for (uint32_t t = 0; t < a.ticks; t++) {
+        const int64_t qo = t * a.q.tick + n * a.q.env + hq * a.q.head;
+        const int64_t ko = t * a.k.tick + n * a.k.env + hq * a.k.head;
+        const GateRegs gate = load_gates(a, bf, n, h, t, true);
+        f32x4 v{0, 0, 0, 0};
+        const int64_t vo = t * a.v.tick + n * a.v.env + h * a.v.head + col;
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++)
+            if (col + c < vd) v[c] = load_one<E>(a.v.p, vo + c);
+        float kr[ROWS], qr[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            const uint32_t row = row0 + i * RG;
+            kr[i] = row < kd ? load_one<E>(a.k.p, ko + row) : 0.0f;
+            qr[i] = row < kd ? load_one<E>(a.q.p, qo + row) : 0.0f;
+        }
+        if (gate.flag) {
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) s[i] = f32x4{0, 0, 0, 0};
+        }
+        const float decay = gate.flag ? 1.0f : __expf(gate.g);
+        f32x4 ks{0, 0, 0, 0}, qs{0, 0, 0, 0};
+        float kq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            s[i] *= decay;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                ks[c] = fmaf(kr[i], s[i][c], ks[c]);
+                qs[c] = fmaf(qr[i], s[i][c], qs[c]);
+            }
+            kq = fmaf(kr[i], qr[i], kq);
+        }
+#pragma unroll
+        for (int d = CG; d < 64; d <<= 1) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                ks[c] += __shfl_xor(ks[c], d);
+                qs[c] += __shfl_xor(qs[c], d);
+            }
+            kq += __shfl_xor(kq, d);
+        }
+        f32x4 u, o;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            u[c] = gate.beta * (v[c] - ks[c]);
+            o[c] = a.scale * fmaf(kq, u[c], qs[c]);
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[i][c] = fmaf(kr[i], u[c], s[i][c]);
+        if (row0 == 0) {
+            const int64_t oo = t * a.o.tick + n * a.o.env + h * a.o.head + col;
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++)
+                if (col + c < vd) reinterpret_cast<E*>(a.o.p)[oo + c] = E(o[c]);
+        }
+    }
+    if (!a.state_out) return;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const uint32_t row = row0 + i * RG;
+        if (row >= kd) continue;
+        float* p = a.state_out + base + (row * vd + col);
+        if (wide) {
+            *reinterpret_cast<f32x4*>(p) = s[i];
+        } else {
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++)
+                if (col + c < vd) p[c] = s[i][c];
+        }
+    }
+}
+
+// ---------------------------------------------------------------- chunks
+template <class E, int D> struct ForwardShared {
+    static constexpr int STRIDE = D + Kind<E>::PAD;
+    E k[C * STRIDE], q[C * STRIDE], v[C * STRIDE];  // v's place takes o
+    System<E> sys;
+    Gates gates;
+};
+
+// One workgroup per state, D / 16 wavefronts, 16 columns of V each: a
+// wavefront has its K x 16 slice of the state in result tiles, which are
+// operands as they are (delta_tiles.h).
+template <class E, int D, bool WIDE>
+__global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a) {
+    typedef ForwardShared<E, D> Shared;
+    constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, W = D / 16, KT = D / 16;
+    constexpr bool bf = sizeof(E) == 2;
+    extern __shared__ __align__(16) char lds[];
+    Shared& s = *reinterpret_cast<Shared*>(lds);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const Lane at0 = Lane::mine();
+    const uint64_t seq = blockIdx.x;
+    const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
+    const uint32_t hq = h / (a.heads / a.qk_heads);
+    const uint32_t kd = a.k_dim, vd = a.v_dim;
+    const uint32_t row = uint32_t(tid) / (D / 8), col = uint32_t(tid) % (D / 8) * 8;  // the thread's piece of a chunk's rows
+    const uint32_t vcol = 16 * wave + at0.col;                                      // its column of a result
+    const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
+
+    f32x4 state[KT];
+#pragma unroll
+    for (int i = 0; i < KT; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const uint32_t kr = 16 * i + 4 * at0.quad + r;
+            const bool in = kr < kd && vcol < vd;
+            const float x = a.state ? a.state[seq * kd * vd + (in ? kr * vd + vcol : 0u)] : 0.0f;
+            state[i][r] = in ? x : 0.0f;
+        }
+    // the matrices' upper right block stays 0
+    if (wave < 2 * N) {
+        E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * System<E>::PLANE;
+#pragma unroll
+        for (int i = 0; i < 4; i++) m[(16 + at0.col) * CP + 4 * at0.quad + i] = E(0.0f);
+    }
+
+    Piece<E> pk, pq, pv;
+    GateRegs gate{0.0f, 0.0f, 0u};
+    const auto fetch = [&](uint32_t c) {
+        const uint32_t at = c * C + row;
+        const bool in = at < a.ticks;
+        const int64_t t = in ? at : 0;
+        pk = load_piece<E, WIDE>(a.k, t * a.k.tick + n * a.k.env + hq * a.k.head, kd, col, in);
+        pq = load_piece<E, WIDE>(a.q, t * a.q.tick + n * a.q.env + hq * a.q.head, kd, col, in);
+        pv = load_piece<E, WIDE>(a.v, t * a.v.tick + n * a.v.env + h * a.v.head, vd, col, in);
+        if (wave == 0) {
+            const int64_t tg = int64_t(c) * C + lane;
+            gate = load_gates(a, bf, n, h, tg, lane < C && tg < a.ticks);
+        }
+    };
+    fetch(0);
+    for (uint32_t c = 0; c < chunks; c++) {
+        const Lane l = Lane::fresh();
+        piece_to_ordered(s.k + row * ST, col, pk);
+        piece_to_ordered(s.q + row * ST, col, pq);
+        piece_to_lds(s.v + row * ST + col, pv);
+        if (wave == 0) put_gates(s.gates, gate);
+        __syncthreads();
+        if (c + 1 < chunks) fetch(c + 1);
+        if (a.chunk_states && c > 0 && 16 * wave < int(vd)) {
+            f32x4* p = state_tiles(a, seq, c, wave);
+#pragma unroll
+            for (int i = 0; i < KT; i++)
+                if (16 * i < int(kd)) p[64 * i + lane] = state[i];
+        }
+        // the chunk's scores and A: tiles (0,0), (1,1), (1,0)
+        if (wave < 3) {
+            const int i0 = wave ? 16 : 0, j0 = wave == 1 ? 16 : 0;
+            f32x4 kk{0, 0, 0, 0}, qk{0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < D; x += 32) {
+                const auto kj = ordered_row(l, s.k, ST, j0, x);
+                mma(kk, ordered_row(l, s.k, ST, i0, x), kj);
+                mma(qk, ordered_row(l, s.q, ST, i0, x), kj);
+            }
+            const f32x4 d = decay_tile(l, s.gates, i0, j0);
+            f32x4 am, pm;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int i = i0 + 4 * l.quad + r;
+                am[r] = i > j0 + l.col ? s.gates.beta[i] * d[r] * kk[r] : 0.0f;
+                pm[r] = a.scale * d[r] * qk[r];
+            }
+            put_tile(l, s.sys.scores, CP, System<E>::PLANE, j0, i0, pm);
+            if (wave < 2)
+                solve_diagonal(l, s.sys, wave, am);
+            else
+                put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
+        }
+        // the state's part of the ticks
+        f32x4 ks[2] = {}, qs[2] = {};
+#pragma unroll
+        for (int x = 0; x < D; x += 32) {
+            const auto st = frag_of<E>(state[x / 16], state[x / 16 + 1]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                mma(ks[i], ordered_row(l, s.k, ST, 16 * i, x), st);
+                mma(qs[i], ordered_row(l, s.q, ST, 16 * i, x), st);
+            }
+        }
+        f32x4 r[2], u[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int t = 16 * i + 4 * l.quad + e;
+                const float g = s.gates.before[t];
+                r[i][e] = s.gates.beta[t] * (float(s.v[t * ST + 16 * wave + l.col]) - g * ks[i][e]);
+                qs[i][e] *= a.scale * g;
+            }
+        __syncthreads();
+        solve(l, s.sys, r, u);
+        // o = scale gamma (q S) + scores u
+        {
+            const auto uf = frag_of<E>(u[0], u[1]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E>::PLANE, 0, 16 * i), uf);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int t = 16 * i + 4 * l.quad + e;
+                s.v[t * ST + 16 * wave + l.col] = E(qs[i][e]);
+                u[i][e] *= s.gates.after[t];
+            }
+        // S <- gamma_C S + K^T u
+        const float total = s.gates.before[C - 1];
+        const auto uf = frag_of<E>(u[0], u[1]);
+#pragma unroll
+        for (int i = 0; i < KT; i++) {
+            state[i] *= total;
+            mma(state[i], ordered_col(l, s.k, ST, 16 * i), uf);
+        }
+        __syncthreads();
+        const int64_t t = int64_t(c) * C + row;
+        if (t < a.ticks && col < vd)
+            store_piece<E, WIDE>(a.o, t * a.o.tick + n * a.o.env + h * a.o.head, vd, col, piece_from_lds(s.v + row * ST + col));
+    }
+    const Lane l = Lane::fresh();
+    if (a.state_out && 16 * wave + l.col < int(vd)) {
+        float* p = a.state_out + seq * kd * vd + 16 * wave + l.col;
+#pragma unroll
+        for (int i = 0; i < KT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t kr = 16 * i + 4 * l.quad + r;
+                if (kr < kd) p[kr * vd] = state[i][r];
+            }
+    }
+}
+
+template <class E, int D, bool WIDE>
+hipError_t forward(const Args& a, hipStream_t stream) {
+    constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
+    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, WIDE>);
+    if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
+    forward_kernel<E, D, WIDE><<<dim3(a.envs * a.heads), dim3(D * 4), bytes, stream>>>(a);
+    return hipGetLastError();
+}
+template <class E>
+hipError_t forward(const Args& a, hipStream_t stream) {
+    const bool narrow = a.k_dim <= 64 && a.v_dim <= 64;
+    const bool wide = (a.q.wide & a.k.wide & a.v.wide & a.o.wide) && a.k_dim % 8 == 0 && a.v_dim % 8 == 0;
+    if (wide) return narrow ? forward<E, 64, true>(a, stream) : forward<E, 128, true>(a, stream);
+    return narrow ? forward<E, 64, false>(a, stream) : forward<E, 128, false>(a, stream);
+}
+
+template <class E>
+hipError_t recurrent(const Args& a, hipStream_t stream) {
+    const uint64_t seqs = uint64_t(a.envs) * a.heads;
+    if (a.k_dim <= 64) {
+        const uint64_t waves = seqs * ((a.v_dim + 63) / 64);
+        recurrent_kernel<E, 16, 16><<<dim3(uint32_t((waves + 3) / 4)), dim3(256), 0, stream>>>(a);
+    } else {
+        const uint64_t waves = seqs * ((a.v_dim + 31) / 32);
+        recurrent_kernel<E, 8, 16><<<dim3(uint32_t((waves + 3) / 4)), dim3(256), 0, stream>>>(a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_recurrent(const Args& a, bool bf, hipStream_t stream) {
+    return bf ? recurrent<bf16>(a, stream) : recurrent<float>(a, stream);
+}
+
+hipError_t launch_forward(const Args& a, bool bf, hipStream_t stream) {
+    return bf ? forward<bf16>(a, stream) : forward<float>(a, stream);
+}
+
+}  // namespace delta

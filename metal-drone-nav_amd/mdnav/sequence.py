@@ -1,0 +1,195 @@
+"""Operators of recurrent policies over torch tensors on the GPU: the gated
+delta rule, whole rollouts with gradients (``delta_rule``) and one tick of a
+fleet in place (``delta_rule_step``), and the norms around a block
+(``block_norm``).
+
+Unlike ``ops``, which copies numpy arrays to the device and back, these take
+device tensors as they are, run on torch's current stream and return device
+tensors.  Rows are time-major, [ticks][envs][heads][width], as the rollout
+buffers are; any strides go as long as the width is contiguous, so
+``x.transpose(0, 1)`` of batch-first rows needs no copy.
+
+torch is imported here and nowhere else in the package, and it has to be
+imported before the library is first used: both need the same HIP runtime in
+the process, and the one loaded first is taken.
+"""
+import ctypes
+
+import torch
+
+from .native import MdnError, P, check, lib
+
+F32, BF16 = 0, 1
+_DTYPES = {torch.float32: F32, torch.bfloat16: BF16}
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("data", P), ("tick", ctypes.c_int64), ("env", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class _DeltaRule(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("ticks", "envs", "qk_heads", "heads", "k_dim", "v_dim", "dtype",
+                                               "gate_dtype")]
+    _fields_ += [("scale", ctypes.c_float)]
+    _fields_ += [(n, _Rows) for n in ("q", "k", "v", "g", "beta", "o")]
+    _fields_ += [("reset", P), ("reset_tick", ctypes.c_int64), ("reset_env", ctypes.c_int64), ("state", P),
+                 ("state_out", P)]
+
+
+_one_runtime = None
+
+
+def _library():
+    """The library, once it is known to share torch's HIP runtime: streams and
+    memory of another runtime in the process would not be the same."""
+    global _one_runtime
+    L = lib()
+    if _one_runtime is None:
+        with open("/proc/self/maps") as f:
+            paths = {line.split()[-1] for line in f if "libamdhip64.so" in line}
+        _one_runtime = len(paths) <= 1
+    if not _one_runtime:
+        raise MdnError("two HIP runtimes are loaded: import torch before the first use of mdnav's library")
+    return L
+
+
+def _device(named):
+    """The GPU that all tensors are on."""
+    device = None
+    for name, t in named:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s is no tensor" % name)
+        if not t.is_cuda:
+            raise ValueError("%s is not on a GPU" % name)
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError("%s is on %s, other arguments on %s" % (name, t.device, device))
+    return device
+
+
+def _rows(t):
+    """A [ticks][envs][heads][width] (or, gates, [ticks][envs][heads]) tensor."""
+    return _Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _wide(t):
+    """The tensor with a contiguous width."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _shape(name, t, shape):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+
+
+class _Call:
+    """Checked arguments of one delta rule call: the C struct and what it points to."""
+
+    def __init__(self, q, k, v, g, beta, state, reset, scale):
+        self.device = _device([("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta), ("state", state),
+                               ("reset", reset)])
+        if q.dim() != 4 or v.dim() != 4:
+            raise ValueError("q, k and v are [ticks][envs][heads][width]")
+        t, n, hq, kd = q.shape
+        h, vd = v.shape[2:]
+        _shape("k", k, q.shape)
+        _shape("v", v, (t, n, h, vd))
+        _shape("g", g, (t, n, h))
+        _shape("beta", beta, (t, n, h))
+        if hq < 1 or h < 1 or h % hq:
+            raise ValueError("%d query heads do not divide %d value heads" % (hq, h))
+        if not 1 <= kd <= 128 or not 1 <= vd <= 128:
+            raise ValueError("head widths are 1..128, not %d and %d" % (kd, vd))
+        if q.dtype not in _DTYPES:
+            raise TypeError("q is %s: float32 or bfloat16 are taken" % q.dtype)
+        for name, x in (("k", k), ("v", v)):
+            if x.dtype != q.dtype:
+                raise TypeError("%s is %s, q is %s" % (name, x.dtype, q.dtype))
+        if g.dtype != beta.dtype or g.dtype not in (torch.float32, q.dtype):
+            raise TypeError("g and beta are float32 or both of q's type, not %s and %s" % (g.dtype, beta.dtype))
+        if reset is not None:
+            _shape("reset", reset, (t, n))
+            if reset.dtype not in (torch.uint8, torch.bool):
+                raise TypeError("reset is %s: uint8 or bool are taken" % reset.dtype)
+        if state is not None:
+            _shape("state", state, (n, h, kd, vd))
+            if state.dtype != torch.float32:
+                raise TypeError("state is %s: float32 is taken" % state.dtype)
+        self.q, self.k, self.v = _wide(q), _wide(k), _wide(v)
+        self.g, self.beta, self.state, self.reset = g, beta, state, reset
+        self.scale = kd ** -0.5 if scale is None else float(scale)
+        c = _DeltaRule(t, n, hq, h, kd, vd, _DTYPES[q.dtype], _DTYPES[g.dtype], self.scale, _rows(self.q),
+                       _rows(self.k), _rows(self.v), _rows(g), _rows(beta))
+        if reset is not None:
+            c.reset, c.reset_tick, c.reset_env = reset.data_ptr(), reset.stride(0), reset.stride(1)
+        if state is not None:
+            c.state = state.data_ptr()
+        self.c = c
+
+    def stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def bytes_of(self, function, *more):
+        size = ctypes.c_uint64()
+        check(function(ctypes.byref(self.c), *more, ctypes.byref(size)))
+        return size.value
+
+    def buffer(self, size):
+        return torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _forward(call, o, state_out, keep):
+    """One forward call; `keep`: whether a backward pass follows."""
+    L = _library()
+    call.c.o = _rows(o)
+    call.c.state_out = _address(state_out)
+    with torch.cuda.device(call.device):
+        kept = call.buffer(call.bytes_of(L.mdn_op_delta_rule_keep_bytes)) if keep else None
+        size = call.bytes_of(L.mdn_op_delta_rule_workspace_bytes, 0)
+        work = call.buffer(size)
+        check(L.mdn_op_delta_rule_forward(ctypes.byref(call.c), _address(kept), kept.numel() if keep and kept is not None else 0,
+                                          _address(work), size, call.stream()))
+    return kept
+
+
+def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state=False):
+    """The gated delta rule over whole rollouts: (o, final state or None).
+
+    Per environment and head, with a state S of K x V in 32 bits:
+    S <- 0 where ``reset`` is set, S <- exp(g) S, u = beta (v - S^T k),
+    S <- S + k u^T, o = scale S^T q.
+
+    q, k: [ticks][envs][qk heads][K], v: [ticks][envs][heads][V], float32 or
+    bfloat16; the query heads divide the value heads and are shared by
+    consecutive ones.  g (log decay, -inf allowed) and beta:
+    [ticks][envs][heads], float32 or of q's type.  reset: [ticks][envs] uint8 or
+    bool.  state: [envs][heads][K][V] float32 before the first tick (zeros if
+    None).  scale: K ** -0.5 if None.  o has v's shape and q's type.
+    """
+    call = _Call(q, k, v, g, beta, None if state is None else state.contiguous(), reset, scale)
+    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    last = torch.empty(call.c.envs, call.c.heads, call.c.k_dim, call.c.v_dim, device=v.device) if final_state else None
+    _forward(call, o, last, False)
+    return o, last
+
+
+def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None):
+    """One tick of a fleet: o, with ``state`` advanced in place.
+
+    q, k: [envs][qk heads][K], v: [envs][heads][V], g, beta: [envs][heads],
+    reset: [envs], state: contiguous [envs][heads][K][V] float32; otherwise as
+    ``delta_rule``.  No gradients.
+    """
+    if not isinstance(state, torch.Tensor) or not state.is_contiguous():
+        raise ValueError("state is a contiguous tensor: it is advanced in place")
+    call = _Call(q[None], k[None], v[None], g[None], beta[None], state, None if reset is None else reset[None], scale)
+    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    _forward(call, o[None], state, False)
+    return o
