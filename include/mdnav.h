@@ -442,6 +442,19 @@ typedef struct MdnDeltaRule {
  * NULL) receives what the backward pass reads besides the inputs. */
 int mdn_op_delta_rule_forward(const MdnDeltaRule* rule, void* keep, uint64_t keep_bytes, void* workspace,
                               uint64_t workspace_bytes, void* stream);
+/* The gradients, from the same inputs, the forward call's `keep` (NULL if its
+ * size is 0) and the gradients of o and of the final state.  d_q, d_k, d_v
+ * have q's type and shapes, d_g and d_beta the gates'; o and state_out of
+ * `rule` are not read.  A tick flagged as reset has d_g = 0. */
+typedef struct MdnDeltaRuleGrad {
+    MdnRows d_o;
+    const float* d_state_out;         /* or NULL (zeros) */
+    MdnRows d_q, d_k, d_v, d_g, d_beta;
+    float* d_state;                   /* or NULL */
+} MdnDeltaRuleGrad;
+int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad* grad, const void* keep,
+                               uint64_t keep_bytes, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Bytes of `keep`, and of the workspace of a forward (0) or backward (1) call. */
 int mdn_op_delta_rule_keep_bytes(const MdnDeltaRule* rule, uint64_t* bytes);
 int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backward, uint64_t* bytes);
 

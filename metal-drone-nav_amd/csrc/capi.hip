@@ -2241,6 +2241,12 @@ uint64_t delta_keep_bytes(const delta::Args& a) {
     return chunks > 1 ? (chunks - 1) * a.envs * a.heads * delta::state_tile_words(a) * sizeof(float) : 0;
 }
 
+// d_q and d_k of every value head, where heads share them.
+uint64_t delta_partial_bytes(const delta::Args& a) {
+    if (a.heads == a.qk_heads) return 0;
+    return 2 * uint64_t(a.ticks) * a.envs * a.heads * a.k_dim * sizeof(float);
+}
+
 }  // namespace
 
 extern "C" {
@@ -2257,8 +2263,7 @@ int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backwar
     delta::Args a;
     if (int rc = delta_args("mdn_op_delta_rule_workspace_bytes", rule, &a)) return rc;
     if (!bytes) return fail(MDN_E_ARG, "mdn_op_delta_rule_workspace_bytes: null");
-    (void)backward;
-    *bytes = 0;
+    *bytes = backward ? delta_partial_bytes(a) : 0;
     return MDN_OK;
 }
 
@@ -2278,6 +2283,56 @@ int mdn_op_delta_rule_forward(const MdnDeltaRule* rule, void* keep, uint64_t kee
         HIP_TRY(delta::launch_recurrent(a, bf, st));
     else
         HIP_TRY(delta::launch_forward(a, bf, st));
+    return MDN_OK;
+}
+
+int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad* grad, const void* keep,
+                               uint64_t keep_bytes, void* workspace, uint64_t workspace_bytes, void* stream) {
+    const std::string who = "mdn_op_delta_rule_backward: ";
+    delta::Args a;
+    if (int rc = delta_args("mdn_op_delta_rule_backward", rule, &a)) return rc;
+    if (!grad) return fail(MDN_E_ARG, who + "null");
+    if (a.envs == 0) return MDN_OK;
+    const bool bf = rule->dtype == MDN_BF16;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.ticks == 0) {
+        if (!grad->d_state) return MDN_OK;
+        return fail(MDN_E_ARG, who + "no ticks: the state's gradient is d_state_out");
+    }
+    if (!grad->d_o.data || !grad->d_q.data || !grad->d_k.data || !grad->d_v.data || !grad->d_g.data || !grad->d_beta.data)
+        return fail(MDN_E_ARG, who + "null rows");
+    if (keep_bytes < delta_keep_bytes(a) || (delta_keep_bytes(a) && !keep))
+        return fail(MDN_E_ARG, who + "keep is too small");
+    if (workspace_bytes < delta_partial_bytes(a) || (delta_partial_bytes(a) && !workspace))
+        return fail(MDN_E_ARG, who + "workspace is too small");
+    a.chunk_states = static_cast<float*>(const_cast<void*>(keep));
+    const uint32_t size = size_of(rule->dtype), T = a.ticks, N = a.envs, H = a.heads, Q = a.qk_heads;
+    delta::GradArgs d{};
+    d.d_o = device_rows(grad->d_o, size, T, N, H);
+    d.d_state_out = grad->d_state_out;
+    d.d_state = grad->d_state;
+    d.d_v = device_rows(grad->d_v, size, T, N, H);
+    d.d_g = device_rows(grad->d_g, size, T, N, H);
+    d.d_beta = device_rows(grad->d_beta, size, T, N, H);
+    if (H == Q) {
+        d.d_q = device_rows(grad->d_q, size, T, N, Q);
+        d.d_k = device_rows(grad->d_k, size, T, N, Q);
+        HIP_TRY(delta::launch_backward(a, d, bf, st));
+        return MDN_OK;
+    }
+    const int64_t head = a.k_dim, env = head * H, tick = env * N;
+    const auto contiguous = [&](const MdnRows& r) {
+        return r.head == head && (N == 1 || r.env == head * Q) && (T == 1 || r.tick == head * Q * N);
+    };
+    if (!contiguous(grad->d_q) || !contiguous(grad->d_k))
+        return fail(MDN_E_ARG, who + "d_q and d_k of shared heads must be contiguous");
+    float* part = static_cast<float*>(workspace);
+    d.partial = 1;
+    d.d_q = delta::Rows{reinterpret_cast<char*>(part), tick, env, head, 0u};
+    d.d_k = delta::Rows{reinterpret_cast<char*>(part + uint64_t(T) * N * H * a.k_dim), tick, env, head, 0u};
+    HIP_TRY(delta::launch_backward(a, d, bf, st));
+    HIP_TRY(delta::launch_sum_heads(part, grad->d_q.data, uint64_t(T) * N, Q, H / Q, a.k_dim, bf, st));
+    HIP_TRY(delta::launch_sum_heads(part + uint64_t(T) * N * H * a.k_dim, grad->d_k.data, uint64_t(T) * N, Q, H / Q, a.k_dim, bf, st));
     return MDN_OK;
 }
 

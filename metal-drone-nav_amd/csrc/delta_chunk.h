@@ -135,6 +135,10 @@ struct Gates {
     float after[C];    // gamma_C / gamma_i, 0 before the last flag
     int episode[C];    // flags up to and with tick i
 };
+// Whether tick i is an episode's first: nothing before it reaches it.
+__device__ __forceinline__ bool gate_is_flag(const Gates& s, int i) {
+    return s.episode[i] != (i ? s.episode[i - 1] : 0);
+}
 
 struct GateRegs { float g, beta; uint32_t flag; };
 

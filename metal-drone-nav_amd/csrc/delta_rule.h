@@ -38,6 +38,21 @@ inline __host__ __device__ uint64_t state_tile_words(const Args& a) {
     return uint64_t((a.k_dim + 15) / 16) * ((a.v_dim + 15) / 16) * 256;
 }
 
+// The backward pass: gradients of o and of the final state in, of the inputs
+// out.  Where several value heads share a query head, d_q and d_k are fp32
+// rows of every value head (`partial`) and sum_heads adds them up.
+struct GradArgs {
+    Rows d_o;
+    const float* d_state_out;  // [envs][heads][k][v] or null (zeros)
+    Rows d_q, d_k, d_v, d_g, d_beta;
+    uint32_t partial;
+    float* d_state;            // or null
+};
+
+hipError_t launch_backward(const Args& a, const GradArgs& d, bool bf16, hipStream_t stream);
+// out[row][qk head][width] = sum of the `shared` heads of in[row][head][width]
+hipError_t launch_sum_heads(const float* in, void* out, uint64_t rows, uint32_t qk_heads, uint32_t shared, uint32_t width,
+                            bool bf16, hipStream_t stream);
 hipError_t launch_recurrent(const Args& a, bool bf16, hipStream_t stream);
 hipError_t launch_forward(const Args& a, bool bf16, hipStream_t stream);
 

@@ -126,6 +126,10 @@ template <> __device__ __forceinline__ Half<float, 1> half_of<float>(f32x4 x) {
     return f;
 }
 
+// Element e of an operand of caller's rows.
+__device__ __forceinline__ float first_term(const Frag<bf16, 1>& f, int e) { return float(f.t[0][e]); }
+__device__ __forceinline__ float first_term(const Frag<float, 1>& f, int e) { return f.t[e >> 2][e & 3]; }
+
 // ---- LDS to operands.  `m` is a matrix with rows `stride` elements apart.
 // Along a row: the lane's row or column of the operand is row `r0 + l % 16`,
 // the summed axis runs along the row from `c0`.

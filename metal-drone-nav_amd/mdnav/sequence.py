@@ -16,6 +16,7 @@ the process, and the one loaded first is taken.
 import ctypes
 
 import torch
+import torch.autograd.function
 
 from .native import MdnError, P, check, lib
 
@@ -34,6 +35,12 @@ class _DeltaRule(ctypes.Structure):
     _fields_ += [(n, _Rows) for n in ("q", "k", "v", "g", "beta", "o")]
     _fields_ += [("reset", P), ("reset_tick", ctypes.c_int64), ("reset_env", ctypes.c_int64), ("state", P),
                  ("state_out", P)]
+
+
+class _DeltaRuleGrad(ctypes.Structure):
+    _fields_ = [("d_o", _Rows), ("d_state_out", P)]
+    _fields_ += [(n, _Rows) for n in ("d_q", "d_k", "d_v", "d_g", "d_beta")]
+    _fields_ += [("d_state", P)]
 
 
 _one_runtime = None
@@ -154,9 +161,57 @@ def _forward(call, o, state_out, keep):
         kept = call.buffer(call.bytes_of(L.mdn_op_delta_rule_keep_bytes)) if keep else None
         size = call.bytes_of(L.mdn_op_delta_rule_workspace_bytes, 0)
         work = call.buffer(size)
-        check(L.mdn_op_delta_rule_forward(ctypes.byref(call.c), _address(kept), kept.numel() if keep and kept is not None else 0,
+        check(L.mdn_op_delta_rule_forward(ctypes.byref(call.c), _address(kept), 0 if kept is None else kept.numel(),
                                           _address(work), size, call.stream()))
     return kept
+
+
+def _backward(call, kept, d_o, d_state_out, want_state):
+    """(d_q, d_k, d_v, d_g, d_beta, d_state or None)"""
+    L = _library()
+    c = call.c
+    with torch.cuda.device(call.device):
+        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (call.q, call.k, call.v, call.g, call.beta)]
+        d_state = torch.empty(c.envs, c.heads, c.k_dim, c.v_dim, device=call.device) if want_state else None
+        size = call.bytes_of(L.mdn_op_delta_rule_workspace_bytes, 1)
+        work = call.buffer(size)
+        d = _DeltaRuleGrad(_rows(d_o), _address(d_state_out), *[_rows(x) for x in grads], _address(d_state))
+        check(L.mdn_op_delta_rule_backward(ctypes.byref(c), ctypes.byref(d), _address(kept),
+                                           0 if kept is None else kept.numel(), _address(work), size, call.stream()))
+    return (*grads, d_state)
+
+
+class _DeltaRuleFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, reset, scale, final_state):
+        call = _Call(q, k, v, g, beta, state, reset, scale)
+        o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        last = _final_state(call) if final_state else None
+        kept = _forward(call, o, last, True)
+        ctx.scale, ctx.has_state = scale, state is not None
+        ctx.save_for_backward(q, k, v, g, beta, state, reset, kept)
+        ctx.set_materialize_grads(False)
+        return o, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, d_last):
+        q, k, v, g, beta, state, reset, kept = ctx.saved_tensors
+        if d_o is None and d_last is None:
+            return (None,) * 9
+        call = _Call(q, k, v, g, beta, state, reset, ctx.scale)
+        d_o = torch.zeros_like(v) if d_o is None else _wide(d_o)
+        want_state = ctx.has_state and ctx.needs_input_grad[5]
+        if q.shape[0] == 0:  # nothing happens to the state
+            d_state = None if not want_state else torch.zeros_like(state) if d_last is None else d_last
+            return (*[torch.zeros_like(x) for x in (q, k, v, g, beta)], d_state, None, None, None)
+        grads = _backward(call, kept, d_o, None if d_last is None else d_last.contiguous(), want_state)
+        return (*grads, None, None, None)
+
+
+def _final_state(call):
+    c = call.c
+    return torch.empty(c.envs, c.heads, c.k_dim, c.v_dim, device=call.device)
 
 
 def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state=False):
@@ -171,11 +226,15 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state
     consecutive ones.  g (log decay, -inf allowed) and beta:
     [ticks][envs][heads], float32 or of q's type.  reset: [ticks][envs] uint8 or
     bool.  state: [envs][heads][K][V] float32 before the first tick (zeros if
-    None).  scale: K ** -0.5 if None.  o has v's shape and q's type.
+    None).  scale: K ** -0.5 if None.  o has v's shape and q's type.  Gradients
+    reach every tensor argument but reset; a flagged tick has none for g.
     """
-    call = _Call(q, k, v, g, beta, None if state is None else state.contiguous(), reset, scale)
+    state = None if state is None else state.contiguous()
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state)):
+        return _DeltaRuleFunction.apply(q, k, v, g, beta, state, reset, scale, final_state)
+    call = _Call(q, k, v, g, beta, state, reset, scale)
     o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    last = torch.empty(call.c.envs, call.c.heads, call.c.k_dim, call.c.v_dim, device=v.device) if final_state else None
+    last = _final_state(call) if final_state else None
     _forward(call, o, last, False)
     return o, last
 

@@ -37,6 +37,69 @@ def rule(q, k, v, g, beta, state=None, reset=None, scale=None):
     return o, s
 
 
+def rule_gradients(q, k, v, g, beta, state, reset, d_o, d_state, scale=None):
+    """The definition's gradients in float64, tick by tick in reverse."""
+    t, n, hq, kd = q.shape
+    h, vd = v.shape[2:]
+    shared = h // hq
+    scale = kd ** -0.5 if scale is None else scale
+    q, k = (np.repeat(x.astype(np.float64), shared, axis=2) for x in (q, k))
+    s = np.zeros((n, h, kd, vd)) if state is None else state.astype(np.float64)
+    keep = np.ones((t, n)) if reset is None else (reset == 0).astype(np.float64)
+    before, after, error = [], [], []
+    for i in range(t):
+        s = np.where(keep[i][:, None, None, None] != 0, s, 0.0)
+        s = s * np.exp(g[i].astype(np.float64))[..., None, None]
+        before.append(s)
+        error.append(v[i] - np.einsum("nhkv,nhk->nhv", s, k[i]))
+        s = s + k[i][..., None] * (beta[i].astype(np.float64)[..., None] * error[-1])[..., None, :]
+        after.append(s)
+    out = {name: np.zeros(x.shape) for name, x in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta))}
+    grad = np.zeros_like(s) if d_state is None else d_state.astype(np.float64)
+    for i in reversed(range(t)):
+        b = beta[i].astype(np.float64)[..., None]
+        out["q"][i] = scale * np.einsum("nhkv,nhv->nhk", after[i], d_o[i])
+        grad = grad + scale * q[i][..., None] * d_o[i][..., None, :]
+        du = np.einsum("nhkv,nhk->nhv", grad, k[i])
+        out["beta"][i] = (du * error[i]).sum(-1)
+        out["v"][i] = b * du
+        out["k"][i] = np.einsum("nhkv,nhv->nhk", grad, b * error[i]) - np.einsum("nhkv,nhv->nhk", before[i], b * du)
+        grad = grad - k[i][..., None] * (b * du)[..., None, :]
+        out["g"][i] = (grad * before[i]).sum((-1, -2)) * keep[i][:, None]
+        grad = np.where(keep[i][:, None, None, None] != 0, grad * np.exp(g[i].astype(np.float64))[..., None, None], 0.0)
+    for name in ("q", "k"):
+        out[name] = out[name].reshape(t, n, hq, shared, kd).sum(3)
+    out["state"] = grad
+    return out
+
+
+def test_the_gradients_here_match_differences():
+    """rule_gradients against central differences of rule(): every input, with
+    resets, shared heads and the final state's gradient."""
+    rng = np.random.default_rng(3)
+    t, n, hq, h, kd, vd = 6, 2, 1, 2, 3, 4
+    x = dict(q=rng.normal(size=(t, n, hq, kd)), k=0.6 * rng.normal(size=(t, n, hq, kd)), v=rng.normal(size=(t, n, h, vd)),
+             g=-rng.uniform(0.01, 0.5, (t, n, h)), beta=rng.uniform(0.1, 0.9, (t, n, h)),
+             state=rng.normal(size=(n, h, kd, vd)))
+    reset = np.zeros((t, n), np.uint8)
+    reset[2, 0] = reset[4, 1] = 1
+    d_o, d_s = rng.normal(size=(t, n, h, vd)), rng.normal(size=(n, h, kd, vd))
+
+    def value(y):
+        o, s = rule(y["q"], y["k"], y["v"], y["g"], y["beta"], y["state"], reset)
+        return (o * d_o).sum() + (s * d_s).sum()
+
+    grads = rule_gradients(**x, reset=reset, d_o=d_o, d_state=d_s)
+    for name, array in x.items():
+        for at in np.ndindex(array.shape):
+            y = {m: a.copy() for m, a in x.items()}
+            y[name][at] += 1e-6
+            up = value(y)
+            y[name][at] -= 2e-6
+            # a difference of values near 10 over 2e-6 in float64: 1e-9 of rounding, 1e-11 of the third derivative
+            assert abs((up - value(y)) / 2e-6 - grads[name][at]) < 1e-7, (name, at)
+
+
 def inputs(t, n, hq, h, kd, vd, dtype, seed=0, resets=0.1, gates="f32", state=True):
     """Device tensors of a rollout; keys of an environment resemble each other."""
     gen = torch.Generator().manual_seed(seed)
@@ -127,3 +190,24 @@ def test_ticks_one_at_a_time_match_the_definition(shape, dtype):
     want_o, want_s = rule(**host(x))
     near("o", torch.stack(rows), want_o, dtype)
     near("state", state, want_s, "f32")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_gradients_match_the_definition(shape, dtype):
+    """Every gradient, the final state's in and the starting state's out; on
+    half of the shapes the gates have the rows' type."""
+    from mdnav import sequence
+    print("case: delta_rule gradients", shape, dtype, flush=True)
+    x = inputs(*shape, dtype, seed=2 + sum(shape), gates=dtype if sum(shape) % 2 else "f32")
+    leaves = {name: x[name].requires_grad_() for name in ("q", "k", "v", "g", "beta", "state")}
+    gen = torch.Generator().manual_seed(9)
+    d_o = torch.randn(x["v"].shape, generator=gen).to(TORCH[dtype]).cuda()
+    d_s = torch.randn(x["state"].shape, generator=gen).cuda()
+    o, last = sequence.delta_rule(**x, final_state=True)
+    got = torch.autograd.grad([o, last], list(leaves.values()), [d_o, d_s])
+    want = rule_gradients(**host(x), d_o=d_o.double().cpu().numpy(), d_state=d_s.double().cpu().numpy())
+    for (name, leaf), grad in zip(leaves.items(), got):
+        assert grad.dtype == leaf.dtype
+        near("d_" + name, grad, want[name], dtype)
