@@ -458,6 +458,44 @@ int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad*
 int mdn_op_delta_rule_keep_bytes(const MdnDeltaRule* rule, uint64_t* bytes);
 int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backward, uint64_t* bytes);
 
+/* The norms around a block, fused with its gate and residual scale: per row
+ *     n = y / rms(y),  s = residual x + gate n w_post,  h = s / rms(s) w_pre
+ * with rms(y) = sqrt(mean(y^2) + epsilon); y is the block's output, x the
+ * residual stream before it, s the stream after it and h the next block's
+ * input.  x and s have x_dtype, y and h y_dtype (MDN_F32 with MDN_F32 or
+ * MDN_BF16, or MDN_BF16 with MDN_BF16); all arithmetic is fp32.  width is
+ * 1..8192.  Row r of an array starts (r / inner_count) outer + (r %
+ * inner_count) inner elements from its data. */
+typedef struct MdnNormRows {
+    void* data;
+    int64_t outer, inner;
+} MdnNormRows;
+#define MDN_GATE_NONE 0u     /* ones */
+#define MDN_GATE_CHANNEL 1u  /* gate[width] */
+#define MDN_GATE_ROW 2u      /* one value per row */
+#define MDN_GATE_ELEMENT 3u  /* rows of `width` values, of y_dtype */
+typedef struct MdnBlockNorm {
+    uint64_t rows;
+    uint32_t inner_count, width;
+    uint32_t x_dtype, y_dtype, gate_kind, gate_dtype; /* gate_dtype: MDN_F32 or y_dtype */
+    float epsilon;
+    MdnNormRows x, y, gate, s, h;
+    const float *w_post, *w_pre, *residual;           /* [width]; residual may be NULL (ones) */
+    float* stats;                                     /* [rows][2] for the backward pass, or NULL */
+} MdnBlockNorm;
+int mdn_op_block_norm_forward(const MdnBlockNorm* norm, void* stream);
+
+/* The gradients, from the same inputs, the forward call's stats and the
+ * gradients of s and h (data NULL: zeros).  d_gate has the gate's shape and
+ * type, d_residual is written if residual was given. */
+typedef struct MdnBlockNormGrad {
+    MdnNormRows d_s, d_h, d_x, d_y, d_gate;
+    float *d_w_post, *d_w_pre, *d_residual;
+} MdnBlockNormGrad;
+int mdn_op_block_norm_backward(const MdnBlockNorm* norm, const MdnBlockNormGrad* grad, void* workspace,
+                               uint64_t workspace_bytes, void* stream);
+int mdn_op_block_norm_workspace_bytes(const MdnBlockNorm* norm, uint64_t* bytes);
+
 /* Test support, no counterpart in the reference: the kernels divide by
  * constants (plant mass and rotor time constants, the RK4 weight 6, the
  * observation scales) as (float)((double)x * (1.0 / (double)b)).  For each

@@ -16,6 +16,7 @@
 #include <string>
 #include <vector>
 
+#include "block_norm.h"
 #include "delta_rule.h"
 #include "kernel_args.h"
 #include "mdnav.h"
@@ -2333,6 +2334,97 @@ int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad*
     HIP_TRY(delta::launch_backward(a, d, bf, st));
     HIP_TRY(delta::launch_sum_heads(part, grad->d_q.data, uint64_t(T) * N, Q, H / Q, a.k_dim, bf, st));
     HIP_TRY(delta::launch_sum_heads(part + uint64_t(T) * N * H * a.k_dim, grad->d_k.data, uint64_t(T) * N, Q, H / Q, a.k_dim, bf, st));
+    return MDN_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+int norm_args(const char* name, const MdnBlockNorm* n, blocknorm::Args* out) {
+    const std::string who = std::string(name) + ": ";
+    if (!n) return fail(MDN_E_ARG, who + "null");
+    if (n->width < 1 || n->width > blocknorm::MAX_WIDTH) return fail(MDN_E_ARG, who + "width must be 1..8192");
+    if (n->x_dtype > MDN_BF16 || n->y_dtype > MDN_BF16 || (n->x_dtype == MDN_BF16 && n->y_dtype != MDN_BF16))
+        return fail(MDN_E_ARG, who + "x_dtype and y_dtype must be MDN_F32, both MDN_BF16, or MDN_F32 with MDN_BF16");
+    if (n->gate_kind > MDN_GATE_ELEMENT) return fail(MDN_E_ARG, who + "unknown gate_kind");
+    if (n->gate_kind != MDN_GATE_NONE && n->gate_dtype != MDN_F32 && n->gate_dtype != n->y_dtype)
+        return fail(MDN_E_ARG, who + "gate_dtype must be MDN_F32 or y_dtype");
+    if (n->gate_kind == MDN_GATE_ELEMENT && n->gate_dtype != n->y_dtype)
+        return fail(MDN_E_ARG, who + "a gate per element has y_dtype");
+    if (n->inner_count < 1) return fail(MDN_E_ARG, who + "inner_count must be at least 1");
+    if (n->rows > (1ull << 40)) return fail(MDN_E_ARG, who + "too many rows");
+    if (!n->w_post || !n->w_pre) return fail(MDN_E_ARG, who + "null weights");
+    if (n->rows && (!n->x.data || !n->y.data || (n->gate_kind != MDN_GATE_NONE && !n->gate.data)))
+        return fail(MDN_E_ARG, who + "null rows");
+    blocknorm::Args a{};
+    const auto rows = [](const MdnNormRows& r) { return blocknorm::Rows{static_cast<char*>(r.data), r.outer, r.inner}; };
+    a.rows = n->rows; a.inner_count = n->inner_count; a.width = n->width;
+    a.gate_kind = n->gate_kind; a.gate_f32 = n->gate_dtype == MDN_F32; a.eps = n->epsilon;
+    a.x = rows(n->x); a.y = rows(n->y); a.gate = rows(n->gate); a.s = rows(n->s); a.h = rows(n->h);
+    a.w_post = n->w_post; a.w_pre = n->w_pre; a.residual = n->residual; a.stats = n->stats;
+    *out = a;
+    return MDN_OK;
+}
+
+// Whether every row of an array starts at a multiple of 16 bytes.
+bool norm_wide(const blocknorm::Args& a, const blocknorm::Rows& r, uint32_t size) {
+    if (!r.p) return true;
+    const uint64_t inner = a.rows < a.inner_count ? a.rows : a.inner_count;
+    return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && (inner <= 1 || r.inner * int64_t(size) % 16 == 0) &&
+           (a.rows <= a.inner_count || r.outer * int64_t(size) % 16 == 0);
+}
+bool norm_inputs_wide(const blocknorm::Args& a, const MdnBlockNorm* n) {
+    const auto vector = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const uint32_t sx = size_of(n->x_dtype), sy = size_of(n->y_dtype);
+    return norm_wide(a, a.x, sx) && norm_wide(a, a.y, sy) && vector(n->w_post) && vector(n->w_pre) && vector(n->residual) &&
+           (n->gate_kind != MDN_GATE_CHANNEL || vector(n->gate.data)) &&
+           (n->gate_kind != MDN_GATE_ELEMENT || norm_wide(a, a.gate, sy));
+}
+
+}  // namespace
+
+extern "C" {
+
+int mdn_op_block_norm_forward(const MdnBlockNorm* norm, void* stream) {
+    blocknorm::Args a;
+    if (int rc = norm_args("mdn_op_block_norm_forward", norm, &a)) return rc;
+    if (a.rows == 0) return MDN_OK;
+    if (!a.s.p || !a.h.p) return fail(MDN_E_ARG, "mdn_op_block_norm_forward: null rows");
+    a.wide = norm_inputs_wide(a, norm) && norm_wide(a, a.s, size_of(norm->x_dtype)) && norm_wide(a, a.h, size_of(norm->y_dtype));
+    HIP_TRY(blocknorm::launch_forward(a, norm->x_dtype, norm->y_dtype, static_cast<hipStream_t>(stream)));
+    return MDN_OK;
+}
+
+int mdn_op_block_norm_workspace_bytes(const MdnBlockNorm* norm, uint64_t* bytes) {
+    blocknorm::Args a;
+    if (int rc = norm_args("mdn_op_block_norm_workspace_bytes", norm, &a)) return rc;
+    if (!bytes) return fail(MDN_E_ARG, "mdn_op_block_norm_workspace_bytes: null");
+    *bytes = uint64_t(blocknorm::parts(a, norm->y_dtype)) * 4 * a.width * sizeof(float);
+    return MDN_OK;
+}
+
+int mdn_op_block_norm_backward(const MdnBlockNorm* norm, const MdnBlockNormGrad* grad, void* workspace,
+                               uint64_t workspace_bytes, void* stream) {
+    const std::string who = "mdn_op_block_norm_backward: ";
+    blocknorm::Args a;
+    if (int rc = norm_args("mdn_op_block_norm_backward", norm, &a)) return rc;
+    if (!grad) return fail(MDN_E_ARG, who + "null");
+    if (!grad->d_w_post || !grad->d_w_pre || (a.residual && !grad->d_residual)) return fail(MDN_E_ARG, who + "null weights");
+    const bool gate = a.gate_kind != MDN_GATE_NONE;
+    if (a.rows && (!grad->d_x.data || !grad->d_y.data || !a.stats)) return fail(MDN_E_ARG, who + "null rows");
+    if (gate && !grad->d_gate.data && (a.rows || a.gate_kind == MDN_GATE_CHANNEL)) return fail(MDN_E_ARG, who + "null rows");
+    const uint64_t need = uint64_t(blocknorm::parts(a, norm->y_dtype)) * 4 * a.width * sizeof(float);
+    if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, who + "workspace is too small");
+    const auto rows = [](const MdnNormRows& r) { return blocknorm::Rows{static_cast<char*>(r.data), r.outer, r.inner}; };
+    blocknorm::GradArgs d{};
+    d.d_s = rows(grad->d_s); d.d_h = rows(grad->d_h); d.d_x = rows(grad->d_x); d.d_y = rows(grad->d_y); d.d_gate = rows(grad->d_gate);
+    d.d_w_post = grad->d_w_post; d.d_w_pre = grad->d_w_pre; d.d_residual = grad->d_residual;
+    d.parts = static_cast<float*>(workspace);
+    const uint32_t sx = size_of(norm->x_dtype), sy = size_of(norm->y_dtype);
+    a.wide = norm_inputs_wide(a, norm) && norm_wide(a, d.d_s, sx) && norm_wide(a, d.d_h, sy) && norm_wide(a, d.d_x, sx) &&
+             norm_wide(a, d.d_y, sy) && (a.gate_kind != MDN_GATE_ELEMENT || norm_wide(a, d.d_gate, sy));
+    HIP_TRY(blocknorm::launch_backward(a, d, norm->x_dtype, norm->y_dtype, static_cast<hipStream_t>(stream)));
     return MDN_OK;
 }
 

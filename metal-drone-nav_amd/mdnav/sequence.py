@@ -43,6 +43,23 @@ class _DeltaRuleGrad(ctypes.Structure):
     _fields_ += [("d_state", P)]
 
 
+class _NormRows(ctypes.Structure):
+    _fields_ = [("data", P), ("outer", ctypes.c_int64), ("inner", ctypes.c_int64)]
+
+
+class _BlockNorm(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_uint64)]
+    _fields_ += [(n, ctypes.c_uint32) for n in ("inner_count", "width", "x_dtype", "y_dtype", "gate_kind", "gate_dtype")]
+    _fields_ += [("epsilon", ctypes.c_float)]
+    _fields_ += [(n, _NormRows) for n in ("x", "y", "gate", "s", "h")]
+    _fields_ += [(n, P) for n in ("w_post", "w_pre", "residual", "stats")]
+
+
+class _BlockNormGrad(ctypes.Structure):
+    _fields_ = [(n, _NormRows) for n in ("d_s", "d_h", "d_x", "d_y", "d_gate")]
+    _fields_ += [(n, P) for n in ("d_w_post", "d_w_pre", "d_residual")]
+
+
 _one_runtime = None
 
 
@@ -252,3 +269,172 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None):
     o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     _forward(call, o[None], state, False)
     return o
+
+
+# ---------------------------------------------------------------- norms around a block
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_ELEMENT = 0, 1, 2, 3
+
+
+def _norm_rows(t, width):
+    """A tensor whose last axis is a row, as two strides: (tensor, rows, count of the inner axis)."""
+    t = t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    lead, strides = t.shape[:-1], t.stride()[:-1]
+    # join neighbouring axes that are one; at most two may remain
+    axes = []
+    for size, stride in zip(lead, strides):
+        if size == 1:
+            continue
+        if axes and axes[-1][1] == size * stride:
+            axes[-1] = (axes[-1][0] * size, stride)
+        else:
+            axes.append((size, stride))
+    return t, axes
+
+
+class _NormCall:
+    """Checked arguments of one norm block call."""
+
+    def __init__(self, x, y, w_post, w_pre, gate, residual_scale, eps):
+        self.device = _device([("x", x), ("y", y), ("w_post", w_post), ("w_pre", w_pre), ("gate", gate),
+                               ("residual_scale", residual_scale)])
+        if x.dim() < 1:
+            raise ValueError("x is [..., width]")
+        _shape("y", y, x.shape)
+        width = x.shape[-1]
+        if not 1 <= width <= 8192:
+            raise ValueError("the width is 1..8192, not %d" % width)
+        if x.dtype not in _DTYPES or y.dtype not in _DTYPES or (x.dtype, y.dtype) == (torch.bfloat16, torch.float32):
+            raise TypeError("x and y are float32, both bfloat16, or float32 and bfloat16, not %s and %s" % (x.dtype, y.dtype))
+        for name, w in (("w_post", w_post), ("w_pre", w_pre), ("residual_scale", residual_scale)):
+            if w is None and name == "residual_scale":
+                continue
+            _shape(name, w, (width,))
+            if w.dtype != torch.float32:
+                raise TypeError("%s is %s: float32 is taken" % (name, w.dtype))
+        self.kind = GATE_NONE
+        if gate is not None:
+            if gate.dtype not in (torch.float32, y.dtype):
+                raise TypeError("gate is %s: float32 or y's type are taken" % gate.dtype)
+            if tuple(gate.shape) == (width,) and (x.dim() > 1 or width > 1):
+                self.kind = GATE_CHANNEL
+            elif tuple(gate.shape) == tuple(x.shape[:-1]) + (1,):
+                self.kind = GATE_ROW
+            elif tuple(gate.shape) == tuple(x.shape):
+                self.kind = GATE_ELEMENT
+                if gate.dtype != y.dtype:
+                    raise TypeError("a gate per element is of y's type, %s, not %s" % (y.dtype, gate.dtype))
+            else:
+                raise ValueError("gate has shape %s, expected %s, %s or %s" % (
+                    tuple(gate.shape), (width,), tuple(x.shape[:-1]) + (1,), tuple(x.shape)))
+        self.x, self.y, self.gate = x, y, gate
+        self.w_post, self.w_pre = w_post.contiguous(), w_pre.contiguous()
+        self.residual = None if residual_scale is None else residual_scale.contiguous()
+        self.shape, self.width, self.rows, self.eps = x.shape, width, x.numel() // width, float(eps)
+        self.inner = x.shape[-2] if x.dim() > 1 and self.rows else 1
+
+    def layout(self, t):
+        """The rows of `t`, [..., width or 1]; a layout of more than two strides is copied."""
+        t, axes = _norm_rows(t, self.width)
+        if not axes:
+            return t, _NormRows(t.data_ptr(), 0, 0)
+        if len(axes) == 1:
+            return t, _NormRows(t.data_ptr(), axes[0][1] * self.inner, axes[0][1])
+        if len(axes) == 2 and axes[1][0] == self.inner:
+            return t, _NormRows(t.data_ptr(), axes[0][1], axes[1][1])
+        t = t.contiguous()
+        return t, _NormRows(t.data_ptr(), t.shape[-1] * self.inner, t.shape[-1])
+
+    def struct(self, s, h, stats):
+        """The C struct, and the tensors it points to."""
+        kept = [s, h, stats]
+        c = _BlockNorm(self.rows, self.inner, self.width, _DTYPES[self.x.dtype], _DTYPES[self.y.dtype], self.kind,
+                       0 if self.gate is None else _DTYPES[self.gate.dtype], self.eps)
+        for name in ("x", "y"):
+            t, rows = self.layout(getattr(self, name))
+            kept.append(t)
+            setattr(c, name, rows)
+        if self.kind == GATE_CHANNEL:
+            t = self.gate.contiguous()
+            kept.append(t)
+            c.gate = _NormRows(t.data_ptr(), 0, 0)
+        elif self.kind != GATE_NONE:
+            t, c.gate = self.layout(self.gate)
+            kept.append(t)
+        if s is not None:
+            c.s, c.h = self.layout(s)[1], self.layout(h)[1]
+        c.w_post, c.w_pre = self.w_post.data_ptr(), self.w_pre.data_ptr()
+        c.residual, c.stats = _address(self.residual), _address(stats)
+        return c, kept
+
+    def forward(self, keep):
+        L = _library()
+        s = torch.empty(self.shape, dtype=self.x.dtype, device=self.device)
+        h = torch.empty(self.shape, dtype=self.y.dtype, device=self.device)
+        stats = torch.empty(self.rows, 2, device=self.device) if keep else None
+        with torch.cuda.device(self.device):
+            c, kept = self.struct(s, h, stats)
+            check(L.mdn_op_block_norm_forward(ctypes.byref(c), torch.cuda.current_stream().cuda_stream))
+        return s, h, stats
+
+    def backward(self, stats, d_s, d_h):
+        L = _library()
+        with torch.cuda.device(self.device):
+            c, kept = self.struct(None, None, stats)
+            d = _BlockNormGrad()
+            for name, t in (("d_s", d_s), ("d_h", d_h)):
+                if t is not None:
+                    t, rows = self.layout(t)
+                    kept.append(t)
+                    setattr(d, name, rows)
+            d_x = torch.empty(self.shape, dtype=self.x.dtype, device=self.device)
+            d_y = torch.empty(self.shape, dtype=self.y.dtype, device=self.device)
+            d.d_x, d.d_y = self.layout(d_x)[1], self.layout(d_y)[1]
+            d_gate = None
+            if self.kind != GATE_NONE:
+                d_gate = torch.empty(self.gate.shape, dtype=self.gate.dtype, device=self.device)
+                d.d_gate = _NormRows(d_gate.data_ptr(), 0, 0) if self.kind == GATE_CHANNEL else self.layout(d_gate)[1]
+            sums = torch.empty(2 if self.residual is None else 3, self.width, device=self.device)
+            d.d_w_post, d.d_w_pre = sums[0].data_ptr(), sums[1].data_ptr()
+            if self.residual is not None:
+                d.d_residual = sums[2].data_ptr()
+            size = ctypes.c_uint64()
+            check(L.mdn_op_block_norm_workspace_bytes(ctypes.byref(c), ctypes.byref(size)))
+            work = torch.empty(size.value, dtype=torch.uint8, device=self.device) if size.value else None
+            check(L.mdn_op_block_norm_backward(ctypes.byref(c), ctypes.byref(d), _address(work), size.value,
+                                               torch.cuda.current_stream().cuda_stream))
+        return d_x, d_y, sums[0], sums[1], d_gate, None if self.residual is None else sums[2]
+
+
+class _BlockNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, w_post, w_pre, gate, residual_scale, eps):
+        s, h, stats = _NormCall(x, y, w_post, w_pre, gate, residual_scale, eps).forward(True)
+        ctx.eps = eps
+        ctx.save_for_backward(x, y, w_post, w_pre, gate, residual_scale, stats)
+        ctx.set_materialize_grads(False)
+        return s, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_s, d_h):
+        x, y, w_post, w_pre, gate, residual_scale, stats = ctx.saved_tensors
+        if d_s is None and d_h is None:
+            return (None,) * 7
+        return (*_NormCall(x, y, w_post, w_pre, gate, residual_scale, ctx.eps).backward(stats, d_s, d_h), None)
+
+
+def block_norm(x, y, w_post, w_pre, gate=None, residual_scale=None, eps=1e-6):
+    """The norms around a block, with its gate and residual scale: (s, h).
+
+    n = y / rms(y), s = residual_scale x + gate n w_post, h = s / rms(s) w_pre:
+    x is the residual stream [..., width], y the block's output, s the stream
+    after it and h the next block's input.  x and y are float32, both bfloat16,
+    or float32 and bfloat16; s has x's type, h has y's.  w_post, w_pre and
+    residual_scale (ones if None) are [width] float32.  gate (ones if None):
+    [width], one value per row [..., 1], or one per element, float32 or, per
+    element always, of y's type.  Gradients reach every tensor argument.
+    """
+    args = (x, y, w_post, w_pre, gate, residual_scale)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
+        return _BlockNormFunction.apply(*args, eps)
+    return _NormCall(*args, eps).forward(False)[:2]
