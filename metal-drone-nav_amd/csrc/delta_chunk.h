@@ -40,43 +40,95 @@ __device__ __forceinline__ f32x4* state_tiles(const Args& a, uint64_t seq, uint3
            wave * ((a.k_dim + 15) / 16) * 64;
 }
 
+// A wavefront's 16 columns of a state [K][V] as result tiles; `col` is the lane's column.
+template <int KT>
+__device__ __forceinline__ void load_state(f32x4 (&x)[KT], const float* p, uint32_t kd, uint32_t vd, Lane l, uint32_t col) {
+#pragma unroll
+    for (int i = 0; i < KT; i++) x[i] = f32x4{0, 0, 0, 0};
+    if (!p || col >= vd) return;
+    if (kd == 16 * KT) {
+#pragma unroll
+        for (int i = 0; i < KT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[i][r] = p[uint32_t(16 * i + 4 * l.quad + r) * vd + col];
+    } else {
+#pragma unroll
+        for (int i = 0; i < KT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t kr = 16 * i + 4 * l.quad + r;
+                const float y = p[(kr < kd ? kr : 0u) * vd + col];
+                x[i][r] = kr < kd ? y : 0.0f;
+            }
+    }
+}
+template <int KT>
+__device__ __forceinline__ void store_state(float* p, const f32x4 (&x)[KT], uint32_t kd, uint32_t vd, Lane l, uint32_t col) {
+    if (col >= vd) return;
+#pragma unroll
+    for (int i = 0; i < KT; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const uint32_t kr = 16 * i + 4 * l.quad + r;
+            if (kr < kd) p[kr * vd + col] = x[i][r];
+        }
+}
+
 // ---- eight elements of a row, in registers.  WIDE: rows start at multiples
 // of 16 bytes and widths are multiples of eight elements; a piece is then
 // wholly inside its row or wholly past it, and moves in 16-byte words.
 template <class E> struct Piece { uint4 w[sizeof(E) / 2]; };
 
-// What is past the row's end or the last tick reads as 0 (`base` is then
-// some other row of the array).
+// What is past the row's end or the last tick is some other part of the array
+// until mask_piece() makes it 0: where the piece is used, not where it is
+// loaded, which would wait for it.
 template <class E, bool WIDE>
-__device__ __forceinline__ Piece<E> load_piece(const Rows& r, int64_t base, uint32_t dim, uint32_t col, bool row_in) {
+__device__ __forceinline__ Piece<E> load_piece(const Rows& r, int64_t base, uint32_t dim, uint32_t col) {
     constexpr int W = sizeof(E) / 2;
     Piece<E> out;
     const E* p = reinterpret_cast<const E*>(r.p) + base;
     if (WIDE) {
-        const bool in = row_in && col < dim;
         const uint4* q = reinterpret_cast<const uint4*>(p + (col < dim ? col : 0u));
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            const uint4 x = q[i];
-            out.w[i] = uint4{in ? x.x : 0u, in ? x.y : 0u, in ? x.z : 0u, in ? x.w : 0u};
-        }
+        for (int i = 0; i < W; i++) out.w[i] = q[i];
     } else {
         uint32_t word[4 * W];
 #pragma unroll
         for (uint32_t i = 0; i < 4 * W; i++) {
             if (sizeof(E) == 4) {
                 const uint32_t c = col + i;
-                const uint32_t x = reinterpret_cast<const uint32_t*>(p)[c < dim ? c : 0u];
-                word[i] = row_in && c < dim ? x : 0u;
+                word[i] = reinterpret_cast<const uint32_t*>(p)[c < dim ? c : 0u];
             } else {
                 const uint32_t c = col + 2 * i;
                 const uint32_t lo = reinterpret_cast<const uint16_t*>(p)[c < dim ? c : 0u];
                 const uint32_t hi = reinterpret_cast<const uint16_t*>(p)[c + 1 < dim ? c + 1 : 0u];
-                word[i] = (row_in && c < dim ? lo : 0u) | (row_in && c + 1 < dim ? hi << 16 : 0u);
+                word[i] = lo | hi << 16;
             }
         }
 #pragma unroll
         for (int i = 0; i < W; i++) out.w[i] = uint4{word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]};
+    }
+    return out;
+}
+template <class E, bool WIDE>
+__device__ __forceinline__ Piece<E> mask_piece(const Piece<E>& x, uint32_t dim, uint32_t col, bool row_in) {
+    constexpr int W = sizeof(E) / 2;
+    Piece<E> out;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        const uint32_t word[4] = {x.w[i].x, x.w[i].y, x.w[i].z, x.w[i].w};
+        uint32_t y[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            if (WIDE) {
+                y[e] = row_in && col < dim ? word[e] : 0u;
+            } else {
+                const uint32_t c = col + (4 * i + e) * (4 / sizeof(E));
+                y[e] = row_in && c < dim ? word[e] : 0u;
+                if (sizeof(E) == 2 && c + 1 >= dim) y[e] &= 0xffffu;
+            }
+        }
+        out.w[i] = uint4{y[0], y[1], y[2], y[3]};
     }
     return out;
 }
@@ -205,9 +257,13 @@ __device__ __forceinline__ void invert_block(Lane l, const float* at, int stride
             const f32x4 col = *reinterpret_cast<const f32x4*>(at + j * stride + 4 * q);
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                if (4 * q + r > j) v[4 * q + r] -= col[r] * v[j];
+                if (4 * q + r > j) v[4 * q + r] = fmaf(-col[r], v[j], v[4 * q + r]);
         }
-        if (j % 4 == 3) asm volatile("" ::: "memory");  // else all of A's block is loaded first, 160 registers
+        // done before A's next columns are read: else all of the block is loaded first, 160 registers
+        if (j % 2 == 1)
+            asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]),
+                              "+v"(v[8]), "+v"(v[9]), "+v"(v[10]), "+v"(v[11]), "+v"(v[12]), "+v"(v[13]), "+v"(v[14]),
+                              "+v"(v[15])::"memory");
     }
 #pragma unroll
     for (int q = 0; q < 4; q++) x[q] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};

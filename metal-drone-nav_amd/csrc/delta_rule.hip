@@ -8,13 +8,19 @@ namespace delta {
 namespace {
 
 // ---------------------------------------------------------------- recurrent
+// The sum over the lanes that share l % CG.
+template <int CG> __device__ __forceinline__ float sum_columns(float x) {
+    if (CG <= 8) x += from_lane<0x128>(x);  // row_ror by 8
+    return sum_rows32(sum_rows16(x));
+}
+
 // One wavefront has all K rows of 4 CG columns of a state in registers for
 // the whole call: lane l the four columns 4 (l % CG) of rows l / CG, + 64 / CG, ..
 // Columns of a state do not meet in a tick (u_c needs column c of S only), so
 // wavefronts need no exchange; a tick's two sums over K are made in the lane,
 // then over the 64 / CG lanes of a column.
 template <class E, int CG, int ROWS>
-__global__ void __launch_bounds__(256, 4) recurrent_kernel(Args a) {
+__global__ void __launch_bounds__(256, 3) recurrent_kernel(Args a) {
     constexpr int RG = 64 / CG;  // rows of a step of the loop over K
     const int lane = int(threadIdx.x) & 63;
     const uint32_t slices = (a.v_dim + 4 * CG - 1) / (4 * CG);
@@ -80,14 +86,11 @@ __global__ void __launch_bounds__(256, 4) recurrent_kernel(Args a) {
             kq = fmaf(kr[i], qr[i], kq);
         }
 #pragma unroll
-        for (int d = CG; d < 64; d <<= 1) {
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                ks[c] += __shfl_xor(ks[c], d);
-                qs[c] += __shfl_xor(qs[c], d);
-            }
-            kq += __shfl_xor(kq, d);
+        for (int c = 0; c < 4; c++) {
+            ks[c] = sum_columns<CG>(ks[c]);
+            qs[c] = sum_columns<CG>(qs[c]);
         }
+        kq = sum_columns<CG>(kq);
         f32x4 u, o;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
@@ -126,14 +129,14 @@ template <class E, int D> struct ForwardShared {
     static constexpr int STRIDE = D + Kind<E>::PAD;
     E k[C * STRIDE], q[C * STRIDE], v[C * STRIDE];  // v's place takes o
     System<E> sys;
-    Gates gates;
+    Gates gates[2];  // of this chunk and the next
 };
 
 // One workgroup per state, D / 16 wavefronts, 16 columns of V each: a
 // wavefront has its K x 16 slice of the state in result tiles, which are
 // operands as they are (delta_tiles.h).
 template <class E, int D, bool WIDE>
-__global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a) {
+__global__ void __launch_bounds__(D * 4, D == 64 ? (sizeof(E) == 2 && WIDE ? 4 : 3) : 2) forward_kernel(Args a) {
     typedef ForwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, W = D / 16, KT = D / 16;
     constexpr bool bf = sizeof(E) == 2;
@@ -150,15 +153,7 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a)
     const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
 
     f32x4 state[KT];
-#pragma unroll
-    for (int i = 0; i < KT; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const uint32_t kr = 16 * i + 4 * at0.quad + r;
-            const bool in = kr < kd && vcol < vd;
-            const float x = a.state ? a.state[seq * kd * vd + (in ? kr * vd + vcol : 0u)] : 0.0f;
-            state[i][r] = in ? x : 0.0f;
-        }
+    load_state(state, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, at0, vcol);
     // the matrices' upper right block stays 0
     if (wave < 2 * N) {
         E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * System<E>::PLANE;
@@ -170,23 +165,29 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a)
     GateRegs gate{0.0f, 0.0f, 0u};
     const auto fetch = [&](uint32_t c) {
         const uint32_t at = c * C + row;
-        const bool in = at < a.ticks;
-        const int64_t t = in ? at : 0;
-        pk = load_piece<E, WIDE>(a.k, t * a.k.tick + n * a.k.env + hq * a.k.head, kd, col, in);
-        pq = load_piece<E, WIDE>(a.q, t * a.q.tick + n * a.q.env + hq * a.q.head, kd, col, in);
-        pv = load_piece<E, WIDE>(a.v, t * a.v.tick + n * a.v.env + h * a.v.head, vd, col, in);
-        if (wave == 0) {
-            const int64_t tg = int64_t(c) * C + lane;
-            gate = load_gates(a, bf, n, h, tg, lane < C && tg < a.ticks);
-        }
+        const int64_t t = at < a.ticks ? at : 0;
+        pk = load_piece<E, WIDE>(a.k, t * a.k.tick + n * a.k.env + hq * a.k.head, kd, col);
+        pq = load_piece<E, WIDE>(a.q, t * a.q.tick + n * a.q.env + hq * a.q.head, kd, col);
+        pv = load_piece<E, WIDE>(a.v, t * a.v.tick + n * a.v.env + h * a.v.head, vd, col);
     };
+    // the last wavefront has no tile of A: it makes the next chunk's decays meanwhile
+    const auto fetch_gates = [&](uint32_t c) {
+        const int64_t t = int64_t(c) * C + lane;
+        gate = load_gates(a, bf, n, h, t, lane < C && t < a.ticks);
+    };
+    if (wave == W - 1) {
+        fetch_gates(0);
+        put_gates(s.gates[0], gate);
+        fetch_gates(1);
+    }
     fetch(0);
     for (uint32_t c = 0; c < chunks; c++) {
         const Lane l = Lane::fresh();
-        piece_to_ordered(s.k + row * ST, col, pk);
-        piece_to_ordered(s.q + row * ST, col, pq);
-        piece_to_lds(s.v + row * ST + col, pv);
-        if (wave == 0) put_gates(s.gates, gate);
+        const Gates& gates = s.gates[c & 1];
+        const bool in = c * C + row < a.ticks;
+        piece_to_ordered(s.k + row * ST, col, mask_piece<E, WIDE>(pk, kd, col, in));
+        piece_to_ordered(s.q + row * ST, col, mask_piece<E, WIDE>(pq, kd, col, in));
+        piece_to_lds(s.v + row * ST + col, mask_piece<E, WIDE>(pv, vd, col, in));
         __syncthreads();
         if (c + 1 < chunks) fetch(c + 1);
         if (a.chunk_states && c > 0 && 16 * wave < int(vd)) {
@@ -205,12 +206,12 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a)
                 mma(kk, ordered_row(l, s.k, ST, i0, x), kj);
                 mma(qk, ordered_row(l, s.q, ST, i0, x), kj);
             }
-            const f32x4 d = decay_tile(l, s.gates, i0, j0);
+            const f32x4 d = decay_tile(l, gates, i0, j0);
             f32x4 am, pm;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = i0 + 4 * l.quad + r;
-                am[r] = i > j0 + l.col ? s.gates.beta[i] * d[r] * kk[r] : 0.0f;
+                am[r] = i > j0 + l.col ? gates.beta[i] * d[r] * kk[r] : 0.0f;
                 pm[r] = a.scale * d[r] * qk[r];
             }
             put_tile(l, s.sys.scores, CP, System<E>::PLANE, j0, i0, pm);
@@ -218,6 +219,10 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a)
                 solve_diagonal(l, s.sys, wave, am);
             else
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
+        }
+        if (wave == W - 1 && c + 1 < chunks) {
+            put_gates(s.gates[(c + 1) & 1], gate);
+            fetch_gates(c + 2);
         }
         // the state's part of the ticks
         f32x4 ks[2] = {}, qs[2] = {};
@@ -236,8 +241,8 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int t = 16 * i + 4 * l.quad + e;
-                const float g = s.gates.before[t];
-                r[i][e] = s.gates.beta[t] * (float(s.v[t * ST + 16 * wave + l.col]) - g * ks[i][e]);
+                const float g = gates.before[t];
+                r[i][e] = gates.beta[t] * (float(s.v[t * ST + 16 * wave + l.col]) - g * ks[i][e]);
                 qs[i][e] *= a.scale * g;
             }
         __syncthreads();
@@ -254,10 +259,10 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a)
             for (int e = 0; e < 4; e++) {
                 const int t = 16 * i + 4 * l.quad + e;
                 s.v[t * ST + 16 * wave + l.col] = E(qs[i][e]);
-                u[i][e] *= s.gates.after[t];
+                u[i][e] *= gates.after[t];
             }
         // S <- gamma_C S + K^T u
-        const float total = s.gates.before[C - 1];
+        const float total = gates.before[C - 1];
         const auto uf = frag_of<E>(u[0], u[1]);
 #pragma unroll
         for (int i = 0; i < KT; i++) {
@@ -270,16 +275,7 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 3 : 2) forward_kernel(Args a)
             store_piece<E, WIDE>(a.o, t * a.o.tick + n * a.o.env + h * a.o.head, vd, col, piece_from_lds(s.v + row * ST + col));
     }
     const Lane l = Lane::fresh();
-    if (a.state_out && 16 * wave + l.col < int(vd)) {
-        float* p = a.state_out + seq * kd * vd + 16 * wave + l.col;
-#pragma unroll
-        for (int i = 0; i < KT; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint32_t kr = 16 * i + 4 * l.quad + r;
-                if (kr < kd) p[kr * vd] = state[i][r];
-            }
-    }
+    if (a.state_out) store_state(a.state_out + seq * kd * vd, state, kd, vd, l, 16 * wave + l.col);
 }
 
 template <class E, int D, bool WIDE>

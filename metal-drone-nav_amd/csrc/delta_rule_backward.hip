@@ -38,17 +38,11 @@ template <class E, int D> struct BackwardShared {
     float through[D / HALVES * TS];                   // S, then G, transposed: [v][k]
     System<E> sys;
     E d_scores[N * System<E>::PLANE], d_a[N * System<E>::PLANE];  // scale D dP and E, [j][i]
-    Gates gates;
+    Gates gates[2];  // of this chunk and the next
     float beta_v[W][C], a[W][C], b[W][C], dot[W];
     double m_row[3][16], m_col[3][16];
     float beta_a[3][16];
 };
-
-__device__ __forceinline__ float sum16(float x) {
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
-    return x;
-}
 
 template <class E>
 __device__ __forceinline__ void put_grad(const Rows& r, int64_t at, float x, bool partial) {
@@ -87,16 +81,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     f32x4 g[KT];  // G, K x 16
     {
         const Lane l = Lane::fresh();
-        const uint32_t vc = 16 * wave + l.col;
-#pragma unroll
-        for (int i = 0; i < KT; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint32_t kr = 16 * i + 4 * l.quad + r;
-                const bool in = kr < kd && vc < vd;
-                const float x = d.d_state_out ? d.d_state_out[seq * kd * vd + (in ? kr * vd + vc : 0u)] : 0.0f;
-                g[i][r] = in ? x : 0.0f;
-            }
+        load_state(g, d.d_state_out ? d.d_state_out + seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
         // the matrices' upper right blocks stay 0
         if (wave < N) {
             E* m[4] = {s.sys.scores, s.sys.inv, s.d_scores, s.d_a};
@@ -110,25 +95,31 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     GateRegs gate{0.0f, 0.0f, 0u};
     const auto fetch = [&](uint32_t c) {
         const uint32_t at = c * C + row;
-        const bool in = at < a.ticks;
-        const int64_t t = in ? at : 0;
-        pk = load_piece<E, WIDE>(a.k, t * a.k.tick + n * a.k.env + hq * a.k.head, kd, col, in);
-        pq = load_piece<E, WIDE>(a.q, t * a.q.tick + n * a.q.env + hq * a.q.head, kd, col, in);
-        po = load_piece<E, WIDE>(d.d_o, t * d.d_o.tick + n * d.d_o.env + h * d.d_o.head, vd, col, in);
-        if (wave == 0) {
-            const int64_t tg = int64_t(c) * C + lane;
-            gate = load_gates(a, bf, n, h, tg, lane < C && tg < a.ticks);
-        }
+        const int64_t t = at < a.ticks ? at : 0;
+        pk = load_piece<E, WIDE>(a.k, t * a.k.tick + n * a.k.env + hq * a.k.head, kd, col);
+        pq = load_piece<E, WIDE>(a.q, t * a.q.tick + n * a.q.env + hq * a.q.head, kd, col);
+        po = load_piece<E, WIDE>(d.d_o, t * d.d_o.tick + n * d.d_o.env + h * d.d_o.head, vd, col);
     };
+    // the last wavefront has no tile of A: it makes the next chunk's decays meanwhile
+    const auto fetch_gates = [&](uint32_t c) {
+        const int64_t t = int64_t(c) * C + lane;
+        gate = load_gates(a, bf, n, h, t, lane < C && t < a.ticks);
+    };
+    if (wave == Shared::W - 1) {
+        fetch_gates(chunks - 1);
+        put_gates(s.gates[(chunks - 1) & 1], gate);
+        if (chunks > 1) fetch_gates(chunks - 2);
+    }
     fetch(chunks - 1);
     for (uint32_t c = chunks; c-- > 0;) {
         const Lane l = Lane::fresh();
         const uint32_t vc = 16 * wave + l.col;  // the lane's column of V, and of K
+        const Gates& gates = s.gates[c & 1];
         const uint32_t left = a.ticks - c * C;  // ticks from the chunk's first
-        piece_to_ordered(s.k + row * ST, col, pk);
-        piece_to_ordered(s.q + row * ST, col, pq);
-        piece_to_ordered(s.d_o + row * ST, col, po);
-        if (wave == 0) put_gates(s.gates, gate);
+        const bool in = c * C + row < a.ticks;
+        piece_to_ordered(s.k + row * ST, col, mask_piece<E, WIDE>(pk, kd, col, in));
+        piece_to_ordered(s.q + row * ST, col, mask_piece<E, WIDE>(pq, kd, col, in));
+        piece_to_ordered(s.d_o + row * ST, col, mask_piece<E, WIDE>(po, vd, col, in));
         // S and V, in result layout
         f32x4 st[KT], x[2];
         if (c > 0) {
@@ -139,15 +130,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 if (16 * i < int(kd) && 16 * wave < int(vd)) st[i] = p[64 * i + lane];
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < KT; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint32_t kr = 16 * i + 4 * l.quad + r;
-                    const bool in = kr < kd && vc < vd;
-                    const float y = a.state ? a.state[seq * kd * vd + (in ? kr * vd + vc : 0u)] : 0.0f;
-                    st[i][r] = in ? y : 0.0f;
-                }
+            load_state(st, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, l, vc);
         }
 #pragma unroll
         for (int i = 0; i < 2; i++)
@@ -172,13 +155,13 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 mma(kk, ordered_row(l, s.k, ST, i0, y), kj);
                 mma(qk, ordered_row(l, s.q, ST, i0, y), kj);
             }
-            dec = decay_tile(l, s.gates, i0, j0);
+            dec = decay_tile(l, gates, i0, j0);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = i0 + 4 * l.quad + r;
                 if (i <= j0 + l.col) kk[r] = 0.0f;
                 kk[r] *= dec[r];
-                am[r] = s.gates.beta[i] * kk[r];
+                am[r] = gates.beta[i] * kk[r];
                 pm[r] = a.scale * dec[r] * qk[r];
             }
             put_tile(l, s.sys.scores, CP, SP, j0, i0, pm);
@@ -186,6 +169,10 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 solve_diagonal(l, s.sys, wave, am);
             else
                 put_tile(l, s.sys.inv, CP, SP, 0, 16, am);
+        }
+        if (wave == Shared::W - 1 && c > 0) {
+            put_gates(s.gates[(c - 1) & 1], gate);
+            if (c > 1) fetch_gates(c - 2);
         }
         // X, and the part of dU through G
         f32x4 dr[2] = {zero, zero}, du[2] = {zero, zero};
@@ -207,9 +194,9 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int t = 16 * i + 4 * l.quad + e;
-                    x[i][e] -= s.gates.before[t] * ks[i][e];
-                    dr[i][e] = s.gates.beta[t] * x[i][e];
-                    du[i][e] *= s.gates.after[t];
+                    x[i][e] -= gates.before[t] * ks[i][e];
+                    dr[i][e] = gates.beta[t] * x[i][e];
+                    du[i][e] *= gates.after[t];
                 }
         }
         if (HALVES == 1 || 16 * wave < VH)
@@ -220,9 +207,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
         for (int i = 0; i < KT; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) dot = fmaf(st[i][r], g[i][r], dot);
-        dot = sum16(dot);
-        dot += __shfl_xor(dot, 16);
-        dot += __shfl_xor(dot, 32);
+        dot = sum_rows32(sum_rows16(sum16(dot)));
         if (lane == 0) s.dot[wave] = dot;
         __syncthreads();
 
@@ -246,11 +231,11 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 const uint32_t t = 16 * i + 4 * l.quad + e;
                 const float sum = sum16(dr[i][e] * x[i][e]);
                 if (l.col == 0) s.beta_v[wave][t] = sum;
-                const float beta = s.gates.beta[t];
+                const float beta = gates.beta[t];
                 if (t < left && vc < vd)
                     reinterpret_cast<E*>(d.d_v.p)[int64_t(c * C + t) * d.d_v.tick + n * d.d_v.env + h * d.d_v.head + vc] =
                         E(beta * dr[i][e]);
-                dr[i][e] *= beta * s.gates.before[t];  // from here on gamma beta R
+                dr[i][e] *= beta * gates.before[t];  // from here on gamma beta R
             }
         __syncthreads();
 
@@ -271,18 +256,14 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 const float m = dp[r] * pm[r] + da[r] * am[r];
                 m_row[r] = double(m);
                 m_col += double(m);
-                float b = da[r] * kk[r];
-#pragma unroll
-                for (int y = 1; y < 16; y <<= 1) {
-                    m_row[r] += __shfl_xor(m_row[r], y);
-                    b += __shfl_xor(b, y);
-                }
+                m_row[r] = sum16(m_row[r]);
+                const float b = sum16(da[r] * kk[r]);
                 if (l.col == 0) {
                     s.m_row[wave][4 * l.quad + r] = m_row[r];
                     s.beta_a[wave][4 * l.quad + r] = b;
                 }
                 dp[r] *= a.scale * dec[r];
-                da[r] *= s.gates.beta[i] * dec[r];
+                da[r] *= gates.beta[i] * dec[r];
             }
             m_col += __shfl_xor(m_col, 16);
             m_col += __shfl_xor(m_col, 32);
@@ -333,10 +314,10 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 const int t = 16 * i + 4 * l.quad + e;
                 const int at = t * ST + place(16 * wave) + 8 * (l.col >> 2) + (l.col & 3);
                 const float qv = float(s.q[at]), kv = float(s.k[at]);
-                const float before = s.gates.before[t];
+                const float before = gates.before[t];
                 dq[i][e] *= a.scale * before;
-                dk[i][e] *= -s.gates.beta[t] * before;
-                dkg[i][e] *= s.gates.after[t];
+                dk[i][e] *= -gates.beta[t] * before;
+                dkg[i][e] *= gates.after[t];
                 const float pa = sum16(fmaf(qv, dq[i][e], kv * dk[i][e])), pb = sum16(kv * dkg[i][e]);
                 if (l.col == 0) {
                     s.a[wave][t] = pa;
@@ -369,13 +350,13 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 }
         // G before the chunk
         {
-            const float total = s.gates.before[C - 1];
+            const float total = gates.before[C - 1];
             const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
             f32x4 lo, hi;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                lo[e] = a.scale * s.gates.before[4 * l.quad + e] * first_term(of, e);
-                hi[e] = a.scale * s.gates.before[16 + 4 * l.quad + e] * first_term(of, 4 + e);
+                lo[e] = a.scale * gates.before[4 * l.quad + e] * first_term(of, e);
+                hi[e] = a.scale * gates.before[16 + 4 * l.quad + e] * first_term(of, 4 + e);
             }
             const auto of2 = frag_of<E>(lo, hi);
             const auto rf = frag_of<E>(-dr[0], -dr[1]);
@@ -410,7 +391,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 if (t >= y) before += up;
             }
             before -= double(pb);
-            const float dg = gate_is_flag(s.gates, t) ? 0.0f : float(after + before + double(s.gates.before[C - 1]) * double(all));
+            const float dg = gate_is_flag(gates, t) ? 0.0f : float(after + before + double(gates.before[C - 1]) * double(all));
             if (lane < C && uint32_t(t) < left) {
                 const int64_t at = int64_t(c * C + t);
                 put_gate(a, d.d_g, at * d.d_g.tick + n * d.d_g.env + h * d.d_g.head, dg, bf);
@@ -420,17 +401,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     }
     if (d.d_state) {
         const Lane l = Lane::fresh();
-        const uint32_t vc = 16 * wave + l.col;
-        if (vc < vd) {
-            float* p = d.d_state + seq * kd * vd + vc;
-#pragma unroll
-            for (int i = 0; i < KT; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint32_t kr = 16 * i + 4 * l.quad + r;
-                    if (kr < kd) p[kr * vd] = g[i][r];
-                }
-        }
+        store_state(d.d_state + seq * kd * vd, g, kd, vd, l, 16 * wave + l.col);
     }
 }
 
