@@ -18,7 +18,6 @@ struct Args {
     uint32_t inner_count, width;
     uint32_t gate_kind, gate_f32;
     float eps;
-    uint32_t wide;  // every row starts at a multiple of 16 bytes
     Rows x, y, gate, s, h;
     const float *w_post, *w_pre, *residual;  // residual may be null (ones)
     float* stats;                            // [rows][2]: 1 / rms of y and of s; null in a forward call without gradients

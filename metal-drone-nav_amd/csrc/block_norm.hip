@@ -28,69 +28,90 @@ __device__ __forceinline__ int64_t row_at(const Rows& r, const Args& a, uint64_t
     return int64_t(row / a.inner_count) * r.outer + int64_t(row % a.inner_count) * r.inner;
 }
 
-// Where a lane's elements are.  VEC (widths of whole pieces): pieces of W
-// neighbours, moved in 16-byte words if all rows are aligned to them (`wide`)
-// and one by one if not, so that alignment does not change the order of a sum;
-// otherwise neighbouring lanes have neighbouring elements.
-template <int W, bool VEC>
-__device__ __forceinline__ uint32_t place(uint32_t p, uint32_t e, uint32_t lane, uint32_t group) {
-    return VEC ? (p * group + lane) * W + e : (p * W + e) * group + lane;
-}
+// A lane's elements: P pieces of W neighbours, a piece per lane and then the
+// next ones.  A piece moves in 16-byte words at whatever address the row
+// starts (global memory takes words at any multiple of the element's size);
+// the piece that the row ends in moves one element at a time.
+template <int W> __device__ __forceinline__ uint32_t place(uint32_t p, uint32_t lane, uint32_t group) { return (p * group + lane) * W; }
 
-template <class T, int P, int W, bool VEC>
-__device__ __forceinline__ void load(float (&out)[P][W], const T* row, uint32_t lane, uint32_t group, uint32_t width, bool wide) {
+typedef uint32_t Word __attribute__((ext_vector_type(4)));
+template <class T> struct Words;
+template <> struct Words<float> { typedef Word type __attribute__((aligned(4))); };
+template <> struct Words<bf16> { typedef Word type __attribute__((aligned(2))); };
+
+// A lane's part of a row as it is in memory: loaded a row ahead, and turned
+// into fp32 where it is used (that costs an instruction each time and saves
+// half of the registers).  Elements past the row's end are 0.
+template <class T, int P, int W> struct Raw { Word w[P][W * sizeof(T) / 16]; };
+
+template <class T, int P, int W>
+__device__ __forceinline__ void fetch(Raw<T, P, W>& out, const T* row, uint32_t lane, uint32_t group, uint32_t width) {
+    constexpr int N = W * sizeof(T) / 16, PER = 16 / sizeof(T);
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        if (VEC && wide) {
-            constexpr int PER = 16 / sizeof(T);
-            const uint32_t at = place<W, true>(p, 0, lane, group);
-            const bool in = at < width;
-            const T* q = row + (in ? at : 0u);
+        const uint32_t at = place<W>(p, lane, group);
+        if (at + W <= width) {
 #pragma unroll
-            for (int w = 0; w < W; w += PER) {
-                union { uint4 u; T t[PER]; } v;
-                v.u = *reinterpret_cast<const uint4*>(q + w);
-#pragma unroll
-                for (int e = 0; e < PER; e++) out[p][w + e] = in ? float(v.t[e]) : 0.0f;
-            }
+            for (int w = 0; w < N; w++) out.w[p][w] = *reinterpret_cast<const typename Words<T>::type*>(row + at + w * PER);
         } else {
 #pragma unroll
-            for (int e = 0; e < W; e++) {
-                const uint32_t at = place<W, VEC>(p, e, lane, group);
-                const float v = float(row[at < width ? at : 0u]);
-                out[p][e] = at < width ? v : 0.0f;
-            }
+            for (int w = 0; w < N; w++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t c = at + w * PER + i * (4 / sizeof(T));
+                    uint32_t bits = 0;
+                    if (sizeof(T) == 4) {
+                        if (c < width) bits = reinterpret_cast<const uint32_t*>(row)[c];
+                    } else {
+                        if (c < width) bits = reinterpret_cast<const uint16_t*>(row)[c];
+                        if (c + 1 < width) bits |= uint32_t(reinterpret_cast<const uint16_t*>(row)[c + 1]) << 16;
+                    }
+                    out.w[p][w][i] = bits;
+                }
         }
     }
 }
-template <class T, int P, int W, bool VEC>
-__device__ __forceinline__ void store(T* row, const float (&in)[P][W], uint32_t lane, uint32_t group, uint32_t width, bool wide) {
+// Element e of piece p in fp32.
+template <class T, int P, int W>
+__device__ __forceinline__ float value(const Raw<T, P, W>& in, int p, int e) {
+    if (sizeof(T) == 2) {
+        const uint32_t pair = in.w[p][e / 8][e / 2 % 4];
+        return __builtin_bit_cast(float, e % 2 ? pair & 0xffff0000u : pair << 16);
+    }
+    return __builtin_bit_cast(float, uint32_t(in.w[p][e / 4][e % 4]));
+}
+template <class T, int P, int W>
+__device__ __forceinline__ void load(float (&out)[P][W], const T* row, uint32_t lane, uint32_t group, uint32_t width) {
+    Raw<T, P, W> raw;
+    fetch<T, P, W>(raw, row, lane, group, width);
 #pragma unroll
-    for (int p = 0; p < P; p++) {
-        if (VEC && wide) {
-            constexpr int PER = 16 / sizeof(T);
-            const uint32_t at = place<W, true>(p, 0, lane, group);
-            if (at >= width) continue;
+    for (int p = 0; p < P; p++)
 #pragma unroll
-            for (int w = 0; w < W; w += PER) {
-                union { uint4 u; T t[PER]; } v;
+        for (int e = 0; e < W; e++) out[p][e] = value(raw, p, e);
+}
+// One piece.
+template <class T, int W>
+__device__ __forceinline__ void store(T* row, const float (&in)[W], uint32_t at, uint32_t width) {
+    constexpr int N = W * sizeof(T) / 16, PER = 16 / sizeof(T);
+    if (at + W <= width) {
 #pragma unroll
-                for (int e = 0; e < PER; e++) v.t[e] = T(in[p][w + e]);
-                *reinterpret_cast<uint4*>(row + at + w) = v.u;
-            }
-        } else {
+        for (int w = 0; w < N; w++) {
+            union { Word u; T t[PER]; } v;
 #pragma unroll
-            for (int e = 0; e < W; e++) {
-                const uint32_t at = place<W, VEC>(p, e, lane, group);
-                if (at < width) row[at] = T(in[p][e]);
-            }
+            for (int e = 0; e < PER; e++) v.t[e] = T(in[w * PER + e]);
+            *reinterpret_cast<typename Words<T>::type*>(row + at + w * PER) = v.u;
         }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < W; e++)
+            if (at + e < width) row[at + e] = T(in[e]);
     }
 }
 
-// Sums over a row's lanes.  G 0: the whole workgroup, through LDS.
+// Sums over a row's lanes.  G 0: the whole workgroup, through LDS; `lds` is
+// another one than the last sum's, so that one barrier is enough.
 template <int G, int N, class A>
-__device__ __forceinline__ void row_sum(A (&v)[N], A (*lds)[N]) {
+__device__ __forceinline__ void row_sum(A (&v)[N], A (*lds)[2]) {
     constexpr int IN_WAVE = G == 0 ? 64 : G;
 #pragma unroll
     for (int d = 1; d < IN_WAVE; d <<= 1)
@@ -98,7 +119,6 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A (*lds)[N]) {
         for (int i = 0; i < N; i++) v[i] += __shfl_xor(v[i], d);
     if (G == 0) {
         const uint32_t waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
-        __syncthreads();  // the last sum's readers are done
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int i = 0; i < N; i++) lds[wave][i] = v[i];
@@ -111,61 +131,140 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A (*lds)[N]) {
     }
 }
 
+// The channels' vectors: in registers for the whole call where a row has at
+// most a wavefront's lanes, else in LDS (a workgroup's rows share them, and
+// the registers are needed for the row and for the next one).
+template <int G, int P, int W> struct Channels {
+    float v[P][W];
+    __device__ __forceinline__ void init(const float* from, float*, uint32_t lane, uint32_t group, uint32_t width) {
+        load<float, P, W>(v, from, lane, group, width);
+    }
+    __device__ __forceinline__ float at(int p, int e, const float*, uint32_t, uint32_t) const { return v[p][e]; }
+};
+template <int P, int W> struct Channels<0, P, W> {
+    __device__ __forceinline__ void init(const float* from, float* lds, uint32_t lane, uint32_t group, uint32_t width) {
+        float v[P][W];
+        load<float, P, W>(v, from, lane, group, width);
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int e = 0; e < W; e++) lds[place<W>(p, lane, group) + e] = v[p][e];
+    }
+    __device__ __forceinline__ float at(int p, int e, const float* lds, uint32_t lane, uint32_t group) const {
+        return lds[place<W>(p, lane, group) + e];
+    }
+};
+
 template <class TY>
 __device__ __forceinline__ float one_gate(const Args& a, int64_t at) {
     return a.gate_f32 ? reinterpret_cast<const float*>(a.gate.p)[at] : float(reinterpret_cast<const TY*>(a.gate.p)[at]);
 }
 
-template <class TX, class TY, int G, int P, int W, bool VEC, int GATE>
-__global__ void __launch_bounds__(G == 0 ? 1024 : 256) forward_kernel(Args a) {
-    __shared__ float lds[16][1];
+// One row's inputs as loaded.
+template <class TX, class TY, int P, int W, int GATE> struct Inputs {
+    Raw<TX, P, W> x;
+    Raw<TY, P, W> y, gate;
+    float one;  // the row's gate
+    __device__ __forceinline__ void fetch_row(const Args& a, uint64_t row, uint32_t lane, uint32_t group) {
+        fetch<TY, P, W>(y, reinterpret_cast<const TY*>(a.y.p) + row_at(a.y, a, row), lane, group, a.width);
+        fetch<TX, P, W>(x, reinterpret_cast<const TX*>(a.x.p) + row_at(a.x, a, row), lane, group, a.width);
+        if (GATE == ELEMENT)
+            fetch<TY, P, W>(gate, reinterpret_cast<const TY*>(a.gate.p) + row_at(a.gate, a, row), lane, group, a.width);
+        one = GATE == ROW ? one_gate<TY>(a, row_at(a.gate, a, row)) : 1.0f;
+    }
+};
+// The channels' vectors, with the gate's if it is one.
+template <class TX, class TY, int G, int P, int W, int GATE> struct Weights {
+    Channels<G, P, W> post, pre, residual;
+    float gate[P][W];
+    float* lds;
+    uint32_t size, lane, group;
+    bool scaled;
+    __device__ __forceinline__ void init(const Args& a, float* shared, uint32_t l, uint32_t g) {
+        lds = shared;
+        lane = l;
+        group = g;
+        size = g * P * W;
+        scaled = a.residual != nullptr;
+        post.init(a.w_post, lds, l, g, a.width);
+        pre.init(a.w_pre, lds + size, l, g, a.width);
+        if (scaled) residual.init(a.residual, lds + 2 * size, l, g, a.width);
+        if (GATE == CHANNEL) {
+            if (a.gate_f32)
+                load<float, P, W>(gate, reinterpret_cast<const float*>(a.gate.p), l, g, a.width);
+            else
+                load<TY, P, W>(gate, reinterpret_cast<const TY*>(a.gate.p), l, g, a.width);
+        }
+        // (a lane reads back only what it wrote: no barrier)
+    }
+    __device__ __forceinline__ float post_at(int p, int e) const { return post.at(p, e, lds, lane, group); }
+    __device__ __forceinline__ float pre_at(int p, int e) const { return pre.at(p, e, lds + size, lane, group); }
+    __device__ __forceinline__ float residual_at(int p, int e) const { return residual.at(p, e, lds + 2 * size, lane, group); }
+    typedef Inputs<TX, TY, P, W, GATE> In;
+    __device__ __forceinline__ float gate_at(const In& in, int p, int e) const {
+        return GATE == NONE ? 1.0f : GATE == ROW ? in.one : GATE == ELEMENT ? value(in.gate, p, e) : gate[p][e];
+    }
+    // s from b = y / rms(y) w_post
+    __device__ __forceinline__ float s(const In& in, int p, int e, float b) const {
+        const float gb = GATE == NONE ? b : gate_at(in, p, e) * b, x = value(in.x, p, e);
+        return scaled ? fmaf(residual_at(p, e), x, gb) : x + gb;
+    }
+};
+
+// A wavefront whose lanes share rows has a row in scalar registers.
+template <int G> __device__ __forceinline__ uint32_t row_in_group() {
+    if (G == 0) return 0;
+    const uint32_t r = threadIdx.x / G;
+    return G == 64 ? __builtin_amdgcn_readfirstlane(r) : r;
+}
+
+template <class TX, class TY, int G, int P, int W, int GATE>
+__global__ void __launch_bounds__(G == 0 ? 512 : 256) forward_kernel(Args a) {
+    __shared__ float lds[2][8][2];
+    extern __shared__ __align__(16) float channels[];
     const uint32_t group = G == 0 ? blockDim.x : G, per = G == 0 ? 1 : 256 / G;
     const uint32_t lane = threadIdx.x % group, width = a.width;
-    float wp[P][W], wq[P][W], res[P][W], gate[P][W];
-    load<float, P, W, VEC>(wp, a.w_post, lane, group, width, a.wide);
-    load<float, P, W, VEC>(wq, a.w_pre, lane, group, width, a.wide);
-    if (a.residual) load<float, P, W, VEC>(res, a.residual, lane, group, width, a.wide);
-    if (GATE == CHANNEL) {
-        if (a.gate_f32)
-            load<float, P, W, VEC>(gate, reinterpret_cast<const float*>(a.gate.p), lane, group, width, a.wide);
-        else
-            load<TY, P, W, VEC>(gate, reinterpret_cast<const TY*>(a.gate.p), lane, group, width, a.wide);
-    }
+    Weights<TX, TY, G, P, W, GATE> wt;
+    wt.init(a, channels, lane, group);
     const uint64_t step = uint64_t(gridDim.x) * per;
-    for (uint64_t first = uint64_t(blockIdx.x) * per; first < a.rows; first += step) {
-        const uint64_t mine = first + (G == 0 ? 0 : threadIdx.x / group);
-        const uint64_t row = mine < a.rows ? mine : a.rows - 1;  // lanes past the end repeat the last row's loads
-        float x[P][W], y[P][W];
-        load<TY, P, W, VEC>(y, reinterpret_cast<const TY*>(a.y.p) + row_at(a.y, a, row), lane, group, width, a.wide);
-        load<TX, P, W, VEC>(x, reinterpret_cast<const TX*>(a.x.p) + row_at(a.x, a, row), lane, group, width, a.wide);
-        if (GATE == ELEMENT) load<TY, P, W, VEC>(gate, reinterpret_cast<const TY*>(a.gate.p) + row_at(a.gate, a, row), lane, group, width, a.wide);
-        const float gr = GATE == ROW ? one_gate<TY>(a, row_at(a.gate, a, row)) : 1.0f;
+    Inputs<TX, TY, P, W, GATE> now, next;
+    const uint64_t mine0 = uint64_t(blockIdx.x) * per + row_in_group<G>();
+    // lanes past the end repeat the last row's loads
+    next.fetch_row(a, mine0 < a.rows ? mine0 : a.rows - 1, lane, group);
+    for (uint64_t mine = mine0, first = uint64_t(blockIdx.x) * per; first < a.rows; first += step, mine += step) {
+        const uint64_t row = mine < a.rows ? mine : a.rows - 1;
+        now = next;
+        if (first + step < a.rows) next.fetch_row(a, mine + step < a.rows ? mine + step : a.rows - 1, lane, group);
         float sum[1] = {0.0f};
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
-            for (int e = 0; e < W; e++) sum[0] = fmaf(y[p][e], y[p][e], sum[0]);
-        row_sum<G>(sum, lds);
+            for (int e = 0; e < W; e++) {
+                const float y = value(now.y, p, e);
+                sum[0] = fmaf(y, y, sum[0]);
+            }
+        row_sum<G>(sum, lds[0]);
         const float ry = 1.0f / sqrtf(sum[0] / float(width) + a.eps);
         sum[0] = 0.0f;
+        float s[P][W];
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int e = 0; e < W; e++) {
-                const float b = y[p][e] * ry * wp[p][e];
-                const float gb = GATE == NONE ? b : (GATE == ROW ? gr : gate[p][e]) * b;
-                x[p][e] = a.residual ? fmaf(res[p][e], x[p][e], gb) : x[p][e] + gb;
-                sum[0] = fmaf(x[p][e], x[p][e], sum[0]);
+                s[p][e] = wt.s(now, p, e, value(now.y, p, e) * ry * wt.post_at(p, e));
+                sum[0] = fmaf(s[p][e], s[p][e], sum[0]);
             }
-        row_sum<G>(sum, lds);
+        row_sum<G>(sum, lds[1]);
         const float rs = 1.0f / sqrtf(sum[0] / float(width) + a.eps);
         if (mine < a.rows) {
-            store<TX, P, W, VEC>(reinterpret_cast<TX*>(a.s.p) + row_at(a.s, a, row), x, lane, group, width, a.wide);
 #pragma unroll
-            for (int p = 0; p < P; p++)
+            for (int p = 0; p < P; p++) {
+                const uint32_t at = place<W>(p, lane, group);
+                store<TX, W>(reinterpret_cast<TX*>(a.s.p) + row_at(a.s, a, row), s[p], at, width);
 #pragma unroll
-                for (int e = 0; e < W; e++) x[p][e] = x[p][e] * rs * wq[p][e];
-            store<TY, P, W, VEC>(reinterpret_cast<TY*>(a.h.p) + row_at(a.h, a, row), x, lane, group, width, a.wide);
+                for (int e = 0; e < W; e++) s[p][e] = s[p][e] * rs * wt.pre_at(p, e);
+                store<TY, W>(reinterpret_cast<TY*>(a.h.p) + row_at(a.h, a, row), s[p], at, width);
+            }
             if (a.stats && lane == 0) {
                 a.stats[2 * row] = ry;
                 a.stats[2 * row + 1] = rs;
@@ -181,55 +280,48 @@ __global__ void __launch_bounds__(G == 0 ? 1024 : 256) forward_kernel(Args a) {
 template <int G> struct Sum { typedef float type; };
 template <> struct Sum<16> { typedef double type; };
 
-template <class TX, class TY, int G, int P, int W, bool VEC, int GATE>
-__global__ void __launch_bounds__(G == 0 ? 1024 : 256) backward_kernel(Args a, GradArgs d) {
+template <class TX, class TY, int G, int P, int W, int GATE>
+__global__ void __launch_bounds__(G == 0 ? 512 : 256) backward_kernel(Args a, GradArgs d) {
     typedef typename Sum<G>::type A;
     constexpr int SUMS = GATE == ROW ? 2 : 1;
-    __shared__ A lds[16][2];
-    extern __shared__ float columns[];
+    __shared__ A lds[2][8][2];
+    extern __shared__ __align__(16) float channels[];
     const uint32_t group = G == 0 ? blockDim.x : G, per = G == 0 ? 1 : 256 / G;
     const uint32_t lane = threadIdx.x % group, width = a.width;
-    float wp[P][W], wq[P][W], res[P][W], gate[P][W];
+    // column sums of t gate n, dh s / rms(s), t x, t n w_post
     float c_post[P][W] = {}, c_pre[P][W] = {}, c_res[P][W] = {}, c_gate[P][W] = {};
-    load<float, P, W, VEC>(wp, a.w_post, lane, group, width, a.wide);
-    load<float, P, W, VEC>(wq, a.w_pre, lane, group, width, a.wide);
-    if (a.residual) load<float, P, W, VEC>(res, a.residual, lane, group, width, a.wide);
-    if (GATE == CHANNEL) {
-        if (a.gate_f32)
-            load<float, P, W, VEC>(gate, reinterpret_cast<const float*>(a.gate.p), lane, group, width, a.wide);
-        else
-            load<TY, P, W, VEC>(gate, reinterpret_cast<const TY*>(a.gate.p), lane, group, width, a.wide);
-    }
+    Weights<TX, TY, G, P, W, GATE> wt;
+    wt.init(a, channels, lane, group);
     const uint64_t step = uint64_t(gridDim.x) * per;
-    for (uint64_t first = uint64_t(blockIdx.x) * per; first < a.rows; first += step) {
-        const uint64_t mine = first + (G == 0 ? 0 : threadIdx.x / group);
+    struct Row {
+        Inputs<TX, TY, P, W, GATE> in;
+        Raw<TX, P, W> ds;
+        Raw<TY, P, W> dh;
+        float ry, rs;
+    } now = {}, next = {};
+    const auto fetch_row = [&](Row& to, uint64_t mine) {
+        const uint64_t row = mine < a.rows ? mine : a.rows - 1;  // lanes past the end repeat the last row's loads
+        to.in.fetch_row(a, row, lane, group);
+        if (d.d_h.p) fetch<TY, P, W>(to.dh, reinterpret_cast<const TY*>(d.d_h.p) + row_at(d.d_h, a, row), lane, group, width);
+        if (d.d_s.p) fetch<TX, P, W>(to.ds, reinterpret_cast<const TX*>(d.d_s.p) + row_at(d.d_s, a, row), lane, group, width);
+        to.ry = a.stats[2 * row];
+        to.rs = a.stats[2 * row + 1];
+    };
+    const uint64_t mine0 = uint64_t(blockIdx.x) * per + row_in_group<G>();
+    fetch_row(next, mine0);
+    for (uint64_t mine = mine0, first = uint64_t(blockIdx.x) * per; first < a.rows; first += step, mine += step) {
         const bool in = mine < a.rows;
         const uint64_t row = in ? mine : a.rows - 1;
-        float x[P][W], y[P][W], dh[P][W], t[P][W];
-        load<TY, P, W, VEC>(y, reinterpret_cast<const TY*>(a.y.p) + row_at(a.y, a, row), lane, group, width, a.wide);
-        load<TX, P, W, VEC>(x, reinterpret_cast<const TX*>(a.x.p) + row_at(a.x, a, row), lane, group, width, a.wide);
-        if (GATE == ELEMENT) load<TY, P, W, VEC>(gate, reinterpret_cast<const TY*>(a.gate.p) + row_at(a.gate, a, row), lane, group, width, a.wide);
-        if (d.d_h.p)
-            load<TY, P, W, VEC>(dh, reinterpret_cast<const TY*>(d.d_h.p) + row_at(d.d_h, a, row), lane, group, width, a.wide);
-        if (d.d_s.p)
-            load<TX, P, W, VEC>(t, reinterpret_cast<const TX*>(d.d_s.p) + row_at(d.d_s, a, row), lane, group, width, a.wide);
-#pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int e = 0; e < W; e++) {
-                if (!d.d_h.p) dh[p][e] = 0.0f;
-                if (!d.d_s.p) t[p][e] = 0.0f;
-            }
-        const float gr = GATE == ROW ? one_gate<TY>(a, row_at(a.gate, a, row)) : 1.0f;
-        A ry = a.stats[2 * row], rs = a.stats[2 * row + 1];
-        const float keep = in ? 1.0f : 0.0f;
+        now = next;
+        if (first + step < a.rows) fetch_row(next, mine + step);
+        A ry = now.ry, rs = now.rs;
         if (G == 16) {
             A squares[1] = {0};
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
-                for (int e = 0; e < W; e++) squares[0] += A(y[p][e]) * A(y[p][e]);
-            row_sum<G>(squares, reinterpret_cast<A(*)[1]>(lds));
+                for (int e = 0; e < W; e++) squares[0] += A(value(now.in.y, p, e)) * A(value(now.in.y, p, e));
+            row_sum<G>(squares, lds[0]);
             ry = A(1) / sqrt(squares[0] / A(width) + A(a.eps));
         }
         const float ryf = float(ry);
@@ -238,48 +330,51 @@ __global__ void __launch_bounds__(G == 0 ? 1024 : 256) backward_kernel(Args a, G
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int e = 0; e < W; e++) {
-                const float b = y[p][e] * ryf * wp[p][e];
-                const float gb = GATE == NONE ? b : (GATE == ROW ? gr : gate[p][e]) * b;
-                const float s = a.residual ? fmaf(res[p][e], x[p][e], gb) : x[p][e] + gb;
-                sum[0] += A(dh[p][e] * wq[p][e]) * A(s);
+                const float s = wt.s(now.in, p, e, value(now.in.y, p, e) * ryf * wt.post_at(p, e));
+                sum[0] += A(value(now.dh, p, e) * wt.pre_at(p, e)) * A(s);
                 if (G == 16) sum[G == 16 ? 1 : 0] += A(s) * A(s);
+                if (P > 1 && e == W - 1) asm volatile("" : "+v"(sum[0])::"memory");  // the next piece's channels are read after this one's use
             }
-        row_sum<G>(sum, reinterpret_cast<A(*)[G == 16 ? 2 : 1]>(lds));
+        row_sum<G>(sum, lds[0]);
         if (G == 16) rs = A(1) / sqrt(sum[G == 16 ? 1 : 0] / A(width) + A(a.eps));
-        const float rsf = float(rs);
+        const float rsf = float(rs), keep = in ? 1.0f : 0.0f;
         const A back = sum[0] / A(width) * rs * rs * rs;
         A sums[SUMS] = {};
-        float dgate[P][W];
+        float dn[P][W];
 #pragma unroll
-        for (int p = 0; p < P; p++)
+        for (int p = 0; p < P; p++) {
+            float out[W], dgate[W];
 #pragma unroll
             for (int e = 0; e < W; e++) {
-                const float nn = y[p][e] * ryf, b = nn * wp[p][e];
-                const float gv = GATE == NONE ? 1.0f : GATE == ROW ? gr : gate[p][e];
-                const float gb = GATE == NONE ? b : gv * b;
-                const float s = a.residual ? fmaf(res[p][e], x[p][e], gb) : x[p][e] + gb;
-                const float all = float(A(t[p][e]) + (rs * A(dh[p][e] * wq[p][e]) - back * A(s)));
-                c_pre[p][e] = fmaf(keep * dh[p][e], s * rsf, c_pre[p][e]);
-                c_post[p][e] = fmaf(keep * all, gv * nn, c_post[p][e]);
-                c_res[p][e] = fmaf(keep * all, x[p][e], c_res[p][e]);
-                if (GATE == CHANNEL) c_gate[p][e] = fmaf(keep * all, b, c_gate[p][e]);
-                if (GATE == ELEMENT) dgate[p][e] = all * b;
-                if (GATE == ROW) sums[SUMS - 1] += A(all) * A(b);
-                x[p][e] = a.residual ? res[p][e] * all : all;
-                const float dn = all * gv * wp[p][e];
-                t[p][e] = dn;
-                sums[0] += A(dn) * A(y[p][e]);
+                const float y = value(now.in.y, p, e), x = value(now.in.x, p, e), dh = value(now.dh, p, e);
+                const float n = y * ryf, w = wt.post_at(p, e), b = n * w, s = wt.s(now.in, p, e, b), gv = wt.gate_at(now.in, p, e);
+                const float t = float(A(value(now.ds, p, e)) + (rs * A(dh * wt.pre_at(p, e)) - back * A(s)));
+                c_pre[p][e] = fmaf(keep * dh, s * rsf, c_pre[p][e]);
+                c_post[p][e] = fmaf(keep * t, gv * n, c_post[p][e]);
+                c_res[p][e] = fmaf(keep * t, x, c_res[p][e]);
+                if (GATE == CHANNEL) c_gate[p][e] = fmaf(keep * t, b, c_gate[p][e]);
+                if (GATE == ELEMENT) dgate[e] = t * b;
+                if (GATE == ROW) sums[SUMS - 1] += A(t) * A(b);
+                out[e] = wt.scaled ? wt.residual_at(p, e) * t : t;
+                dn[p][e] = t * gv * w;
+                sums[0] += A(dn[p][e]) * A(y);
             }
-        row_sum<G>(sums, reinterpret_cast<A(*)[SUMS]>(lds));
+            if (in) {
+                const uint32_t at = place<W>(p, lane, group);
+                store<TX, W>(reinterpret_cast<TX*>(d.d_x.p) + row_at(d.d_x, a, row), out, at, width);
+                if (GATE == ELEMENT) store<TY, W>(reinterpret_cast<TY*>(d.d_gate.p) + row_at(d.d_gate, a, row), dgate, at, width);
+            }
+            if (P > 1) asm volatile("" : "+v"(sums[0])::"memory");
+        }
+        row_sum<G>(sums, lds[1]);
         const A pull = sums[0] / A(width) * ry * ry * ry;
         if (in) {
 #pragma unroll
-            for (int p = 0; p < P; p++)
+            for (int p = 0; p < P; p++) {
 #pragma unroll
-                for (int e = 0; e < W; e++) y[p][e] = float(ry * A(t[p][e]) - pull * A(y[p][e]));
-            store<TX, P, W, VEC>(reinterpret_cast<TX*>(d.d_x.p) + row_at(d.d_x, a, row), x, lane, group, width, a.wide);
-            store<TY, P, W, VEC>(reinterpret_cast<TY*>(d.d_y.p) + row_at(d.d_y, a, row), y, lane, group, width, a.wide);
-            if (GATE == ELEMENT) store<TY, P, W, VEC>(reinterpret_cast<TY*>(d.d_gate.p) + row_at(d.d_gate, a, row), dgate, lane, group, width, a.wide);
+                for (int e = 0; e < W; e++) dn[p][e] = float(ry * A(dn[p][e]) - pull * A(value(now.in.y, p, e)));
+                store<TY, W>(reinterpret_cast<TY*>(d.d_y.p) + row_at(d.d_y, a, row), dn[p], place<W>(p, lane, group), width);
+            }
             if (GATE == ROW && lane == 0) {
                 const int64_t at = row_at(d.d_gate, a, row);
                 if (a.gate_f32)
@@ -290,9 +385,8 @@ __global__ void __launch_bounds__(G == 0 ? 1024 : 256) backward_kernel(Args a, G
         }
     }
     // the workgroup's column sums: its groups of lanes add theirs up in order
-    float* out = d.parts + uint64_t(blockIdx.x) * 4 * width;
-    for (int c = 0; c < 4; c++) {
-        float(&v)[P][W] = c == 0 ? c_post : c == 1 ? c_pre : c == 2 ? c_res : c_gate;
+    float* parts = d.parts + uint64_t(blockIdx.x) * 4 * width;
+    const auto column_sum = [&](const float(&v)[P][W], float* out) {
         if (G != 0) {
             for (uint32_t r = 0; r < per; r++) {
                 __syncthreads();
@@ -301,36 +395,46 @@ __global__ void __launch_bounds__(G == 0 ? 1024 : 256) backward_kernel(Args a, G
                     for (int p = 0; p < P; p++)
 #pragma unroll
                         for (int e = 0; e < W; e++) {
-                            float& to = columns[place<W, VEC>(p, e, lane, group)];
+                            float& to = channels[place<W>(p, lane, group) + e];
                             to = r ? to + v[p][e] : v[p][e];
                         }
             }
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < width; i += 256) out[uint64_t(c) * width + i] = columns[i];
+            for (uint32_t i = threadIdx.x; i < width; i += 256) out[i] = channels[i];
         } else {
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
-                for (int e = 0; e < W; e++) {
-                    const uint32_t at = place<W, VEC>(p, e, lane, group);
-                    if (at < width) out[uint64_t(c) * width + at] = v[p][e];
-                }
+                for (int e = 0; e < W; e++)
+                    if (place<W>(p, lane, group) + e < width) out[place<W>(p, lane, group) + e] = v[p][e];
         }
-    }
+    };
+    column_sum(c_post, parts);
+    column_sum(c_pre, parts + width);
+    column_sum(c_res, parts + 2 * uint64_t(width));
+    column_sum(c_gate, parts + 3 * uint64_t(width));
 }
 
-// Adds up the workgroups' rows of column sums: 64 columns and 4 quarters of the rows per workgroup.
-__global__ void __launch_bounds__(256) columns_kernel(const float* parts, uint32_t count, uint32_t width, float* post, float* pre,
-                                                      float* res, char* gate, uint32_t gate_f32) {
-    __shared__ float lds[4][64];
-    const uint32_t at = blockIdx.x * 64 + (threadIdx.x & 63), quarter = threadIdx.x >> 6;
-    float sum = 0.0f;
-    if (at < 4 * width)
-        for (uint32_t i = quarter; i < count; i += 4) sum += parts[uint64_t(i) * 4 * width + at];
-    lds[quarter][threadIdx.x & 63] = sum;
+// Adds up the workgroups' rows of column sums: 64 columns per workgroup, a
+// sixteenth of the rows per wavefront, eight loads in flight.
+__global__ void __launch_bounds__(1024) columns_kernel(const float* parts, uint32_t count, uint32_t width, float* post, float* pre,
+                                                       float* res, char* gate, uint32_t gate_f32) {
+    __shared__ float lds[16][64];
+    const uint32_t at = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+    float part[8] = {};
+    if (at < 4 * width) {
+        uint32_t i = slice;
+        for (; i + 7 * 16 < count; i += 8 * 16)
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) part[j] += parts[uint64_t(i + 16 * j) * 4 * width + at];
+        for (uint32_t j = 0; i < count; i += 16, j++) part[j & 7] += parts[uint64_t(i) * 4 * width + at];
+    }
+    lds[slice][threadIdx.x & 63] = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
     __syncthreads();
-    if (quarter != 0 || at >= 4 * width) return;
-    sum = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+    if (slice != 0 || at >= 4 * width) return;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) sum += lds[i][threadIdx.x];
     const uint32_t which = at / width, c = at % width;
     if (which == 0) post[c] = sum;
     if (which == 1) pre[c] = sum;
@@ -343,81 +447,89 @@ __global__ void __launch_bounds__(256) columns_kernel(const float* parts, uint32
     }
 }
 
-// The lanes of a row: pieces of W elements over G lanes, P each.
-struct Shape { uint32_t lanes, pieces; };  // lanes 16, 32, 64, or a workgroup's threads
+// The lanes of a row: one piece of W elements each on a part of a wavefront,
+// one, or a workgroup of at most 512; up to 16 elements a lane in wider rows.
+struct Shape { uint32_t lanes, pieces; };
 inline Shape shape_of(uint32_t width, uint32_t w) {
     const uint32_t pieces = (width + w - 1) / w;
     if (pieces <= 16) return {16, 1};
     if (pieces <= 32) return {32, 1};
     if (pieces <= 64) return {64, 1};
-    if (pieces <= 128) return {64, 2};
-    const uint32_t p = pieces <= 512 ? 1 : 2;
+    const uint32_t p = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
     return {((pieces + p - 1) / p + 63) / 64 * 64, p};
 }
+// Workgroups, each with several rows in turn: enough to fill the GPU's 256 compute units.
 inline uint32_t blocks_of(const Args& a, const Shape& s) {
     const uint64_t per = s.lanes > 64 ? 1 : 256 / s.lanes;
     const uint64_t most = (a.rows + per - 1) / per;
-    const uint64_t full = s.lanes > 64 ? 256 * (s.lanes <= 512 ? 3 : 2) : 1024;
+    const uint64_t full = 256 * (s.lanes > 64 ? (s.lanes * s.pieces <= 256 ? 4 : 2) : 4);
     return uint32_t(most < full ? most : full);
 }
+// LDS for the channels' vectors of a row that takes a workgroup.
+inline uint32_t channel_bytes(const Shape& s, uint32_t w) { return s.lanes > 64 ? 3 * s.lanes * s.pieces * w * 4 : 0; }
 
-template <class TX, class TY, int W, bool VEC, int GATE>
-hipError_t forward(const Args& a, hipStream_t st) {
-    const Shape s = shape_of(a.width, W);
-    const bool block = s.lanes > 64;
-    const uint64_t per = block ? 1 : 256 / s.lanes;
-    const uint64_t rows = (a.rows + per - 1) / per;
-    const dim3 grid(uint32_t(rows < 4096 ? rows : 4096)), wg(256);
-    if (block && s.pieces == 1) forward_kernel<TX, TY, 0, 1, W, VEC, GATE><<<grid, dim3(s.lanes), 0, st>>>(a);
-    else if (block) forward_kernel<TX, TY, 0, 2, W, VEC, GATE><<<grid, dim3(s.lanes), 0, st>>>(a);
-    else if (s.lanes == 16) forward_kernel<TX, TY, 16, 1, W, VEC, GATE><<<grid, wg, 0, st>>>(a);
-    else if (s.lanes == 32) forward_kernel<TX, TY, 32, 1, W, VEC, GATE><<<grid, wg, 0, st>>>(a);
-    else if (s.pieces == 1) forward_kernel<TX, TY, 64, 1, W, VEC, GATE><<<grid, wg, 0, st>>>(a);
-    else forward_kernel<TX, TY, 64, 2, W, VEC, GATE><<<grid, wg, 0, st>>>(a);
+template <class K, class... X>
+hipError_t launch(K kernel, uint32_t blocks, uint32_t threads, uint32_t bytes, hipStream_t st, X... args) {
+    if (bytes > 64 * 1024)
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
+            return e;
+    kernel<<<dim3(blocks), dim3(threads), bytes, st>>>(args...);
     return hipGetLastError();
 }
-template <class TX, class TY, int W, bool VEC, int GATE>
+
+template <class TX, class TY, int W, int GATE>
+hipError_t forward(const Args& a, hipStream_t st) {
+    const Shape s = shape_of(a.width, W);
+    const uint64_t per = s.lanes > 64 ? 1 : 256 / s.lanes;
+    const uint64_t rows = (a.rows + per - 1) / per;
+    const uint32_t most = s.lanes > 64 ? 2 * blocks_of(a, s) : 4096, grid = uint32_t(rows < most ? rows : most), bytes = channel_bytes(s, W);
+    if constexpr (W == 4)
+        if (s.lanes > 64 && s.pieces == 4) return launch(forward_kernel<TX, TY, 0, 4, W, GATE>, grid, s.lanes, bytes, st, a);
+    if (s.lanes > 64 && s.pieces == 2) return launch(forward_kernel<TX, TY, 0, 2, W, GATE>, grid, s.lanes, bytes, st, a);
+    if (s.lanes > 64) return launch(forward_kernel<TX, TY, 0, 1, W, GATE>, grid, s.lanes, bytes, st, a);
+    if (s.lanes == 16) return launch(forward_kernel<TX, TY, 16, 1, W, GATE>, grid, 256, 0, st, a);
+    if (s.lanes == 32) return launch(forward_kernel<TX, TY, 32, 1, W, GATE>, grid, 256, 0, st, a);
+    return launch(forward_kernel<TX, TY, 64, 1, W, GATE>, grid, 256, 0, st, a);
+}
+template <class TX, class TY, int W, int GATE>
 hipError_t backward(const Args& a, const GradArgs& d, hipStream_t st) {
     const Shape s = shape_of(a.width, W);
-    const dim3 grid(blocks_of(a, s)), wg(256);
-    const uint32_t columns = s.lanes > 64 ? 0 : s.lanes * s.pieces * W * 4;
-    if (s.lanes > 64 && s.pieces == 1) backward_kernel<TX, TY, 0, 1, W, VEC, GATE><<<grid, dim3(s.lanes), 0, st>>>(a, d);
-    else if (s.lanes > 64) backward_kernel<TX, TY, 0, 2, W, VEC, GATE><<<grid, dim3(s.lanes), 0, st>>>(a, d);
-    else if (s.lanes == 16) backward_kernel<TX, TY, 16, 1, W, VEC, GATE><<<grid, wg, columns, st>>>(a, d);
-    else if (s.lanes == 32) backward_kernel<TX, TY, 32, 1, W, VEC, GATE><<<grid, wg, columns, st>>>(a, d);
-    else if (s.pieces == 1) backward_kernel<TX, TY, 64, 1, W, VEC, GATE><<<grid, wg, columns, st>>>(a, d);
-    else backward_kernel<TX, TY, 64, 2, W, VEC, GATE><<<grid, wg, columns, st>>>(a, d);
-    return hipGetLastError();
+    const uint32_t grid = blocks_of(a, s), bytes = s.lanes > 64 ? channel_bytes(s, W) : s.lanes * W * 4;
+    if constexpr (W == 4)
+        if (s.lanes > 64 && s.pieces == 4) return launch(backward_kernel<TX, TY, 0, 4, W, GATE>, grid, s.lanes, bytes, st, a, d);
+    if (s.lanes > 64 && s.pieces == 2) return launch(backward_kernel<TX, TY, 0, 2, W, GATE>, grid, s.lanes, bytes, st, a, d);
+    if (s.lanes > 64) return launch(backward_kernel<TX, TY, 0, 1, W, GATE>, grid, s.lanes, bytes, st, a, d);
+    if (s.lanes == 16) return launch(backward_kernel<TX, TY, 16, 1, W, GATE>, grid, 256, bytes, st, a, d);
+    if (s.lanes == 32) return launch(backward_kernel<TX, TY, 32, 1, W, GATE>, grid, 256, bytes, st, a, d);
+    return launch(backward_kernel<TX, TY, 64, 1, W, GATE>, grid, 256, bytes, st, a, d);
 }
 
 template <class TY> constexpr int words() { return 16 / int(sizeof(TY)); }
 
-template <class TX, class TY, bool VEC, class F>
+template <class TX, class TY, class F>
 hipError_t by_gate(const Args& a, F f) {
     switch (a.gate_kind) {
-        case CHANNEL: return f.template run<TX, TY, VEC, CHANNEL>();
-        case ROW: return f.template run<TX, TY, VEC, ROW>();
-        case ELEMENT: return f.template run<TX, TY, VEC, ELEMENT>();
-        default: return f.template run<TX, TY, VEC, NONE>();
+        case CHANNEL: return f.template run<TX, TY, CHANNEL>();
+        case ROW: return f.template run<TX, TY, ROW>();
+        case ELEMENT: return f.template run<TX, TY, ELEMENT>();
+        default: return f.template run<TX, TY, NONE>();
     }
 }
 template <class F>
 hipError_t by_type(const Args& a, uint32_t x_type, uint32_t y_type, F f) {
-    const bool vec = a.width % (y_type == MDN_BF16 ? 8 : 4) == 0;
-    if (x_type == MDN_BF16) return vec ? by_gate<bf16, bf16, true>(a, f) : by_gate<bf16, bf16, false>(a, f);
-    if (y_type == MDN_BF16) return vec ? by_gate<float, bf16, true>(a, f) : by_gate<float, bf16, false>(a, f);
-    return vec ? by_gate<float, float, true>(a, f) : by_gate<float, float, false>(a, f);
+    if (x_type == MDN_BF16) return by_gate<bf16, bf16>(a, f);
+    return y_type == MDN_BF16 ? by_gate<float, bf16>(a, f) : by_gate<float, float>(a, f);
 }
 struct Forward {
     const Args& a;
     hipStream_t st;
-    template <class TX, class TY, bool VEC, int GATE> hipError_t run() { return forward<TX, TY, words<TY>(), VEC, GATE>(a, st); }
+    template <class TX, class TY, int GATE> hipError_t run() { return forward<TX, TY, words<TY>(), GATE>(a, st); }
 };
 struct Backward {
     const Args& a;
     const GradArgs& d;
     hipStream_t st;
-    template <class TX, class TY, bool VEC, int GATE> hipError_t run() { return backward<TX, TY, words<TY>(), VEC, GATE>(a, d, st); }
+    template <class TX, class TY, int GATE> hipError_t run() { return backward<TX, TY, words<TY>(), GATE>(a, d, st); }
 };
 
 }  // namespace
@@ -434,7 +546,7 @@ hipError_t launch_backward(const Args& a, const GradArgs& d, uint32_t x_type, ui
     const uint32_t count = parts(a, y_type);
     if (count)
         if (hipError_t e = by_type(a, x_type, y_type, Backward{a, d, stream})) return e;
-    columns_kernel<<<dim3((4 * a.width + 63) / 64), dim3(256), 0, stream>>>(
+    columns_kernel<<<dim3((4 * a.width + 63) / 64), dim3(1024), 0, stream>>>(
         d.parts, count, a.width, d.d_w_post, d.d_w_pre, a.residual ? d.d_residual : nullptr,
         a.gate_kind == CHANNEL ? d.d_gate.p : nullptr, a.gate_f32);
     return hipGetLastError();

@@ -2367,21 +2367,6 @@ int norm_args(const char* name, const MdnBlockNorm* n, blocknorm::Args* out) {
     return MDN_OK;
 }
 
-// Whether every row of an array starts at a multiple of 16 bytes.
-bool norm_wide(const blocknorm::Args& a, const blocknorm::Rows& r, uint32_t size) {
-    if (!r.p) return true;
-    const uint64_t inner = a.rows < a.inner_count ? a.rows : a.inner_count;
-    return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && (inner <= 1 || r.inner * int64_t(size) % 16 == 0) &&
-           (a.rows <= a.inner_count || r.outer * int64_t(size) % 16 == 0);
-}
-bool norm_inputs_wide(const blocknorm::Args& a, const MdnBlockNorm* n) {
-    const auto vector = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    const uint32_t sx = size_of(n->x_dtype), sy = size_of(n->y_dtype);
-    return norm_wide(a, a.x, sx) && norm_wide(a, a.y, sy) && vector(n->w_post) && vector(n->w_pre) && vector(n->residual) &&
-           (n->gate_kind != MDN_GATE_CHANNEL || vector(n->gate.data)) &&
-           (n->gate_kind != MDN_GATE_ELEMENT || norm_wide(a, a.gate, sy));
-}
-
 }  // namespace
 
 extern "C" {
@@ -2391,7 +2376,6 @@ int mdn_op_block_norm_forward(const MdnBlockNorm* norm, void* stream) {
     if (int rc = norm_args("mdn_op_block_norm_forward", norm, &a)) return rc;
     if (a.rows == 0) return MDN_OK;
     if (!a.s.p || !a.h.p) return fail(MDN_E_ARG, "mdn_op_block_norm_forward: null rows");
-    a.wide = norm_inputs_wide(a, norm) && norm_wide(a, a.s, size_of(norm->x_dtype)) && norm_wide(a, a.h, size_of(norm->y_dtype));
     HIP_TRY(blocknorm::launch_forward(a, norm->x_dtype, norm->y_dtype, static_cast<hipStream_t>(stream)));
     return MDN_OK;
 }
@@ -2421,9 +2405,6 @@ int mdn_op_block_norm_backward(const MdnBlockNorm* norm, const MdnBlockNormGrad*
     d.d_s = rows(grad->d_s); d.d_h = rows(grad->d_h); d.d_x = rows(grad->d_x); d.d_y = rows(grad->d_y); d.d_gate = rows(grad->d_gate);
     d.d_w_post = grad->d_w_post; d.d_w_pre = grad->d_w_pre; d.d_residual = grad->d_residual;
     d.parts = static_cast<float*>(workspace);
-    const uint32_t sx = size_of(norm->x_dtype), sy = size_of(norm->y_dtype);
-    a.wide = norm_inputs_wide(a, norm) && norm_wide(a, d.d_s, sx) && norm_wide(a, d.d_h, sy) && norm_wide(a, d.d_x, sx) &&
-             norm_wide(a, d.d_y, sy) && (a.gate_kind != MDN_GATE_ELEMENT || norm_wide(a, d.d_gate, sy));
     HIP_TRY(blocknorm::launch_backward(a, d, norm->x_dtype, norm->y_dtype, static_cast<hipStream_t>(stream)));
     return MDN_OK;
 }
