@@ -2196,15 +2196,7 @@ namespace {
 
 constexpr uint64_t kMostBlocks = 0x7fffffffull;  // of a grid
 
-uint32_t size_of(uint32_t dtype) { return dtype == MDN_BF16 ? 2u : 4u; }
-
-// Rows for a kernel; `ticks`, `envs` and `heads` bound the strides that matter.
-delta::Rows device_rows(const MdnRows& r, uint32_t size, uint32_t ticks, uint32_t envs, uint32_t heads) {
-    delta::Rows out{static_cast<char*>(r.data), r.tick, r.env, r.head, 0u};
-    const auto words = [&](int64_t stride, uint32_t count) { return count <= 1 || (stride * int64_t(size)) % 16 == 0; };
-    out.wide = reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && words(r.tick, ticks) && words(r.env, envs) && words(r.head, heads);
-    return out;
-}
+delta::Rows device_rows(const MdnRows& r) { return delta::Rows{static_cast<char*>(r.data), r.tick, r.env, r.head}; }
 
 int delta_args(const char* name, const MdnDeltaRule* d, delta::Args* out) {
     const std::string who = std::string(name) + ": ";
@@ -2220,17 +2212,16 @@ int delta_args(const char* name, const MdnDeltaRule* d, delta::Args* out) {
     const bool any = d->ticks && d->envs;
     if (any && (!d->q.data || !d->k.data || !d->v.data || !d->g.data || !d->beta.data))
         return fail(MDN_E_ARG, who + "null rows");
-    const uint32_t size = size_of(d->dtype), T = d->ticks, N = d->envs, H = d->heads, Q = d->qk_heads;
     delta::Args a{};
-    a.ticks = T; a.envs = N; a.qk_heads = Q; a.heads = H; a.k_dim = d->k_dim; a.v_dim = d->v_dim;
+    a.ticks = d->ticks; a.envs = d->envs; a.qk_heads = d->qk_heads; a.heads = d->heads; a.k_dim = d->k_dim; a.v_dim = d->v_dim;
     a.gate_f32 = d->gate_dtype == MDN_F32;
     a.scale = d->scale;
-    a.q = device_rows(d->q, size, T, N, Q);
-    a.k = device_rows(d->k, size, T, N, Q);
-    a.v = device_rows(d->v, size, T, N, H);
-    a.o = device_rows(d->o, size, T, N, H);
-    a.g = device_rows(d->g, size, T, N, H);
-    a.beta = device_rows(d->beta, size, T, N, H);
+    a.q = device_rows(d->q);
+    a.k = device_rows(d->k);
+    a.v = device_rows(d->v);
+    a.o = device_rows(d->o);
+    a.g = device_rows(d->g);
+    a.beta = device_rows(d->beta);
     a.reset = d->reset; a.reset_tick = d->reset_tick; a.reset_env = d->reset_env;
     a.state = d->state; a.state_out = d->state_out;
     *out = a;
@@ -2307,17 +2298,17 @@ int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad*
     if (workspace_bytes < delta_partial_bytes(a) || (delta_partial_bytes(a) && !workspace))
         return fail(MDN_E_ARG, who + "workspace is too small");
     a.chunk_states = static_cast<float*>(const_cast<void*>(keep));
-    const uint32_t size = size_of(rule->dtype), T = a.ticks, N = a.envs, H = a.heads, Q = a.qk_heads;
+    const uint32_t T = a.ticks, N = a.envs, H = a.heads, Q = a.qk_heads;
     delta::GradArgs d{};
-    d.d_o = device_rows(grad->d_o, size, T, N, H);
+    d.d_o = device_rows(grad->d_o);
     d.d_state_out = grad->d_state_out;
     d.d_state = grad->d_state;
-    d.d_v = device_rows(grad->d_v, size, T, N, H);
-    d.d_g = device_rows(grad->d_g, size, T, N, H);
-    d.d_beta = device_rows(grad->d_beta, size, T, N, H);
+    d.d_v = device_rows(grad->d_v);
+    d.d_g = device_rows(grad->d_g);
+    d.d_beta = device_rows(grad->d_beta);
     if (H == Q) {
-        d.d_q = device_rows(grad->d_q, size, T, N, Q);
-        d.d_k = device_rows(grad->d_k, size, T, N, Q);
+        d.d_q = device_rows(grad->d_q);
+        d.d_k = device_rows(grad->d_k);
         HIP_TRY(delta::launch_backward(a, d, bf, st));
         return MDN_OK;
     }
@@ -2329,8 +2320,8 @@ int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad*
         return fail(MDN_E_ARG, who + "d_q and d_k of shared heads must be contiguous");
     float* part = static_cast<float*>(workspace);
     d.partial = 1;
-    d.d_q = delta::Rows{reinterpret_cast<char*>(part), tick, env, head, 0u};
-    d.d_k = delta::Rows{reinterpret_cast<char*>(part + uint64_t(T) * N * H * a.k_dim), tick, env, head, 0u};
+    d.d_q = delta::Rows{reinterpret_cast<char*>(part), tick, env, head};
+    d.d_k = delta::Rows{reinterpret_cast<char*>(part + uint64_t(T) * N * H * a.k_dim), tick, env, head};
     HIP_TRY(delta::launch_backward(a, d, bf, st));
     HIP_TRY(delta::launch_sum_heads(part, grad->d_q.data, uint64_t(T) * N, Q, H / Q, a.k_dim, bf, st));
     HIP_TRY(delta::launch_sum_heads(part + uint64_t(T) * N * H * a.k_dim, grad->d_k.data, uint64_t(T) * N, Q, H / Q, a.k_dim, bf, st));

@@ -74,108 +74,112 @@ __device__ __forceinline__ void store_state(float* p, const f32x4 (&x)[KT], uint
         }
 }
 
-// ---- eight elements of a row, in registers.  WIDE: rows start at multiples
-// of 16 bytes and widths are multiples of eight elements; a piece is then
-// wholly inside its row or wholly past it, and moves in 16-byte words.
-template <class E> struct Piece { uint4 w[sizeof(E) / 2]; };
+// ---- rows of one state's array: its env's and head's start, and the ticks' stride
+template <class E> struct Track {
+    E* p;
+    int64_t tick;
+    __device__ __forceinline__ Track(const Rows& r, uint32_t n, uint32_t h)
+        : p(reinterpret_cast<E*>(r.p) + int64_t(n) * r.env + int64_t(h) * r.head), tick(r.tick) {}
+    __device__ __forceinline__ E* row(uint32_t t) const { return p + int64_t(t) * tick; }
+};
 
-// What is past the row's end or the last tick is some other part of the array
-// until mask_piece() makes it 0: where the piece is used, not where it is
-// loaded, which would wait for it.
-template <class E, bool WIDE>
-__device__ __forceinline__ Piece<E> load_piece(const Rows& r, int64_t base, uint32_t dim, uint32_t col) {
-    constexpr int W = sizeof(E) / 2;
+// ---- eight elements of a row, in registers.  Whole pieces move in 16-byte
+// words wherever the row starts (global memory takes them at any multiple of
+// an element's size), the piece that a row ends in one element at a time.
+typedef uint32_t Word __attribute__((ext_vector_type(4)));
+template <class E> struct Words;
+template <> struct Words<float> { typedef Word type __attribute__((aligned(4))); };
+template <> struct Words<bf16> { typedef Word type __attribute__((aligned(2))); };
+template <class E> struct Piece { Word w[sizeof(E) / 2]; };
+
+template <class E>
+__device__ __forceinline__ Piece<E> load_piece(const E* row, uint32_t dim, uint32_t col) {
+    constexpr int W = sizeof(E) / 2, PER = 16 / sizeof(E);
     Piece<E> out;
-    const E* p = reinterpret_cast<const E*>(r.p) + base;
-    if (WIDE) {
-        const uint4* q = reinterpret_cast<const uint4*>(p + (col < dim ? col : 0u));
+    if (col + 8 <= dim) {
 #pragma unroll
-        for (int i = 0; i < W; i++) out.w[i] = q[i];
-    } else {
-        uint32_t word[4 * W];
-#pragma unroll
-        for (uint32_t i = 0; i < 4 * W; i++) {
-            if (sizeof(E) == 4) {
-                const uint32_t c = col + i;
-                word[i] = reinterpret_cast<const uint32_t*>(p)[c < dim ? c : 0u];
-            } else {
-                const uint32_t c = col + 2 * i;
-                const uint32_t lo = reinterpret_cast<const uint16_t*>(p)[c < dim ? c : 0u];
-                const uint32_t hi = reinterpret_cast<const uint16_t*>(p)[c + 1 < dim ? c + 1 : 0u];
-                word[i] = lo | hi << 16;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < W; i++) out.w[i] = uint4{word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]};
-    }
-    return out;
-}
-template <class E, bool WIDE>
-__device__ __forceinline__ Piece<E> mask_piece(const Piece<E>& x, uint32_t dim, uint32_t col, bool row_in) {
-    constexpr int W = sizeof(E) / 2;
-    Piece<E> out;
-#pragma unroll
-    for (int i = 0; i < W; i++) {
-        const uint32_t word[4] = {x.w[i].x, x.w[i].y, x.w[i].z, x.w[i].w};
-        uint32_t y[4];
-#pragma unroll
-        for (uint32_t e = 0; e < 4; e++) {
-            if (WIDE) {
-                y[e] = row_in && col < dim ? word[e] : 0u;
-            } else {
-                const uint32_t c = col + (4 * i + e) * (4 / sizeof(E));
-                y[e] = row_in && c < dim ? word[e] : 0u;
-                if (sizeof(E) == 2 && c + 1 >= dim) y[e] &= 0xffffu;
-            }
-        }
-        out.w[i] = uint4{y[0], y[1], y[2], y[3]};
-    }
-    return out;
-}
-template <class E, bool WIDE>
-__device__ __forceinline__ void store_piece(const Rows& r, int64_t base, uint32_t dim, uint32_t col, const Piece<E>& in) {
-    constexpr int W = sizeof(E) / 2;
-    E* p = reinterpret_cast<E*>(r.p) + base + col;
-    if (WIDE) {
-        if (col < dim)
-#pragma unroll
-            for (int i = 0; i < W; i++) reinterpret_cast<uint4*>(p)[i] = in.w[i];
+        for (int i = 0; i < W; i++) out.w[i] = *reinterpret_cast<const typename Words<E>::type*>(row + col + i * PER);
     } else {
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            const uint32_t word[4] = {in.w[i].x, in.w[i].y, in.w[i].z, in.w[i].w};
+        for (int i = 0; i < W; i++)
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) {
+            for (int e = 0; e < 4; e++) {
+                const uint32_t c = col + i * PER + e * (4 / sizeof(E));
+                uint32_t bits = 0;
                 if (sizeof(E) == 4) {
-                    if (col + 4 * i + e < dim) reinterpret_cast<uint32_t*>(p)[4 * i + e] = word[e];
+                    if (c < dim) bits = reinterpret_cast<const uint32_t*>(row)[c];
                 } else {
-                    const uint32_t at = 2 * (4 * i + e);
-                    if (col + at < dim) reinterpret_cast<uint16_t*>(p)[at] = uint16_t(word[e]);
-                    if (col + at + 1 < dim) reinterpret_cast<uint16_t*>(p)[at + 1] = uint16_t(word[e] >> 16);
+                    if (c < dim) bits = reinterpret_cast<const uint16_t*>(row)[c];
+                    if (c + 1 < dim) bits |= uint32_t(reinterpret_cast<const uint16_t*>(row)[c + 1]) << 16;
+                }
+                out.w[i][e] = bits;
+            }
+    }
+    return out;
+}
+// Rows past the last tick: zeros, where the piece is used (where it is loaded
+// the selection would wait for it).
+template <class E>
+__device__ __forceinline__ Piece<E> mask_piece(const Piece<E>& x, bool in) {
+    Piece<E> out;
+#pragma unroll
+    for (int i = 0; i < int(sizeof(E) / 2); i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) out.w[i][e] = in ? x.w[i][e] : 0u;
+    return out;
+}
+template <class E>
+__device__ __forceinline__ void store_piece(E* row, uint32_t dim, uint32_t col, const Piece<E>& in) {
+    constexpr int W = sizeof(E) / 2, PER = 16 / sizeof(E);
+    if (col + 8 <= dim) {
+#pragma unroll
+        for (int i = 0; i < W; i++) *reinterpret_cast<typename Words<E>::type*>(row + col + i * PER) = in.w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t c = col + i * PER + e * (4 / sizeof(E)), bits = in.w[i][e];
+                if (sizeof(E) == 4) {
+                    if (c < dim) reinterpret_cast<uint32_t*>(row)[c] = bits;
+                } else {
+                    if (c < dim) reinterpret_cast<uint16_t*>(row)[c] = uint16_t(bits);
+                    if (c + 1 < dim) reinterpret_cast<uint16_t*>(row)[c + 1] = uint16_t(bits >> 16);
                 }
             }
-        }
     }
 }
+// A thread's piece of a chunk's rows: pieces of a row, then rows; there are
+// at least as many threads as pieces.
+struct Spot {
+    uint32_t row, col;
+    bool on;
+    __device__ __forceinline__ explicit Spot(uint32_t dim) {
+        const uint32_t per = (dim + 7) / 8;
+        row = threadIdx.x / per;
+        col = threadIdx.x % per * 8;
+        on = row < uint32_t(CHUNK);
+    }
+};
 // To a row in the order of place(); `m` is the row's start.
 __device__ __forceinline__ void piece_to_ordered(bf16* m, uint32_t col, const Piece<bf16>& in) {
-    *reinterpret_cast<uint2*>(m + place(int(col))) = uint2{in.w[0].x, in.w[0].y};
-    *reinterpret_cast<uint2*>(m + place(int(col)) + 8) = uint2{in.w[0].z, in.w[0].w};
+    *reinterpret_cast<uint2*>(m + place(int(col))) = uint2{in.w[0][0], in.w[0][1]};
+    *reinterpret_cast<uint2*>(m + place(int(col)) + 8) = uint2{in.w[0][2], in.w[0][3]};
 }
 __device__ __forceinline__ void piece_to_ordered(float* m, uint32_t col, const Piece<float>& in) {
-    *reinterpret_cast<uint4*>(m + place(int(col))) = in.w[0];
-    *reinterpret_cast<uint4*>(m + place(int(col)) + 8) = in.w[1];
+    *reinterpret_cast<Word*>(m + place(int(col))) = in.w[0];
+    *reinterpret_cast<Word*>(m + place(int(col)) + 8) = in.w[1];
 }
 template <class E>
 __device__ __forceinline__ void piece_to_lds(E* m, const Piece<E>& in) {
 #pragma unroll
-    for (int i = 0; i < int(sizeof(E) / 2); i++) reinterpret_cast<uint4*>(m)[i] = in.w[i];
+    for (int i = 0; i < int(sizeof(E) / 2); i++) reinterpret_cast<Word*>(m)[i] = in.w[i];
 }
 template <class E>
 __device__ __forceinline__ Piece<E> piece_from_lds(const E* m) {
     Piece<E> out;
 #pragma unroll
-    for (int i = 0; i < int(sizeof(E) / 2); i++) out.w[i] = reinterpret_cast<const uint4*>(m)[i];
+    for (int i = 0; i < int(sizeof(E) / 2); i++) out.w[i] = reinterpret_cast<const Word*>(m)[i];
     return out;
 }
 
@@ -193,6 +197,13 @@ __device__ __forceinline__ bool gate_is_flag(const Gates& s, int i) {
 }
 
 struct GateRegs { float g, beta; uint32_t flag; };
+
+// LDS columns past a head's width stay 0: they are operands.
+__device__ __forceinline__ void clear_lds(void* lds, uint32_t bytes) {
+    for (uint32_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+        *reinterpret_cast<Word*>(static_cast<char*>(lds) + i) = Word{0, 0, 0, 0};
+    __syncthreads();
+}
 
 // Tick `t` of lane t - t0; a tick past the end adds nothing and decays nothing.
 __device__ __forceinline__ GateRegs load_gates(const Args& a, bool bf, uint32_t n, uint32_t h, int64_t t, bool in) {

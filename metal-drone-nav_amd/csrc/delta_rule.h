@@ -17,7 +17,6 @@ constexpr uint32_t MAX_DIM = 128; // widest head
 struct Rows {
     char* p;
     int64_t tick, env, head;  // strides in elements
-    uint32_t wide;            // base and strides are multiples of 16 bytes
 };
 
 struct Args {
@@ -36,6 +35,13 @@ struct Args {
 // chunk, [v / 16][k / 16] tiles of 64 lanes x 4 values.
 inline __host__ __device__ uint64_t state_tile_words(const Args& a) {
     return uint64_t((a.k_dim + 15) / 16) * ((a.v_dim + 15) / 16) * 256;
+}
+
+// Wavefronts of a chunk's workgroup: one for each 16 columns of a head, and at
+// least four (three hold the chunk's tiles of A, the last makes decays).
+inline __host__ uint32_t waves_of(const Args& a) {
+    const uint32_t dim = a.k_dim > a.v_dim ? a.k_dim : a.v_dim, waves = (dim + 15) / 16;
+    return waves < 4 ? 4 : waves;
 }
 
 // The backward pass: gradients of o and of the final state in, of the inputs

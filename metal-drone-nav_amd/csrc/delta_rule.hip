@@ -132,50 +132,59 @@ template <class E, int D> struct ForwardShared {
     Gates gates[2];  // of this chunk and the next
 };
 
-// One workgroup per state, D / 16 wavefronts, 16 columns of V each: a
-// wavefront has its K x 16 slice of the state in result tiles, which are
-// operands as they are (delta_tiles.h).
-template <class E, int D, bool WIDE>
-__global__ void __launch_bounds__(D * 4, D == 64 ? (sizeof(E) == 2 && WIDE ? 4 : 3) : 2) forward_kernel(Args a) {
+// One workgroup per state, a wavefront for each 16 columns of V (at least
+// four): a wavefront has its K x 16 slice of the state in result tiles, which
+// are operands as they are (delta_tiles.h).  D, 64 or 128, is what registers
+// and LDS rows are sized for; narrower heads leave out whole steps of 32.
+template <class E, int D>
+__global__ void __launch_bounds__(D * 4, D == 64 ? 4 : 2) forward_kernel(Args a) {
     typedef ForwardShared<E, D> Shared;
-    constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, W = D / 16, KT = D / 16;
+    constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16;
     constexpr bool bf = sizeof(E) == 2;
     extern __shared__ __align__(16) char lds[];
     Shared& s = *reinterpret_cast<Shared*>(lds);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const Lane at0 = Lane::mine();
+    const int waves = blockDim.x >> 6;
     const uint64_t seq = blockIdx.x;
     const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
     const uint32_t hq = h / (a.heads / a.qk_heads);
     const uint32_t kd = a.k_dim, vd = a.v_dim;
-    const uint32_t row = uint32_t(tid) / (D / 8), col = uint32_t(tid) % (D / 8) * 8;  // the thread's piece of a chunk's rows
-    const uint32_t vcol = 16 * wave + at0.col;                                      // its column of a result
+    const Spot ks_(kd), vs_(vd);  // the thread's piece of k and q, and of v and o
+    const Track<const E> rows_k(a.k, n, hq), rows_q(a.q, n, hq), rows_v(a.v, n, h);
+    const Track<E> rows_o(a.o, n, h);
     const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
+    if (kd < D || vd < D) clear_lds(lds, sizeof(Shared));
 
     f32x4 state[KT];
-    load_state(state, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, at0, vcol);
-    // the matrices' upper right block stays 0
-    if (wave < 2 * N) {
-        E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * System<E>::PLANE;
+    {
+        const Lane l = Lane::mine();
+        load_state(state, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+        // the matrices' upper right block stays 0
+        if (wave < 2 * N) {
+            E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * System<E>::PLANE;
 #pragma unroll
-        for (int i = 0; i < 4; i++) m[(16 + at0.col) * CP + 4 * at0.quad + i] = E(0.0f);
+            for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
+        }
     }
-
     Piece<E> pk, pq, pv;
     GateRegs gate{0.0f, 0.0f, 0u};
     const auto fetch = [&](uint32_t c) {
-        const uint32_t at = c * C + row;
-        const int64_t t = at < a.ticks ? at : 0;
-        pk = load_piece<E, WIDE>(a.k, t * a.k.tick + n * a.k.env + hq * a.k.head, kd, col);
-        pq = load_piece<E, WIDE>(a.q, t * a.q.tick + n * a.q.env + hq * a.q.head, kd, col);
-        pv = load_piece<E, WIDE>(a.v, t * a.v.tick + n * a.v.env + h * a.v.head, vd, col);
+        if (ks_.on) {
+            const uint32_t at = c * C + ks_.row, t = at < a.ticks ? at : 0u;
+            pk = load_piece<E>(rows_k.row(t), kd, ks_.col);
+            pq = load_piece<E>(rows_q.row(t), kd, ks_.col);
+        }
+        if (vs_.on) {
+            const uint32_t at = c * C + vs_.row, t = at < a.ticks ? at : 0u;
+            pv = load_piece<E>(rows_v.row(t), vd, vs_.col);
+        }
     };
     // the last wavefront has no tile of A: it makes the next chunk's decays meanwhile
     const auto fetch_gates = [&](uint32_t c) {
         const int64_t t = int64_t(c) * C + lane;
         gate = load_gates(a, bf, n, h, t, lane < C && t < a.ticks);
     };
-    if (wave == W - 1) {
+    if (wave == waves - 1) {
         fetch_gates(0);
         put_gates(s.gates[0], gate);
         fetch_gates(1);
@@ -184,10 +193,12 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? (sizeof(E) == 2 && WIDE ? 4 :
     for (uint32_t c = 0; c < chunks; c++) {
         const Lane l = Lane::fresh();
         const Gates& gates = s.gates[c & 1];
-        const bool in = c * C + row < a.ticks;
-        piece_to_ordered(s.k + row * ST, col, mask_piece<E, WIDE>(pk, kd, col, in));
-        piece_to_ordered(s.q + row * ST, col, mask_piece<E, WIDE>(pq, kd, col, in));
-        piece_to_lds(s.v + row * ST + col, mask_piece<E, WIDE>(pv, vd, col, in));
+        if (ks_.on) {
+            const bool in = c * C + ks_.row < a.ticks;
+            piece_to_ordered(s.k + ks_.row * ST, ks_.col, mask_piece<E>(pk, in));
+            piece_to_ordered(s.q + ks_.row * ST, ks_.col, mask_piece<E>(pq, in));
+        }
+        if (vs_.on) piece_to_lds(s.v + vs_.row * ST + vs_.col, mask_piece<E>(pv, c * C + vs_.row < a.ticks));
         __syncthreads();
         if (c + 1 < chunks) fetch(c + 1);
         if (a.chunk_states && c > 0 && 16 * wave < int(vd)) {
@@ -202,6 +213,7 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? (sizeof(E) == 2 && WIDE ? 4 :
             f32x4 kk{0, 0, 0, 0}, qk{0, 0, 0, 0};
 #pragma unroll
             for (int x = 0; x < D; x += 32) {
+                if (x >= int(kd)) continue;
                 const auto kj = ordered_row(l, s.k, ST, j0, x);
                 mma(kk, ordered_row(l, s.k, ST, i0, x), kj);
                 mma(qk, ordered_row(l, s.q, ST, i0, x), kj);
@@ -220,78 +232,79 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? (sizeof(E) == 2 && WIDE ? 4 :
             else
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
         }
-        if (wave == W - 1 && c + 1 < chunks) {
+        if (wave == waves - 1 && c + 1 < chunks) {
             put_gates(s.gates[(c + 1) & 1], gate);
             fetch_gates(c + 2);
         }
         // the state's part of the ticks
-        f32x4 ks[2] = {}, qs[2] = {};
+        f32x4 ks[2] = {}, qs[2] = {}, r[2], u[2];
+        if (16 * wave < int(vd)) {
 #pragma unroll
-        for (int x = 0; x < D; x += 32) {
-            const auto st = frag_of<E>(state[x / 16], state[x / 16 + 1]);
+            for (int x = 0; x < D; x += 32) {
+                if (x >= int(kd)) continue;
+                const auto st = frag_of<E>(state[x / 16], state[x / 16 + 1]);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                mma(ks[i], ordered_row(l, s.k, ST, 16 * i, x), st);
-                mma(qs[i], ordered_row(l, s.q, ST, 16 * i, x), st);
+                for (int i = 0; i < 2; i++) {
+                    mma(ks[i], ordered_row(l, s.k, ST, 16 * i, x), st);
+                    mma(qs[i], ordered_row(l, s.q, ST, 16 * i, x), st);
+                }
             }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int t = 16 * i + 4 * l.quad + e;
+                    const float g = gates.before[t];
+                    r[i][e] = gates.beta[t] * (float(s.v[t * ST + 16 * wave + l.col]) - g * ks[i][e]);
+                    qs[i][e] *= a.scale * g;
+                }
         }
-        f32x4 r[2], u[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int t = 16 * i + 4 * l.quad + e;
-                const float g = gates.before[t];
-                r[i][e] = gates.beta[t] * (float(s.v[t * ST + 16 * wave + l.col]) - g * ks[i][e]);
-                qs[i][e] *= a.scale * g;
-            }
         __syncthreads();
-        solve(l, s.sys, r, u);
-        // o = scale gamma (q S) + scores u
-        {
+        if (16 * wave < int(vd)) {
+            solve(l, s.sys, r, u);
+            // o = scale gamma (q S) + scores u
+            {
+                const auto uf = frag_of<E>(u[0], u[1]);
+#pragma unroll
+                for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E>::PLANE, 0, 16 * i), uf);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int t = 16 * i + 4 * l.quad + e;
+                    s.v[t * ST + 16 * wave + l.col] = E(qs[i][e]);
+                    u[i][e] *= gates.after[t];
+                }
+            // S <- gamma_C S + K^T u
+            const float total = gates.before[C - 1];
             const auto uf = frag_of<E>(u[0], u[1]);
 #pragma unroll
-            for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E>::PLANE, 0, 16 * i), uf);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int t = 16 * i + 4 * l.quad + e;
-                s.v[t * ST + 16 * wave + l.col] = E(qs[i][e]);
-                u[i][e] *= gates.after[t];
+            for (int i = 0; i < KT; i++) {
+                if (16 * i >= int(kd)) continue;
+                state[i] *= total;
+                mma(state[i], ordered_col(l, s.k, ST, 16 * i), uf);
             }
-        // S <- gamma_C S + K^T u
-        const float total = gates.before[C - 1];
-        const auto uf = frag_of<E>(u[0], u[1]);
-#pragma unroll
-        for (int i = 0; i < KT; i++) {
-            state[i] *= total;
-            mma(state[i], ordered_col(l, s.k, ST, 16 * i), uf);
         }
         __syncthreads();
-        const int64_t t = int64_t(c) * C + row;
-        if (t < a.ticks && col < vd)
-            store_piece<E, WIDE>(a.o, t * a.o.tick + n * a.o.env + h * a.o.head, vd, col, piece_from_lds(s.v + row * ST + col));
+        if (vs_.on && c * C + vs_.row < a.ticks)
+            store_piece<E>(rows_o.row(c * C + vs_.row), vd, vs_.col, piece_from_lds(s.v + vs_.row * ST + vs_.col));
     }
     const Lane l = Lane::fresh();
     if (a.state_out) store_state(a.state_out + seq * kd * vd, state, kd, vd, l, 16 * wave + l.col);
 }
 
-template <class E, int D, bool WIDE>
+template <class E, int D>
 hipError_t forward(const Args& a, hipStream_t stream) {
     constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
-    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, WIDE>);
+    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    forward_kernel<E, D, WIDE><<<dim3(a.envs * a.heads), dim3(D * 4), bytes, stream>>>(a);
+    forward_kernel<E, D><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a);
     return hipGetLastError();
 }
 template <class E>
 hipError_t forward(const Args& a, hipStream_t stream) {
-    const bool narrow = a.k_dim <= 64 && a.v_dim <= 64;
-    const bool wide = (a.q.wide & a.k.wide & a.v.wide & a.o.wide) && a.k_dim % 8 == 0 && a.v_dim % 8 == 0;
-    if (wide) return narrow ? forward<E, 64, true>(a, stream) : forward<E, 128, true>(a, stream);
-    return narrow ? forward<E, 64, false>(a, stream) : forward<E, 128, false>(a, stream);
+    return a.k_dim <= 64 && a.v_dim <= 64 ? forward<E, 64>(a, stream) : forward<E, 128>(a, stream);
 }
 
 template <class E>

@@ -34,78 +34,88 @@ template <class E, int D> struct BackwardShared {
     static constexpr int PLANE = D * CP;
     static constexpr int W = D / 16;
     E k[C * STRIDE], q[C * STRIDE], d_o[C * STRIDE];  // ordered rows
+    E v[C * STRIDE];
+    // from here on the gradients' rows take the place of what is done with
     E u[N * PLANE], r[N * PLANE];                     // U and R transposed, [v][tick]
     float through[D / HALVES * TS];                   // S, then G, transposed: [v][k]
+    // inv and scores give their places to E = beta D dA and to scale D dP
     System<E> sys;
-    E d_scores[N * System<E>::PLANE], d_a[N * System<E>::PLANE];  // scale D dP and E, [j][i]
     Gates gates[2];  // of this chunk and the next
-    float beta_v[W][C], a[W][C], b[W][C], dot[W];
+    __align__(16) float beta_v[W][C], a[W][C], b[W][C], dot[W];
     double m_row[3][16], m_col[3][16];
-    float beta_a[3][16];
+    __align__(16) float beta_a[3][16];
 };
 
-template <class E>
-__device__ __forceinline__ void put_grad(const Rows& r, int64_t at, float x, bool partial) {
-    if (partial)
-        reinterpret_cast<float*>(r.p)[at] = x;
-    else
-        reinterpret_cast<E*>(r.p)[at] = E(x);
-}
-__device__ __forceinline__ void put_gate(const Args& a, const Rows& r, int64_t at, float x, bool bf) {
-    if (a.gate_f32 || !bf)
+template <class E> __device__ __forceinline__ void put_gate(const Args& a, const Rows& r, int64_t at, float x) {
+    if (a.gate_f32 || sizeof(E) == 4)
         reinterpret_cast<float*>(r.p)[at] = x;
     else
         reinterpret_cast<bf16*>(r.p)[at] = bf16(x);
 }
 
-// One workgroup per state, D / 16 wavefronts.  A wavefront has 16 columns of V
-// (its slices of S, G, U and R) and, for the gradients of q and k, 16 columns
-// of K; U, R, S and G change hands through LDS.
-template <class E, int D, bool WIDE>
+// One workgroup per state, a wavefront for each 16 columns (at least four).  A
+// wavefront has 16 columns of V (its slices of S, G, U and R) and, for the
+// gradients of q and k, 16 columns of K; U, R, S and G change hands through
+// LDS.  F is the type of the rows of d_q and d_k.
+template <class E, class F, int D>
 __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) {
     typedef BackwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16, SP = System<E>::PLANE, PL = Shared::PLANE;
     constexpr int HALVES = Shared::HALVES, TS = Shared::TS, VH = D / HALVES;
+    constexpr int FT = D + Kind<F>::PAD;  // row of d_q and d_k in LDS
+    static_assert(sizeof(F) * 2 * C * FT + sizeof(E) * C * ST <= sizeof(Shared::u) + sizeof(Shared::r) + sizeof(Shared::through), "");
     constexpr bool bf = sizeof(E) == 2;
     extern __shared__ __align__(16) char lds[];
     Shared& s = *reinterpret_cast<Shared*>(lds);
+    F* const dq_rows = reinterpret_cast<F*>(s.u);
+    F* const dk_rows = dq_rows + C * FT;
+    E* const dv_rows = reinterpret_cast<E*>(dk_rows + C * FT);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int waves = blockDim.x >> 6;
     const uint64_t seq = blockIdx.x;
     const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
     const uint32_t hq = h / (a.heads / a.qk_heads), hg = d.partial ? h : hq;
-    const uint32_t kd = a.k_dim, vd = a.v_dim;
-    const uint32_t row = uint32_t(tid) / (D / 8), col = uint32_t(tid) % (D / 8) * 8;
+    const int kd = a.k_dim, vd = a.v_dim;
+    const bool v_wave = 16 * wave < vd, k_wave = 16 * wave < kd;
+    const Spot on_k(kd), on_v(vd);
+    const Track<const E> rows_k(a.k, n, hq), rows_q(a.q, n, hq), rows_v(a.v, n, h), rows_do(d.d_o, n, h);
+    const Track<F> rows_dq(d.d_q, n, hg), rows_dk(d.d_k, n, hg);
+    const Track<E> rows_dv(d.d_v, n, h);
     const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
     const f32x4 zero{0, 0, 0, 0};
+    if (kd < D || vd < D) clear_lds(lds, sizeof(Shared));
 
     f32x4 g[KT];  // G, K x 16
     {
         const Lane l = Lane::fresh();
         load_state(g, d.d_state_out ? d.d_state_out + seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
         // the matrices' upper right blocks stay 0
-        if (wave < N) {
-            E* m[4] = {s.sys.scores, s.sys.inv, s.d_scores, s.d_a};
+        if (wave < 2 * N) {
+            E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * SP;
 #pragma unroll
-            for (int x = 0; x < 4; x++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) m[x][wave * SP + (16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
+            for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
         }
     }
-    Piece<E> pk, pq, po;
+    Piece<E> pk, pq, pv, po;
     GateRegs gate{0.0f, 0.0f, 0u};
     const auto fetch = [&](uint32_t c) {
-        const uint32_t at = c * C + row;
-        const int64_t t = at < a.ticks ? at : 0;
-        pk = load_piece<E, WIDE>(a.k, t * a.k.tick + n * a.k.env + hq * a.k.head, kd, col);
-        pq = load_piece<E, WIDE>(a.q, t * a.q.tick + n * a.q.env + hq * a.q.head, kd, col);
-        po = load_piece<E, WIDE>(d.d_o, t * d.d_o.tick + n * d.d_o.env + h * d.d_o.head, vd, col);
+        if (on_k.on) {
+            const uint32_t at = c * C + on_k.row, t = at < a.ticks ? at : 0u;
+            pk = load_piece<E>(rows_k.row(t), kd, on_k.col);
+            pq = load_piece<E>(rows_q.row(t), kd, on_k.col);
+        }
+        if (on_v.on) {
+            const uint32_t at = c * C + on_v.row, t = at < a.ticks ? at : 0u;
+            pv = load_piece<E>(rows_v.row(t), vd, on_v.col);
+            po = load_piece<E>(rows_do.row(t), vd, on_v.col);
+        }
     };
     // the last wavefront has no tile of A: it makes the next chunk's decays meanwhile
     const auto fetch_gates = [&](uint32_t c) {
         const int64_t t = int64_t(c) * C + lane;
         gate = load_gates(a, bf, n, h, t, lane < C && t < a.ticks);
     };
-    if (wave == Shared::W - 1) {
+    if (wave == waves - 1) {
         fetch_gates(chunks - 1);
         put_gates(s.gates[(chunks - 1) & 1], gate);
         if (chunks > 1) fetch_gates(chunks - 2);
@@ -113,34 +123,28 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     fetch(chunks - 1);
     for (uint32_t c = chunks; c-- > 0;) {
         const Lane l = Lane::fresh();
-        const uint32_t vc = 16 * wave + l.col;  // the lane's column of V, and of K
         const Gates& gates = s.gates[c & 1];
         const uint32_t left = a.ticks - c * C;  // ticks from the chunk's first
-        const bool in = c * C + row < a.ticks;
-        piece_to_ordered(s.k + row * ST, col, mask_piece<E, WIDE>(pk, kd, col, in));
-        piece_to_ordered(s.q + row * ST, col, mask_piece<E, WIDE>(pq, kd, col, in));
-        piece_to_ordered(s.d_o + row * ST, col, mask_piece<E, WIDE>(po, vd, col, in));
-        // S and V, in result layout
-        f32x4 st[KT], x[2];
+        if (on_k.on) {
+            piece_to_ordered(s.k + on_k.row * ST, on_k.col, mask_piece<E>(pk, on_k.row < left));
+            piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
+        }
+        if (on_v.on) {
+            piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
+            piece_to_ordered(s.d_o + on_v.row * ST, on_v.col, mask_piece<E>(po, on_v.row < left));
+        }
+        // S in result layout
+        f32x4 st[KT];
         if (c > 0) {
             const f32x4* p = state_tiles(a, seq, c, wave);
 #pragma unroll
             for (int i = 0; i < KT; i++) {
                 st[i] = zero;
-                if (16 * i < int(kd) && 16 * wave < int(vd)) st[i] = p[64 * i + lane];
+                if (16 * i < kd && v_wave) st[i] = p[64 * i + lane];
             }
         } else {
-            load_state(st, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, l, vc);
+            load_state(st, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
         }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t t = 16 * i + 4 * l.quad + e;
-                const bool in = t < left && vc < vd;
-                const float y = load_one<E>(a.v.p, (in ? int64_t(c * C + t) * a.v.tick : 0) + n * a.v.env + h * a.v.head + (in ? vc : 0u));
-                x[i][e] = in ? y : 0.0f;
-            }
         __syncthreads();
         if (c > 0) fetch(c - 1);
 
@@ -151,6 +155,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             f32x4 qk = zero;
 #pragma unroll
             for (int y = 0; y < D; y += 32) {
+                if (y >= kd) continue;
                 const auto kj = ordered_row(l, s.k, ST, j0, y);
                 mma(kk, ordered_row(l, s.k, ST, i0, y), kj);
                 mma(qk, ordered_row(l, s.q, ST, i0, y), kj);
@@ -170,16 +175,17 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             else
                 put_tile(l, s.sys.inv, CP, SP, 0, 16, am);
         }
-        if (wave == Shared::W - 1 && c > 0) {
+        if (wave == waves - 1 && c > 0) {
             put_gates(s.gates[(c - 1) & 1], gate);
             if (c > 1) fetch_gates(c - 2);
         }
         // X, and the part of dU through G
-        f32x4 dr[2] = {zero, zero}, du[2] = {zero, zero};
-        {
+        f32x4 x[2], dr[2] = {zero, zero}, du[2] = {zero, zero};
+        if (v_wave) {
             f32x4 ks[2] = {zero, zero};
 #pragma unroll
             for (int y = 0; y < D; y += 32) {
+                if (y >= kd) continue;
                 const auto sf = frag_of<E>(st[y / 16], st[y / 16 + 1]);
                 const auto gf = frag_of<E>(g[y / 16], g[y / 16 + 1]);
 #pragma unroll
@@ -194,14 +200,15 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int t = 16 * i + 4 * l.quad + e;
-                    x[i][e] -= gates.before[t] * ks[i][e];
+                    x[i][e] = float(s.v[t * ST + 16 * wave + l.col]) - gates.before[t] * ks[i][e];
                     dr[i][e] = gates.beta[t] * x[i][e];
                     du[i][e] *= gates.after[t];
                 }
-        }
-        if (HALVES == 1 || 16 * wave < VH)
+            if (HALVES == 1 || 16 * wave < VH)
 #pragma unroll
-            for (int i = 0; i < KT; i++) put_tile(l, s.through, TS, 0, 16 * wave, 16 * i, st[i]);
+                for (int i = 0; i < KT; i++)
+                    if (16 * i < kd) put_tile(l, s.through, TS, 0, 16 * wave, 16 * i, st[i]);
+        }
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < KT; i++)
@@ -212,7 +219,8 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
         __syncthreads();
 
         // U and R
-        {
+        f32x4 dv[2];
+        if (v_wave) {
             f32x4 u[2];
             solve(l, s.sys, dr, u);
 #pragma unroll
@@ -222,54 +230,55 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             for (int i = 0; i < 2; i++) mma(du[i], row_frag<N>(l, s.sys.scores, CP, SP, 16 * i, 0), of);
             solve_transposed(l, s.sys, du, dr);
 #pragma unroll
-            for (int i = 0; i < 2; i++) put_tile(l, s.r, CP, PL, 16 * wave, 16 * i, dr[i]);
-        }
+            for (int i = 0; i < 2; i++) {
+                put_tile(l, s.r, CP, PL, 16 * wave, 16 * i, dr[i]);
+                f32x4 sum;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t t = 16 * i + 4 * l.quad + e;
-                const float sum = sum16(dr[i][e] * x[i][e]);
-                if (l.col == 0) s.beta_v[wave][t] = sum;
-                const float beta = gates.beta[t];
-                if (t < left && vc < vd)
-                    reinterpret_cast<E*>(d.d_v.p)[int64_t(c * C + t) * d.d_v.tick + n * d.d_v.env + h * d.d_v.head + vc] =
-                        E(beta * dr[i][e]);
-                dr[i][e] *= beta * gates.before[t];  // from here on gamma beta R
+                for (int e = 0; e < 4; e++) {
+                    const int t = 16 * i + 4 * l.quad + e;
+                    const float beta = gates.beta[t];
+                    sum[e] = sum16(dr[i][e] * x[i][e]);
+                    dv[i][e] = beta * dr[i][e];
+                    dr[i][e] = dv[i][e] * gates.before[t];  // from here on gamma beta R
+                }
+                if (l.col == 0) *reinterpret_cast<f32x4*>(&s.beta_v[wave][16 * i + 4 * l.quad]) = sum;
             }
+        }
         __syncthreads();
 
         // dP and dA, by the wavefronts that hold P and A
-        f32x4 dp = zero, da = zero;
         if (wave < 3) {
+            f32x4 dp = zero, da = zero;
 #pragma unroll
             for (int y = 0; y < D; y += 32) {
+                if (y >= vd) continue;
                 const auto uj = col_frag<N>(l, s.u, CP, PL, y, j0);
                 mma(dp, ordered_row(l, s.d_o, ST, i0, y), uj);
                 mma(da, col_frag<N>(l, s.r, CP, PL, y, i0), uj);
             }
             double m_row[4], m_col = 0.0;
+            f32x4 b;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = i0 + 4 * l.quad + r;
                 da[r] = i > j0 + l.col ? -da[r] : 0.0f;
-                const float m = dp[r] * pm[r] + da[r] * am[r];
-                m_row[r] = double(m);
-                m_col += double(m);
-                m_row[r] = sum16(m_row[r]);
-                const float b = sum16(da[r] * kk[r]);
-                if (l.col == 0) {
-                    s.m_row[wave][4 * l.quad + r] = m_row[r];
-                    s.beta_a[wave][4 * l.quad + r] = b;
-                }
+                const double m = double(dp[r] * pm[r] + da[r] * am[r]);
+                m_row[r] = sum16(m);
+                m_col += m;
+                b[r] = sum16(da[r] * kk[r]);
                 dp[r] *= a.scale * dec[r];
                 da[r] *= gates.beta[i] * dec[r];
+            }
+            if (l.col == 0) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) s.m_row[wave][4 * l.quad + r] = m_row[r];
+                *reinterpret_cast<f32x4*>(&s.beta_a[wave][4 * l.quad]) = b;
             }
             m_col += __shfl_xor(m_col, 16);
             m_col += __shfl_xor(m_col, 32);
             if (l.quad == 0) s.m_col[wave][l.col] = m_col;
-            put_tile(l, s.d_scores, CP, SP, j0, i0, dp);
-            put_tile(l, s.d_a, CP, SP, j0, i0, da);
+            put_tile(l, s.sys.scores, CP, SP, j0, i0, dp);  // scale D dP, and E
+            put_tile(l, s.sys.inv, CP, SP, j0, i0, da);
         }
         // through S
         f32x4 dq[2] = {zero, zero}, dk[2] = {zero, zero}, dkg[2] = {zero, zero};
@@ -277,79 +286,80 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
         for (int half = 0; half < HALVES; half++) {
             if (half > 0) {
                 __syncthreads();
-                if (16 * wave >= VH)
+                if (16 * wave >= VH && v_wave)
 #pragma unroll
-                    for (int i = 0; i < KT; i++) put_tile(l, s.through, TS, 0, 16 * wave - VH, 16 * i, st[i]);
+                    for (int i = 0; i < KT; i++)
+                        if (16 * i < kd) put_tile(l, s.through, TS, 0, 16 * wave - VH, 16 * i, st[i]);
                 __syncthreads();
             }
+            if (k_wave)
 #pragma unroll
-            for (int y = 0; y < VH; y += 32) {
-                const auto sf = frag_of<E>(col4(l, s.through, TS, y, 16 * wave), col4(l, s.through, TS, y + 16, 16 * wave));
+                for (int y = 0; y < VH; y += 32) {
+                    if (half * VH + y >= vd) continue;
+                    const auto sf = frag_of<E>(col4(l, s.through, TS, y, 16 * wave), col4(l, s.through, TS, y + 16, 16 * wave));
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    mma(dq[i], ordered_row(l, s.d_o, ST, 16 * i, half * VH + y), sf);
-                    mma(dk[i], col_frag<N>(l, s.r, CP, PL, half * VH + y, 16 * i), sf);
+                    for (int i = 0; i < 2; i++) {
+                        mma(dq[i], ordered_row(l, s.d_o, ST, 16 * i, half * VH + y), sf);
+                        mma(dk[i], col_frag<N>(l, s.r, CP, PL, half * VH + y, 16 * i), sf);
+                    }
                 }
-            }
         }
         // through G
 #pragma unroll
         for (int half = 0; half < HALVES; half++) {
             __syncthreads();
-            if (HALVES == 1 || (16 * wave >= VH) == (half == 1))
+            if (v_wave && (HALVES == 1 || (16 * wave >= VH) == (half == 1)))
 #pragma unroll
-                for (int i = 0; i < KT; i++) put_tile(l, s.through, TS, 0, 16 * wave - half * VH, 16 * i, g[i]);
+                for (int i = 0; i < KT; i++)
+                    if (16 * i < kd) put_tile(l, s.through, TS, 0, 16 * wave - half * VH, 16 * i, g[i]);
             __syncthreads();
+            if (k_wave)
 #pragma unroll
-            for (int y = 0; y < VH; y += 32) {
-                const auto gf = frag_of<E>(col4(l, s.through, TS, y, 16 * wave), col4(l, s.through, TS, y + 16, 16 * wave));
+                for (int y = 0; y < VH; y += 32) {
+                    if (half * VH + y >= vd) continue;
+                    const auto gf = frag_of<E>(col4(l, s.through, TS, y, 16 * wave), col4(l, s.through, TS, y + 16, 16 * wave));
 #pragma unroll
-                for (int i = 0; i < 2; i++) mma(dkg[i], col_frag<N>(l, s.u, CP, PL, half * VH + y, 16 * i), gf);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int t = 16 * i + 4 * l.quad + e;
-                const int at = t * ST + place(16 * wave) + 8 * (l.col >> 2) + (l.col & 3);
-                const float qv = float(s.q[at]), kv = float(s.k[at]);
-                const float before = gates.before[t];
-                dq[i][e] *= a.scale * before;
-                dk[i][e] *= -gates.beta[t] * before;
-                dkg[i][e] *= gates.after[t];
-                const float pa = sum16(fmaf(qv, dq[i][e], kv * dk[i][e])), pb = sum16(kv * dkg[i][e]);
-                if (l.col == 0) {
-                    s.a[wave][t] = pa;
-                    s.b[wave][t] = pb;
+                    for (int i = 0; i < 2; i++) mma(dkg[i], col_frag<N>(l, s.u, CP, PL, half * VH + y, 16 * i), gf);
                 }
-                dk[i][e] += dkg[i][e];
+        }
+        if (k_wave) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                f32x4 pa, pb;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int t = 16 * i + 4 * l.quad + e;
+                    const int at = t * ST + place(16 * wave) + 8 * (l.col >> 2) + (l.col & 3);
+                    const float qv = float(s.q[at]), kv = float(s.k[at]), before = gates.before[t];
+                    dq[i][e] *= a.scale * before;
+                    dk[i][e] *= -gates.beta[t] * before;
+                    dkg[i][e] *= gates.after[t];
+                    pa[e] = sum16(fmaf(qv, dq[i][e], kv * dk[i][e]));
+                    pb[e] = sum16(kv * dkg[i][e]);
+                    dk[i][e] += dkg[i][e];
+                }
+                if (l.col == 0) {
+                    *reinterpret_cast<f32x4*>(&s.a[wave][16 * i + 4 * l.quad]) = pa;
+                    *reinterpret_cast<f32x4*>(&s.b[wave][16 * i + 4 * l.quad]) = pb;
+                }
             }
-        // inside the chunk
-        {
+            // inside the chunk
             const auto kf = ordered_col(l, s.k, ST, 16 * wave);
             const auto qf = ordered_col(l, s.q, ST, 16 * wave);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                mma(dq[i], col_frag<N>(l, s.d_scores, CP, SP, 0, 16 * i), kf);
-                mma(dk[i], row_frag<N>(l, s.d_scores, CP, SP, 16 * i, 0), qf);
-                mma(dk[i], row_frag<N>(l, s.d_a, CP, SP, 16 * i, 0), kf);
-                mma(dk[i], col_frag<N>(l, s.d_a, CP, SP, 0, 16 * i), kf);
+                const auto pc = col_frag<N>(l, s.sys.scores, CP, SP, 0, 16 * i);
+                const auto pr = row_frag<N>(l, s.sys.scores, CP, SP, 16 * i, 0);
+                mma(dq[i], pc, kf);
+                mma(dk[i], pr, qf);
+                const auto ec = col_frag<N>(l, s.sys.inv, CP, SP, 0, 16 * i);
+                const auto er = row_frag<N>(l, s.sys.inv, CP, SP, 16 * i, 0);
+                mma(dk[i], er, kf);
+                mma(dk[i], ec, kf);
             }
         }
-        if (vc < kd)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t t = 16 * i + 4 * l.quad + e;
-                    if (t >= left) continue;
-                    const int64_t at = int64_t(c * C + t);
-                    put_grad<E>(d.d_q, at * d.d_q.tick + n * d.d_q.env + hg * d.d_q.head + vc, dq[i][e], d.partial);
-                    put_grad<E>(d.d_k, at * d.d_k.tick + n * d.d_k.env + hg * d.d_k.head + vc, dk[i][e], d.partial);
-                }
         // G before the chunk
-        {
+        if (v_wave) {
             const float total = gates.before[C - 1];
             const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
             f32x4 lo, hi;
@@ -362,21 +372,38 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             const auto rf = frag_of<E>(-dr[0], -dr[1]);
 #pragma unroll
             for (int i = 0; i < KT; i++) {
+                if (16 * i >= kd) continue;
                 g[i] *= total;
                 mma(g[i], ordered_col(l, s.q, ST, 16 * i), of2);
                 mma(g[i], ordered_col(l, s.k, ST, 16 * i), rf);
             }
         }
         __syncthreads();
+        // the rows' gradients, through LDS to whole rows
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int t = 16 * i + 4 * l.quad + e;
+                if (k_wave) {
+                    dq_rows[t * FT + 16 * wave + l.col] = F(dq[i][e]);
+                    dk_rows[t * FT + 16 * wave + l.col] = F(dk[i][e]);
+                }
+                if (v_wave) dv_rows[t * ST + 16 * wave + l.col] = E(dv[i][e]);
+            }
         if (wave == 0) {
             const int t = lane & 31;
             float pa = 0.0f, pb = 0.0f, beta = 0.0f, all = 0.0f;
 #pragma unroll
             for (int w = 0; w < Shared::W; w++) {
-                pa += s.a[w][t];
-                pb += s.b[w][t];
-                beta += s.beta_v[w][t];
-                all += s.dot[w];
+                if (16 * w < kd) {
+                    pa += s.a[w][t];
+                    pb += s.b[w][t];
+                }
+                if (16 * w < vd) {
+                    beta += s.beta_v[w][t];
+                    all += s.dot[w];
+                }
             }
             // tiles (0,0), (1,1), (1,0)
             const double mr = t < 16 ? s.m_row[0][t] : s.m_row[1][t - 16] + s.m_row[2][t - 16];
@@ -394,9 +421,23 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             const float dg = gate_is_flag(gates, t) ? 0.0f : float(after + before + double(gates.before[C - 1]) * double(all));
             if (lane < C && uint32_t(t) < left) {
                 const int64_t at = int64_t(c * C + t);
-                put_gate(a, d.d_g, at * d.d_g.tick + n * d.d_g.env + h * d.d_g.head, dg, bf);
-                put_gate(a, d.d_beta, at * d.d_beta.tick + n * d.d_beta.env + h * d.d_beta.head, beta, bf);
+                put_gate<E>(a, d.d_g, at * d.d_g.tick + n * d.d_g.env + h * d.d_g.head, dg);
+                put_gate<E>(a, d.d_beta, at * d.d_beta.tick + n * d.d_beta.env + h * d.d_beta.head, beta);
             }
+        }
+        __syncthreads();
+        if (on_k.on && on_k.row < left) {
+            store_piece<F>(rows_dq.row(c * C + on_k.row), kd, on_k.col, piece_from_lds(dq_rows + on_k.row * FT + on_k.col));
+            store_piece<F>(rows_dk.row(c * C + on_k.row), kd, on_k.col, piece_from_lds(dk_rows + on_k.row * FT + on_k.col));
+        }
+        if (on_v.on && on_v.row < left)
+            store_piece<E>(rows_dv.row(c * C + on_v.row), vd, on_v.col, piece_from_lds(dv_rows + on_v.row * ST + on_v.col));
+        // `through` is next written after the next chunk's first barrier, u and
+        // r after its second.  Their columns past a narrow head's width are
+        // operands too and have to be 0 again.
+        if (kd < D || vd < D) {
+            __syncthreads();
+            clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
         }
     }
     if (d.d_state) {
@@ -416,27 +457,25 @@ __global__ void sum_heads_kernel(const float* in, E* out, uint64_t count, uint32
     }
 }
 
-template <class E, int D, bool WIDE>
+template <class E, class F, int D>
 hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
     constexpr uint32_t bytes = sizeof(BackwardShared<E, D>);
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
-    const void* f = reinterpret_cast<const void*>(&backward_kernel<E, D, WIDE>);
+    const void* f = reinterpret_cast<const void*>(&backward_kernel<E, F, D>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    backward_kernel<E, D, WIDE><<<dim3(a.envs * a.heads), dim3(D * 4), bytes, stream>>>(a, d);
+    backward_kernel<E, F, D><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a, d);
     return hipGetLastError();
 }
-template <class E>
+template <class E, class F>
 hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
-    const bool narrow = a.k_dim <= 64 && a.v_dim <= 64;
-    const bool wide = (a.q.wide & a.k.wide & d.d_o.wide) && a.k_dim % 8 == 0 && a.v_dim % 8 == 0;
-    if (wide) return narrow ? backward<E, 64, true>(a, d, stream) : backward<E, 128, true>(a, d, stream);
-    return narrow ? backward<E, 64, false>(a, d, stream) : backward<E, 128, false>(a, d, stream);
+    return a.k_dim <= 64 && a.v_dim <= 64 ? backward<E, F, 64>(a, d, stream) : backward<E, F, 128>(a, d, stream);
 }
 
 }  // namespace
 
 hipError_t launch_backward(const Args& a, const GradArgs& d, bool bf, hipStream_t stream) {
-    return bf ? backward<bf16>(a, d, stream) : backward<float>(a, d, stream);
+    if (!bf) return backward<float, float>(a, d, stream);
+    return d.partial ? backward<bf16, float>(a, d, stream) : backward<bf16, bf16>(a, d, stream);
 }
 
 hipError_t launch_sum_heads(const float* in, void* out, uint64_t rows, uint32_t qk_heads, uint32_t shared, uint32_t width,
