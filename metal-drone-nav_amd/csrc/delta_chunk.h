@@ -184,13 +184,15 @@ __device__ __forceinline__ Piece<E> piece_from_lds(const E* m) {
 }
 
 // ---- decays of a chunk, in LDS
-struct Gates {
+struct __align__(16) Gates {
     double sum[C];     // g_1 + .. + g_i, in 64 bits: differences of nearby sums keep their digits
     float beta[C];
     float before[C];   // gamma_i, 0 after a flag
     float after[C];    // gamma_C / gamma_i, 0 before the last flag
     int episode[C];    // flags up to and with tick i
 };
+// Four neighbouring values.
+__device__ __forceinline__ f32x4 four(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 // Whether tick i is an episode's first: nothing before it reaches it.
 __device__ __forceinline__ bool gate_is_flag(const Gates& s, int i) {
     return s.episode[i] != (i ? s.episode[i - 1] : 0);
@@ -223,13 +225,8 @@ __device__ __forceinline__ void put_gates(Gates& s, const GateRegs& r) {
     const int i = l & 31;
     const int episode = __popc(flags & (0xffffffffu >> (31 - i)));
     const int last = __popc(flags);
-    double sum = r.flag ? 0.0 : double(r.g);
-#pragma unroll
-    for (int d = 1; d < C; d <<= 1) {
-        const double up = __shfl_up(sum, d, C);
-        if (i >= d) sum += up;
-    }
-    const double total = __shfl(sum, C - 1, C);
+    const double sum = scan_up32(r.flag ? 0.0 : double(r.g), l);
+    const double total = lane_value(sum, C - 1);
     if (l < C) {
         s.sum[i] = sum;
         s.beta[i] = r.beta;
@@ -241,43 +238,62 @@ __device__ __forceinline__ void put_gates(Gates& s, const GateRegs& r) {
 
 // D of a tile's entries: rows i0 + 4 (l / 16) + r, column j0 + l % 16; 0 above the diagonal.
 __device__ __forceinline__ f32x4 decay_tile(Lane l, const Gates& s, int i0, int j0) {
-    const int j = j0 + l.col;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    typedef double f64x2 __attribute__((ext_vector_type(2)));
+    const int j = j0 + l.col, i = i0 + 4 * l.quad;
     const double sj = s.sum[j];
     const int ej = s.episode[j];
+    const i32x4 ei = *reinterpret_cast<const i32x4*>(s.episode + i);
+    const f64x2 lo = *reinterpret_cast<const f64x2*>(s.sum + i), hi = *reinterpret_cast<const f64x2*>(s.sum + i + 2);
+    const double si[4] = {lo[0], lo[1], hi[0], hi[1]};
     f32x4 d;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        const int i = i0 + 4 * l.quad + r;
-        d[r] = (i >= j && s.episode[i] == ej) ? __expf(float(s.sum[i] - sj)) : 0.0f;
+        const float x = __expf(float(si[r] - sj));
+        d[r] = int(i + r >= j) & int(ei[r] == ej) ? x : 0.0f;
     }
     return d;
 }
 
-// ---- the triangular system.  X = the inverse of 1 + A for a diagonal block,
-// by substitution: lane c of each 16 has column c, rows leave in order and
-// subtract themselves from the rows below (A's column j from LDS, the same
-// address in all lanes).  `at` holds the block of A transposed, [j][i].
-__device__ __forceinline__ void invert_block(Lane l, const float* at, int stride, f32x4 x[4]) {
-    float v[16];
+// ---- the triangular system.  The inverse X of 1 + A for a diagonal block, by
+// substitution, A and X as result tiles: lane l has rows 4 (l / 16) .. + 3 of
+// column l % 16.  The rows of one quad of 16 lanes leave in order (A's entries
+// come from the quad's lane of their column by DPP), then go to the quads
+// below, which subtract them from their own rows.
+template <int J> __device__ __forceinline__ float row_lane(float x) { return from_lane<0x150 + J>(x); }  // row_newbcast
+
+template <int Q> __device__ __forceinline__ void invert_quad(f32x4 a, f32x4& x, int quad) {
+    f32x4 y = x;
+    y[1] = fmaf(-row_lane<4 * Q>(a[1]), y[0], y[1]);
+    y[2] = fmaf(-row_lane<4 * Q>(a[2]), y[0], y[2]);
+    y[3] = fmaf(-row_lane<4 * Q>(a[3]), y[0], y[3]);
+    y[2] = fmaf(-row_lane<4 * Q + 1>(a[2]), y[1], y[2]);
+    y[3] = fmaf(-row_lane<4 * Q + 1>(a[3]), y[1], y[3]);
+    y[3] = fmaf(-row_lane<4 * Q + 2>(a[3]), y[2], y[3]);
+    if (quad == Q) x = y;
+    if (Q == 3) return;
+    f32x4 done;
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = i == l.col ? 1.0f : 0.0f;
+    for (int r = 0; r < 4; r++) done[r] = from_quad<Q>(x[r]);
+    y = x;
 #pragma unroll
-    for (int j = 0; j < 15; j++) {
-#pragma unroll
-        for (int q = (j + 1) / 4; q < 4; q++) {
-            const f32x4 col = *reinterpret_cast<const f32x4*>(at + j * stride + 4 * q);
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (4 * q + r > j) v[4 * q + r] = fmaf(-col[r], v[j], v[4 * q + r]);
-        }
-        // done before A's next columns are read: else all of the block is loaded first, 160 registers
-        if (j % 2 == 1)
-            asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]),
-                              "+v"(v[8]), "+v"(v[9]), "+v"(v[10]), "+v"(v[11]), "+v"(v[12]), "+v"(v[13]), "+v"(v[14]),
-                              "+v"(v[15])::"memory");
+    for (int r = 0; r < 4; r++) {
+        y[r] = fmaf(-row_lane<4 * Q>(a[r]), done[0], y[r]);
+        y[r] = fmaf(-row_lane<4 * Q + 1>(a[r]), done[1], y[r]);
+        y[r] = fmaf(-row_lane<4 * Q + 2>(a[r]), done[2], y[r]);
+        y[r] = fmaf(-row_lane<4 * Q + 3>(a[r]), done[3], y[r]);
     }
+    if (quad > Q) x = y;
+}
+__device__ __forceinline__ f32x4 invert_block(Lane l, f32x4 a) {
+    f32x4 x;
 #pragma unroll
-    for (int q = 0; q < 4; q++) x[q] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+    for (int r = 0; r < 4; r++) x[r] = 4 * l.quad + r == l.col ? 1.0f : 0.0f;
+    invert_quad<0>(a, x, l.quad);
+    invert_quad<1>(a, x, l.quad);
+    invert_quad<2>(a, x, l.quad);
+    invert_quad<3>(a, x, l.quad);
+    return x;
 }
 
 // The chunk's small matrices in LDS.  All are stored transposed, [j][i]:
@@ -286,28 +302,9 @@ __device__ __forceinline__ void invert_block(Lane l, const float* at, int stride
 template <class E> struct System {
     static constexpr int N = Kind<E>::MID;
     static constexpr int PLANE = C * CP;
-    float at[2][16 * 20];      // the diagonal blocks of A
     E inv[N * PLANE];          // [j][i]: the diagonal blocks' inverses; A_10 at [j][16 + i]
     E scores[N * PLANE];       // scale D (q_i k_j)
 };
-
-// The wavefront that holds a diagonal block of A in a result tile inverts it
-// and stores the inverse.
-template <class E>
-__device__ __forceinline__ void solve_diagonal(Lane l, System<E>& s, int block, f32x4 a) {
-    float* at = s.at[block];
-    *reinterpret_cast<f32x4*>(at + l.col * 20 + 4 * l.quad) = a;
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wavefront's own writes
-    f32x4 x[4];
-    invert_block(l, at, 20, x);
-    // all four quads hold the same columns; quad q stores rows 4 q .. 4 q + 3
-    f32x4 mine = x[0];
-    if (l.quad == 1) mine = x[1];
-    if (l.quad == 2) mine = x[2];
-    if (l.quad == 3) mine = x[3];
-    put_tile(l, s.inv, CP, System<E>::PLANE, 16 * block, 16 * block, mine);
-}
 
 // U = (1 + A)^-1 R for 16 columns of R, as two result tiles.
 template <class E>

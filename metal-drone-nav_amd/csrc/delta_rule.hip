@@ -136,24 +136,24 @@ template <class E, int D> struct ForwardShared {
 // four): a wavefront has its K x 16 slice of the state in result tiles, which
 // are operands as they are (delta_tiles.h).  D, 64 or 128, is what registers
 // and LDS rows are sized for; narrower heads leave out whole steps of 32.
-template <class E, int D>
-__global__ void __launch_bounds__(D * 4, D == 64 ? 4 : 2) forward_kernel(Args a) {
+template <class E, int D, bool FULL>
+__global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
     typedef ForwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16;
     constexpr bool bf = sizeof(E) == 2;
     extern __shared__ __align__(16) char lds[];
     Shared& s = *reinterpret_cast<Shared*>(lds);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int waves = blockDim.x >> 6;
+    const int waves = FULL ? D / 16 : blockDim.x >> 6;
     const uint64_t seq = blockIdx.x;
     const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
     const uint32_t hq = h / (a.heads / a.qk_heads);
-    const uint32_t kd = a.k_dim, vd = a.v_dim;
+    const uint32_t kd = FULL ? D : a.k_dim, vd = FULL ? D : a.v_dim;
     const Spot ks_(kd), vs_(vd);  // the thread's piece of k and q, and of v and o
     const Track<const E> rows_k(a.k, n, hq), rows_q(a.q, n, hq), rows_v(a.v, n, h);
     const Track<E> rows_o(a.o, n, h);
     const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
-    if (kd < D || vd < D) clear_lds(lds, sizeof(Shared));
+    if (!FULL) clear_lds(lds, sizeof(Shared));
 
     f32x4 state[KT];
     {
@@ -219,16 +219,14 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 4 : 2) forward_kernel(Args a)
                 mma(qk, ordered_row(l, s.q, ST, i0, x), kj);
             }
             const f32x4 d = decay_tile(l, gates, i0, j0);
-            f32x4 am, pm;
+            f32x4 am = four(gates.beta + i0 + 4 * l.quad) * d * kk;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = i0 + 4 * l.quad + r;
-                am[r] = i > j0 + l.col ? gates.beta[i] * d[r] * kk[r] : 0.0f;
-                pm[r] = a.scale * d[r] * qk[r];
-            }
+            for (int r = 0; r < 4; r++)
+                if (i0 + 4 * l.quad + r <= j0 + l.col) am[r] = 0.0f;
+            const f32x4 pm = a.scale * d * qk;
             put_tile(l, s.sys.scores, CP, System<E>::PLANE, j0, i0, pm);
             if (wave < 2)
-                solve_diagonal(l, s.sys, wave, am);
+                put_tile(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
             else
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
         }
@@ -250,14 +248,14 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 4 : 2) forward_kernel(Args a)
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 2; i++) {
+                const int t = 16 * i + 4 * l.quad;
+                const f32x4 g = four(gates.before + t);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int t = 16 * i + 4 * l.quad + e;
-                    const float g = gates.before[t];
-                    r[i][e] = gates.beta[t] * (float(s.v[t * ST + 16 * wave + l.col]) - g * ks[i][e]);
-                    qs[i][e] *= a.scale * g;
-                }
+                for (int e = 0; e < 4; e++) r[i][e] = float(s.v[(t + e) * ST + 16 * wave + l.col]);
+                r[i] = four(gates.beta + t) * (r[i] - g * ks[i]);
+                qs[i] *= a.scale * g;
+            }
         }
         __syncthreads();
         if (16 * wave < int(vd)) {
@@ -269,13 +267,12 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 4 : 2) forward_kernel(Args a)
                 for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E>::PLANE, 0, 16 * i), uf);
             }
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 2; i++) {
+                const int t = 16 * i + 4 * l.quad;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int t = 16 * i + 4 * l.quad + e;
-                    s.v[t * ST + 16 * wave + l.col] = E(qs[i][e]);
-                    u[i][e] *= gates.after[t];
-                }
+                for (int e = 0; e < 4; e++) s.v[(t + e) * ST + 16 * wave + l.col] = E(qs[i][e]);
+                u[i] *= four(gates.after + t);
+            }
             // S <- gamma_C S + K^T u
             const float total = gates.before[C - 1];
             const auto uf = frag_of<E>(u[0], u[1]);
@@ -294,13 +291,18 @@ __global__ void __launch_bounds__(D * 4, D == 64 ? 4 : 2) forward_kernel(Args a)
     if (a.state_out) store_state(a.state_out + seq * kd * vd, state, kd, vd, l, 16 * wave + l.col);
 }
 
-template <class E, int D>
+template <class E, int D, bool FULL>
 hipError_t forward(const Args& a, hipStream_t stream) {
     constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
-    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D>);
+    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, FULL>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    forward_kernel<E, D><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a);
+    forward_kernel<E, D, FULL><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a);
     return hipGetLastError();
+}
+// FULL: heads as wide as the kernel's tiles, without the branches for narrower ones.
+template <class E, int D>
+hipError_t forward(const Args& a, hipStream_t stream) {
+    return a.k_dim == D && a.v_dim == D ? forward<E, D, true>(a, stream) : forward<E, D, false>(a, stream);
 }
 template <class E>
 hipError_t forward(const Args& a, hipStream_t stream) {

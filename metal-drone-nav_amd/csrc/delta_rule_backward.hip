@@ -57,7 +57,7 @@ template <class E> __device__ __forceinline__ void put_gate(const Args& a, const
 // wavefront has 16 columns of V (its slices of S, G, U and R) and, for the
 // gradients of q and k, 16 columns of K; U, R, S and G change hands through
 // LDS.  F is the type of the rows of d_q and d_k.
-template <class E, class F, int D>
+template <class E, class F, int D, bool FULL>
 __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) {
     typedef BackwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16, SP = System<E>::PLANE, PL = Shared::PLANE;
@@ -71,19 +71,19 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     F* const dk_rows = dq_rows + C * FT;
     E* const dv_rows = reinterpret_cast<E*>(dk_rows + C * FT);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int waves = blockDim.x >> 6;
+    const int waves = FULL ? D / 16 : blockDim.x >> 6;
     const uint64_t seq = blockIdx.x;
     const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
     const uint32_t hq = h / (a.heads / a.qk_heads), hg = d.partial ? h : hq;
-    const int kd = a.k_dim, vd = a.v_dim;
-    const bool v_wave = 16 * wave < vd, k_wave = 16 * wave < kd;
+    const int kd = FULL ? D : int(a.k_dim), vd = FULL ? D : int(a.v_dim);
+    const bool v_wave = FULL || 16 * wave < vd, k_wave = FULL || 16 * wave < kd;
     const Spot on_k(kd), on_v(vd);
     const Track<const E> rows_k(a.k, n, hq), rows_q(a.q, n, hq), rows_v(a.v, n, h), rows_do(d.d_o, n, h);
     const Track<F> rows_dq(d.d_q, n, hg), rows_dk(d.d_k, n, hg);
     const Track<E> rows_dv(d.d_v, n, h);
     const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
     const f32x4 zero{0, 0, 0, 0};
-    if (kd < D || vd < D) clear_lds(lds, sizeof(Shared));
+    if (!FULL) clear_lds(lds, sizeof(Shared));
 
     f32x4 g[KT];  // G, K x 16
     {
@@ -161,17 +161,15 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 mma(qk, ordered_row(l, s.q, ST, i0, y), kj);
             }
             dec = decay_tile(l, gates, i0, j0);
+            kk *= dec;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = i0 + 4 * l.quad + r;
-                if (i <= j0 + l.col) kk[r] = 0.0f;
-                kk[r] *= dec[r];
-                am[r] = gates.beta[i] * kk[r];
-                pm[r] = a.scale * dec[r] * qk[r];
-            }
+            for (int r = 0; r < 4; r++)
+                if (i0 + 4 * l.quad + r <= j0 + l.col) kk[r] = 0.0f;
+            am = four(gates.beta + i0 + 4 * l.quad) * kk;
+            pm = a.scale * dec * qk;
             put_tile(l, s.sys.scores, CP, SP, j0, i0, pm);
             if (wave < 2)
-                solve_diagonal(l, s.sys, wave, am);
+                put_tile(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
             else
                 put_tile(l, s.sys.inv, CP, SP, 0, 16, am);
         }
@@ -196,14 +194,14 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 2; i++) {
+                const int t = 16 * i + 4 * l.quad;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int t = 16 * i + 4 * l.quad + e;
-                    x[i][e] = float(s.v[t * ST + 16 * wave + l.col]) - gates.before[t] * ks[i][e];
-                    dr[i][e] = gates.beta[t] * x[i][e];
-                    du[i][e] *= gates.after[t];
-                }
+                for (int e = 0; e < 4; e++) x[i][e] = float(s.v[(t + e) * ST + 16 * wave + l.col]);
+                x[i] -= four(gates.before + t) * ks[i];
+                dr[i] = four(gates.beta + t) * x[i];
+                du[i] *= four(gates.after + t);
+            }
             if (HALVES == 1 || 16 * wave < VH)
 #pragma unroll
                 for (int i = 0; i < KT; i++)
@@ -232,15 +230,11 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 put_tile(l, s.r, CP, PL, 16 * wave, 16 * i, dr[i]);
-                f32x4 sum;
+                f32x4 sum = dr[i] * x[i];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int t = 16 * i + 4 * l.quad + e;
-                    const float beta = gates.beta[t];
-                    sum[e] = sum16(dr[i][e] * x[i][e]);
-                    dv[i][e] = beta * dr[i][e];
-                    dr[i][e] = dv[i][e] * gates.before[t];  // from here on gamma beta R
-                }
+                for (int e = 0; e < 4; e++) sum[e] = sum16(sum[e]);
+                dv[i] = four(gates.beta + 16 * i + 4 * l.quad) * dr[i];
+                dr[i] = dv[i] * four(gates.before + 16 * i + 4 * l.quad);  // from here on gamma beta R
                 if (l.col == 0) *reinterpret_cast<f32x4*>(&s.beta_v[wave][16 * i + 4 * l.quad]) = sum;
             }
         }
@@ -260,15 +254,14 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             f32x4 b;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int i = i0 + 4 * l.quad + r;
-                da[r] = i > j0 + l.col ? -da[r] : 0.0f;
+                da[r] = i0 + 4 * l.quad + r > j0 + l.col ? -da[r] : 0.0f;
                 const double m = double(dp[r] * pm[r] + da[r] * am[r]);
                 m_row[r] = sum16(m);
                 m_col += m;
                 b[r] = sum16(da[r] * kk[r]);
-                dp[r] *= a.scale * dec[r];
-                da[r] *= gates.beta[i] * dec[r];
             }
+            dp *= a.scale * dec;
+            da *= four(gates.beta + i0 + 4 * l.quad) * dec;
             if (l.col == 0) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) s.m_row[wave][4 * l.quad + r] = m_row[r];
@@ -325,19 +318,20 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
         if (k_wave) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
+                const int t = 16 * i + 4 * l.quad;
+                const f32x4 before = four(gates.before + t);
+                dq[i] *= a.scale * before;
+                dk[i] *= -four(gates.beta + t) * before;
+                dkg[i] *= four(gates.after + t);
                 f32x4 pa, pb;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int t = 16 * i + 4 * l.quad + e;
-                    const int at = t * ST + place(16 * wave) + 8 * (l.col >> 2) + (l.col & 3);
-                    const float qv = float(s.q[at]), kv = float(s.k[at]), before = gates.before[t];
-                    dq[i][e] *= a.scale * before;
-                    dk[i][e] *= -gates.beta[t] * before;
-                    dkg[i][e] *= gates.after[t];
+                    const int at = (t + e) * ST + place(16 * wave) + 8 * (l.col >> 2) + (l.col & 3);
+                    const float qv = float(s.q[at]), kv = float(s.k[at]);
                     pa[e] = sum16(fmaf(qv, dq[i][e], kv * dk[i][e]));
                     pb[e] = sum16(kv * dkg[i][e]);
-                    dk[i][e] += dkg[i][e];
                 }
+                dk[i] += dkg[i];
                 if (l.col == 0) {
                     *reinterpret_cast<f32x4*>(&s.a[wave][16 * i + 4 * l.quad]) = pa;
                     *reinterpret_cast<f32x4*>(&s.b[wave][16 * i + 4 * l.quad]) = pb;
@@ -365,9 +359,11 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             f32x4 lo, hi;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                lo[e] = a.scale * gates.before[4 * l.quad + e] * first_term(of, e);
-                hi[e] = a.scale * gates.before[16 + 4 * l.quad + e] * first_term(of, 4 + e);
+                lo[e] = first_term(of, e);
+                hi[e] = first_term(of, 4 + e);
             }
+            lo *= a.scale * four(gates.before + 4 * l.quad);
+            hi *= a.scale * four(gates.before + 16 + 4 * l.quad);
             const auto of2 = frag_of<E>(lo, hi);
             const auto rf = frag_of<E>(-dr[0], -dr[1]);
 #pragma unroll
@@ -396,28 +392,18 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             float pa = 0.0f, pb = 0.0f, beta = 0.0f, all = 0.0f;
 #pragma unroll
             for (int w = 0; w < Shared::W; w++) {
-                if (16 * w < kd) {
-                    pa += s.a[w][t];
-                    pb += s.b[w][t];
-                }
-                if (16 * w < vd) {
-                    beta += s.beta_v[w][t];
-                    all += s.dot[w];
-                }
+                // (what no wavefront writes in a narrow head stays 0)
+                pa += s.a[w][t];
+                pb += s.b[w][t];
+                beta += s.beta_v[w][t];
+                all += s.dot[w];
             }
             // tiles (0,0), (1,1), (1,0)
-            const double mr = t < 16 ? s.m_row[0][t] : s.m_row[1][t - 16] + s.m_row[2][t - 16];
-            const double mc = t < 16 ? s.m_col[0][t] + s.m_col[2][t] : s.m_col[1][t - 16];
-            beta += t < 16 ? s.beta_a[0][t] : s.beta_a[1][t - 16] + s.beta_a[2][t - 16];
-            double after = double(pa) + mr - mc;  // summed over the ticks from t on
-            double before = double(pb);           // summed over the ticks before t
-#pragma unroll
-            for (int y = 1; y < C; y <<= 1) {
-                const double down = __shfl_down(after, y, C), up = __shfl_up(before, y, C);
-                if (t + y < C) after += down;
-                if (t >= y) before += up;
-            }
-            before -= double(pb);
+            const int hi = t >> 4, in = t & 15;
+            const double mr = s.m_row[hi][in] + (hi ? s.m_row[2][in] : 0.0), mc = s.m_col[hi][in] + (hi ? 0.0 : s.m_col[2][in]);
+            beta += s.beta_a[hi][in] + (hi ? s.beta_a[2][in] : 0.0f);
+            const double after = scan_down32(double(pa) + mr - mc, lane);      // over the ticks from t on
+            const double before = scan_up32(double(pb), lane) - double(pb);   // over the ticks before t
             const float dg = gate_is_flag(gates, t) ? 0.0f : float(after + before + double(gates.before[C - 1]) * double(all));
             if (lane < C && uint32_t(t) < left) {
                 const int64_t at = int64_t(c * C + t);
@@ -435,7 +421,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
         // `through` is next written after the next chunk's first barrier, u and
         // r after its second.  Their columns past a narrow head's width are
         // operands too and have to be 0 again.
-        if (kd < D || vd < D) {
+        if (!FULL) {
             __syncthreads();
             clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
         }
@@ -457,14 +443,18 @@ __global__ void sum_heads_kernel(const float* in, E* out, uint64_t count, uint32
     }
 }
 
-template <class E, class F, int D>
+template <class E, class F, int D, bool FULL>
 hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
     constexpr uint32_t bytes = sizeof(BackwardShared<E, D>);
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
-    const void* f = reinterpret_cast<const void*>(&backward_kernel<E, F, D>);
+    const void* f = reinterpret_cast<const void*>(&backward_kernel<E, F, D, FULL>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    backward_kernel<E, F, D><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a, d);
+    backward_kernel<E, F, D, FULL><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a, d);
     return hipGetLastError();
+}
+template <class E, class F, int D>
+hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
+    return a.k_dim == D && a.v_dim == D ? backward<E, F, D, true>(a, d, stream) : backward<E, F, D, false>(a, d, stream);
 }
 template <class E, class F>
 hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {

@@ -71,6 +71,37 @@ __device__ __forceinline__ float sum_rows32(float x) {
     return __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
 }
 
+// Inclusive sums over lanes 0..31, upwards (lane i: lanes 0..i) and downwards
+// (lanes i..31): by DPP shifts inside each 16, then the other 16's total.
+__device__ __forceinline__ double lane_value(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b)), lane)), hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b >> 32)), lane));
+    return __builtin_bit_cast(double, uint64_t(lo) | uint64_t(hi) << 32);
+}
+__device__ __forceinline__ double scan_up32(double x, int lane) {
+    x += from_lane<0x111>(x);  // row_shr 1, 2, 4, 8: 0 where there is no such lane
+    x += from_lane<0x112>(x);
+    x += from_lane<0x114>(x);
+    x += from_lane<0x118>(x);
+    const double low = lane_value(x, 15);
+    return (lane & 16) ? x + low : x;
+}
+__device__ __forceinline__ double scan_down32(double x, int lane) {
+    x += from_lane<0x101>(x);  // row_shl
+    x += from_lane<0x102>(x);
+    x += from_lane<0x104>(x);
+    x += from_lane<0x108>(x);
+    const double high = lane_value(x, 16);
+    return (lane & 16) ? x : x + high;
+}
+// Lanes 16 Q .. 16 Q + 15 to all four sixteens.
+template <int Q> __device__ __forceinline__ float from_quad(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    const unsigned half = Q & 2 ? r[1] : r[0];
+    const auto t = __builtin_amdgcn_permlane16_swap(half, half, false, false);
+    return __builtin_bit_cast(float, unsigned(Q & 1 ? t[1] : t[0]));
+}
+
 template <class E> struct Kind;
 template <> struct Kind<bf16> {
     static constexpr int MID = 2;  // terms of a computed operand
