@@ -83,6 +83,33 @@ template <class E> struct Track {
     __device__ __forceinline__ E* row(uint32_t t) const { return p + int64_t(t) * tick; }
 };
 
+// Whose rows a workgroup is at: a state (env and heads) and a chunk of its
+// ticks.  Workgroups stay for several states and load the next chunk's rows,
+// of this state or the next one, while they compute.
+struct At {
+    uint64_t seq;
+    uint32_t c, n, h, hq;
+    __device__ __forceinline__ At(const Args& a, uint64_t s, uint32_t chunk) : seq(s), c(chunk) { split(a); }
+    __device__ __forceinline__ void split(const Args& a) {
+        n = uint32_t(seq) / a.heads;  // (states number less than 2^31)
+        h = uint32_t(seq) % a.heads;
+        hq = h / (a.heads / a.qk_heads);
+    }
+    __device__ __forceinline__ bool valid(const Args& a) const { return seq < uint64_t(a.envs) * a.heads; }
+    __device__ __forceinline__ void forth(const Args& a, uint32_t chunks) {
+        if (++c < chunks) return;
+        c = 0;
+        seq += gridDim.x;
+        split(a);
+    }
+    __device__ __forceinline__ void back(const Args& a, uint32_t chunks) {
+        if (c-- > 0) return;
+        c = chunks - 1;
+        seq += gridDim.x;
+        split(a);
+    }
+};
+
 // ---- eight elements of a row, in registers.  Whole pieces move in 16-byte
 // words wherever the row starts (global memory takes them at any multiple of
 // an element's size), the piece that a row ends in one element at a time.

@@ -44,6 +44,18 @@ inline __host__ uint32_t waves_of(const Args& a) {
     return waves < 4 ? 4 : waves;
 }
 
+// Workgroups of a chunk kernel: as many as the GPU holds at once, which then
+// go through the states in turn, or one for each state.
+inline __host__ uint32_t resident_blocks(const void* kernel, const Args& a, uint32_t bytes) {
+    const uint32_t states = a.envs * a.heads;
+    int device = 0, units = 0, per = 0;
+    if (hipGetDevice(&device) != hipSuccess || hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, int(64 * waves_of(a)), bytes) != hipSuccess || units * per < 1)
+        return states;
+    const uint32_t most = uint32_t(units) * uint32_t(per);
+    return states < most ? states : most;
+}
+
 // The backward pass: gradients of o and of the final state in, of the inputs
 // out.  Where several value heads share a query head, d_q and d_k are fp32
 // rows of every value head (`partial`) and sum_heads adds them up.

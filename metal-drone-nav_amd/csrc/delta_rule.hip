@@ -145,64 +145,65 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
     Shared& s = *reinterpret_cast<Shared*>(lds);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int waves = FULL ? D / 16 : blockDim.x >> 6;
-    const uint64_t seq = blockIdx.x;
-    const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
-    const uint32_t hq = h / (a.heads / a.qk_heads);
     const uint32_t kd = FULL ? D : a.k_dim, vd = FULL ? D : a.v_dim;
-    const Spot ks_(kd), vs_(vd);  // the thread's piece of k and q, and of v and o
-    const Track<const E> rows_k(a.k, n, hq), rows_q(a.q, n, hq), rows_v(a.v, n, h);
-    const Track<E> rows_o(a.o, n, h);
+    const Spot on_k(kd), on_v(vd);  // the thread's piece of k and q, and of v and o
     const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
     if (!FULL) clear_lds(lds, sizeof(Shared));
-
-    f32x4 state[KT];
-    {
+    // the matrices' upper right block stays 0
+    if (wave < 2 * N) {
         const Lane l = Lane::mine();
-        load_state(state, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
-        // the matrices' upper right block stays 0
-        if (wave < 2 * N) {
-            E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * System<E>::PLANE;
+        E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * System<E>::PLANE;
 #pragma unroll
-            for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
-        }
+        for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
+    f32x4 state[KT];
     Piece<E> pk, pq, pv;
-    GateRegs gate{0.0f, 0.0f, 0u};
-    const auto fetch = [&](uint32_t c) {
-        if (ks_.on) {
-            const uint32_t at = c * C + ks_.row, t = at < a.ticks ? at : 0u;
-            pk = load_piece<E>(rows_k.row(t), kd, ks_.col);
-            pq = load_piece<E>(rows_q.row(t), kd, ks_.col);
+    const auto fetch = [&](const At& at) {
+        if (on_k.on) {
+            const uint32_t x = at.c * C + on_k.row, t = x < a.ticks ? x : 0u;
+            pk = load_piece<E>(Track<const E>(a.k, at.n, at.hq).row(t), kd, on_k.col);
+            pq = load_piece<E>(Track<const E>(a.q, at.n, at.hq).row(t), kd, on_k.col);
         }
-        if (vs_.on) {
-            const uint32_t at = c * C + vs_.row, t = at < a.ticks ? at : 0u;
-            pv = load_piece<E>(rows_v.row(t), vd, vs_.col);
+        if (on_v.on) {
+            const uint32_t x = at.c * C + on_v.row, t = x < a.ticks ? x : 0u;
+            pv = load_piece<E>(Track<const E>(a.v, at.n, at.h).row(t), vd, on_v.col);
         }
     };
-    // the last wavefront has no tile of A: it makes the next chunk's decays meanwhile
-    const auto fetch_gates = [&](uint32_t c) {
-        const int64_t t = int64_t(c) * C + lane;
-        gate = load_gates(a, bf, n, h, t, lane < C && t < a.ticks);
-    };
-    if (wave == waves - 1) {
-        fetch_gates(0);
-        put_gates(s.gates[0], gate);
-        fetch_gates(1);
-    }
-    fetch(0);
-    for (uint32_t c = 0; c < chunks; c++) {
+    const auto fetch_state = [&](const At& at) {
         const Lane l = Lane::fresh();
-        const Gates& gates = s.gates[c & 1];
-        if (ks_.on) {
-            const bool in = c * C + ks_.row < a.ticks;
-            piece_to_ordered(s.k + ks_.row * ST, ks_.col, mask_piece<E>(pk, in));
-            piece_to_ordered(s.q + ks_.row * ST, ks_.col, mask_piece<E>(pq, in));
+        load_state(state, a.state ? a.state + at.seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+    };
+    // the last wavefront has no tile of A: it makes the next chunk's decays
+    // meanwhile, from what it loaded a chunk before that
+    GateRegs gate{0.0f, 0.0f, 0u};
+    const auto fetch_gates = [&](const At& at) {
+        const int64_t t = int64_t(at.c) * C + lane;
+        gate = load_gates(a, bf, at.n, at.h, t, lane < C && t < a.ticks);
+    };
+    At now(a, blockIdx.x, 0), next = now, later = now;
+    next.forth(a, chunks);
+    later = next;
+    later.forth(a, chunks);
+    fetch(now);
+    if (wave == waves - 1) {
+        fetch_gates(now);
+        put_gates(s.gates[0], gate);
+        if (next.valid(a)) fetch_gates(next);
+    }
+    fetch_state(now);
+    for (uint32_t turn = 0; now.valid(a); turn ^= 1) {
+        const Lane l = Lane::fresh();
+        const Gates& gates = s.gates[turn];
+        const uint32_t left = a.ticks - now.c * C;  // ticks from the chunk's first
+        if (on_k.on) {
+            piece_to_ordered(s.k + on_k.row * ST, on_k.col, mask_piece<E>(pk, on_k.row < left));
+            piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
         }
-        if (vs_.on) piece_to_lds(s.v + vs_.row * ST + vs_.col, mask_piece<E>(pv, c * C + vs_.row < a.ticks));
+        if (on_v.on) piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
         __syncthreads();
-        if (c + 1 < chunks) fetch(c + 1);
-        if (a.chunk_states && c > 0 && 16 * wave < int(vd)) {
-            f32x4* p = state_tiles(a, seq, c, wave);
+        if (next.valid(a)) fetch(next);
+        if (a.chunk_states && now.c > 0 && 16 * wave < int(vd)) {
+            f32x4* p = state_tiles(a, now.seq, now.c, wave);
 #pragma unroll
             for (int i = 0; i < KT; i++)
                 if (16 * i < int(kd)) p[64 * i + lane] = state[i];
@@ -230,9 +231,9 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
             else
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
         }
-        if (wave == waves - 1 && c + 1 < chunks) {
-            put_gates(s.gates[(c + 1) & 1], gate);
-            fetch_gates(c + 2);
+        if (wave == waves - 1 && next.valid(a)) {
+            put_gates(s.gates[turn ^ 1], gate);
+            if (later.valid(a)) fetch_gates(later);
         }
         // the state's part of the ticks
         f32x4 ks[2] = {}, qs[2] = {}, r[2], u[2];
@@ -284,11 +285,17 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
             }
         }
         __syncthreads();
-        if (vs_.on && c * C + vs_.row < a.ticks)
-            store_piece<E>(rows_o.row(c * C + vs_.row), vd, vs_.col, piece_from_lds(s.v + vs_.row * ST + vs_.col));
+        if (on_v.on && on_v.row < left)
+            store_piece<E>(Track<E>(a.o, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
+                           piece_from_lds(s.v + on_v.row * ST + on_v.col));
+        if (now.c + 1 == chunks) {
+            if (a.state_out) store_state(a.state_out + now.seq * kd * vd, state, kd, vd, l, 16 * wave + l.col);
+            if (next.valid(a)) fetch_state(next);
+        }
+        now = next;
+        next = later;
+        later.forth(a, chunks);
     }
-    const Lane l = Lane::fresh();
-    if (a.state_out) store_state(a.state_out + seq * kd * vd, state, kd, vd, l, 16 * wave + l.col);
 }
 
 template <class E, int D, bool FULL>
@@ -296,7 +303,7 @@ hipError_t forward(const Args& a, hipStream_t stream) {
     constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
     const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, FULL>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    forward_kernel<E, D, FULL><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a);
+    forward_kernel<E, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(a);
     return hipGetLastError();
 }
 // FULL: heads as wide as the kernel's tiles, without the branches for narrower ones.

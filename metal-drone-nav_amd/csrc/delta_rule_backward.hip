@@ -72,59 +72,70 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     E* const dv_rows = reinterpret_cast<E*>(dk_rows + C * FT);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int waves = FULL ? D / 16 : blockDim.x >> 6;
-    const uint64_t seq = blockIdx.x;
-    const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
-    const uint32_t hq = h / (a.heads / a.qk_heads), hg = d.partial ? h : hq;
     const int kd = FULL ? D : int(a.k_dim), vd = FULL ? D : int(a.v_dim);
     const bool v_wave = FULL || 16 * wave < vd, k_wave = FULL || 16 * wave < kd;
     const Spot on_k(kd), on_v(vd);
-    const Track<const E> rows_k(a.k, n, hq), rows_q(a.q, n, hq), rows_v(a.v, n, h), rows_do(d.d_o, n, h);
-    const Track<F> rows_dq(d.d_q, n, hg), rows_dk(d.d_k, n, hg);
-    const Track<E> rows_dv(d.d_v, n, h);
     const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
     const f32x4 zero{0, 0, 0, 0};
     if (!FULL) clear_lds(lds, sizeof(Shared));
-
-    f32x4 g[KT];  // G, K x 16
-    {
-        const Lane l = Lane::fresh();
-        load_state(g, d.d_state_out ? d.d_state_out + seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
-        // the matrices' upper right blocks stay 0
-        if (wave < 2 * N) {
-            E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * SP;
+    // the matrices' upper right blocks stay 0
+    if (wave < 2 * N) {
+        const Lane l = Lane::mine();
+        E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * SP;
 #pragma unroll
-            for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
-        }
+        for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
+    f32x4 g[KT], st[KT];  // G and S, K x 16, in result layout
     Piece<E> pk, pq, pv, po;
-    GateRegs gate{0.0f, 0.0f, 0u};
-    const auto fetch = [&](uint32_t c) {
+    const auto fetch = [&](const At& at) {
         if (on_k.on) {
-            const uint32_t at = c * C + on_k.row, t = at < a.ticks ? at : 0u;
-            pk = load_piece<E>(rows_k.row(t), kd, on_k.col);
-            pq = load_piece<E>(rows_q.row(t), kd, on_k.col);
+            const uint32_t x = at.c * C + on_k.row, t = x < a.ticks ? x : 0u;
+            pk = load_piece<E>(Track<const E>(a.k, at.n, at.hq).row(t), kd, on_k.col);
+            pq = load_piece<E>(Track<const E>(a.q, at.n, at.hq).row(t), kd, on_k.col);
         }
         if (on_v.on) {
-            const uint32_t at = c * C + on_v.row, t = at < a.ticks ? at : 0u;
-            pv = load_piece<E>(rows_v.row(t), vd, on_v.col);
-            po = load_piece<E>(rows_do.row(t), vd, on_v.col);
+            const uint32_t x = at.c * C + on_v.row, t = x < a.ticks ? x : 0u;
+            pv = load_piece<E>(Track<const E>(a.v, at.n, at.h).row(t), vd, on_v.col);
+            po = load_piece<E>(Track<const E>(d.d_o, at.n, at.h).row(t), vd, on_v.col);
         }
     };
-    // the last wavefront has no tile of A: it makes the next chunk's decays meanwhile
-    const auto fetch_gates = [&](uint32_t c) {
-        const int64_t t = int64_t(c) * C + lane;
-        gate = load_gates(a, bf, n, h, t, lane < C && t < a.ticks);
-    };
-    if (wave == waves - 1) {
-        fetch_gates(chunks - 1);
-        put_gates(s.gates[(chunks - 1) & 1], gate);
-        if (chunks > 1) fetch_gates(chunks - 2);
-    }
-    fetch(chunks - 1);
-    for (uint32_t c = chunks; c-- > 0;) {
+    const auto fetch_state = [&](const At& at) {
         const Lane l = Lane::fresh();
-        const Gates& gates = s.gates[c & 1];
-        const uint32_t left = a.ticks - c * C;  // ticks from the chunk's first
+        if (at.c > 0) {
+            const f32x4* p = state_tiles(a, at.seq, at.c, wave);
+#pragma unroll
+            for (int i = 0; i < KT; i++) {
+                st[i] = zero;
+                if (16 * i < kd && v_wave) st[i] = p[64 * i + lane];
+            }
+        } else {
+            load_state(st, a.state ? a.state + at.seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+        }
+    };
+    // the last wavefront has no tile of A: it makes the next chunk's decays
+    // meanwhile, from what it loaded a chunk before that
+    GateRegs gate{0.0f, 0.0f, 0u};
+    const auto fetch_gates = [&](const At& at) {
+        const int64_t t = int64_t(at.c) * C + lane;
+        gate = load_gates(a, bf, at.n, at.h, t, lane < C && t < a.ticks);
+    };
+    At now(a, blockIdx.x, chunks - 1), next = now, later = now;
+    next.back(a, chunks);
+    later = next;
+    later.back(a, chunks);
+    fetch(now);
+    fetch_state(now);
+    if (wave == waves - 1) {
+        fetch_gates(now);
+        put_gates(s.gates[0], gate);
+        if (next.valid(a)) fetch_gates(next);
+    }
+    for (uint32_t turn = 0; now.valid(a); turn ^= 1) {
+        const Lane l = Lane::fresh();
+        const Gates& gates = s.gates[turn];
+        const uint32_t left = a.ticks - now.c * C;  // ticks from the chunk's first
+        if (now.c == chunks - 1)
+            load_state(g, d.d_state_out ? d.d_state_out + now.seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
         if (on_k.on) {
             piece_to_ordered(s.k + on_k.row * ST, on_k.col, mask_piece<E>(pk, on_k.row < left));
             piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
@@ -133,20 +144,8 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
             piece_to_ordered(s.d_o + on_v.row * ST, on_v.col, mask_piece<E>(po, on_v.row < left));
         }
-        // S in result layout
-        f32x4 st[KT];
-        if (c > 0) {
-            const f32x4* p = state_tiles(a, seq, c, wave);
-#pragma unroll
-            for (int i = 0; i < KT; i++) {
-                st[i] = zero;
-                if (16 * i < kd && v_wave) st[i] = p[64 * i + lane];
-            }
-        } else {
-            load_state(st, a.state ? a.state + seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
-        }
         __syncthreads();
-        if (c > 0) fetch(c - 1);
+        if (next.valid(a)) fetch(next);
 
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0), kept by their wavefronts
         f32x4 dec = zero, kk = zero, pm = zero, am = zero;
@@ -173,9 +172,9 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             else
                 put_tile(l, s.sys.inv, CP, SP, 0, 16, am);
         }
-        if (wave == waves - 1 && c > 0) {
-            put_gates(s.gates[(c - 1) & 1], gate);
-            if (c > 1) fetch_gates(c - 2);
+        if (wave == waves - 1 && next.valid(a)) {
+            put_gates(s.gates[turn ^ 1], gate);
+            if (later.valid(a)) fetch_gates(later);
         }
         // X, and the part of dU through G
         f32x4 x[2], dr[2] = {zero, zero}, du[2] = {zero, zero};
@@ -297,6 +296,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                     }
                 }
         }
+        if (next.valid(a)) fetch_state(next);  // S is done with
         // through G
 #pragma unroll
         for (int half = 0; half < HALVES; half++) {
@@ -406,18 +406,22 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             const double before = scan_up32(double(pb), lane) - double(pb);   // over the ticks before t
             const float dg = gate_is_flag(gates, t) ? 0.0f : float(after + before + double(gates.before[C - 1]) * double(all));
             if (lane < C && uint32_t(t) < left) {
-                const int64_t at = int64_t(c * C + t);
-                put_gate<E>(a, d.d_g, at * d.d_g.tick + n * d.d_g.env + h * d.d_g.head, dg);
-                put_gate<E>(a, d.d_beta, at * d.d_beta.tick + n * d.d_beta.env + h * d.d_beta.head, beta);
+                const int64_t at = int64_t(now.c * C + t);
+                put_gate<E>(a, d.d_g, at * d.d_g.tick + int64_t(now.n) * d.d_g.env + int64_t(now.h) * d.d_g.head, dg);
+                put_gate<E>(a, d.d_beta, at * d.d_beta.tick + int64_t(now.n) * d.d_beta.env + int64_t(now.h) * d.d_beta.head, beta);
             }
         }
         __syncthreads();
+        const uint32_t hg = d.partial ? now.h : now.hq;
         if (on_k.on && on_k.row < left) {
-            store_piece<F>(rows_dq.row(c * C + on_k.row), kd, on_k.col, piece_from_lds(dq_rows + on_k.row * FT + on_k.col));
-            store_piece<F>(rows_dk.row(c * C + on_k.row), kd, on_k.col, piece_from_lds(dk_rows + on_k.row * FT + on_k.col));
+            const uint32_t t = now.c * C + on_k.row;
+            store_piece<F>(Track<F>(d.d_q, now.n, hg).row(t), kd, on_k.col, piece_from_lds(dq_rows + on_k.row * FT + on_k.col));
+            store_piece<F>(Track<F>(d.d_k, now.n, hg).row(t), kd, on_k.col, piece_from_lds(dk_rows + on_k.row * FT + on_k.col));
         }
         if (on_v.on && on_v.row < left)
-            store_piece<E>(rows_dv.row(c * C + on_v.row), vd, on_v.col, piece_from_lds(dv_rows + on_v.row * ST + on_v.col));
+            store_piece<E>(Track<E>(d.d_v, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
+                           piece_from_lds(dv_rows + on_v.row * ST + on_v.col));
+        if (now.c == 0 && d.d_state) store_state(d.d_state + now.seq * kd * vd, g, kd, vd, l, 16 * wave + l.col);
         // `through` is next written after the next chunk's first barrier, u and
         // r after its second.  Their columns past a narrow head's width are
         // operands too and have to be 0 again.
@@ -425,10 +429,9 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             __syncthreads();
             clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
         }
-    }
-    if (d.d_state) {
-        const Lane l = Lane::fresh();
-        store_state(d.d_state + seq * kd * vd, g, kd, vd, l, 16 * wave + l.col);
+        now = next;
+        next = later;
+        later.back(a, chunks);
     }
 }
 
@@ -449,7 +452,7 @@ hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
     const void* f = reinterpret_cast<const void*>(&backward_kernel<E, F, D, FULL>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    backward_kernel<E, F, D, FULL><<<dim3(a.envs * a.heads), dim3(64 * waves_of(a)), bytes, stream>>>(a, d);
+    backward_kernel<E, F, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(a, d);
     return hipGetLastError();
 }
 template <class E, class F, int D>
