@@ -28,16 +28,11 @@ template <class E>
 __device__ __forceinline__ float load_one(const char* p, int64_t i) {
     return float(reinterpret_cast<const E*>(p)[i]);
 }
-__device__ __forceinline__ float load_gate(const Args& a, const Rows& r, int64_t i, bool bf) {
-    if (a.gate_f32 || !bf) return reinterpret_cast<const float*>(r.p)[i];
-    return float(reinterpret_cast<const bf16*>(r.p)[i]);
-}
 
 // Wavefront `wave`'s tiles of the state before chunk `c` >= 1.
-__device__ __forceinline__ f32x4* state_tiles(const Args& a, uint64_t seq, uint32_t c, int wave) {
-    const uint64_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
-    return reinterpret_cast<f32x4*>(a.chunk_states + (seq * (chunks - 1) + c - 1) * state_tile_words(a)) +
-           wave * ((a.k_dim + 15) / 16) * 64;
+__device__ __forceinline__ f32x4* state_tiles(float* p, uint64_t seq, uint32_t chunks, uint32_t c, uint32_t kd, uint32_t vd, int wave) {
+    const uint32_t kt = (kd + 15) / 16, vt = (vd + 15) / 16;
+    return reinterpret_cast<f32x4*>(p) + ((seq * (chunks - 1) + c - 1) * (kt * vt) + wave * kt) * 64;
 }
 
 // A wavefront's 16 columns of a state [K][V] as result tiles; `col` is the lane's column.
@@ -74,12 +69,28 @@ __device__ __forceinline__ void store_state(float* p, const f32x4 (&x)[KT], uint
         }
 }
 
+// ---- a kernel's arguments, read from the kernel's argument memory where they
+// are used.  A chunk kernel has more of them than scalar registers: kept
+// across the loop they are spilled to lanes of vector registers, and each use
+// costs vector instructions.
+struct Call {
+    Args a;
+    GradArgs d;
+};
+typedef __attribute__((address_space(4))) const Call KernelCall;
+typedef __attribute__((address_space(4))) const Rows KernelRows;
+__device__ __forceinline__ KernelCall* fresh_call() {
+    KernelCall* p = (KernelCall*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 // ---- rows of one state's array: its env's and head's start, and the ticks' stride
 template <class E> struct Track {
     E* p;
     int64_t tick;
-    __device__ __forceinline__ Track(const Rows& r, uint32_t n, uint32_t h)
-        : p(reinterpret_cast<E*>(r.p) + int64_t(n) * r.env + int64_t(h) * r.head), tick(r.tick) {}
+    __device__ __forceinline__ Track(KernelRows* r, uint32_t n, uint32_t h)
+        : p(reinterpret_cast<E*>(r->p) + int64_t(n) * r->env + int64_t(h) * r->head), tick(r->tick) {}
     __device__ __forceinline__ E* row(uint32_t t) const { return p + int64_t(t) * tick; }
 };
 
@@ -87,26 +98,24 @@ template <class E> struct Track {
 // ticks.  Workgroups stay for several states and load the next chunk's rows,
 // of this state or the next one, while they compute.
 struct At {
-    uint64_t seq;
-    uint32_t c, n, h, hq;
-    __device__ __forceinline__ At(const Args& a, uint64_t s, uint32_t chunk) : seq(s), c(chunk) { split(a); }
-    __device__ __forceinline__ void split(const Args& a) {
-        n = uint32_t(seq) / a.heads;  // (states number less than 2^31)
-        h = uint32_t(seq) % a.heads;
-        hq = h / (a.heads / a.qk_heads);
+    uint32_t seq, c, n, h, hq;
+    __device__ __forceinline__ void split(uint32_t heads, uint32_t shared) {
+        n = seq / heads;
+        h = seq % heads;
+        hq = h / shared;
     }
-    __device__ __forceinline__ bool valid(const Args& a) const { return seq < uint64_t(a.envs) * a.heads; }
-    __device__ __forceinline__ void forth(const Args& a, uint32_t chunks) {
+    // to the next chunk, or the one before, and then to the next state
+    __device__ __forceinline__ void forth(uint32_t chunks, uint32_t heads, uint32_t shared) {
         if (++c < chunks) return;
         c = 0;
         seq += gridDim.x;
-        split(a);
+        split(heads, shared);
     }
-    __device__ __forceinline__ void back(const Args& a, uint32_t chunks) {
+    __device__ __forceinline__ void back(uint32_t chunks, uint32_t heads, uint32_t shared) {
         if (c-- > 0) return;
         c = chunks - 1;
         seq += gridDim.x;
-        split(a);
+        split(heads, shared);
     }
 };
 
@@ -234,25 +243,30 @@ __device__ __forceinline__ void clear_lds(void* lds, uint32_t bytes) {
     __syncthreads();
 }
 
-// Tick `t` of lane t - t0; a tick past the end adds nothing and decays nothing.
-__device__ __forceinline__ GateRegs load_gates(const Args& a, bool bf, uint32_t n, uint32_t h, int64_t t, bool in) {
+__device__ __forceinline__ float one_gate(const char* p, int64_t i, bool f32) {
+    return f32 ? reinterpret_cast<const float*>(p)[i] : float(reinterpret_cast<const bf16*>(p)[i]);
+}
+// One tick's; a tick past the end adds nothing and decays nothing.
+template <class E, class A>
+__device__ __forceinline__ GateRegs load_gates(const A* a, uint32_t n, uint32_t h, uint32_t t, bool in) {
     GateRegs r{0.0f, 0.0f, 0u};
     if (in) {
-        r.g = load_gate(a, a.g, t * a.g.tick + n * a.g.env + h * a.g.head, bf);
-        r.beta = load_gate(a, a.beta, t * a.beta.tick + n * a.beta.env + h * a.beta.head, bf);
-        r.flag = a.reset ? a.reset[t * a.reset_tick + n * a.reset_env] != 0 : 0u;
-        if (r.g < NO_DECAY) r.flag = 1u;
+        const bool f32 = a->gate_f32 || sizeof(E) == 4;
+        r.g = one_gate(a->g.p, int64_t(t) * a->g.tick + int64_t(n) * a->g.env + int64_t(h) * a->g.head, f32);
+        r.beta = one_gate(a->beta.p, int64_t(t) * a->beta.tick + int64_t(n) * a->beta.env + int64_t(h) * a->beta.head, f32);
+        if (a->reset) r.flag = a->reset[int64_t(t) * a->reset_tick + int64_t(n) * a->reset_env] != 0;
     }
     return r;
 }
 // By one wavefront, lanes 0..31 its ticks (the others are given zeros).
 __device__ __forceinline__ void put_gates(Gates& s, const GateRegs& r) {
     const int l = int(threadIdx.x) & 63;
-    const uint32_t flags = uint32_t(__ballot(r.flag != 0));
+    const bool flag = r.flag != 0 || r.g < NO_DECAY;
+    const uint32_t flags = uint32_t(__ballot(flag));
     const int i = l & 31;
     const int episode = __popc(flags & (0xffffffffu >> (31 - i)));
     const int last = __popc(flags);
-    const double sum = scan_up32(r.flag ? 0.0 : double(r.g), l);
+    const double sum = scan_up32(flag ? 0.0 : double(r.g), l);
     const double total = lane_value(sum, C - 1);
     if (l < C) {
         s.sum[i] = sum;

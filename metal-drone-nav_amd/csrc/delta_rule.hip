@@ -51,11 +51,11 @@ __global__ void __launch_bounds__(256, 3) recurrent_kernel(Args a) {
             }
         }
     }
-    constexpr bool bf = sizeof(E) == 2;
     for (uint32_t t = 0; t < a.ticks; t++) {
         const int64_t qo = t * a.q.tick + n * a.q.env + hq * a.q.head;
         const int64_t ko = t * a.k.tick + n * a.k.env + hq * a.k.head;
-        const GateRegs gate = load_gates(a, bf, n, h, t, true);
+        GateRegs gate = load_gates<E>(&a, n, h, t, true);
+        gate.flag |= gate.g < NO_DECAY;
         f32x4 v{0, 0, 0, 0};
         const int64_t vo = t * a.v.tick + n * a.v.env + h * a.v.head + col;
 #pragma unroll
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256, 3) recurrent_kernel(Args a) {
 // ---------------------------------------------------------------- chunks
 template <class E, int D> struct ForwardShared {
     static constexpr int STRIDE = D + Kind<E>::PAD;
-    E k[C * STRIDE], q[C * STRIDE], v[C * STRIDE];  // v's place takes o
+    E k[C * STRIDE], q[C * STRIDE], v[C * STRIDE], o[C * STRIDE];
     System<E> sys;
     Gates gates[2];  // of this chunk and the next
 };
@@ -137,17 +137,18 @@ template <class E, int D> struct ForwardShared {
 // are operands as they are (delta_tiles.h).  D, 64 or 128, is what registers
 // and LDS rows are sized for; narrower heads leave out whole steps of 32.
 template <class E, int D, bool FULL>
-__global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
+__global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
     typedef ForwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16;
-    constexpr bool bf = sizeof(E) == 2;
     extern __shared__ __align__(16) char lds[];
     Shared& s = *reinterpret_cast<Shared*>(lds);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int waves = FULL ? D / 16 : blockDim.x >> 6;
-    const uint32_t kd = FULL ? D : a.k_dim, vd = FULL ? D : a.v_dim;
+    const uint32_t kd = FULL ? D : call.a.k_dim, vd = FULL ? D : call.a.v_dim;
+    const uint32_t ticks = call.a.ticks, chunks = (ticks + CHUNK - 1) / CHUNK;
+    const uint32_t heads = call.a.heads, shared = heads / call.a.qk_heads, states = call.a.envs * heads;
+    const float scale = call.a.scale;
     const Spot on_k(kd), on_v(vd);  // the thread's piece of k and q, and of v and o
-    const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
     if (!FULL) clear_lds(lds, sizeof(Shared));
     // the matrices' upper right block stays 0
     if (wave < 2 * N) {
@@ -159,54 +160,64 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
     f32x4 state[KT];
     Piece<E> pk, pq, pv;
     const auto fetch = [&](const At& at) {
+        KernelCall* k = fresh_call();
         if (on_k.on) {
-            const uint32_t x = at.c * C + on_k.row, t = x < a.ticks ? x : 0u;
-            pk = load_piece<E>(Track<const E>(a.k, at.n, at.hq).row(t), kd, on_k.col);
-            pq = load_piece<E>(Track<const E>(a.q, at.n, at.hq).row(t), kd, on_k.col);
+            const uint32_t x = at.c * C + on_k.row, t = x < ticks ? x : 0u;
+            pk = load_piece<E>(Track<const E>(&k->a.k, at.n, at.hq).row(t), kd, on_k.col);
+            pq = load_piece<E>(Track<const E>(&k->a.q, at.n, at.hq).row(t), kd, on_k.col);
         }
         if (on_v.on) {
-            const uint32_t x = at.c * C + on_v.row, t = x < a.ticks ? x : 0u;
-            pv = load_piece<E>(Track<const E>(a.v, at.n, at.h).row(t), vd, on_v.col);
+            const uint32_t x = at.c * C + on_v.row, t = x < ticks ? x : 0u;
+            pv = load_piece<E>(Track<const E>(&k->a.v, at.n, at.h).row(t), vd, on_v.col);
         }
     };
-    const auto fetch_state = [&](const At& at) {
-        const Lane l = Lane::fresh();
-        load_state(state, a.state ? a.state + at.seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
-    };
-    // the last wavefront has no tile of A: it makes the next chunk's decays
-    // meanwhile, from what it loaded a chunk before that
-    GateRegs gate{0.0f, 0.0f, 0u};
-    const auto fetch_gates = [&](const At& at) {
-        const int64_t t = int64_t(at.c) * C + lane;
-        gate = load_gates(a, bf, at.n, at.h, t, lane < C && t < a.ticks);
-    };
-    At now(a, blockIdx.x, 0), next = now, later = now;
-    next.forth(a, chunks);
-    later = next;
-    later.forth(a, chunks);
-    fetch(now);
-    if (wave == waves - 1) {
-        fetch_gates(now);
-        put_gates(s.gates[0], gate);
-        if (next.valid(a)) fetch_gates(next);
-    }
-    fetch_state(now);
-    for (uint32_t turn = 0; now.valid(a); turn ^= 1) {
-        const Lane l = Lane::fresh();
-        const Gates& gates = s.gates[turn];
-        const uint32_t left = a.ticks - now.c * C;  // ticks from the chunk's first
+    const auto put_rows = [&](const At& at) {
+        const uint32_t left = ticks - at.c * C;
         if (on_k.on) {
             piece_to_ordered(s.k + on_k.row * ST, on_k.col, mask_piece<E>(pk, on_k.row < left));
             piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
         }
         if (on_v.on) piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
-        __syncthreads();
-        if (next.valid(a)) fetch(next);
-        if (a.chunk_states && now.c > 0 && 16 * wave < int(vd)) {
-            f32x4* p = state_tiles(a, now.seq, now.c, wave);
+    };
+    const auto fetch_state = [&](const At& at) {
+        const Lane l = Lane::fresh();
+        const float* p = fresh_call()->a.state;
+        load_state(state, p ? p + uint64_t(at.seq) * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+    };
+    // the last wavefront has no tile of A: it makes the next chunk's decays
+    // meanwhile, from what it loaded a chunk before that
+    GateRegs gate{0.0f, 0.0f, 0u};
+    const auto fetch_gates = [&](const At& at) {
+        const uint32_t t = at.c * C + lane;
+        gate = load_gates<E>(&fresh_call()->a, at.n, at.h, t, lane < C && t < ticks);
+    };
+    At now{blockIdx.x, 0, 0, 0, 0};
+    now.split(heads, shared);
+    At next = now, later;
+    next.forth(chunks, heads, shared);
+    later = next;
+    later.forth(chunks, heads, shared);
+    fetch(now);
+    if (wave == waves - 1) {
+        fetch_gates(now);
+        put_gates(s.gates[0], gate);
+        if (next.seq < states) fetch_gates(next);
+    }
+    fetch_state(now);
+    put_rows(now);
+    __syncthreads();
+    for (uint32_t turn = 0; now.seq < states; turn ^= 1) {
+        const Lane l = Lane::fresh();
+        const Gates& gates = s.gates[turn];
+        const uint32_t left = ticks - now.c * C;  // ticks from the chunk's first
+        if (next.seq < states) fetch(next);
+        if (now.c > 0 && 16 * wave < int(vd)) {
+            if (float* keep = fresh_call()->a.chunk_states) {
+                f32x4* p = state_tiles(keep, now.seq, chunks, now.c, kd, vd, wave);
 #pragma unroll
-            for (int i = 0; i < KT; i++)
-                if (16 * i < int(kd)) p[64 * i + lane] = state[i];
+                for (int i = 0; i < KT; i++)
+                    if (16 * i < int(kd)) p[64 * i + lane] = state[i];
+            }
         }
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0)
         if (wave < 3) {
@@ -224,16 +235,16 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
 #pragma unroll
             for (int r = 0; r < 4; r++)
                 if (i0 + 4 * l.quad + r <= j0 + l.col) am[r] = 0.0f;
-            const f32x4 pm = a.scale * d * qk;
+            const f32x4 pm = scale * d * qk;
             put_tile(l, s.sys.scores, CP, System<E>::PLANE, j0, i0, pm);
             if (wave < 2)
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
             else
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
         }
-        if (wave == waves - 1 && next.valid(a)) {
+        if (wave == waves - 1 && next.seq < states) {
             put_gates(s.gates[turn ^ 1], gate);
-            if (later.valid(a)) fetch_gates(later);
+            if (later.seq < states) fetch_gates(later);
         }
         // the state's part of the ticks
         f32x4 ks[2] = {}, qs[2] = {}, r[2], u[2];
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) r[i][e] = float(s.v[(t + e) * ST + 16 * wave + l.col]);
                 r[i] = four(gates.beta + t) * (r[i] - g * ks[i]);
-                qs[i] *= a.scale * g;
+                qs[i] *= scale * g;
             }
         }
         __syncthreads();
@@ -271,7 +282,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
             for (int i = 0; i < 2; i++) {
                 const int t = 16 * i + 4 * l.quad;
 #pragma unroll
-                for (int e = 0; e < 4; e++) s.v[(t + e) * ST + 16 * wave + l.col] = E(qs[i][e]);
+                for (int e = 0; e < 4; e++) s.o[(t + e) * ST + 16 * wave + l.col] = E(qs[i][e]);
                 u[i] *= four(gates.after + t);
             }
             // S <- gamma_C S + K^T u
@@ -285,16 +296,21 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Args a) {
             }
         }
         __syncthreads();
+        // the next chunk's rows go to LDS before this one's leave: loads and
+        // stores are counted in order, and the loads would wait for the stores
+        if (next.seq < states) put_rows(next);
         if (on_v.on && on_v.row < left)
-            store_piece<E>(Track<E>(a.o, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
-                           piece_from_lds(s.v + on_v.row * ST + on_v.col));
+            store_piece<E>(Track<E>(&fresh_call()->a.o, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
+                           piece_from_lds(s.o + on_v.row * ST + on_v.col));
         if (now.c + 1 == chunks) {
-            if (a.state_out) store_state(a.state_out + now.seq * kd * vd, state, kd, vd, l, 16 * wave + l.col);
-            if (next.valid(a)) fetch_state(next);
+            if (float* p = fresh_call()->a.state_out)
+                store_state(p + uint64_t(now.seq) * kd * vd, state, kd, vd, l, 16 * wave + l.col);
+            if (next.seq < states) fetch_state(next);
         }
         now = next;
         next = later;
-        later.forth(a, chunks);
+        later.forth(chunks, heads, shared);
+        __syncthreads();
     }
 }
 
@@ -303,7 +319,7 @@ hipError_t forward(const Args& a, hipStream_t stream) {
     constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
     const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, FULL>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    forward_kernel<E, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(a);
+    forward_kernel<E, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, GradArgs{}});
     return hipGetLastError();
 }
 // FULL: heads as wide as the kernel's tiles, without the branches for narrower ones.

@@ -46,25 +46,17 @@ template <class E, int D> struct BackwardShared {
     __align__(16) float beta_a[3][16];
 };
 
-template <class E> __device__ __forceinline__ void put_gate(const Args& a, const Rows& r, int64_t at, float x) {
-    if (a.gate_f32 || sizeof(E) == 4)
-        reinterpret_cast<float*>(r.p)[at] = x;
-    else
-        reinterpret_cast<bf16*>(r.p)[at] = bf16(x);
-}
-
 // One workgroup per state, a wavefront for each 16 columns (at least four).  A
 // wavefront has 16 columns of V (its slices of S, G, U and R) and, for the
 // gradients of q and k, 16 columns of K; U, R, S and G change hands through
 // LDS.  F is the type of the rows of d_q and d_k.
 template <class E, class F, int D, bool FULL>
-__global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) {
+__global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
     typedef BackwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16, SP = System<E>::PLANE, PL = Shared::PLANE;
     constexpr int HALVES = Shared::HALVES, TS = Shared::TS, VH = D / HALVES;
     constexpr int FT = D + Kind<F>::PAD;  // row of d_q and d_k in LDS
     static_assert(sizeof(F) * 2 * C * FT + sizeof(E) * C * ST <= sizeof(Shared::u) + sizeof(Shared::r) + sizeof(Shared::through), "");
-    constexpr bool bf = sizeof(E) == 2;
     extern __shared__ __align__(16) char lds[];
     Shared& s = *reinterpret_cast<Shared*>(lds);
     F* const dq_rows = reinterpret_cast<F*>(s.u);
@@ -72,10 +64,12 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     E* const dv_rows = reinterpret_cast<E*>(dk_rows + C * FT);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int waves = FULL ? D / 16 : blockDim.x >> 6;
-    const int kd = FULL ? D : int(a.k_dim), vd = FULL ? D : int(a.v_dim);
+    const int kd = FULL ? D : int(call.a.k_dim), vd = FULL ? D : int(call.a.v_dim);
     const bool v_wave = FULL || 16 * wave < vd, k_wave = FULL || 16 * wave < kd;
+    const uint32_t ticks = call.a.ticks, chunks = (ticks + CHUNK - 1) / CHUNK;
+    const uint32_t heads = call.a.heads, shared = heads / call.a.qk_heads, states = call.a.envs * heads;
+    const float scale = call.a.scale;
     const Spot on_k(kd), on_v(vd);
-    const uint32_t chunks = (a.ticks + CHUNK - 1) / CHUNK;
     const f32x4 zero{0, 0, 0, 0};
     if (!FULL) clear_lds(lds, sizeof(Shared));
     // the matrices' upper right blocks stay 0
@@ -88,54 +82,20 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
     f32x4 g[KT], st[KT];  // G and S, K x 16, in result layout
     Piece<E> pk, pq, pv, po;
     const auto fetch = [&](const At& at) {
+        KernelCall* k = fresh_call();
         if (on_k.on) {
-            const uint32_t x = at.c * C + on_k.row, t = x < a.ticks ? x : 0u;
-            pk = load_piece<E>(Track<const E>(a.k, at.n, at.hq).row(t), kd, on_k.col);
-            pq = load_piece<E>(Track<const E>(a.q, at.n, at.hq).row(t), kd, on_k.col);
+            const uint32_t x = at.c * C + on_k.row, t = x < ticks ? x : 0u;
+            pk = load_piece<E>(Track<const E>(&k->a.k, at.n, at.hq).row(t), kd, on_k.col);
+            pq = load_piece<E>(Track<const E>(&k->a.q, at.n, at.hq).row(t), kd, on_k.col);
         }
         if (on_v.on) {
-            const uint32_t x = at.c * C + on_v.row, t = x < a.ticks ? x : 0u;
-            pv = load_piece<E>(Track<const E>(a.v, at.n, at.h).row(t), vd, on_v.col);
-            po = load_piece<E>(Track<const E>(d.d_o, at.n, at.h).row(t), vd, on_v.col);
+            const uint32_t x = at.c * C + on_v.row, t = x < ticks ? x : 0u;
+            pv = load_piece<E>(Track<const E>(&k->a.v, at.n, at.h).row(t), vd, on_v.col);
+            po = load_piece<E>(Track<const E>(&k->d.d_o, at.n, at.h).row(t), vd, on_v.col);
         }
     };
-    const auto fetch_state = [&](const At& at) {
-        const Lane l = Lane::fresh();
-        if (at.c > 0) {
-            const f32x4* p = state_tiles(a, at.seq, at.c, wave);
-#pragma unroll
-            for (int i = 0; i < KT; i++) {
-                st[i] = zero;
-                if (16 * i < kd && v_wave) st[i] = p[64 * i + lane];
-            }
-        } else {
-            load_state(st, a.state ? a.state + at.seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
-        }
-    };
-    // the last wavefront has no tile of A: it makes the next chunk's decays
-    // meanwhile, from what it loaded a chunk before that
-    GateRegs gate{0.0f, 0.0f, 0u};
-    const auto fetch_gates = [&](const At& at) {
-        const int64_t t = int64_t(at.c) * C + lane;
-        gate = load_gates(a, bf, at.n, at.h, t, lane < C && t < a.ticks);
-    };
-    At now(a, blockIdx.x, chunks - 1), next = now, later = now;
-    next.back(a, chunks);
-    later = next;
-    later.back(a, chunks);
-    fetch(now);
-    fetch_state(now);
-    if (wave == waves - 1) {
-        fetch_gates(now);
-        put_gates(s.gates[0], gate);
-        if (next.valid(a)) fetch_gates(next);
-    }
-    for (uint32_t turn = 0; now.valid(a); turn ^= 1) {
-        const Lane l = Lane::fresh();
-        const Gates& gates = s.gates[turn];
-        const uint32_t left = a.ticks - now.c * C;  // ticks from the chunk's first
-        if (now.c == chunks - 1)
-            load_state(g, d.d_state_out ? d.d_state_out + now.seq * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+    const auto put_rows = [&](const At& at) {
+        const uint32_t left = ticks - at.c * C;
         if (on_k.on) {
             piece_to_ordered(s.k + on_k.row * ST, on_k.col, mask_piece<E>(pk, on_k.row < left));
             piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
@@ -144,8 +104,53 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
             piece_to_ordered(s.d_o + on_v.row * ST, on_v.col, mask_piece<E>(po, on_v.row < left));
         }
-        __syncthreads();
-        if (next.valid(a)) fetch(next);
+    };
+    const auto fetch_state = [&](const At& at) {
+        const Lane l = Lane::fresh();
+        KernelCall* k = fresh_call();
+        if (at.c > 0) {
+            const f32x4* p = state_tiles(k->a.chunk_states, at.seq, chunks, at.c, kd, vd, wave);
+#pragma unroll
+            for (int i = 0; i < KT; i++) {
+                st[i] = zero;
+                if (16 * i < kd && v_wave) st[i] = p[64 * i + lane];
+            }
+        } else {
+            const float* p = k->a.state;
+            load_state(st, p ? p + uint64_t(at.seq) * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+        }
+    };
+    // the last wavefront has no tile of A: it makes the next chunk's decays
+    // meanwhile, from what it loaded a chunk before that
+    GateRegs gate{0.0f, 0.0f, 0u};
+    const auto fetch_gates = [&](const At& at) {
+        const uint32_t t = at.c * C + lane;
+        gate = load_gates<E>(&fresh_call()->a, at.n, at.h, t, lane < C && t < ticks);
+    };
+    At now{blockIdx.x, chunks - 1, 0, 0, 0};
+    now.split(heads, shared);
+    At next = now, later;
+    next.back(chunks, heads, shared);
+    later = next;
+    later.back(chunks, heads, shared);
+    fetch(now);
+    fetch_state(now);
+    if (wave == waves - 1) {
+        fetch_gates(now);
+        put_gates(s.gates[0], gate);
+        if (next.seq < states) fetch_gates(next);
+    }
+    put_rows(now);
+    __syncthreads();
+    for (uint32_t turn = 0; now.seq < states; turn ^= 1) {
+        const Lane l = Lane::fresh();
+        const Gates& gates = s.gates[turn];
+        const uint32_t left = ticks - now.c * C;  // ticks from the chunk's first
+        if (now.c == chunks - 1) {
+            const float* p = fresh_call()->d.d_state_out;
+            load_state(g, p ? p + uint64_t(now.seq) * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+        }
+        if (next.seq < states) fetch(next);
 
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0), kept by their wavefronts
         f32x4 dec = zero, kk = zero, pm = zero, am = zero;
@@ -165,16 +170,16 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             for (int r = 0; r < 4; r++)
                 if (i0 + 4 * l.quad + r <= j0 + l.col) kk[r] = 0.0f;
             am = four(gates.beta + i0 + 4 * l.quad) * kk;
-            pm = a.scale * dec * qk;
+            pm = scale * dec * qk;
             put_tile(l, s.sys.scores, CP, SP, j0, i0, pm);
             if (wave < 2)
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
             else
                 put_tile(l, s.sys.inv, CP, SP, 0, 16, am);
         }
-        if (wave == waves - 1 && next.valid(a)) {
+        if (wave == waves - 1 && next.seq < states) {
             put_gates(s.gates[turn ^ 1], gate);
-            if (later.valid(a)) fetch_gates(later);
+            if (later.seq < states) fetch_gates(later);
         }
         // X, and the part of dU through G
         f32x4 x[2], dr[2] = {zero, zero}, du[2] = {zero, zero};
@@ -259,7 +264,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 m_col += m;
                 b[r] = sum16(da[r] * kk[r]);
             }
-            dp *= a.scale * dec;
+            dp *= scale * dec;
             da *= four(gates.beta + i0 + 4 * l.quad) * dec;
             if (l.col == 0) {
 #pragma unroll
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                     }
                 }
         }
-        if (next.valid(a)) fetch_state(next);  // S is done with
+        if (next.seq < states) fetch_state(next);  // S is done with
         // through G
 #pragma unroll
         for (int half = 0; half < HALVES; half++) {
@@ -320,7 +325,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             for (int i = 0; i < 2; i++) {
                 const int t = 16 * i + 4 * l.quad;
                 const f32x4 before = four(gates.before + t);
-                dq[i] *= a.scale * before;
+                dq[i] *= scale * before;
                 dk[i] *= -four(gates.beta + t) * before;
                 dkg[i] *= four(gates.after + t);
                 f32x4 pa, pb;
@@ -362,8 +367,8 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
                 lo[e] = first_term(of, e);
                 hi[e] = first_term(of, 4 + e);
             }
-            lo *= a.scale * four(gates.before + 4 * l.quad);
-            hi *= a.scale * four(gates.before + 16 + 4 * l.quad);
+            lo *= scale * four(gates.before + 4 * l.quad);
+            hi *= scale * four(gates.before + 16 + 4 * l.quad);
             const auto of2 = frag_of<E>(lo, hi);
             const auto rf = frag_of<E>(-dr[0], -dr[1]);
 #pragma unroll
@@ -406,32 +411,47 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Args a, GradArgs d) 
             const double before = scan_up32(double(pb), lane) - double(pb);   // over the ticks before t
             const float dg = gate_is_flag(gates, t) ? 0.0f : float(after + before + double(gates.before[C - 1]) * double(all));
             if (lane < C && uint32_t(t) < left) {
-                const int64_t at = int64_t(now.c * C + t);
-                put_gate<E>(a, d.d_g, at * d.d_g.tick + int64_t(now.n) * d.d_g.env + int64_t(now.h) * d.d_g.head, dg);
-                put_gate<E>(a, d.d_beta, at * d.d_beta.tick + int64_t(now.n) * d.d_beta.env + int64_t(now.h) * d.d_beta.head, beta);
+                KernelCall* k = fresh_call();
+                const bool f32 = k->a.gate_f32 || sizeof(E) == 4;
+                const uint32_t at = now.c * C + t;
+                if (f32) {
+                    *Track<float>(&k->d.d_g, now.n, now.h).row(at) = dg;
+                    *Track<float>(&k->d.d_beta, now.n, now.h).row(at) = beta;
+                } else {
+                    *Track<bf16>(&k->d.d_g, now.n, now.h).row(at) = bf16(dg);
+                    *Track<bf16>(&k->d.d_beta, now.n, now.h).row(at) = bf16(beta);
+                }
             }
         }
+        // the next chunk's rows and S are waited for before this one's gradients
+        // leave: loads and stores are counted in order, and the loads would
+        // wait for the stores
+        if (next.seq < states) put_rows(next);
+#pragma unroll
+        for (int i = 0; i < KT; i++) asm volatile("" : "+v"(st[i]));
+        asm volatile("" : "+v"(gate.g), "+v"(gate.beta), "+v"(gate.flag));
         __syncthreads();
-        const uint32_t hg = d.partial ? now.h : now.hq;
+        KernelCall* k = fresh_call();
+        const uint32_t hg = k->d.partial ? now.h : now.hq;
         if (on_k.on && on_k.row < left) {
             const uint32_t t = now.c * C + on_k.row;
-            store_piece<F>(Track<F>(d.d_q, now.n, hg).row(t), kd, on_k.col, piece_from_lds(dq_rows + on_k.row * FT + on_k.col));
-            store_piece<F>(Track<F>(d.d_k, now.n, hg).row(t), kd, on_k.col, piece_from_lds(dk_rows + on_k.row * FT + on_k.col));
+            store_piece<F>(Track<F>(&k->d.d_q, now.n, hg).row(t), kd, on_k.col, piece_from_lds(dq_rows + on_k.row * FT + on_k.col));
+            store_piece<F>(Track<F>(&k->d.d_k, now.n, hg).row(t), kd, on_k.col, piece_from_lds(dk_rows + on_k.row * FT + on_k.col));
         }
         if (on_v.on && on_v.row < left)
-            store_piece<E>(Track<E>(d.d_v, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
+            store_piece<E>(Track<E>(&k->d.d_v, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
                            piece_from_lds(dv_rows + on_v.row * ST + on_v.col));
-        if (now.c == 0 && d.d_state) store_state(d.d_state + now.seq * kd * vd, g, kd, vd, l, 16 * wave + l.col);
-        // `through` is next written after the next chunk's first barrier, u and
-        // r after its second.  Their columns past a narrow head's width are
-        // operands too and have to be 0 again.
-        if (!FULL) {
-            __syncthreads();
-            clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
-        }
+        if (now.c == 0)
+            if (float* p = k->d.d_state) store_state(p + uint64_t(now.seq) * kd * vd, g, kd, vd, l, 16 * wave + l.col);
+        // u, r and `through` take the next chunk's operands.  `through` is the
+        // first, before the next barrier: all have to have read their gradients'
+        // rows.  In narrow heads the columns past the width are operands too
+        // and have to be 0 again.
+        __syncthreads();
+        if (!FULL) clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
         now = next;
         next = later;
-        later.back(a, chunks);
+        later.back(chunks, heads, shared);
     }
 }
 
@@ -452,7 +472,7 @@ hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
     const void* f = reinterpret_cast<const void*>(&backward_kernel<E, F, D, FULL>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    backward_kernel<E, F, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(a, d);
+    backward_kernel<E, F, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, d});
     return hipGetLastError();
 }
 template <class E, class F, int D>
