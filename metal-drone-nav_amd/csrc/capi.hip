@@ -2224,14 +2224,17 @@ int delta_args(const char* name, const MdnDeltaRule* d, delta::Args* out) {
     a.beta = device_rows(d->beta);
     a.reset = d->reset; a.reset_tick = d->reset_tick; a.reset_env = d->reset_env;
     a.state = d->state; a.state_out = d->state_out;
+    delta::cut(a);
     *out = a;
     return MDN_OK;
 }
 
-uint64_t delta_keep_bytes(const delta::Args& a) {
+// What the backward pass reads: the states between chunks, and M of the segments of a cut state.
+uint64_t delta_chunk_state_bytes(const delta::Args& a) {
     const uint64_t chunks = (uint64_t(a.ticks) + delta::CHUNK - 1) / delta::CHUNK;
     return chunks > 1 ? (chunks - 1) * a.envs * a.heads * delta::state_tile_words(a) * sizeof(float) : 0;
 }
+uint64_t delta_keep_bytes(const delta::Args& a) { return delta_chunk_state_bytes(a) + delta::seg_move_words(a) * sizeof(float); }
 
 // d_q and d_k of every value head, where heads share them.
 uint64_t delta_partial_bytes(const delta::Args& a) {
@@ -2255,7 +2258,8 @@ int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backwar
     delta::Args a;
     if (int rc = delta_args("mdn_op_delta_rule_workspace_bytes", rule, &a)) return rc;
     if (!bytes) return fail(MDN_E_ARG, "mdn_op_delta_rule_workspace_bytes: null");
-    *bytes = backward ? delta_partial_bytes(a) : 0;
+    // forward: the segments' states and, if nothing is kept, their M
+    *bytes = (backward ? delta_partial_bytes(a) : delta::seg_move_words(a) * sizeof(float)) + delta::seg_state_words(a) * sizeof(float);
     return MDN_OK;
 }
 
@@ -2263,12 +2267,14 @@ int mdn_op_delta_rule_forward(const MdnDeltaRule* rule, void* keep, uint64_t kee
                               uint64_t workspace_bytes, void* stream) {
     delta::Args a;
     if (int rc = delta_args("mdn_op_delta_rule_forward", rule, &a)) return rc;
-    (void)workspace;
-    (void)workspace_bytes;
     if (a.envs == 0) return MDN_OK;
     if (a.ticks && !a.o.p) return fail(MDN_E_ARG, "mdn_op_delta_rule_forward: null rows");
     if (keep && keep_bytes < delta_keep_bytes(a)) return fail(MDN_E_ARG, "mdn_op_delta_rule_forward: keep is too small");
+    const uint64_t need = (delta::seg_state_words(a) + delta::seg_move_words(a)) * sizeof(float);
+    if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_delta_rule_forward: workspace is too small");
     a.chunk_states = keep && delta_keep_bytes(a) ? static_cast<float*>(keep) : nullptr;
+    a.seg_states = static_cast<float*>(workspace);
+    a.seg_moves = a.chunk_states ? a.chunk_states + delta_chunk_state_bytes(a) / sizeof(float) : a.seg_states + delta::seg_state_words(a);
     const bool bf = rule->dtype == MDN_BF16;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (a.ticks <= 1 && !a.chunk_states)
@@ -2295,9 +2301,11 @@ int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad*
         return fail(MDN_E_ARG, who + "null rows");
     if (keep_bytes < delta_keep_bytes(a) || (delta_keep_bytes(a) && !keep))
         return fail(MDN_E_ARG, who + "keep is too small");
-    if (workspace_bytes < delta_partial_bytes(a) || (delta_partial_bytes(a) && !workspace))
-        return fail(MDN_E_ARG, who + "workspace is too small");
+    const uint64_t need = delta_partial_bytes(a) + delta::seg_state_words(a) * sizeof(float);
+    if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, who + "workspace is too small");
     a.chunk_states = static_cast<float*>(const_cast<void*>(keep));
+    a.seg_moves = a.chunk_states + delta_chunk_state_bytes(a) / sizeof(float);
+    a.seg_grads = static_cast<float*>(workspace) + delta_partial_bytes(a) / sizeof(float);
     const uint32_t T = a.ticks, N = a.envs, H = a.heads, Q = a.qk_heads;
     delta::GradArgs d{};
     d.d_o = device_rows(grad->d_o);

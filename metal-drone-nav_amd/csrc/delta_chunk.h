@@ -94,28 +94,40 @@ template <class E> struct Track {
     __device__ __forceinline__ E* row(uint32_t t) const { return p + int64_t(t) * tick; }
 };
 
-// Whose rows a workgroup is at: a state (env and heads) and a chunk of its
-// ticks.  Workgroups stay for several states and load the next chunk's rows,
-// of this state or the next one, while they compute.
+// Whose rows a workgroup is at: a state (env and heads), a segment of its
+// ticks and a chunk of that.  Workgroups stay for several segments and load
+// the next chunk's rows, of this one or the next, while they compute.
+struct Plan {
+    uint32_t heads, shared, chunks, segments, segment, jobs, total;
+    // `jobs` of a state: its segments, or what runs ahead of them
+    __device__ __forceinline__ Plan(const Args& a, uint32_t j)
+        : heads(a.heads), shared(a.heads / a.qk_heads), chunks((a.ticks + CHUNK - 1) / CHUNK), segments(a.segments),
+          segment(a.segment), jobs(j), total(a.envs * a.heads * j) {}
+};
 struct At {
-    uint32_t seq, c, n, h, hq;
-    __device__ __forceinline__ void split(uint32_t heads, uint32_t shared) {
-        n = seq / heads;
-        h = seq % heads;
-        hq = h / shared;
+    uint32_t job, c, first, end;  // the chunk, its segment's first, and the first after it
+    uint32_t state, seg, part, n, h, hq;
+    // job -> state and job of the state; the caller's `seg`, `part` of those
+    template <class F> __device__ __forceinline__ void split(const Plan& p, F which) {
+        state = job / p.jobs;
+        which(*this, job % p.jobs);
+        n = state / p.heads;
+        h = state % p.heads;
+        hq = h / p.shared;
+        first = seg * p.segment;
+        end = first + p.segment < p.chunks ? first + p.segment : p.chunks;
     }
-    // to the next chunk, or the one before, and then to the next state
-    __device__ __forceinline__ void forth(uint32_t chunks, uint32_t heads, uint32_t shared) {
-        if (++c < chunks) return;
-        c = 0;
-        seq += gridDim.x;
-        split(heads, shared);
+    template <class F> __device__ __forceinline__ void forth(const Plan& p, F which) {
+        if (++c < end) return;
+        job += gridDim.x;
+        split(p, which);
+        c = first;
     }
-    __device__ __forceinline__ void back(uint32_t chunks, uint32_t heads, uint32_t shared) {
-        if (c-- > 0) return;
-        c = chunks - 1;
-        seq += gridDim.x;
-        split(heads, shared);
+    template <class F> __device__ __forceinline__ void back(const Plan& p, F which) {
+        if (c-- > first) return;
+        job += gridDim.x;
+        split(p, which);
+        c = end - 1;
     }
 };
 

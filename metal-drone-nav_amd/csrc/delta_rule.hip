@@ -136,7 +136,11 @@ template <class E, int D> struct ForwardShared {
 // four): a wavefront has its K x 16 slice of the state in result tiles, which
 // are operands as they are (delta_tiles.h).  D, 64 or 128, is what registers
 // and LDS rows are sized for; narrower heads leave out whole steps of 32.
-template <class E, int D, bool FULL>
+//
+// AHEAD: what the segments of a cut state need before they run.  Part 0 of a
+// segment starts from zeros (the first from the state) and leaves B, part 1
+// starts from the identity with no v and leaves M; neither has outputs.
+template <class E, int D, bool FULL, bool AHEAD>
 __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
     typedef ForwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16;
@@ -145,8 +149,13 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int waves = FULL ? D / 16 : blockDim.x >> 6;
     const uint32_t kd = FULL ? D : call.a.k_dim, vd = FULL ? D : call.a.v_dim;
-    const uint32_t ticks = call.a.ticks, chunks = (ticks + CHUNK - 1) / CHUNK;
-    const uint32_t heads = call.a.heads, shared = heads / call.a.qk_heads, states = call.a.envs * heads;
+    const uint32_t ticks = call.a.ticks;
+    const Plan plan(call.a, AHEAD ? 2 * call.a.segments - 3 : call.a.segments);
+    const auto which = [&](At& at, uint32_t j) {
+        // AHEAD: part 0 of all segments but the last, then part 1 of all but the first and the last
+        at.part = AHEAD && j >= plan.segments - 1 ? 1 : 0;
+        at.seg = at.part ? j - (plan.segments - 1) + 1 : j;
+    };
     const float scale = call.a.scale;
     const Spot on_k(kd), on_v(vd);  // the thread's piece of k and q, and of v and o
     if (!FULL) clear_lds(lds, sizeof(Shared));
@@ -164,7 +173,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         if (on_k.on) {
             const uint32_t x = at.c * C + on_k.row, t = x < ticks ? x : 0u;
             pk = load_piece<E>(Track<const E>(&k->a.k, at.n, at.hq).row(t), kd, on_k.col);
-            pq = load_piece<E>(Track<const E>(&k->a.q, at.n, at.hq).row(t), kd, on_k.col);
+            if (!AHEAD) pq = load_piece<E>(Track<const E>(&k->a.q, at.n, at.hq).row(t), kd, on_k.col);
         }
         if (on_v.on) {
             const uint32_t x = at.c * C + on_v.row, t = x < ticks ? x : 0u;
@@ -175,14 +184,24 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         const uint32_t left = ticks - at.c * C;
         if (on_k.on) {
             piece_to_ordered(s.k + on_k.row * ST, on_k.col, mask_piece<E>(pk, on_k.row < left));
-            piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
+            if (!AHEAD) piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
         }
-        if (on_v.on) piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
+        if (on_v.on) piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left && (!AHEAD || at.part == 0)));
     };
     const auto fetch_state = [&](const At& at) {
         const Lane l = Lane::fresh();
-        const float* p = fresh_call()->a.state;
-        load_state(state, p ? p + uint64_t(at.seq) * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+        KernelCall* k = fresh_call();
+        const uint64_t words = kd * vd;
+        const float* p = k->a.state;
+        if (p) p += at.state * words;
+        if (at.seg > 0) p = AHEAD ? nullptr : k->a.seg_states + (uint64_t(at.state) * plan.segments + at.seg) * words;
+        load_state(state, p, kd, vd, l, 16 * wave + l.col);
+        if (AHEAD && at.part)
+#pragma unroll
+            for (int i = 0; i < KT; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    state[i][r] = 16 * i + 4 * l.quad + r == 16 * wave + l.col && uint32_t(16 * wave + l.col) < kd ? 1.0f : 0.0f;
     };
     // the last wavefront has no tile of A: it makes the next chunk's decays
     // meanwhile, from what it loaded a chunk before that
@@ -191,29 +210,32 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         const uint32_t t = at.c * C + lane;
         gate = load_gates<E>(&fresh_call()->a, at.n, at.h, t, lane < C && t < ticks);
     };
-    At now{blockIdx.x, 0, 0, 0, 0};
-    now.split(heads, shared);
-    At next = now, later;
-    next.forth(chunks, heads, shared);
+    At now, next, later;
+    now.job = blockIdx.x;
+    now.split(plan, which);
+    now.c = now.first;
+    next = now;
+    next.forth(plan, which);
     later = next;
-    later.forth(chunks, heads, shared);
+    later.forth(plan, which);
     fetch(now);
     if (wave == waves - 1) {
         fetch_gates(now);
         put_gates(s.gates[0], gate);
-        if (next.seq < states) fetch_gates(next);
+        if (next.job < plan.total) fetch_gates(next);
     }
     fetch_state(now);
     put_rows(now);
     __syncthreads();
-    for (uint32_t turn = 0; now.seq < states; turn ^= 1) {
+    for (uint32_t turn = 0; now.job < plan.total; turn ^= 1) {
         const Lane l = Lane::fresh();
         const Gates& gates = s.gates[turn];
         const uint32_t left = ticks - now.c * C;  // ticks from the chunk's first
-        if (next.seq < states) fetch(next);
-        if (now.c > 0 && 16 * wave < int(vd)) {
+        if (next.job < plan.total) fetch(next);
+        const uint32_t cols = AHEAD && now.part ? kd : vd;  // of the state
+        if (!AHEAD && now.c > 0 && 16 * wave < int(vd)) {
             if (float* keep = fresh_call()->a.chunk_states) {
-                f32x4* p = state_tiles(keep, now.seq, chunks, now.c, kd, vd, wave);
+                f32x4* p = state_tiles(keep, now.state, plan.chunks, now.c, kd, vd, wave);
 #pragma unroll
                 for (int i = 0; i < KT; i++)
                     if (16 * i < int(kd)) p[64 * i + lane] = state[i];
@@ -228,7 +250,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
                 if (x >= int(kd)) continue;
                 const auto kj = ordered_row(l, s.k, ST, j0, x);
                 mma(kk, ordered_row(l, s.k, ST, i0, x), kj);
-                mma(qk, ordered_row(l, s.q, ST, i0, x), kj);
+                if (!AHEAD) mma(qk, ordered_row(l, s.q, ST, i0, x), kj);
             }
             const f32x4 d = decay_tile(l, gates, i0, j0);
             f32x4 am = four(gates.beta + i0 + 4 * l.quad) * d * kk;
@@ -236,19 +258,19 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             for (int r = 0; r < 4; r++)
                 if (i0 + 4 * l.quad + r <= j0 + l.col) am[r] = 0.0f;
             const f32x4 pm = scale * d * qk;
-            put_tile(l, s.sys.scores, CP, System<E>::PLANE, j0, i0, pm);
+            if (!AHEAD) put_tile(l, s.sys.scores, CP, System<E>::PLANE, j0, i0, pm);
             if (wave < 2)
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
             else
                 put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
         }
-        if (wave == waves - 1 && next.seq < states) {
+        if (wave == waves - 1 && next.job < plan.total) {
             put_gates(s.gates[turn ^ 1], gate);
-            if (later.seq < states) fetch_gates(later);
+            if (later.job < plan.total) fetch_gates(later);
         }
         // the state's part of the ticks
         f32x4 ks[2] = {}, qs[2] = {}, r[2], u[2];
-        if (16 * wave < int(vd)) {
+        if (16 * wave < int(cols)) {
 #pragma unroll
             for (int x = 0; x < D; x += 32) {
                 if (x >= int(kd)) continue;
@@ -256,7 +278,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     mma(ks[i], ordered_row(l, s.k, ST, 16 * i, x), st);
-                    mma(qs[i], ordered_row(l, s.q, ST, 16 * i, x), st);
+                    if (!AHEAD) mma(qs[i], ordered_row(l, s.q, ST, 16 * i, x), st);
                 }
             }
 #pragma unroll
@@ -270,10 +292,10 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             }
         }
         __syncthreads();
-        if (16 * wave < int(vd)) {
+        if (16 * wave < int(cols)) {
             solve(l, s.sys, r, u);
             // o = scale gamma (q S) + scores u
-            {
+            if (!AHEAD) {
                 const auto uf = frag_of<E>(u[0], u[1]);
 #pragma unroll
                 for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E>::PLANE, 0, 16 * i), uf);
@@ -282,7 +304,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             for (int i = 0; i < 2; i++) {
                 const int t = 16 * i + 4 * l.quad;
 #pragma unroll
-                for (int e = 0; e < 4; e++) s.o[(t + e) * ST + 16 * wave + l.col] = E(qs[i][e]);
+                for (int e = 0; e < 4 && !AHEAD; e++) s.o[(t + e) * ST + 16 * wave + l.col] = E(qs[i][e]);
                 u[i] *= four(gates.after + t);
             }
             // S <- gamma_C S + K^T u
@@ -298,29 +320,114 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         __syncthreads();
         // the next chunk's rows go to LDS before this one's leave: loads and
         // stores are counted in order, and the loads would wait for the stores
-        if (next.seq < states) put_rows(next);
-        if (on_v.on && on_v.row < left)
+        if (next.job < plan.total) put_rows(next);
+        if (!AHEAD && on_v.on && on_v.row < left)
             store_piece<E>(Track<E>(&fresh_call()->a.o, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
                            piece_from_lds(s.o + on_v.row * ST + on_v.col));
-        if (now.c + 1 == chunks) {
-            if (float* p = fresh_call()->a.state_out)
-                store_state(p + uint64_t(now.seq) * kd * vd, state, kd, vd, l, 16 * wave + l.col);
-            if (next.seq < states) fetch_state(next);
+        if (now.c + 1 == now.end) {
+            KernelCall* k = fresh_call();
+            float* p = now.seg + 1 == plan.segments ? k->a.state_out : nullptr;
+            if (p) p += uint64_t(now.state) * kd * vd;
+            const uint64_t slot = uint64_t(now.state) * plan.segments + now.seg;
+            if (AHEAD) p = now.part ? k->a.seg_moves + slot * kd * kd : k->a.seg_states + (slot + 1) * kd * vd;
+            if (p) store_state(p, state, kd, cols, l, 16 * wave + l.col);
+            if (next.job < plan.total) fetch_state(next);
         }
         now = next;
         next = later;
-        later.forth(chunks, heads, shared);
+        later.forth(plan, which);
         __syncthreads();
     }
 }
 
+// ---------------------------------------------------------------- joining segments
+// A workgroup per 16 columns of a state, a wavefront for each 16 rows: it has
+// its rows of M ahead of the product, and the columns' last values come from
+// LDS.
+template <class E, bool TRANSPOSED>
+__global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
+    constexpr int D = int(MAX_DIM), N = Kind<E>::MID, ST = D + Kind<E>::PAD, PL = 16 * ST;
+    __shared__ __align__(16) E last[2][N * PL];  // [column][row]
+    const Lane l = Lane::mine();
+    const int kd = a.k_dim, vd = a.v_dim, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t slices = (vd + 15) / 16, state = blockIdx.x / slices, col = blockIdx.x % slices * 16 + l.col;
+    float* const own = seg + uint64_t(state) * a.segments * kd * vd;
+    const float* const moves = a.seg_moves + uint64_t(state) * a.segments * kd * kd;
+    // the wavefront's tile of the value before or after segment s
+    const auto tile_at = [&](uint32_t s, int r) { return own + uint64_t(s) * kd * vd + uint32_t(16 * wave + 4 * l.quad + r) * vd + col; };
+    const auto load_tile = [&](uint32_t s) {
+        f32x4 x{0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (16 * wave + 4 * l.quad + r < kd && int(col) < vd) x[r] = *tile_at(s, r);
+        return x;
+    };
+    f32x4 m[D / 16];
+    const auto fetch = [&](uint32_t s) {
+        const float* p = moves + uint64_t(s) * kd * kd;
+        const int r = 16 * wave + l.col;
+        if (!TRANSPOSED && kd % 4 == 0) {  // four neighbours in one word
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                const int c = 16 * k + 4 * l.quad;
+                const bool in = r < kd && c < kd;
+                const f32x4 v = *reinterpret_cast<const f32x4*>(p + (in ? r * kd + c : 0));
+#pragma unroll
+                for (int e = 0; e < 4; e++) m[k][e] = in ? v[e] : 0.0f;
+            }
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int c = 16 * k + 4 * l.quad + e;
+                const bool in = r < kd && c < kd;
+                const float v = p[in ? (TRANSPOSED ? c * kd + r : r * kd + c) : 0];
+                m[k][e] = in ? v : 0.0f;
+            }
+    };
+    uint32_t s = TRANSPOSED ? a.segments - 2 : 1;
+    fetch(s);
+    put_tile(l, last[0], ST, PL, 0, 16 * wave, load_tile(s));
+    f32x4 next = load_tile(TRANSPOSED ? s - 1 : s + 1);
+    __syncthreads();
+    for (uint32_t left = a.segments - 2, turn = 0; left > 0; left--, turn ^= 1) {
+        Frag<E, N> mf[D / 32];
+#pragma unroll
+        for (int k = 0; k < D / 32; k++) mf[k] = frag_of<E>(m[2 * k], m[2 * k + 1]);
+        s = TRANSPOSED ? s - 1 : s + 1;
+        f32x4 y = next;
+        if (left > 1) {
+            fetch(s);
+            next = load_tile(TRANSPOSED ? s - 1 : s + 1);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 32; k++) mma(y, mf[k], row_frag<N>(l, last[turn], ST, PL, 0, 32 * k));
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (16 * wave + 4 * l.quad + r < kd && int(col) < vd) *tile_at(s, r) = y[r];
+        put_tile(l, last[turn ^ 1], ST, PL, 0, 16 * wave, y);
+        __syncthreads();
+    }
+}
+
+template <class E, int D, bool FULL, bool AHEAD>
+hipError_t chunks(const Args& a, hipStream_t stream) {
+    constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
+    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, FULL, AHEAD>);
+    if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
+    const uint32_t jobs = a.envs * a.heads * (AHEAD ? 2 * a.segments - 3 : a.segments);
+    forward_kernel<E, D, FULL, AHEAD><<<dim3(resident_blocks(f, a, jobs, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, GradArgs{}});
+    return hipGetLastError();
+}
 template <class E, int D, bool FULL>
 hipError_t forward(const Args& a, hipStream_t stream) {
-    constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
-    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, FULL>);
-    if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    forward_kernel<E, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, GradArgs{}});
-    return hipGetLastError();
+    if (a.segments > 1) {
+        if (hipError_t e = chunks<E, D, FULL, true>(a, stream)) return e;
+        if (hipError_t e = launch_join(a, a.seg_states, false, sizeof(E) == 2, stream)) return e;
+    }
+    return chunks<E, D, FULL, false>(a, stream);
 }
 // FULL: heads as wide as the kernel's tiles, without the branches for narrower ones.
 template <class E, int D>
@@ -349,6 +456,16 @@ hipError_t recurrent(const Args& a, hipStream_t stream) {
 
 hipError_t launch_recurrent(const Args& a, bool bf, hipStream_t stream) {
     return bf ? recurrent<bf16>(a, stream) : recurrent<float>(a, stream);
+}
+
+hipError_t launch_join(const Args& a, float* seg, bool transposed, bool bf, hipStream_t stream) {
+    if (a.segments < 3) return hipSuccess;
+    const dim3 grid(a.envs * a.heads * ((a.v_dim + 15) / 16)), wg(512);
+    if (bf && transposed) join_kernel<bf16, true><<<grid, wg, 0, stream>>>(a, seg);
+    else if (bf) join_kernel<bf16, false><<<grid, wg, 0, stream>>>(a, seg);
+    else if (transposed) join_kernel<float, true><<<grid, wg, 0, stream>>>(a, seg);
+    else join_kernel<float, false><<<grid, wg, 0, stream>>>(a, seg);
+    return hipGetLastError();
 }
 
 hipError_t launch_forward(const Args& a, bool bf, hipStream_t stream) {

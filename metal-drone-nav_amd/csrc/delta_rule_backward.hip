@@ -27,17 +27,17 @@ namespace {
 template <class E, int D> struct BackwardShared {
     static constexpr int STRIDE = D + Kind<E>::PAD;
     static constexpr int N = Kind<E>::MID;
-    // S and G pass through LDS, transposed, in fp32; both 128-wide operands
-    // and the fp32 rows do not fit beside each other, and take halves of V
+    // S and G pass through LDS, transposed, as operands; of 128 columns in fp32
+    // the rows and these do not fit beside each other, and take halves of V
     static constexpr int HALVES = sizeof(E) == 4 && D == 128 ? 2 : 1;
-    static constexpr int TS = D + 4;
+    static constexpr int TP = D / HALVES * STRIDE;
     static constexpr int PLANE = D * CP;
     static constexpr int W = D / 16;
     E k[C * STRIDE], q[C * STRIDE], d_o[C * STRIDE];  // ordered rows
     E v[C * STRIDE];
     // from here on the gradients' rows take the place of what is done with
     E u[N * PLANE], r[N * PLANE];                     // U and R transposed, [v][tick]
-    float through[D / HALVES * TS];                   // S, then G, transposed: [v][k]
+    E through[N * TP];                                // S, then G, transposed: [v][k]
     // inv and scores give their places to E = beta D dA and to scale D dP
     System<E> sys;
     Gates gates[2];  // of this chunk and the next
@@ -50,11 +50,15 @@ template <class E, int D> struct BackwardShared {
 // wavefront has 16 columns of V (its slices of S, G, U and R) and, for the
 // gradients of q and k, 16 columns of K; U, R, S and G change hands through
 // LDS.  F is the type of the rows of d_q and d_k.
-template <class E, class F, int D, bool FULL>
+//
+// AHEAD: what the segments of a cut state need before they run, the gradient
+// that each would pass to the one before it if it received none itself (the
+// last one receives the final state's).
+template <class E, class F, int D, bool FULL, bool AHEAD>
 __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
     typedef BackwardShared<E, D> Shared;
     constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16, SP = System<E>::PLANE, PL = Shared::PLANE;
-    constexpr int HALVES = Shared::HALVES, TS = Shared::TS, VH = D / HALVES;
+    constexpr int HALVES = Shared::HALVES, TP = Shared::TP, VH = D / HALVES;
     constexpr int FT = D + Kind<F>::PAD;  // row of d_q and d_k in LDS
     static_assert(sizeof(F) * 2 * C * FT + sizeof(E) * C * ST <= sizeof(Shared::u) + sizeof(Shared::r) + sizeof(Shared::through), "");
     extern __shared__ __align__(16) char lds[];
@@ -66,8 +70,12 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
     const int waves = FULL ? D / 16 : blockDim.x >> 6;
     const int kd = FULL ? D : int(call.a.k_dim), vd = FULL ? D : int(call.a.v_dim);
     const bool v_wave = FULL || 16 * wave < vd, k_wave = FULL || 16 * wave < kd;
-    const uint32_t ticks = call.a.ticks, chunks = (ticks + CHUNK - 1) / CHUNK;
-    const uint32_t heads = call.a.heads, shared = heads / call.a.qk_heads, states = call.a.envs * heads;
+    const uint32_t ticks = call.a.ticks;
+    const Plan plan(call.a, AHEAD ? call.a.segments - 1 : call.a.segments);
+    const auto which = [&](At& at, uint32_t j) {
+        at.part = 0;
+        at.seg = AHEAD ? j + 1 : j;
+    };
     const float scale = call.a.scale;
     const Spot on_k(kd), on_v(vd);
     const f32x4 zero{0, 0, 0, 0};
@@ -90,7 +98,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         }
         if (on_v.on) {
             const uint32_t x = at.c * C + on_v.row, t = x < ticks ? x : 0u;
-            pv = load_piece<E>(Track<const E>(&k->a.v, at.n, at.h).row(t), vd, on_v.col);
+            if (!AHEAD) pv = load_piece<E>(Track<const E>(&k->a.v, at.n, at.h).row(t), vd, on_v.col);
             po = load_piece<E>(Track<const E>(&k->d.d_o, at.n, at.h).row(t), vd, on_v.col);
         }
     };
@@ -101,7 +109,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             piece_to_ordered(s.q + on_k.row * ST, on_k.col, mask_piece<E>(pq, on_k.row < left));
         }
         if (on_v.on) {
-            piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
+            if (!AHEAD) piece_to_lds(s.v + on_v.row * ST + on_v.col, mask_piece<E>(pv, on_v.row < left));
             piece_to_ordered(s.d_o + on_v.row * ST, on_v.col, mask_piece<E>(po, on_v.row < left));
         }
     };
@@ -109,7 +117,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         const Lane l = Lane::fresh();
         KernelCall* k = fresh_call();
         if (at.c > 0) {
-            const f32x4* p = state_tiles(k->a.chunk_states, at.seq, chunks, at.c, kd, vd, wave);
+            const f32x4* p = state_tiles(k->a.chunk_states, at.state, plan.chunks, at.c, kd, vd, wave);
 #pragma unroll
             for (int i = 0; i < KT; i++) {
                 st[i] = zero;
@@ -117,7 +125,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             }
         } else {
             const float* p = k->a.state;
-            load_state(st, p ? p + uint64_t(at.seq) * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+            load_state(st, p ? p + uint64_t(at.state) * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
         }
     };
     // the last wavefront has no tile of A: it makes the next chunk's decays
@@ -127,30 +135,36 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         const uint32_t t = at.c * C + lane;
         gate = load_gates<E>(&fresh_call()->a, at.n, at.h, t, lane < C && t < ticks);
     };
-    At now{blockIdx.x, chunks - 1, 0, 0, 0};
-    now.split(heads, shared);
-    At next = now, later;
-    next.back(chunks, heads, shared);
+    At now, next, later;
+    now.job = blockIdx.x;
+    now.split(plan, which);
+    now.c = now.end - 1;
+    next = now;
+    next.back(plan, which);
     later = next;
-    later.back(chunks, heads, shared);
+    later.back(plan, which);
     fetch(now);
-    fetch_state(now);
+    if (!AHEAD) fetch_state(now);
     if (wave == waves - 1) {
         fetch_gates(now);
         put_gates(s.gates[0], gate);
-        if (next.seq < states) fetch_gates(next);
+        if (next.job < plan.total) fetch_gates(next);
     }
     put_rows(now);
     __syncthreads();
-    for (uint32_t turn = 0; now.seq < states; turn ^= 1) {
+    for (uint32_t turn = 0; now.job < plan.total; turn ^= 1) {
         const Lane l = Lane::fresh();
         const Gates& gates = s.gates[turn];
         const uint32_t left = ticks - now.c * C;  // ticks from the chunk's first
-        if (now.c == chunks - 1) {
-            const float* p = fresh_call()->d.d_state_out;
-            load_state(g, p ? p + uint64_t(now.seq) * kd * vd : nullptr, kd, vd, l, 16 * wave + l.col);
+        if (now.c == now.end - 1) {
+            KernelCall* k = fresh_call();
+            const float* p = k->d.d_state_out;
+            if (p) p += uint64_t(now.state) * kd * vd;
+            if (now.seg + 1 < plan.segments)
+                p = AHEAD ? nullptr : k->a.seg_grads + (uint64_t(now.state) * plan.segments + now.seg) * kd * vd;
+            load_state(g, p, kd, vd, l, 16 * wave + l.col);
         }
-        if (next.seq < states) fetch(next);
+        if (next.job < plan.total) fetch(next);
 
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0), kept by their wavefronts
         f32x4 dec = zero, kk = zero, pm = zero, am = zero;
@@ -177,9 +191,9 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             else
                 put_tile(l, s.sys.inv, CP, SP, 0, 16, am);
         }
-        if (wave == waves - 1 && next.seq < states) {
+        if (wave == waves - 1 && next.job < plan.total) {
             put_gates(s.gates[turn ^ 1], gate);
-            if (later.seq < states) fetch_gates(later);
+            if (later.job < plan.total) fetch_gates(later);
         }
         // X, and the part of dU through G
         f32x4 x[2], dr[2] = {zero, zero}, du[2] = {zero, zero};
@@ -188,8 +202,14 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
 #pragma unroll
             for (int y = 0; y < D; y += 32) {
                 if (y >= kd) continue;
-                const auto sf = frag_of<E>(st[y / 16], st[y / 16 + 1]);
                 const auto gf = frag_of<E>(g[y / 16], g[y / 16 + 1]);
+                if (AHEAD) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) mma(du[i], ordered_row(l, s.k, ST, 16 * i, y), gf);
+                    continue;
+                }
+                const auto sf = frag_of<E>(st[y / 16], st[y / 16 + 1]);
+                if (HALVES == 1 || 16 * wave < VH) put_frag(l, s.through, ST, TP, 16 * wave, y, sf);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const auto kf = ordered_row(l, s.k, ST, 16 * i, y);
@@ -201,48 +221,88 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             for (int i = 0; i < 2; i++) {
                 const int t = 16 * i + 4 * l.quad;
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[i][e] = float(s.v[(t + e) * ST + 16 * wave + l.col]);
+                for (int e = 0; e < 4; e++) x[i][e] = AHEAD ? 0.0f : float(s.v[(t + e) * ST + 16 * wave + l.col]);
+                du[i] *= four(gates.after + t);
+                if (AHEAD) continue;
                 x[i] -= four(gates.before + t) * ks[i];
                 dr[i] = four(gates.beta + t) * x[i];
-                du[i] *= four(gates.after + t);
             }
-            if (HALVES == 1 || 16 * wave < VH)
-#pragma unroll
-                for (int i = 0; i < KT; i++)
-                    if (16 * i < kd) put_tile(l, s.through, TS, 0, 16 * wave, 16 * i, st[i]);
         }
-        float dot = 0.0f;
+        if (!AHEAD) {
+            float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < KT; i++)
+            for (int i = 0; i < KT; i++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) dot = fmaf(st[i][r], g[i][r], dot);
-        dot = sum_rows32(sum_rows16(sum16(dot)));
-        if (lane == 0) s.dot[wave] = dot;
+                for (int r = 0; r < 4; r++) dot = fmaf(st[i][r], g[i][r], dot);
+            dot = sum_rows32(sum_rows16(sum16(dot)));
+            if (lane == 0) s.dot[wave] = dot;
+        }
         __syncthreads();
 
         // U and R
         f32x4 dv[2];
         if (v_wave) {
-            f32x4 u[2];
-            solve(l, s.sys, dr, u);
+            if (!AHEAD) {
+                f32x4 u[2];
+                solve(l, s.sys, dr, u);
 #pragma unroll
-            for (int i = 0; i < 2; i++) put_tile(l, s.u, CP, PL, 16 * wave, 16 * i, u[i]);
+                for (int i = 0; i < 2; i++) put_tile(l, s.u, CP, PL, 16 * wave, 16 * i, u[i]);
+            }
             const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
 #pragma unroll
             for (int i = 0; i < 2; i++) mma(du[i], row_frag<N>(l, s.sys.scores, CP, SP, 16 * i, 0), of);
             solve_transposed(l, s.sys, du, dr);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                put_tile(l, s.r, CP, PL, 16 * wave, 16 * i, dr[i]);
+                if (!AHEAD) put_tile(l, s.r, CP, PL, 16 * wave, 16 * i, dr[i]);
                 f32x4 sum = dr[i] * x[i];
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum[e] = sum16(sum[e]);
+                for (int e = 0; e < 4 && !AHEAD; e++) sum[e] = sum16(sum[e]);
                 dv[i] = four(gates.beta + 16 * i + 4 * l.quad) * dr[i];
                 dr[i] = dv[i] * four(gates.before + 16 * i + 4 * l.quad);  // from here on gamma beta R
-                if (l.col == 0) *reinterpret_cast<f32x4*>(&s.beta_v[wave][16 * i + 4 * l.quad]) = sum;
+                if (!AHEAD && l.col == 0) *reinterpret_cast<f32x4*>(&s.beta_v[wave][16 * i + 4 * l.quad]) = sum;
             }
         }
         __syncthreads();
+
+        // G before the chunk
+        const auto step_back = [&] {
+            if (!v_wave) return;
+            const float total = gates.before[C - 1];
+            const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
+            f32x4 lo, hi;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                lo[e] = first_term(of, e);
+                hi[e] = first_term(of, 4 + e);
+            }
+            lo *= scale * four(gates.before + 4 * l.quad);
+            hi *= scale * four(gates.before + 16 + 4 * l.quad);
+            const auto of2 = frag_of<E>(lo, hi);
+            const auto rf = frag_of<E>(-dr[0], -dr[1]);
+#pragma unroll
+            for (int i = 0; i < KT; i++) {
+                if (16 * i >= kd) continue;
+                g[i] *= total;
+                mma(g[i], ordered_col(l, s.q, ST, 16 * i), of2);
+                mma(g[i], ordered_col(l, s.k, ST, 16 * i), rf);
+            }
+        };
+        if constexpr (AHEAD) {
+            step_back();
+            // all have read k, q and d_o, and the matrices
+            __syncthreads();
+            if (next.job < plan.total) put_rows(next);
+            if (now.c == now.first) {
+                float* p = fresh_call()->a.seg_grads + (uint64_t(now.state) * plan.segments + now.seg - 1) * kd * vd;
+                store_state(p, g, kd, vd, l, 16 * wave + l.col);
+            }
+            __syncthreads();
+            now = next;
+            next = later;
+            later.back(plan, which);
+            continue;
+        }
 
         // dP and dA, by the wavefronts that hold P and A
         if (wave < 3) {
@@ -285,15 +345,15 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 __syncthreads();
                 if (16 * wave >= VH && v_wave)
 #pragma unroll
-                    for (int i = 0; i < KT; i++)
-                        if (16 * i < kd) put_tile(l, s.through, TS, 0, 16 * wave - VH, 16 * i, st[i]);
+                    for (int y = 0; y < D; y += 32)
+                        if (y < kd) put_frag(l, s.through, ST, TP, 16 * wave - VH, y, frag_of<E>(st[y / 16], st[y / 16 + 1]));
                 __syncthreads();
             }
             if (k_wave)
 #pragma unroll
                 for (int y = 0; y < VH; y += 32) {
                     if (half * VH + y >= vd) continue;
-                    const auto sf = frag_of<E>(col4(l, s.through, TS, y, 16 * wave), col4(l, s.through, TS, y + 16, 16 * wave));
+                    const auto sf = col_frag<N>(l, s.through, ST, TP, y, 16 * wave);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         mma(dq[i], ordered_row(l, s.d_o, ST, 16 * i, half * VH + y), sf);
@@ -301,21 +361,25 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                     }
                 }
         }
-        if (next.seq < states) fetch_state(next);  // S is done with
+        if (next.job < plan.total) fetch_state(next);  // S is done with
         // through G
 #pragma unroll
         for (int half = 0; half < HALVES; half++) {
             __syncthreads();
             if (v_wave && (HALVES == 1 || (16 * wave >= VH) == (half == 1)))
 #pragma unroll
-                for (int i = 0; i < KT; i++)
-                    if (16 * i < kd) put_tile(l, s.through, TS, 0, 16 * wave - half * VH, 16 * i, g[i]);
+                for (int y = 0; y < D; y += 32) {
+                    if (y >= kd) continue;
+                    // 64 wide, the operand is kept from above; 128 wide the registers do not reach
+                    if (FULL && D > 64 && sizeof(E) == 2) asm volatile("" : "+v"(g[y / 16]), "+v"(g[y / 16 + 1]));
+                    put_frag(l, s.through, ST, TP, 16 * wave - half * VH, y, frag_of<E>(g[y / 16], g[y / 16 + 1]));
+                }
             __syncthreads();
             if (k_wave)
 #pragma unroll
                 for (int y = 0; y < VH; y += 32) {
                     if (half * VH + y >= vd) continue;
-                    const auto gf = frag_of<E>(col4(l, s.through, TS, y, 16 * wave), col4(l, s.through, TS, y + 16, 16 * wave));
+                    const auto gf = col_frag<N>(l, s.through, ST, TP, y, 16 * wave);
 #pragma unroll
                     for (int i = 0; i < 2; i++) mma(dkg[i], col_frag<N>(l, s.u, CP, PL, half * VH + y, 16 * i), gf);
                 }
@@ -357,28 +421,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 mma(dk[i], ec, kf);
             }
         }
-        // G before the chunk
-        if (v_wave) {
-            const float total = gates.before[C - 1];
-            const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
-            f32x4 lo, hi;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                lo[e] = first_term(of, e);
-                hi[e] = first_term(of, 4 + e);
-            }
-            lo *= scale * four(gates.before + 4 * l.quad);
-            hi *= scale * four(gates.before + 16 + 4 * l.quad);
-            const auto of2 = frag_of<E>(lo, hi);
-            const auto rf = frag_of<E>(-dr[0], -dr[1]);
-#pragma unroll
-            for (int i = 0; i < KT; i++) {
-                if (16 * i >= kd) continue;
-                g[i] *= total;
-                mma(g[i], ordered_col(l, s.q, ST, 16 * i), of2);
-                mma(g[i], ordered_col(l, s.k, ST, 16 * i), rf);
-            }
-        }
+        step_back();
         __syncthreads();
         // the rows' gradients, through LDS to whole rows
 #pragma unroll
@@ -426,7 +469,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         // the next chunk's rows and S are waited for before this one's gradients
         // leave: loads and stores are counted in order, and the loads would
         // wait for the stores
-        if (next.seq < states) put_rows(next);
+        if (next.job < plan.total) put_rows(next);
 #pragma unroll
         for (int i = 0; i < KT; i++) asm volatile("" : "+v"(st[i]));
         asm volatile("" : "+v"(gate.g), "+v"(gate.beta), "+v"(gate.flag));
@@ -442,7 +485,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             store_piece<E>(Track<E>(&k->d.d_v, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
                            piece_from_lds(dv_rows + on_v.row * ST + on_v.col));
         if (now.c == 0)
-            if (float* p = k->d.d_state) store_state(p + uint64_t(now.seq) * kd * vd, g, kd, vd, l, 16 * wave + l.col);
+            if (float* p = k->d.d_state) store_state(p + uint64_t(now.state) * kd * vd, g, kd, vd, l, 16 * wave + l.col);
         // u, r and `through` take the next chunk's operands.  `through` is the
         // first, before the next barrier: all have to have read their gradients'
         // rows.  In narrow heads the columns past the width are operands too
@@ -451,7 +494,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         if (!FULL) clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
         now = next;
         next = later;
-        later.back(chunks, heads, shared);
+        later.back(plan, which);
     }
 }
 
@@ -466,14 +509,23 @@ __global__ void sum_heads_kernel(const float* in, E* out, uint64_t count, uint32
     }
 }
 
-template <class E, class F, int D, bool FULL>
-hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
+template <class E, class F, int D, bool FULL, bool AHEAD>
+hipError_t chunks(const Args& a, const GradArgs& d, hipStream_t stream) {
     constexpr uint32_t bytes = sizeof(BackwardShared<E, D>);
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
-    const void* f = reinterpret_cast<const void*>(&backward_kernel<E, F, D, FULL>);
+    const void* f = reinterpret_cast<const void*>(&backward_kernel<E, F, D, FULL, AHEAD>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
-    backward_kernel<E, F, D, FULL><<<dim3(resident_blocks(f, a, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, d});
+    const uint32_t jobs = a.envs * a.heads * (AHEAD ? a.segments - 1 : a.segments);
+    backward_kernel<E, F, D, FULL, AHEAD><<<dim3(resident_blocks(f, a, jobs, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, d});
     return hipGetLastError();
+}
+template <class E, class F, int D, bool FULL>
+hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
+    if (a.segments > 1) {
+        if (hipError_t e = chunks<E, E, D, FULL, true>(a, d, stream)) return e;
+        if (hipError_t e = launch_join(a, a.seg_grads, true, sizeof(E) == 2, stream)) return e;
+    }
+    return chunks<E, F, D, FULL, false>(a, d, stream);
 }
 template <class E, class F, int D>
 hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {

@@ -319,6 +319,21 @@ __device__ __forceinline__ void put_tile(Lane l, float* m, int stride, int, int 
     *reinterpret_cast<f32x4*>(m + l.col * stride + 4 * l.quad + c0 * stride + r0) = x;
 }
 
+// Two result tiles that are an operand already (32 places from r0).
+__device__ __forceinline__ void put_frag(Lane l, bf16* m, int stride, int plane, int c0, int r0, const Frag<bf16, 2>& f) {
+    bf16* p = m + l.col * stride + 4 * l.quad + c0 * stride + r0;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        *reinterpret_cast<bf16x4*>(p + i * plane) = __builtin_shufflevector(f.t[i], f.t[i], 0, 1, 2, 3);
+        *reinterpret_cast<bf16x4*>(p + i * plane + 16) = __builtin_shufflevector(f.t[i], f.t[i], 4, 5, 6, 7);
+    }
+}
+__device__ __forceinline__ void put_frag(Lane l, float* m, int stride, int, int c0, int r0, const Frag<float, 1>& f) {
+    float* p = m + l.col * stride + 4 * l.quad + c0 * stride + r0;
+    *reinterpret_cast<f32x4*>(p) = f.t[0];
+    *reinterpret_cast<f32x4*>(p + 16) = f.t[1];
+}
+
 }  // namespace delta
 
 #endif

@@ -157,6 +157,11 @@ SHAPES = [
     (65, 2, 2, 4, 40, 72),
     (130, 1, 1, 1, 127, 101),
     (300, 1, 1, 2, 16, 48),
+    # few states of many ticks: segments side by side
+    (517, 1, 1, 1, 64, 64),
+    (700, 2, 1, 2, 128, 128),
+    (1500, 1, 1, 3, 40, 100),
+    (2100, 3, 1, 1, 33, 7),
 ]
 
 
