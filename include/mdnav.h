@@ -438,8 +438,8 @@ typedef struct MdnDeltaRule {
     float* state_out;                 /* the same after the last tick, or NULL; may be `state` itself */
 } MdnDeltaRule;
 
-/* All ticks of a rollout.  `keep` (mdn_op_delta_rule_keep_bytes of it, or
- * NULL) receives what the backward pass reads besides the inputs. */
+/* All ticks of a rollout.  `keep` (or NULL) receives what the backward pass
+ * reads besides the inputs. */
 int mdn_op_delta_rule_forward(const MdnDeltaRule* rule, void* keep, uint64_t keep_bytes, void* workspace,
                               uint64_t workspace_bytes, void* stream);
 /* The gradients, from the same inputs, the forward call's `keep` (NULL if its
@@ -454,9 +454,12 @@ typedef struct MdnDeltaRuleGrad {
 } MdnDeltaRuleGrad;
 int mdn_op_delta_rule_backward(const MdnDeltaRule* rule, const MdnDeltaRuleGrad* grad, const void* keep,
                                uint64_t keep_bytes, void* workspace, uint64_t workspace_bytes, void* stream);
-/* Bytes of `keep`, and of the workspace of a forward (0) or backward (1) call. */
-int mdn_op_delta_rule_keep_bytes(const MdnDeltaRule* rule, uint64_t* bytes);
-int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backward, uint64_t* bytes);
+/* Bytes of `keep` and of the calls' workspaces, by the sizes in `rule` alone
+ * (one tick needs none). */
+typedef struct MdnDeltaRuleSizes {
+    uint64_t keep, forward_workspace, backward_workspace;
+} MdnDeltaRuleSizes;
+int mdn_op_delta_rule_sizes(const MdnDeltaRule* rule, MdnDeltaRuleSizes* sizes);
 
 /* The norms around a block, fused with its gate and residual scale: per row
  *     n = y / rms(y),  s = residual x + gate n w_post,  h = s / rms(s) w_pre

@@ -2198,7 +2198,7 @@ constexpr uint64_t kMostBlocks = 0x7fffffffull;  // of a grid
 
 delta::Rows device_rows(const MdnRows& r) { return delta::Rows{static_cast<char*>(r.data), r.tick, r.env, r.head}; }
 
-int delta_args(const char* name, const MdnDeltaRule* d, delta::Args* out) {
+int delta_args(const char* name, const MdnDeltaRule* d, delta::Args* out, bool rows = true) {
     const std::string who = std::string(name) + ": ";
     if (!d) return fail(MDN_E_ARG, who + "null");
     if (d->dtype > MDN_BF16) return fail(MDN_E_ARG, who + "dtype must be MDN_F32 or MDN_BF16");
@@ -2209,8 +2209,7 @@ int delta_args(const char* name, const MdnDeltaRule* d, delta::Args* out) {
         return fail(MDN_E_ARG, who + "qk_heads must divide heads");
     if (uint64_t(d->envs) * d->heads > kMostBlocks / 16) return fail(MDN_E_ARG, who + "too many states");
     if (d->ticks > 0x7fffff00u) return fail(MDN_E_ARG, who + "too many ticks");
-    const bool any = d->ticks && d->envs;
-    if (any && (!d->q.data || !d->k.data || !d->v.data || !d->g.data || !d->beta.data))
+    if (rows && d->ticks && d->envs && (!d->q.data || !d->k.data || !d->v.data || !d->g.data || !d->beta.data))
         return fail(MDN_E_ARG, who + "null rows");
     delta::Args a{};
     a.ticks = d->ticks; a.envs = d->envs; a.qk_heads = d->qk_heads; a.heads = d->heads; a.k_dim = d->k_dim; a.v_dim = d->v_dim;
@@ -2246,20 +2245,14 @@ uint64_t delta_partial_bytes(const delta::Args& a) {
 
 extern "C" {
 
-int mdn_op_delta_rule_keep_bytes(const MdnDeltaRule* rule, uint64_t* bytes) {
+int mdn_op_delta_rule_sizes(const MdnDeltaRule* rule, MdnDeltaRuleSizes* sizes) {
     delta::Args a;
-    if (int rc = delta_args("mdn_op_delta_rule_keep_bytes", rule, &a)) return rc;
-    if (!bytes) return fail(MDN_E_ARG, "mdn_op_delta_rule_keep_bytes: null");
-    *bytes = delta_keep_bytes(a);
-    return MDN_OK;
-}
-
-int mdn_op_delta_rule_workspace_bytes(const MdnDeltaRule* rule, uint32_t backward, uint64_t* bytes) {
-    delta::Args a;
-    if (int rc = delta_args("mdn_op_delta_rule_workspace_bytes", rule, &a)) return rc;
-    if (!bytes) return fail(MDN_E_ARG, "mdn_op_delta_rule_workspace_bytes: null");
-    // forward: the segments' states and, if nothing is kept, their M
-    *bytes = (backward ? delta_partial_bytes(a) : delta::seg_move_words(a) * sizeof(float)) + delta::seg_state_words(a) * sizeof(float);
+    if (int rc = delta_args("mdn_op_delta_rule_sizes", rule, &a, false)) return rc;
+    if (!sizes) return fail(MDN_E_ARG, "mdn_op_delta_rule_sizes: null");
+    const uint64_t segments = delta::seg_state_words(a) * sizeof(float);
+    sizes->keep = delta_keep_bytes(a);
+    sizes->forward_workspace = segments + delta::seg_move_words(a) * sizeof(float);  // (M where nothing is kept)
+    sizes->backward_workspace = delta_partial_bytes(a) + segments;
     return MDN_OK;
 }
 

@@ -30,7 +30,7 @@ EXPORTS = [
     "mdn_op_sample_loss_and_grad", "mdn_op_adam_update", "mdn_op_ppo_self_tests", "mdn_sim_validate_rollout",
     "mdn_checkpoint_read_params", "mdn_op_normalize_noalloc", "mdn_sim_get_bank", "mdn_sim_set_camera",
     "mdn_sim_get_camera", "mdn_ppo_grad_norm_summary", "mdn_lppo_grad_norm_summary", "mdn_op_delta_rule_forward", "mdn_op_delta_rule_backward",
-    "mdn_op_delta_rule_keep_bytes", "mdn_op_delta_rule_workspace_bytes",
+    "mdn_op_delta_rule_sizes",
     "mdn_op_block_norm_forward", "mdn_op_block_norm_backward", "mdn_op_block_norm_workspace_bytes",
 ]
 
@@ -135,8 +135,7 @@ def lib():
         _sig(L, "mdn_lppo_grad_norm_summary", I32, P, P)
         _sig(L, "mdn_op_delta_rule_forward", I32, P, P, U64, P, U64, P)
         _sig(L, "mdn_op_delta_rule_backward", I32, P, P, P, U64, P, U64, P)
-        _sig(L, "mdn_op_delta_rule_keep_bytes", I32, P, ctypes.POINTER(U64))
-        _sig(L, "mdn_op_delta_rule_workspace_bytes", I32, P, U32, ctypes.POINTER(U64))
+        _sig(L, "mdn_op_delta_rule_sizes", I32, P, P)
         _sig(L, "mdn_op_block_norm_forward", I32, P, P)
         _sig(L, "mdn_op_block_norm_backward", I32, P, P, P, U64, P)
         _sig(L, "mdn_op_block_norm_workspace_bytes", I32, P, ctypes.POINTER(U64))

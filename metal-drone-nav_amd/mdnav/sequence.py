@@ -43,6 +43,10 @@ class _DeltaRuleGrad(ctypes.Structure):
     _fields_ += [("d_state", P)]
 
 
+class _Sizes(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint64) for n in ("keep", "forward_workspace", "backward_workspace")]
+
+
 class _NormRows(ctypes.Structure):
     _fields_ = [("data", P), ("outer", ctypes.c_int64), ("inner", ctypes.c_int64)]
 
@@ -77,26 +81,41 @@ def _library():
     return L
 
 
-def _device(named):
+def _device(names, tensors):
     """The GPU that all tensors are on."""
     device = None
-    for name, t in named:
+    for name, t in zip(names, tensors):
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError("%s is no tensor" % name)
-        if not t.is_cuda:
-            raise ValueError("%s is not on a GPU" % name)
         if device is None:
             device = t.device
+            if device.type != "cuda":
+                raise ValueError("%s is not on a GPU" % name)
         elif t.device != device:
             raise ValueError("%s is on %s, other arguments on %s" % (name, t.device, device))
     return device
 
 
-def _rows(t):
-    """A [ticks][envs][heads][width] (or, gates, [ticks][envs][heads]) tensor."""
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+def _on(device, call, *args):
+    """call(*args) with `device` the current GPU."""
+    if torch.cuda.current_device() == device.index:
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _buffer(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def _wide(t):
@@ -105,107 +124,111 @@ def _wide(t):
 
 
 def _shape(name, t, shape):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+
+
+def _rows(t, one_tick=False):
+    """A [ticks][envs][heads][width] (or, gates, [ticks][envs][heads]) tensor; `one_tick`: without the ticks."""
+    strides = t.stride()
+    return _Rows(t.data_ptr(), 0, strides[0], strides[1]) if one_tick else _Rows(t.data_ptr(), *strides[:3])
 
 
 class _Call:
     """Checked arguments of one delta rule call: the C struct and what it points to."""
 
-    def __init__(self, q, k, v, g, beta, state, reset, scale):
-        self.device = _device([("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta), ("state", state),
-                               ("reset", reset)])
-        if q.dim() != 4 or v.dim() != 4:
-            raise ValueError("q, k and v are [ticks][envs][heads][width]")
-        t, n, hq, kd = q.shape
-        h, vd = v.shape[2:]
-        _shape("k", k, q.shape)
-        _shape("v", v, (t, n, h, vd))
-        _shape("g", g, (t, n, h))
-        _shape("beta", beta, (t, n, h))
+    NAMES = ("q", "k", "v", "g", "beta", "state", "reset")
+
+    def __init__(self, q, k, v, g, beta, state, reset, scale, one_tick=False):
+        self.device = _device(self.NAMES, (q, k, v, g, beta, state, reset))
+        lead = 1 if one_tick else 2
+        if q.dim() != lead + 2 or v.dim() != lead + 2:
+            raise ValueError("q, k and v are %s[envs][heads][width]" % ("" if one_tick else "[ticks]"))
+        sq, sv = q.shape, v.shape
+        hq, kd = sq[lead:]
+        h, vd = sv[lead:]
+        t, n = (1, sq[0]) if one_tick else sq[:2]
+        _shape("k", k, sq)
+        _shape("v", v, (*sq[:lead], h, vd))
+        _shape("g", g, sv[:-1])
+        _shape("beta", beta, sv[:-1])
         if hq < 1 or h < 1 or h % hq:
             raise ValueError("%d query heads do not divide %d value heads" % (hq, h))
         if not 1 <= kd <= 128 or not 1 <= vd <= 128:
             raise ValueError("head widths are 1..128, not %d and %d" % (kd, vd))
-        if q.dtype not in _DTYPES:
-            raise TypeError("q is %s: float32 or bfloat16 are taken" % q.dtype)
-        for name, x in (("k", k), ("v", v)):
-            if x.dtype != q.dtype:
-                raise TypeError("%s is %s, q is %s" % (name, x.dtype, q.dtype))
-        if g.dtype != beta.dtype or g.dtype not in (torch.float32, q.dtype):
+        dtype = q.dtype
+        if dtype not in _DTYPES:
+            raise TypeError("q is %s: float32 or bfloat16 are taken" % dtype)
+        if k.dtype != dtype or v.dtype != dtype:
+            raise TypeError("q is %s, k %s and v %s: one type is taken" % (dtype, k.dtype, v.dtype))
+        if g.dtype != beta.dtype or g.dtype not in (torch.float32, dtype):
             raise TypeError("g and beta are float32 or both of q's type, not %s and %s" % (g.dtype, beta.dtype))
         if reset is not None:
-            _shape("reset", reset, (t, n))
+            _shape("reset", reset, sq[:lead])
             if reset.dtype not in (torch.uint8, torch.bool):
                 raise TypeError("reset is %s: uint8 or bool are taken" % reset.dtype)
         if state is not None:
             _shape("state", state, (n, h, kd, vd))
             if state.dtype != torch.float32:
                 raise TypeError("state is %s: float32 is taken" % state.dtype)
-        self.q, self.k, self.v = _wide(q), _wide(k), _wide(v)
-        self.g, self.beta, self.state, self.reset = g, beta, state, reset
-        self.scale = kd ** -0.5 if scale is None else float(scale)
-        c = _DeltaRule(t, n, hq, h, kd, vd, _DTYPES[q.dtype], _DTYPES[g.dtype], self.scale, _rows(self.q),
-                       _rows(self.k), _rows(self.v), _rows(g), _rows(beta))
+        self.q, self.k, self.v, self.g, self.beta = _wide(q), _wide(k), _wide(v), g, beta
+        self.state, self.reset = state, reset
+        self.c = c = _DeltaRule(t, n, hq, h, kd, vd, _DTYPES[dtype], _DTYPES[g.dtype], kd ** -0.5 if scale is None else scale,
+                                _rows(self.q, one_tick), _rows(self.k, one_tick), _rows(self.v, one_tick),
+                                _rows(g, one_tick), _rows(beta, one_tick))
         if reset is not None:
-            c.reset, c.reset_tick, c.reset_env = reset.data_ptr(), reset.stride(0), reset.stride(1)
+            c.reset = reset.data_ptr()
+            if one_tick:
+                c.reset_env = reset.stride(0)
+            else:
+                c.reset_tick, c.reset_env = reset.stride()
         if state is not None:
             c.state = state.data_ptr()
-        self.c = c
 
-    def stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+    def output(self):
+        return torch.empty(self.v.shape, dtype=self.v.dtype, device=self.device)
 
-    def bytes_of(self, function, *more):
-        size = ctypes.c_uint64()
-        check(function(ctypes.byref(self.c), *more, ctypes.byref(size)))
-        return size.value
+    def states(self):
+        c = self.c
+        return torch.empty(c.envs, c.heads, c.k_dim, c.v_dim, device=self.device)
 
-    def buffer(self, size):
-        return torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+    def forward(self, o, state_out, keep):
+        """One call over all ticks; `keep`: whether a backward pass follows.  What that reads, and its workspace."""
+        L = _library()
+        c = self.c
+        c.o, c.state_out = _rows(o), _address(state_out)
+        sizes = _Sizes()
+        check(L.mdn_op_delta_rule_sizes(ctypes.byref(c), ctypes.byref(sizes)))
+        kept = _buffer(sizes.keep, self.device) if keep else None
+        work = _buffer(sizes.forward_workspace, self.device)
+        check(L.mdn_op_delta_rule_forward(ctypes.byref(c), _address(kept), sizes.keep if keep else 0, _address(work),
+                                          sizes.forward_workspace, _stream(self.device)))
+        return kept, sizes
 
+    def step(self, o, state):
+        """One tick, which needs no buffers."""
+        c = self.c
+        c.o, c.state_out = _rows(o, True), state.data_ptr()
+        check(_library().mdn_op_delta_rule_forward(ctypes.byref(c), None, 0, None, 0, _stream(self.device)))
 
-def _address(t):
-    return None if t is None else t.data_ptr()
-
-
-def _forward(call, o, state_out, keep):
-    """One forward call; `keep`: whether a backward pass follows."""
-    L = _library()
-    call.c.o = _rows(o)
-    call.c.state_out = _address(state_out)
-    with torch.cuda.device(call.device):
-        kept = call.buffer(call.bytes_of(L.mdn_op_delta_rule_keep_bytes)) if keep else None
-        size = call.bytes_of(L.mdn_op_delta_rule_workspace_bytes, 0)
-        work = call.buffer(size)
-        check(L.mdn_op_delta_rule_forward(ctypes.byref(call.c), _address(kept), 0 if kept is None else kept.numel(),
-                                          _address(work), size, call.stream()))
-    return kept
-
-
-def _backward(call, kept, d_o, d_state_out, want_state):
-    """(d_q, d_k, d_v, d_g, d_beta, d_state or None)"""
-    L = _library()
-    c = call.c
-    with torch.cuda.device(call.device):
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (call.q, call.k, call.v, call.g, call.beta)]
-        d_state = torch.empty(c.envs, c.heads, c.k_dim, c.v_dim, device=call.device) if want_state else None
-        size = call.bytes_of(L.mdn_op_delta_rule_workspace_bytes, 1)
-        work = call.buffer(size)
+    def backward(self, kept, sizes, d_o, d_state_out, want_state):
+        """(d_q, d_k, d_v, d_g, d_beta, d_state or None)"""
+        grads = [torch.empty(x.shape, dtype=x.dtype, device=self.device) for x in (self.q, self.k, self.v, self.g, self.beta)]
+        d_state = self.states() if want_state else None
+        work = _buffer(sizes.backward_workspace, self.device)
         d = _DeltaRuleGrad(_rows(d_o), _address(d_state_out), *[_rows(x) for x in grads], _address(d_state))
-        check(L.mdn_op_delta_rule_backward(ctypes.byref(c), ctypes.byref(d), _address(kept),
-                                           0 if kept is None else kept.numel(), _address(work), size, call.stream()))
-    return (*grads, d_state)
+        check(_library().mdn_op_delta_rule_backward(ctypes.byref(self.c), ctypes.byref(d), _address(kept), sizes.keep,
+                                                    _address(work), sizes.backward_workspace, _stream(self.device)))
+        return (*grads, d_state)
 
 
 class _DeltaRuleFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, reset, scale, final_state):
         call = _Call(q, k, v, g, beta, state, reset, scale)
-        o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        last = _final_state(call) if final_state else None
-        kept = _forward(call, o, last, True)
-        ctx.scale, ctx.has_state = scale, state is not None
+        o, last = call.output(), call.states() if final_state else None
+        kept, ctx.sizes = _on(call.device, call.forward, o, last, True)
+        ctx.scale = scale
         ctx.save_for_backward(q, k, v, g, beta, state, reset, kept)
         ctx.set_materialize_grads(False)
         return o, last
@@ -213,22 +236,17 @@ class _DeltaRuleFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_last):
-        q, k, v, g, beta, state, reset, kept = ctx.saved_tensors
         if d_o is None and d_last is None:
             return (None,) * 9
-        call = _Call(q, k, v, g, beta, state, reset, ctx.scale)
+        q, k, v, g, beta, state, reset, kept = ctx.saved_tensors
         d_o = torch.zeros_like(v) if d_o is None else _wide(d_o)
-        want_state = ctx.has_state and ctx.needs_input_grad[5]
+        d_last = None if d_last is None else d_last.contiguous()
+        want_state = state is not None and ctx.needs_input_grad[5]
         if q.shape[0] == 0:  # nothing happens to the state
             d_state = None if not want_state else torch.zeros_like(state) if d_last is None else d_last
             return (*[torch.zeros_like(x) for x in (q, k, v, g, beta)], d_state, None, None, None)
-        grads = _backward(call, kept, d_o, None if d_last is None else d_last.contiguous(), want_state)
-        return (*grads, None, None, None)
-
-
-def _final_state(call):
-    c = call.c
-    return torch.empty(c.envs, c.heads, c.k_dim, c.v_dim, device=call.device)
+        call = _Call(q, k, v, g, beta, state, reset, ctx.scale)
+        return (*_on(call.device, call.backward, kept, ctx.sizes, d_o, d_last, want_state), None, None, None)
 
 
 def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state=False):
@@ -250,9 +268,8 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state)):
         return _DeltaRuleFunction.apply(q, k, v, g, beta, state, reset, scale, final_state)
     call = _Call(q, k, v, g, beta, state, reset, scale)
-    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    last = _final_state(call) if final_state else None
-    _forward(call, o, last, False)
+    o, last = call.output(), call.states() if final_state else None
+    _on(call.device, call.forward, o, last, False)
     return o, last
 
 
@@ -265,9 +282,9 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None):
     """
     if not isinstance(state, torch.Tensor) or not state.is_contiguous():
         raise ValueError("state is a contiguous tensor: it is advanced in place")
-    call = _Call(q[None], k[None], v[None], g[None], beta[None], state, None if reset is None else reset[None], scale)
-    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    _forward(call, o[None], state, False)
+    call = _Call(q, k, v, g, beta, state, reset, scale, one_tick=True)
+    o = call.output()
+    _on(call.device, call.step, o, state)
     return o
 
 
@@ -275,35 +292,21 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None):
 GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_ELEMENT = 0, 1, 2, 3
 
 
-def _norm_rows(t, width):
-    """A tensor whose last axis is a row, as two strides: (tensor, rows, count of the inner axis)."""
-    t = t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
-    lead, strides = t.shape[:-1], t.stride()[:-1]
-    # join neighbouring axes that are one; at most two may remain
-    axes = []
-    for size, stride in zip(lead, strides):
-        if size == 1:
-            continue
-        if axes and axes[-1][1] == size * stride:
-            axes[-1] = (axes[-1][0] * size, stride)
-        else:
-            axes.append((size, stride))
-    return t, axes
-
-
 class _NormCall:
     """Checked arguments of one norm block call."""
 
+    NAMES = ("x", "y", "w_post", "w_pre", "gate", "residual_scale")
+
     def __init__(self, x, y, w_post, w_pre, gate, residual_scale, eps):
-        self.device = _device([("x", x), ("y", y), ("w_post", w_post), ("w_pre", w_pre), ("gate", gate),
-                               ("residual_scale", residual_scale)])
-        if x.dim() < 1:
+        self.device = _device(self.NAMES, (x, y, w_post, w_pre, gate, residual_scale))
+        shape = x.shape
+        if len(shape) < 1:
             raise ValueError("x is [..., width]")
-        _shape("y", y, x.shape)
-        width = x.shape[-1]
+        _shape("y", y, shape)
+        width = shape[-1]
         if not 1 <= width <= 8192:
             raise ValueError("the width is 1..8192, not %d" % width)
-        if x.dtype not in _DTYPES or y.dtype not in _DTYPES or (x.dtype, y.dtype) == (torch.bfloat16, torch.float32):
+        if x.dtype not in _DTYPES or y.dtype not in _DTYPES or (x.dtype == torch.bfloat16 and y.dtype == torch.float32):
             raise TypeError("x and y are float32, both bfloat16, or float32 and bfloat16, not %s and %s" % (x.dtype, y.dtype))
         for name, w in (("w_post", w_post), ("w_pre", w_pre), ("residual_scale", residual_scale)):
             if w is None and name == "residual_scale":
@@ -313,102 +316,100 @@ class _NormCall:
                 raise TypeError("%s is %s: float32 is taken" % (name, w.dtype))
         self.kind = GATE_NONE
         if gate is not None:
-            if gate.dtype not in (torch.float32, y.dtype):
+            if gate.dtype != torch.float32 and gate.dtype != y.dtype:
                 raise TypeError("gate is %s: float32 or y's type are taken" % gate.dtype)
-            if tuple(gate.shape) == (width,) and (x.dim() > 1 or width > 1):
+            if gate.shape == (width,) and (len(shape) > 1 or width > 1):
                 self.kind = GATE_CHANNEL
-            elif tuple(gate.shape) == tuple(x.shape[:-1]) + (1,):
+                gate = gate.contiguous()
+            elif gate.shape == (*shape[:-1], 1):
                 self.kind = GATE_ROW
-            elif tuple(gate.shape) == tuple(x.shape):
+            elif gate.shape == shape:
                 self.kind = GATE_ELEMENT
                 if gate.dtype != y.dtype:
                     raise TypeError("a gate per element is of y's type, %s, not %s" % (y.dtype, gate.dtype))
             else:
                 raise ValueError("gate has shape %s, expected %s, %s or %s" % (
-                    tuple(gate.shape), (width,), tuple(x.shape[:-1]) + (1,), tuple(x.shape)))
+                    tuple(gate.shape), (width,), (*shape[:-1], 1), tuple(shape)))
         self.x, self.y, self.gate = x, y, gate
         self.w_post, self.w_pre = w_post.contiguous(), w_pre.contiguous()
         self.residual = None if residual_scale is None else residual_scale.contiguous()
-        self.shape, self.width, self.rows, self.eps = x.shape, width, x.numel() // width, float(eps)
-        self.inner = x.shape[-2] if x.dim() > 1 and self.rows else 1
+        self.shape, self.width, self.rows = shape, width, x.numel() // width
+        self.inner = shape[-2] if len(shape) > 1 and self.rows else 1
+        self.c = c = _BlockNorm(self.rows, self.inner, width, _DTYPES[x.dtype], _DTYPES[y.dtype], self.kind,
+                                0 if gate is None else _DTYPES[gate.dtype], eps)
+        self.kept = []  # copies that the struct points to
+        c.x, c.y = self.layout(x), self.layout(y)
+        if self.kind == GATE_CHANNEL:
+            c.gate.data = gate.data_ptr()
+        elif self.kind != GATE_NONE:
+            c.gate = self.layout(gate)
+        c.w_post, c.w_pre, c.residual = self.w_post.data_ptr(), self.w_pre.data_ptr(), _address(self.residual)
 
     def layout(self, t):
-        """The rows of `t`, [..., width or 1]; a layout of more than two strides is copied."""
-        t, axes = _norm_rows(t, self.width)
-        if not axes:
-            return t, _NormRows(t.data_ptr(), 0, 0)
-        if len(axes) == 1:
-            return t, _NormRows(t.data_ptr(), axes[0][1] * self.inner, axes[0][1])
-        if len(axes) == 2 and axes[1][0] == self.inner:
-            return t, _NormRows(t.data_ptr(), axes[0][1], axes[1][1])
-        t = t.contiguous()
-        return t, _NormRows(t.data_ptr(), t.shape[-1] * self.inner, t.shape[-1])
+        """The rows of `t`, [..., width or 1], as two strides; another layout is copied."""
+        if not t.is_contiguous():
+            axes = [] if t.shape[-1] == 1 or t.stride(-1) == 1 else None
+            if axes is not None:
+                # join neighbouring axes that are one
+                for size, stride in zip(t.shape[:-1], t.stride()[:-1]):
+                    if size == 1:
+                        continue
+                    if axes and axes[-1][1] == size * stride:
+                        axes[-1] = (axes[-1][0] * size, stride)
+                    else:
+                        axes.append((size, stride))
+                if len(axes) <= 1:
+                    stride = axes[0][1] if axes else 0
+                    return _NormRows(t.data_ptr(), stride * self.inner, stride)
+                if len(axes) == 2 and axes[1][0] == self.inner:
+                    return _NormRows(t.data_ptr(), axes[0][1], axes[1][1])
+            t = t.contiguous()
+            self.kept.append(t)
+        return _NormRows(t.data_ptr(), t.shape[-1] * self.inner, t.shape[-1])
 
-    def struct(self, s, h, stats):
-        """The C struct, and the tensors it points to."""
-        kept = [s, h, stats]
-        c = _BlockNorm(self.rows, self.inner, self.width, _DTYPES[self.x.dtype], _DTYPES[self.y.dtype], self.kind,
-                       0 if self.gate is None else _DTYPES[self.gate.dtype], self.eps)
-        for name in ("x", "y"):
-            t, rows = self.layout(getattr(self, name))
-            kept.append(t)
-            setattr(c, name, rows)
-        if self.kind == GATE_CHANNEL:
-            t = self.gate.contiguous()
-            kept.append(t)
-            c.gate = _NormRows(t.data_ptr(), 0, 0)
-        elif self.kind != GATE_NONE:
-            t, c.gate = self.layout(self.gate)
-            kept.append(t)
-        if s is not None:
-            c.s, c.h = self.layout(s)[1], self.layout(h)[1]
-        c.w_post, c.w_pre = self.w_post.data_ptr(), self.w_pre.data_ptr()
-        c.residual, c.stats = _address(self.residual), _address(stats)
-        return c, kept
+    def like(self, t):
+        return torch.empty(t.shape, dtype=t.dtype, device=self.device)
 
     def forward(self, keep):
         L = _library()
-        s = torch.empty(self.shape, dtype=self.x.dtype, device=self.device)
-        h = torch.empty(self.shape, dtype=self.y.dtype, device=self.device)
+        s, h = self.like(self.x), self.like(self.y)
         stats = torch.empty(self.rows, 2, device=self.device) if keep else None
-        with torch.cuda.device(self.device):
-            c, kept = self.struct(s, h, stats)
-            check(L.mdn_op_block_norm_forward(ctypes.byref(c), torch.cuda.current_stream().cuda_stream))
+        c = self.c
+        c.s, c.h, c.stats = self.layout(s), self.layout(h), _address(stats)
+        check(L.mdn_op_block_norm_forward(ctypes.byref(c), _stream(self.device)))
         return s, h, stats
 
     def backward(self, stats, d_s, d_h):
         L = _library()
-        with torch.cuda.device(self.device):
-            c, kept = self.struct(None, None, stats)
-            d = _BlockNormGrad()
-            for name, t in (("d_s", d_s), ("d_h", d_h)):
-                if t is not None:
-                    t, rows = self.layout(t)
-                    kept.append(t)
-                    setattr(d, name, rows)
-            d_x = torch.empty(self.shape, dtype=self.x.dtype, device=self.device)
-            d_y = torch.empty(self.shape, dtype=self.y.dtype, device=self.device)
-            d.d_x, d.d_y = self.layout(d_x)[1], self.layout(d_y)[1]
-            d_gate = None
-            if self.kind != GATE_NONE:
-                d_gate = torch.empty(self.gate.shape, dtype=self.gate.dtype, device=self.device)
-                d.d_gate = _NormRows(d_gate.data_ptr(), 0, 0) if self.kind == GATE_CHANNEL else self.layout(d_gate)[1]
-            sums = torch.empty(2 if self.residual is None else 3, self.width, device=self.device)
-            d.d_w_post, d.d_w_pre = sums[0].data_ptr(), sums[1].data_ptr()
-            if self.residual is not None:
-                d.d_residual = sums[2].data_ptr()
-            size = ctypes.c_uint64()
-            check(L.mdn_op_block_norm_workspace_bytes(ctypes.byref(c), ctypes.byref(size)))
-            work = torch.empty(size.value, dtype=torch.uint8, device=self.device) if size.value else None
-            check(L.mdn_op_block_norm_backward(ctypes.byref(c), ctypes.byref(d), _address(work), size.value,
-                                               torch.cuda.current_stream().cuda_stream))
-        return d_x, d_y, sums[0], sums[1], d_gate, None if self.residual is None else sums[2]
+        c, d = self.c, _BlockNormGrad()
+        c.stats = _address(stats)
+        if d_s is not None:
+            d.d_s = self.layout(d_s)
+        if d_h is not None:
+            d.d_h = self.layout(d_h)
+        d_x, d_y, d_gate = self.like(self.x), self.like(self.y), None
+        d.d_x, d.d_y = self.layout(d_x), self.layout(d_y)
+        if self.kind != GATE_NONE:
+            d_gate = self.like(self.gate)
+            d.d_gate = self.layout(d_gate) if self.kind != GATE_CHANNEL else _NormRows(d_gate.data_ptr(), 0, 0)
+        d_post, d_pre, d_scale = torch.empty(3, self.width, device=self.device).unbind()
+        d.d_w_post, d.d_w_pre = d_post.data_ptr(), d_pre.data_ptr()
+        if self.residual is None:
+            d_scale = None
+        else:
+            d.d_residual = d_scale.data_ptr()
+        size = ctypes.c_uint64()
+        check(L.mdn_op_block_norm_workspace_bytes(ctypes.byref(c), ctypes.byref(size)))
+        work = _buffer(size.value, self.device)
+        check(L.mdn_op_block_norm_backward(ctypes.byref(c), ctypes.byref(d), _address(work), size.value, _stream(self.device)))
+        return d_x, d_y, d_post, d_pre, d_gate, d_scale
 
 
 class _BlockNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, w_post, w_pre, gate, residual_scale, eps):
-        s, h, stats = _NormCall(x, y, w_post, w_pre, gate, residual_scale, eps).forward(True)
+        call = _NormCall(x, y, w_post, w_pre, gate, residual_scale, eps)
+        s, h, stats = _on(call.device, call.forward, True)
         ctx.eps = eps
         ctx.save_for_backward(x, y, w_post, w_pre, gate, residual_scale, stats)
         ctx.set_materialize_grads(False)
@@ -417,10 +418,11 @@ class _BlockNormFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_s, d_h):
-        x, y, w_post, w_pre, gate, residual_scale, stats = ctx.saved_tensors
         if d_s is None and d_h is None:
             return (None,) * 7
-        return (*_NormCall(x, y, w_post, w_pre, gate, residual_scale, ctx.eps).backward(stats, d_s, d_h), None)
+        x, y, w_post, w_pre, gate, residual_scale, stats = ctx.saved_tensors
+        call = _NormCall(x, y, w_post, w_pre, gate, residual_scale, ctx.eps)
+        return (*_on(call.device, call.backward, stats, d_s, d_h), None)
 
 
 def block_norm(x, y, w_post, w_pre, gate=None, residual_scale=None, eps=1e-6):
@@ -437,4 +439,5 @@ def block_norm(x, y, w_post, w_pre, gate=None, residual_scale=None, eps=1e-6):
     args = (x, y, w_post, w_pre, gate, residual_scale)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
         return _BlockNormFunction.apply(*args, eps)
-    return _NormCall(*args, eps).forward(False)[:2]
+    call = _NormCall(*args, eps)
+    return _on(call.device, call.forward, False)[:2]
