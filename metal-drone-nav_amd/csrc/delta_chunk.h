@@ -352,36 +352,36 @@ __device__ __forceinline__ f32x4 invert_block(Lane l, f32x4 a) {
 // The chunk's small matrices in LDS.  All are stored transposed, [j][i]:
 // read across rows they are the operand with rows i, along a row the one with
 // rows j.
-template <class E> struct System {
-    static constexpr int N = Kind<E>::MID;
+template <class E, int TERMS = Kind<E>::MID> struct System {
+    static constexpr int N = TERMS;
     static constexpr int PLANE = C * CP;
     E inv[N * PLANE];          // [j][i]: the diagonal blocks' inverses; A_10 at [j][16 + i]
     E scores[N * PLANE];       // scale D (q_i k_j)
 };
 
 // U = (1 + A)^-1 R for 16 columns of R, as two result tiles.
-template <class E>
-__device__ __forceinline__ void solve(Lane l, const System<E>& s, const f32x4 r[2], f32x4 u[2]) {
-    constexpr int N = Kind<E>::MID, P = System<E>::PLANE;
+template <class E, int N>
+__device__ __forceinline__ void solve(Lane l, const System<E, N>& s, const f32x4 r[2], f32x4 u[2]) {
+    constexpr int P = System<E, N>::PLANE;
     const f32x4 zero{0, 0, 0, 0};
     u[0] = zero;
-    mma(u[0], col_half<N>(l, s.inv, CP, P, 0, 0), half_of<E>(r[0]));
+    mma(u[0], col_half<N>(l, s.inv, CP, P, 0, 0), half_of<E, N>(r[0]));
     f32x4 below = zero;
-    mma(below, col_half<N>(l, s.inv, CP, P, 0, 16), half_of<E>(u[0]));
+    mma(below, col_half<N>(l, s.inv, CP, P, 0, 16), half_of<E, N>(u[0]));
     u[1] = zero;
-    mma(u[1], col_half<N>(l, s.inv, CP, P, 16, 16), half_of<E>(r[1] - below));
+    mma(u[1], col_half<N>(l, s.inv, CP, P, 16, 16), half_of<E, N>(r[1] - below));
 }
 // R = (1 + A)^-T U.
-template <class E>
-__device__ __forceinline__ void solve_transposed(Lane l, const System<E>& s, const f32x4 u[2], f32x4 r[2]) {
-    constexpr int N = Kind<E>::MID, P = System<E>::PLANE;
+template <class E, int N>
+__device__ __forceinline__ void solve_transposed(Lane l, const System<E, N>& s, const f32x4 u[2], f32x4 r[2]) {
+    constexpr int P = System<E, N>::PLANE;
     const f32x4 zero{0, 0, 0, 0};
     r[1] = zero;
-    mma(r[1], row_half<N>(l, s.inv, CP, P, 16, 16), half_of<E>(u[1]));
+    mma(r[1], row_half<N>(l, s.inv, CP, P, 16, 16), half_of<E, N>(u[1]));
     f32x4 above = zero;
-    mma(above, row_half<N>(l, s.inv, CP, P, 0, 16), half_of<E>(r[1]));
+    mma(above, row_half<N>(l, s.inv, CP, P, 0, 16), half_of<E, N>(r[1]));
     r[0] = zero;
-    mma(r[0], row_half<N>(l, s.inv, CP, P, 0, 0), half_of<E>(u[0] - above));
+    mma(r[0], row_half<N>(l, s.inv, CP, P, 0, 0), half_of<E, N>(u[0] - above));
 }
 
 }  // namespace delta

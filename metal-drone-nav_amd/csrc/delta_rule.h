@@ -97,9 +97,8 @@ hipError_t launch_backward(const Args& a, const GradArgs& d, bool bf16, hipStrea
 // out[row][qk head][width] = sum of the `shared` heads of in[row][head][width]
 hipError_t launch_sum_heads(const float* in, void* out, uint64_t rows, uint32_t qk_heads, uint32_t shared, uint32_t width,
                             bool bf16, hipStream_t stream);
-// seg[s + 1] += M_s seg[s] for s = 1.. in turn, or, of gradients, seg[s - 1] +=
-// M_s^T seg[s] downwards.
-hipError_t launch_join(const Args& a, float* seg, bool transposed, bool bf16, hipStream_t stream);
+// seg_grads[s - 1] += M_s^T seg_grads[s], from the last segment but one downwards.
+hipError_t launch_join_grads(const Args& a, bool bf16, hipStream_t stream);
 hipError_t launch_recurrent(const Args& a, bool bf16, hipStream_t stream);
 hipError_t launch_forward(const Args& a, bool bf16, hipStream_t stream);
 

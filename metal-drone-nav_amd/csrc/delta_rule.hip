@@ -125,10 +125,10 @@ __global__ void __launch_bounds__(256, 3) recurrent_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- chunks
-template <class E, int D> struct ForwardShared {
+template <class E, int D, int N> struct ForwardShared {
     static constexpr int STRIDE = D + Kind<E>::PAD;
     E k[C * STRIDE], q[C * STRIDE], v[C * STRIDE], o[C * STRIDE];
-    System<E> sys;
+    System<E, N> sys;
     Gates gates[2];  // of this chunk and the next
 };
 
@@ -140,10 +140,10 @@ template <class E, int D> struct ForwardShared {
 // AHEAD: what the segments of a cut state need before they run.  Part 0 of a
 // segment starts from zeros (the first from the state) and leaves B, part 1
 // starts from the identity with no v and leaves M; neither has outputs.
-template <class E, int D, bool FULL, bool AHEAD>
+template <class E, int N, int D, bool FULL, bool AHEAD>
 __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
-    typedef ForwardShared<E, D> Shared;
-    constexpr int ST = Shared::STRIDE, N = Kind<E>::MID, KT = D / 16;
+    typedef ForwardShared<E, D, N> Shared;
+    constexpr int ST = Shared::STRIDE, KT = D / 16;
     extern __shared__ __align__(16) char lds[];
     Shared& s = *reinterpret_cast<Shared*>(lds);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -160,9 +160,9 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
     const Spot on_k(kd), on_v(vd);  // the thread's piece of k and q, and of v and o
     if (!FULL) clear_lds(lds, sizeof(Shared));
     // the matrices' upper right block stays 0
-    if (wave < 2 * N) {
+    for (int p = wave; p < 2 * N; p += waves) {
         const Lane l = Lane::mine();
-        E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * System<E>::PLANE;
+        E* m = (p & 1 ? s.sys.scores : s.sys.inv) + (p >> 1) * System<E, N>::PLANE;
 #pragma unroll
         for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
@@ -258,11 +258,11 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             for (int r = 0; r < 4; r++)
                 if (i0 + 4 * l.quad + r <= j0 + l.col) am[r] = 0.0f;
             const f32x4 pm = scale * d * qk;
-            if (!AHEAD) put_tile(l, s.sys.scores, CP, System<E>::PLANE, j0, i0, pm);
+            if (!AHEAD) put_tile<N>(l, s.sys.scores, CP, System<E, N>::PLANE, j0, i0, pm);
             if (wave < 2)
-                put_tile(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
+                put_tile<N>(l, s.sys.inv, CP, System<E, N>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
             else
-                put_tile(l, s.sys.inv, CP, System<E>::PLANE, 0, 16, am);
+                put_tile<N>(l, s.sys.inv, CP, System<E, N>::PLANE, 0, 16, am);
         }
         if (wave == waves - 1 && next.job < plan.total) {
             put_gates(s.gates[turn ^ 1], gate);
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
 #pragma unroll
             for (int x = 0; x < D; x += 32) {
                 if (x >= int(kd)) continue;
-                const auto st = frag_of<E>(state[x / 16], state[x / 16 + 1]);
+                const auto st = frag_of<E, N>(state[x / 16], state[x / 16 + 1]);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     mma(ks[i], ordered_row(l, s.k, ST, 16 * i, x), st);
@@ -296,9 +296,9 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             solve(l, s.sys, r, u);
             // o = scale gamma (q S) + scores u
             if (!AHEAD) {
-                const auto uf = frag_of<E>(u[0], u[1]);
+                const auto uf = frag_of<E, N>(u[0], u[1]);
 #pragma unroll
-                for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E>::PLANE, 0, 16 * i), uf);
+                for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E, N>::PLANE, 0, 16 * i), uf);
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             }
             // S <- gamma_C S + K^T u
             const float total = gates.before[C - 1];
-            const auto uf = frag_of<E>(u[0], u[1]);
+            const auto uf = frag_of<E, N>(u[0], u[1]);
 #pragma unroll
             for (int i = 0; i < KT; i++) {
                 if (16 * i >= int(kd)) continue;
@@ -344,9 +344,9 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
 // A workgroup per 16 columns of a state, a wavefront for each 16 rows: it has
 // its rows of M ahead of the product, and the columns' last values come from
 // LDS.
-template <class E, bool TRANSPOSED>
+template <class E, int N, bool TRANSPOSED>
 __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
-    constexpr int D = int(MAX_DIM), N = Kind<E>::MID, ST = D + Kind<E>::PAD, PL = 16 * ST;
+    constexpr int D = int(MAX_DIM), ST = D + Kind<E>::PAD, PL = 16 * ST;
     __shared__ __align__(16) E last[2][N * PL];  // [column][row]
     const Lane l = Lane::mine();
     const int kd = a.k_dim, vd = a.v_dim, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -389,13 +389,13 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
     };
     uint32_t s = TRANSPOSED ? a.segments - 2 : 1;
     fetch(s);
-    put_tile(l, last[0], ST, PL, 0, 16 * wave, load_tile(s));
+    put_tile<N>(l, last[0], ST, PL, 0, 16 * wave, load_tile(s));
     f32x4 next = load_tile(TRANSPOSED ? s - 1 : s + 1);
     __syncthreads();
     for (uint32_t left = a.segments - 2, turn = 0; left > 0; left--, turn ^= 1) {
         Frag<E, N> mf[D / 32];
 #pragma unroll
-        for (int k = 0; k < D / 32; k++) mf[k] = frag_of<E>(m[2 * k], m[2 * k + 1]);
+        for (int k = 0; k < D / 32; k++) mf[k] = frag_of<E, N>(m[2 * k], m[2 * k + 1]);
         s = TRANSPOSED ? s - 1 : s + 1;
         f32x4 y = next;
         if (left > 1) {
@@ -407,36 +407,42 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
 #pragma unroll
         for (int r = 0; r < 4; r++)
             if (16 * wave + 4 * l.quad + r < kd && int(col) < vd) *tile_at(s, r) = y[r];
-        put_tile(l, last[turn ^ 1], ST, PL, 0, 16 * wave, y);
+        put_tile<N>(l, last[turn ^ 1], ST, PL, 0, 16 * wave, y);
         __syncthreads();
     }
 }
 
-template <class E, int D, bool FULL, bool AHEAD>
+template <class E, int N, int D, bool FULL, bool AHEAD>
 hipError_t chunks(const Args& a, hipStream_t stream) {
-    constexpr uint32_t bytes = sizeof(ForwardShared<E, D>);
-    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, D, FULL, AHEAD>);
+    constexpr uint32_t bytes = sizeof(ForwardShared<E, D, N>);
+    const void* f = reinterpret_cast<const void*>(&forward_kernel<E, N, D, FULL, AHEAD>);
     if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes))) return e;
     const uint32_t jobs = a.envs * a.heads * (AHEAD ? 2 * a.segments - 3 : a.segments);
-    forward_kernel<E, D, FULL, AHEAD><<<dim3(resident_blocks(f, a, jobs, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, GradArgs{}});
+    forward_kernel<E, N, D, FULL, AHEAD><<<dim3(resident_blocks(f, a, jobs, bytes)), dim3(64 * waves_of(a)), bytes, stream>>>(Call{a, GradArgs{}});
     return hipGetLastError();
 }
-template <class E, int D, bool FULL>
+template <class E, int N, bool TRANSPOSED>
+hipError_t join(const Args& a, float* seg, hipStream_t stream) {
+    if (a.segments < 3) return hipSuccess;
+    join_kernel<E, N, TRANSPOSED><<<dim3(a.envs * a.heads * ((a.v_dim + 15) / 16)), dim3(512), 0, stream>>>(a, seg);
+    return hipGetLastError();
+}
+template <class E, int N, int D, bool FULL>
 hipError_t forward(const Args& a, hipStream_t stream) {
     if (a.segments > 1) {
-        if (hipError_t e = chunks<E, D, FULL, true>(a, stream)) return e;
-        if (hipError_t e = launch_join(a, a.seg_states, false, sizeof(E) == 2, stream)) return e;
+        if (hipError_t e = chunks<E, N, D, FULL, true>(a, stream)) return e;
+        if (hipError_t e = join<E, N, false>(a, a.seg_states, stream)) return e;
     }
-    return chunks<E, D, FULL, false>(a, stream);
+    return chunks<E, N, D, FULL, false>(a, stream);
 }
 // FULL: heads as wide as the kernel's tiles, without the branches for narrower ones.
-template <class E, int D>
+template <class E, int N, int D>
 hipError_t forward(const Args& a, hipStream_t stream) {
-    return a.k_dim == D && a.v_dim == D ? forward<E, D, true>(a, stream) : forward<E, D, false>(a, stream);
+    return a.k_dim == D && a.v_dim == D ? forward<E, N, D, true>(a, stream) : forward<E, N, D, false>(a, stream);
 }
-template <class E>
+template <class E, int N>
 hipError_t forward(const Args& a, hipStream_t stream) {
-    return a.k_dim <= 64 && a.v_dim <= 64 ? forward<E, 64>(a, stream) : forward<E, 128>(a, stream);
+    return a.k_dim <= 64 && a.v_dim <= 64 ? forward<E, N, 64>(a, stream) : forward<E, N, 128>(a, stream);
 }
 
 template <class E>
@@ -458,18 +464,13 @@ hipError_t launch_recurrent(const Args& a, bool bf, hipStream_t stream) {
     return bf ? recurrent<bf16>(a, stream) : recurrent<float>(a, stream);
 }
 
-hipError_t launch_join(const Args& a, float* seg, bool transposed, bool bf, hipStream_t stream) {
-    if (a.segments < 3) return hipSuccess;
-    const dim3 grid(a.envs * a.heads * ((a.v_dim + 15) / 16)), wg(512);
-    if (bf && transposed) join_kernel<bf16, true><<<grid, wg, 0, stream>>>(a, seg);
-    else if (bf) join_kernel<bf16, false><<<grid, wg, 0, stream>>>(a, seg);
-    else if (transposed) join_kernel<float, true><<<grid, wg, 0, stream>>>(a, seg);
-    else join_kernel<float, false><<<grid, wg, 0, stream>>>(a, seg);
-    return hipGetLastError();
+hipError_t launch_join_grads(const Args& a, bool bf, hipStream_t stream) {
+    return bf ? join<bf16, Kind<bf16>::MID, true>(a, a.seg_grads, stream) : join<float, 1, true>(a, a.seg_grads, stream);
 }
 
 hipError_t launch_forward(const Args& a, bool bf, hipStream_t stream) {
-    return bf ? forward<bf16>(a, stream) : forward<float>(a, stream);
+    if (!bf) return forward<float, 1>(a, stream);
+    return a.state_out ? forward<bf16, 3>(a, stream) : forward<bf16, 2>(a, stream);
 }
 
 }  // namespace delta

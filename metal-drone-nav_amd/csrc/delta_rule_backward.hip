@@ -81,9 +81,9 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
     const f32x4 zero{0, 0, 0, 0};
     if (!FULL) clear_lds(lds, sizeof(Shared));
     // the matrices' upper right blocks stay 0
-    if (wave < 2 * N) {
+    for (int p = wave; p < 2 * N; p += waves) {
         const Lane l = Lane::mine();
-        E* m = (wave & 1 ? s.sys.scores : s.sys.inv) + (wave >> 1) * SP;
+        E* m = (p & 1 ? s.sys.scores : s.sys.inv) + (p >> 1) * SP;
 #pragma unroll
         for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
@@ -185,11 +185,11 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 if (i0 + 4 * l.quad + r <= j0 + l.col) kk[r] = 0.0f;
             am = four(gates.beta + i0 + 4 * l.quad) * kk;
             pm = scale * dec * qk;
-            put_tile(l, s.sys.scores, CP, SP, j0, i0, pm);
+            put_tile<N>(l, s.sys.scores, CP, SP, j0, i0, pm);
             if (wave < 2)
-                put_tile(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
+                put_tile<N>(l, s.sys.inv, CP, System<E>::PLANE, 16 * wave, 16 * wave, invert_block(l, am));
             else
-                put_tile(l, s.sys.inv, CP, SP, 0, 16, am);
+                put_tile<N>(l, s.sys.inv, CP, SP, 0, 16, am);
         }
         if (wave == waves - 1 && next.job < plan.total) {
             put_gates(s.gates[turn ^ 1], gate);
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 f32x4 u[2];
                 solve(l, s.sys, dr, u);
 #pragma unroll
-                for (int i = 0; i < 2; i++) put_tile(l, s.u, CP, PL, 16 * wave, 16 * i, u[i]);
+                for (int i = 0; i < 2; i++) put_tile<N>(l, s.u, CP, PL, 16 * wave, 16 * i, u[i]);
             }
             const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
 #pragma unroll
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             solve_transposed(l, s.sys, du, dr);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                if (!AHEAD) put_tile(l, s.r, CP, PL, 16 * wave, 16 * i, dr[i]);
+                if (!AHEAD) put_tile<N>(l, s.r, CP, PL, 16 * wave, 16 * i, dr[i]);
                 f32x4 sum = dr[i] * x[i];
 #pragma unroll
                 for (int e = 0; e < 4 && !AHEAD; e++) sum[e] = sum16(sum[e]);
@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             m_col += __shfl_xor(m_col, 16);
             m_col += __shfl_xor(m_col, 32);
             if (l.quad == 0) s.m_col[wave][l.col] = m_col;
-            put_tile(l, s.sys.scores, CP, SP, j0, i0, dp);  // scale D dP, and E
-            put_tile(l, s.sys.inv, CP, SP, j0, i0, da);
+            put_tile<N>(l, s.sys.scores, CP, SP, j0, i0, dp);  // scale D dP, and E
+            put_tile<N>(l, s.sys.inv, CP, SP, j0, i0, da);
         }
         // through S
         f32x4 dq[2] = {zero, zero}, dk[2] = {zero, zero}, dkg[2] = {zero, zero};
@@ -523,7 +523,7 @@ template <class E, class F, int D, bool FULL>
 hipError_t backward(const Args& a, const GradArgs& d, hipStream_t stream) {
     if (a.segments > 1) {
         if (hipError_t e = chunks<E, E, D, FULL, true>(a, d, stream)) return e;
-        if (hipError_t e = launch_join(a, a.seg_grads, true, sizeof(E) == 2, stream)) return e;
+        if (hipError_t e = launch_join_grads(a, sizeof(E) == 2, stream)) return e;
     }
     return chunks<E, F, D, FULL, false>(a, d, stream);
 }

@@ -9,13 +9,14 @@
 //
 // Rounding.  The rows a caller passes in bfloat16 are operands as they are.
 // What the chunk computes (states, solved rows, scores) is held in fp32 and
-// enters a bfloat16 product as the sum of two bfloat16 values, 16 to 17
-// significand bits; products of two such operands leave out the lowest of
-// the four terms.  One rounding to bfloat16 (8 bits) per operand was not
-// taken: it moves the fp32 results (final state, gradients) by 2e-3, the
-// two-term form by a few 1e-6, and the kernels are bound by memory and
-// latency, not by the matrix cores.  fp32 rows use the fp32 matrix cores with
-// no rounding.
+// enters a bfloat16 product as the sum of N bfloat16 values: two (16 to 17
+// significand bits) where results are bfloat16 or gradients, three (all 24)
+// where the fp32 state is a result; products of two such operands leave out
+// the terms below the last kept one.  One rounding to bfloat16 (8 bits) per
+// operand was not taken: it moves the fp32 results by 2e-3 of their norm, two
+// terms by 4e-6, three by 1e-7, and the kernels are bound by memory, latency
+// and vector instructions, not by the matrix cores.  fp32 rows use the fp32
+// matrix cores with no rounding.
 #ifndef MDNAV_DELTA_TILES_H
 #define MDNAV_DELTA_TILES_H
 
@@ -104,7 +105,7 @@ template <int Q> __device__ __forceinline__ float from_quad(float x) {
 
 template <class E> struct Kind;
 template <> struct Kind<bf16> {
-    static constexpr int MID = 2;  // terms of a computed operand
+    static constexpr int MID = 2;  // terms of a computed operand, if it is not three
     static constexpr int PAD = 8;  // elements past a row: 16 bytes
 };
 template <> struct Kind<float> {
@@ -152,37 +153,45 @@ __device__ __forceinline__ void mma(f32x4& acc, const Half<float, 1>& a, const H
 }
 
 // ---- fp32 values to operands
-__device__ __forceinline__ void split4(f32x4 x, bf16x4& hi, bf16x4& lo) {
-    hi = __builtin_convertvector(x, bf16x4);
-    lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x4), bf16x4);
+template <int N> __device__ __forceinline__ void split4(f32x4 x, bf16x4 (&t)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        t[i] = __builtin_convertvector(x, bf16x4);
+        if (i + 1 < N) x -= __builtin_convertvector(t[i], f32x4);
+    }
 }
-template <class E> __device__ __forceinline__ Frag<E, Kind<E>::MID> frag_of(f32x4 x, f32x4 y);
-template <> __device__ __forceinline__ Frag<bf16, 2> frag_of<bf16>(f32x4 x, f32x4 y) {
-    bf16x4 xh, xl, yh, yl;
-    split4(x, xh, xl);
-    split4(y, yh, yl);
-    Frag<bf16, 2> f;
-    f.t[0] = __builtin_shufflevector(xh, yh, 0, 1, 2, 3, 4, 5, 6, 7);
-    f.t[1] = __builtin_shufflevector(xl, yl, 0, 1, 2, 3, 4, 5, 6, 7);
-    return f;
-}
-template <> __device__ __forceinline__ Frag<float, 1> frag_of<float>(f32x4 x, f32x4 y) {
-    Frag<float, 1> f;
-    f.t[0] = x;
-    f.t[1] = y;
-    return f;
-}
-template <class E> __device__ __forceinline__ Half<E, Kind<E>::MID> half_of(f32x4 x);
-template <> __device__ __forceinline__ Half<bf16, 2> half_of<bf16>(f32x4 x) {
-    Half<bf16, 2> f;
-    split4(x, f.t[0], f.t[1]);
-    return f;
-}
-template <> __device__ __forceinline__ Half<float, 1> half_of<float>(f32x4 x) {
-    Half<float, 1> f;
-    f.t[0] = x;
-    return f;
-}
+template <class E, int N> struct Make;
+template <int N> struct Make<bf16, N> {
+    __device__ __forceinline__ static Frag<bf16, N> frag(f32x4 x, f32x4 y) {
+        bf16x4 xt[N], yt[N];
+        split4(x, xt);
+        split4(y, yt);
+        Frag<bf16, N> f;
+#pragma unroll
+        for (int i = 0; i < N; i++) f.t[i] = __builtin_shufflevector(xt[i], yt[i], 0, 1, 2, 3, 4, 5, 6, 7);
+        return f;
+    }
+    __device__ __forceinline__ static Half<bf16, N> half(f32x4 x) {
+        Half<bf16, N> f;
+        split4(x, f.t);
+        return f;
+    }
+};
+template <> struct Make<float, 1> {
+    __device__ __forceinline__ static Frag<float, 1> frag(f32x4 x, f32x4 y) {
+        Frag<float, 1> f;
+        f.t[0] = x;
+        f.t[1] = y;
+        return f;
+    }
+    __device__ __forceinline__ static Half<float, 1> half(f32x4 x) {
+        Half<float, 1> f;
+        f.t[0] = x;
+        return f;
+    }
+};
+template <class E, int N = Kind<E>::MID> __device__ __forceinline__ Frag<E, N> frag_of(f32x4 x, f32x4 y) { return Make<E, N>::frag(x, y); }
+template <class E, int N = Kind<E>::MID> __device__ __forceinline__ Half<E, N> half_of(f32x4 x) { return Make<E, N>::half(x); }
 
 // Element e of an operand of caller's rows.
 __device__ __forceinline__ float first_term(const Frag<bf16, 1>& f, int e) { return float(f.t[0][e]); }
@@ -308,17 +317,18 @@ __device__ __forceinline__ Half<float, 1> col_half(Lane l, const float* m, int s
 
 // A result tile to LDS, transposed: column c of the tile becomes row c0 + c of
 // the matrix, whose places r0 + 4 (l / 16) .. + 3 the lane writes at once.
+template <int N>
 __device__ __forceinline__ void put_tile(Lane l, bf16* m, int stride, int plane, int c0, int r0, f32x4 x) {
-    bf16x4 hi, lo;
-    split4(x, hi, lo);
+    bf16x4 t[N];
+    split4(x, t);
     bf16* p = m + l.col * stride + 4 * l.quad + c0 * stride + r0;
-    *reinterpret_cast<bf16x4*>(p) = hi;
-    *reinterpret_cast<bf16x4*>(p + plane) = lo;
+#pragma unroll
+    for (int i = 0; i < N; i++) *reinterpret_cast<bf16x4*>(p + i * plane) = t[i];
 }
+template <int N>
 __device__ __forceinline__ void put_tile(Lane l, float* m, int stride, int, int c0, int r0, f32x4 x) {
     *reinterpret_cast<f32x4*>(m + l.col * stride + 4 * l.quad + c0 * stride + r0) = x;
 }
-
 // Two result tiles that are an operand already (32 places from r0).
 __device__ __forceinline__ void put_frag(Lane l, bf16* m, int stride, int plane, int c0, int r0, const Frag<bf16, 2>& f) {
     bf16* p = m + l.col * stride + 4 * l.quad + c0 * stride + r0;
