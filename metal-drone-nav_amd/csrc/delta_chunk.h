@@ -237,6 +237,7 @@ struct __align__(16) Gates {
     float beta[C];
     float before[C];   // gamma_i, 0 after a flag
     float after[C];    // gamma_C / gamma_i, 0 before the last flag
+    float decay[C];    // exp(g_i)
     int episode[C];    // flags up to and with tick i
 };
 // Four neighbouring values.
@@ -283,6 +284,7 @@ __device__ __forceinline__ void put_gates(Gates& s, const GateRegs& r) {
     if (l < C) {
         s.sum[i] = sum;
         s.beta[i] = r.beta;
+        s.decay[i] = __expf(r.g);
         s.episode[i] = episode;
         s.before[i] = episode == 0 ? __expf(float(sum)) : 0.0f;
         s.after[i] = episode == last ? __expf(float(total - sum)) : 0.0f;
@@ -382,6 +384,51 @@ __device__ __forceinline__ void solve_transposed(Lane l, const System<E, N>& s, 
     mma(above, row_half<N>(l, s.inv, CP, P, 0, 16), half_of<E, N>(r[1]));
     r[0] = zero;
     mma(r[0], row_half<N>(l, s.inv, CP, P, 0, 0), half_of<E, N>(u[0] - above));
+}
+
+// ---- chunks with infinities or NaN.  A matrix product spreads them: 0 times
+// NaN is NaN, so what a tick may not see (a later tick, an episode before a
+// flag) would reach it.  A chunk where such a value turns up in the products'
+// operands is taken tick by tick instead, by the definition.
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+// Whether all are finite and of ordinary size (their sum is).
+__device__ __forceinline__ bool finite(f32x4 x) { return finite((x[0] + x[1]) + (x[2] + x[3])); }
+
+// Four neighbouring places of an ordered row, as fp32: rows 16 i + 4 quad .. + 3 of a state's column.
+template <class E> __device__ __forceinline__ f32x4 ordered4(Lane l, const E* row, int i) {
+    const E* p = row + (i >> 1) * 32 + 8 * l.quad + (i & 1) * 4;
+    return f32x4{float(p[0]), float(p[1]), float(p[2]), float(p[3])};
+}
+// The decayed state of a tick, in place.
+template <int KT> __device__ __forceinline__ void decay_state(f32x4 (&s)[KT], const Gates& gates, int t) {
+    const bool flag = gate_is_flag(gates, t);
+    const float decay = gates.decay[t];
+#pragma unroll
+    for (int i = 0; i < KT; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[i][r] = flag ? 0.0f : s[i][r] * decay;
+}
+// x^T S for the lane's column.
+template <class E, int KT> __device__ __forceinline__ float column_dot(Lane l, const f32x4 (&s)[KT], const E* row) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KT; i++) {
+        const f32x4 k = ordered4(l, row, i);
+#pragma unroll
+        for (int r = 0; r < 4; r++) sum = fmaf(k[r], s[i][r], sum);
+        asm volatile("" : "+v"(sum)::"memory");  // a row at a time: this is not to take registers from the products
+    }
+    return sum_rows32(sum_rows16(sum));
+}
+// S <- S + k u^T.
+template <class E, int KT> __device__ __forceinline__ void add_outer(Lane l, f32x4 (&s)[KT], const E* row, float u) {
+#pragma unroll
+    for (int i = 0; i < KT; i++) {
+        const f32x4 k = ordered4(l, row, i);
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[i][r] = fmaf(k[r], u, s[i][r]);
+        asm volatile("" : "+v"(s[i])::"memory");
+    }
 }
 
 }  // namespace delta

@@ -130,6 +130,7 @@ template <class E, int D, int N> struct ForwardShared {
     E k[C * STRIDE], q[C * STRIDE], v[C * STRIDE], o[C * STRIDE];
     System<E, N> sys;
     Gates gates[2];  // of this chunk and the next
+    int odd[2];      // whether a chunk has infinities or NaN
 };
 
 // One workgroup per state, a wavefront for each 16 columns of V (at least
@@ -166,7 +167,9 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
 #pragma unroll
         for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
+    if (tid < 2) s.odd[tid] = 0;
     f32x4 state[KT];
+    bool flagged = false;  // AHEAD: an episode of the segment has ended, M is 0 whatever comes after
     Piece<E> pk, pq, pv;
     const auto fetch = [&](const At& at) {
         KernelCall* k = fresh_call();
@@ -242,6 +245,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             }
         }
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0)
+        bool odd = false;
         if (wave < 3) {
             const int i0 = wave ? 16 : 0, j0 = wave == 1 ? 16 : 0;
             f32x4 kk{0, 0, 0, 0}, qk{0, 0, 0, 0};
@@ -252,7 +256,9 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
                 mma(kk, ordered_row(l, s.k, ST, i0, x), kj);
                 if (!AHEAD) mma(qk, ordered_row(l, s.q, ST, i0, x), kj);
             }
+            if (!FULL) settle(kk, qk);
             const f32x4 d = decay_tile(l, gates, i0, j0);
+            odd = !finite(kk) | !finite(d);
             f32x4 am = four(gates.beta + i0 + 4 * l.quad) * d * kk;
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -283,6 +289,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
+                if (!FULL) settle(ks[i], qs[i]);
                 const int t = 16 * i + 4 * l.quad;
                 const f32x4 g = four(gates.before + t);
 #pragma unroll
@@ -290,9 +297,25 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
                 r[i] = four(gates.beta + t) * (r[i] - g * ks[i]);
                 qs[i] *= scale * g;
             }
+            odd |= !finite(r[0] + r[1]);
         }
+        if (__any(odd)) s.odd[turn] = 1;
         __syncthreads();
-        if (16 * wave < int(cols)) {
+        if (tid == 0) s.odd[turn ^ 1] = 0;
+        if (__builtin_amdgcn_readfirstlane(s.odd[turn])) {
+            const uint32_t ticks_here = left < uint32_t(C) ? left : uint32_t(C);
+#pragma unroll 1
+            for (uint32_t t = 0; t < ticks_here && 16 * wave < int(cols); t++) {
+                const E* k = s.k + t * ST;
+                decay_state(state, gates, t);
+                const float v = float(s.v[t * ST + 16 * wave + l.col]);
+                add_outer(l, state, k, gates.beta[t] * (v - column_dot(l, state, k)));
+                if (!AHEAD) {
+                    const float o = scale * column_dot(l, state, s.q + t * ST);
+                    if (l.quad == 0) s.o[t * ST + 16 * wave + l.col] = E(o);
+                }
+            }
+        } else if (16 * wave < int(cols)) {
             solve(l, s.sys, r, u);
             // o = scale gamma (q S) + scores u
             if (!AHEAD) {
@@ -316,6 +339,8 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
                 state[i] *= total;
                 mma(state[i], ordered_col(l, s.k, ST, 16 * i), uf);
             }
+#pragma unroll
+            for (int i = 0; i < KT && !FULL; i++) settle(state[i]);
         }
         __syncthreads();
         // the next chunk's rows go to LDS before this one's leave: loads and
@@ -324,7 +349,11 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         if (!AHEAD && on_v.on && on_v.row < left)
             store_piece<E>(Track<E>(&fresh_call()->a.o, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
                            piece_from_lds(s.o + on_v.row * ST + on_v.col));
+        if (AHEAD) flagged = (now.c > now.first && flagged) | (__builtin_amdgcn_readfirstlane(gates.episode[C - 1]) != 0);
         if (now.c + 1 == now.end) {
+            if (AHEAD && now.part && flagged)
+#pragma unroll
+                for (int i = 0; i < KT; i++) state[i] = f32x4{0, 0, 0, 0};
             KernelCall* k = fresh_call();
             float* p = now.seg + 1 == plan.segments ? k->a.state_out : nullptr;
             if (p) p += uint64_t(now.state) * kd * vd;
@@ -394,6 +423,11 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
     __syncthreads();
     for (uint32_t left = a.segments - 2, turn = 0; left > 0; left--, turn ^= 1) {
         Frag<E, N> mf[D / 32];
+        bool moved = false;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) moved |= m[k][e] != 0.0f;
 #pragma unroll
         for (int k = 0; k < D / 32; k++) mf[k] = frag_of<E, N>(m[2 * k], m[2 * k + 1]);
         s = TRANSPOSED ? s - 1 : s + 1;
@@ -402,8 +436,10 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
             fetch(s);
             next = load_tile(TRANSPOSED ? s - 1 : s + 1);
         }
+        // (a segment with an episode's first tick has M = 0, whatever came before it)
+        if (__any(moved))
 #pragma unroll
-        for (int k = 0; k < D / 32; k++) mma(y, mf[k], row_frag<N>(l, last[turn], ST, PL, 0, 32 * k));
+            for (int k = 0; k < D / 32; k++) mma(y, mf[k], row_frag<N>(l, last[turn], ST, PL, 0, 32 * k));
 #pragma unroll
         for (int r = 0; r < 4; r++)
             if (16 * wave + 4 * l.quad + r < kd && int(col) < vd) *tile_at(s, r) = y[r];

@@ -41,10 +41,22 @@ template <class E, int D> struct BackwardShared {
     // inv and scores give their places to E = beta D dA and to scale D dP
     System<E> sys;
     Gates gates[2];  // of this chunk and the next
+    int odd[2];      // whether a chunk has infinities or NaN
+    float odd_sums[2][W];
     __align__(16) float beta_v[W][C], a[W][C], b[W][C], dot[W];
     double m_row[3][16], m_col[3][16];
     __align__(16) float beta_a[3][16];
 };
+
+template <class E> __device__ __forceinline__ void put_gate(KernelCall* k, const At& now, uint32_t tick, float dg, float db) {
+    if (k->a.gate_f32 || sizeof(E) == 4) {
+        *Track<float>(&k->d.d_g, now.n, now.h).row(tick) = dg;
+        *Track<float>(&k->d.d_beta, now.n, now.h).row(tick) = db;
+    } else {
+        *Track<bf16>(&k->d.d_g, now.n, now.h).row(tick) = bf16(dg);
+        *Track<bf16>(&k->d.d_beta, now.n, now.h).row(tick) = bf16(db);
+    }
+}
 
 // One workgroup per state, a wavefront for each 16 columns (at least four).  A
 // wavefront has 16 columns of V (its slices of S, G, U and R) and, for the
@@ -87,6 +99,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
 #pragma unroll
         for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
+    if (tid < 2) s.odd[tid] = 0;
     f32x4 g[KT], st[KT];  // G and S, K x 16, in result layout
     Piece<E> pk, pq, pv, po;
     const auto fetch = [&](const At& at) {
@@ -135,6 +148,15 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         const uint32_t t = at.c * C + lane;
         gate = load_gates<E>(&fresh_call()->a, at.n, at.h, t, lane < C && t < ticks);
     };
+    // G before a segment: for the one before it, or the state's gradient
+    const auto leave = [&](const At& at, const f32x4(&x)[KT]) {
+        KernelCall* k = fresh_call();
+        float* p = at.seg == 0 ? k->d.d_state : nullptr;
+        if (p) p += uint64_t(at.state) * kd * vd;
+        if (AHEAD) p = k->a.seg_grads + (uint64_t(at.state) * plan.segments + at.seg - 1) * kd * vd;
+        const Lane l = Lane::fresh();
+        if (p) store_state(p, x, kd, vd, l, 16 * wave + l.col);
+    };
     At now, next, later;
     now.job = blockIdx.x;
     now.split(plan, which);
@@ -169,6 +191,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0), kept by their wavefronts
         f32x4 dec = zero, kk = zero, pm = zero, am = zero;
         const int i0 = wave ? 16 : 0, j0 = wave == 1 ? 16 : 0;
+        bool odd = false;
         if (wave < 3) {
             f32x4 qk = zero;
 #pragma unroll
@@ -178,7 +201,9 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 mma(kk, ordered_row(l, s.k, ST, i0, y), kj);
                 mma(qk, ordered_row(l, s.q, ST, i0, y), kj);
             }
+            if (!FULL) settle(kk, qk);
             dec = decay_tile(l, gates, i0, j0);
+            odd = !finite(kk + qk) | !finite(dec) | !finite(four(gates.beta + i0 + 4 * l.quad));
             kk *= dec;
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -222,12 +247,21 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 const int t = 16 * i + 4 * l.quad;
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[i][e] = AHEAD ? 0.0f : float(s.v[(t + e) * ST + 16 * wave + l.col]);
+                if (!FULL) settle(ks[i], du[i]);
                 du[i] *= four(gates.after + t);
                 if (AHEAD) continue;
                 x[i] -= four(gates.before + t) * ks[i];
                 dr[i] = four(gates.beta + t) * x[i];
             }
         }
+        if (v_wave) {
+            const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum += first_term(of, e);
+            odd |= !finite(du[0] + du[1]) | !finite(x[0] + x[1]) | !finite(sum);
+        }
+        if (__any(odd)) s.odd[turn] = 1;
         if (!AHEAD) {
             float dot = 0.0f;
 #pragma unroll
@@ -238,6 +272,105 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             if (lane == 0) s.dot[wave] = dot;
         }
         __syncthreads();
+
+        if (tid == 0) s.odd[turn ^ 1] = 0;
+        if (__builtin_amdgcn_readfirstlane(s.odd[turn])) {
+            // by the definition, from the chunk's last tick to its first
+            KernelCall* call_now = fresh_call();
+            float* const parts = reinterpret_cast<float*>(s.u);  // [wavefront][d_q, d_k][K]
+#pragma unroll 1
+            for (int t = int(left < uint32_t(C) ? left : uint32_t(C)) - 1; t >= 0; t--) {
+                const E *k = s.k + t * ST, *q = s.q + t * ST;
+                const float beta = gates.beta[t], decay = gates.decay[t];
+                const bool flag = gate_is_flag(gates, t);
+                const uint32_t at = now.c * C + t;
+                if (v_wave) {
+                    const float o = float(s.d_o[t * ST + place(16 * wave) + 8 * (l.col >> 2) + (l.col & 3)]);
+                    float error = 0.0f;
+                    if (!AHEAD) {
+                        fetch_state(now);  // S before the chunk, which becomes S before the tick's update
+#pragma unroll 1
+                        for (int j = 0; j < t; j++) {
+                            const E* kj = s.k + j * ST;
+                            decay_state(st, gates, j);
+                            add_outer(l, st, kj,
+                                      gates.beta[j] * (float(s.v[j * ST + 16 * wave + l.col]) - column_dot(l, st, kj)));
+                        }
+                        decay_state(st, gates, t);
+                        error = float(s.v[t * ST + 16 * wave + l.col]) - column_dot(l, st, k);
+                    }
+                    const float u = beta * error;
+                    add_outer(l, g, q, scale * o);
+                    const float du = column_dot(l, g, k), dv = beta * du;
+                    float dg = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < KT && !AHEAD; i++) {
+                        const f32x4 kr = ordered4(l, k, i);
+                        f32x4 pq, pk;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            pq[r] = sum16(scale * fmaf(kr[r], u, st[i][r]) * o);
+                            pk[r] = sum16(g[i][r] * u - st[i][r] * dv);
+                            dg = fmaf(fmaf(-kr[r], dv, g[i][r]), st[i][r], dg);
+                        }
+                        if (l.col == 0) {
+                            *reinterpret_cast<f32x4*>(parts + (2 * wave) * D + 16 * i + 4 * l.quad) = pq;
+                            *reinterpret_cast<f32x4*>(parts + (2 * wave + 1) * D + 16 * i + 4 * l.quad) = pk;
+                        }
+                        asm volatile("" : "+v"(dg)::"memory");
+                    }
+                    add_outer(l, g, k, -dv);
+#pragma unroll
+                    for (int i = 0; i < KT; i++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) g[i][r] = flag ? 0.0f : g[i][r] * decay;
+                    if (!AHEAD) {
+                        dg = sum_rows32(sum_rows16(sum16(dg)));
+                        const float db = sum16(16 * wave + l.col < vd ? du * error : 0.0f);
+                        if (lane == 0) {
+                            s.odd_sums[0][wave] = dg;
+                            s.odd_sums[1][wave] = db;
+                        }
+                        if (l.quad == 0 && 16 * wave + l.col < vd)
+                            Track<E>(&call_now->d.d_v, now.n, now.h).row(at)[16 * wave + l.col] = E(dv);
+                    }
+                }
+                if (AHEAD) continue;
+                __syncthreads();
+                const int v_waves = (vd + 15) / 16;
+                const uint32_t hg = call_now->d.partial ? now.h : now.hq;
+                if (tid < kd) {
+                    float dq = 0.0f, dk = 0.0f;
+                    for (int w = 0; w < v_waves; w++) {
+                        dq += parts[2 * w * D + tid];
+                        dk += parts[(2 * w + 1) * D + tid];
+                    }
+                    Track<F>(&call_now->d.d_q, now.n, hg).row(at)[tid] = F(dq);
+                    Track<F>(&call_now->d.d_k, now.n, hg).row(at)[tid] = F(dk);
+                }
+                if (tid == 0) {
+                    float dg = 0.0f, db = 0.0f;
+                    for (int w = 0; w < v_waves; w++) {
+                        dg += s.odd_sums[0][w];
+                        db += s.odd_sums[1][w];
+                    }
+                    put_gate<E>(call_now, now, at, flag ? 0.0f : dg, db);
+                }
+                __syncthreads();
+            }
+            __syncthreads();
+            if (next.job < plan.total) {
+                put_rows(next);
+                if (!AHEAD) fetch_state(next);
+            }
+            if (now.c == now.first) leave(now, g);
+            if (!FULL) clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
+            __syncthreads();
+            now = next;
+            next = later;
+            later.back(plan, which);
+            continue;
+        }
 
         // U and R
         f32x4 dv[2];
@@ -287,16 +420,15 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 mma(g[i], ordered_col(l, s.q, ST, 16 * i), of2);
                 mma(g[i], ordered_col(l, s.k, ST, 16 * i), rf);
             }
+#pragma unroll
+            for (int i = 0; i < KT && !FULL; i++) settle(g[i]);
         };
         if constexpr (AHEAD) {
             step_back();
             // all have read k, q and d_o, and the matrices
             __syncthreads();
             if (next.job < plan.total) put_rows(next);
-            if (now.c == now.first) {
-                float* p = fresh_call()->a.seg_grads + (uint64_t(now.state) * plan.segments + now.seg - 1) * kd * vd;
-                store_state(p, g, kd, vd, l, 16 * wave + l.col);
-            }
+            if (now.c == now.first) leave(now, g);
             __syncthreads();
             now = next;
             next = later;
@@ -314,6 +446,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 mma(dp, ordered_row(l, s.d_o, ST, i0, y), uj);
                 mma(da, col_frag<N>(l, s.r, CP, PL, y, i0), uj);
             }
+            if (!FULL) settle(dp, da);
             double m_row[4], m_col = 0.0;
             f32x4 b;
 #pragma unroll
@@ -387,6 +520,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         if (k_wave) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
+                if (!FULL) settle(dq[i], dk[i], dkg[i]);
                 const int t = 16 * i + 4 * l.quad;
                 const f32x4 before = four(gates.before + t);
                 dq[i] *= scale * before;
@@ -454,16 +588,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             const double before = scan_up32(double(pb), lane) - double(pb);   // over the ticks before t
             const float dg = gate_is_flag(gates, t) ? 0.0f : float(after + before + double(gates.before[C - 1]) * double(all));
             if (lane < C && uint32_t(t) < left) {
-                KernelCall* k = fresh_call();
-                const bool f32 = k->a.gate_f32 || sizeof(E) == 4;
-                const uint32_t at = now.c * C + t;
-                if (f32) {
-                    *Track<float>(&k->d.d_g, now.n, now.h).row(at) = dg;
-                    *Track<float>(&k->d.d_beta, now.n, now.h).row(at) = beta;
-                } else {
-                    *Track<bf16>(&k->d.d_g, now.n, now.h).row(at) = bf16(dg);
-                    *Track<bf16>(&k->d.d_beta, now.n, now.h).row(at) = bf16(beta);
-                }
+                put_gate<E>(fresh_call(), now, now.c * C + t, dg, beta);
             }
         }
         // the next chunk's rows and S are waited for before this one's gradients
@@ -484,8 +609,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         if (on_v.on && on_v.row < left)
             store_piece<E>(Track<E>(&k->d.d_v, now.n, now.h).row(now.c * C + on_v.row), vd, on_v.col,
                            piece_from_lds(dv_rows + on_v.row * ST + on_v.col));
-        if (now.c == 0)
-            if (float* p = k->d.d_state) store_state(p + uint64_t(now.state) * kd * vd, g, kd, vd, l, 16 * wave + l.col);
+        if (now.c == now.first) leave(now, g);
         // u, r and `through` take the next chunk's operands.  `through` is the
         // first, before the next barrier: all have to have read their gradients'
         // rows.  In narrow heads the columns past the width are operands too

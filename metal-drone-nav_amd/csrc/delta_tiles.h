@@ -152,6 +152,18 @@ __device__ __forceinline__ void mma(f32x4& acc, const Half<float, 1>& a, const H
     for (int s = 0; s < 4; s++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.t[0][s], b.t[0][s], acc, 0, 0, 0);
 }
 
+__device__ __forceinline__ void settle_one(f32x4& a) { asm volatile("" : "+v"(a)); }
+// Results that a loop with early ends may have written last: what reads them
+// comes at least 16 wait states later.  The compiler sees to that itself, but
+// where a loop over matrix products is unrolled and can end after each pass,
+// it has been seen to count the way through all passes and not the short one
+// (hipcc of ROCm 7.2: results of heads of at most 16 columns were read before
+// they were there).  A matrix product here is done after at most 11.
+template <class... X> __device__ __forceinline__ void settle(f32x4& a, X&... more) {
+    asm volatile("s_nop 15" : "+v"(a));
+    (settle_one(more), ...);
+}
+
 // ---- fp32 values to operands
 template <int N> __device__ __forceinline__ void split4(f32x4 x, bf16x4 (&t)[N]) {
 #pragma unroll

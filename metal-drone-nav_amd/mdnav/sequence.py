@@ -264,8 +264,9 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state
     None).  scale: K ** -0.5 if None.  o has v's shape and q's type.  Gradients
     reach every tensor argument but reset; a flagged tick has none for g.
     """
-    state = None if state is None else state.contiguous()
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state)):
+    if isinstance(state, torch.Tensor):
+        state = state.contiguous()
+    if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, g, beta, state)):
         return _DeltaRuleFunction.apply(q, k, v, g, beta, state, reset, scale, final_state)
     call = _Call(q, k, v, g, beta, state, reset, scale)
     o, last = call.output(), call.states() if final_state else None

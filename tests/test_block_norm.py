@@ -272,3 +272,44 @@ def test_refusals_on_the_gpu():
             (lambda: sequence.block_norm(torch.zeros(1, 8193).cuda(), torch.zeros(1, 8193).cuda(), w, w), ValueError, "8192")):
         with pytest.raises(error, match=match):
             bad()
+
+
+def test_the_c_entries_refuse():
+    """What the C entries check themselves, before anything is launched."""
+    import ctypes
+    from mdnav import native, sequence
+    lib = native.lib()
+    some = 4096
+    good = sequence._BlockNorm(3, 1, 64, 0, 0, 1, 0, 1e-6)
+    for name in ("x", "y", "gate", "s", "h"):
+        getattr(good, name).data = some
+    good.w_post = good.w_pre = good.stats = some
+
+    def refused(text, **fields):
+        c = sequence._BlockNorm.from_buffer_copy(good)
+        for name, value in fields.items():
+            setattr(c, name, value)
+        assert lib.mdn_op_block_norm_forward(ctypes.byref(c), None) == -1
+        assert text in lib.mdn_last_error().decode(), lib.mdn_last_error()
+
+    refused("1..8192", width=0)
+    refused("1..8192", width=8193)
+    refused("x_dtype", x_dtype=1)
+    refused("x_dtype", y_dtype=2)
+    refused("gate_kind", gate_kind=4)
+    refused("gate_dtype", gate_dtype=1)
+    refused("inner_count", inner_count=0)
+    refused("null weights", w_pre=None)
+    refused("null rows", x=sequence._NormRows())
+    refused("null rows", h=sequence._NormRows())
+    assert lib.mdn_op_block_norm_forward(None, None) == -1
+    empty = sequence._BlockNorm.from_buffer_copy(good)
+    empty.rows = 0
+    assert lib.mdn_op_block_norm_forward(ctypes.byref(empty), None) == 0
+    grad = sequence._BlockNormGrad()
+    assert lib.mdn_op_block_norm_backward(ctypes.byref(good), ctypes.byref(grad), None, 0, None) == -1
+    for name in ("d_s", "d_h", "d_x", "d_y", "d_gate"):
+        getattr(grad, name).data = some
+    grad.d_w_post = grad.d_w_pre = some
+    assert lib.mdn_op_block_norm_backward(ctypes.byref(good), ctypes.byref(grad), None, 0, None) == -1
+    assert "workspace is too small" in lib.mdn_last_error().decode()
