@@ -2270,7 +2270,7 @@ int mdn_op_delta_rule_forward(const MdnDeltaRule* rule, void* keep, uint64_t kee
     a.seg_moves = a.chunk_states ? a.chunk_states + delta_chunk_state_bytes(a) / sizeof(float) : a.seg_states + delta::seg_state_words(a);
     const bool bf = rule->dtype == MDN_BF16;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a.ticks <= 1 && !a.chunk_states)
+    if (a.ticks <= delta::recurrent_ticks(a, bf) && !a.chunk_states)
         HIP_TRY(delta::launch_recurrent(a, bf, st));
     else
         HIP_TRY(delta::launch_forward(a, bf, st));

@@ -39,14 +39,21 @@ struct Args {
 };
 
 // The segments.  Each costs its chunks three times (B, M and the outputs) but
-// for the first; 30,011 ticks of two envs and eight 128-wide heads went from 4,140 us
-// in one piece to 660 us (332 ahead, 92 joining, 228).  A workgroup for each of the 256 compute units or
-// more needs no cut: with 128 states and fewer there are at least four
-// segments to a state.
+// for the first, and the join: that pays while most compute units would idle.
+// In one piece against cut, in us, bf16, forward and forward with backward:
+//   2 states 128 x 128:   512 ticks 75 : 54 and 301 : 231, 4,096 ticks 553 : 136 and 2,215 : 284
+//   64 states 128 x 128:  512 ticks 79 : 81 and 307 : 234, 4,096 ticks 585 : 351 and 2,340 : 1,121
+//   128 states 128 x 128: 512 ticks 80 : 120 and 316 : 360, 1,024 ticks 151 : 176 and 610 : 591,
+//                         4,096 ticks 615 : 527 and 2,437 : 1,943
+//   128 states 64 x 64:   512 ticks 62 : 64 and 226 : 231, 1,024 ticks 114 : 96 and 391 : 253
+//   170 states 128 x 128: 4,096 ticks 631 : 576 and 2,532 : 2,439, 1,024 ticks 152 : 191 and 631 : 714
+// So: up to 128 states, at least four segments of at least four chunks each, and
+// of sixteen where there are more than 64 states of wide heads.
 inline void cut(Args& a) {
     const uint32_t states = a.envs * a.heads, chunks = (a.ticks + CHUNK - 1) / CHUNK;
+    const uint32_t least = states > 64 && (a.k_dim > 64 || a.v_dim > 64) ? 16 : 4;  // chunks of a segment
     uint32_t segments = states && states <= 128 ? 512 / states : 1;
-    if (segments > chunks / 4) segments = chunks / 4;
+    if (segments > chunks / least) segments = chunks / least;
     if (segments < 4) segments = 1;
     a.segment = (chunks + segments - 1) / (segments ? segments : 1);
     a.segments = a.segment ? (chunks + a.segment - 1) / a.segment : 1;
@@ -99,6 +106,20 @@ hipError_t launch_sum_heads(const float* in, void* out, uint64_t rows, uint32_t 
                             bool bf16, hipStream_t stream);
 // seg_grads[s - 1] += M_s^T seg_grads[s], from the last segment but one downwards.
 hipError_t launch_join_grads(const Args& a, bool bf16, hipStream_t stream);
+// The ticks up to which the recurrent kernel is taken.  It reads and writes a
+// state as fast as a copy does but works its ticks off on the vector units; the
+// chunk kernel costs much the same for 1 tick and 16, more in fp32 and where
+// heads do not fill its tiles.  Recurrent against chunks, in us:
+//   bf16, 16,384 states 64 x 64:  1 tick 106 : 173, 4 ticks 131 : 160, 6 ticks 153 : 161, 8 ticks 173 : 162
+//   bf16, 8,192 states 128 x 128: 1 tick 204 : 259, 4 ticks 231 : 243, 6 ticks 266 : 246
+//   bf16, 4,096 states 91 x 87:   1 tick 74 : 160, 8 ticks 127 : 188, 12 ticks 163 : 200
+//   bf16, 16,384 states 32 x 32:  1 tick 30 : 153, 12 ticks 99 : 155
+//   fp32, 16,384 states 64 x 64:  1 tick 104 : 248, 8 ticks 164 : 252, 12 ticks 203 : 257
+//   fp32, 8,192 states 128 x 128: 1 tick 202 : 397, 8 ticks 310 : 400, 12 ticks 394 : 406
+inline uint32_t recurrent_ticks(const Args& a, bool bf16) {
+    const bool full = a.k_dim == a.v_dim && (a.k_dim == 64 || a.k_dim == 128);
+    return bf16 && full ? 4 : 12;
+}
 hipError_t launch_recurrent(const Args& a, bool bf16, hipStream_t stream);
 hipError_t launch_forward(const Args& a, bool bf16, hipStream_t stream);
 

@@ -14,77 +14,139 @@ template <int CG> __device__ __forceinline__ float sum_columns(float x) {
     return sum_rows32(sum_rows16(x));
 }
 
+// Four neighbours of a row of `dim` from `col` on, those past its end 0.
+struct __attribute__((aligned(4))) Four32 { float x[4]; };
+struct __attribute__((aligned(2))) Four16 { bf16 x[4]; };
+template <class E> struct FourOf;
+template <> struct FourOf<float> { typedef Four32 type; };
+template <> struct FourOf<bf16> { typedef Four16 type; };
+template <class E> __device__ __forceinline__ typename FourOf<E>::type load_four(const E* row, uint32_t dim, uint32_t col) {
+    typename FourOf<E>::type r;
+    if (col + 4 <= dim) {
+        r = *reinterpret_cast<const typename FourOf<E>::type*>(row + col);
+    } else {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) r.x[c] = col + c < dim ? row[col + c] : E(0.0f);
+    }
+    return r;
+}
+template <class E> __device__ __forceinline__ void store_four(E* row, uint32_t dim, uint32_t col, f32x4 x) {
+    typename FourOf<E>::type r;
+#pragma unroll
+    for (int c = 0; c < 4; c++) r.x[c] = E(x[c]);
+    if (col + 4 <= dim) {
+        *reinterpret_cast<typename FourOf<E>::type*>(row + col) = r;
+    } else {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++)
+            if (col + c < dim) row[col + c] = r.x[c];
+    }
+}
+
 // One wavefront has all K rows of 4 CG columns of a state in registers for
-// the whole call: lane l the four columns 4 (l % CG) of rows l / CG, + 64 / CG, ..
-// Columns of a state do not meet in a tick (u_c needs column c of S only), so
-// wavefronts need no exchange; a tick's two sums over K are made in the lane,
-// then over the 64 / CG lanes of a column.
-template <class E, int CG, int ROWS>
-__global__ void __launch_bounds__(256, 3) recurrent_kernel(Args a) {
-    constexpr int RG = 64 / CG;  // rows of a step of the loop over K
-    const int lane = int(threadIdx.x) & 63;
+// the whole call: lane l the four columns 4 (l % CG) of rows l / CG, + 64 / CG,
+// ..  (a load of the wavefront then covers neighbouring rows).  Columns of a
+// state do not meet in a tick (u_c needs column c of S only), so wavefronts
+// need no exchange; a tick's two sums over K are made in the lane, then over
+// the 64 / CG lanes of a column.  k and q are loaded an element a lane and
+// handed round through LDS, where a lane's rows are neighbours.
+//
+// Bound by memory: a tick of 32,768 states 64 x 64 in bf16 (1.09 GB with the
+// rows) takes 193 us, 5.6 TB/s; of 18,006 states 40 x 72, rows of 288 bytes,
+// 91 us for 0.42 GB.  Lanes with 16 neighbouring rows each, whose k and q are
+// plain wide loads, took 193 and 147 us: their loads touch more cache lines in
+// rows that do not fill them.  Each further tick of 16,384 states adds 8.5 us,
+// vector work.
+template <class E, int CG>
+__global__ void __launch_bounds__(256, CG == 8 ? 3 : 4) recurrent_kernel(Args a) {
+    constexpr int RG = 64 / CG, ROWS = 16;  // rows of a step, most steps
+    __shared__ __align__(16) float rows_of[4][2][RG][ROWS];
+    const int lane = int(threadIdx.x) & 63, wave_here = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t slices = (a.v_dim + 4 * CG - 1) / (4 * CG);
-    const uint64_t wave = uint64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t wave = uint64_t(blockIdx.x) * 4 + wave_here;
     if (wave >= uint64_t(a.envs) * a.heads * slices) return;
     const uint32_t slice = uint32_t(wave % slices);
     const uint64_t seq = wave / slices;
     const uint32_t n = uint32_t(seq / a.heads), h = uint32_t(seq % a.heads);
     const uint32_t hq = h / (a.heads / a.qk_heads);
-    const uint32_t col = slice * 4 * CG + 4 * (lane % CG), row0 = lane / CG;
     const uint32_t kd = a.k_dim, vd = a.v_dim;
-    const bool wide = (vd & 3u) == 0 && col < vd;
+    const int steps = int((kd + RG - 1) / RG);
+    const uint32_t col = slice * 4 * CG + 4 * (lane % CG), row0 = lane / CG;
     const uint64_t base = seq * kd * vd;
+    // a tick's inputs, loaded a tick ahead
+    constexpr int EACH = RG * ROWS / 64;
+    GateRegs gate;
+    float ke[EACH], qe[EACH];
+    typename FourOf<E>::type vp;
+    const auto fetch = [&](uint32_t t) {
+        const E* k = reinterpret_cast<const E*>(a.k.p) + (t * a.k.tick + n * a.k.env + hq * a.k.head);
+        const E* q = reinterpret_cast<const E*>(a.q.p) + (t * a.q.tick + n * a.q.env + hq * a.q.head);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const uint32_t row = lane + 64 * i;
+            ke[i] = row < kd ? float(k[row]) : 0.0f;
+            qe[i] = row < kd ? float(q[row]) : 0.0f;
+        }
+        vp = load_four(reinterpret_cast<const E*>(a.v.p) + (t * a.v.tick + n * a.v.env + h * a.v.head), vd, col);
+        gate = load_gates<E>(&a, n, h, t, true);
+    };
+    // over the lane's rows, four at a time
+    const auto each_row = [&](auto&& f) {
+#pragma unroll
+        for (int i0 = 0; i0 < ROWS; i0 += 4)
+            if (i0 < steps) {
+#pragma unroll
+                for (int i = i0; i < i0 + 4; i++) f(i);
+            }
+    };
+    if (a.ticks) fetch(0);
     f32x4 s[ROWS];
     const bool cleared = a.reset && a.ticks && a.reset[n * a.reset_env] != 0;  // the first tick reads no state
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-        const uint32_t row = row0 + i * RG;
+    each_row([&](int i) {
         s[i] = f32x4{0, 0, 0, 0};
+        const uint32_t row = row0 + i * RG;
         if (a.state && !cleared && row < kd) {
-            const float* p = a.state + base + (row * vd + col);
-            if (wide) {
-                s[i] = *reinterpret_cast<const f32x4*>(p);
-            } else {
-#pragma unroll
-                for (uint32_t c = 0; c < 4; c++)
-                    if (col + c < vd) s[i][c] = p[c];
-            }
+            const Four32 x = load_four(a.state + base + row * vd, vd, col);
+            s[i] = f32x4{x.x[0], x.x[1], x.x[2], x.x[3]};
         }
-    }
+    });
     for (uint32_t t = 0; t < a.ticks; t++) {
-        const int64_t qo = t * a.q.tick + n * a.q.env + hq * a.q.head;
-        const int64_t ko = t * a.k.tick + n * a.k.env + hq * a.k.head;
-        GateRegs gate = load_gates<E>(&a, n, h, t, true);
-        gate.flag |= gate.g < NO_DECAY;
-        f32x4 v{0, 0, 0, 0};
-        const int64_t vo = t * a.v.tick + n * a.v.env + h * a.v.head + col;
 #pragma unroll
-        for (uint32_t c = 0; c < 4; c++)
-            if (col + c < vd) v[c] = load_one<E>(a.v.p, vo + c);
-        float kr[ROWS], qr[ROWS];
-#pragma unroll
-        for (int i = 0; i < ROWS; i++) {
-            const uint32_t row = row0 + i * RG;
-            kr[i] = row < kd ? load_one<E>(a.k.p, ko + row) : 0.0f;
-            qr[i] = row < kd ? load_one<E>(a.q.p, qo + row) : 0.0f;
+        for (int i = 0; i < EACH; i++) {
+            const int row = lane + 64 * i;
+            rows_of[wave_here][0][row % RG][row / RG] = ke[i];
+            rows_of[wave_here][1][row % RG][row / RG] = qe[i];
         }
-        if (gate.flag) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        f32x4 kr[ROWS / 4], qr[ROWS / 4];
+#pragma unroll
+        for (int i = 0; i < ROWS / 4; i++) {
+            kr[i] = *reinterpret_cast<const f32x4*>(&rows_of[wave_here][0][row0][4 * i]);
+            qr[i] = *reinterpret_cast<const f32x4*>(&rows_of[wave_here][1][row0][4 * i]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const f32x4 v{float(vp.x[0]), float(vp.x[1]), float(vp.x[2]), float(vp.x[3])};
+        const float beta = gate.beta, g = gate.g;
+        const bool flag = gate.flag || g < NO_DECAY;
+        if (t + 1 < a.ticks) fetch(t + 1);
+        if (flag) {
 #pragma unroll
             for (int i = 0; i < ROWS; i++) s[i] = f32x4{0, 0, 0, 0};
         }
-        const float decay = gate.flag ? 1.0f : __expf(gate.g);
+        const float decay = flag ? 1.0f : __expf(g);
         f32x4 ks{0, 0, 0, 0}, qs{0, 0, 0, 0};
         float kq = 0.0f;
-#pragma unroll
-        for (int i = 0; i < ROWS; i++) {
+        each_row([&](int i) {
             s[i] *= decay;
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                ks[c] = fmaf(kr[i], s[i][c], ks[c]);
-                qs[c] = fmaf(qr[i], s[i][c], qs[c]);
+                ks[c] = fmaf(kr[i / 4][i % 4], s[i][c], ks[c]);
+                qs[c] = fmaf(qr[i / 4][i % 4], s[i][c], qs[c]);
             }
-            kq = fmaf(kr[i], qr[i], kq);
-        }
+            kq = fmaf(kr[i / 4][i % 4], qr[i / 4][i % 4], kq);
+        });
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             ks[c] = sum_columns<CG>(ks[c]);
@@ -94,34 +156,20 @@ __global__ void __launch_bounds__(256, 3) recurrent_kernel(Args a) {
         f32x4 u, o;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            u[c] = gate.beta * (v[c] - ks[c]);
+            u[c] = beta * (v[c] - ks[c]);
             o[c] = a.scale * fmaf(kq, u[c], qs[c]);
         }
+        each_row([&](int i) {
 #pragma unroll
-        for (int i = 0; i < ROWS; i++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) s[i][c] = fmaf(kr[i], u[c], s[i][c]);
-        if (row0 == 0) {
-            const int64_t oo = t * a.o.tick + n * a.o.env + h * a.o.head + col;
-#pragma unroll
-            for (uint32_t c = 0; c < 4; c++)
-                if (col + c < vd) reinterpret_cast<E*>(a.o.p)[oo + c] = E(o[c]);
-        }
+            for (int c = 0; c < 4; c++) s[i][c] = fmaf(kr[i / 4][i % 4], u[c], s[i][c]);
+        });
+        if (row0 == 0) store_four(reinterpret_cast<E*>(a.o.p) + (t * a.o.tick + n * a.o.env + h * a.o.head), vd, col, o);
     }
     if (!a.state_out) return;
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) {
+    each_row([&](int i) {
         const uint32_t row = row0 + i * RG;
-        if (row >= kd) continue;
-        float* p = a.state_out + base + (row * vd + col);
-        if (wide) {
-            *reinterpret_cast<f32x4*>(p) = s[i];
-        } else {
-#pragma unroll
-            for (uint32_t c = 0; c < 4; c++)
-                if (col + c < vd) p[c] = s[i][c];
-        }
-    }
+        if (row < kd) store_four(a.state_out + base + row * vd, vd, col, s[i]);
+    });
 }
 
 // ---------------------------------------------------------------- chunks
@@ -481,16 +529,17 @@ hipError_t forward(const Args& a, hipStream_t stream) {
     return a.k_dim <= 64 && a.v_dim <= 64 ? forward<E, N, 64>(a, stream) : forward<E, N, 128>(a, stream);
 }
 
+// Wavefronts of 32 columns have room for 128 rows, those of 64 for 64; in heads
+// of at most 32 columns half the lanes of the wider ones would idle.
 template <class E>
 hipError_t recurrent(const Args& a, hipStream_t stream) {
-    const uint64_t seqs = uint64_t(a.envs) * a.heads;
-    if (a.k_dim <= 64) {
-        const uint64_t waves = seqs * ((a.v_dim + 63) / 64);
-        recurrent_kernel<E, 16, 16><<<dim3(uint32_t((waves + 3) / 4)), dim3(256), 0, stream>>>(a);
-    } else {
-        const uint64_t waves = seqs * ((a.v_dim + 31) / 32);
-        recurrent_kernel<E, 8, 16><<<dim3(uint32_t((waves + 3) / 4)), dim3(256), 0, stream>>>(a);
-    }
+    const uint32_t cols = a.k_dim > 64 || a.v_dim <= 32 ? 32 : 64;
+    const uint64_t waves = uint64_t(a.envs) * a.heads * ((a.v_dim + cols - 1) / cols);
+    const dim3 grid(uint32_t((waves + 3) / 4));
+    if (cols == 64)
+        recurrent_kernel<E, 16><<<grid, dim3(256), 0, stream>>>(a);
+    else
+        recurrent_kernel<E, 8><<<grid, dim3(256), 0, stream>>>(a);
     return hipGetLastError();
 }
 
