@@ -425,7 +425,8 @@ typedef struct MdnRows {
  * g is the logarithm of the decay (-inf allowed) and beta the strength of the
  * write.  qk_heads divides heads: value head h reads query and key head
  * h / (heads / qk_heads).  k_dim and v_dim are 1..128, ticks and envs may be
- * 0 (the state then passes through). */
+ * 0 (the state then passes through).  An infinity or NaN reaches what the
+ * formulas bring it to, later ticks of its episode, and nothing else. */
 typedef struct MdnDeltaRule {
     uint32_t ticks, envs, qk_heads, heads, k_dim, v_dim;
     uint32_t dtype;       /* of q, k, v and o: MDN_F32 or MDN_BF16 */

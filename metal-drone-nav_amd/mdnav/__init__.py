@@ -6,7 +6,8 @@ Host-side Python face of the C ABI in include/mdnav.h: ``Sim`` and
 (cpu_reference.hpp:112-615), all running on the HIP library
 ``lib/libmdnav.so``.  ``abi`` holds the struct layouts, ``ops`` the stateless
 operators.  Importing is cheap; the library loads on first use and raises if
-it is missing.
+it is missing.  ``mdnav.sequence``, imported by itself, has the operators of
+recurrent policies over torch tensors.
 """
 from . import abi  # noqa: F401
 from .native import MdnError  # noqa: F401
