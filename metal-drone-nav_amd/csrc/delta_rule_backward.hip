@@ -27,9 +27,11 @@ namespace {
 template <class E, int D> struct BackwardShared {
     static constexpr int STRIDE = D + Kind<E>::PAD;
     static constexpr int N = Kind<E>::MID;
-    // S and G pass through LDS, transposed, as operands; of 128 columns in fp32
-    // the rows and these do not fit beside each other, and take halves of V
-    static constexpr int HALVES = sizeof(E) == 4 && D == 128 ? 2 : 1;
+    // S and G pass through LDS, transposed, as operands; in fp32 in halves of V:
+    // of 128 columns they would not fit beside the rows, of 64 a compute unit
+    // would have room for one workgroup and not two (4,096 states, 64 ticks: 465
+    // us whole, 369 in halves)
+    static constexpr int HALVES = sizeof(E) == 4 ? 2 : 1;
     static constexpr int TP = D / HALVES * STRIDE;
     static constexpr int PLANE = D * CP;
     static constexpr int W = D / 16;
