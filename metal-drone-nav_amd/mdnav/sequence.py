@@ -107,7 +107,12 @@ def _on(device, call, *args):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    # torch.cuda.current_stream(device).cuda_stream without the object around it: 0.1 and not 1.9 us of a call
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _address(t):
@@ -186,7 +191,7 @@ class _Call:
             c.state = state.data_ptr()
 
     def output(self):
-        return torch.empty(self.v.shape, dtype=self.v.dtype, device=self.device)
+        return _like(self.v)
 
     def states(self):
         c = self.c
@@ -213,7 +218,7 @@ class _Call:
 
     def backward(self, kept, sizes, d_o, d_state_out, want_state):
         """(d_q, d_k, d_v, d_g, d_beta, d_state or None)"""
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=self.device) for x in (self.q, self.k, self.v, self.g, self.beta)]
+        grads = [_like(x) for x in (self.q, self.k, self.v, self.g, self.beta)]
         d_state = self.states() if want_state else None
         work = _buffer(sizes.backward_workspace, self.device)
         d = _DeltaRuleGrad(_rows(d_o), _address(d_state_out), *[_rows(x) for x in grads], _address(d_state))
@@ -368,15 +373,16 @@ class _NormCall:
             self.kept.append(t)
         return _NormRows(t.data_ptr(), t.shape[-1] * self.inner, t.shape[-1])
 
-    def like(self, t):
-        return torch.empty(t.shape, dtype=t.dtype, device=self.device)
+    def made(self, t):
+        """The layout of a contiguous [..., width] tensor."""
+        return _NormRows(t.data_ptr(), self.width * self.inner, self.width)
 
     def forward(self, keep):
         L = _library()
-        s, h = self.like(self.x), self.like(self.y)
+        s, h = _like(self.x), _like(self.y)
         stats = torch.empty(self.rows, 2, device=self.device) if keep else None
         c = self.c
-        c.s, c.h, c.stats = self.layout(s), self.layout(h), _address(stats)
+        c.s, c.h, c.stats = self.made(s), self.made(h), _address(stats)
         check(L.mdn_op_block_norm_forward(ctypes.byref(c), _stream(self.device)))
         return s, h, stats
 
@@ -388,10 +394,10 @@ class _NormCall:
             d.d_s = self.layout(d_s)
         if d_h is not None:
             d.d_h = self.layout(d_h)
-        d_x, d_y, d_gate = self.like(self.x), self.like(self.y), None
-        d.d_x, d.d_y = self.layout(d_x), self.layout(d_y)
+        d_x, d_y, d_gate = _like(self.x), _like(self.y), None
+        d.d_x, d.d_y = self.made(d_x), self.made(d_y)
         if self.kind != GATE_NONE:
-            d_gate = self.like(self.gate)
+            d_gate = _like(self.gate)
             d.d_gate = self.layout(d_gate) if self.kind != GATE_CHANNEL else _NormRows(d_gate.data_ptr(), 0, 0)
         d_post, d_pre, d_scale = torch.empty(3, self.width, device=self.device).unbind()
         d.d_w_post, d.d_w_pre = d_post.data_ptr(), d_pre.data_ptr()
