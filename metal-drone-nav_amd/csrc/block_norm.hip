@@ -10,11 +10,16 @@
 //     t = ds + z / rms(s) - s mean(z s) / rms(s)^3      (the whole gradient of s)
 //     dx = r t,   d_gate = t n w_post,   dn = t gate w_post,
 //     dy = dn / rms(y) - y mean(dn y) / rms(y)^3
-// and the column sums of dh s / rms(s), t gate n, t x (and t n w_post for a gate
+// with sum(dn y) = sum((ds + z / rms(s)) gate w_post y) - mean(z s) / rms(s)^3
+// sum(s gate w_post y), so that a row's sums are made at once: a row of a
+// workgroup has one barrier.  The column sums are those
+// of dh s / rms(s), t gate n, t x (and t n w_post for a gate
 // per channel).  A lane always has the same columns and adds up its rows' terms
 // in registers; workgroups write one row of sums each and a second kernel adds
 // those up in a fixed order: no atomics, the same bits every time.
 #include "block_norm.h"
+
+#include "lane_sums.h"
 
 namespace blocknorm {
 namespace {
@@ -113,27 +118,33 @@ __device__ __forceinline__ void store(T* row, const float (&in)[W], uint32_t at,
     }
 }
 
-// Sums over a row's lanes.  G 0: the whole workgroup, through LDS; `lds` is
-// another one than the last sum's, so that one barrier is enough.
+// Sums over a row's lanes.  G 0: the whole workgroup, through LDS, where each
+// sixteen lanes add up the wavefronts' sums; `lds` is another one than the last
+// sum's, so that one barrier is enough, and 0 past the workgroup's wavefronts.
+constexpr int WAVES = 16;
 template <int G, int N, class A>
-__device__ __forceinline__ void row_sum(A (&v)[N], A (*lds)[2]) {
-    constexpr int IN_WAVE = G == 0 ? 64 : G;
+__device__ __forceinline__ void row_sum(A (&v)[N], A (*lds)[N]) {
 #pragma unroll
-    for (int d = 1; d < IN_WAVE; d <<= 1)
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] += __shfl_xor(v[i], d);
+    for (int i = 0; i < N; i++) {
+        v[i] = lanes::sum16(v[i]);
+        if (G == 0 || G >= 32) v[i] = lanes::sum_rows16(v[i]);
+        if (G == 0 || G >= 64) v[i] = lanes::sum_rows32(v[i]);
+    }
     if (G == 0) {
-        const uint32_t waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
-            for (int i = 0; i < N; i++) lds[wave][i] = v[i];
+            for (int i = 0; i < N; i++) lds[threadIdx.x >> 6][i] = v[i];
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = 0;
-        for (uint32_t w = 0; w < waves; w++)
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] += lds[w][i];
+        for (int i = 0; i < N; i++) v[i] = lanes::sum16(lds[threadIdx.x & 15][i]);
     }
+}
+template <int G, int N, class A> __device__ __forceinline__ void clear_sums(A (*lds)[WAVES][N]) {
+    if (G != 0) return;
+    if (threadIdx.x < 2 * WAVES)
+#pragma unroll
+        for (int i = 0; i < N; i++) lds[threadIdx.x / WAVES][threadIdx.x % WAVES][i] = 0;
+    __syncthreads();
 }
 
 // The channels' vectors: in registers for the whole call where a row has at
@@ -223,9 +234,13 @@ template <int G> __device__ __forceinline__ uint32_t row_in_group() {
     return G == 64 ? __builtin_amdgcn_readfirstlane(r) : r;
 }
 
+// Bound by memory: 262,144 x 256 in bfloat16 (0.54 GB) takes 95 us, 5.7 TB/s;
+// 32,768 x 5,120 with a gate per element (1.68 GB) 314 us, 5.3 TB/s; 37,000 x
+// 181 in fp32, rows of 724 bytes (0.11 GB), 24 us, 4.4 TB/s.
 template <class TX, class TY, int G, int P, int W, int GATE>
 __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) forward_kernel(Args a) {
-    __shared__ float lds[2][12][2];
+    __shared__ float lds[2][WAVES][1];
+    clear_sums<G>(lds);
     extern __shared__ __align__(16) float channels[];
     const uint32_t group = G == 0 ? blockDim.x : G, per = G == 0 ? 1 : 256 / G;
     const uint32_t lane = threadIdx.x % group, width = a.width;
@@ -282,14 +297,24 @@ __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) forward_kerne
 // difference of large parts (in a row of one element it is the share of
 // epsilon): there the row's sums and differences are formed in 64 bits, and
 // the norms again from the row.  Wider rows take them in 32 bits.
+//
+// Bound by memory: 262,144 x 256 in bfloat16 (0.81 GB) takes 165 us, 4.9 TB/s;
+// 32,768 x 5,120 with a gate per element (2.68 GB) 720 us, 3.7 TB/s: its column
+// sums, the row and the next one fill the registers that one workgroup of ten
+// wavefronts a compute unit has, so one row is on its way while one is worked on
+// (vector units busy 29 % of the time).  Measured there: two rows ahead, which
+// spills, 882 us; two sums a row one after the other through LDS 784 us (and
+// 209 us in the first case).
 template <int G> struct Sum { typedef float type; };
 template <> struct Sum<16> { typedef double type; };
 
 template <class TX, class TY, int G, int P, int W, int GATE>
 __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) backward_kernel(Args a, GradArgs d) {
     typedef typename Sum<G>::type A;
-    constexpr int SUMS = GATE == ROW ? 2 : 1;
-    __shared__ A lds[2][12][2];
+    constexpr bool AGAIN = G == 16;  // the norms are made again
+    constexpr int SUMS = AGAIN ? 5 : 3;
+    __shared__ A lds[2][WAVES][SUMS];
+    clear_sums<G>(lds);
     extern __shared__ __align__(16) float channels[];
     const uint32_t group = G == 0 ? blockDim.x : G, per = G == 0 ? 1 : 256 / G;
     const uint32_t lane = threadIdx.x % group, width = a.width;
@@ -314,79 +339,81 @@ __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) backward_kern
     };
     const uint64_t mine0 = uint64_t(blockIdx.x) * per + row_in_group<G>();
     fetch_row(next, mine0);
-    for (uint64_t mine = mine0, first = uint64_t(blockIdx.x) * per; first < a.rows; first += step, mine += step) {
+    for (uint64_t mine = mine0, first = uint64_t(blockIdx.x) * per, turn = 0; first < a.rows; first += step, mine += step, turn ^= 1) {
         const bool in = mine < a.rows;
         const uint64_t row = in ? mine : a.rows - 1;
         now = next;
         if (first + step < a.rows) fetch_row(next, mine + step);
         A ry = now.ry, rs = now.rs;
-        if (G == 16) {
+        if (AGAIN) {
             A squares[1] = {0};
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
                 for (int e = 0; e < W; e++) squares[0] += A(value(now.in.y, p, e)) * A(value(now.in.y, p, e));
-            row_sum<G>(squares, lds[0]);
+            row_sum<G, 1, A>(squares, nullptr);
             ry = A(1) / sqrt(squares[0] / A(width) + A(a.eps));
         }
         const float ryf = float(ry);
-        A sum[G == 16 ? 2 : 1] = {};
+        // z s, what t is made of (z without rs where that is not known yet) times gate w_post y, s times that
+        A sum[SUMS] = {};
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int e = 0; e < W; e++) {
-                const float s = wt.s(now.in, p, e, value(now.in.y, p, e) * ryf * wt.post_at(p, e));
-                sum[0] += A(value(now.dh, p, e) * wt.pre_at(p, e)) * A(s);
-                if (G == 16) sum[G == 16 ? 1 : 0] += A(s) * A(s);
+                const float y = value(now.in.y, p, e), w = wt.post_at(p, e), s = wt.s(now.in, p, e, y * ryf * w);
+                const A z = value(now.dh, p, e) * wt.pre_at(p, e), ds = value(now.ds, p, e);
+                const A wy = (GATE == ROW ? A(w) : A(wt.gate_at(now.in, p, e)) * A(w)) * A(y);
+                sum[0] += z * A(s);
+                sum[1] += (AGAIN ? z : ds + rs * z) * wy;
+                sum[2] += A(s) * wy;
+                if (AGAIN) {
+                    sum[SUMS - 2] += ds * wy;
+                    sum[SUMS - 1] += A(s) * A(s);
+                }
                 if (P > 1 && e == W - 1) asm volatile("" : "+v"(sum[0])::"memory");  // the next piece's channels are read after this one's use
             }
-        row_sum<G>(sum, lds[0]);
-        if (G == 16) rs = A(1) / sqrt(sum[G == 16 ? 1 : 0] / A(width) + A(a.eps));
+        row_sum<G>(sum, lds[turn]);
+        if (AGAIN) {
+            rs = A(1) / sqrt(sum[SUMS - 1] / A(width) + A(a.eps));
+            sum[1] = sum[SUMS - 2] + rs * sum[1];
+        }
         const float rsf = float(rs), keep = in ? 1.0f : 0.0f;
         const A back = sum[0] / A(width) * rs * rs * rs;
-        A sums[SUMS] = {};
-        float dn[P][W];
+        const A along = sum[1] - back * sum[2];  // t w_post y, times the gate if it is not the row's
+        const A pull = along * (GATE == ROW ? A(now.in.one) : A(1)) / A(width) * ry * ry * ry;
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            float out[W], dgate[W];
+            float out[W], dgate[W], dy[W];
 #pragma unroll
             for (int e = 0; e < W; e++) {
                 const float y = value(now.in.y, p, e), x = value(now.in.x, p, e), dh = value(now.dh, p, e);
                 const float n = y * ryf, w = wt.post_at(p, e), b = n * w, s = wt.s(now.in, p, e, b), gv = wt.gate_at(now.in, p, e);
-                const float t = float(A(value(now.ds, p, e)) + (rs * A(dh * wt.pre_at(p, e)) - back * A(s)));
+                const A ta = A(value(now.ds, p, e)) + (rs * A(dh * wt.pre_at(p, e)) - back * A(s));
+                const float t = float(ta);
                 c_pre[p][e] = fmaf(keep * dh, s * rsf, c_pre[p][e]);
                 c_post[p][e] = fmaf(keep * t, gv * n, c_post[p][e]);
                 c_res[p][e] = fmaf(keep * t, x, c_res[p][e]);
                 if (GATE == CHANNEL) c_gate[p][e] = fmaf(keep * t, b, c_gate[p][e]);
                 if (GATE == ELEMENT) dgate[e] = t * b;
-                if (GATE == ROW) sums[SUMS - 1] += A(t) * A(b);
                 out[e] = wt.scaled ? wt.residual_at(p, e) * t : t;
-                dn[p][e] = t * gv * w;
-                sums[0] += A(dn[p][e]) * A(y);
+                dy[e] = float(ry * (ta * (A(gv) * A(w))) - pull * A(y));
             }
             if (in) {
                 const uint32_t at = place<W>(p, lane, group);
                 store<TX, W>(reinterpret_cast<TX*>(d.d_x.p) + row_at(d.d_x, a, row), out, at, width);
                 if (GATE == ELEMENT) store<TY, W>(reinterpret_cast<TY*>(d.d_gate.p) + row_at(d.d_gate, a, row), dgate, at, width);
+                store<TY, W>(reinterpret_cast<TY*>(d.d_y.p) + row_at(d.d_y, a, row), dy, at, width);
             }
-            if (P > 1) asm volatile("" : "+v"(sums[0])::"memory");
+            if (P > 1) asm volatile("" ::: "memory");
         }
-        row_sum<G>(sums, lds[1]);
-        const A pull = sums[0] / A(width) * ry * ry * ry;
-        if (in) {
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-#pragma unroll
-                for (int e = 0; e < W; e++) dn[p][e] = float(ry * A(dn[p][e]) - pull * A(value(now.in.y, p, e)));
-                store<TY, W>(reinterpret_cast<TY*>(d.d_y.p) + row_at(d.d_y, a, row), dn[p], place<W>(p, lane, group), width);
-            }
-            if (GATE == ROW && lane == 0) {
-                const int64_t at = row_at(d.d_gate, a, row);
-                if (a.gate_f32)
-                    reinterpret_cast<float*>(d.d_gate.p)[at] = float(sums[SUMS - 1]);
-                else
-                    reinterpret_cast<TY*>(d.d_gate.p)[at] = TY(float(sums[SUMS - 1]));
-            }
+        if (in && GATE == ROW && lane == 0) {
+            const int64_t at = row_at(d.d_gate, a, row);
+            const float value = float(ry * along);
+            if (a.gate_f32)
+                reinterpret_cast<float*>(d.d_gate.p)[at] = value;
+            else
+                reinterpret_cast<TY*>(d.d_gate.p)[at] = TY(value);
         }
     }
     // the workgroup's column sums: its groups of lanes add theirs up in order
@@ -421,7 +448,8 @@ __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) backward_kern
 }
 
 // Adds up the workgroups' rows of column sums: 64 columns per workgroup, a
-// sixteenth of the rows per wavefront, eight loads in flight.
+// sixteenth of the rows per wavefront, eight loads in flight.  5 us for 256
+// rows of 4 x 5,120 columns: a launch and three round trips to memory.
 __global__ void __launch_bounds__(1024) columns_kernel(const float* parts, uint32_t count, uint32_t width, float* post, float* pre,
                                                        float* res, char* gate, uint32_t gate_f32) {
     __shared__ float lds[16][64];

@@ -20,10 +20,14 @@
 #ifndef MDNAV_DELTA_TILES_H
 #define MDNAV_DELTA_TILES_H
 
+#include "lane_sums.h"
+
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 namespace delta {
+
+using namespace lanes;
 
 typedef __bf16 bf16;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -45,33 +49,7 @@ struct Lane {
     }
 };
 
-// ---- sums over lanes, without LDS
-template <int CTRL> __device__ __forceinline__ float from_lane(float x) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
-template <int CTRL> __device__ __forceinline__ double from_lane(double x) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, 0xf, 0xf, true));
-    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, 0xf, 0xf, true));
-    return __builtin_bit_cast(double, uint64_t(lo) | uint64_t(hi) << 32);
-}
-// Over the 16 lanes with the same l / 16: neighbours, pairs, then mirrored eights and sixteens.
-template <class T> __device__ __forceinline__ T sum16(T x) {
-    x += from_lane<0xB1>(x);
-    x += from_lane<0x4E>(x);
-    x += from_lane<0x141>(x);
-    return x + from_lane<0x140>(x);
-}
-// Over lanes l, l ^ 16, and over l, l ^ 32.
-__device__ __forceinline__ float sum_rows16(float x) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
-    return __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
-}
-__device__ __forceinline__ float sum_rows32(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
-    return __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
-}
-
+// ---- sums over lanes, without LDS (lane_sums.h), and running ones
 // Inclusive sums over lanes 0..31, upwards (lane i: lanes 0..i) and downwards
 // (lanes i..31): by DPP shifts inside each 16, then the other 16's total.
 __device__ __forceinline__ double lane_value(double x, int lane) {
