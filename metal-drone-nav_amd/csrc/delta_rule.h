@@ -33,7 +33,7 @@ struct Args {
     // run side by side (cut()): a state that a segment begins with is a linear
     // function of the one the last segment began with, S' = M S + B.
     uint32_t segments, segment;
-    float* seg_states;        // [state][segments][k][v]: B of the segment before, then the state before the segment
+    float* seg_states;        // [state][segments][k][v]: B of the segment before (the first has the state), then the state before the segment
     float* seg_moves;         // [state][segments][k][k]: M
     float* seg_grads;         // [state][segments][k][v]: the same for the state's gradient after the segment
 };

@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         const uint64_t words = kd * vd;
         const float* p = k->a.state;
         if (p) p += at.state * words;
-        if (at.seg > 0) p = AHEAD ? nullptr : k->a.seg_states + (uint64_t(at.state) * plan.segments + at.seg) * words;
+        if (AHEAD && at.seg > 0) p = nullptr;
+        if (!AHEAD && plan.segments > 1) p = k->a.seg_states + (uint64_t(at.state) * plan.segments + at.seg) * words;
         load_state(state, p, kd, vd, l, 16 * wave + l.col);
         if (AHEAD && at.part)
 #pragma unroll
@@ -293,6 +294,9 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         const uint32_t left = ticks - now.c * C;  // ticks from the chunk's first
         if (next.job < plan.total) fetch(next);
         const uint32_t cols = AHEAD && now.part ? kd : vd;  // of the state
+        // the main pass takes the first segment's state from here: the caller's
+        // may be state_out too, which the last segment writes when it likes
+        if (AHEAD && now.c == 0) store_state(fresh_call()->a.seg_states + uint64_t(now.state) * plan.segments * kd * vd, state, kd, vd, l, 16 * wave + l.col);
         if (!AHEAD && now.c > 0 && 16 * wave < int(vd)) {
             if (float* keep = fresh_call()->a.chunk_states) {
                 f32x4* p = state_tiles(keep, now.state, plan.chunks, now.c, kd, vd, wave);

@@ -504,3 +504,18 @@ def test_the_c_entries_refuse():
     grad = sequence._DeltaRuleGrad()
     assert lib.mdn_op_delta_rule_backward(ctypes.byref(rule_), ctypes.byref(grad), None, 0, None, 0, None) == -1
     assert "null rows" in lib.mdn_last_error().decode()
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(1, 3, 1, 2, 64, 64), (70, 3, 1, 2, 64, 48), (1500, 2, 1, 1, 64, 64), (2500, 1, 1, 2, 128, 128)], ids=str)
+def test_a_state_replaced_in_place(shape):
+    """The C entry takes the same buffer for the state before and after, of one tick, in chunks and in segments."""
+    from mdnav import sequence
+    x = inputs(*shape, "bf16", seed=8, resets=0)
+    want_o, want_s = sequence.delta_rule(**x, final_state=True)
+    for _ in range(3):
+        state = x["state"].clone()
+        call = sequence._Call(x["q"], x["k"], x["v"], x["g"], x["beta"], state, x["reset"], None)
+        o = call.output()
+        call.forward(o, state, False)
+        assert torch.equal(o, want_o) and torch.equal(state, want_s)
