@@ -378,7 +378,8 @@ __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) backward_kern
             rs = A(1) / sqrt(sum[SUMS - 1] / A(width) + A(a.eps));
             sum[1] = sum[SUMS - 2] + rs * sum[1];
         }
-        const float rsf = float(rs), keep = in ? 1.0f : 0.0f;
+        if (!in) continue;
+        const float rsf = float(rs);
         const A back = sum[0] / A(width) * rs * rs * rs;
         const A along = sum[1] - back * sum[2];  // t w_post y, times the gate if it is not the row's
         const A pull = along * (GATE == ROW ? A(now.in.one) : A(1)) / A(width) * ry * ry * ry;
@@ -391,23 +392,21 @@ __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) backward_kern
                 const float n = y * ryf, w = wt.post_at(p, e), b = n * w, s = wt.s(now.in, p, e, b), gv = wt.gate_at(now.in, p, e);
                 const A ta = A(value(now.ds, p, e)) + (rs * A(dh * wt.pre_at(p, e)) - back * A(s));
                 const float t = float(ta);
-                c_pre[p][e] = fmaf(keep * dh, s * rsf, c_pre[p][e]);
-                c_post[p][e] = fmaf(keep * t, gv * n, c_post[p][e]);
-                c_res[p][e] = fmaf(keep * t, x, c_res[p][e]);
-                if (GATE == CHANNEL) c_gate[p][e] = fmaf(keep * t, b, c_gate[p][e]);
+                c_pre[p][e] = fmaf(dh, s * rsf, c_pre[p][e]);
+                c_post[p][e] = fmaf(t, gv * n, c_post[p][e]);
+                c_res[p][e] = fmaf(t, x, c_res[p][e]);
+                if (GATE == CHANNEL) c_gate[p][e] = fmaf(t, b, c_gate[p][e]);
                 if (GATE == ELEMENT) dgate[e] = t * b;
                 out[e] = wt.scaled ? wt.residual_at(p, e) * t : t;
                 dy[e] = float(ry * (ta * (A(gv) * A(w))) - pull * A(y));
             }
-            if (in) {
-                const uint32_t at = place<W>(p, lane, group);
-                store<TX, W>(reinterpret_cast<TX*>(d.d_x.p) + row_at(d.d_x, a, row), out, at, width);
-                if (GATE == ELEMENT) store<TY, W>(reinterpret_cast<TY*>(d.d_gate.p) + row_at(d.d_gate, a, row), dgate, at, width);
-                store<TY, W>(reinterpret_cast<TY*>(d.d_y.p) + row_at(d.d_y, a, row), dy, at, width);
-            }
+            const uint32_t at = place<W>(p, lane, group);
+            store<TX, W>(reinterpret_cast<TX*>(d.d_x.p) + row_at(d.d_x, a, row), out, at, width);
+            if (GATE == ELEMENT) store<TY, W>(reinterpret_cast<TY*>(d.d_gate.p) + row_at(d.d_gate, a, row), dgate, at, width);
+            store<TY, W>(reinterpret_cast<TY*>(d.d_y.p) + row_at(d.d_y, a, row), dy, at, width);
             if (P > 1) asm volatile("" ::: "memory");
         }
-        if (in && GATE == ROW && lane == 0) {
+        if (GATE == ROW && lane == 0) {
             const int64_t at = row_at(d.d_gate, a, row);
             const float value = float(ry * along);
             if (a.gate_f32)

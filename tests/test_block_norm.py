@@ -313,3 +313,22 @@ def test_the_c_entries_refuse():
     grad.d_w_post = grad.d_w_pre = some
     assert lib.mdn_op_block_norm_backward(ctypes.byref(good), ctypes.byref(grad), None, 0, None) == -1
     assert "workspace is too small" in lib.mdn_last_error().decode()
+
+
+@gpu
+@pytest.mark.parametrize("width", [24, 64, 181, 300, 2100])
+def test_an_infinite_gradient_in_the_last_row(width):
+    """It reaches its row and its columns' sums as an infinity, also where lanes past the last row repeat its loads."""
+    from mdnav import sequence
+    x, _, _ = inputs((5, width), "channel", F32, F32, seed=6)
+    leaves = {name: t.requires_grad_() for name, t in x.items()}
+    s, h = sequence.block_norm(**leaves)
+    d_s, d_h = torch.full_like(s, 0.5), torch.full_like(h, 0.25)
+    d_s[4, 3] = float("inf")
+    got = torch.autograd.grad([s, h], list(leaves.values()), [d_s, d_h])
+    with np.errstate(all="ignore"):
+        want = gradients(**host(x), d_s=d_s.double().cpu().numpy(), d_h=d_h.double().cpu().numpy())
+    for name, grad in zip(leaves, got):
+        a, b = grad.double().cpu().numpy(), want[name]
+        assert np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(np.isinf(a), np.isinf(b)), name
+        assert np.array_equal(np.sign(a[np.isinf(a)]), np.sign(b[np.isinf(b)])), name
