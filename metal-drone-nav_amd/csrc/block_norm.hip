@@ -127,8 +127,8 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A (*lds)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
         v[i] = lanes::sum16(v[i]);
-        if (G == 0 || G >= 32) v[i] = lanes::sum_rows16(v[i]);
-        if (G == 0 || G >= 64) v[i] = lanes::sum_rows32(v[i]);
+        if constexpr (G == 0 || G >= 32) v[i] = lanes::sum_rows16(v[i]);
+        if constexpr (G == 0 || G >= 64) v[i] = lanes::sum_rows32(v[i]);
     }
     if (G == 0) {
         if ((threadIdx.x & 63) == 0)

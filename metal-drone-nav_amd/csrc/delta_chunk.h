@@ -24,11 +24,6 @@ constexpr int CP = C + 8;  // row of a chunk x chunk matrix in LDS
 // of decays stay finite (-inf included).
 constexpr float NO_DECAY = -104.0f;
 
-template <class E>
-__device__ __forceinline__ float load_one(const char* p, int64_t i) {
-    return float(reinterpret_cast<const E*>(p)[i]);
-}
-
 // Wavefront `wave`'s tiles of the state before chunk `c` >= 1.
 __device__ __forceinline__ f32x4* state_tiles(float* p, uint64_t seq, uint32_t chunks, uint32_t c, uint32_t kd, uint32_t vd, int wave) {
     const uint32_t kt = (kd + 15) / 16, vt = (vd + 15) / 16;

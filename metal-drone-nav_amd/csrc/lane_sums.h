@@ -32,8 +32,6 @@ __device__ __forceinline__ float sum_rows32(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
     return __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
 }
-__device__ __forceinline__ double sum_rows16(double x) { return x + __shfl_xor(x, 16); }
-__device__ __forceinline__ double sum_rows32(double x) { return x + __shfl_xor(x, 32); }
 
 }  // namespace lanes
 
