@@ -481,6 +481,9 @@ __global__ void __launch_bounds__(1024) columns_kernel(const float* parts, uint3
 
 // The lanes of a row: one piece of W elements each on a part of a wavefront,
 // one, or a workgroup of at most most_lanes(); up to 16 elements a lane in wider rows.
+// 262,144 x 256 in bfloat16 on halves of wavefronts and on whole ones: 90 : 166 us
+// forward, 175 : 481 backward; 1,048,576 x 64 in fp32 on quarters and on whole ones
+// 205 : 473 and 376 : 835.
 struct Shape { uint32_t lanes, pieces; };
 inline Shape shape_of(uint32_t width, uint32_t w, uint32_t lanes_1, uint32_t lanes_2) {
     const uint32_t pieces = (width + w - 1) / w;
