@@ -284,13 +284,17 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None):
 
     q, k: [envs][qk heads][K], v: [envs][heads][V], g, beta: [envs][heads],
     reset: [envs], state: contiguous [envs][heads][K][V] float32; otherwise as
-    ``delta_rule``.  No gradients.
+    ``delta_rule``.  No gradients: autograd sees ``state`` change, as by any
+    operation in place, so a backward pass that still reads the old one raises.
     """
     if not isinstance(state, torch.Tensor) or not state.is_contiguous():
         raise ValueError("state is a contiguous tensor: it is advanced in place")
+    if state.requires_grad and torch.is_grad_enabled():
+        raise ValueError("state requires gradients, which a tick in place has none for")
     call = _Call(q, k, v, g, beta, state, reset, scale, one_tick=True)
     o = call.output()
     _on(call.device, call.step, o, state)
+    torch.autograd.graph.increment_version(state)
     return o
 
 

@@ -519,3 +519,24 @@ def test_a_state_replaced_in_place(shape):
         o = call.output()
         call.forward(o, state, False)
         assert torch.equal(o, want_o) and torch.equal(state, want_s)
+
+
+@gpu
+def test_a_tick_in_place_is_seen_by_autograd():
+    """A backward pass that would read the state of before the tick raises; a state that wants gradients is refused."""
+    from mdnav import sequence
+    x = inputs(5, 3, 1, 2, 16, 16, "f32", seed=9)
+    x["v"].requires_grad_()
+    tick = [x[name][0].detach() for name in ("q", "k", "v", "g", "beta")]
+    o, _ = sequence.delta_rule(**x)
+    before = x["state"]._version
+    sequence.delta_rule_step(*tick, x["state"])
+    assert x["state"]._version == before + 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        o.sum().backward()
+    learned = x["state"].clone().requires_grad_()
+    with pytest.raises(ValueError, match="gradients"):
+        sequence.delta_rule_step(*tick, learned)
+    with torch.no_grad():
+        sequence.delta_rule_step(*tick, learned)
+    assert not torch.equal(learned, x["state"])
