@@ -14,6 +14,7 @@ imported before the library is first used: both need the same HIP runtime in
 the process, and the one loaded first is taken.
 """
 import ctypes
+import struct
 
 import torch
 import torch.autograd.function
@@ -64,6 +65,17 @@ class _BlockNormGrad(ctypes.Structure):
     _fields_ += [(n, P) for n in ("d_w_post", "d_w_pre", "d_residual")]
 
 
+# The structs as packed bytes, made of plain numbers in one call each: 2.2 us
+# for a tick's, where nested ctypes objects took 4.1.
+_RULE = struct.Struct("=8If4x29q")
+_RULE_GRAD = struct.Struct("=26q")
+_ROWS = struct.Struct("=4q")
+_NORM = struct.Struct("=Q6If4x19q")
+_NORM_OUT = struct.Struct("=6q")
+_NORM_GRAD = struct.Struct("=18q")
+assert _RULE.size == ctypes.sizeof(_DeltaRule) and _NORM.size == ctypes.sizeof(_BlockNorm)
+assert _RULE_GRAD.size == ctypes.sizeof(_DeltaRuleGrad) and _NORM_GRAD.size == ctypes.sizeof(_BlockNormGrad)
+
 _one_runtime = None
 
 
@@ -83,7 +95,13 @@ def _library():
 
 def _device(names, tensors):
     """The GPU that all tensors are on."""
-    device = None
+    try:
+        index = tensors[0].get_device()  # (half the time of as many comparisons of devices)
+        if index >= 0 and all([t is None or t.get_device() == index for t in tensors]):
+            return tensors[0].device
+    except AttributeError:
+        pass
+    device = None  # which one is not
     for name, t in zip(names, tensors):
         if t is None:
             continue
@@ -136,7 +154,7 @@ def _shape(name, t, shape):
 def _rows(t, one_tick=False):
     """A [ticks][envs][heads][width] (or, gates, [ticks][envs][heads]) tensor; `one_tick`: without the ticks."""
     strides = t.stride()
-    return _Rows(t.data_ptr(), 0, strides[0], strides[1]) if one_tick else _Rows(t.data_ptr(), *strides[:3])
+    return (t.data_ptr(), 0, strides[0], strides[1]) if one_tick else (t.data_ptr(), *strides[:3])
 
 
 class _Call:
@@ -178,17 +196,13 @@ class _Call:
                 raise TypeError("state is %s: float32 is taken" % state.dtype)
         self.q, self.k, self.v, self.g, self.beta = _wide(q), _wide(k), _wide(v), g, beta
         self.state, self.reset = state, reset
-        self.c = c = _DeltaRule(t, n, hq, h, kd, vd, _DTYPES[dtype], _DTYPES[g.dtype], kd ** -0.5 if scale is None else scale,
-                                _rows(self.q, one_tick), _rows(self.k, one_tick), _rows(self.v, one_tick),
-                                _rows(g, one_tick), _rows(beta, one_tick))
+        first = (0, 0, 0)
         if reset is not None:
-            c.reset = reset.data_ptr()
-            if one_tick:
-                c.reset_env = reset.stride(0)
-            else:
-                c.reset_tick, c.reset_env = reset.stride()
-        if state is not None:
-            c.state = state.data_ptr()
+            first = (reset.data_ptr(), 0, reset.stride(0)) if one_tick else (reset.data_ptr(), *reset.stride())
+        self.c = _DeltaRule.from_buffer_copy(_RULE.pack(
+            t, n, hq, h, kd, vd, _DTYPES[dtype], _DTYPES[g.dtype], kd ** -0.5 if scale is None else scale,
+            *_rows(self.q, one_tick), *_rows(self.k, one_tick), *_rows(self.v, one_tick), *_rows(g, one_tick),
+            *_rows(beta, one_tick), 0, 0, 0, 0, *first, 0 if state is None else state.data_ptr(), 0))
 
     def output(self):
         return _like(self.v)
@@ -201,7 +215,8 @@ class _Call:
         """One call over all ticks; `keep`: whether a backward pass follows.  What that reads, and its workspace."""
         L = _library()
         c = self.c
-        c.o, c.state_out = _rows(o), _address(state_out)
+        _ROWS.pack_into(c, _DeltaRule.o.offset, *_rows(o))
+        c.state_out = _address(state_out)
         sizes = _Sizes()
         check(L.mdn_op_delta_rule_sizes(ctypes.byref(c), ctypes.byref(sizes)))
         kept = _buffer(sizes.keep, self.device) if keep else None
@@ -213,7 +228,8 @@ class _Call:
     def step(self, o, state):
         """One tick, which needs no buffers."""
         c = self.c
-        c.o, c.state_out = _rows(o, True), state.data_ptr()
+        _ROWS.pack_into(c, _DeltaRule.o.offset, *_rows(o, True))
+        c.state_out = state.data_ptr()
         check(_library().mdn_op_delta_rule_forward(ctypes.byref(c), None, 0, None, 0, _stream(self.device)))
 
     def backward(self, kept, sizes, d_o, d_state_out, want_state):
@@ -221,7 +237,10 @@ class _Call:
         grads = [_like(x) for x in (self.q, self.k, self.v, self.g, self.beta)]
         d_state = self.states() if want_state else None
         work = _buffer(sizes.backward_workspace, self.device)
-        d = _DeltaRuleGrad(_rows(d_o), _address(d_state_out), *[_rows(x) for x in grads], _address(d_state))
+        dq, dk, dv, dg, db = [_rows(x) for x in grads]
+        d = _DeltaRuleGrad.from_buffer_copy(_RULE_GRAD.pack(
+            *_rows(d_o), 0 if d_state_out is None else d_state_out.data_ptr(), *dq, *dk, *dv, *dg, *db,
+            0 if d_state is None else d_state.data_ptr()))
         check(_library().mdn_op_delta_rule_backward(ctypes.byref(self.c), ctypes.byref(d), _address(kept), sizes.keep,
                                                     _address(work), sizes.backward_workspace, _stream(self.device)))
         return (*grads, d_state)
@@ -345,15 +364,12 @@ class _NormCall:
         self.residual = None if residual_scale is None else residual_scale.contiguous()
         self.shape, self.width, self.rows = shape, width, x.numel() // width
         self.inner = shape[-2] if len(shape) > 1 and self.rows else 1
-        self.c = c = _BlockNorm(self.rows, self.inner, width, _DTYPES[x.dtype], _DTYPES[y.dtype], self.kind,
-                                0 if gate is None else _DTYPES[gate.dtype], eps)
         self.kept = []  # copies that the struct points to
-        c.x, c.y = self.layout(x), self.layout(y)
-        if self.kind == GATE_CHANNEL:
-            c.gate.data = gate.data_ptr()
-        elif self.kind != GATE_NONE:
-            c.gate = self.layout(gate)
-        c.w_post, c.w_pre, c.residual = self.w_post.data_ptr(), self.w_pre.data_ptr(), _address(self.residual)
+        rows = (0, 0, 0) if gate is None else (gate.data_ptr(), 0, 0) if self.kind == GATE_CHANNEL else self.layout(gate)
+        self.c = _BlockNorm.from_buffer_copy(_NORM.pack(
+            self.rows, self.inner, width, _DTYPES[x.dtype], _DTYPES[y.dtype], self.kind, 0 if gate is None else _DTYPES[gate.dtype],
+            eps, *self.layout(x), *self.layout(y), *rows, 0, 0, 0, 0, 0, 0, self.w_post.data_ptr(), self.w_pre.data_ptr(),
+            0 if self.residual is None else self.residual.data_ptr(), 0))
 
     def layout(self, t):
         """The rows of `t`, [..., width or 1], as two strides; another layout is copied."""
@@ -370,45 +386,42 @@ class _NormCall:
                         axes.append((size, stride))
                 if len(axes) <= 1:
                     stride = axes[0][1] if axes else 0
-                    return _NormRows(t.data_ptr(), stride * self.inner, stride)
+                    return t.data_ptr(), stride * self.inner, stride
                 if len(axes) == 2 and axes[1][0] == self.inner:
-                    return _NormRows(t.data_ptr(), axes[0][1], axes[1][1])
+                    return t.data_ptr(), axes[0][1], axes[1][1]
             t = t.contiguous()
             self.kept.append(t)
-        return _NormRows(t.data_ptr(), t.shape[-1] * self.inner, t.shape[-1])
+        return t.data_ptr(), t.shape[-1] * self.inner, t.shape[-1]
 
     def made(self, t):
         """The layout of a contiguous [..., width] tensor."""
-        return _NormRows(t.data_ptr(), self.width * self.inner, self.width)
+        return t.data_ptr(), self.width * self.inner, self.width
 
     def forward(self, keep):
         L = _library()
         s, h = _like(self.x), _like(self.y)
         stats = torch.empty(self.rows, 2, device=self.device) if keep else None
         c = self.c
-        c.s, c.h, c.stats = self.made(s), self.made(h), _address(stats)
+        _NORM_OUT.pack_into(c, _BlockNorm.s.offset, *self.made(s), *self.made(h))
+        c.stats = _address(stats)
         check(L.mdn_op_block_norm_forward(ctypes.byref(c), _stream(self.device)))
         return s, h, stats
 
     def backward(self, stats, d_s, d_h):
         L = _library()
-        c, d = self.c, _BlockNormGrad()
+        c, none = self.c, (0, 0, 0)
         c.stats = _address(stats)
-        if d_s is not None:
-            d.d_s = self.layout(d_s)
-        if d_h is not None:
-            d.d_h = self.layout(d_h)
-        d_x, d_y, d_gate = _like(self.x), _like(self.y), None
-        d.d_x, d.d_y = self.made(d_x), self.made(d_y)
+        d_x, d_y = _like(self.x), _like(self.y)
+        d_gate, gate = None, none
         if self.kind != GATE_NONE:
             d_gate = _like(self.gate)
-            d.d_gate = self.layout(d_gate) if self.kind != GATE_CHANNEL else _NormRows(d_gate.data_ptr(), 0, 0)
+            gate = self.layout(d_gate) if self.kind != GATE_CHANNEL else (d_gate.data_ptr(), 0, 0)
         d_post, d_pre, d_scale = torch.empty(3, self.width, device=self.device).unbind()
-        d.d_w_post, d.d_w_pre = d_post.data_ptr(), d_pre.data_ptr()
         if self.residual is None:
             d_scale = None
-        else:
-            d.d_residual = d_scale.data_ptr()
+        d = _BlockNormGrad.from_buffer_copy(_NORM_GRAD.pack(
+            *(none if d_s is None else self.layout(d_s)), *(none if d_h is None else self.layout(d_h)), *self.made(d_x),
+            *self.made(d_y), *gate, d_post.data_ptr(), d_pre.data_ptr(), 0 if d_scale is None else d_scale.data_ptr()))
         size = ctypes.c_uint64()
         check(L.mdn_op_block_norm_workspace_bytes(ctypes.byref(c), ctypes.byref(size)))
         work = _buffer(size.value, self.device)
