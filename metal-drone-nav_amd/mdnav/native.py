@@ -29,9 +29,9 @@ EXPORTS = [
     "mdn_navwid_write", "mdn_op_actor_forward", "mdn_op_critic_forward", "mdn_op_gaussian_log_prob",
     "mdn_op_sample_loss_and_grad", "mdn_op_adam_update", "mdn_op_ppo_self_tests", "mdn_sim_validate_rollout",
     "mdn_checkpoint_read_params", "mdn_op_normalize_noalloc", "mdn_sim_get_bank", "mdn_sim_set_camera",
-    "mdn_sim_get_camera", "mdn_ppo_grad_norm_summary", "mdn_lppo_grad_norm_summary", "mdn_op_delta_rule_forward", "mdn_op_delta_rule_backward",
-    "mdn_op_delta_rule_sizes",
-    "mdn_op_block_norm_forward", "mdn_op_block_norm_backward", "mdn_op_block_norm_workspace_bytes",
+    "mdn_sim_get_camera", "mdn_ppo_grad_norm_summary", "mdn_lppo_grad_norm_summary", "mdn_op_delta_rule_forward",
+    "mdn_op_delta_rule_backward", "mdn_op_delta_rule_sizes", "mdn_op_block_norm_forward", "mdn_op_block_norm_backward",
+    "mdn_op_block_norm_workspace_bytes",
 ]
 
 P = ctypes.c_void_p
