@@ -209,7 +209,7 @@ class _Call:
 
     def states(self):
         c = self.c
-        return torch.empty(c.envs, c.heads, c.k_dim, c.v_dim, device=self.device)
+        return torch.empty(c.envs, c.heads, c.k_dim, c.v_dim, dtype=torch.float32, device=self.device)
 
     def forward(self, o, state_out, keep):
         """One call over all ticks; `keep`: whether a backward pass follows.  What that reads, and its workspace."""
@@ -400,7 +400,7 @@ class _NormCall:
     def forward(self, keep):
         L = _library()
         s, h = _like(self.x), _like(self.y)
-        stats = torch.empty(self.rows, 2, device=self.device) if keep else None
+        stats = torch.empty(self.rows, 2, dtype=torch.float32, device=self.device) if keep else None
         c = self.c
         _NORM_OUT.pack_into(c, _BlockNorm.s.offset, *self.made(s), *self.made(h))
         c.stats = _address(stats)
@@ -416,7 +416,7 @@ class _NormCall:
         if self.kind != GATE_NONE:
             d_gate = _like(self.gate)
             gate = self.layout(d_gate) if self.kind != GATE_CHANNEL else (d_gate.data_ptr(), 0, 0)
-        d_post, d_pre, d_scale = torch.empty(3, self.width, device=self.device).unbind()
+        d_post, d_pre, d_scale = torch.empty(3, self.width, dtype=torch.float32, device=self.device).unbind()
         if self.residual is None:
             d_scale = None
         d = _BlockNormGrad.from_buffer_copy(_NORM_GRAD.pack(
