@@ -17,6 +17,7 @@ import ctypes
 import struct
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.autograd.function
 
 from .native import MdnError, P, check, lib
@@ -114,6 +115,16 @@ def _device(names, tensors):
         elif t.device != device:
             raise ValueError("%s is on %s, other arguments on %s" % (name, t.device, device))
     return device
+
+
+def _no_tangents(*tensors):
+    """Forward-mode derivatives, which there are none of here: the kernels see a dual tensor's value alone, and a
+    result without a tangent would read as a derivative of zero."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("forward-mode derivatives are not available, only gradients")
 
 
 def _on(device, call, *args):
@@ -288,6 +299,7 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state
     None).  scale: K ** -0.5 if None.  o has v's shape and q's type.  Gradients
     reach every tensor argument but reset; a flagged tick has none for g.
     """
+    _no_tangents(q, k, v, g, beta, state)
     if isinstance(state, torch.Tensor):
         state = state.contiguous()
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, g, beta, state)):
@@ -306,6 +318,7 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None):
     ``delta_rule``.  No gradients: autograd sees ``state`` change, as by any
     operation in place, so a backward pass that still reads the old one raises.
     """
+    _no_tangents(q, k, v, g, beta, state)
     if not isinstance(state, torch.Tensor) or not state.is_contiguous():
         raise ValueError("state is a contiguous tensor: it is advanced in place")
     if state.requires_grad and torch.is_grad_enabled():
@@ -461,6 +474,7 @@ def block_norm(x, y, w_post, w_pre, gate=None, residual_scale=None, eps=1e-6):
     element always, of y's type.  Gradients reach every tensor argument.
     """
     args = (x, y, w_post, w_pre, gate, residual_scale)
+    _no_tangents(*args)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
         return _BlockNormFunction.apply(*args, eps)
     call = _NormCall(*args, eps)

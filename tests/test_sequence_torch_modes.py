@@ -71,3 +71,27 @@ def test_another_default_type_changes_nothing(default_dtype):
         runs.append(outs + list(torch.autograd.grad(outs, leaves, [torch.ones_like(t) for t in outs])))
     for a, b in zip(*runs):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor has a tangent that no result would have: every operator raises for one in any argument,
+    with and without gradients of other arguments, and takes plain tensors at the same level as ever."""
+    import torch.autograd.forward_ad as forward_ad
+    from mdnav import sequence
+    rows, gates, state, weight = torch.zeros(2, 3, 1, 4), torch.zeros(2, 3, 1), torch.zeros(3, 1, 4, 4), torch.ones(4)
+    calls = ((sequence.delta_rule, [rows, rows, rows, gates, gates, state]),
+             (sequence.delta_rule_step, [rows[0], rows[0], rows[0], gates[0], gates[0], state]),
+             (sequence.block_norm, [rows, rows, weight, weight, weight, weight]))
+    for call, args in calls:
+        for i in range(len(args)):
+            for grad in (False, True):
+                with forward_ad.dual_level():
+                    some = [a.clone() for a in args]
+                    some[i - 1].requires_grad_(grad and i > 0)
+                    some[i] = forward_ad.make_dual(some[i], torch.ones_like(some[i]))
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(*some)
+                    with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(*some)
+        with forward_ad.dual_level(), pytest.raises(ValueError, match="GPU"):
+            call(*args)
