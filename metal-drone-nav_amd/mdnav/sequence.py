@@ -7,7 +7,8 @@ Unlike ``ops``, which copies numpy arrays to the device and back, these take
 device tensors as they are, run on torch's current stream and return device
 tensors.  Rows are time-major, [ticks][envs][heads][width], as the rollout
 buffers are; any strides go as long as the width is contiguous, so
-``x.transpose(0, 1)`` of batch-first rows needs no copy.
+``x.transpose(0, 1)`` of batch-first rows needs no copy.  A lazily negated view
+(``is_neg()``, of a conjugate's imaginary part) is to be resolved before.
 
 torch is imported here and nowhere else in the package, and it has to be
 imported before the library is first used: both need the same HIP runtime in
@@ -125,6 +126,12 @@ def _no_tangents(*tensors):
     for t in tensors:
         if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError("forward-mode derivatives are not available, only gradients")
+
+
+def _number(name, x):
+    """Refuses a tensor that wants the gradient which a plain number has none of."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        raise TypeError("%s is a number: it has no gradient" % name)
 
 
 def _on(device, call, *args):
@@ -299,7 +306,8 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state
     None).  scale: K ** -0.5 if None.  o has v's shape and q's type.  Gradients
     reach every tensor argument but reset; a flagged tick has none for g.
     """
-    _no_tangents(q, k, v, g, beta, state)
+    _no_tangents(q, k, v, g, beta, state, scale)
+    _number("scale", scale)
     if isinstance(state, torch.Tensor):
         state = state.contiguous()
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, g, beta, state)):
@@ -318,7 +326,8 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None):
     ``delta_rule``.  No gradients: autograd sees ``state`` change, as by any
     operation in place, so a backward pass that still reads the old one raises.
     """
-    _no_tangents(q, k, v, g, beta, state)
+    _no_tangents(q, k, v, g, beta, state, scale)
+    _number("scale", scale)
     if not isinstance(state, torch.Tensor) or not state.is_contiguous():
         raise ValueError("state is a contiguous tensor: it is advanced in place")
     if state.requires_grad and torch.is_grad_enabled():
@@ -474,7 +483,8 @@ def block_norm(x, y, w_post, w_pre, gate=None, residual_scale=None, eps=1e-6):
     element always, of y's type.  Gradients reach every tensor argument.
     """
     args = (x, y, w_post, w_pre, gate, residual_scale)
-    _no_tangents(*args)
+    _no_tangents(*args, eps)
+    _number("eps", eps)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
         return _BlockNormFunction.apply(*args, eps)
     call = _NormCall(*args, eps)

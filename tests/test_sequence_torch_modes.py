@@ -95,3 +95,20 @@ def test_forward_mode_derivatives_are_refused():
                         call(*some)
         with forward_ad.dual_level(), pytest.raises(ValueError, match="GPU"):
             call(*args)
+
+
+def test_numbers_that_want_gradients_are_refused():
+    """``scale`` and ``eps`` are numbers; a learned one would silently get no gradient."""
+    from mdnav import sequence
+    rows, gates, state, weight = torch.zeros(2, 3, 1, 4), torch.zeros(2, 3, 1), torch.zeros(3, 1, 4, 4), torch.ones(4)
+    learned = torch.tensor(0.5, requires_grad=True)
+    calls = (lambda x: sequence.delta_rule(rows, rows, rows, gates, gates, scale=x),
+             lambda x: sequence.delta_rule_step(rows[0], rows[0], rows[0], gates[0], gates[0], state, scale=x),
+             lambda x: sequence.block_norm(rows, rows, weight, weight, eps=x))
+    for call in calls:
+        with pytest.raises(TypeError, match="is a number"):
+            call(learned)
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+            call(learned)
+        with pytest.raises(ValueError, match="GPU"):
+            call(learned.detach())
