@@ -381,10 +381,14 @@ __device__ __forceinline__ void solve_transposed(Lane l, const System<E, N>& s, 
     mma(r[0], row_half<N>(l, s.inv, CP, P, 0, 0), half_of<E, N>(u[0] - above));
 }
 
-// ---- chunks with infinities or NaN.  A matrix product spreads them: 0 times
-// NaN is NaN, so what a tick may not see (a later tick, an episode before a
-// flag) would reach it.  A chunk where such a value turns up in the products'
-// operands is taken tick by tick instead, by the definition.
+// ---- chunks with infinities or NaN, passed in or made of numbers that grow
+// past fp32 inside the chunk.  A matrix product spreads them: 0 times NaN is
+// NaN, so what a tick may not see (a later tick, an episode before a flag)
+// would reach it.  For the same reason none gets lost on the way: an operand
+// that is not finite leaves a result that is not, in every column whose
+// ticks could meet it, and a mask is a factor of 0.  So the results are looked
+// at, before any is stored, and a chunk where one is not finite is taken tick
+// by tick instead, by the definition.
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 // Whether all are finite and of ordinary size (their sum is).
 __device__ __forceinline__ bool finite(f32x4 x) { return finite((x[0] + x[1]) + (x[2] + x[3])); }

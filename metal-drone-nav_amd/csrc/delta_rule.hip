@@ -178,7 +178,6 @@ template <class E, int D, int N> struct ForwardShared {
     E k[C * STRIDE], q[C * STRIDE], v[C * STRIDE], o[C * STRIDE];
     System<E, N> sys;
     Gates gates[2];  // of this chunk and the next
-    int odd[2];      // whether a chunk has infinities or NaN
 };
 
 // One workgroup per state, a wavefront for each 16 columns of V (at least
@@ -224,7 +223,6 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
 #pragma unroll
         for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
-    if (tid < 2) s.odd[tid] = 0;
     f32x4 state[KT];
     bool flagged = false;  // AHEAD: an episode of the segment has ended, M is 0 whatever comes after
     Piece<E> pk, pq, pv;
@@ -306,7 +304,6 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             }
         }
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0)
-        bool odd = false;
         if (wave < 3) {
             const int i0 = wave ? 16 : 0, j0 = wave == 1 ? 16 : 0;
             f32x4 kk{0, 0, 0, 0}, qk{0, 0, 0, 0};
@@ -319,7 +316,6 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
             }
             if (!FULL) settle(kk, qk);
             const f32x4 d = decay_tile(l, gates, i0, j0);
-            odd = !finite(kk) | !finite(d);
             f32x4 am = four(gates.beta + i0 + 4 * l.quad) * d * kk;
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -358,25 +354,12 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
                 r[i] = four(gates.beta + t) * (r[i] - g * ks[i]);
                 qs[i] *= scale * g;
             }
-            odd |= !finite(r[0] + r[1]);
         }
-        if (__any(odd)) s.odd[turn] = 1;
         __syncthreads();
-        if (tid == 0) s.odd[turn ^ 1] = 0;
-        if (__builtin_amdgcn_readfirstlane(s.odd[turn])) {
-            const uint32_t ticks_here = left < uint32_t(C) ? left : uint32_t(C);
-#pragma unroll 1
-            for (uint32_t t = 0; t < ticks_here && 16 * wave < int(cols); t++) {
-                const E* k = s.k + t * ST;
-                decay_state(state, gates, t);
-                const float v = float(s.v[t * ST + 16 * wave + l.col]);
-                add_outer(l, state, k, gates.beta[t] * (v - column_dot(l, state, k)));
-                if (!AHEAD) {
-                    const float o = scale * column_dot(l, state, s.q + t * ST);
-                    if (l.quad == 0) s.o[t * ST + 16 * wave + l.col] = E(o);
-                }
-            }
-        } else if (16 * wave < int(cols)) {
+        // the columns' outputs and what they add to the state; where one of
+        // these is not finite, the chunk by the definition
+        bool odd = false;
+        if (16 * wave < int(cols)) {
             solve(l, s.sys, r, u);
             // o = scale gamma (q S) + scores u
             if (!AHEAD) {
@@ -384,13 +367,41 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) mma(qs[i], col_frag<N>(l, s.sys.scores, CP, System<E, N>::PLANE, 0, 16 * i), uf);
             }
+            f32x4 sum = qs[0] + qs[1];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int t = 16 * i + 4 * l.quad;
 #pragma unroll
                 for (int e = 0; e < 4 && !AHEAD; e++) s.o[(t + e) * ST + 16 * wave + l.col] = E(qs[i][e]);
                 u[i] *= four(gates.after + t);
+                sum += u[i];
             }
+            odd = __any(!finite(sum));
+            asm volatile("" : "+v"(u[0]), "+v"(u[1]));  // (kept as they are, or three-term instances spill)
+        }
+        if (__builtin_expect(odd, 0)) {
+            // (copied, or the products' registers would follow this loop's order)
+            f32x4 sx[KT];
+#pragma unroll
+            for (int i = 0; i < KT; i++) {
+                sx[i] = state[i];
+                asm volatile("" : "+v"(sx[i]));
+            }
+            const uint32_t ticks_here = left < uint32_t(C) ? left : uint32_t(C);
+#pragma unroll 1
+            for (uint32_t t = 0; t < ticks_here; t++) {
+                const E* k = s.k + t * ST;
+                decay_state(sx, gates, t);
+                const float v = float(s.v[t * ST + 16 * wave + l.col]);
+                add_outer(l, sx, k, gates.beta[t] * (v - column_dot(l, sx, k)));
+                if (!AHEAD) {
+                    const float o = scale * column_dot(l, sx, s.q + t * ST);
+                    if (l.quad == 0) s.o[t * ST + 16 * wave + l.col] = E(o);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < KT; i++) state[i] = sx[i];
+        } else if (16 * wave < int(cols)) {
             // S <- gamma_C S + K^T u
             const float total = gates.before[C - 1];
             const auto uf = frag_of<E, N>(u[0], u[1]);
