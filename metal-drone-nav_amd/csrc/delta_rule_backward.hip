@@ -43,7 +43,7 @@ template <class E, int D> struct BackwardShared {
     // inv and scores give their places to E = beta D dA and to scale D dP
     System<E> sys;
     Gates gates[2];  // of this chunk and the next
-    int odd[2];      // whether a chunk has infinities or NaN
+    int odd;         // whether the chunk has results that are not finite
     float odd_sums[2][W];
     __align__(16) float beta_v[W][C], a[W][C], b[W][C], dot[W];
     double m_row[3][16], m_col[3][16];
@@ -109,7 +109,6 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
 #pragma unroll
         for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
-    if (tid < 2) s.odd[tid] = 0;
     f32x4 g[KT], st[KT];  // G and S, K x 16, in result layout
     Piece<E> pk, pq, pv, po;
     const auto fetch = [&](const At& at) {
@@ -201,7 +200,6 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
         // the chunk's scores and A: tiles (0,0), (1,1), (1,0), kept by their wavefronts
         f32x4 dec = zero, kk = zero, pm = zero, am = zero;
         const int i0 = wave ? 16 : 0, j0 = wave == 1 ? 16 : 0;
-        bool odd = false;
         if (wave < 3) {
             f32x4 qk = zero;
 #pragma unroll
@@ -213,7 +211,6 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             }
             if (!FULL) settle(kk, qk);
             dec = decay_tile(l, gates, i0, j0);
-            odd = !finite(kk + qk) | !finite(dec) | !finite(four(gates.beta + i0 + 4 * l.quad));
             kk *= dec;
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -264,14 +261,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 dr[i] = four(gates.beta + t) * x[i];
             }
         }
-        if (v_wave) {
-            const auto of = ordered_col(l, s.d_o, ST, 16 * wave);
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) sum += first_term(of, e);
-            odd |= !finite(du[0] + du[1]) | !finite(x[0] + x[1]) | !finite(sum);
-        }
-        if (__any(odd)) s.odd[turn] = 1;
+        bool odd = false;  // a result is not finite
         if (!AHEAD) {
             float dot = 0.0f;
 #pragma unroll
@@ -280,12 +270,20 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 for (int r = 0; r < 4; r++) dot = fmaf(st[i][r], g[i][r], dot);
             dot = sum_rows32(sum_rows16(sum16(dot)));
             if (lane == 0) s.dot[wave] = dot;
+            odd = !finite(dot);
         }
         __syncthreads();
+        if (!AHEAD && tid == 0) s.odd = 0;
 
-        if (tid == 0) s.odd[turn ^ 1] = 0;
-        if (__builtin_amdgcn_readfirstlane(s.odd[turn])) {
-            // by the definition, from the chunk's last tick to its first
+        // The chunk by the definition, from its last tick to its first; G in a
+        // copy, or the products' registers would follow this loop's order.
+        const auto by_definition = [&] {
+            f32x4 gx[KT];
+#pragma unroll
+            for (int i = 0; i < KT; i++) {
+                gx[i] = g[i];
+                asm volatile("" : "+v"(gx[i]));
+            }
             KernelCall* call_now = fresh_call();
             float* const parts = reinterpret_cast<float*>(s.u);  // [wavefront][d_q, d_k][K]
 #pragma unroll 1
@@ -310,8 +308,8 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                         error = float(s.v[t * ST + 16 * wave + l.col]) - column_dot(l, st, k);
                     }
                     const float u = beta * error;
-                    add_outer(l, g, q, scale * o);
-                    const float du = column_dot(l, g, k), dv = beta * du;
+                    add_outer(l, gx, q, scale * o);
+                    const float du = column_dot(l, gx, k), dv = beta * du;
                     float dg = 0.0f;
 #pragma unroll
                     for (int i = 0; i < KT && !AHEAD; i++) {
@@ -320,8 +318,8 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             pq[r] = sum16(scale * fmaf(kr[r], u, st[i][r]) * o);
-                            pk[r] = sum16(g[i][r] * u - st[i][r] * dv);
-                            dg = fmaf(fmaf(-kr[r], dv, g[i][r]), st[i][r], dg);
+                            pk[r] = sum16(gx[i][r] * u - st[i][r] * dv);
+                            dg = fmaf(fmaf(-kr[r], dv, gx[i][r]), st[i][r], dg);
                         }
                         if (l.col == 0) {
                             *reinterpret_cast<f32x4*>(parts + (2 * wave) * D + 16 * i + 4 * l.quad) = pq;
@@ -329,11 +327,11 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                         }
                         asm volatile("" : "+v"(dg)::"memory");
                     }
-                    add_outer(l, g, k, -dv);
+                    add_outer(l, gx, k, -dv);
 #pragma unroll
                     for (int i = 0; i < KT; i++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) g[i][r] = flag ? 0.0f : g[i][r] * decay;
+                        for (int r = 0; r < 4; r++) gx[i][r] = flag ? 0.0f : gx[i][r] * decay;
                     if (!AHEAD) {
                         dg = sum_rows32(sum_rows16(sum16(dg)));
                         const float db = sum16(16 * wave + l.col < vd ? du * error : 0.0f);
@@ -368,19 +366,9 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 }
                 __syncthreads();
             }
-            __syncthreads();
-            if (next.job < plan.total) {
-                put_rows(next);
-                if (!AHEAD) fetch_state(next);
-            }
-            if (now.c == now.first) leave(now, g);
-            if (!FULL) clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
-            __syncthreads();
-            now = next;
-            next = later;
-            later.back(plan, which);
-            continue;
-        }
+#pragma unroll
+            for (int i = 0; i < KT; i++) g[i] = gx[i];
+        };
 
         // U and R
         f32x4 dv[2];
@@ -404,6 +392,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 dv[i] = four(gates.beta + 16 * i + 4 * l.quad) * dr[i];
                 dr[i] = dv[i] * four(gates.before + 16 * i + 4 * l.quad);  // from here on gamma beta R
                 if (!AHEAD && l.col == 0) *reinterpret_cast<f32x4*>(&s.beta_v[wave][16 * i + 4 * l.quad]) = sum;
+                odd |= !finite(dr[i] + sum);
             }
         }
         __syncthreads();
@@ -434,7 +423,10 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             for (int i = 0; i < KT && !FULL; i++) settle(g[i]);
         };
         if constexpr (AHEAD) {
-            step_back();
+            if (__builtin_expect(__any(odd), 0))
+                by_definition();
+            else
+                step_back();
             // all have read k, q and d_o, and the matrices
             __syncthreads();
             if (next.job < plan.total) put_rows(next);
@@ -469,6 +461,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
             }
             dp *= scale * dec;
             da *= four(gates.beta + i0 + 4 * l.quad) * dec;
+            odd |= !finite(float(m_col)) | !finite(b);
             if (l.col == 0) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) s.m_row[wave][4 * l.quad + r] = m_row[r];
@@ -544,6 +537,7 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                     pa[e] = sum16(fmaf(qv, dq[i][e], kv * dk[i][e]));
                     pb[e] = sum16(kv * dkg[i][e]);
                 }
+                odd |= !finite(pa + pb);
                 dk[i] += dkg[i];
                 if (l.col == 0) {
                     *reinterpret_cast<f32x4*>(&s.a[wave][16 * i + 4 * l.quad]) = pa;
@@ -564,9 +558,26 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 mma(dk[i], er, kf);
                 mma(dk[i], ec, kf);
             }
+            odd |= !finite((dq[0] + dq[1]) + (dk[0] + dk[1]));
+        }
+        if (__any(odd)) s.odd = 1;
+        __syncthreads();
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(s.odd), 0)) {
+            by_definition();
+            __syncthreads();
+            if (next.job < plan.total) {
+                put_rows(next);
+                fetch_state(next);
+            }
+            if (now.c == now.first) leave(now, g);
+            if (!FULL) clear_lds(s.u, sizeof(s.u) + sizeof(s.r) + sizeof(s.through));
+            __syncthreads();
+            now = next;
+            next = later;
+            later.back(plan, which);
+            continue;
         }
         step_back();
-        __syncthreads();
         // the rows' gradients, through LDS to whole rows
 #pragma unroll
         for (int i = 0; i < 2; i++)
@@ -601,14 +612,14 @@ __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
                 put_gate<E>(fresh_call(), now, now.c * C + t, dg, beta);
             }
         }
-        // the next chunk's rows and S are waited for before this one's gradients
-        // leave: loads and stores are counted in order, and the loads would
-        // wait for the stores
+        __syncthreads();
+        // all have read k, q and d_o.  The next chunk's rows and S are waited for
+        // before this one's gradients leave: loads and stores are counted in
+        // order, and the loads would wait for the stores
         if (next.job < plan.total) put_rows(next);
 #pragma unroll
         for (int i = 0; i < KT; i++) asm volatile("" : "+v"(st[i]));
         asm volatile("" : "+v"(gate.g), "+v"(gate.beta), "+v"(gate.flag));
-        __syncthreads();
         KernelCall* k = fresh_call();
         const uint32_t hg = k->d.partial ? now.h : now.hq;
         if (on_k.on && on_k.row < left) {

@@ -1,5 +1,5 @@
 """The gated delta rule where finite inputs outgrow fp32: an infinity that arises inside a rollout reaches later
-ticks of its episode and nothing else.
+ticks of its episode (in reverse, earlier ones) and nothing else.
 
 The definition is taken in float64, where the same numbers stay finite; ticks that fp32 has left are not compared, all
 others are, tick by tick in their own norm.  Tolerances as in test_sequence_ops.py, whose bounds hold for every row."""
@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch  # before the library: one HIP runtime in the process
 
-from test_sequence_ops import NORM, TORCH, host, inputs, rule
+from test_sequence_ops import NORM, TORCH, host, inputs, rule, rule_gradients
 
 gpu = pytest.mark.gpu
 
@@ -82,3 +82,27 @@ def test_values_that_outgrow_fp32_stay_in_their_episode(shape, dtype, final):
         groups_near("o", o, want_o, env, each(*spans), dtype)
         if final:
             groups_near("state", last[None], want_s[None], env, each((0, 1)), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_gradients_that_outgrow_fp32_stay_in_their_episode(shape, dtype):
+    from mdnav import sequence
+    print("case: overflow gradients", shape, dtype, flush=True)
+    x, d_o, first = growing(shape, dtype)
+    leaves = {name: x[name].requires_grad_() for name in ("q", "k", "v", "g", "beta", "state")}
+    o, _ = sequence.delta_rule(**x)
+    got = dict(zip(leaves, torch.autograd.grad([o], list(leaves.values()), [d_o])))
+    want = rule_gradients(**host(x), d_o=d_o.double().cpu().numpy(), d_state=None)
+    t, turn = shape[0], first + FLAG + 6  # past the tick with the large query or gradient
+    for env in range(6):
+        spans = [(first + FLAG, turn), (turn, t)] + ([(0, first)] if first else [])
+        if env >= 4:
+            spans += [(first, first + 2), (first + 2, first + FLAG)]
+        # a group's norm, as a row can be a small difference of its neighbours: in one here (env 3, the flagged tick
+        # of the 40 x 72 heads) the definition itself, in fp32, is 3.8e-5 of the row's own norm away
+        for name in ("q", "k", "v", "g", "beta"):
+            groups_near("d_" + name, got[name], want[name], env, [slice(*s) for s in spans], dtype)
+        if first or env >= 4:
+            groups_near("d_state", got["state"][None], want["state"][None], env, each((0, 1)), dtype)
