@@ -34,7 +34,7 @@ struct Args {
     // function of the one the last segment began with, S' = M S + B.
     uint32_t segments, segment;
     float* seg_states;        // [state][segments][k][v]: B of the segment before (the first has the state), then the state before the segment
-    float* seg_moves;         // [state][segments][k][k]: M
+    float* seg_moves;         // [state][segments][k][k]: M; then [state][segments] words, 1 where an episode's first tick is in the segment
     float* seg_grads;         // [state][segments][k][v]: the same for the state's gradient after the segment
 };
 
@@ -62,7 +62,10 @@ inline uint64_t seg_state_words(const Args& a) {
     return a.segments > 1 ? uint64_t(a.envs) * a.heads * a.segments * a.k_dim * a.v_dim : 0;
 }
 inline uint64_t seg_move_words(const Args& a) {
-    return a.segments > 1 ? uint64_t(a.envs) * a.heads * a.segments * a.k_dim * a.k_dim : 0;
+    return a.segments > 1 ? uint64_t(a.envs) * a.heads * a.segments * (uint64_t(a.k_dim) * a.k_dim + 1) : 0;
+}
+inline __host__ __device__ uint32_t* seg_flags(float* moves, uint32_t states, uint32_t segments, uint32_t k_dim) {
+    return reinterpret_cast<uint32_t*>(moves + uint64_t(states) * segments * k_dim * k_dim);
 }
 
 // chunk_states keeps result tiles as they are in registers: of each state and

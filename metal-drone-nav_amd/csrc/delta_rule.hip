@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
         for (int i = 0; i < 4; i++) m[(16 + l.col) * CP + 4 * l.quad + i] = E(0.0f);
     }
     f32x4 state[KT];
-    bool flagged = false;  // AHEAD: an episode of the segment has ended, M is 0 whatever comes after
+    bool flagged = false;  // AHEAD: an episode has begun in the segment, nothing of the state before it is left
     Piece<E> pk, pq, pv;
     const auto fetch = [&](const At& at) {
         KernelCall* k = fresh_call();
@@ -423,15 +423,13 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
                            piece_from_lds(s.o + on_v.row * ST + on_v.col));
         if (AHEAD) flagged = (now.c > now.first && flagged) | (__builtin_amdgcn_readfirstlane(gates.episode[C - 1]) != 0);
         if (now.c + 1 == now.end) {
-            if (AHEAD && now.part && flagged)
-#pragma unroll
-                for (int i = 0; i < KT; i++) state[i] = f32x4{0, 0, 0, 0};
             KernelCall* k = fresh_call();
             float* p = now.seg + 1 == plan.segments ? k->a.state_out : nullptr;
             if (p) p += uint64_t(now.state) * kd * vd;
             const uint64_t slot = uint64_t(now.state) * plan.segments + now.seg;
             if (AHEAD) p = now.part ? k->a.seg_moves + slot * kd * kd : k->a.seg_states + (slot + 1) * kd * vd;
             if (p) store_state(p, state, kd, cols, l, 16 * wave + l.col);
+            if (AHEAD && now.part && tid == 0) seg_flags(k->a.seg_moves, k->a.envs * k->a.heads, plan.segments, kd)[slot] = flagged;
             if (next.job < plan.total) fetch_state(next);
         }
         now = next;
@@ -465,7 +463,9 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
         return x;
     };
     f32x4 m[D / 16];
+    uint32_t flagged = 0;  // M is not looked at: what is before the flag is gone, NaN too, which M = 0 would not end
     const auto fetch = [&](uint32_t s) {
+        flagged = seg_flags(a.seg_moves, a.envs * a.heads, a.segments, kd)[uint64_t(state) * a.segments + s];
         const float* p = moves + uint64_t(s) * kd * kd;
         const int r = 16 * wave + l.col;
         if (!TRANSPOSED && kd % 4 == 0) {  // four neighbours in one word: 102 us and not 244
@@ -496,11 +496,7 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
     __syncthreads();
     for (uint32_t left = a.segments - 2, turn = 0; left > 0; left--, turn ^= 1) {
         Frag<E, N> mf[D / 32];
-        bool moved = false;
-#pragma unroll
-        for (int k = 0; k < D / 16; k++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) moved |= m[k][e] != 0.0f;
+        const bool moved = __builtin_amdgcn_readfirstlane(flagged) == 0;
 #pragma unroll
         for (int k = 0; k < D / 32; k++) mf[k] = frag_of<E, N>(m[2 * k], m[2 * k + 1]);
         s = TRANSPOSED ? s - 1 : s + 1;
@@ -509,8 +505,7 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
             fetch(s);
             next = load_tile(TRANSPOSED ? s - 1 : s + 1);
         }
-        // (a segment with an episode's first tick has M = 0, whatever came before it)
-        if (__any(moved))
+        if (moved)
 #pragma unroll
             for (int k = 0; k < D / 32; k++) mma(y, mf[k], row_frag<N>(l, last[turn], ST, PL, 0, 32 * k));
 #pragma unroll
