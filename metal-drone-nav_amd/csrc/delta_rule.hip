@@ -505,9 +505,21 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
             fetch(s);
             next = load_tile(TRANSPOSED ? s - 1 : s + 1);
         }
-        if (moved)
+        if (moved) {
+            // a column of zeros stays one, also where M has outgrown fp32
+            const f32x4 own = y;
+            bool some = false;
 #pragma unroll
-            for (int k = 0; k < D / 32; k++) mma(y, mf[k], row_frag<N>(l, last[turn], ST, PL, 0, 32 * k));
+            for (int k = 0; k < D / 32; k++) {
+                const Frag<E, N> x = row_frag<N>(l, last[turn], ST, PL, 0, 32 * k);
+#pragma unroll
+                for (int e = 0; e < 8; e++) some |= first_term(x, e) != 0.0f;
+                mma(y, mf[k], x);
+            }
+            const float any = sum_rows32(sum_rows16(some ? 1.0f : 0.0f));
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] = any != 0.0f ? y[r] : own[r];
+        }
 #pragma unroll
         for (int r = 0; r < 4; r++)
             if (16 * wave + 4 * l.quad + r < kd && int(col) < vd) *tile_at(s, r) = y[r];

@@ -183,8 +183,8 @@ template <> struct Make<float, 1> {
 template <class E, int N = Kind<E>::MID> __device__ __forceinline__ Frag<E, N> frag_of(f32x4 x, f32x4 y) { return Make<E, N>::frag(x, y); }
 template <class E, int N = Kind<E>::MID> __device__ __forceinline__ Half<E, N> half_of(f32x4 x) { return Make<E, N>::half(x); }
 
-// Element e of an operand of caller's rows.
-__device__ __forceinline__ float first_term(const Frag<bf16, 1>& f, int e) { return float(f.t[0][e]); }
+// Element e of an operand (of a computed one, its first term).
+template <int N> __device__ __forceinline__ float first_term(const Frag<bf16, N>& f, int e) { return float(f.t[0][e]); }
 __device__ __forceinline__ float first_term(const Frag<float, 1>& f, int e) { return f.t[e >> 2][e & 3]; }
 
 // ---- LDS to operands.  `m` is a matrix with rows `stride` elements apart.

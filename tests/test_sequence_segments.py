@@ -54,3 +54,37 @@ def test_nan_outlives_decays_in_reverse(shape, dtype):
     assert np.isnan(want["v"][0, 1, 0, 1]) and np.isfinite(want["v"][:, 0]).all()
     for (name, _), grad in zip(leaves.items(), got):
         same_where_finite("d_" + name, grad, want[name], dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES + [(100, 4, 1, 1, 64, 64), (12, 4, 1, 2, 40, 24)], ids=str)
+def test_a_map_that_outgrows_fp32_leaves_zeros_alone(shape, dtype):
+    """Keys of length 10 multiply what a state holds by 99 a tick: a segment's map overflows, but columns with
+    nothing in them stay empty, and so do their gradients."""
+    from mdnav import sequence
+    print("case: growing maps", shape, dtype, flush=True)
+    t, n, hq, h, kd, vd = shape
+    x = inputs(*shape, dtype, seed=32, resets=0, gates=dtype)
+    x["k"][:, 1] *= 10.0
+    x["beta"][:, 1] = 1.0
+    x["g"][:, 1] = 0.0
+    for name in ("v", "state"):
+        (x[name][:, 1] if name == "v" else x[name][1])[...] = 0.0
+    x["v"][t // 2, 1, 0, 5] = 1.0  # one column overflows after this
+    leaves = {name: x[name].requires_grad_() for name in ("q", "k", "v", "g", "beta", "state")}
+    o, last = sequence.delta_rule(**x, final_state=True)
+    others = [c for c in range(vd) if c != 5]
+    assert not o[:, 1][..., others].any() and not last[1][..., others].any()
+    assert not o[:t // 2, 1].any()
+    d_o = torch.randn(x["v"].shape, generator=torch.Generator().manual_seed(2)).to(TORCH[dtype]).cuda()
+    d_o[:, 1] = 0.0
+    x["v"].data[t // 2, 1, 0, 5] = 0.0
+    o, last = sequence.delta_rule(**x)
+    assert not o[:, 1].any()
+    got = dict(zip(leaves, torch.autograd.grad([o], list(leaves.values()), [d_o])))
+    want = rule_gradients(**host(x), d_o=d_o.double().cpu().numpy(), d_state=None)
+    for name, grad in got.items():
+        here = grad[1] if name == "state" else grad[:, 1]
+        assert not here.any(), name
+        same_where_finite("d_" + name, grad, want[name], dtype)
