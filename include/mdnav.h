@@ -425,8 +425,25 @@ typedef struct MdnRows {
  * g is the logarithm of the decay (-inf allowed) and beta the strength of the
  * write.  qk_heads divides heads: value head h reads query and key head
  * h / (heads / qk_heads).  k_dim and v_dim are 1..128, ticks and envs may be
- * 0 (the state then passes through).  An infinity or NaN reaches what the
- * formulas bring it to, later ticks of its episode, and nothing else. */
+ * 0 (the state then passes through).
+ *
+ * The state is held in fp32, and fp32 rows are multiplied in fp32.  With
+ * bfloat16 rows, calls of more than a few ticks (mdn_op_delta_rule_forward
+ * takes chunks of 32) multiply what they compute, the state among it, as sums
+ * of bfloat16 values: of three, which is all of fp32, where state_out is
+ * asked for, else of two, 16 to 17 bits (4e-6 of the results' norm, below
+ * their own rounding to bfloat16; a rounding can fall on the other side, so o
+ * has not the same last bits with state_out and without).  The backward pass
+ * takes two, in its fp32 results too: d_state, and d_g and d_beta of fp32
+ * gates.  Decays are exp(g) to a relative error of |g| 2^-24.
+ *
+ * An infinity or NaN, passed in or risen inside, reaches what the formulas
+ * bring it to, later ticks of its episode, and nothing else.  A g below -104,
+ * whose exp is 0 in fp32, ends an episode as reset does, whatever the state
+ * holds.  Few long states are worked on in segments of 128 ticks or more: a
+ * segment over which keys and strengths multiply a state past fp32
+ * (beta |k|^2 above 2, tick after tick) leaves NaN in columns of the state
+ * that are not all zeros, and in reverse in those of its gradient. */
 typedef struct MdnDeltaRule {
     uint32_t ticks, envs, qk_heads, heads, k_dim, v_dim;
     uint32_t dtype;       /* of q, k, v and o: MDN_F32 or MDN_BF16 */

@@ -305,6 +305,13 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state
     bool.  state: [envs][heads][K][V] float32 before the first tick (zeros if
     None).  scale: K ** -0.5 if None.  o has v's shape and q's type.  Gradients
     reach every tensor argument but reset; a flagged tick has none for g.
+
+    The state is held in 32 bits.  Products of float32 rows are float32; with
+    bfloat16 rows the state and what else is computed enter products with 16
+    to 17 bits, with all 24 where ``final_state`` is asked for (o then differs
+    by roundings to bfloat16 that fall on the other side), and gradients with
+    16 to 17, those in float32 (state, float32 g and beta) too.  A g below
+    -104 clears the state as ``reset`` does.
     """
     _no_tangents(q, k, v, g, beta, state, scale)
     _number("scale", scale)
