@@ -41,14 +41,16 @@ struct Args {
 // The segments.  Each costs its chunks three times (B, M and the outputs) but
 // for the first, and the join: that pays while most compute units would idle.
 // In one piece against cut, in us, bf16, forward and forward with backward:
-//   2 states 128 x 128:   512 ticks 75 : 54 and 301 : 231, 4,096 ticks 553 : 136 and 2,215 : 284
-//   64 states 128 x 128:  512 ticks 79 : 81 and 307 : 234, 4,096 ticks 585 : 351 and 2,340 : 1,121
-//   128 states 128 x 128: 512 ticks 80 : 120 and 316 : 360, 1,024 ticks 151 : 176 and 610 : 591,
-//                         4,096 ticks 615 : 527 and 2,437 : 1,943
-//   128 states 64 x 64:   512 ticks 62 : 64 and 226 : 231, 1,024 ticks 114 : 96 and 391 : 253
-//   170 states 128 x 128: 4,096 ticks 631 : 576 and 2,532 : 2,439, 1,024 ticks 152 : 191 and 631 : 714
+//   2 states 128 x 128:   512 ticks 77 : 51 and 280 : 184, 4,096 ticks 607 : 130 and 2,222 : 270
+//   64 states 128 x 128:  512 ticks 81 : 79 and 312 : 209, 4,096 ticks 705 : 378 and 2,530 : 1,177
+//   128 states 128 x 128: 512 ticks 96 : 130 and 332 : 363, 1,024 ticks 187 : 196 and 666 : 610,
+//                         4,096 ticks 725 : 592 and 2,680 : 2,033
+//   128 states 64 x 64:   512 ticks 58 : 60 and 213 : 182, 1,024 ticks 142 : 100 and 423 : 262
+//   170 states 128 x 128: 1,024 ticks 191 : 260 and 689 : 814, 4,096 ticks 756 : 839 and 2,803 : 2,853
 // So: up to 128 states, at least four segments of at least four chunks each, and
-// of sixteen where there are more than 64 states of wide heads.
+// of sixteen where there are more than 64 states of wide heads.  (170 states 64 x
+// 64, of which a compute unit holds several, would gain too: 1,024 ticks 145 :
+// 116 and 441 : 344.)
 inline void cut(Args& a) {
     const uint32_t states = a.envs * a.heads, chunks = (a.ticks + CHUNK - 1) / CHUNK;
     const uint32_t least = states > 64 && (a.k_dim > 64 || a.v_dim > 64) ? 16 : 4;  // chunks of a segment
@@ -112,16 +114,27 @@ hipError_t launch_join_grads(const Args& a, bool bf16, hipStream_t stream);
 // The ticks up to which the recurrent kernel is taken.  It reads and writes a
 // state as fast as a copy does but works its ticks off on the vector units; the
 // chunk kernel costs much the same for 1 tick and 16, more in fp32 and where
-// heads do not fill its tiles.  Recurrent against chunks, in us:
-//   bf16, 16,384 states 64 x 64:  1 tick 106 : 173, 4 ticks 131 : 160, 6 ticks 153 : 161, 8 ticks 173 : 162
-//   bf16, 8,192 states 128 x 128: 1 tick 204 : 259, 4 ticks 231 : 243, 6 ticks 266 : 246
-//   bf16, 4,096 states 91 x 87:   1 tick 74 : 160, 8 ticks 127 : 188, 12 ticks 163 : 200
-//   bf16, 16,384 states 32 x 32:  1 tick 30 : 153, 12 ticks 99 : 155
-//   fp32, 16,384 states 64 x 64:  1 tick 104 : 248, 8 ticks 164 : 252, 12 ticks 203 : 257
-//   fp32, 8,192 states 128 x 128: 1 tick 202 : 397, 8 ticks 310 : 400, 12 ticks 394 : 406
+// heads do not fill its tiles.  Recurrent against chunks, in us, with a final
+// state : without one:
+//   bf16, 16,384 states 64 x 64:   1 tick 108 : 161 and 51 : 108, 4 ticks 137 : 165 and 93 : 109, 8 ticks 187 : 168 and 141 : 111
+//   bf16, 8,192 states 128 x 128:  1 tick 207 : 251 and 97 : 147, 4 ticks 254 : 255 and 174 : 153, 6 ticks 297 : 257 and 219 : 157
+//   bf16, 8,192 states 128 x 64:   4 ticks 140 : 171 and 95 : 120, 8 ticks 185 : 173 and 144 : 120, 12 ticks 236 : 175 and 195 : 121
+//   bf16, 16,384 states 64 x 32:   4 ticks 84 : 132 and 65 : 90, 6 ticks 105 : 133 and 86 : 90
+//   bf16, 8,192 states 128 x 32:   8 ticks 104 : 154 and 79 : 111, 12 ticks 132 : 156 and 107 : 113
+//   bf16, 8,192 states 64 x 128:   8 ticks 182 : 326 and 138 : 250, 12 ticks 231 : 329 and 186 : 251
+//   bf16, 8,192 states 96 x 96:    8 ticks 221 : 399 and 179 : 305, 12 ticks 289 : 400 and 248 : 307
+//   bf16, 4,096 states 91 x 87:    8 ticks 141 : 205 and 111 : 167, 12 ticks 181 : 208 and 150 : 168
+//   bf16, 16,384 states 48 x 48:   8 ticks 175 : 233 and 142 : 140, 12 ticks 224 : 237 and 191 : 143
+//   bf16, 16,384 states 32 x 32:   8 ticks 98 : 177 and 91 : 122, 12 ticks 136 : 179 and 128 : 123
+//   fp32, 16,384 states 64 x 64:   8 ticks 169 : 255 and 125 : 223, 12 ticks 206 : 259 and 166 : 226
+//   fp32, 8,192 states 128 x 128:  8 ticks 324 : 400 and 231 : 323, 12 ticks 407 : 405 and 313 : 327
+// (calls in a row, each with inputs of its own, as all sides of choices here).
+// So in bfloat16, where a state's rows fill the tiles and its columns half of
+// them, 4; in other heads of up to 64 without a final state 8; else 12.
 inline uint32_t recurrent_ticks(const Args& a, bool bf16) {
-    const bool full = a.k_dim == a.v_dim && (a.k_dim == 64 || a.k_dim == 128);
-    return bf16 && full ? 4 : 12;
+    if (!bf16) return 12;
+    if ((a.k_dim == 64 || a.k_dim == 128) && a.v_dim <= a.k_dim && 2 * a.v_dim >= a.k_dim) return 4;
+    return a.k_dim <= 64 && a.v_dim <= 64 && !a.state_out ? 8 : 12;
 }
 hipError_t launch_recurrent(const Args& a, bool bf16, hipStream_t stream);
 hipError_t launch_forward(const Args& a, bool bf16, hipStream_t stream);

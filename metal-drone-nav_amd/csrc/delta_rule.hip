@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
         flagged = seg_flags(a.seg_moves, a.envs * a.heads, a.segments, kd)[uint64_t(state) * a.segments + s];
         const float* p = moves + uint64_t(s) * kd * kd;
         const int r = 16 * wave + l.col;
-        if (!TRANSPOSED && kd % 4 == 0) {  // four neighbours in one word: 102 us and not 244
+        if (!TRANSPOSED && kd % 4 == 0) {  // four neighbours in one word: a call of 16 states 128 x 128 of 30,011 ticks 785 us and not 986
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
                 const int c = 16 * k + 4 * l.quad;
@@ -552,10 +552,11 @@ hipError_t forward(const Args& a, hipStream_t stream) {
     return chunks<E, N, D, FULL, false>(a, stream);
 }
 // FULL: heads as wide as the kernel's tiles, without the branches for narrower
-// ones.  With it and without, in us: 32,768 states 64 x 64 of 32 ticks in bfloat16
-// 279 : 288 and backward 844 : 971, in fp32 498 : 512 and 1,362 : 1,502; 5,120
-// states 128 x 128 of 64 ticks in bfloat16 224 : 230 and 649 : 764, in fp32 424 :
-// 459 and 1,388 : 1,369.
+// ones.  With it and without, in us, forward and forward with backward: 32,768
+// states 64 x 64 of 32 ticks in bfloat16 264 : 264 and 997 : 1,114, in fp32 472 : 505
+// and 1,822 : 2,544 (without it also S and G whole, not in halves); 5,120 states 128 x
+// 128 of 64 ticks in bfloat16 188 : 196 and 807 : 905, in fp32 406 : 423 and 1,547 :
+// 1,839.
 template <class E, int N, int D>
 hipError_t forward(const Args& a, hipStream_t stream) {
     return a.k_dim == D && a.v_dim == D ? forward<E, N, D, true>(a, stream) : forward<E, N, D, false>(a, stream);
@@ -566,12 +567,18 @@ hipError_t forward(const Args& a, hipStream_t stream) {
 }
 
 // Wavefronts of 32 columns have room for 128 rows, those of 64 for 64; in heads
-// of at most 32 columns half the lanes of the wider ones would idle (a tick of
-// 16,384 states 32 x 32: 20 us in narrow ones, 31 in wide ones; of 18,006 states
-// 40 x 72, two wide or three narrow ones each: 63 us in wide ones, 75 in narrow ones).
+// of at most 32 columns half the lanes of the wider ones would idle.  A tick in
+// place in narrow : wide ones, in us: 16,384 states 32 x 32 in bf16 36 : 62,
+// in fp32 37 : 56; 64 x 64 in bf16 105 : 118, in fp32 111 : 110; 18,006 states 48 x 48
+// in bf16 90 : 103, in fp32 99 : 96; of 40 x 72 128 : 125 and 144 : 107; 12,000 of 64 x 96
+// 113 : 165 and 122 : 137.  Each further tick costs narrow ones more (twice as many
+// hand k and q round): 4 ticks of 16,384 states 64 x 64 in bf16 156 : 137; and so do
+// few rows: a tick of 16 x 64, 47 : 34.  So narrow ones for at most 32 columns, and
+// in bf16 for one tick of more rows, where they leave at most 16 columns idle.
 template <class E>
 hipError_t recurrent(const Args& a, hipStream_t stream) {
-    const uint32_t cols = a.k_dim > 64 || a.v_dim <= 32 ? 32 : 64;
+    const bool one = sizeof(E) == 2 && a.ticks == 1 && a.state_out && a.k_dim > 32 && (0u - a.v_dim) % 32 <= 16;
+    const uint32_t cols = a.k_dim > 64 || a.v_dim <= 32 || one ? 32 : 64;
     const uint64_t waves = uint64_t(a.envs) * a.heads * ((a.v_dim + cols - 1) / cols);
     const dim3 grid(uint32_t((waves + 3) / 4));
     if (cols == 64)
