@@ -234,9 +234,10 @@ template <int G> __device__ __forceinline__ uint32_t row_in_group() {
     return G == 64 ? __builtin_amdgcn_readfirstlane(r) : r;
 }
 
-// Bound by memory: 262,144 x 256 in bfloat16 (0.54 GB) takes 95 us, 5.7 TB/s;
-// 32,768 x 5,120 with a gate per element (1.68 GB) 314 us, 5.3 TB/s; 37,000 x
-// 181 in fp32, rows of 724 bytes (0.11 GB), 24 us, 4.4 TB/s.
+// Bound by memory, under a profiler: 262,144 x 256 in bfloat16 (0.54 GB) takes 92
+// us, 5.8 TB/s, with the stream in fp32 (0.81 GB) 147; 32,768 x 5,120 with a gate
+// per element (1.68 GB) 317 us, 5.3 TB/s, with the stream in fp32 (2.35 GB) 462; 37,000 x
+// 181 in fp32, rows of 724 bytes (0.11 GB), 30 us, 3.6 TB/s (24 us from the cache).
 template <class TX, class TY, int G, int P, int W, int GATE>
 __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) forward_kernel(Args a) {
     __shared__ float lds[2][WAVES][1];
@@ -298,13 +299,14 @@ __global__ void __launch_bounds__(G == 0 ? most_lanes(P, W) : 256) forward_kerne
 // epsilon): there the row's sums and differences are formed in 64 bits, and
 // the norms again from the row.  Wider rows take them in 32 bits.
 //
-// Bound by memory: 262,144 x 256 in bfloat16 (0.81 GB) takes 165 us, 4.9 TB/s;
-// 32,768 x 5,120 with a gate per element (2.68 GB) 720 us, 3.7 TB/s: its column
-// sums, the row and the next one fill the registers that one workgroup of ten
-// wavefronts a compute unit has, so one row is on its way while one is worked on
-// (vector units busy 29 % of the time).  Measured there: two rows ahead, which
-// spills, 882 us; two sums a row one after the other through LDS 784 us (and
-// 209 us in the first case).
+// Bound by memory, under a profiler: 262,144 x 256 in bfloat16 (0.81 GB) takes 160
+// us, 5.0 TB/s, with the stream in fp32 (1.21 GB) 234; 32,768 x 5,120 with a gate per
+// element (2.68 GB) 700 to 780 us, 3.6 TB/s, with the stream in fp32 (3.69 GB) 774: its
+// column sums, the row and the next one fill the registers that one workgroup of
+// ten wavefronts a compute unit has, so one row is on its way while one is worked
+// on (vector units busy 37 % of the time, a wavefront waits 69 % of its).  Measured
+// there beside 720 us: two rows ahead, which spills, 882; two sums a row one after
+// the other through LDS 784 (and 209 beside 165 in the first case).
 template <int G> struct Sum { typedef float type; };
 template <> struct Sum<16> { typedef double type; };
 
@@ -481,9 +483,9 @@ __global__ void __launch_bounds__(1024) columns_kernel(const float* parts, uint3
 
 // The lanes of a row: one piece of W elements each on a part of a wavefront,
 // one, or a workgroup of at most most_lanes(); up to 16 elements a lane in wider rows.
-// 262,144 x 256 in bfloat16 on halves of wavefronts and on whole ones: 90 : 166 us
-// forward, 175 : 481 backward; 1,048,576 x 64 in fp32 on quarters and on whole ones
-// 205 : 473 and 376 : 835.
+// 262,144 x 256 in bfloat16 on halves of wavefronts and on whole ones: 99 : 168 us
+// forward, 265 : 686 with the backward pass; 1,048,576 x 64 in fp32 on quarters and on
+// whole ones 214 : 468 and 589 : 1,334 (calls in a row, each with inputs of its own).
 struct Shape { uint32_t lanes, pieces; };
 inline Shape shape_of(uint32_t width, uint32_t w, uint32_t lanes_1, uint32_t lanes_2) {
     const uint32_t pieces = (width + w - 1) / w;
@@ -495,7 +497,7 @@ inline Shape shape_of(uint32_t width, uint32_t w, uint32_t lanes_1, uint32_t lan
 }
 inline Shape backward_shape(uint32_t width, uint32_t w) { return shape_of(width, w, most_lanes(1, w), most_lanes(2, w)); }
 // Forward, where a lane needs few registers, two workgroups of half the lanes
-// are faster than one: 298 against 320 us at 32,768 x 5,120 bfloat16.
+// are faster than one: 330 against 365 us at 32,768 x 5,120 bfloat16 (measured so too).
 inline Shape forward_shape(uint32_t width, uint32_t w) { return shape_of(width, w, 512, 512); }
 // Workgroups, each with several rows in turn: enough to fill the GPU's 256 compute units.
 inline uint32_t blocks_of(const Args& a, const Shape& s) {

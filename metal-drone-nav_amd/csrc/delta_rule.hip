@@ -51,12 +51,12 @@ template <class E> __device__ __forceinline__ void store_four(E* row, uint32_t d
 // the 64 / CG lanes of a column.  k and q are loaded an element a lane and
 // handed round through LDS, where a lane's rows are neighbours.
 //
-// Bound by memory: a tick of 32,768 states 64 x 64 in bf16 (1.09 GB with the
-// rows) takes 193 us, 5.6 TB/s; of 18,006 states 40 x 72, rows of 288 bytes,
-// 91 us for 0.42 GB.  Lanes with 16 neighbouring rows each, whose k and q are
-// plain wide loads, took 193 and 147 us: their loads touch more cache lines in
-// rows that do not fill them.  Each further tick of 16,384 states adds 8.5 us,
-// vector work.
+// Bound by memory: a tick in place of 32,768 states 64 x 64 in bf16 (1.09 GB with
+// the rows) takes 200 us, 5.5 TB/s; of 18,006 states 40 x 72, rows of 288 bytes,
+// 118 to 125 us for 0.42 GB.  Lanes with 16 neighbouring rows each, whose k and q
+// are plain wide loads, were as fast in the first and took 1.6 times as long in
+// the second: their loads touch more cache lines in rows that do not fill them.
+// Each further tick of 16,384 states 64 x 64 adds 10 to 13 us, vector work.
 template <class E, int CG>
 __global__ void __launch_bounds__(256, CG == 8 ? 3 : 4) recurrent_kernel(Args a) {
     constexpr int RG = 64 / CG, ROWS = 16;  // rows of a step, most steps
@@ -190,13 +190,15 @@ template <class E, int D, int N> struct ForwardShared {
 // starts from the identity with no v and leaves M; neither has outputs.
 //
 // Bound by the issue of vector instructions (the products' operands are split
-// and scaled between the matrix cores): 32,768 states 64 x 64 of 128 ticks in
-// bfloat16 (2.7 GB) take 870 us, 3.1 TB/s, with the vector units issuing 64 % and
-// the matrix cores busy 16 % of the time; of 32 ticks 280 us.  5,120 states
-// 128 x 128 of 64 ticks 225 us; 6,000 of 40 x 72, 37 ticks, in fp32, 322 us,
-// where the fp32 matrix cores (four places of the summed axis each) and waits
-// between them count.  Chunks of 32 ticks: of 16 there would be twice the
-// passes over the state, of 64 a triangle that takes four times the work.
+// and scaled between the matrix cores) and the waits between them: 32,768 states
+// 64 x 64 of 128 ticks in bfloat16 (2.7 GB) take 852 to 882 us, 3.1 TB/s, with the
+// vector units issuing 60 % and the matrix cores busy 16 % of the time and a
+// wavefront waiting 53 % of its; with a final state, in three terms, 1,100 to 1,140;
+// of 32 ticks 262 to 269 us.  5,120 states 128 x 128 of 64 ticks 189 us, with a
+// final state 278; 6,000 of 40 x 72, 37 ticks, in fp32, 313 us, where the fp32 matrix
+// cores (four places of the summed axis each) and waits between them count.
+// Chunks of 32 ticks: of 16 there would be twice the passes over the state, of
+// 64 a triangle that takes four times the work.
 template <class E, int N, int D, bool FULL, bool AHEAD>
 __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
     typedef ForwardShared<E, D, N> Shared;
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(D * 4, 4) forward_kernel(Call call) {
 // A workgroup per 16 columns of a state, a wavefront for each 16 rows: it has
 // its rows of M ahead of the product, and the columns' last values come from
 // LDS.  Bound by the latency of its steps, one after the other: 30 segments
-// of 16 states 128 x 128 take 89 us, 3 us each.
+// of 16 states 128 x 128 take 82 us under a profiler, 3 us each.
 template <class E, int N, bool TRANSPOSED>
 __global__ void __launch_bounds__(512) join_kernel(Args a, float* seg) {
     constexpr int D = int(MAX_DIM), ST = D + Kind<E>::PAD, PL = 16 * ST;
@@ -553,10 +555,9 @@ hipError_t forward(const Args& a, hipStream_t stream) {
 }
 // FULL: heads as wide as the kernel's tiles, without the branches for narrower
 // ones.  With it and without, in us, forward and forward with backward: 32,768
-// states 64 x 64 of 32 ticks in bfloat16 264 : 264 and 997 : 1,114, in fp32 472 : 505
-// and 1,822 : 2,544 (without it also S and G whole, not in halves); 5,120 states 128 x
-// 128 of 64 ticks in bfloat16 188 : 196 and 807 : 905, in fp32 406 : 423 and 1,547 :
-// 1,839.
+// states 64 x 64 of 32 ticks in bfloat16 269 : 270 and 1,000 : 1,113, in fp32 473 : 500
+// and 1,792 : 1,974; 5,120 states 128 x 128 of 64 ticks in bfloat16 190 : 196 and 806 :
+// 904, in fp32 405 : 421 and 1,545 : 1,835.
 template <class E, int N, int D>
 hipError_t forward(const Args& a, hipStream_t stream) {
     return a.k_dim == D && a.v_dim == D ? forward<E, N, D, true>(a, stream) : forward<E, N, D, false>(a, stream);

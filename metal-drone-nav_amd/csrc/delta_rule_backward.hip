@@ -29,8 +29,8 @@ template <class E, int D> struct BackwardShared {
     static constexpr int N = Kind<E>::MID;
     // S and G pass through LDS, transposed, as operands; in fp32 in halves of V:
     // of 128 columns they would not fit beside the rows, of 64 a compute unit
-    // would have room for one workgroup and not two (4,096 states, 64 ticks: 465
-    // us whole, 369 in halves)
+    // would have room for one workgroup and not two (4,096 states 48 x 48, 64
+    // ticks, forward and backward: 698 us whole, 516 in halves)
     static constexpr int HALVES = sizeof(E) == 4 ? 2 : 1;
     static constexpr int TP = D / HALVES * STRIDE;
     static constexpr int PLANE = D * CP;
@@ -71,11 +71,12 @@ template <class E> __device__ __forceinline__ void put_gate(KernelCall* k, const
 //
 // Bound by vector instructions and the waits between the chunk's products, each
 // of which needs the last one's result: two wavefronts on a SIMD hold S, G and a
-// chunk's rows.  32,768 states 64 x 64 of 32 ticks in bfloat16 (1.3 GB) take 786
-// us, vector units 42 % and matrix cores 12 % busy; 5,120 states 128 x 128 of 64
-// ticks 605 us; 6,000 of 40 x 72, 37 ticks, in fp32, 1,125 us: there 155 KB of LDS
-// leave one workgroup of five wavefronts a compute unit.  The states before the
-// chunks come from the forward pass, one K x V for 32 ticks of rows.
+// chunk's rows.  32,768 states 64 x 64 of 32 ticks in bfloat16 (1.3 GB) take 752 to
+// 773 us under a profiler, vector units 43 % and matrix cores 13 % busy, in fp32
+// 1,356; 5,120 states 128 x 128 of 64 ticks 615 us, in fp32 1,161; 6,000 of 40 x 72, 37
+// ticks, in fp32, 1,160 us: there 155 KB of LDS leave one workgroup of five wavefronts
+// a compute unit, which wait 61 % of the time.  The states before the chunks come
+// from the forward pass, one K x V for 32 ticks of rows.
 template <class E, class F, int D, bool FULL, bool AHEAD>
 __global__ void __launch_bounds__(D * 4, 2) backward_kernel(Call call) {
     typedef BackwardShared<E, D> Shared;

@@ -136,7 +136,8 @@ __device__ __forceinline__ void settle_one(f32x4& a) { asm volatile("" : "+v"(a)
 // where a loop over matrix products is unrolled and can end after each pass,
 // it has been seen to count the way through all passes and not the short one
 // (hipcc of ROCm 7.2: results of heads of at most 16 columns were read before
-// they were there).  A matrix product here is done after at most 11.
+// they were there).  A matrix product here is done after at most 11; the code
+// as built has no such read on any path (tests/test_matrix_waits.py).
 template <class... X> __device__ __forceinline__ void settle(f32x4& a, X&... more) {
     asm volatile("s_nop 15" : "+v"(a));
     (settle_one(more), ...);
