@@ -438,9 +438,9 @@ typedef struct MdnRows {
  * gates.  Decays are exp(g) to a relative error of |g| 2^-24.
  *
  * An infinity or NaN, passed in or risen inside, reaches what the formulas
- * bring it to, later ticks of its episode, and nothing else.  A g below -104,
- * whose exp is 0 in fp32, ends an episode as reset does, whatever the state
- * holds.  Few long states are worked on in segments of 128 ticks or more: a
+ * bring it to, later ticks of its episode, and nothing else.  The g of a tick
+ * with reset is not looked at, and a g below -104, whose exp is 0 in fp32, ends
+ * an episode as reset does, whatever the state holds.  Few long states are worked on in segments of 128 ticks or more: a
  * segment over which keys and strengths multiply a state past fp32
  * (beta |k|^2 above 2, tick after tick) leaves NaN in columns of the state
  * that are not all zeros, and in reverse in those of its gradient. */

@@ -311,7 +311,8 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None, final_state
     to 17 bits, with all 24 where ``final_state`` is asked for (o then differs
     by roundings to bfloat16 that fall on the other side), and gradients with
     16 to 17, those in float32 (state, float32 g and beta) too.  A g below
-    -104 clears the state as ``reset`` does.
+    -104 clears the state as ``reset`` does; the g of a flagged tick is not
+    looked at.
     """
     _no_tangents(q, k, v, g, beta, state, scale)
     _number("scale", scale)
