@@ -517,6 +517,52 @@ int mdn_op_block_norm_backward(const MdnBlockNorm* norm, const MdnBlockNormGrad*
                                uint64_t workspace_bytes, void* stream);
 int mdn_op_block_norm_workspace_bytes(const MdnBlockNorm* norm, uint64_t* bytes);
 
+/* ---- Operators of a policy network and its loss, under the same rules as
+ * those of recurrent policies above.
+ *
+ * The linear layer and the gated feed-forward block, per row x of `in` values:
+ *     y = residual + act(x W^T + b)                     (gated == 0)
+ *     y = act(x W^T + b) * (x W_up^T + b_up)            (gated == 1)
+ * with weights [out][in].  Every array has dtype; sums are fp32 and a result
+ * is rounded once (fp32 rows are multiplied in fp32).  An MdnMatrix names rows
+ * `row` elements apart (0 broadcasts an input) with contiguous columns.
+ * in and out are 1..65,536, rows below 2^31 and may be 0. */
+typedef struct MdnMatrix {
+    void* data;
+    int64_t row;
+} MdnMatrix;
+#define MDN_ACT_NONE 0u
+#define MDN_ACT_RELU 1u
+#define MDN_ACT_TANH 2u
+#define MDN_ACT_SIGMOID 3u
+#define MDN_ACT_SILU 4u       /* z sigmoid(z) */
+#define MDN_ACT_GELU 5u       /* z Phi(z), Phi the normal distribution */
+#define MDN_ACT_GELU_TANH 6u  /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+typedef struct MdnDense {
+    uint64_t rows;
+    uint32_t in, out, dtype, activation, gated;
+    MdnMatrix x, w, w_up, residual, y;  /* residual: data NULL for none, and with gated */
+    const void *b, *b_up;               /* [out], or NULL */
+} MdnDense;
+/* The workspace depends on sizes, strides and addresses (operands that do not
+ * lie in 16-byte words are copied there): it is asked for with the struct of
+ * the call. */
+int mdn_op_dense_forward_bytes(const MdnDense* dense, uint64_t* bytes);
+int mdn_op_dense_forward(const MdnDense* dense, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* The gradients, from the same inputs and the gradient of y, which is also
+ * the residual's.  Those whose data is NULL are not wanted; `residual` and
+ * `y` of `dense` are not read.  What the activation had as its argument is
+ * made again, bit for bit; its gradient enters the products that follow
+ * rounded to dtype, and the biases' unrounded. */
+typedef struct MdnDenseGrad {
+    MdnMatrix d_y, d_x, d_w, d_w_up;
+    void *d_b, *d_b_up;
+} MdnDenseGrad;
+int mdn_op_dense_backward_bytes(const MdnDense* dense, const MdnDenseGrad* grad, uint64_t* bytes);
+int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void* workspace, uint64_t workspace_bytes,
+                          void* stream);
+
 /* Test support, no counterpart in the reference: the kernels divide by
  * constants (plant mass and rotor time constants, the RK4 weight 6, the
  * observation scales) as (float)((double)x * (1.0 / (double)b)).  For each

@@ -18,6 +18,7 @@
 
 #include "block_norm.h"
 #include "delta_rule.h"
+#include "dense.h"
 #include "kernel_args.h"
 #include "mdnav.h"
 #include "mdnav_host.h"
@@ -2398,6 +2399,89 @@ int mdn_op_block_norm_backward(const MdnBlockNorm* norm, const MdnBlockNormGrad*
     d.d_w_post = grad->d_w_post; d.d_w_pre = grad->d_w_pre; d.d_residual = grad->d_residual;
     d.parts = static_cast<float*>(workspace);
     HIP_TRY(blocknorm::launch_backward(a, d, norm->x_dtype, norm->y_dtype, static_cast<hipStream_t>(stream)));
+    return MDN_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- operators of a policy network
+namespace {
+
+dense::Matrix matrix(const MdnMatrix& m) { return dense::Matrix{static_cast<char*>(m.data), m.row}; }
+
+int dense_args(const char* name, const MdnDense* d, dense::Args* out) {
+    const std::string who = std::string(name) + ": ";
+    if (!d) return fail(MDN_E_ARG, who + "null");
+    if (d->dtype > MDN_BF16) return fail(MDN_E_ARG, who + "dtype must be MDN_F32 or MDN_BF16");
+    if (d->activation > MDN_ACT_GELU_TANH) return fail(MDN_E_ARG, who + "unknown activation");
+    if (d->gated > 1) return fail(MDN_E_ARG, who + "gated must be 0 or 1");
+    if (d->in < 1 || d->in > dense::MAX_WIDTH || d->out < 1 || d->out > dense::MAX_WIDTH)
+        return fail(MDN_E_ARG, who + "in and out must be 1..65536");
+    if (d->rows > 0x7fffff00ull) return fail(MDN_E_ARG, who + "too many rows");
+    if (!d->w.data || (d->gated && !d->w_up.data)) return fail(MDN_E_ARG, who + "null weights");
+    if (d->rows && !d->x.data) return fail(MDN_E_ARG, who + "null rows");
+    if (d->gated && d->residual.data) return fail(MDN_E_ARG, who + "a gated block has no residual");
+    if (!d->gated && (d->w_up.data || d->b_up)) return fail(MDN_E_ARG, who + "w_up and b_up belong to a gated block");
+    dense::Args a{};
+    a.rows = d->rows; a.in = d->in; a.out = d->out; a.activation = d->activation; a.gated = d->gated; a.bf = d->dtype == MDN_BF16;
+    a.x = matrix(d->x); a.w[0] = matrix(d->w); a.w[1] = matrix(d->w_up); a.residual = matrix(d->residual); a.y = matrix(d->y);
+    a.b[0] = static_cast<const char*>(d->b); a.b[1] = static_cast<const char*>(d->b_up);
+    *out = a;
+    return MDN_OK;
+}
+int dense_grad_args(const char* name, const MdnDense* dense, const MdnDenseGrad* g, dense::Args* a, dense::GradArgs* out) {
+    if (int rc = dense_args(name, dense, a)) return rc;
+    const std::string who = std::string(name) + ": ";
+    if (!g) return fail(MDN_E_ARG, who + "null");
+    if (!a->gated && (g->d_w_up.data || g->d_b_up)) return fail(MDN_E_ARG, who + "d_w_up and d_b_up belong to a gated block");
+    if (a->rows && !g->d_y.data) return fail(MDN_E_ARG, who + "null rows");
+    dense::GradArgs d{};
+    d.d_y = matrix(g->d_y); d.d_x = matrix(g->d_x); d.d_w[0] = matrix(g->d_w); d.d_w[1] = matrix(g->d_w_up);
+    d.d_b[0] = static_cast<char*>(g->d_b); d.d_b[1] = static_cast<char*>(g->d_b_up);
+    *out = d;
+    return MDN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mdn_op_dense_forward_bytes(const MdnDense* dense, uint64_t* bytes) {
+    dense::Args a;
+    if (int rc = dense_args("mdn_op_dense_forward_bytes", dense, &a)) return rc;
+    if (!bytes) return fail(MDN_E_ARG, "mdn_op_dense_forward_bytes: null");
+    *bytes = a.rows ? dense::forward_bytes(a) : 0;
+    return MDN_OK;
+}
+
+int mdn_op_dense_forward(const MdnDense* dense, void* workspace, uint64_t workspace_bytes, void* stream) {
+    dense::Args a;
+    if (int rc = dense_args("mdn_op_dense_forward", dense, &a)) return rc;
+    if (a.rows == 0) return MDN_OK;
+    if (!a.y.p) return fail(MDN_E_ARG, "mdn_op_dense_forward: null rows");
+    const uint64_t need = dense::forward_bytes(a);
+    if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_dense_forward: workspace is too small");
+    HIP_TRY(dense::forward(a, static_cast<char*>(workspace), static_cast<hipStream_t>(stream)));
+    return MDN_OK;
+}
+
+int mdn_op_dense_backward_bytes(const MdnDense* dense, const MdnDenseGrad* grad, uint64_t* bytes) {
+    dense::Args a;
+    dense::GradArgs d;
+    if (int rc = dense_grad_args("mdn_op_dense_backward_bytes", dense, grad, &a, &d)) return rc;
+    if (!bytes) return fail(MDN_E_ARG, "mdn_op_dense_backward_bytes: null");
+    *bytes = a.rows ? dense::backward_bytes(a, d) : 0;
+    return MDN_OK;
+}
+
+int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void* workspace, uint64_t workspace_bytes,
+                          void* stream) {
+    dense::Args a;
+    dense::GradArgs d;
+    if (int rc = dense_grad_args("mdn_op_dense_backward", dense, grad, &a, &d)) return rc;
+    const uint64_t need = a.rows ? dense::backward_bytes(a, d) : 0;
+    if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_dense_backward: workspace is too small");
+    HIP_TRY(dense::backward(a, d, static_cast<char*>(workspace), static_cast<hipStream_t>(stream)));
     return MDN_OK;
 }
 

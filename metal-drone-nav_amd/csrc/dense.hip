@@ -1,0 +1,558 @@
+// dense.hip — the linear layer y = residual + act(x W^T + b) and the gated
+// feed-forward block y = act(x Wg^T + bg) * (x Wu^T + bu), with gradients.
+//
+// Forward: one product (dense_tiles.h) whose tile holds, for the gated block,
+// the same columns of both projections, so that a lane has z of the gate and of
+// the other at the same place; bias, activation and product or residual are
+// made from the fp32 sums, which are rounded once.
+//
+// Backward: z is made again by the same product, bit for bit, with
+//     dz = dy act'(z)        or  dzg = dy zu act'(zg),  dzu = dy act(zg)
+// in its epilogue, rounded once to the rows' type (the matrix cores' operand),
+// and the column sums that are the biases' gradients, from the unrounded
+// values.  Then dx = dz W (of the gated block, both terms in one sum) and
+// dW = dz^T x, the latter's long sum over rows cut into parts that a second
+// kernel adds up in order: no atomics, the same bits every time.
+#include "dense.h"
+
+#include "dense_act.h"
+#include "dense_tiles.h"
+#include "lane_sums.h"
+
+namespace dense {
+namespace {
+
+enum Result { LINEAR, GATED, SLOPE, GATED_SLOPE, STORE, PART };
+constexpr bool two_weights(int r) { return r == GATED || r == GATED_SLOPE; }
+
+struct Job {
+    Side m, n;
+    uint32_t k, segments;                // of the sum; segments: 2 adds a second product of m.p2 and n.p2
+    uint32_t m_tiles, n_tiles;
+    uint32_t splits, split_k;            // PART, STORE: pieces of k; blockIdx.y = batch splits + piece
+    uint32_t act;
+    Matrix y, y2, residual, dy, dz;      // y2: of a second batch (m.p2, n.p)
+    const char* bias[2];
+    uint32_t dz_half;                    // columns from dzg to dzu
+    float* sums;                         // [m_tiles WM][2][n] or null
+};
+
+__device__ __forceinline__ f32x4 four(const f32x16& v, int g) { return f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]}; }
+
+// ---------------------------------------------------------------- the product
+// BN counts the rows of LDS: of the gated block's projections, half each.
+template <class T, int BM, int BN, int WM, int WN, int STAGES, bool MC, bool NC, int RESULT>
+__global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
+    constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+    constexpr bool N2 = two_weights(RESULT);
+    constexpr int OUT = N2 ? BN / 2 : BN;  // columns of the result
+    static_assert(TM >= 1 && TN >= (N2 ? 2 : 1), "");
+    typedef Staged<T, BM, W, MC, false> SideM;
+    typedef Staged<T, BN, W, NC, N2> SideN;
+    constexpr uint32_t STAGE = SideM::BYTES + SideN::BYTES;
+    constexpr int LOADS = SideM::LOADS + SideN::LOADS;
+    extern __shared__ __align__(16) char shared[];
+    const uint32_t lds = uint32_t(uintptr_t((__attribute__((address_space(3))) char*)shared));
+
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wm = wave / WN, wn = wave % WN;
+    // Workgroups go to the 8 XCDs in turn: each gets a run of tiles, n first
+    // inside a band of 8 tiles, so that what its L2 holds is used again.
+    uint32_t mt, nt;
+    {
+        const uint32_t tiles = a.m_tiles * a.n_tiles, xcd = blockIdx.x & 7, per = tiles / 8, rest = tiles % 8;
+        uint32_t t = xcd * per + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+        const uint32_t band = t / (8 * a.m_tiles), in = t - band * 8 * a.m_tiles;
+        const uint32_t wide = a.n_tiles - band * 8 < 8 ? a.n_tiles - band * 8 : 8;
+        mt = in / wide;
+        nt = band * 8 + in % wide;
+    }
+    uint32_t k_first = 0, k_end = a.k;
+    const uint32_t batch = blockIdx.y / a.splits, piece = blockIdx.y % a.splits;
+    if (RESULT == PART || RESULT == STORE) {
+        k_first = piece * a.split_k;
+        k_end = k_first + a.split_k < a.k ? k_first + a.split_k : a.k;
+    }
+    SideM sm;
+    SideN sn;
+    {
+        Side m = a.m;
+        if ((RESULT == PART || RESULT == STORE) && batch) m.p = a.m.p2;
+        sm.init(m, mt * BM, wave, lane);
+        sn.init(a.n, nt * OUT, wave, lane);
+    }
+    typename SideM::Reader rm;
+    typename SideN::Reader rn;
+    rm.init(lane);
+    rn.init(lane);
+
+    f32x16 acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; i++)
+#pragma unroll
+        for (int j = 0; j < TM; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+
+    const uint32_t steps = (k_end - k_first + step_of<T>() - 1) / step_of<T>(), total = steps * a.segments;
+    uint32_t next = 0, next_k = k_first, into = 0;  // the step to load, its k, its stage
+    bool second = false;
+    const auto fetch = [&]() {
+        const uint32_t to = lds + into * STAGE;
+        if (next_k + step_of<T>() <= k_end) {
+            sm.load(to, next_k, wave, second);
+            sn.load(to + SideM::BYTES, next_k, wave, second);
+        } else {
+            sm.load_end(to, next_k, k_end, wave, second);
+            sn.load_end(to + SideM::BYTES, next_k, k_end, wave, second);
+        }
+        next++;
+        next_k += step_of<T>();
+        if (next == steps) {
+            next_k = k_first;
+            second = true;
+        }
+        into = into + 1 == STAGES ? 0 : into + 1;
+    };
+    for (int s = 0; s < STAGES - 1; s++)
+        if (uint32_t(s) < total) fetch();
+    uint32_t from = 0;
+    for (uint32_t s = 0; s < total; s++) {
+        // this step's words are there for all, and all have read the step before it
+        if (STAGES > 2 && s + STAGES - 2 < total)
+            landed<LOADS*(STAGES - 2)>();
+        else
+            landed<0>();
+        if (next < total) fetch();
+        const uint32_t at_m = lds + from * STAGE, at_n = at_m + SideM::BYTES;
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) {
+            Frag<T> fm[TM], fn[TN];
+#pragma unroll
+            for (int i = 0; i < TN; i++) {
+                const uint32_t row = N2 ? (i < TN / 2 ? 0 : BN / 2) + wn * (OUT / WN) + 32 * (i % (TN / 2 > 0 ? TN / 2 : 1)) : wn * (BN / WN) + 32 * i;
+                fn[i] = rn.get(at_n, row, kk);
+            }
+#pragma unroll
+            for (int j = 0; j < TM; j++) fm[j] = rm.get(at_m, wm * (BM / WM) + 32 * j, kk);
+#pragma unroll
+            for (int i = 0; i < TN; i++)
+#pragma unroll
+                for (int j = 0; j < TM; j++) mma(acc[i][j], fn[i], fm[j]);
+        }
+        from = from + 1 == STAGES ? 0 : from + 1;
+    }
+
+    // ---- the result
+    const uint32_t m0 = mt * BM + wm * (BM / WM) + (lane & 31), n0 = nt * OUT + wn * (OUT / WN) + 4 * (lane >> 5);
+    const uint32_t mc = a.m.count, nc = a.n.count;
+    constexpr int TO = N2 ? TN / 2 : TN;
+#pragma unroll
+    for (int i = 0; i < TO; i++) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const uint32_t n = n0 + 32 * i + 8 * g;
+            if constexpr (RESULT == STORE || RESULT == PART) {
+                const Matrix& y = batch ? a.y2 : a.y;
+#pragma unroll
+                for (int j = 0; j < TM; j++) {
+                    const uint32_t m = m0 + 32 * j;
+                    if (m >= mc || n >= nc) continue;
+                    const f32x4 v = four(acc[i][j], g);
+                    if constexpr (RESULT == STORE)
+                        store4<T>(row_of<T>(y, m), n, nc, v);
+                    else
+                        store4<float>(row_of<float>(y, m) + uint64_t(piece) * mc * y.ld * 4, n, nc, v);
+                }
+            } else {
+                f32x4 b0 = {0.0f, 0.0f, 0.0f, 0.0f}, b1 = b0;
+                if (a.bias[0]) b0 = load4<T>(a.bias[0], n, nc);
+                if (N2 && a.bias[1]) b1 = load4<T>(a.bias[1], n, nc);
+                f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+#pragma unroll
+                for (int j = 0; j < TM; j++) {
+                    const uint32_t m = m0 + 32 * j;
+                    const f32x4 z0 = four(acc[i][j], g) + b0;
+                    f32x4 z1;
+                    if constexpr (N2) z1 = four(acc[TO + i][j], g) + b1;
+                    if (m >= mc) continue;
+                    if constexpr (RESULT == LINEAR || RESULT == GATED) {
+                        if (n >= nc) continue;
+                        f32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e] = act_of<T>(a.act, z0[e]);
+                        if constexpr (RESULT == GATED) v = v * z1;
+                        if (RESULT == LINEAR && a.residual.p) v = load4<T>(row_of<T>(a.residual, m), n, nc) + v;
+                        store4<T>(row_of<T>(a.y, m), n, nc, v);
+                    } else {
+                        // zeros past the last column: the next products read whole words
+                        f32x4 d0 = load4<T>(row_of<T>(a.dy, m), n, nc), d1 = d0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float slope;
+                            const float v = act_of<T>(a.act, z0[e], slope);
+                            if constexpr (N2) {
+                                d1[e] = n + e < nc ? d0[e] * v : 0.0f;
+                                d0[e] = n + e < nc ? d0[e] * z1[e] * slope : 0.0f;
+                            } else
+                                d0[e] = n + e < nc ? d0[e] * slope : 0.0f;
+                        }
+                        s0 += d0;
+                        if (N2) s1 += d1;
+                        const uint32_t wide = uint32_t(a.dz_half);
+                        store4<T>(row_of<T>(a.dz, m), n, wide, d0);
+                        if (N2) store4<T>(row_of<T>(a.dz, m) + uint64_t(wide) * sizeof(T), n, wide, d1);
+                    }
+                }
+                if constexpr (RESULT == SLOPE || RESULT == GATED_SLOPE) {
+                    if (a.sums) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            s0[e] = lanes::sum_rows16(lanes::sum16(s0[e]));
+                            if (N2) s1[e] = lanes::sum_rows16(lanes::sum16(s1[e]));
+                        }
+                        if ((lane & 31) == 0 && n < nc) {
+                            char* to = reinterpret_cast<char*>(a.sums + uint64_t(mt * WM + wm) * 2 * nc);
+                            store4<float>(to, n, nc, s0);
+                            if (N2) store4<float>(to + uint64_t(nc) * 4, n, nc, s1);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- what is left
+// Rows with words of their own: row r of `to` (ld elements, a multiple of a
+// word's) is row r of `from`, zeros behind it.
+template <class T>
+__global__ void __launch_bounds__(256) lay_out_kernel(Matrix from, Matrix to, uint64_t rows, uint32_t width) {
+    const uint32_t words = uint32_t(to.ld) / per_word<T>();
+    const uint64_t all = rows * words;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += uint64_t(gridDim.x) * 256) {
+        const uint64_t row = i / words;
+        const uint32_t c = uint32_t(i - row * words) * per_word<T>();
+        const T* src = reinterpret_cast<const T*>(from.p) + int64_t(row) * from.ld + c;
+        T v[per_word<T>()];
+#pragma unroll
+        for (uint32_t e = 0; e < per_word<T>(); e++) v[e] = c + e < width ? src[e] : T(0.0f);
+        T* dst = reinterpret_cast<T*>(to.p) + row * to.ld + c;
+#pragma unroll
+        for (uint32_t e = 0; e < per_word<T>(); e += 4)
+            *reinterpret_cast<typename Four<T>::type*>(dst + e) = typename Four<T>::type{v[e], v[e + 1], v[e + 2], v[e + 3]};
+    }
+}
+
+// Adds up the parts of a product, in order: to[r][c] = sum of from[s][r][c].
+template <class T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float* from, uint32_t parts, Matrix to, uint32_t rows, uint32_t width) {
+    const uint64_t all = uint64_t(rows) * width;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += uint64_t(gridDim.x) * 256) {
+        float v = 0.0f;
+        for (uint32_t s = 0; s < parts; s++) v += from[s * all + i];
+        const uint64_t row = i / width;
+        reinterpret_cast<T*>(to.p)[int64_t(row) * to.ld + int64_t(i - row * width)] = T(v);
+    }
+}
+
+// Column sums of rows, in two steps: blockIdx.y's share of the rows to a row
+// of sums, 64 columns a workgroup, a quarter of the share a wavefront.
+template <class T>
+__global__ void __launch_bounds__(256) column_sums_kernel(Matrix from, uint64_t rows, uint32_t width, uint64_t share, float* sums) {
+    __shared__ float part[4][64];
+    const uint32_t c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+    const uint64_t first = blockIdx.y * share, end = first + share < rows ? first + share : rows;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < width) {
+        const T* p = reinterpret_cast<const T*>(from.p) + c;
+        uint64_t r = first + slice;
+        for (; r + 12 < end; r += 16)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] += float(p[int64_t(r + 4 * i) * from.ld]);
+        for (; r < end; r += 4) v[0] += float(p[int64_t(r) * from.ld]);
+    }
+    part[slice][threadIdx.x & 63] = (v[0] + v[1]) + (v[2] + v[3]);
+    __syncthreads();
+    if (slice == 0 && c < width)
+        sums[uint64_t(blockIdx.y) * width + c] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+}
+// Rows of sums, `pitch` apart, to a vector: 64 columns a workgroup, a sixteenth of the rows a wavefront.
+template <class T>
+__global__ void __launch_bounds__(1024) add_sums_kernel(const float* sums, uint32_t count, uint64_t pitch, uint32_t width, char* to) {
+    __shared__ float part[16][64];
+    const uint32_t c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < width) {
+        uint32_t i = slice;
+        for (; i + 48 < count; i += 64)
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += sums[uint64_t(i + 16 * j) * pitch + c];
+        for (; i < count; i += 16) v[0] += sums[uint64_t(i) * pitch + c];
+    }
+    part[slice][threadIdx.x & 63] = (v[0] + v[1]) + (v[2] + v[3]);
+    __syncthreads();
+    if (slice != 0 || c >= width) return;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s += part[i][threadIdx.x];
+    reinterpret_cast<T*>(to)[c] = T(s);
+}
+
+// ---------------------------------------------------------------- launches
+uint32_t blocks_for(uint64_t items, uint32_t per, uint32_t most) {
+    const uint64_t n = (items + per - 1) / per;
+    return uint32_t(n < most ? (n ? n : 1) : most);
+}
+
+template <class T, int BM, int BN, int WM, int WN, int STAGES, bool MC, bool NC, int RESULT>
+hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
+    constexpr uint32_t OUT = two_weights(RESULT) ? BN / 2 : BN, bytes = STAGES * (BM + BN) * STEP_BYTES;
+    static_assert(bytes <= 160 * 1024, "");
+    a.m_tiles = (a.m.count + BM - 1) / BM;
+    a.n_tiles = (a.n.count + OUT - 1) / OUT;
+    const auto kernel = product_kernel<T, BM, BN, WM, WN, STAGES, MC, NC, RESULT>;
+    if (bytes > 64 * 1024)
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
+            return e;
+    kernel<<<dim3(a.m_tiles * a.n_tiles, batches * a.splits), dim3(64 * WM * WN), bytes, st>>>(a);
+    return hipGetLastError();
+}
+
+// The tile of a product of m x n results: the largest whose tiles fill the 256 compute units.
+enum Tile { SMALL, MIDDLE, LARGE };
+Tile tile_of(uint64_t m, uint64_t n, uint64_t times) {
+    const auto tiles = [&](uint64_t b) { return (m + b - 1) / b * ((n + b - 1) / b) * times; };
+    if (tiles(256) >= 256) return LARGE;
+    return tiles(128) >= 256 ? MIDDLE : SMALL;
+}
+
+template <class T, bool MC, bool NC, int RESULT>
+hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
+    if (tile == LARGE) return launch<T, 256, 256, 2, 4, 2, MC, NC, RESULT>(a, batches, st);
+    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 2, MC, NC, RESULT>(a, batches, st);
+    if constexpr (two_weights(RESULT))
+        return launch<T, 64, 128, 2, 2, 3, MC, NC, RESULT>(a, batches, st);
+    else
+        return launch<T, 64, 64, 2, 2, 4, MC, NC, RESULT>(a, batches, st);
+}
+
+// ---- memory
+constexpr uint64_t ALIGN = 256;
+uint64_t aligned(uint64_t bytes) { return (bytes + ALIGN - 1) / ALIGN * ALIGN; }
+
+// A matrix whose rows move in 16-byte words as they are.
+bool in_words(const Matrix& m, uint32_t width, uint32_t size) {
+    return width % (16 / size) == 0 && (m.ld * size) % 16 == 0 && reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld >= 0 &&
+           m.ld * size <= (1 << 22);
+}
+uint32_t pieces_of(const Args& a) { return a.gated ? 2 : 1; }
+uint32_t words_of(uint32_t width, uint32_t size) { return (width + 16 / size - 1) / (16 / size) * (16 / size); }
+
+// Where the operands of a call's products lie: as they are, or copied.
+struct Plan {
+    uint32_t size, in_ld, out_ld;  // widths in whole words
+    bool x_copy, w_copy;
+    uint64_t x_bytes, w_bytes;     // w_bytes: of one of the weights
+    Tile forward_tile;
+};
+Plan plan_of(const Args& a) {
+    Plan p{};
+    p.size = a.bf ? 2 : 4;
+    p.in_ld = words_of(a.in, p.size);
+    p.out_ld = words_of(a.out, p.size);
+    p.x_copy = !in_words(a.x, a.in, p.size);
+    p.w_copy = !in_words(a.w[0], a.in, p.size) || (a.gated && (!in_words(a.w[1], a.in, p.size) || a.w[1].ld != a.w[0].ld));
+    p.x_bytes = p.x_copy ? aligned(a.rows * p.in_ld * p.size) : 0;
+    p.w_bytes = p.w_copy ? aligned(uint64_t(a.out) * p.in_ld * p.size) : 0;
+    p.forward_tile = tile_of(a.rows, uint64_t(a.out) * pieces_of(a), 1);
+    return p;
+}
+// Of the backward pass.
+constexpr uint32_t SHARES = 256;  // of rows, in column sums
+struct BackPlan : Plan {
+    bool slope, dz_copy, w_needed, x_needed;
+    uint64_t dz_bytes, sums_bytes, parts_bytes;
+    uint32_t sum_rows, splits, split_k;
+    Tile dx_tile, dw_tile;
+};
+BackPlan back_plan_of(const Args& a, const GradArgs& d) {
+    BackPlan p{};
+    static_cast<Plan&>(p) = plan_of(a);
+    const uint32_t pieces = pieces_of(a);
+    p.slope = a.gated || a.activation != MDN_ACT_NONE;
+    const bool dw = d.d_w[0].p || d.d_w[1].p, dx = d.d_x.p, db = d.d_b[0] || d.d_b[1];
+    p.x_needed = p.slope || dw;
+    p.w_needed = p.slope || dx;
+    if (!p.x_needed) p.x_copy = false, p.x_bytes = 0;
+    if (!p.w_needed) p.w_copy = false, p.w_bytes = 0;
+    p.dz_copy = !p.slope && (dx || dw) && !in_words(d.d_y, a.out, p.size);
+    p.dz_bytes = p.slope || p.dz_copy ? aligned(a.rows * pieces * p.out_ld * p.size) : 0;
+    if (p.slope) {
+        const uint32_t bm = p.forward_tile == LARGE ? 256 : p.forward_tile == MIDDLE ? 128 : 64;
+        p.sum_rows = uint32_t((a.rows + bm - 1) / bm) * 2;
+    } else
+        p.sum_rows = uint32_t(a.rows < 16 * SHARES ? (a.rows + 15) / 16 : SHARES);
+    p.sums_bytes = db ? aligned(uint64_t(p.sum_rows) * 2 * a.out * 4) : 0;
+    p.dx_tile = tile_of(a.rows, a.in, 1);
+    // dW: few results, a long sum. Pieces of at least 512 rows, as many as make 512 workgroups.
+    const uint64_t most = (a.rows + 511) / 512;
+    p.dw_tile = tile_of(a.out, a.in, pieces * most);
+    const uint64_t b = p.dw_tile == LARGE ? 256 : p.dw_tile == MIDDLE ? 128 : 64;
+    const uint64_t tiles = (a.out + b - 1) / b * ((a.in + b - 1) / b) * pieces;
+    const uint64_t want = p.dw_tile == LARGE ? 256 : 512;
+    uint64_t splits = (want + tiles - 1) / tiles;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    p.split_k = uint32_t((a.rows + splits - 1) / splits + 63) / 64 * 64;
+    if (p.split_k == 0) p.split_k = 64;
+    p.splits = uint32_t((a.rows + p.split_k - 1) / p.split_k);
+    if (p.splits < 1) p.splits = 1;
+    p.parts_bytes = dw && p.splits > 1 ? aligned(uint64_t(pieces) * p.splits * a.out * a.in * 4) : 0;
+    return p;
+}
+
+template <class T> hipError_t lay_out(const Matrix& from, const Matrix& to, uint64_t rows, uint32_t width, hipStream_t st) {
+    const uint64_t words = rows * (to.ld / per_word<T>());
+    lay_out_kernel<T><<<dim3(blocks_for(words, 256, 8192)), dim3(256), 0, st>>>(from, to, rows, width);
+    return hipGetLastError();
+}
+// x and the weights in words; copies go to `work`, which is advanced.
+template <class T> hipError_t operands(Args& a, const Plan& p, char*& work, hipStream_t st) {
+    if (p.x_copy) {
+        const Matrix to{work, p.in_ld};
+        if (hipError_t e = lay_out<T>(a.x, to, a.rows, a.in, st)) return e;
+        a.x = to;
+        work += p.x_bytes;
+    }
+    if (p.w_copy)
+        for (uint32_t i = 0; i < pieces_of(a); i++) {
+            const Matrix to{work, p.in_ld};
+            if (hipError_t e = lay_out<T>(a.w[i], to, a.out, a.in, st)) return e;
+            a.w[i] = to;
+            work += p.w_bytes;
+        }
+    return hipSuccess;
+}
+Side side(const Matrix& m, const char* second, uint64_t count, uint32_t size) {
+    return {m.p, second, m.ld * int64_t(size), uint32_t(count)};
+}
+Job forward_job(const Args& a, const Plan& p) {
+    Job j{};
+    j.m = side(a.x, nullptr, a.rows, p.size);
+    j.n = side(a.w[0], a.w[1].p, a.out, p.size);
+    j.k = p.in_ld;
+    j.segments = j.splits = 1;
+    j.split_k = j.k;
+    j.act = a.activation;
+    j.y = a.y;
+    j.residual = a.residual;
+    j.bias[0] = a.b[0];
+    j.bias[1] = a.b[1];
+    return j;
+}
+
+template <class T> hipError_t forward_of(Args a, char* work, hipStream_t st) {
+    const Plan p = plan_of(a);
+    if (hipError_t e = operands<T>(a, p, work, st)) return e;
+    const Job j = forward_job(a, p);
+    return a.gated ? product<T, false, false, GATED>(j, p.forward_tile, 1, st) : product<T, false, false, LINEAR>(j, p.forward_tile, 1, st);
+}
+
+template <class T> hipError_t add_sums(const float* sums, uint32_t count, uint64_t pitch, uint32_t width, char* to, hipStream_t st) {
+    add_sums_kernel<T><<<dim3((width + 63) / 64), dim3(1024), 0, st>>>(sums, count, pitch, width, to);
+    return hipGetLastError();
+}
+
+template <class T> hipError_t backward_of(Args a, const GradArgs& d, char* work, hipStream_t st) {
+    const BackPlan p = back_plan_of(a, d);
+    const uint32_t pieces = pieces_of(a);
+    if (hipError_t e = operands<T>(a, p, work, st)) return e;
+    Matrix dz = d.d_y;
+    if (p.dz_bytes) {
+        dz = Matrix{work, int64_t(pieces) * p.out_ld};
+        work += p.dz_bytes;
+    }
+    float* sums = p.sums_bytes ? reinterpret_cast<float*>(work) : nullptr;
+    work += p.sums_bytes;
+    if (p.slope) {
+        Job j = forward_job(a, p);
+        j.dy = d.d_y;
+        j.dz = dz;
+        j.dz_half = p.out_ld;
+        j.sums = sums;
+        if (hipError_t e = a.gated ? product<T, false, false, GATED_SLOPE>(j, p.forward_tile, 1, st)
+                                   : product<T, false, false, SLOPE>(j, p.forward_tile, 1, st))
+            return e;
+        for (uint32_t i = 0; i < pieces; i++)
+            if (d.d_b[i])
+                if (hipError_t e = add_sums<T>(sums + i * a.out, p.sum_rows, 2 * uint64_t(a.out), a.out, d.d_b[i], st)) return e;
+    } else {
+        if (p.dz_copy)
+            if (hipError_t e = lay_out<T>(d.d_y, dz, a.rows, a.out, st)) return e;
+        if (d.d_b[0]) {
+            const uint64_t share = (a.rows + p.sum_rows - 1) / p.sum_rows;
+            column_sums_kernel<T><<<dim3((a.out + 63) / 64, p.sum_rows), dim3(256), 0, st>>>(d.d_y, a.rows, a.out, share, sums);
+            if (hipError_t e = hipGetLastError()) return e;
+            if (hipError_t e = add_sums<T>(sums, p.sum_rows, a.out, a.out, d.d_b[0], st)) return e;
+        }
+    }
+    const char* dz2 = dz.p + uint64_t(p.out_ld) * p.size;
+    if (d.d_x.p) {
+        Job j{};
+        j.m = side(dz, dz2, a.rows, p.size);
+        j.n = side(a.w[0], a.w[1].p, a.in, p.size);
+        j.k = j.split_k = a.out;
+        j.segments = pieces;
+        j.splits = 1;
+        j.y = d.d_x;
+        if (hipError_t e = product<T, false, true, STORE>(j, p.dx_tile, 1, st)) return e;
+    }
+    if (d.d_w[0].p || d.d_w[1].p) {
+        Job j{};
+        const bool both = d.d_w[0].p && d.d_w[1].p;
+        const uint32_t first = d.d_w[0].p ? 0 : 1;
+        j.m = side(dz, dz2, a.out, p.size);
+        if (first) j.m.p = dz2;
+        j.n = side(a.x, nullptr, a.in, p.size);
+        j.k = uint32_t(a.rows);
+        j.segments = 1;
+        j.splits = p.splits;
+        j.split_k = p.split_k;
+        j.y = d.d_w[first];
+        j.y2 = d.d_w[1];
+        if (p.splits == 1) return product<T, true, true, STORE>(j, p.dw_tile, both ? 2 : 1, st);
+        float* parts = reinterpret_cast<float*>(work);
+        const uint64_t all = uint64_t(a.out) * a.in;
+        j.y = Matrix{reinterpret_cast<char*>(parts), a.in};
+        j.y2 = Matrix{reinterpret_cast<char*>(parts + p.splits * all), a.in};
+        if (hipError_t e = product<T, true, true, PART>(j, p.dw_tile, both ? 2 : 1, st)) return e;
+        for (uint32_t i = 0; i < (both ? 2u : 1u); i++) {
+            add_parts_kernel<T><<<dim3(blocks_for(all, 256, 4096)), dim3(256), 0, st>>>(parts + i * p.splits * all, p.splits,
+                                                                                        d.d_w[first + i], a.out, a.in);
+            if (hipError_t e = hipGetLastError()) return e;
+        }
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+uint64_t forward_bytes(const Args& a) {
+    if (few_rows(a)) return 0;
+    const Plan p = plan_of(a);
+    return p.x_bytes + pieces_of(a) * p.w_bytes;
+}
+uint64_t backward_bytes(const Args& a, const GradArgs& d) {
+    const BackPlan p = back_plan_of(a, d);
+    return p.x_bytes + pieces_of(a) * p.w_bytes + p.dz_bytes + p.sums_bytes + p.parts_bytes;
+}
+hipError_t forward(const Args& a, char* work, hipStream_t st) {
+    if (few_rows(a)) return forward_few(a, st);
+    return a.bf ? forward_of<bf16>(a, work, st) : forward_of<float>(a, work, st);
+}
+hipError_t backward(const Args& a, const GradArgs& d, char* work, hipStream_t st) {
+    return a.bf ? backward_of<bf16>(a, d, work, st) : backward_of<float>(a, d, work, st);
+}
+
+}  // namespace dense

@@ -1,0 +1,105 @@
+// dense_act.h — activations with their slopes, and four neighbours of a row.
+#ifndef MDNAV_DENSE_ACT_H
+#define MDNAV_DENSE_ACT_H
+
+#include "dense.h"
+#include "dense_tiles.h"
+
+namespace dense {
+
+// ---------------------------------------------------------------- activations
+// T: the type that the value is rounded to. bfloat16 leaves room for the
+// faster exponential, whose relative error is |z| 2^-24.
+template <class T> __device__ __forceinline__ float exp_of(float x) { return sizeof(T) == 2 ? __expf(x) : expf(x); }
+template <class T> __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_of<T>(-z)); }
+template <class T> __device__ __forceinline__ float tanh_of(float z) {
+    if (sizeof(T) == 4) return tanhf(z);
+    // 1 - 2 / (e^2z + 1) cancels near 0, where the series' next term is below 2^-17 of the value
+    const float e = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__expf(2.0f * z) + 1.0f), q = z * z;
+    return q < 0.0025f ? z * (1.0f - q * 0.33333333f) : e;
+}
+constexpr float C_TANH = 1.5957691216f;  // 2 sqrt(2 / pi)
+
+template <class T> __device__ __forceinline__ float act_of(uint32_t act, float z) {
+    switch (act) {
+        case MDN_ACT_RELU: return z > 0.0f ? z : z == z ? 0.0f : z;
+        case MDN_ACT_TANH: return tanh_of<T>(z);
+        case MDN_ACT_SIGMOID: return sigmoid<T>(z);
+        case MDN_ACT_SILU: return z * sigmoid<T>(z);
+        case MDN_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);
+        case MDN_ACT_GELU_TANH: return z * sigmoid<T>(C_TANH * z * fmaf(0.044715f * z, z, 1.0f));
+        default: return z;
+    }
+}
+// act(z) and act'(z)
+template <class T> __device__ __forceinline__ float act_of(uint32_t act, float z, float& slope) {
+    switch (act) {
+        case MDN_ACT_RELU: slope = z > 0.0f ? 1.0f : z == z ? 0.0f : z; return act_of<T>(act, z);
+        case MDN_ACT_TANH: {
+            const float t = tanh_of<T>(z);
+            slope = fmaf(-t, t, 1.0f);
+            if (fabsf(z) > 4.0f) {  // 1 - t^2 cancels
+                const float e = exp_of<T>(-2.0f * fabsf(z)), q = 1.0f + e;
+                slope = 4.0f * e / (q * q);
+            }
+            return t;
+        }
+        case MDN_ACT_SIGMOID: {
+            const float s = sigmoid<T>(z);
+            slope = s * sigmoid<T>(-z);
+            return s;
+        }
+        case MDN_ACT_SILU: {
+            const float s = sigmoid<T>(z);
+            slope = s * fmaf(z, sigmoid<T>(-z), 1.0f);
+            return z * s;
+        }
+        case MDN_ACT_GELU: {
+            const float s = 0.5f * erfcf(-0.70710678f * z);
+            slope = fmaf(z * 0.39894228f, exp_of<T>(-0.5f * z * z), s);
+            return z * s;
+        }
+        case MDN_ACT_GELU_TANH: {
+            // beyond 30 the slope is 0 or 1; the polynomial would overflow
+            const float c = fminf(fmaxf(z, -30.0f), 30.0f), u = C_TANH * c * fmaf(0.044715f * c, c, 1.0f);
+            const float s = sigmoid<T>(u);
+            slope = fmaf(c * s * sigmoid<T>(-u), C_TANH * fmaf(0.134145f * c, c, 1.0f), s) + 0.0f * z;
+            return z * s;
+        }
+        default: slope = 1.0f; return z;
+    }
+}
+
+// ---------------------------------------------------------------- four neighbours of a row
+template <class T> struct Four;
+template <> struct Four<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Four<bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
+
+template <class T> __device__ __forceinline__ f32x4 load4(const char* row, uint32_t n, uint32_t count) {
+    const T* p = reinterpret_cast<const T*>(row) + n;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n + 4 <= count) {
+        const typename Four<T>::type t = *reinterpret_cast<const typename Four<T>::type*>(p);
+        v = f32x4{float(t[0]), float(t[1]), float(t[2]), float(t[3])};
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            if (n + i < count) v[i] = float(p[i]);
+    }
+    return v;
+}
+template <class T> __device__ __forceinline__ void store4(char* row, uint32_t n, uint32_t count, f32x4 v) {
+    T* p = reinterpret_cast<T*>(row) + n;
+    if (n + 4 <= count) {
+        *reinterpret_cast<typename Four<T>::type*>(p) = typename Four<T>::type{T(v[0]), T(v[1]), T(v[2]), T(v[3])};
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            if (n + i < count) p[i] = T(v[i]);
+    }
+}
+template <class T> __device__ __forceinline__ char* row_of(const Matrix& m, uint32_t row) { return m.p + int64_t(row) * m.ld * int64_t(sizeof(T)); }
+
+}  // namespace dense
+
+#endif

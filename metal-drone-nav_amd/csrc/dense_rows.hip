@@ -1,0 +1,145 @@
+// dense_rows.hip — the forward call of few rows: a tick of a few vehicles, whose
+// cost is reading the weights once.
+//
+// A workgroup makes 16 columns of the result for up to 16 MT rows.  Its W
+// wavefronts take turns along k, 128 bytes of each of the 16 weight rows at a
+// time (whole lines, straight to registers, UNROLL of them on their way), as
+// operands of 16 x 16 tiles; their sums meet in LDS.
+#include "dense.h"
+
+#include "dense_tiles.h"
+#include "dense_act.h"
+
+namespace dense {
+namespace {
+
+template <class T> struct Word;
+template <> struct Word<bf16> { typedef bf16x8 type; };
+template <> struct Word<float> { typedef f32x4 type; };
+
+__device__ __forceinline__ void mma16(f32x4& acc, const bf16x8& a, const bf16x8& b) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(f32x4& acc, const f32x4& a, const f32x4& b) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+}
+
+// One word of a row; places past its end are 0.
+template <class T, bool WORDS> __device__ __forceinline__ typename Word<T>::type word_at(const T* row, uint32_t k, uint32_t width) {
+    typedef typename Word<T>::type V;
+    V v;
+#pragma unroll
+    for (uint32_t i = 0; i < per_word<T>(); i++) v[i] = T(0.0f);
+    if (WORDS) {
+        if (k < width) v = *reinterpret_cast<const V*>(row + k);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < per_word<T>(); i++)
+            if (k + i < width) v[i] = row[k + i];
+    }
+    return v;
+}
+
+template <class T, int MT, int W, bool G, bool WORDS>
+__global__ void __launch_bounds__(64 * W) rows_kernel(Args a) {
+    constexpr int N = G ? 2 : 1, UNROLL = WORDS ? (MT * N <= 2 ? 4 : 2) : 1;
+    __shared__ f32x4 part[W][N * MT][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT, rows = uint32_t(a.rows);
+    const T *w[N], *x[MT];
+    const uint32_t n = n0 + (lane & 15) < a.out ? n0 + (lane & 15) : a.out - 1;
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = reinterpret_cast<const T*>(a.w[i].p) + int64_t(n) * a.w[i].ld;
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+        const uint32_t m = m0 + 16 * j + (lane & 15);
+        x[j] = reinterpret_cast<const T*>(a.x.p) + int64_t(m < rows ? m : rows - 1) * a.x.ld;
+    }
+    f32x4 acc[N][MT];
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t step = step_of<T>(), at = (lane >> 4) * per_word<T>();
+    for (uint32_t k = wave * step; k < a.in; k += W * step * UNROLL) {
+        typename Word<T>::type fw[UNROLL][2][N], fx[UNROLL][2][MT];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t c = k + u * W * step + h * (step / 2) + at;
+#pragma unroll
+                for (int i = 0; i < N; i++) fw[u][h][i] = word_at<T, WORDS>(w[i], c, a.in);
+#pragma unroll
+                for (int j = 0; j < MT; j++) fx[u][h][j] = word_at<T, WORDS>(x[j], c, a.in);
+            }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int j = 0; j < MT; j++) mma16(acc[i][j], fw[u][h][i], fx[u][h][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) part[wave][i * MT + j][lane] = acc[i][j];
+    __syncthreads();
+    // a wavefront sums up and finishes every W-th tile of 16 rows
+    for (int j = wave; j < MT; j += W) {
+        f32x4 z[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            z[i] = part[0][i * MT + j][lane];
+#pragma unroll
+            for (int s = 1; s < W; s++) z[i] += part[s][i * MT + j][lane];
+        }
+        const uint32_t m = m0 + 16 * j + (lane & 15), c = n0 + 4 * (lane >> 4);
+        if (m >= rows || c >= a.out) continue;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (a.b[i]) z[i] += load4<T>(a.b[i], c, a.out);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = act_of<T>(a.activation, z[0][e]);
+        if constexpr (G) v = v * z[1];
+        if (!G && a.residual.p) v = load4<T>(row_of<T>(a.residual, m), c, a.out) + v;
+        store4<T>(row_of<T>(a.y, m), c, a.out, v);
+    }
+}
+
+template <class T, int MT, int W, bool G> hipError_t launch(const Args& a, bool words, hipStream_t st) {
+    const dim3 grid((a.out + 15) / 16, uint32_t((a.rows + 16 * MT - 1) / (16 * MT)));
+    if (words)
+        rows_kernel<T, MT, W, G, true><<<grid, dim3(64 * W), 0, st>>>(a);
+    else
+        rows_kernel<T, MT, W, G, false><<<grid, dim3(64 * W), 0, st>>>(a);
+    return hipGetLastError();
+}
+template <class T, int MT, bool G> hipError_t by_waves(const Args& a, bool words, hipStream_t st) {
+    const uint32_t steps = (a.in + step_of<T>() - 1) / step_of<T>();
+    if (steps <= 4) return launch<T, MT, 2, G>(a, words, st);
+    if (steps <= 16) return launch<T, MT, 4, G>(a, words, st);
+    return launch<T, MT, 8, G>(a, words, st);
+}
+template <class T, bool G> hipError_t by_rows(const Args& a, bool words, hipStream_t st) {
+    if (a.rows <= 16) return by_waves<T, 1, G>(a, words, st);
+    return by_waves<T, 2, G>(a, words, st);
+}
+
+}  // namespace
+
+bool few_rows(const Args& a) { return a.rows <= 32; }
+
+hipError_t forward_few(const Args& a, hipStream_t st) {
+    const uint32_t size = a.bf ? 2 : 4, per = 16 / size;
+    const auto words = [&](const Matrix& m) { return m.ld % per == 0 && reinterpret_cast<uintptr_t>(m.p) % 16 == 0; };
+    const bool all = a.in % per == 0 && words(a.x) && words(a.w[0]) && (!a.gated || words(a.w[1]));
+    if (a.bf) return a.gated ? by_rows<bf16, true>(a, all, st) : by_rows<bf16, false>(a, all, st);
+    return a.gated ? by_rows<float, true>(a, all, st) : by_rows<float, false>(a, all, st);
+}
+
+}  // namespace dense

@@ -31,7 +31,8 @@ EXPORTS = [
     "mdn_checkpoint_read_params", "mdn_op_normalize_noalloc", "mdn_sim_get_bank", "mdn_sim_set_camera",
     "mdn_sim_get_camera", "mdn_ppo_grad_norm_summary", "mdn_lppo_grad_norm_summary", "mdn_op_delta_rule_forward",
     "mdn_op_delta_rule_backward", "mdn_op_delta_rule_sizes", "mdn_op_block_norm_forward", "mdn_op_block_norm_backward",
-    "mdn_op_block_norm_workspace_bytes",
+    "mdn_op_block_norm_workspace_bytes", "mdn_op_dense_forward_bytes", "mdn_op_dense_forward",
+    "mdn_op_dense_backward_bytes", "mdn_op_dense_backward",
 ]
 
 P = ctypes.c_void_p
@@ -139,6 +140,10 @@ def lib():
         _sig(L, "mdn_op_block_norm_forward", I32, P, P)
         _sig(L, "mdn_op_block_norm_backward", I32, P, P, P, U64, P)
         _sig(L, "mdn_op_block_norm_workspace_bytes", I32, P, ctypes.POINTER(U64))
+        _sig(L, "mdn_op_dense_forward_bytes", I32, P, ctypes.POINTER(U64))
+        _sig(L, "mdn_op_dense_forward", I32, P, P, U64, P)
+        _sig(L, "mdn_op_dense_backward_bytes", I32, P, P, ctypes.POINTER(U64))
+        _sig(L, "mdn_op_dense_backward", I32, P, P, P, U64, P)
         _lib = L
     return _lib
 

@@ -1,0 +1,186 @@
+"""Operators of a policy network and its loss over torch tensors on the GPU:
+the linear layer with bias, activation and residual (``linear``) and the
+gated feed-forward block (``gated_feed_forward``), both with gradients.
+
+They go with ``sequence``, whose ``block_norm`` has the norms around such a
+block, and follow its rules: device tensors as they are, on torch's current
+stream; a lazily negated view is to be resolved before; torch is imported
+before the library is first used.
+"""
+import ctypes
+import struct
+
+import torch
+import torch.autograd.function
+
+from .native import P, check
+from .sequence import _DTYPES, _address, _buffer, _device, _library, _like, _no_tangents, _on, _shape, _stream, _wide
+
+ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "sigmoid": 3, "silu": 4, "gelu": 5, "gelu_tanh": 6}
+
+
+class _Matrix(ctypes.Structure):
+    _fields_ = [("data", P), ("row", ctypes.c_int64)]
+
+
+class _Dense(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_uint64)]
+    _fields_ += [(n, ctypes.c_uint32) for n in ("in_", "out", "dtype", "activation", "gated")]
+    _fields_ += [(n, _Matrix) for n in ("x", "w", "w_up", "residual", "y")]
+    _fields_ += [("b", P), ("b_up", P)]
+
+
+class _DenseGrad(ctypes.Structure):
+    _fields_ = [(n, _Matrix) for n in ("d_y", "d_x", "d_w", "d_w_up")]
+    _fields_ += [("d_b", P), ("d_b_up", P)]
+
+
+# The structs as packed bytes, made of plain numbers in one call each.
+_DENSE = struct.Struct("=Q5I4x12q")
+_DENSE_GRAD = struct.Struct("=10q")
+assert _DENSE.size == ctypes.sizeof(_Dense) and _DENSE_GRAD.size == ctypes.sizeof(_DenseGrad)
+_NONE = (0, 0)
+
+
+def _matrix(t):
+    """The rows of `t`, [..., width], as an address and the elements from row to row; another layout is copied.
+    The tensor is returned too: it holds the memory."""
+    if t.is_contiguous():
+        return t, (t.data_ptr(), t.shape[-1])
+    t = _wide(t)
+    row = None
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if row is None:
+            row, joined = stride, size * stride
+        elif stride == joined:
+            joined *= size
+        else:
+            t = t.contiguous()
+            return t, (t.data_ptr(), t.shape[-1])
+    return t, (t.data_ptr(), t.shape[-1] if row is None else row)
+
+
+class _DenseCall:
+    """Checked arguments of one call of a linear layer or a gated block: the C struct and what it points to."""
+
+    def __init__(self, names, x, w, w_up, b, b_up, residual, activation):
+        self.device = _device(names, (x, w, w_up, b, b_up, residual))
+        activation = "none" if activation is None else activation
+        if activation not in ACTIVATIONS:
+            raise ValueError("activation is one of %s, not %r" % (", ".join(ACTIVATIONS), activation))
+        if x.dim() < 1:
+            raise ValueError("x is [..., in]")
+        if w.dim() != 2:
+            raise ValueError("%s is [out, in]" % names[1])
+        out, width = w.shape
+        _shape("x", x, (*x.shape[:-1], width))
+        if not 1 <= width <= 65536 or not 1 <= out <= 65536:
+            raise ValueError("widths are 1..65536, not %d and %d" % (width, out))
+        dtype = x.dtype
+        if dtype not in _DTYPES:
+            raise TypeError("x is %s: float32 or bfloat16 are taken" % dtype)
+        self.shape = (*x.shape[:-1], out)
+        for name, t, shape in zip(names[1:], (w, w_up, b, b_up, residual), (w.shape, w.shape, (out,), (out,), self.shape)):
+            if t is None:
+                continue
+            _shape(name, t, shape)
+            if t.dtype != dtype:
+                raise TypeError("%s is %s and x %s: one type is taken" % (name, t.dtype, dtype))
+        self.rows, self.gated, self.dtype = x.numel() // width, w_up is not None, dtype
+        if self.rows > 0x7fffff00:
+            raise ValueError("%d rows are too many" % self.rows)
+        self.x, mx = _matrix(x)
+        self.w, mw = _matrix(w)
+        self.w_up, mu = (None, _NONE) if w_up is None else _matrix(w_up)
+        self.residual, mr = (None, _NONE) if residual is None else _matrix(residual)
+        self.b, self.b_up = (None if t is None else t.contiguous() for t in (b, b_up))
+        self.c = _Dense.from_buffer_copy(_DENSE.pack(
+            self.rows, width, out, _DTYPES[dtype], ACTIVATIONS[activation], self.gated, *mx, *mw, *mu, *mr, *_NONE,
+            _address(self.b) or 0, _address(self.b_up) or 0))
+
+    def forward(self):
+        L = _library()
+        y = torch.empty(self.shape, dtype=self.dtype, device=self.device)
+        c = self.c
+        c.y.data, c.y.row = y.data_ptr(), c.out
+        size = ctypes.c_uint64()
+        check(L.mdn_op_dense_forward_bytes(ctypes.byref(c), ctypes.byref(size)))
+        work = _buffer(size.value, self.device)
+        check(L.mdn_op_dense_forward(ctypes.byref(c), _address(work), size.value, _stream(self.device)))
+        return y
+
+    def backward(self, d_y, want):
+        """(d_x, d_w, d_w_up, d_b, d_b_up), None where `want` is false"""
+        L = _library()
+        d_y, my = _matrix(d_y)
+        made = [_like(t) if wanted and t is not None else None
+                for wanted, t in zip(want, (self.x, self.w, self.w_up, self.b, self.b_up))]
+        if self.rows == 0:
+            return [None if t is None else t.zero_() for t in made]
+        at = [(0 if t is None else t.data_ptr(), 0 if t is None else t.shape[-1]) for t in made]
+        d = _DenseGrad.from_buffer_copy(_DENSE_GRAD.pack(*my, *at[0], *at[1], *at[2], at[3][0], at[4][0]))
+        size = ctypes.c_uint64()
+        check(L.mdn_op_dense_backward_bytes(ctypes.byref(self.c), ctypes.byref(d), ctypes.byref(size)))
+        work = _buffer(size.value, self.device)
+        check(L.mdn_op_dense_backward(ctypes.byref(self.c), ctypes.byref(d), _address(work), size.value,
+                                      _stream(self.device)))
+        return made
+
+
+class _DenseFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, names, activation, x, w, w_up, b, b_up, residual):
+        call = _DenseCall(names, x, w, w_up, b, b_up, residual, activation)
+        ctx.names, ctx.activation, ctx.like = names, activation, residual is not None
+        ctx.save_for_backward(x, w, w_up, b, b_up)
+        return _on(call.device, call.forward)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_y):
+        want = ctx.needs_input_grad
+        d_residual = d_y if ctx.like and want[7] else None
+        if not any(want[2:7]):
+            return (*[None] * 7, d_residual)
+        call = _DenseCall(ctx.names, *ctx.saved_tensors, None, ctx.activation)
+        grads = _on(call.device, call.backward, d_y, want[2:7])
+        return (None, None, *grads, d_residual)
+
+
+def _dense(names, activation, *args):
+    _no_tangents(*args)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
+        return _DenseFunction.apply(names, activation, *args)
+    call = _DenseCall(names, *args, activation)
+    return _on(call.device, call.forward)
+
+
+_LINEAR = ("x", "weight", "weight", "bias", "bias", "residual")
+_GATED = ("x", "w_gate", "w_up", "b_gate", "b_up", "residual")
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """residual + act(x weight^T + bias), rounded once.
+
+    x: [..., in], weight: [out, in], bias: [out], residual: [..., out], all
+    float32 or all bfloat16; widths up to 65,536.  activation: "none" (or
+    None), "relu", "tanh", "sigmoid", "silu", "gelu" or "gelu_tanh".  Any
+    leading strides go; operands whose rows are not whole, aligned 16-byte
+    words are copied first.  Gradients reach every tensor argument; the
+    activation's argument is made again for them and not kept, and its gradient
+    enters the products that follow with the rows' type.
+    """
+    return _dense(_LINEAR, activation, x, weight, None, bias, None, residual)
+
+
+def gated_feed_forward(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
+    """act(x w_gate^T + b_gate) * (x w_up^T + b_up), rounded once.
+
+    x: [..., in], w_gate, w_up: [out, in], b_gate, b_up: [out]; types,
+    activations, strides and gradients as in ``linear``.
+    """
+    if not isinstance(w_up, torch.Tensor):
+        raise TypeError("w_up is no tensor")
+    return _dense(_GATED, activation, x, w_gate, w_up, b_gate, b_up, None)
