@@ -563,6 +563,49 @@ int mdn_op_dense_backward_bytes(const MdnDense* dense, const MdnDenseGrad* grad,
 int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void* workspace, uint64_t workspace_bytes,
                           void* stream);
 
+/* The clipped loss of a policy over discrete choices.  A step has `heads`
+ * independent choices among `choices` each (four commands of so many levels, or
+ * one of many manoeuvres); over its heads
+ *     l = sum of log softmax(logits)[action],  H = sum of the heads' entropies
+ *     r = exp(l - old_log_prob)
+ *     L = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef K - entropy_coef H
+ *     K = exp(ref_log_prob - l) - (ref_log_prob - l) - 1   (0 without ref_log_prob)
+ * and the loss is the mean of L over the steps whose mask is not 0 (all, if
+ * mask is NULL); if none counts, it and its gradient are 0, and nothing of a
+ * step that does not count is looked at.  A logit of -inf rules a choice out.
+ * An action that is none of the choices, and a step all of whose choices are
+ * ruled out, has no log-probability: NaN, and so has the loss.
+ *
+ * Logits are fp32 or bfloat16, [steps][heads][choices] with strides of elements
+ * and contiguous choices; exponentials and their sums are fp32, everything a
+ * step makes of them is 64 bits, and so is the sum where r is so near to the
+ * clip's border that 32 bits could not tell its side.  heads and choices are
+ * at least 1, choices below 2^24, steps heads choices below 2^48. */
+typedef struct MdnChoices {
+    uint64_t steps;
+    uint32_t heads, choices, dtype, action_bytes; /* action_bytes: 4 or 8 (int32_t, int64_t) */
+    const void* logits;
+    int64_t step, head;
+    const void* actions;                          /* [steps][heads] */
+} MdnChoices;
+/* What acting stores: l and H of every step. */
+int mdn_op_choices_log_prob(const MdnChoices* choices, float* log_prob, float* entropy, void* stream);
+
+typedef struct MdnChoiceLoss {
+    const float *old_log_prob, *advantages, *ref_log_prob; /* [steps]; ref_log_prob may be NULL */
+    const uint8_t* mask;                                   /* [steps], or NULL */
+    double clip_low, clip_high, kl_coef, entropy_coef;
+    float* loss; /* [6]: the loss, then the means of -min(..), K, H, r and of r outside the clip's borders */
+} MdnChoiceLoss;
+/* Bytes of `keep`, which the backward pass reads, and of the workspace. */
+int mdn_op_choices_loss_sizes(const MdnChoices* choices, uint64_t* keep, uint64_t* workspace);
+int mdn_op_choices_loss_forward(const MdnChoices* choices, const MdnChoiceLoss* loss, void* keep, uint64_t keep_bytes,
+                                void* workspace, uint64_t workspace_bytes, void* stream);
+/* The gradient of loss[0] by the logits times *d_loss, contiguous and of
+ * their type; `loss` as in the forward call (its result is not read). */
+int mdn_op_choices_loss_backward(const MdnChoices* choices, const MdnChoiceLoss* loss, const void* keep,
+                                 uint64_t keep_bytes, const float* d_loss, void* d_logits, void* stream);
+
 /* Test support, no counterpart in the reference: the kernels divide by
  * constants (plant mass and rotor time constants, the RK4 weight 6, the
  * observation scales) as (float)((double)x * (1.0 / (double)b)).  For each

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "block_norm.h"
+#include "choices.h"
 #include "delta_rule.h"
 #include "dense.h"
 #include "kernel_args.h"
@@ -2482,6 +2483,93 @@ int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void*
     const uint64_t need = a.rows ? dense::backward_bytes(a, d) : 0;
     if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_dense_backward: workspace is too small");
     HIP_TRY(dense::backward(a, d, static_cast<char*>(workspace), static_cast<hipStream_t>(stream)));
+    return MDN_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+int choice_args(const char* name, const MdnChoices* c, choices::Args* out) {
+    const std::string who = std::string(name) + ": ";
+    if (!c) return fail(MDN_E_ARG, who + "null");
+    if (c->dtype > MDN_BF16) return fail(MDN_E_ARG, who + "dtype must be MDN_F32 or MDN_BF16");
+    if (c->action_bytes != 4 && c->action_bytes != 8) return fail(MDN_E_ARG, who + "action_bytes must be 4 or 8");
+    if (c->heads < 1 || c->heads > 65536 || c->choices < 1 || c->choices >= (1u << 24))
+        return fail(MDN_E_ARG, who + "heads must be 1..65536 and choices 1..2^24 - 1");
+    if (c->steps > (1ull << 48) / (uint64_t(c->heads) * c->choices)) return fail(MDN_E_ARG, who + "too many steps");
+    if (c->steps && (!c->logits || !c->actions)) return fail(MDN_E_ARG, who + "null rows");
+    choices::Args a{};
+    a.steps = c->steps; a.heads = c->heads; a.choices = c->choices; a.bf = c->dtype == MDN_BF16; a.index64 = c->action_bytes == 8;
+    a.logits = static_cast<const char*>(c->logits); a.step = c->step; a.head = c->head;
+    a.actions = static_cast<const char*>(c->actions);
+    *out = a;
+    return MDN_OK;
+}
+int choice_loss_args(const char* name, const MdnChoices* c, const MdnChoiceLoss* l, const void* keep, uint64_t keep_bytes,
+                     choices::Args* out) {
+    choices::Args a;
+    if (int rc = choice_args(name, c, &a)) return rc;
+    const std::string who = std::string(name) + ": ";
+    if (!l) return fail(MDN_E_ARG, who + "null");
+    if (a.steps && (!l->old_log_prob || !l->advantages)) return fail(MDN_E_ARG, who + "null rows");
+    if (!(l->clip_low >= 0.0) || !(l->clip_high >= 0.0)) return fail(MDN_E_ARG, who + "clip_low and clip_high must be at least 0");
+    if (l->kl_coef != 0.0 && !l->ref_log_prob) return fail(MDN_E_ARG, who + "kl_coef needs ref_log_prob");
+    if (keep_bytes < choices::keep_floats(a) * sizeof(float) || !keep) return fail(MDN_E_ARG, who + "keep is too small");
+    a.old_log_prob = l->old_log_prob; a.advantages = l->advantages; a.ref_log_prob = l->ref_log_prob; a.mask = l->mask;
+    a.low = l->clip_low; a.high = l->clip_high; a.kl_coef = l->kl_coef; a.entropy_coef = l->entropy_coef;
+    a.loss = l->loss;
+    a.stats = static_cast<float*>(const_cast<void*>(keep));
+    a.slopes = a.stats + a.steps * a.heads * 3;
+    a.one_over = a.slopes + a.steps;
+    *out = a;
+    return MDN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mdn_op_choices_log_prob(const MdnChoices* choices, float* log_prob, float* entropy, void* stream) {
+    choices::Args a;
+    if (int rc = choice_args("mdn_op_choices_log_prob", choices, &a)) return rc;
+    if (a.steps == 0) return MDN_OK;
+    if (!log_prob || !entropy) return fail(MDN_E_ARG, "mdn_op_choices_log_prob: null rows");
+    a.log_prob = log_prob;
+    a.entropy = entropy;
+    HIP_TRY(choices::launch_log_prob(a, static_cast<hipStream_t>(stream)));
+    return MDN_OK;
+}
+
+int mdn_op_choices_loss_sizes(const MdnChoices* choices, uint64_t* keep, uint64_t* workspace) {
+    choices::Args a;
+    if (int rc = choice_args("mdn_op_choices_loss_sizes", choices, &a)) return rc;
+    if (!keep || !workspace) return fail(MDN_E_ARG, "mdn_op_choices_loss_sizes: null");
+    *keep = choices::keep_floats(a) * sizeof(float);
+    *workspace = uint64_t(choices::parts_of(a)) * 6 * sizeof(double);
+    return MDN_OK;
+}
+
+int mdn_op_choices_loss_forward(const MdnChoices* choices, const MdnChoiceLoss* loss, void* keep, uint64_t keep_bytes,
+                                void* workspace, uint64_t workspace_bytes, void* stream) {
+    choices::Args a;
+    if (int rc = choice_loss_args("mdn_op_choices_loss_forward", choices, loss, keep, keep_bytes, &a)) return rc;
+    if (!a.loss) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: null loss");
+    const uint64_t need = uint64_t(choices::parts_of(a)) * 6 * sizeof(double);
+    if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: workspace is too small");
+    a.parts = static_cast<double*>(workspace);
+    HIP_TRY(choices::launch_loss(a, static_cast<hipStream_t>(stream)));
+    return MDN_OK;
+}
+
+int mdn_op_choices_loss_backward(const MdnChoices* choices, const MdnChoiceLoss* loss, const void* keep, uint64_t keep_bytes,
+                                 const float* d_loss, void* d_logits, void* stream) {
+    choices::Args a;
+    if (int rc = choice_loss_args("mdn_op_choices_loss_backward", choices, loss, keep, keep_bytes, &a)) return rc;
+    if (a.steps == 0) return MDN_OK;
+    if (!d_loss || !d_logits) return fail(MDN_E_ARG, "mdn_op_choices_loss_backward: null rows");
+    const choices::GradArgs d{d_loss, static_cast<char*>(d_logits)};
+    HIP_TRY(choices::launch_loss_backward(a, d, static_cast<hipStream_t>(stream)));
     return MDN_OK;
 }
 

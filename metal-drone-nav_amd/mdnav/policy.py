@@ -1,6 +1,8 @@
 """Operators of a policy network and its loss over torch tensors on the GPU:
-the linear layer with bias, activation and residual (``linear``) and the
-gated feed-forward block (``gated_feed_forward``), both with gradients.
+the linear layer with bias, activation and residual (``linear``), the gated
+feed-forward block (``gated_feed_forward``) and the clipped loss of a policy
+over discrete choices (``clipped_loss``), all with gradients, and the
+log-probabilities that acting stores for that loss (``log_prob``).
 
 They go with ``sequence``, whose ``block_norm`` has the norms around such a
 block, and follow its rules: device tensors as they are, on torch's current
@@ -14,7 +16,8 @@ import torch
 import torch.autograd.function
 
 from .native import P, check
-from .sequence import _DTYPES, _address, _buffer, _device, _library, _like, _no_tangents, _on, _shape, _stream, _wide
+from .sequence import (_DTYPES, _address, _buffer, _device, _library, _like, _no_tangents, _number, _on, _shape, _stream,
+                       _wide)
 
 ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "sigmoid": 3, "silu": 4, "gelu": 5, "gelu_tanh": 6}
 
@@ -35,10 +38,25 @@ class _DenseGrad(ctypes.Structure):
     _fields_ += [("d_b", P), ("d_b_up", P)]
 
 
+class _Choices(ctypes.Structure):
+    _fields_ = [("steps", ctypes.c_uint64)]
+    _fields_ += [(n, ctypes.c_uint32) for n in ("heads", "choices", "dtype", "action_bytes")]
+    _fields_ += [("logits", P), ("step", ctypes.c_int64), ("head", ctypes.c_int64), ("actions", P)]
+
+
+class _ChoiceLoss(ctypes.Structure):
+    _fields_ = [(n, P) for n in ("old_log_prob", "advantages", "ref_log_prob", "mask")]
+    _fields_ += [(n, ctypes.c_double) for n in ("clip_low", "clip_high", "kl_coef", "entropy_coef")]
+    _fields_ += [("loss", P)]
+
+
 # The structs as packed bytes, made of plain numbers in one call each.
 _DENSE = struct.Struct("=Q5I4x12q")
 _DENSE_GRAD = struct.Struct("=10q")
 assert _DENSE.size == ctypes.sizeof(_Dense) and _DENSE_GRAD.size == ctypes.sizeof(_DenseGrad)
+_CHOICES = struct.Struct("=Q4I4q")
+_CHOICE_LOSS = struct.Struct("=4q4dq")
+assert _CHOICES.size == ctypes.sizeof(_Choices) and _CHOICE_LOSS.size == ctypes.sizeof(_ChoiceLoss)
 _NONE = (0, 0)
 
 
@@ -184,3 +202,159 @@ def gated_feed_forward(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu
     if not isinstance(w_up, torch.Tensor):
         raise TypeError("w_up is no tensor")
     return _dense(_GATED, activation, x, w_gate, w_up, b_gate, b_up, None)
+
+
+# ---------------------------------------------------------------- discrete choices
+class _ChoiceCall:
+    """Checked logits and actions: the C struct and what it points to."""
+
+    def __init__(self, logits, actions, more=(), names=()):
+        self.device = _device(("logits", "actions", *names), (logits, actions, *more))
+        if logits.dim() < 2:
+            raise ValueError("logits are [..., heads, choices]")
+        heads, choices = logits.shape[-2:]
+        self.shape = logits.shape[:-2]
+        _shape("actions", actions, logits.shape[:-1])
+        if heads < 1 or heads > 65536 or choices < 1 or choices >= 1 << 24:
+            raise ValueError("heads are 1..65536 and choices 1..2^24 - 1, not %d and %d" % (heads, choices))
+        if logits.dtype not in _DTYPES:
+            raise TypeError("logits are %s: float32 or bfloat16 are taken" % logits.dtype)
+        if actions.dtype not in (torch.int64, torch.int32):
+            raise TypeError("actions are %s: int64 or int32 are taken" % actions.dtype)
+        self.steps = logits.numel() // (heads * choices)
+        rows = _wide(logits)
+        try:
+            rows = rows.view(self.steps, heads, choices)
+        except RuntimeError:
+            rows = rows.contiguous().view(self.steps, heads, choices)
+        self.logits, self.actions = rows, actions.contiguous()
+        self.c = _Choices.from_buffer_copy(_CHOICES.pack(
+            self.steps, heads, choices, _DTYPES[logits.dtype], self.actions.element_size(), rows.data_ptr(),
+            rows.stride(0), rows.stride(1), self.actions.data_ptr()))
+
+    def results(self, *shape):
+        return torch.empty(shape, dtype=torch.float32, device=self.device)
+
+    def log_prob(self):
+        log_prob, entropy = self.results(*self.shape), self.results(*self.shape)
+        check(_library().mdn_op_choices_log_prob(ctypes.byref(self.c), log_prob.data_ptr(), entropy.data_ptr(),
+                                                 _stream(self.device)))
+        return log_prob, entropy
+
+
+class _LossCall(_ChoiceCall):
+    """The same with the loss's other arguments."""
+
+    NAMES = ("old_log_prob", "advantages", "ref_log_prob", "mask")
+
+    def __init__(self, logits, actions, old_log_prob, advantages, ref_log_prob, mask, low, high, kl_coef, entropy_coef):
+        rows = (old_log_prob, advantages, ref_log_prob, mask)
+        super().__init__(logits, actions, rows, self.NAMES)
+        for name, t in zip(self.NAMES, rows):
+            if t is None:
+                continue
+            _shape(name, t, self.shape)
+            if name == "mask":
+                if t.dtype not in (torch.uint8, torch.bool):
+                    raise TypeError("mask is %s: uint8 or bool are taken" % t.dtype)
+            elif t.dtype != torch.float32:
+                raise TypeError("%s is %s: float32 is taken" % (name, t.dtype))
+        self.rows = [None if t is None else t.contiguous() for t in rows]
+        self.l = _ChoiceLoss.from_buffer_copy(_CHOICE_LOSS.pack(*(_address(t) or 0 for t in self.rows), low, high, kl_coef,
+                                                                entropy_coef, 0))
+
+    def forward(self):
+        L = _library()
+        keep, work = ctypes.c_uint64(), ctypes.c_uint64()
+        check(L.mdn_op_choices_loss_sizes(ctypes.byref(self.c), ctypes.byref(keep), ctypes.byref(work)))
+        kept, buffer, out = _buffer(keep.value, self.device), _buffer(work.value, self.device), self.results(6)
+        self.l.loss = out.data_ptr()
+        check(L.mdn_op_choices_loss_forward(ctypes.byref(self.c), ctypes.byref(self.l), _address(kept), keep.value,
+                                            _address(buffer), work.value, _stream(self.device)))
+        return out, kept
+
+    def backward(self, kept, d_loss, shape):
+        made = torch.empty(shape, dtype=self.logits.dtype, device=self.device)
+        check(_library().mdn_op_choices_loss_backward(
+            ctypes.byref(self.c), ctypes.byref(self.l), _address(kept), kept.numel(), d_loss.data_ptr(), made.data_ptr(),
+            _stream(self.device)))
+        return made
+
+
+class _LossFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, actions, old_log_prob, advantages, ref_log_prob, mask, *numbers):
+        call = _LossCall(logits, actions, old_log_prob, advantages, ref_log_prob, mask, *numbers)
+        out, kept = _on(call.device, call.forward)
+        ctx.numbers = numbers
+        ctx.save_for_backward(logits, actions, old_log_prob, advantages, ref_log_prob, mask, kept)
+        loss, metrics = out[0].clone(), out[1:]
+        ctx.mark_non_differentiable(metrics)
+        ctx.set_materialize_grads(False)
+        return loss, metrics
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, _):
+        if d_loss is None:
+            return (None,) * 10
+        *rows, kept = ctx.saved_tensors
+        call = _LossCall(*rows, *ctx.numbers)
+        return (_on(call.device, call.backward, kept, d_loss.contiguous(), rows[0].shape), *[None] * 9)
+
+
+def _data(name, x):
+    """Refuses a tensor that wants a gradient where there is none."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        raise TypeError("%s is data: it has no gradient here" % name)
+
+
+def clipped_loss(logits, actions, old_log_prob, advantages, ref_log_prob=None, mask=None, clip=0.2, kl_coef=0.0,
+                 entropy_coef=0.0):
+    """The clipped loss of a policy over discrete choices: (loss, metrics).
+
+    logits: [..., heads, choices], float32 or bfloat16: the independent choices
+    of a step, four commands of so many levels or one of many manoeuvres.
+    actions: [..., heads] int64 or int32.  old_log_prob, advantages,
+    ref_log_prob: [...] float32, mask: [...] bool or uint8.  With l the sum of
+    the heads' log-probabilities, H that of their entropies,
+    r = exp(l - old_log_prob) and K = exp(ref_log_prob - l) -
+    (ref_log_prob - l) - 1 (0 without ref_log_prob), the loss is the mean of
+
+        -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef K - entropy_coef H
+
+    over the steps whose mask is set; ``clip`` is low and high alike, or a pair.
+    metrics: the means of -min(..), K, H, r, and of r outside the borders.  No
+    step that counts: all is 0.  Steps that do not count are not looked at, a
+    logit of -inf rules a choice out, an action that is none of the choices
+    gives NaN.  The gradient reaches the logits alone.
+    """
+    rows = (old_log_prob, advantages, ref_log_prob, mask)
+    _no_tangents(logits, *rows)
+    for name, t in zip(_LossCall.NAMES, rows):
+        _data(name, t)
+    low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    for name, x in (("clip", low), ("clip", high), ("kl_coef", kl_coef), ("entropy_coef", entropy_coef)):
+        _number(name, x)
+    numbers = (float(low), float(high), float(kl_coef), float(entropy_coef))
+    if not (numbers[0] >= 0.0 and numbers[1] >= 0.0):
+        raise ValueError("clip is at least 0, not %r" % (clip,))
+    if numbers[2] != 0.0 and ref_log_prob is None:
+        raise ValueError("kl_coef needs ref_log_prob")
+    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+        return _LossFunction.apply(logits, actions, *rows, *numbers)
+    call = _LossCall(logits, actions, *rows, *numbers)
+    out, _ = _on(call.device, call.forward)
+    return out[0], out[1:]
+
+
+def log_prob(logits, actions):
+    """(log-probability of the actions, entropy), summed over a step's heads, [...] float32: what acting stores.
+
+    logits and actions as in ``clipped_loss``.  No gradients: logits that want
+    one are refused.
+    """
+    _no_tangents(logits)
+    _data("logits", logits)
+    call = _ChoiceCall(logits, actions)
+    return _on(call.device, call.log_prob)
