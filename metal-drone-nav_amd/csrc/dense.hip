@@ -19,6 +19,8 @@
 #include "dense_tiles.h"
 #include "lane_sums.h"
 
+#include <type_traits>
+
 namespace dense {
 namespace {
 
@@ -39,13 +41,73 @@ struct Job {
 
 __device__ __forceinline__ f32x4 four(const f32x16& v, int g) { return f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]}; }
 
+// ---------------------------------------------------------------- results through LDS
+// A lane has four neighbours of one row of a tile, and 32 rows are 32 lines of
+// memory. So a wavefront turns PW columns of 32 rows at a time, in fp32 in LDS
+// of its own, and then has whole pieces of rows: a lane the word of the
+// result's type (N columns) that it moves.
+template <class T, int PW> struct Piece {
+    static constexpr uint32_t N = per_word<T>(), LANES = PW / N, ROWS = 64 / LANES, TURNS = 32 / ROWS, BYTES = 32 * PW * 4;
+    typedef T Word __attribute__((ext_vector_type(N), aligned(sizeof(T))));  // in memory: at any multiple of an element
+
+    // Orders LDS accesses of one wavefront; it serves them in order itself.
+    static __device__ __forceinline__ void order() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // Words of four columns change places by the row, so that no two lanes that LDS serves together meet in a bank.
+    static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t word) { return row * (PW * 4) + ((word ^ (row & (PW / 4 - 1))) << 4); }
+    static __device__ __forceinline__ void put(char* lds, const f32x16& tile, int i, uint32_t lane) {
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<f32x4*>(lds + at(lane & 31, 8 * i + 2 * g + (lane >> 5))) = four(tile, g);
+    }
+    static __device__ __forceinline__ uint32_t row(uint32_t lane, uint32_t turn) { return lane / LANES + turn * ROWS; }
+    static __device__ __forceinline__ uint32_t column(uint32_t lane) { return lane % LANES * N; }
+    static __device__ __forceinline__ void get(const char* lds, uint32_t row, uint32_t lane, float (&z)[N]) {
+#pragma unroll
+        for (uint32_t w = 0; w < N / 4; w++) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(lds + at(row, lane % LANES * (N / 4) + w));
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) z[4 * w + e] = v[e];
+        }
+    }
+    // One word of a row, columns c .. c + N - 1 of `count`; 0 outside.
+    static __device__ __forceinline__ void load(const Matrix& from, uint32_t m, uint32_t c, uint32_t count, float (&z)[N]) {
+        const T* p = reinterpret_cast<const T*>(from.p) + int64_t(m) * from.ld + c;
+        if (c + N <= count) {
+            const Word v = *reinterpret_cast<const Word*>(p);
+#pragma unroll
+            for (uint32_t e = 0; e < N; e++) z[e] = float(v[e]);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < N; e++) z[e] = c + e < count ? float(p[e]) : 0.0f;
+        }
+    }
+    static __device__ __forceinline__ void store(const Matrix& to, uint32_t m, uint32_t c, uint32_t count, const float (&z)[N]) {
+        T* p = reinterpret_cast<T*>(to.p) + int64_t(m) * to.ld + c;
+        if (c + N <= count) {
+            Word v;
+#pragma unroll
+            for (uint32_t e = 0; e < N; e++) v[e] = T(z[e]);
+            *reinterpret_cast<Word*>(p) = v;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < N; e++)
+                if (c + e < count) p[e] = T(z[e]);
+        }
+    }
+};
+
 // ---------------------------------------------------------------- the product
 // BN counts the rows of LDS: of the gated block's projections, half each.
-template <class T, int BM, int BN, int WM, int WN, int STAGES, bool MC, bool NC, int RESULT>
+// PAIRED: the workgroup's two wavefronts on a SIMD take turns, one reads its
+// operands of 1/4 step while the other multiplies (they are a barrier apart).
+template <class T, int BM, int BN, int WM, int WN, int STAGES, bool PAIRED, bool MC, bool NC, int RESULT>
 __global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
     constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr bool N2 = two_weights(RESULT);
-    constexpr int OUT = N2 ? BN / 2 : BN;  // columns of the result
+    constexpr int OUT = N2 ? BN / 2 : BN, TO = N2 ? TN / 2 : TN;  // columns of the result, and a wavefront's tiles of them
     static_assert(TM >= 1 && TN >= (N2 ? 2 : 1), "");
     typedef Staged<T, BM, W, MC, false> SideM;
     typedef Staged<T, BN, W, NC, N2> SideN;
@@ -61,7 +123,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
     uint32_t mt, nt;
     {
         const uint32_t tiles = a.m_tiles * a.n_tiles, xcd = blockIdx.x & 7, per = tiles / 8, rest = tiles % 8;
-        uint32_t t = xcd * per + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+        const uint32_t t = xcd * per + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
         const uint32_t band = t / (8 * a.m_tiles), in = t - band * 8 * a.m_tiles;
         const uint32_t wide = a.n_tiles - band * 8 < 8 ? a.n_tiles - band * 8 : 8;
         mt = in / wide;
@@ -81,19 +143,6 @@ __global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
         sm.init(m, mt * BM, wave, lane);
         sn.init(a.n, nt * OUT, wave, lane);
     }
-    typename SideM::Reader rm;
-    typename SideN::Reader rn;
-    rm.init(lane);
-    rn.init(lane);
-
-    f32x16 acc[TN][TM];
-#pragma unroll
-    for (int i = 0; i < TN; i++)
-#pragma unroll
-        for (int j = 0; j < TM; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-
     const uint32_t steps = (k_end - k_first + step_of<T>() - 1) / step_of<T>(), total = steps * a.segments;
     uint32_t next = 0, next_k = k_first, into = 0;  // the step to load, its k, its stage
     bool second = false;
@@ -116,108 +165,171 @@ __global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
     };
     for (int s = 0; s < STAGES - 1; s++)
         if (uint32_t(s) < total) fetch();
-    uint32_t from = 0;
-    for (uint32_t s = 0; s < total; s++) {
-        // this step's words are there for all, and all have read the step before it
-        if (STAGES > 2 && s + STAGES - 2 < total)
-            landed<LOADS*(STAGES - 2)>();
-        else
-            landed<0>();
-        if (next < total) fetch();
-        const uint32_t at_m = lds + from * STAGE, at_n = at_m + SideM::BYTES;
+
+    typename SideM::Reader rm;
+    typename SideN::Reader rn;
+    rm.init(lane);
+    rn.init(lane);
+    const uint32_t m0 = mt * BM + wm * (BM / WM), n0 = nt * OUT + wn * (OUT / WN);
+    const uint32_t mc = a.m.count, nc = a.n.count;
+    // sums begin with the bias
+    f32x16 acc[TN][TM];
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
-            Frag<T> fm[TM], fn[TN];
+    for (int i = 0; i < TN; i++) {
+        f32x16 b;
 #pragma unroll
-            for (int i = 0; i < TN; i++) {
-                const uint32_t row = N2 ? (i < TN / 2 ? 0 : BN / 2) + wn * (OUT / WN) + 32 * (i % (TN / 2 > 0 ? TN / 2 : 1)) : wn * (BN / WN) + 32 * i;
-                fn[i] = rn.get(at_n, row, kk);
-            }
+        for (int e = 0; e < 16; e++) b[e] = 0.0f;
+        if constexpr (RESULT != STORE && RESULT != PART) {
+            const char* from = a.bias[N2 && i >= TO ? 1 : 0];
+            if (from)
 #pragma unroll
-            for (int j = 0; j < TM; j++) fm[j] = rm.get(at_m, wm * (BM / WM) + 32 * j, kk);
+                for (int g = 0; g < 4; g++) {
+                    const f32x4 v = load4<T>(from, n0 + 32 * (i % TO) + 8 * g + 4 * (lane >> 5), nc);
 #pragma unroll
-            for (int i = 0; i < TN; i++)
-#pragma unroll
-                for (int j = 0; j < TM; j++) mma(acc[i][j], fn[i], fm[j]);
+                    for (int e = 0; e < 4; e++) b[4 * g + e] = v[e];
+                }
         }
-        from = from + 1 == STAGES ? 0 : from + 1;
+#pragma unroll
+        for (int j = 0; j < TM; j++) acc[i][j] = b;
     }
 
-    // ---- the result
-    const uint32_t m0 = mt * BM + wm * (BM / WM) + (lane & 31), n0 = nt * OUT + wn * (OUT / WN) + 4 * (lane >> 5);
-    const uint32_t mc = a.m.count, nc = a.n.count;
-    constexpr int TO = N2 ? TN / 2 : TN;
+    Frag<T> fm[TM], fn[TN];
+    const auto read = [&](uint32_t from, int kk) {
+        const uint32_t at_m = lds + from * STAGE, at_n = at_m + SideM::BYTES;
 #pragma unroll
-    for (int i = 0; i < TO; i++) {
+        for (int i = 0; i < TN; i++)
+            fn[i] = rn.get(at_n, (N2 && i >= TO ? BN / 2 : 0) + wn * (OUT / WN) + 32 * (i % TO), kk);
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const uint32_t n = n0 + 32 * i + 8 * g;
-            if constexpr (RESULT == STORE || RESULT == PART) {
-                const Matrix& y = batch ? a.y2 : a.y;
+        for (int j = 0; j < TM; j++) fm[j] = rm.get(at_m, wm * (BM / WM) + 32 * j, kk);
+    };
+    const auto multiply = [&]() {
 #pragma unroll
-                for (int j = 0; j < TM; j++) {
-                    const uint32_t m = m0 + 32 * j;
-                    if (m >= mc || n >= nc) continue;
-                    const f32x4 v = four(acc[i][j], g);
-                    if constexpr (RESULT == STORE)
-                        store4<T>(row_of<T>(y, m), n, nc, v);
-                    else
-                        store4<float>(row_of<float>(y, m) + uint64_t(piece) * mc * y.ld * 4, n, nc, v);
-                }
-            } else {
-                f32x4 b0 = {0.0f, 0.0f, 0.0f, 0.0f}, b1 = b0;
-                if (a.bias[0]) b0 = load4<T>(a.bias[0], n, nc);
-                if (N2 && a.bias[1]) b1 = load4<T>(a.bias[1], n, nc);
-                f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+        for (int i = 0; i < TN; i++)
 #pragma unroll
-                for (int j = 0; j < TM; j++) {
-                    const uint32_t m = m0 + 32 * j;
-                    const f32x4 z0 = four(acc[i][j], g) + b0;
-                    f32x4 z1;
-                    if constexpr (N2) z1 = four(acc[TO + i][j], g) + b1;
-                    if (m >= mc) continue;
-                    if constexpr (RESULT == LINEAR || RESULT == GATED) {
-                        if (n >= nc) continue;
-                        f32x4 v;
+            for (int j = 0; j < TM; j++) mma(acc[i][j], fn[i], fm[j]);
+    };
+    uint32_t from = 0;
+    if constexpr (PAIRED) {
+        static_assert(STAGES == 2 && W == 8, "");
+        landed<0>();
+        if (wave >= 4) landed<0>();  // the second wavefronts of the SIMDs are a barrier behind
+        for (uint32_t s = 0; s < total; s++) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) v[e] = act_of<T>(a.act, z0[e]);
-                        if constexpr (RESULT == GATED) v = v * z1;
-                        if (RESULT == LINEAR && a.residual.p) v = load4<T>(row_of<T>(a.residual, m), n, nc) + v;
-                        store4<T>(row_of<T>(a.y, m), n, nc, v);
-                    } else {
-                        // zeros past the last column: the next products read whole words
-                        f32x4 d0 = load4<T>(row_of<T>(a.dy, m), n, nc), d1 = d0;
+            for (int kk = 0; kk < 4; kk++) {
+                read(from, kk);
+                // Every wavefront has read the other stage to its end: the ones behind waited
+                // for their last reads of it before the barrier that this one has passed.
+                if (kk == 0 && next < total) fetch();
+                if (kk == 3)
+                    landed<0>();  // the next step's words too, for those who read them after the next barrier
+                else
+                    read_and_met();
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+                multiply();
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                met();
+            }
+            from ^= 1;
+        }
+        if (wave < 4) met();
+    } else {
+        for (uint32_t s = 0; s < total; s++) {
+            // this step's words are there for all, and all have read the step before it
+            if (STAGES > 2 && s + STAGES - 2 < total)
+                landed<LOADS*(STAGES - 2)>();
+            else
+                landed<0>();
+            if (next < total) fetch();
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float slope;
-                            const float v = act_of<T>(a.act, z0[e], slope);
-                            if constexpr (N2) {
-                                d1[e] = n + e < nc ? d0[e] * v : 0.0f;
-                                d0[e] = n + e < nc ? d0[e] * z1[e] * slope : 0.0f;
-                            } else
-                                d0[e] = n + e < nc ? d0[e] * slope : 0.0f;
-                        }
-                        s0 += d0;
-                        if (N2) s1 += d1;
-                        const uint32_t wide = uint32_t(a.dz_half);
-                        store4<T>(row_of<T>(a.dz, m), n, wide, d0);
-                        if (N2) store4<T>(row_of<T>(a.dz, m) + uint64_t(wide) * sizeof(T), n, wide, d1);
+            for (int kk = 0; kk < 4; kk++) {
+                read(from, kk);
+                multiply();
+            }
+            from = from + 1 == STAGES ? 0 : from + 1;
+        }
+        landed<0>();
+    }
+
+    // ---- the result, PW columns of 32 rows at a time
+    constexpr int PT = TO >= 2 ? 2 : 1, PW = 32 * PT;
+    typedef typename std::conditional<RESULT == PART, float, T>::type TR;
+    typedef Piece<TR, PW> Out;
+    constexpr uint32_t REGION = STAGES * STAGE / W, N = Out::N;
+    constexpr bool SLOPES = RESULT == SLOPE || RESULT == GATED_SLOPE;
+    static_assert((N2 ? 2 : 1) * Out::BYTES <= REGION, "");
+    char* own = shared + wave * REGION;
+    Matrix y = (RESULT == STORE || RESULT == PART) && batch ? a.y2 : a.y;
+    if (RESULT == PART) y.p += uint64_t(piece) * mc * y.ld * 4;
+    Matrix dz2 = a.dz;
+    dz2.p += uint64_t(a.dz_half) * sizeof(T);
+#pragma unroll
+    for (int i0 = 0; i0 < TO; i0 += PT) {
+        const uint32_t n = n0 + 32 * i0 + Out::column(lane);
+        float sum[SLOPES ? 2 : 1][N] = {};
+#pragma unroll
+        for (int j = 0; j < TM; j++) {
+            Out::order();
+#pragma unroll
+            for (int i = 0; i < PT; i++) {
+                Out::put(own, acc[i0 + i][j], i, lane);
+                if constexpr (N2) Out::put(own + Out::BYTES, acc[TO + i0 + i][j], i, lane);
+            }
+            Out::order();
+#pragma unroll 1
+            for (uint32_t t = 0; t < Out::TURNS; t++) {
+                const uint32_t m = m0 + 32 * j + Out::row(lane, t);
+                if (m >= mc) break;
+                float z[N], up[N], with[N];
+                Out::get(own, Out::row(lane, t), lane, z);
+                if constexpr (N2) Out::get(own + Out::BYTES, Out::row(lane, t), lane, up);
+                if constexpr (RESULT == LINEAR) {
+                    act_of<T>(a.act, z);
+                    if (a.residual.p) {
+                        Out::load(a.residual, m, n, nc, with);
+#pragma unroll
+                        for (uint32_t e = 0; e < N; e++) z[e] += with[e];
                     }
                 }
-                if constexpr (RESULT == SLOPE || RESULT == GATED_SLOPE) {
-                    if (a.sums) {
+                if constexpr (RESULT == GATED) {
+                    act_of<T>(a.act, z);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            s0[e] = lanes::sum_rows16(lanes::sum16(s0[e]));
-                            if (N2) s1[e] = lanes::sum_rows16(lanes::sum16(s1[e]));
-                        }
-                        if ((lane & 31) == 0 && n < nc) {
-                            char* to = reinterpret_cast<char*>(a.sums + uint64_t(mt * WM + wm) * 2 * nc);
-                            store4<float>(to, n, nc, s0);
-                            if (N2) store4<float>(to + uint64_t(nc) * 4, n, nc, s1);
-                        }
-                    }
+                    for (uint32_t e = 0; e < N; e++) z[e] *= up[e];
                 }
+                if constexpr (SLOPES) {
+                    // zeros past the last column, also where z is none: the next products read whole words
+                    float slope[N];
+                    Out::load(a.dy, m, n, nc, with);
+                    act_of<T>(a.act, z, slope);
+#pragma unroll
+                    for (uint32_t e = 0; e < N; e++) {
+                        if constexpr (N2) {
+                            slope[e] *= up[e];
+                            up[e] = n + e < nc ? with[e] * z[e] : 0.0f;
+                            sum[1][e] += up[e];
+                        }
+                        z[e] = n + e < nc ? with[e] * slope[e] : 0.0f;
+                        sum[0][e] += z[e];
+                    }
+                    Out::store(a.dz, m, n, a.dz_half, z);
+                    if constexpr (N2) Out::store(dz2, m, n, a.dz_half, up);
+                } else
+                    Out::store(y, m, n, nc, z);
+            }
+        }
+        if constexpr (SLOPES) {
+            if (a.sums) {
+                float* to = a.sums + uint64_t(mt * WM + wm) * 2 * nc + n;
+#pragma unroll
+                for (int half = 0; half < (N2 ? 2 : 1); half++)
+#pragma unroll
+                    for (uint32_t e = 0; e < N; e++) {
+                        float v = sum[half][e];
+#pragma unroll
+                        for (uint32_t l = Out::LANES; l < 64; l *= 2) v += __shfl_xor(v, l);
+                        if (lane < Out::LANES && n + e < nc) to[uint64_t(half) * nc + e] = v;
+                    }
             }
         }
     }
@@ -305,13 +417,13 @@ uint32_t blocks_for(uint64_t items, uint32_t per, uint32_t most) {
     return uint32_t(n < most ? (n ? n : 1) : most);
 }
 
-template <class T, int BM, int BN, int WM, int WN, int STAGES, bool MC, bool NC, int RESULT>
+template <class T, int BM, int BN, int WM, int WN, int STAGES, bool PAIRED, bool MC, bool NC, int RESULT>
 hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
     constexpr uint32_t OUT = two_weights(RESULT) ? BN / 2 : BN, bytes = STAGES * (BM + BN) * STEP_BYTES;
     static_assert(bytes <= 160 * 1024, "");
     a.m_tiles = (a.m.count + BM - 1) / BM;
     a.n_tiles = (a.n.count + OUT - 1) / OUT;
-    const auto kernel = product_kernel<T, BM, BN, WM, WN, STAGES, MC, NC, RESULT>;
+    const auto kernel = product_kernel<T, BM, BN, WM, WN, STAGES, PAIRED, MC, NC, RESULT>;
     if (bytes > 64 * 1024)
         if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
             return e;
@@ -329,12 +441,12 @@ Tile tile_of(uint64_t m, uint64_t n, uint64_t times) {
 
 template <class T, bool MC, bool NC, int RESULT>
 hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
-    if (tile == LARGE) return launch<T, 256, 256, 2, 4, 2, MC, NC, RESULT>(a, batches, st);
-    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 2, MC, NC, RESULT>(a, batches, st);
+    if (tile == LARGE) return launch<T, 256, 256, 4, 2, 2, true, MC, NC, RESULT>(a, batches, st);
+    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 2, false, MC, NC, RESULT>(a, batches, st);
     if constexpr (two_weights(RESULT))
-        return launch<T, 64, 128, 2, 2, 3, MC, NC, RESULT>(a, batches, st);
+        return launch<T, 64, 128, 2, 2, 3, false, MC, NC, RESULT>(a, batches, st);
     else
-        return launch<T, 64, 64, 2, 2, 4, MC, NC, RESULT>(a, batches, st);
+        return launch<T, 64, 64, 2, 2, 4, false, MC, NC, RESULT>(a, batches, st);
 }
 
 // ---- memory
@@ -390,7 +502,7 @@ BackPlan back_plan_of(const Args& a, const GradArgs& d) {
     p.dz_bytes = p.slope || p.dz_copy ? aligned(a.rows * pieces * p.out_ld * p.size) : 0;
     if (p.slope) {
         const uint32_t bm = p.forward_tile == LARGE ? 256 : p.forward_tile == MIDDLE ? 128 : 64;
-        p.sum_rows = uint32_t((a.rows + bm - 1) / bm) * 2;
+        p.sum_rows = uint32_t((a.rows + bm - 1) / bm) * (p.forward_tile == LARGE ? 4 : 2);
     } else
         p.sum_rows = uint32_t(a.rows < 16 * SHARES ? (a.rows + 15) / 16 : SHARES);
     p.sums_bytes = db ? aligned(uint64_t(p.sum_rows) * 2 * a.out * 4) : 0;

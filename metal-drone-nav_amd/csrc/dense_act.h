@@ -5,6 +5,8 @@
 #include "dense.h"
 #include "dense_tiles.h"
 
+#include <type_traits>
+
 namespace dense {
 
 // ---------------------------------------------------------------- activations
@@ -20,54 +22,79 @@ template <class T> __device__ __forceinline__ float tanh_of(float z) {
 }
 constexpr float C_TANH = 1.5957691216f;  // 2 sqrt(2 / pi)
 
-template <class T> __device__ __forceinline__ float act_of(uint32_t act, float z) {
-    switch (act) {
-        case MDN_ACT_RELU: return z > 0.0f ? z : z == z ? 0.0f : z;
-        case MDN_ACT_TANH: return tanh_of<T>(z);
-        case MDN_ACT_SIGMOID: return sigmoid<T>(z);
-        case MDN_ACT_SILU: return z * sigmoid<T>(z);
-        case MDN_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);
-        case MDN_ACT_GELU_TANH: return z * sigmoid<T>(C_TANH * z * fmaf(0.044715f * z, z, 1.0f));
-        default: return z;
-    }
+template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z) {
+    if (ACT == MDN_ACT_RELU) return z > 0.0f ? z : z == z ? 0.0f : z;
+    if (ACT == MDN_ACT_TANH) return tanh_of<T>(z);
+    if (ACT == MDN_ACT_SIGMOID) return sigmoid<T>(z);
+    if (ACT == MDN_ACT_SILU) return z * sigmoid<T>(z);
+    if (ACT == MDN_ACT_GELU) return 0.5f * z * erfcf(-0.70710678f * z);
+    if (ACT == MDN_ACT_GELU_TANH) return z * sigmoid<T>(C_TANH * z * fmaf(0.044715f * z, z, 1.0f));
+    return z;
 }
 // act(z) and act'(z)
-template <class T> __device__ __forceinline__ float act_of(uint32_t act, float z, float& slope) {
-    switch (act) {
-        case MDN_ACT_RELU: slope = z > 0.0f ? 1.0f : z == z ? 0.0f : z; return act_of<T>(act, z);
-        case MDN_ACT_TANH: {
-            const float t = tanh_of<T>(z);
-            slope = fmaf(-t, t, 1.0f);
-            if (fabsf(z) > 4.0f) {  // 1 - t^2 cancels
-                const float e = exp_of<T>(-2.0f * fabsf(z)), q = 1.0f + e;
-                slope = 4.0f * e / (q * q);
-            }
-            return t;
-        }
-        case MDN_ACT_SIGMOID: {
-            const float s = sigmoid<T>(z);
-            slope = s * sigmoid<T>(-z);
-            return s;
-        }
-        case MDN_ACT_SILU: {
-            const float s = sigmoid<T>(z);
-            slope = s * fmaf(z, sigmoid<T>(-z), 1.0f);
-            return z * s;
-        }
-        case MDN_ACT_GELU: {
-            const float s = 0.5f * erfcf(-0.70710678f * z);
-            slope = fmaf(z * 0.39894228f, exp_of<T>(-0.5f * z * z), s);
-            return z * s;
-        }
-        case MDN_ACT_GELU_TANH: {
-            // beyond 30 the slope is 0 or 1; the polynomial would overflow
-            const float c = fminf(fmaxf(z, -30.0f), 30.0f), u = C_TANH * c * fmaf(0.044715f * c, c, 1.0f);
-            const float s = sigmoid<T>(u);
-            slope = fmaf(c * s * sigmoid<T>(-u), C_TANH * fmaf(0.134145f * c, c, 1.0f), s) + 0.0f * z;
-            return z * s;
-        }
-        default: slope = 1.0f; return z;
+template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z, float& slope) {
+    if (ACT == MDN_ACT_RELU) {
+        slope = z > 0.0f ? 1.0f : z == z ? 0.0f : z;
+        return act_of<T, ACT>(z);
     }
+    if (ACT == MDN_ACT_TANH) {
+        const float t = tanh_of<T>(z);
+        slope = fmaf(-t, t, 1.0f);
+        if (fabsf(z) > 4.0f) {  // 1 - t^2 cancels
+            const float e = exp_of<T>(-2.0f * fabsf(z)), q = 1.0f + e;
+            slope = 4.0f * e / (q * q);
+        }
+        return t;
+    }
+    if (ACT == MDN_ACT_SIGMOID) {
+        const float s = sigmoid<T>(z);
+        slope = s * sigmoid<T>(-z);
+        return s;
+    }
+    if (ACT == MDN_ACT_SILU) {
+        const float s = sigmoid<T>(z);
+        slope = s * fmaf(z, 1.0f - s, 1.0f);
+        return z * s;
+    }
+    if (ACT == MDN_ACT_GELU) {
+        const float s = 0.5f * erfcf(-0.70710678f * z);
+        slope = fmaf(z * 0.39894228f, exp_of<T>(-0.5f * z * z), s);
+        return z * s;
+    }
+    if (ACT == MDN_ACT_GELU_TANH) {
+        // beyond 30 the slope is 0 or 1; the polynomial would overflow
+        const float c = fminf(fmaxf(z, -30.0f), 30.0f), u = C_TANH * c * fmaf(0.044715f * c, c, 1.0f);
+        const float s = sigmoid<T>(u);
+        slope = fmaf(c * s * (1.0f - s), C_TANH * fmaf(0.134145f * c, c, 1.0f), s) + 0.0f * z;
+        return z * s;
+    }
+    slope = 1.0f;
+    return z;
+}
+// The activation of a call, chosen once for N values.
+template <class F> __device__ __forceinline__ void by_act(uint32_t act, F f) {
+    switch (act) {
+        case MDN_ACT_RELU: return f(std::integral_constant<uint32_t, MDN_ACT_RELU>());
+        case MDN_ACT_TANH: return f(std::integral_constant<uint32_t, MDN_ACT_TANH>());
+        case MDN_ACT_SIGMOID: return f(std::integral_constant<uint32_t, MDN_ACT_SIGMOID>());
+        case MDN_ACT_SILU: return f(std::integral_constant<uint32_t, MDN_ACT_SILU>());
+        case MDN_ACT_GELU: return f(std::integral_constant<uint32_t, MDN_ACT_GELU>());
+        case MDN_ACT_GELU_TANH: return f(std::integral_constant<uint32_t, MDN_ACT_GELU_TANH>());
+        default: return f(std::integral_constant<uint32_t, MDN_ACT_NONE>());
+    }
+}
+template <class T, int N> __device__ __forceinline__ void act_of(uint32_t act, float (&z)[N]) {
+    by_act(act, [&](auto kind) {
+#pragma unroll
+        for (int e = 0; e < N; e++) z[e] = act_of<T, kind()>(z[e]);
+    });
+}
+// z to act(z), and act'(z)
+template <class T, int N> __device__ __forceinline__ void act_of(uint32_t act, float (&z)[N], float (&slope)[N]) {
+    by_act(act, [&](auto kind) {
+#pragma unroll
+        for (int e = 0; e < N; e++) z[e] = act_of<T, kind()>(z[e], slope[e]);
+    });
 }
 
 // ---------------------------------------------------------------- four neighbours of a row

@@ -102,9 +102,9 @@ __global__ void __launch_bounds__(64 * W) rows_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < N; i++)
             if (a.b[i]) z[i] += load4<T>(a.b[i], c, a.out);
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = act_of<T>(a.activation, z[0][e]);
+        float act[4] = {z[0][0], z[0][1], z[0][2], z[0][3]};
+        act_of<T>(a.activation, act);
+        f32x4 v = {act[0], act[1], act[2], act[3]};
         if constexpr (G) v = v * z[1];
         if (!G && a.residual.p) v = load4<T>(row_of<T>(a.residual, m), c, a.out) + v;
         store4<T>(row_of<T>(a.y, m), c, a.out, v);

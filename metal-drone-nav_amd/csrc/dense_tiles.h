@@ -63,6 +63,10 @@ template <int N> __device__ __forceinline__ void landed() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
+// LDS reads are back and all are here; all are here.
+__device__ __forceinline__ void read_and_met() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ void met() { asm volatile("s_barrier" ::: "memory"); }
+
 template <class T> struct Frag;
 template <> struct Frag<bf16> { bf16x8 t; };
 template <> struct Frag<float> { f32x4 t; };
