@@ -101,17 +101,18 @@ template <class T, int PW> struct Piece {
 
 // ---------------------------------------------------------------- the product
 // BN counts the rows of LDS: of the gated block's projections, half each.
-// PAIRED: the workgroup's two wavefronts on a SIMD take turns, one reads its
-// operands of 1/4 step while the other multiplies (they are a barrier apart).
-template <class T, int BM, int BN, int WM, int WN, int STAGES, bool PAIRED, bool MC, bool NC, int RESULT>
-__global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
+// PIPED: one wavefront on each SIMD, whose loads and LDS reads go out between
+// its own products (there is no other to fill the gaps).
+template <class T, int BM, int BN, int WM, int WN, int KB, int STAGES, bool PIPED, bool MC, bool NC, int RESULT>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN == 4 && PIPED ? 1 : 2))) product_kernel(Job a) {
     constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr bool N2 = two_weights(RESULT);
     constexpr int OUT = N2 ? BN / 2 : BN, TO = N2 ? TN / 2 : TN;  // columns of the result, and a wavefront's tiles of them
     static_assert(TM >= 1 && TN >= (N2 ? 2 : 1), "");
-    typedef Staged<T, BM, W, MC, false> SideM;
-    typedef Staged<T, BN, W, NC, N2> SideN;
-    constexpr uint32_t STAGE = SideM::BYTES + SideN::BYTES;
+    typedef Staged<T, BM, W, KB, MC, false> SideM;
+    typedef Staged<T, BN, W, KB, NC, N2> SideN;
+    constexpr uint32_t STAGE = SideM::BYTES + SideN::BYTES, STEP = KB / sizeof(T);
+    constexpr int KK = KB / 32;
     constexpr int LOADS = SideM::LOADS + SideN::LOADS;
     extern __shared__ __align__(16) char shared[];
     const uint32_t lds = uint32_t(uintptr_t((__attribute__((address_space(3))) char*)shared));
@@ -143,28 +144,53 @@ __global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
         sm.init(m, mt * BM, wave, lane);
         sn.init(a.n, nt * OUT, wave, lane);
     }
-    const uint32_t steps = (k_end - k_first + step_of<T>() - 1) / step_of<T>(), total = steps * a.segments;
+    const uint32_t steps = (k_end - k_first + STEP - 1) / STEP, total = steps * a.segments;
     uint32_t next = 0, next_k = k_first, into = 0;  // the step to load, its k, its stage
     bool second = false;
-    const auto fetch = [&]() {
+    const auto load = [&](int i) {
         const uint32_t to = lds + into * STAGE;
-        if (next_k + step_of<T>() <= k_end) {
-            sm.load(to, next_k, wave, second);
-            sn.load(to + SideM::BYTES, next_k, wave, second);
-        } else {
-            sm.load_end(to, next_k, k_end, wave, second);
-            sn.load_end(to + SideM::BYTES, next_k, k_end, wave, second);
-        }
+        i < SideM::LOADS ? sm.load(i, to, next_k, wave, second) : sn.load(i - SideM::LOADS, to + SideM::BYTES, next_k, wave, second);
+    };
+    const auto load_end = [&](int i) {
+        const uint32_t to = lds + into * STAGE;
+        i < SideM::LOADS ? sm.load_end(i, to, next_k, k_end, wave, second)
+                         : sn.load_end(i - SideM::LOADS, to + SideM::BYTES, next_k, k_end, wave, second);
+    };
+    const auto whole = [&]() { return next_k + STEP <= k_end; };
+    const auto loaded = [&]() {
         next++;
-        next_k += step_of<T>();
+        next_k += STEP;
         if (next == steps) {
             next_k = k_first;
             second = true;
         }
         into = into + 1 == STAGES ? 0 : into + 1;
     };
-    for (int s = 0; s < STAGES - 1; s++)
-        if (uint32_t(s) < total) fetch();
+    const auto fetch = [&]() {
+        if (whole()) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) load(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) load_end(i);
+        }
+        loaded();
+    };
+    const auto past_end = [&]() {
+        if (next >= total) next_k = k_end;
+    };
+    if constexpr (PIPED) {
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; s++) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) load_end(i);
+            loaded();
+            past_end();
+        }
+    } else {
+        for (int s = 0; s < STAGES - 1; s++)
+            if (uint32_t(s) < total) fetch();
+    }
 
     typename SideM::Reader rm;
     typename SideN::Reader rn;
@@ -193,47 +219,58 @@ __global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
         for (int j = 0; j < TM; j++) acc[i][j] = b;
     }
 
-    Frag<T> fm[TM], fn[TN];
-    const auto read = [&](uint32_t from, int kk) {
+    constexpr int AHEAD = PIPED ? 2 : 1, READS = TM + TN, MULS = TM * TN;
+    Frag<T> fm[AHEAD][TM], fn[AHEAD][TN];
+    // Operand i of a quarter of the step in stage `from`.
+    const auto read = [&](uint32_t from, int kk, int i) {
         const uint32_t at_m = lds + from * STAGE, at_n = at_m + SideM::BYTES;
-#pragma unroll
-        for (int i = 0; i < TN; i++)
-            fn[i] = rn.get(at_n, (N2 && i >= TO ? BN / 2 : 0) + wn * (OUT / WN) + 32 * (i % TO), kk);
-#pragma unroll
-        for (int j = 0; j < TM; j++) fm[j] = rm.get(at_m, wm * (BM / WM) + 32 * j, kk);
+        if (i < TN)
+            fn[kk % AHEAD][i] = rn.get(at_n, (N2 && i >= TO ? BN / 2 : 0) + wn * (OUT / WN) + 32 * (i % TO), kk);
+        else
+            fm[kk % AHEAD][i - TN] = rm.get(at_m, wm * (BM / WM) + 32 * (i - TN), kk);
     };
-    const auto multiply = [&]() {
-#pragma unroll
-        for (int i = 0; i < TN; i++)
-#pragma unroll
-            for (int j = 0; j < TM; j++) mma(acc[i][j], fn[i], fm[j]);
-    };
+    const auto multiply = [&](int kk, int i) { mma(acc[i / TM][i % TM], fn[kk % AHEAD][i / TM], fm[kk % AHEAD][i % TM]); };
     uint32_t from = 0;
-    if constexpr (PAIRED) {
-        static_assert(STAGES == 2 && W == 8, "");
-        landed<0>();
-        if (wave >= 4) landed<0>();  // the second wavefronts of the SIMDs are a barrier behind
-        for (uint32_t s = 0; s < total; s++) {
+    if constexpr (PIPED) {
+        // A step's last place is read while the one before is multiplied, so its
+        // stage is free from the barrier before the last place's products on, where
+        // the next step has landed too. From there to the same point of the next step
+        // the step STAGES later is loaded, evenly: its loads take half of that time in
+        // the memory pipe. Past the sum's end these are loads of zeros that no one
+        // reads, as the last step's reads of a next one are of what was there.
+        landed<LOADS*(STAGES - 2)>();
+        constexpr int SLOTS = (KK > 2 ? KK - 1 : KK) * MULS;  // products that loads go out behind
+        const auto load_at = [&](auto whole_steps, int slot) {
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                read(from, kk);
-                // Every wavefront has read the other stage to its end: the ones behind waited
-                // for their last reads of it before the barrier that this one has passed.
-                if (kk == 0 && next < total) fetch();
-                if (kk == 3)
-                    landed<0>();  // the next step's words too, for those who read them after the next barrier
-                else
-                    read_and_met();
-                __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_s_setprio(1);
-                multiply();
-                __builtin_amdgcn_s_setprio(0);
-                __builtin_amdgcn_sched_barrier(0);
-                met();
+            for (int l = slot * LOADS / SLOTS; l < (slot + 1) * LOADS / SLOTS; l++) whole_steps() ? load(l) : load_end(l);
+        };
+#pragma unroll
+        for (int i = 0; i < MULS; i++) load_at(std::false_type(), i);
+#pragma unroll
+        for (int i = 0; i < READS; i++) read(from, 0, i);
+        const auto step = [&](auto whole_steps) {
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                if (kk == KK - 1) {
+                    loaded();
+                    past_end();
+                    landed<LOADS*(STAGES - 2)>();
+                    from = from + 1 == STAGES ? 0 : from + 1;
+                }
+#pragma unroll
+                for (int i = 0; i < MULS; i++) {
+                    multiply(kk, i);
+                    if (i < READS) read(from, (kk + 1) % KK, i);
+                    if ((kk + 1) % KK * MULS < SLOTS) load_at(whole_steps, (kk + 1) % KK * MULS + i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-            from ^= 1;
-        }
-        if (wave < 4) met();
+        };
+        // as long as this step's loads and the next one's are whole
+        uint32_t s = 0;
+        for (; next + 1 < total && next_k + 2 * STEP <= k_end; s++) step(std::true_type());
+        for (; s < total; s++) step(std::false_type());
+        landed<0>();
     } else {
         for (uint32_t s = 0; s < total; s++) {
             // this step's words are there for all, and all have read the step before it
@@ -243,9 +280,11 @@ __global__ void __launch_bounds__(64 * WM * WN) product_kernel(Job a) {
                 landed<0>();
             if (next < total) fetch();
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                read(from, kk);
-                multiply();
+            for (int kk = 0; kk < KK; kk++) {
+#pragma unroll
+                for (int i = 0; i < READS; i++) read(from, kk, i);
+#pragma unroll
+                for (int i = 0; i < MULS; i++) multiply(kk, i);
             }
             from = from + 1 == STAGES ? 0 : from + 1;
         }
@@ -417,13 +456,13 @@ uint32_t blocks_for(uint64_t items, uint32_t per, uint32_t most) {
     return uint32_t(n < most ? (n ? n : 1) : most);
 }
 
-template <class T, int BM, int BN, int WM, int WN, int STAGES, bool PAIRED, bool MC, bool NC, int RESULT>
+template <class T, int BM, int BN, int WM, int WN, int KB, int STAGES, bool PIPED, bool MC, bool NC, int RESULT>
 hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
-    constexpr uint32_t OUT = two_weights(RESULT) ? BN / 2 : BN, bytes = STAGES * (BM + BN) * STEP_BYTES;
+    constexpr uint32_t OUT = two_weights(RESULT) ? BN / 2 : BN, bytes = STAGES * (BM + BN) * KB;
     static_assert(bytes <= 160 * 1024, "");
     a.m_tiles = (a.m.count + BM - 1) / BM;
     a.n_tiles = (a.n.count + OUT - 1) / OUT;
-    const auto kernel = product_kernel<T, BM, BN, WM, WN, STAGES, PAIRED, MC, NC, RESULT>;
+    const auto kernel = product_kernel<T, BM, BN, WM, WN, KB, STAGES, PIPED, MC, NC, RESULT>;
     if (bytes > 64 * 1024)
         if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
             return e;
@@ -441,12 +480,12 @@ Tile tile_of(uint64_t m, uint64_t n, uint64_t times) {
 
 template <class T, bool MC, bool NC, int RESULT>
 hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
-    if (tile == LARGE) return launch<T, 256, 256, 4, 2, 2, true, MC, NC, RESULT>(a, batches, st);
-    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 2, false, MC, NC, RESULT>(a, batches, st);
+    if (tile == LARGE) return launch<T, 256, 256, 2, 2, 128, 2, true, MC, NC, RESULT>(a, batches, st);
+    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 128, 2, false, MC, NC, RESULT>(a, batches, st);
     if constexpr (two_weights(RESULT))
-        return launch<T, 64, 128, 2, 2, 3, false, MC, NC, RESULT>(a, batches, st);
+        return launch<T, 64, 128, 2, 2, 128, 3, false, MC, NC, RESULT>(a, batches, st);
     else
-        return launch<T, 64, 64, 2, 2, 4, false, MC, NC, RESULT>(a, batches, st);
+        return launch<T, 64, 64, 2, 2, 128, 4, false, MC, NC, RESULT>(a, batches, st);
 }
 
 // ---- memory
@@ -502,7 +541,7 @@ BackPlan back_plan_of(const Args& a, const GradArgs& d) {
     p.dz_bytes = p.slope || p.dz_copy ? aligned(a.rows * pieces * p.out_ld * p.size) : 0;
     if (p.slope) {
         const uint32_t bm = p.forward_tile == LARGE ? 256 : p.forward_tile == MIDDLE ? 128 : 64;
-        p.sum_rows = uint32_t((a.rows + bm - 1) / bm) * (p.forward_tile == LARGE ? 4 : 2);
+        p.sum_rows = uint32_t((a.rows + bm - 1) / bm) * 2;
     } else
         p.sum_rows = uint32_t(a.rows < 16 * SHARES ? (a.rows + 15) / 16 : SHARES);
     p.sums_bytes = db ? aligned(uint64_t(p.sum_rows) * 2 * a.out * 4) : 0;

@@ -13,6 +13,7 @@
 namespace dense {
 namespace {
 
+template <class T> constexpr uint32_t step_of() { return 128 / sizeof(T); }  // k of a turn
 template <class T> struct Word;
 template <> struct Word<bf16> { typedef bf16x8 type; };
 template <> struct Word<float> { typedef f32x4 type; };

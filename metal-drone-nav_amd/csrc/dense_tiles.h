@@ -1,8 +1,9 @@
 // dense_tiles.h — matrix-core tiles of the policy network's products.
 //
 // A product is C[m][n] = sum over k of P(m, k) Q(n, k).  A workgroup makes a
-// BM x BN tile of C in steps of 128 bytes of k (64 bfloat16 or 32 fp32), which
-// go from memory straight to LDS, STAGES - 1 steps ahead of the products.
+// BM x BN tile of C in steps of KB bytes of k (128: 64 bfloat16 or 32 fp32; or
+// half of that), which go from memory straight to LDS, some steps ahead of the
+// products.
 //
 // A side lies in memory along k ("rows": p[m ld + k]) or along its own index
 // ("columns": p[k ld + m]).  Either way it moves in 16-byte words, a wavefront
@@ -34,8 +35,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t STEP_BYTES = 128;
-template <class T> constexpr uint32_t step_of() { return STEP_BYTES / sizeof(T); }  // k of a step
 template <class T> constexpr uint32_t per_word() { return 16 / sizeof(T); }
 
 // What lanes past the end of k load.
@@ -54,18 +53,14 @@ struct Side {
 __device__ __forceinline__ void to_lds(const char* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0");
 }
-// The same from a base that all lanes share, and a lane's offset.
-__device__ __forceinline__ void to_lds(const char* base, uint32_t off, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0");
+// The same from a base that all lanes share and a lane's offset, to `to` + `more`.
+__device__ __forceinline__ void to_lds(const char* base, uint32_t off, uint32_t to, uint32_t more) {
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base), "i"(more) : "m0", "scc");
 }
 // All but the last N loads have landed, all LDS reads are back; then every wavefront of the workgroup.
 template <int N> __device__ __forceinline__ void landed() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
-
-// LDS reads are back and all are here; all are here.
-__device__ __forceinline__ void read_and_met() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-__device__ __forceinline__ void met() { asm volatile("s_barrier" ::: "memory"); }
 
 template <class T> struct Frag;
 template <> struct Frag<bf16> { bf16x8 t; };
@@ -89,61 +84,57 @@ template <class V> __device__ __forceinline__ V lds_at(uint32_t at) {
 }
 
 // A side's part of one stage: R rows of a step, R a multiple of 32.  W: wavefronts of the workgroup, T2: from two matrices
-// (half of the rows from each, rows only).
-template <class T, int R, int W, bool COLUMNS, bool T2> struct Staged;
+// (half of the rows from each, rows only).  A step has KB / 32 places of two words of k, one to each half of a wavefront.
+template <class T, int R, int W, int KB, bool COLUMNS, bool T2> struct Staged;
 
-template <class T, int R, int W, bool T2> struct Staged<T, R, W, false, T2> {
-    static constexpr int LOADS = R / (8 * W), BYTES = R * 128;
+template <class T, int R, int W, int KB, bool T2> struct Staged<T, R, W, KB, false, T2> {
+    static constexpr int WORDS = KB / 16, LOADS = R * WORDS / (64 * W), BYTES = R * KB;
     static_assert(LOADS >= 1 && (!T2 || LOADS % 2 == 0), "");
     uint32_t off[LOADS];
     const char *p0, *p1;
     uint32_t word;  // of the step, this lane's
 
-    static __device__ __forceinline__ uint32_t exchange(uint32_t row) { return row & 7; }
+    // 256 / KB rows fill the 64 banks.
+    static __device__ __forceinline__ uint32_t exchange(uint32_t row) { return row / (256 / KB) % WORDS; }
     // From row r0; rows past the last repeat it (their results are not stored).
     __device__ __forceinline__ void init(const Side& a, uint32_t r0, uint32_t wave, uint32_t lane) {
         p0 = a.p + int64_t(r0) * a.ld;
         p1 = a.p2 + int64_t(r0) * a.ld;
-        word = (lane & 7) ^ exchange(lane >> 3);
+        static_assert(W % 2 == 0, "");
+        constexpr uint32_t ROWS = 64 / WORDS;
+        word = (lane % WORDS) ^ exchange(wave * ROWS + lane / WORDS);  // (the same in all loads: ROWS W rows change nothing)
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            const uint32_t row = (i * W + wave) * 8 + (lane >> 3);
+            const uint32_t row = (i * W + wave) * ROWS + lane / WORDS;
             const uint32_t in = T2 && i >= LOADS / 2 ? row - R / 2 : row, left = a.count - 1 - r0;
             off[i] = (in < left ? in : left) * uint32_t(a.ld) + 16 * word;
         }
     }
-    __device__ __forceinline__ void load(uint32_t to, uint32_t k0, uint32_t wave, bool second) const {
-        const uint64_t at = uint64_t(k0) * sizeof(T);
-#pragma unroll
-        for (int i = 0; i < LOADS; i++)
-            to_lds(((T2 ? i >= LOADS / 2 : second) ? p1 : p0) + at, off[i], to + (i * W + wave) * 1024);
+    // Load i of the step at k0.
+    __device__ __forceinline__ void load(int i, uint32_t to, uint32_t k0, uint32_t wave, bool second) const {
+        to_lds(((T2 ? i >= LOADS / 2 : second) ? p1 : p0) + uint64_t(k0) * sizeof(T), off[i], to + wave * 1024, i * W * 1024);
     }
-    // The last step of a sum that does not fill it.
-    __device__ __forceinline__ void load_end(uint32_t to, uint32_t k0, uint32_t k_end, uint32_t wave, bool second) const {
-        const uint64_t at = uint64_t(k0) * sizeof(T);
-        const bool in = k0 + word * per_word<T>() < k_end;
-#pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-            const char* from = ((T2 ? i >= LOADS / 2 : second) ? p1 : p0) + at + off[i];
-            to_lds(in ? from : reinterpret_cast<const char*>(zero_word), to + (i * W + wave) * 1024);
-        }
+    // The same of the last step of a sum, which does not fill it.
+    __device__ __forceinline__ void load_end(int i, uint32_t to, uint32_t k0, uint32_t k_end, uint32_t wave, bool second) const {
+        const char* from = ((T2 ? i >= LOADS / 2 : second) ? p1 : p0) + uint64_t(k0) * sizeof(T) + off[i];
+        to_lds(k0 + word * per_word<T>() < k_end ? from : reinterpret_cast<const char*>(zero_word), to + (i * W + wave) * 1024);
     }
-    // A lane's operands: of the 32 rows from `row`, the two words of place kk (0..3) of the step.
+    // A lane's operands: of the 32 rows from `row`, its word of place kk of the step.
     struct Reader {
-        uint32_t at[4];
+        uint32_t at[KB / 32];
         __device__ __forceinline__ void init(uint32_t lane) {
 #pragma unroll
-            for (uint32_t kk = 0; kk < 4; kk++) at[kk] = (lane & 31) * 128 + (((2 * kk + (lane >> 5)) ^ exchange(lane & 31)) << 4);
+            for (uint32_t kk = 0; kk < KB / 32; kk++) at[kk] = (lane & 31) * KB + (((2 * kk + (lane >> 5)) ^ exchange(lane & 31)) << 4);
         }
         __device__ __forceinline__ Frag<T> get(uint32_t base, uint32_t row, int kk) const {
-            return {lds_at<decltype(Frag<T>::t)>(base + at[kk] + row * 128)};
+            return {lds_at<decltype(Frag<T>::t)>(base + at[kk] + row * KB)};
         }
     };
 };
 
-template <class T, int R, int W> struct Staged<T, R, W, true, false> {
-    static constexpr int WORDS = R * sizeof(T) / 16, KS = 64 / WORDS > 0 ? 64 / WORDS : 1;
-    static constexpr int LOADS = R / (8 * W), BYTES = R * 128;
+template <class T, int R, int W, int KB> struct Staged<T, R, W, KB, true, false> {
+    static constexpr int WORDS = R * sizeof(T) / 16, KS = 64 / WORDS;
+    static constexpr int LOADS = R * KB / (1024 * W), BYTES = R * KB;
     static_assert(LOADS >= 1 && WORDS <= 64, "");
     uint32_t off[LOADS];
     const char *p0, *p1;
@@ -165,16 +156,12 @@ template <class T, int R, int W> struct Staged<T, R, W, true, false> {
             off[i] = k * uint32_t(a.ld) + 16 * (word < last ? word : last);
         }
     }
-    __device__ __forceinline__ void load(uint32_t to, uint32_t k0, uint32_t wave, bool second) const {
-        const char* from = (second ? p1 : p0) + int64_t(k0) * ld;
-#pragma unroll
-        for (int i = 0; i < LOADS; i++) to_lds(from, off[i], to + (i * W + wave) * 1024);
+    __device__ __forceinline__ void load(int i, uint32_t to, uint32_t k0, uint32_t wave, bool second) const {
+        to_lds((second ? p1 : p0) + int64_t(k0) * ld, off[i], to + wave * 1024, i * W * 1024);
     }
-    __device__ __forceinline__ void load_end(uint32_t to, uint32_t k0, uint32_t k_end, uint32_t wave, bool second) const {
-        const char* from = (second ? p1 : p0) + int64_t(k0) * ld;
-#pragma unroll
-        for (int i = 0; i < LOADS; i++)
-            to_lds(k0 + i * W * KS + k_in < k_end ? from + off[i] : reinterpret_cast<const char*>(zero_word), to + (i * W + wave) * 1024);
+    __device__ __forceinline__ void load_end(int i, uint32_t to, uint32_t k0, uint32_t k_end, uint32_t wave, bool second) const {
+        const char* from = (second ? p1 : p0) + int64_t(k0) * ld + off[i];
+        to_lds(k0 + i * W * KS + k_in < k_end ? from : reinterpret_cast<const char*>(zero_word), to + (i * W + wave) * 1024);
     }
     struct Reader {
         uint32_t lane;
