@@ -595,14 +595,14 @@ typedef struct MdnChoiceLoss {
     const float *old_log_prob, *advantages, *ref_log_prob; /* [steps]; ref_log_prob may be NULL */
     const uint8_t* mask;                                   /* [steps], or NULL */
     double clip_low, clip_high, kl_coef, entropy_coef;
-    float* loss; /* [6]: the loss, then the means of -min(..), K, H, r and of r outside the clip's borders */
+    float *loss, *metrics; /* [1], and [5]: the means of -min(..), K, H, r and of r outside the clip's borders */
 } MdnChoiceLoss;
-/* Bytes of `keep`, which the backward pass reads, and of the workspace. */
+/* Bytes of `keep`, 16-byte aligned, which the backward pass reads, and of the workspace. */
 int mdn_op_choices_loss_sizes(const MdnChoices* choices, uint64_t* keep, uint64_t* workspace);
 int mdn_op_choices_loss_forward(const MdnChoices* choices, const MdnChoiceLoss* loss, void* keep, uint64_t keep_bytes,
                                 void* workspace, uint64_t workspace_bytes, void* stream);
-/* The gradient of loss[0] by the logits times *d_loss, contiguous and of
- * their type; `loss` as in the forward call (its result is not read). */
+/* The gradient of the loss by the logits times *d_loss, contiguous and of
+ * their type; `loss` as in the forward call (its results are not read). */
 int mdn_op_choices_loss_backward(const MdnChoices* choices, const MdnChoiceLoss* loss, const void* keep,
                                  uint64_t keep_bytes, const float* d_loss, void* d_logits, void* stream);
 

@@ -2519,8 +2519,10 @@ int choice_loss_args(const char* name, const MdnChoices* c, const MdnChoiceLoss*
     a.old_log_prob = l->old_log_prob; a.advantages = l->advantages; a.ref_log_prob = l->ref_log_prob; a.mask = l->mask;
     a.low = l->clip_low; a.high = l->clip_high; a.kl_coef = l->kl_coef; a.entropy_coef = l->entropy_coef;
     a.loss = l->loss;
-    a.stats = static_cast<float*>(const_cast<void*>(keep));
-    a.slopes = a.stats + a.steps * a.heads * 3;
+    a.metrics = l->metrics;
+    if (reinterpret_cast<uintptr_t>(keep) % alignof(choices::Stat)) return fail(MDN_E_ARG, who + "keep must be 16-byte aligned");
+    a.stats = static_cast<choices::Stat*>(const_cast<void*>(keep));
+    a.slopes = reinterpret_cast<float*>(a.stats + a.steps * a.heads);
     a.one_over = a.slopes + a.steps;
     *out = a;
     return MDN_OK;
@@ -2554,7 +2556,7 @@ int mdn_op_choices_loss_forward(const MdnChoices* choices, const MdnChoiceLoss* 
                                 void* workspace, uint64_t workspace_bytes, void* stream) {
     choices::Args a;
     if (int rc = choice_loss_args("mdn_op_choices_loss_forward", choices, loss, keep, keep_bytes, &a)) return rc;
-    if (!a.loss) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: null loss");
+    if (!a.loss || !a.metrics) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: null results");
     const uint64_t need = uint64_t(choices::parts_of(a)) * 6 * sizeof(double);
     if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: workspace is too small");
     a.parts = static_cast<double*>(workspace);

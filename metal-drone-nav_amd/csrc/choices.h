@@ -9,6 +9,9 @@
 
 namespace choices {
 
+// Of a row: the largest logit, the sum of exponentials below it, the entropy and the chosen logit.
+struct __align__(16) Stat { float m, s, entropy, chosen; };
+
 struct Args {
     uint64_t steps;
     uint32_t heads, choices, bf, index64;
@@ -21,8 +24,9 @@ struct Args {
     const float *old_log_prob, *advantages, *ref_log_prob;
     const uint8_t* mask;
     double low, high, kl_coef, entropy_coef;
-    float* loss;           // the loss, then its five terms
-    float* stats;          // [steps][heads][3]: the largest logit, log of the sum of exponentials, entropy
+    float* loss;
+    float* metrics;        // the means of its five terms
+    Stat* stats;           // [steps][heads]
     float* slopes;         // [steps]: of the loss (not yet a mean) by the log-probability; NaN-free 0 where masked
     double* parts;         // [workgroups][6]
     float* one_over;       // 1 / the steps that count

@@ -8,18 +8,21 @@
 //     dz = dL/dl (1[action] - p) + entropy p (log p + H)
 // over the number of those steps.
 //
-// Forward reads the logits once: G lanes have a step and go through its heads,
-// each lane with a running maximum m, s = sum exp(z - m) and t = sum exp(z - m)
-// (z - m), so that log-sum-exp is m + log s and the entropy log s - t / s.
-// Words of 16 bytes in fp32; what a step makes of them, and the sums over
-// steps, in 64 bits, since the means are small differences of many terms.
+// Forward reads the logits once. A lane keeps the largest logit m that it has
+// seen, s = sum 2^y and t = sum y 2^y with y = (z - m) log2 e, in fp32, a few
+// 16-byte words at a time; a row's lanes join theirs at the end, so log-sum-exp
+// is m + log s and the entropy log s - t log 2 / s. m, s and the entropy of every
+// row are kept. What a step makes of its rows is 64 bits, as are the sums over
+// steps, since the means are small differences of many terms; that takes some
+// hundreds of instructions and registers that the rows need, so a second kernel
+// does it, a step to a lane, and a third adds up the workgroups' sums.
 //
 // Whether r is past the clip's border decides over a step's whole gradient.
-// Where r in 32-bit sums is so near that their error could decide, the
-// step's exponentials are summed again in 64 bits.
+// Where r of 32-bit sums is so near that their error could decide, the step's
+// exponentials are summed again in 64 bits.
 //
 // Backward reads the logits once more and writes their gradient: a step's
-// statistics are three floats a head and the slope.
+// statistics are four floats a head and the slope.
 #include "choices.h"
 
 #include "lane_sums.h"
@@ -34,202 +37,319 @@ template <> struct Words<float> { typedef Word type __attribute__((aligned(4)));
 template <> struct Words<bf16> { typedef Word type __attribute__((aligned(2))); };
 template <class T> constexpr uint32_t per_word() { return 16 / sizeof(T); }
 
-// Elements at .. at + per_word - 1 of a row in fp32; past its end, -inf (a choice that has no share).
-template <class T> __device__ __forceinline__ void load(float (&z)[per_word<T>()], const T* row, uint32_t at, uint32_t count) {
+// Elements at .. at + per_word - 1 of a row as they are; past its end, -inf (a choice that has no share).
+template <class T> __device__ __forceinline__ Word fetch(const T* row, uint32_t at, uint32_t count) {
     constexpr uint32_t N = per_word<T>();
-    if (at + N <= count) {
-        const Word w = *reinterpret_cast<const typename Words<T>::type*>(row + at);
+    if (at + N <= count) return *reinterpret_cast<const typename Words<T>::type*>(row + at);
+    union { Word u; T t[N]; } v;
 #pragma unroll
-        for (uint32_t e = 0; e < N; e++)
-            z[e] = sizeof(T) == 4 ? __builtin_bit_cast(float, uint32_t(w[e]))
-                                  : __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-    } else {
+    for (uint32_t e = 0; e < N; e++) v.t[e] = at + e < count ? row[at + e] : T(-__builtin_inff());
+    return v.u;
+}
+// The same in fp32.
+template <class T> __device__ __forceinline__ void spread(float (&z)[per_word<T>()], const Word& w) {
 #pragma unroll
-        for (uint32_t e = 0; e < N; e++) z[e] = at + e < count ? float(row[at + e]) : -__builtin_inff();
-    }
+    for (uint32_t e = 0; e < per_word<T>(); e++)
+        z[e] = sizeof(T) == 4 ? __builtin_bit_cast(float, uint32_t(w[e]))
+                              : __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
 }
 
-// A running maximum and sums.
+constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f, LOWEST = -3.402823466e38f;
+
+// A row's or a lane's largest logit and sums (2^y in hardware: 1 unit in the last place).
 struct Sums {
     float m, s, t;
-    static __device__ __forceinline__ Sums none() { return {-__builtin_inff(), 0.0f, 0.0f}; }
-    __device__ __forceinline__ void rescale(float to) {  // to >= m, above -inf
-        const float by = m == to ? 1.0f : expf(m - to), gap = m - to;
-        t = s > 0.0f ? by * fmaf(s, gap, t) : by * t;    // (no sum yet: m may be -inf)
+    static __device__ __forceinline__ Sums none() { return {LOWEST, 0.0f, 0.0f}; }
+    __device__ __forceinline__ void rescale(float to) {
+        const float y = (m - to) * LOG2E, by = __builtin_amdgcn_exp2f(y);
+        t = by * fmaf(s, fmaxf(y, -1000.0f), t);  // (y may be -inf where there is nothing yet)
         s *= by;
         m = to;
     }
-    template <int N> __device__ __forceinline__ void add(const float (&z)[N]) {
-        float top = z[0];
+    template <int W, int N> __device__ __forceinline__ void add(const float (&z)[W][N]) {
+        float top = m;
 #pragma unroll
-        for (int e = 1; e < N; e++) top = fmaxf(top, z[e]);
-        if (!(top > -__builtin_inff())) {  // nothing to add, or NaN alone
+        for (int w = 0; w < W; w++)
 #pragma unroll
-            for (int e = 0; e < N; e++)
-                if (z[e] != z[e]) s = z[e];
-            return;
-        }
+            for (int e = 0; e < N; e++) top = fmaxf(top, z[w][e]);
         if (top > m) rescale(top);
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            const float x = z[e] - m, p = expf(x);
-            s += p;
-            t += p > 0.0f ? p * x : 0.0f;
-        }
-    }
-    __device__ __forceinline__ void join(const Sums& o) {
-        const float top = fmaxf(m, o.m);
-        if (top > -__builtin_inff()) {
-            Sums b = o;
-            rescale(top);
-            b.rescale(top);
-            s += b.s;
-            t += b.t;
-        } else
-            s += o.s;
+        for (int w = 0; w < W; w++)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float y = (z[w][e] - m) * LOG2E, p = __builtin_amdgcn_exp2f(y);
+                s += p;
+                t = fmaf(p, fmaxf(y, -1000.0f), t);  // a choice ruled out: 0, and not 0 times -inf
+            }
     }
 };
-__device__ __forceinline__ Sums from_lane(const Sums& a, int mask) {
-    return {__shfl_xor(a.m, mask), __shfl_xor(a.s, mask), __shfl_xor(a.t, mask)};
-}
-
-// What a group of lanes has a row with: a part of a wavefront, or (0) a workgroup of 1,024.
-template <int G> struct Group {
-    static constexpr uint32_t LANES = G ? G : 1024, PER = G ? 256 / G : 1, THREADS = G ? 256 : 1024;
-    static __device__ __forceinline__ Sums join(Sums a) {
-#pragma unroll
-        for (int i = 1; i < (G ? G : 64); i *= 2) a.join(from_lane(a, i));
-        if constexpr (G == 0) {
-            __shared__ Sums lds[16];
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
-            __syncthreads();
-            a = lds[threadIdx.x & 15];
-#pragma unroll
-            for (int i = 1; i < 16; i *= 2) a.join(from_lane(a, i));
-        }
-        return a;
+// Over the G lanes that have a row: neighbours, pairs, mirrored eights and sixteens, then other rows of sixteen.
+template <int G, class F> __device__ __forceinline__ float over_lanes(float x, F f) {
+    x = f(x, lanes::from_lane<0xB1>(x));
+    x = f(x, lanes::from_lane<0x4E>(x));
+    if (G >= 8) x = f(x, lanes::from_lane<0x141>(x));
+    if (G >= 16) x = f(x, lanes::from_lane<0x140>(x));
+    if (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+        x = f(__builtin_bit_cast(float, unsigned(r[0])), __builtin_bit_cast(float, unsigned(r[1])));
     }
-    static __device__ __forceinline__ double sum(double a) {
-#pragma unroll
-        for (int i = 1; i < (G ? G : 64); i *= 2) a += __shfl_xor(a, i);
-        if constexpr (G == 0) {
-            __shared__ double lds[16];
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
-            __syncthreads();
-            a = lds[threadIdx.x & 15];
-#pragma unroll
-            for (int i = 1; i < 16; i *= 2) a += __shfl_xor(a, i);
-        }
-        return a;
+    if (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+        x = f(__builtin_bit_cast(float, unsigned(r[0])), __builtin_bit_cast(float, unsigned(r[1])));
     }
-};
-
-__device__ __forceinline__ int64_t action_of(const Args& a, uint64_t step, uint32_t head) {
-    const uint64_t at = step * a.heads + head;
-    return a.index64 ? reinterpret_cast<const int64_t*>(a.actions)[at] : reinterpret_cast<const int32_t*>(a.actions)[at];
+    return x;
+}
+template <int G> __device__ __forceinline__ float lanes_max(float x) {
+    return over_lanes<G>(x, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int G> __device__ __forceinline__ float lanes_sum(float x) {
+    return over_lanes<G>(x, [](float a, float b) { return a + b; });
+}
+template <int G> __device__ __forceinline__ double lanes_sum(double x) {
+#pragma unroll
+    for (int i = 1; i < G; i *= 2) x += __shfl_xor(x, i);
+    return x;
+}
+template <int G> __device__ __forceinline__ Sums join(Sums a) {
+    const float top = lanes_max<G>(a.m);
+    a.rescale(top);
+    return {top, lanes_sum<G>(a.s), lanes_sum<G>(a.t)};
 }
 
-template <class T, int G> __device__ __forceinline__ double exact_log_sum(const T* row, uint32_t lane, uint32_t count, float m) {
-    double s = 0.0;
-    for (uint32_t i = lane; i < count; i += Group<G>::LANES) s += exp(double(float(row[i])) - double(m));
-    return log(Group<G>::sum(s));
+__device__ __forceinline__ int64_t action_of(const Args& a, uint64_t row) {
+    return a.index64 ? reinterpret_cast<const int64_t*>(a.actions)[row] : reinterpret_cast<const int32_t*>(a.actions)[row];
+}
+template <class T> __device__ __forceinline__ const T* row_of(const Args& a, uint64_t step, uint32_t head) {
+    return reinterpret_cast<const T*>(a.logits) + int64_t(step) * a.step + int64_t(head) * a.head;
+}
+// The chosen logit; an action that is none has no log-probability.
+template <class T> __device__ __forceinline__ float chosen(const T* row, int64_t action, uint32_t count) {
+    return action >= 0 && action < int64_t(count) ? float(row[action]) : __builtin_nanf("");
 }
 
-// LOSS false: log-probabilities and entropies alone.
-template <class T, int G, bool LOSS>
-__global__ void __launch_bounds__(Group<G>::THREADS) forward_kernel(Args a) {
-    constexpr uint32_t N = per_word<T>(), LANES = Group<G>::LANES, PER = Group<G>::PER;
+// Lanes of a row: G of a wavefront, or (0) a workgroup of WIDE.
+constexpr uint32_t WIDE = 512;
+template <int G> constexpr uint32_t lanes_of() { return G ? G : WIDE; }
+template <int G> constexpr uint32_t threads_of() { return G ? 256 : WIDE; }
+
+// A row's sums, of which this lane has the words first, first + lanes, ..
+template <class T, int G, int W> __device__ __forceinline__ Sums sum_row(const T* row, uint32_t lane, uint32_t count, uint32_t words) {
+    Sums r = Sums::none();
+    for (uint32_t first = lane; first < words; first += W * lanes_of<G>()) {
+        Word got[W];
+        float z[W][per_word<T>()];
+#pragma unroll
+        for (uint32_t w = 0; w < W; w++) got[w] = fetch<T>(row, (first + w * lanes_of<G>()) * per_word<T>(), count);
+#pragma unroll
+        for (uint32_t w = 0; w < W; w++) spread<T>(z[w], got[w]);
+        r.add(z);
+    }
+    if constexpr (G != 0) return join<G>(r);
+    __shared__ float lds[3][16];
+    r = join<64>(r);
+    __syncthreads();
+    if (threadIdx.x < 16 * 3) lds[threadIdx.x / 16][threadIdx.x % 16] = threadIdx.x < 16 ? LOWEST : 0.0f;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        lds[0][threadIdx.x >> 6] = r.m;
+        lds[1][threadIdx.x >> 6] = r.s;
+        lds[2][threadIdx.x >> 6] = r.t;
+    }
+    __syncthreads();
+    return join<16>(Sums{lds[0][threadIdx.x & 15], lds[1][threadIdx.x & 15], lds[2][threadIdx.x & 15]});
+}
+__device__ __forceinline__ float entropy_of(const Sums& r) {
+    return LN2 * __builtin_amdgcn_logf(r.s) - LN2 * r.t * __builtin_amdgcn_rcpf(r.s);
+}
+
+// The statistics of rows, R of them at once in a group of lanes, W words each.
+template <class T, int G, int R, int W>
+__global__ void __launch_bounds__(threads_of<G>()) rows_kernel(Args a) {
+    constexpr uint32_t LANES = lanes_of<G>(), GROUPS = threads_of<G>() / LANES, N = per_word<T>();
     const uint32_t lane = threadIdx.x % LANES, words = (a.choices + N - 1) / N;
-    double total[6] = {};
-    for (uint64_t first = uint64_t(blockIdx.x) * PER; first < a.steps; first += uint64_t(gridDim.x) * PER) {
-        const uint64_t step = first + threadIdx.x / LANES;
-        if (step >= a.steps) continue;
-        if (LOSS && a.mask && !a.mask[step]) {
-            if (lane == 0) a.slopes[step] = 0.0f;
-            continue;
+    const uint64_t rows = a.steps * a.heads, per = uint64_t(GROUPS) * R;
+    const bool even = a.step == int64_t(a.heads) * a.head;  // rows are all `head` apart
+    for (uint64_t first = blockIdx.x * per; first < rows; first += gridDim.x * per) {
+        Sums r[R];
+        const T* at[R];
+        int64_t action[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const uint64_t row = first + i * GROUPS + threadIdx.x / LANES, in = row < rows ? row : rows - 1;
+            action[i] = action_of(a, in);
+            at[i] = even ? reinterpret_cast<const T*>(a.logits) + int64_t(in) * a.head : row_of<T>(a, in / a.heads, uint32_t(in % a.heads));
         }
-        double l = 0.0, entropy = 0.0;
-        const auto each_head = [&](bool again) {
-            l = entropy = 0.0;
+        if constexpr (R > 1) {
+            Word got[R];
+            float z[R][1][N];
+#pragma unroll
+            for (int i = 0; i < R; i++) got[i] = fetch<T>(at[i], lane * N, a.choices);
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                spread<T>(z[i][0], got[i]);
+                r[i] = Sums::none();
+                r[i].add(z[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < R; i++) r[i] = join<G>(r[i]);
+        } else
+            r[0] = sum_row<T, G, W>(at[0], lane, a.choices, words);
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const uint64_t row = first + i * GROUPS + threadIdx.x / LANES;
+            if (lane == 0 && row < rows) a.stats[row] = Stat{r[i].m, r[i].s, entropy_of(r[i]), chosen(at[i], action[i], a.choices)};
+        }
+    }
+}
+
+// The error of r, relative: a row's sum is off by 2^-23 for an exponential, by
+// as much times the mean |y| (at most the logarithm of the choices, 24, and a
+// little) for its argument, and by 2^-24 for each addition that a term passes.
+__device__ __forceinline__ bool near_border(const Args& a, double r) {
+    const double terms = double(a.choices < 256 ? a.choices : 256);
+    const double room = double(a.heads) * 1.2e-7 * (30.0 + 0.5 * terms) * r;
+    return fabs(r - (1.0 - a.low)) < room || fabs(r - (1.0 + a.high)) < room;
+}
+// 2^y in 64 bits, y <= 0: the series of 2^f, |f| <= 1/2, whose next term is below 2^-52.
+__device__ __forceinline__ double exp2_of(double y) {
+    if (!(y > -1000.0)) return y == y ? 0.0 : y;
+    const double n = rint(y), x = (y - n) * 0.693147180559945309417;
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, x, 1.0 / 479001600.0);
+    p = fma(p, x, 1.0 / 39916800.0);
+    p = fma(p, x, 1.0 / 3628800.0);
+    p = fma(p, x, 1.0 / 362880.0);
+    p = fma(p, x, 1.0 / 40320.0);
+    p = fma(p, x, 1.0 / 5040.0);
+    p = fma(p, x, 1.0 / 720.0);
+    p = fma(p, x, 1.0 / 120.0);
+    p = fma(p, x, 1.0 / 24.0);
+    p = fma(p, x, 1.0 / 6.0);
+    p = fma(p, x, 0.5);
+    p = fma(p, x, 1.0);
+    p = fma(p, x, 1.0);
+    return ldexp(p, int(n));
+}
+// l with sums in 64 bits, by a workgroup of 256 that is all here.
+template <class T> __device__ __forceinline__ double exact_log_prob(const Args& a, uint64_t step) {
+    __shared__ double lds[4];
+    constexpr uint32_t N = per_word<T>();
+    double l = 0.0;
+    for (uint32_t h = 0; h < a.heads; h++) {
+        const T* row = row_of<T>(a, step, h);
+        const Stat stat = a.stats[step * a.heads + h];
+        double s = 0.0;
+        for (uint32_t at = threadIdx.x * N; at < a.choices; at += 256 * N) {
+            float z[N];
+            spread<T>(z, fetch<T>(row, at, a.choices));
+#pragma unroll
+            for (uint32_t e = 0; e < N; e++) s += exp2_of((double(z[e]) - double(stat.m)) * 1.44269504088896340736);
+        }
+        s = lanes_sum<64>(s);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+        __syncthreads();
+        l += double(stat.chosen) - double(stat.m) - log((lds[0] + lds[1]) + (lds[2] + lds[3]));
+    }
+    return l;
+}
+
+// Every step's loss and slope, a step to a lane, and the workgroup's sums over steps.
+template <class T>
+__global__ void __launch_bounds__(256) steps_kernel(Args a) {
+    double total[6] = {};
+    for (uint64_t first = uint64_t(blockIdx.x) * 256; first < a.steps; first += uint64_t(gridDim.x) * 256) {
+        const uint64_t step = first + threadIdx.x;
+        const bool have = step < a.steps, counts = have && (!a.mask || a.mask[step]);
+        double l = 0.0, r = 0.0, entropy = 0.0;
+        if (counts) {
+            double product = 1.0;  // of the sums: one logarithm for many
             for (uint32_t h = 0; h < a.heads; h++) {
-                const T* row = reinterpret_cast<const T*>(a.logits) + int64_t(step) * a.step + int64_t(h) * a.head;
-                Sums sums = Sums::none();
-                for (uint32_t w = lane; w < words; w += LANES) {
-                    float z[N];
-                    load<T>(z, row, w * N, a.choices);
-                    sums.add(z);
-                }
-                sums = Group<G>::join(sums);
-                const double log_sum = again ? exact_log_sum<T, G>(row, lane, a.choices, sums.m) : log(double(sums.s));
-                const int64_t at = action_of(a, step, h);
-                // an action that is none has no log-probability
-                const double z = at >= 0 && at < int64_t(a.choices) ? double(float(row[at])) : __builtin_nan("");
-                const double own = log_sum - double(sums.t) / double(sums.s);
-                l += (z - double(sums.m)) - log_sum;
-                entropy += own;
-                if (LOSS && lane == 0) {
-                    float* to = a.stats + (step * a.heads + h) * 3;
-                    to[0] = sums.m;
-                    to[1] = float(log_sum);
-                    to[2] = float(own);
+                const Stat stat = a.stats[step * a.heads + h];
+                l += double(stat.chosen) - double(stat.m);
+                product *= double(stat.s);
+                entropy += double(stat.entropy);
+                if ((h & 31) == 31) {  // a sum is below 2^25
+                    l -= log(product);
+                    product = 1.0;
                 }
             }
-        };
-        each_head(false);
-        if constexpr (!LOSS) {
-            if (lane == 0) {
-                a.log_prob[step] = float(l);
-                a.entropy[step] = float(entropy);
-            }
-        } else {
-            const double old = a.old_log_prob[step], adv = a.advantages[step];
-            double r = exp(l - old);
-            // The 32-bit sums' error: 2^-23 an exponential, and 2^-24 for each of the additions that a term passes.
-            const double room = double(a.heads) * 6e-8 * (12.0 + double(words / LANES + 1) * N);
-            if (fabs(r - (1.0 - a.low)) < room * r || fabs(r - (1.0 + a.high)) < room * r) {
-                each_head(true);
-                r = exp(l - old);
-            }
-            const double inside = fmin(fmax(r, 1.0 - a.low), 1.0 + a.high);
+            l -= log(product);
+            r = exp(l - double(a.old_log_prob[step]));
+        }
+        // steps that 64 bits decide, one after the other by the workgroup
+        const bool near = counts && near_border(a, r);
+        if (__syncthreads_or(near)) {
+            __shared__ uint64_t open[4];
+            const uint64_t mine = __ballot(near);
+            if ((threadIdx.x & 63) == 0) open[threadIdx.x >> 6] = mine;
+            __syncthreads();
+            for (uint32_t wave = 0; wave < 4; wave++)
+                for (uint64_t left = open[wave]; left; left &= left - 1) {
+                    const uint32_t who = wave * 64 + uint32_t(__builtin_ctzll(left));
+                    const double exact = exact_log_prob<T>(a, first + who);
+                    if (threadIdx.x == who) {
+                        l = exact;
+                        r = exp(l - double(a.old_log_prob[step]));
+                    }
+                }
+            __syncthreads();  // before the next steps' flags
+        }
+        double slope = 0.0;
+        if (counts) {
+            const double adv = a.advantages[step], inside = fmin(fmax(r, 1.0 - a.low), 1.0 + a.high);
             const bool cut = inside * adv < r * adv;
-            double slope = cut ? 0.0 : -adv * r, kl = 0.0;
+            slope = cut ? 0.0 : -adv * r;
+            total[0] -= cut ? inside * adv : r * adv;
             if (a.ref_log_prob) {
                 const double far = double(a.ref_log_prob[step]) - l, e = expm1(far);
-                kl = e - far;
+                total[1] += e - far;
                 slope -= a.kl_coef * e;
             }
-            if (lane == 0) {
-                a.slopes[step] = float(slope);
-                total[0] -= cut ? inside * adv : r * adv;
-                total[1] += kl;
-                total[2] += entropy;
-                total[3] += r;
-                total[4] += inside == r ? 0.0 : 1.0;
-                total[5] += 1.0;
-            }
+            total[2] += entropy;
+            total[3] += r;
+            total[4] += inside == r ? 0.0 : 1.0;
+            total[5] += 1.0;
         }
+        if (have) a.slopes[step] = float(slope);
     }
-    if constexpr (LOSS) {
-        __shared__ double lds[6];
-        // in the order of the workgroup's lanes: the same bits every time
+    // in the order of the lanes: the same bits every time
+    __shared__ double waves[6][4];
 #pragma unroll
-        for (int i = 0; i < 6; i++) {
-            const double v = Group<G ? 64 : 0>::sum(total[i]);
-            if (G == 0) {
-                if (threadIdx.x == 0) lds[i] = v;
-            } else {
-                __shared__ double waves[4];
-                if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
-                __syncthreads();
-                if (threadIdx.x == 0) lds[i] = (waves[0] + waves[1]) + (waves[2] + waves[3]);
-                __syncthreads();
+    for (int i = 0; i < 6; i++) {
+        const double v = lanes_sum<64>(total[i]);
+        if ((threadIdx.x & 63) == 0) waves[i][threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x < 6)
+        a.parts[uint64_t(blockIdx.x) * 6 + threadIdx.x] =
+            (waves[threadIdx.x][0] + waves[threadIdx.x][1]) + (waves[threadIdx.x][2] + waves[threadIdx.x][3]);
+}
+
+// Acting: log-probabilities and entropies in one launch, G lanes to a step.
+template <class T, int G, int W>
+__global__ void __launch_bounds__(threads_of<G>()) act_kernel(Args a) {
+    constexpr uint32_t LANES = lanes_of<G>(), PER = threads_of<G>() / LANES, N = per_word<T>();
+    const uint32_t lane = threadIdx.x % LANES, words = (a.choices + N - 1) / N;
+    for (uint64_t first = uint64_t(blockIdx.x) * PER; first < a.steps; first += uint64_t(gridDim.x) * PER) {
+        const uint64_t at = first + threadIdx.x / LANES, step = at < a.steps ? at : a.steps - 1;
+        double l = 0.0, product = 1.0, entropy = 0.0;
+        for (uint32_t h = 0; h < a.heads; h++) {
+            const T* row = row_of<T>(a, step, h);
+            const double logit = chosen(row, action_of(a, step * a.heads + h), a.choices);
+            const Sums r = sum_row<T, G, W>(row, lane, a.choices, words);
+            l += logit - double(r.m);
+            product *= double(r.s);
+            entropy += double(entropy_of(r));
+            if ((h & 31) == 31) {
+                l -= log(product);
+                product = 1.0;
             }
         }
-        if (threadIdx.x == 0)
-#pragma unroll
-            for (int i = 0; i < 6; i++) a.parts[uint64_t(blockIdx.x) * 6 + i] = lds[i];
+        if (lane == 0 && at < a.steps) {
+            a.log_prob[step] = float(l - log(product));
+            a.entropy[step] = float(entropy);
+        }
     }
 }
 
@@ -239,125 +359,150 @@ __global__ void __launch_bounds__(384) finish_kernel(Args a, uint32_t count) {
     const uint32_t which = threadIdx.x >> 6, lane = threadIdx.x & 63;
     double v = 0.0;
     for (uint32_t i = lane; i < count; i += 64) v += a.parts[uint64_t(i) * 6 + which];
-    v = Group<64>::sum(v);
+    v = lanes_sum<64>(v);
     if (lane == 0) sums[which] = v;
     __syncthreads();
     if (threadIdx.x == 0) {
         const double by = sums[5] > 0.0 ? 1.0 / sums[5] : 0.0;  // no step counts: all is 0
         a.loss[0] = float((sums[0] + a.kl_coef * sums[1] - a.entropy_coef * sums[2]) * by);
 #pragma unroll
-        for (int i = 0; i < 5; i++) a.loss[1 + i] = float(sums[i] * by);
+        for (int i = 0; i < 5; i++) a.metrics[i] = float(sums[i] * by);
         a.one_over[0] = float(by);
     }
 }
 
+// G lanes have a row, or (0) a workgroup.
 template <class T, int G>
-__global__ void __launch_bounds__(Group<G>::THREADS) backward_kernel(Args a, GradArgs d) {
-    constexpr uint32_t N = per_word<T>(), LANES = Group<G>::LANES, PER = Group<G>::PER;
+__global__ void __launch_bounds__(threads_of<G>()) backward_kernel(Args a, GradArgs d) {
+    constexpr uint32_t N = per_word<T>(), LANES = lanes_of<G>(), PER = threads_of<G>() / LANES;
     const uint32_t lane = threadIdx.x % LANES, words = (a.choices + N - 1) / N;
     const float by = a.one_over[0] * d.d_loss[0], pull = float(a.entropy_coef) * by;
-    const uint64_t rows = a.steps * a.heads;
-    for (uint64_t row = uint64_t(blockIdx.x) * PER + threadIdx.x / LANES; row < rows; row += uint64_t(gridDim.x) * PER) {
-        const uint64_t step = row / a.heads;
-        const uint32_t head = uint32_t(row - step * a.heads);
-        T* out = reinterpret_cast<T*>(d.d_logits) + row * a.choices;
+    for (uint64_t step = uint64_t(blockIdx.x) * PER + threadIdx.x / LANES; step < a.steps; step += uint64_t(gridDim.x) * PER) {
         const bool counts = !a.mask || a.mask[step];
-        const T* in = reinterpret_cast<const T*>(a.logits) + int64_t(step) * a.step + int64_t(head) * a.head;
-        const float *stat = a.stats + row * 3, slope = a.slopes[step] * by;
-        const float m = stat[0], log_sum = stat[1], entropy = stat[2];
-        const int64_t chosen = action_of(a, step, head);
-        for (uint32_t w = lane; w < words; w += LANES) {
-            float z[N];
-            if (counts) {
-                load<T>(z, in, w * N, a.choices);
+        const float slope = a.slopes[step] * by;
+        for (uint32_t h = 0; h < a.heads; h++) {
+            const T* in = row_of<T>(a, step, h);
+            const uint64_t row = step * a.heads + h;
+            T* out = reinterpret_cast<T*>(d.d_logits) + row * a.choices;
+            const Stat stat = a.stats[row];
+            const float m = stat.m, log_sum = LN2 * __builtin_amdgcn_logf(stat.s), entropy = stat.entropy;
+            const int64_t at = action_of(a, row);
+            for (uint32_t w = lane; w < words; w += LANES) {
+                float z[N];
+                if (counts) {
+                    spread<T>(z, fetch<T>(in, w * N, a.choices));
 #pragma unroll
-                for (uint32_t e = 0; e < N; e++) {
-                    const float lp = (z[e] - m) - log_sum, p = expf(lp);
-                    const float free = p > 0.0f ? p * (lp + entropy) : p;
-                    z[e] = fmaf(slope, (int64_t(w) * N + e == chosen ? 1.0f : 0.0f) - p, pull * free);
+                    for (uint32_t e = 0; e < N; e++) {
+                        const float lp = (z[e] - m) - log_sum, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+                        const float free = p > 0.0f ? p * (lp + entropy) : p;
+                        z[e] = fmaf(slope, (int64_t(w * N + e) == at ? 1.0f : 0.0f) - p, pull * free);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < N; e++) z[e] = 0.0f;
                 }
-            } else {
+                if (w * N + N <= a.choices) {
+                    union { Word u; T t[N]; } v;
 #pragma unroll
-                for (uint32_t e = 0; e < N; e++) z[e] = 0.0f;
-            }
-            if (w * N + N <= a.choices) {
-                union { Word u; T t[N]; } v;
+                    for (uint32_t e = 0; e < N; e++) v.t[e] = T(z[e]);
+                    *reinterpret_cast<typename Words<T>::type*>(out + w * N) = v.u;
+                } else {
 #pragma unroll
-                for (uint32_t e = 0; e < N; e++) v.t[e] = T(z[e]);
-                *reinterpret_cast<typename Words<T>::type*>(out + w * N) = v.u;
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < N; e++)
-                    if (w * N + e < a.choices) out[w * N + e] = T(z[e]);
+                    for (uint32_t e = 0; e < N; e++)
+                        if (w * N + e < a.choices) out[w * N + e] = T(z[e]);
+                }
             }
         }
     }
 }
 
 // ---------------------------------------------------------------- launches
-// Lanes of a row: as many as it has words, up to a wavefront; a workgroup where
-// a lane would have more than 16 words.
-int lanes_of(const Args& a) {
+// Lanes of a row, and words of each: a word a lane up to a wavefront, then up
+// to four; a workgroup for wider rows.
+struct Shape { uint32_t lanes, words; };
+Shape shape_of(const Args& a) {
     const uint32_t n = a.bf ? 8 : 4, words = (a.choices + n - 1) / n;
-    return words <= 4 ? 4 : words <= 8 ? 8 : words <= 16 ? 16 : words <= 32 ? 32 : words <= 1024 ? 64 : 0;
+    if (words <= 4) return {4, 1};
+    if (words <= 8) return {8, 1};
+    if (words <= 16) return {16, 1};
+    if (words <= 32) return {32, 1};
+    if (words <= 64) return {64, 1};
+    return words <= 256 ? Shape{64, 4} : Shape{0, 0};
 }
-uint32_t blocks_of(uint64_t rows, int lanes, uint32_t most) {
-    const uint64_t per = lanes ? 256 / lanes : 1, n = (rows + per - 1) / per;
+constexpr uint32_t UNITS = 256;
+uint32_t blocks_of(uint64_t items, uint64_t per, uint64_t most) {
+    const uint64_t n = (items + per - 1) / per;
     return uint32_t(n < most ? n : most);
 }
-constexpr uint32_t MOST_BLOCKS = 2048;
+uint32_t step_blocks(const Args& a) { return blocks_of(a.steps, 256, 4 * UNITS); }
 
-struct Forward {
-    const Args& a;
-    hipStream_t st;
-    uint32_t blocks;
-    bool loss;
-    template <class T, int G> void run() const {
-        if (loss)
-            forward_kernel<T, G, true><<<dim3(blocks), dim3(Group<G>::THREADS), 0, st>>>(a);
-        else
-            forward_kernel<T, G, false><<<dim3(blocks), dim3(Group<G>::THREADS), 0, st>>>(a);
-    }
-};
-struct Backward {
-    const Args& a;
-    const GradArgs& d;
-    hipStream_t st;
-    uint32_t blocks;
-    template <class T, int G> void run() const { backward_kernel<T, G><<<dim3(blocks), dim3(Group<G>::THREADS), 0, st>>>(a, d); }
-};
-template <class T, class F> void by_lanes(int lanes, const F& f) {
-    switch (lanes) {
-        case 4: return f.template run<T, 4>();
-        case 8: return f.template run<T, 8>();
-        case 16: return f.template run<T, 16>();
-        case 32: return f.template run<T, 32>();
-        case 64: return f.template run<T, 64>();
-        default: return f.template run<T, 0>();
+template <class T> void rows(const Args& a, hipStream_t st) {
+    const Shape s = shape_of(a);
+    const uint64_t n = a.steps * a.heads;
+    const auto grid = [&](uint64_t per) { return dim3(blocks_of(n, per, 64 * UNITS)); };
+    if (!s.lanes) return rows_kernel<T, 0, 1, 4><<<grid(1), dim3(WIDE), 0, st>>>(a);
+    if (s.words == 4) return rows_kernel<T, 64, 1, 4><<<grid(4), dim3(256), 0, st>>>(a);
+    switch (s.lanes) {
+        case 4: return rows_kernel<T, 4, 4, 1><<<grid(256), dim3(256), 0, st>>>(a);
+        case 8: return rows_kernel<T, 8, 4, 1><<<grid(128), dim3(256), 0, st>>>(a);
+        case 16: return rows_kernel<T, 16, 4, 1><<<grid(64), dim3(256), 0, st>>>(a);
+        case 32: return rows_kernel<T, 32, 4, 1><<<grid(32), dim3(256), 0, st>>>(a);
+        default: return rows_kernel<T, 64, 4, 1><<<grid(16), dim3(256), 0, st>>>(a);
     }
 }
-template <class F> hipError_t by_type(const Args& a, const F& f) {
-    a.bf ? by_lanes<bf16>(lanes_of(a), f) : by_lanes<float>(lanes_of(a), f);
-    return hipGetLastError();
+template <class T> void act(const Args& a, hipStream_t st) {
+    const Shape s = shape_of(a);
+    const auto grid = [&](uint64_t per) { return dim3(blocks_of(a.steps, per, 64 * UNITS)); };
+    if (!s.lanes) return act_kernel<T, 0, 4><<<grid(1), dim3(WIDE), 0, st>>>(a);
+    if (s.words == 4) return act_kernel<T, 64, 4><<<grid(4), dim3(256), 0, st>>>(a);
+    switch (s.lanes) {
+        case 4: return act_kernel<T, 4, 1><<<grid(64), dim3(256), 0, st>>>(a);
+        case 8: return act_kernel<T, 8, 1><<<grid(32), dim3(256), 0, st>>>(a);
+        case 16: return act_kernel<T, 16, 1><<<grid(16), dim3(256), 0, st>>>(a);
+        case 32: return act_kernel<T, 32, 1><<<grid(8), dim3(256), 0, st>>>(a);
+        default: return act_kernel<T, 64, 1><<<grid(4), dim3(256), 0, st>>>(a);
+    }
+}
+template <class T> void backward(const Args& a, const GradArgs& d, hipStream_t st) {
+    const Shape s = shape_of(a);
+    const uint64_t per = s.lanes ? 256 / s.lanes : 1, n = (a.steps + per - 1) / per;
+    const dim3 grid(uint32_t(n < (1u << 16) ? n : (1u << 16))), block(s.lanes ? 256 : WIDE);
+    switch (s.lanes) {
+        case 4: return backward_kernel<T, 4><<<grid, block, 0, st>>>(a, d);
+        case 8: return backward_kernel<T, 8><<<grid, block, 0, st>>>(a, d);
+        case 16: return backward_kernel<T, 16><<<grid, block, 0, st>>>(a, d);
+        case 32: return backward_kernel<T, 32><<<grid, block, 0, st>>>(a, d);
+        case 64: return backward_kernel<T, 64><<<grid, block, 0, st>>>(a, d);
+        default: return backward_kernel<T, 0><<<grid, block, 0, st>>>(a, d);
+    }
 }
 
 }  // namespace
 
-uint64_t keep_floats(const Args& a) { return a.steps * a.heads * 3 + a.steps + 1; }
-uint32_t parts_of(const Args& a) { return blocks_of(a.steps, lanes_of(a), MOST_BLOCKS); }
+uint64_t keep_floats(const Args& a) { return a.steps * a.heads * 4 + a.steps + 1; }
+uint32_t parts_of(const Args& a) { return step_blocks(a); }
 
-hipError_t launch_log_prob(const Args& a, hipStream_t st) { return by_type(a, Forward{a, st, parts_of(a), false}); }
-
+hipError_t launch_log_prob(const Args& a, hipStream_t st) {
+    a.bf ? act<bf16>(a, st) : act<float>(a, st);
+    return hipGetLastError();
+}
 hipError_t launch_loss(const Args& a, hipStream_t st) {
     const uint32_t count = parts_of(a);
-    if (count)
-        if (hipError_t e = by_type(a, Forward{a, st, count, true})) return e;
+    if (count) {
+        a.bf ? rows<bf16>(a, st) : rows<float>(a, st);
+        if (hipError_t e = hipGetLastError()) return e;
+        if (a.bf)
+            steps_kernel<bf16><<<dim3(count), dim3(256), 0, st>>>(a);
+        else
+            steps_kernel<float><<<dim3(count), dim3(256), 0, st>>>(a);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
     finish_kernel<<<dim3(1), dim3(384), 0, st>>>(a, count);
     return hipGetLastError();
 }
-
 hipError_t launch_loss_backward(const Args& a, const GradArgs& d, hipStream_t st) {
-    return by_type(a, Backward{a, d, st, blocks_of(a.steps * a.heads, lanes_of(a), 1u << 16)});
+    a.bf ? backward<bf16>(a, d, st) : backward<float>(a, d, st);
+    return hipGetLastError();
 }
 
 }  // namespace choices

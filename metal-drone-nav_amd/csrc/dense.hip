@@ -1,3 +1,9 @@
+#ifndef MIDK
+#define MIDK 128
+#define MIDS 2
+#define MIDP false
+#define MIDW 2
+#endif
 // dense.hip — the linear layer y = residual + act(x W^T + b) and the gated
 // feed-forward block y = act(x Wg^T + bg) * (x Wu^T + bu), with gradients.
 //
@@ -49,6 +55,7 @@ __device__ __forceinline__ f32x4 four(const f32x16& v, int g) { return f32x4{v[4
 template <class T, int PW> struct Piece {
     static constexpr uint32_t N = per_word<T>(), LANES = PW / N, ROWS = 64 / LANES, TURNS = 32 / ROWS, BYTES = 32 * PW * 4;
     typedef T Word __attribute__((ext_vector_type(N), aligned(sizeof(T))));  // in memory: at any multiple of an element
+    typedef T LdsWord __attribute__((ext_vector_type(N)));
 
     // Orders LDS accesses of one wavefront; it serves them in order itself.
     static __device__ __forceinline__ void order() {
@@ -73,16 +80,16 @@ template <class T, int PW> struct Piece {
         }
     }
     // One word of a row, columns c .. c + N - 1 of `count`; 0 outside.
-    static __device__ __forceinline__ void load(const Matrix& from, uint32_t m, uint32_t c, uint32_t count, float (&z)[N]) {
+    static __device__ __forceinline__ LdsWord load(const Matrix& from, uint32_t m, uint32_t c, uint32_t count) {
         const T* p = reinterpret_cast<const T*>(from.p) + int64_t(m) * from.ld + c;
+        LdsWord v;
         if (c + N <= count) {
-            const Word v = *reinterpret_cast<const Word*>(p);
-#pragma unroll
-            for (uint32_t e = 0; e < N; e++) z[e] = float(v[e]);
+            v = *reinterpret_cast<const Word*>(p);
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < N; e++) z[e] = c + e < count ? float(p[e]) : 0.0f;
+            for (uint32_t e = 0; e < N; e++) v[e] = c + e < count ? p[e] : T(0.0f);
         }
+        return v;
     }
     static __device__ __forceinline__ void store(const Matrix& to, uint32_t m, uint32_t c, uint32_t count, const float (&z)[N]) {
         T* p = reinterpret_cast<T*>(to.p) + int64_t(m) * to.ld + c;
@@ -99,12 +106,18 @@ template <class T, int PW> struct Piece {
     }
 };
 
+// A wavefront's LDS for pieces of 32 or 64 columns, of both projections and of what is beside them; which fits into `room`.
+template <class T, bool N2> constexpr uint32_t piece_bytes(int tiles) {
+    return tiles == 2 ? (N2 ? 2 : 1) * Piece<T, 64>::BYTES + Piece<T, 64>::TURNS * 1024 : (N2 ? 2 : 1) * Piece<T, 32>::BYTES + Piece<T, 32>::TURNS * 1024;
+}
+template <class T, bool N2> constexpr int piece_tiles(int tiles, uint32_t room) { return tiles >= 2 && piece_bytes<T, N2>(2) <= room ? 2 : 1; }
+
 // ---------------------------------------------------------------- the product
 // BN counts the rows of LDS: of the gated block's projections, half each.
 // PIPED: one wavefront on each SIMD, whose loads and LDS reads go out between
 // its own products (there is no other to fill the gaps).
 template <class T, int BM, int BN, int WM, int WN, int KB, int STAGES, bool PIPED, bool MC, bool NC, int RESULT>
-__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN == 4 && PIPED ? 1 : 2))) product_kernel(Job a) {
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(BM == 256 ? 1 : MIDW))) product_kernel(Job a) {
     constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr bool N2 = two_weights(RESULT);
     constexpr int OUT = N2 ? BN / 2 : BN, TO = N2 ? TN / 2 : TN;  // columns of the result, and a wavefront's tiles of them
@@ -292,17 +305,32 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     }
 
     // ---- the result, PW columns of 32 rows at a time
-    constexpr int PT = TO >= 2 ? 2 : 1, PW = 32 * PT;
     typedef typename std::conditional<RESULT == PART, float, T>::type TR;
+    constexpr int PT = piece_tiles<TR, N2>(TO, STAGES * STAGE / W), PW = 32 * PT;
+    constexpr uint32_t REGION = piece_bytes<TR, N2>(PT);
     typedef Piece<TR, PW> Out;
-    constexpr uint32_t REGION = STAGES * STAGE / W, N = Out::N;
+    constexpr uint32_t N = Out::N;
     constexpr bool SLOPES = RESULT == SLOPE || RESULT == GATED_SLOPE;
-    static_assert((N2 ? 2 : 1) * Out::BYTES <= REGION, "");
+    constexpr uint32_t BESIDE = (N2 ? 2 : 1) * Out::BYTES;
     char* own = shared + wave * REGION;
     Matrix y = (RESULT == STORE || RESULT == PART) && batch ? a.y2 : a.y;
     if (RESULT == PART) y.p += uint64_t(piece) * mc * y.ld * 4;
     Matrix dz2 = a.dz;
     dz2.p += uint64_t(a.dz_half) * sizeof(T);
+    // What is beside a piece, the residual or the gradient of y, is loaded while
+    // the piece before it is worked on, and waits in LDS.
+    const bool beside = SLOPES || (RESULT == LINEAR && a.residual.p);
+    const Matrix side = RESULT == LINEAR ? a.residual : a.dy;
+    typename Out::LdsWord words[Out::TURNS];
+    const auto load_beside = [&](int i0, int j) {
+        const uint32_t n = n0 + 32 * i0 + Out::column(lane);
+#pragma unroll
+        for (uint32_t t = 0; t < Out::TURNS; t++) {
+            const uint32_t m = m0 + 32 * j + Out::row(lane, t);
+            if (m < mc) words[t] = Out::load(side, m, n, nc);
+        }
+    };
+    if (beside) load_beside(0, 0);
 #pragma unroll
     for (int i0 = 0; i0 < TO; i0 += PT) {
         const uint32_t n = n0 + 32 * i0 + Out::column(lane);
@@ -315,6 +343,15 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
                 Out::put(own, acc[i0 + i][j], i, lane);
                 if constexpr (N2) Out::put(own + Out::BYTES, acc[TO + i0 + i][j], i, lane);
             }
+            if (beside) {
+#pragma unroll
+                for (uint32_t t = 0; t < Out::TURNS; t++)
+                    *reinterpret_cast<typename Out::LdsWord*>(own + BESIDE + t * 1024 + lane * 16) = words[t];
+                if (j + 1 < TM)
+                    load_beside(i0, j + 1);
+                else if (i0 + PT < TO)
+                    load_beside(i0 + PT, 0);
+            }
             Out::order();
 #pragma unroll 1
             for (uint32_t t = 0; t < Out::TURNS; t++) {
@@ -323,13 +360,16 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
                 float z[N], up[N], with[N];
                 Out::get(own, Out::row(lane, t), lane, z);
                 if constexpr (N2) Out::get(own + Out::BYTES, Out::row(lane, t), lane, up);
+                if (beside) {
+                    const auto word = *reinterpret_cast<const typename Out::LdsWord*>(own + BESIDE + t * 1024 + lane * 16);
+#pragma unroll
+                    for (uint32_t e = 0; e < N; e++) with[e] = float(word[e]);
+                }
                 if constexpr (RESULT == LINEAR) {
                     act_of<T>(a.act, z);
-                    if (a.residual.p) {
-                        Out::load(a.residual, m, n, nc, with);
+                    if (beside)
 #pragma unroll
                         for (uint32_t e = 0; e < N; e++) z[e] += with[e];
-                    }
                 }
                 if constexpr (RESULT == GATED) {
                     act_of<T>(a.act, z);
@@ -339,7 +379,6 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
                 if constexpr (SLOPES) {
                     // zeros past the last column, also where z is none: the next products read whole words
                     float slope[N];
-                    Out::load(a.dy, m, n, nc, with);
                     act_of<T>(a.act, z, slope);
 #pragma unroll
                     for (uint32_t e = 0; e < N; e++) {
@@ -458,7 +497,10 @@ uint32_t blocks_for(uint64_t items, uint32_t per, uint32_t most) {
 
 template <class T, int BM, int BN, int WM, int WN, int KB, int STAGES, bool PIPED, bool MC, bool NC, int RESULT>
 hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
-    constexpr uint32_t OUT = two_weights(RESULT) ? BN / 2 : BN, bytes = STAGES * (BM + BN) * KB;
+    constexpr bool N2 = two_weights(RESULT);
+    typedef typename std::conditional<RESULT == PART, float, T>::type TR;
+    constexpr uint32_t OUT = N2 ? BN / 2 : BN, stages = STAGES * (BM + BN) * KB, room = stages / (WM * WN);
+    constexpr uint32_t pieces = WM * WN * piece_bytes<TR, N2>(piece_tiles<TR, N2>(OUT / WN / 32, room)), bytes = pieces > stages ? pieces : stages;
     static_assert(bytes <= 160 * 1024, "");
     a.m_tiles = (a.m.count + BM - 1) / BM;
     a.n_tiles = (a.n.count + OUT - 1) / OUT;
@@ -470,18 +512,40 @@ hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
     return hipGetLastError();
 }
 
-// The tile of a product of m x n results: the largest whose tiles fill the 256 compute units.
+// The tile of a product: the one of the least estimated time.  A compute unit
+// takes one large tile at a time and two of the others; measured, in us: a step
+// of 128 bytes of k alone on a compute unit and beside another tile, and what a
+// tile takes besides (512 x 2,048 x 2,048 in bfloat16: 15, 26 and 48 us on small,
+// middle and large tiles; 32,768 x 5,120 to 1,280: 775, 506 and 405; 262,144 x 184
+// to 256: 103, 65 and 93).
 enum Tile { SMALL, MIDDLE, LARGE };
-Tile tile_of(uint64_t m, uint64_t n, uint64_t times) {
-    const auto tiles = [&](uint64_t b) { return (m + b - 1) / b * ((n + b - 1) / b) * times; };
-    if (tiles(256) >= 256) return LARGE;
-    return tiles(128) >= 256 ? MIDDLE : SMALL;
+constexpr uint32_t UNITS = 256;
+struct Cost { uint32_t m, n; float alone, beside, rest; };
+// of: bfloat16 or not, projections of a gated block beside each other or one
+Cost cost_of(Tile t, bool bf, bool two) {
+    switch (t) {
+        case SMALL: return {64, 64, (bf ? 0.38f : 0.55f) * (two ? 1.6f : 1.0f), (bf ? 0.48f : 1.02f) * (two ? 1.8f : 1.0f), two ? 2.2f : 1.8f};
+        case MIDDLE: return {128, two ? 64u : 128u, bf ? 0.72f : 2.1f, bf ? (two ? 1.05f : 1.25f) : 4.1f, two ? 3.4f : 4.6f};
+        default: return {256, two ? 128u : 256u, bf ? 1.77f : 8.2f, bf ? 3.54f : 16.4f, two ? 9.0f : 16.0f};
+    }
+}
+float time_of(Tile t, bool bf, bool two, uint64_t m, uint64_t n, uint64_t k, uint64_t times) {
+    const Cost c = cost_of(t, bf, two);
+    const uint64_t tiles = (m + c.m - 1) / c.m * ((n + c.n - 1) / c.n) * times, each = (tiles + UNITS - 1) / UNITS;
+    const float steps = float((k * (bf ? 2 : 4) + 127) / 128), rest = t == LARGE ? 2.0f * c.rest : c.rest;
+    return float(each / 2) * (steps * c.beside + rest) + (each & 1 ? steps * c.alone + c.rest : 0.0f);
+}
+Tile tile_of(bool bf, bool two, uint64_t m, uint64_t n, uint64_t k) {
+    Tile best = SMALL;
+    for (Tile t : {MIDDLE, LARGE})
+        if (time_of(t, bf, two, m, n, k, 1) < time_of(best, bf, two, m, n, k, 1)) best = t;
+    return best;
 }
 
 template <class T, bool MC, bool NC, int RESULT>
 hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
     if (tile == LARGE) return launch<T, 256, 256, 2, 2, 128, 2, true, MC, NC, RESULT>(a, batches, st);
-    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 128, 2, false, MC, NC, RESULT>(a, batches, st);
+    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, MIDK, MIDS, MIDP, MC, NC, RESULT>(a, batches, st);
     if constexpr (two_weights(RESULT))
         return launch<T, 64, 128, 2, 2, 128, 3, false, MC, NC, RESULT>(a, batches, st);
     else
@@ -516,7 +580,7 @@ Plan plan_of(const Args& a) {
     p.w_copy = !in_words(a.w[0], a.in, p.size) || (a.gated && (!in_words(a.w[1], a.in, p.size) || a.w[1].ld != a.w[0].ld));
     p.x_bytes = p.x_copy ? aligned(a.rows * p.in_ld * p.size) : 0;
     p.w_bytes = p.w_copy ? aligned(uint64_t(a.out) * p.in_ld * p.size) : 0;
-    p.forward_tile = tile_of(a.rows, uint64_t(a.out) * pieces_of(a), 1);
+    p.forward_tile = tile_of(a.bf, a.gated, a.rows, a.out, a.in);
     return p;
 }
 // Of the backward pass.
@@ -545,20 +609,23 @@ BackPlan back_plan_of(const Args& a, const GradArgs& d) {
     } else
         p.sum_rows = uint32_t(a.rows < 16 * SHARES ? (a.rows + 15) / 16 : SHARES);
     p.sums_bytes = db ? aligned(uint64_t(p.sum_rows) * 2 * a.out * 4) : 0;
-    p.dx_tile = tile_of(a.rows, a.in, 1);
-    // dW: few results, a long sum. Pieces of at least 512 rows, as many as make 512 workgroups.
-    const uint64_t most = (a.rows + 511) / 512;
-    p.dw_tile = tile_of(a.out, a.in, pieces * most);
-    const uint64_t b = p.dw_tile == LARGE ? 256 : p.dw_tile == MIDDLE ? 128 : 64;
-    const uint64_t tiles = (a.out + b - 1) / b * ((a.in + b - 1) / b) * pieces;
-    const uint64_t want = p.dw_tile == LARGE ? 256 : 512;
-    uint64_t splits = (want + tiles - 1) / tiles;
-    if (splits > most) splits = most;
-    if (splits < 1) splits = 1;
-    p.split_k = uint32_t((a.rows + splits - 1) / splits + 63) / 64 * 64;
-    if (p.split_k == 0) p.split_k = 64;
-    p.splits = uint32_t((a.rows + p.split_k - 1) / p.split_k);
-    if (p.splits < 1) p.splits = 1;
+    p.dx_tile = tile_of(a.bf, false, a.rows, a.in, uint64_t(a.out) * pieces);
+    // dW has few results and a long sum, which is cut into pieces of at least 256
+    // rows: as many as are worth the 4.5 TB/s at which their fp32 results are
+    // written and added up.
+    float least = 0.0f;
+    uint32_t rows = 0;
+    const uint64_t most = (a.rows + 255) / 256;
+    for (uint32_t splits = 1; splits <= (most < 64 ? most : 64); splits++) {
+        const uint32_t k = uint32_t((a.rows + splits - 1) / splits + 63) / 64 * 64;
+        const float parts = splits == 1 ? 0.0f : 5.0f + float(splits) * float(a.out) * float(a.in) * float(pieces) * 8.0f / 4.5e6f;
+        for (Tile t : {SMALL, MIDDLE, LARGE}) {
+            const float time = time_of(t, a.bf, false, a.out, a.in, k, uint64_t(pieces) * splits) + parts;
+            if (rows == 0 || time < least) least = time, rows = k, p.dw_tile = t;
+        }
+    }
+    p.split_k = rows;
+    p.splits = uint32_t((a.rows + rows - 1) / rows);
     p.parts_bytes = dw && p.splits > 1 ? aligned(uint64_t(pieces) * p.splits * a.out * a.in * 4) : 0;
     return p;
 }

@@ -47,7 +47,7 @@ class _Choices(ctypes.Structure):
 class _ChoiceLoss(ctypes.Structure):
     _fields_ = [(n, P) for n in ("old_log_prob", "advantages", "ref_log_prob", "mask")]
     _fields_ += [(n, ctypes.c_double) for n in ("clip_low", "clip_high", "kl_coef", "entropy_coef")]
-    _fields_ += [("loss", P)]
+    _fields_ += [("loss", P), ("metrics", P)]
 
 
 # The structs as packed bytes, made of plain numbers in one call each.
@@ -55,7 +55,7 @@ _DENSE = struct.Struct("=Q5I4x12q")
 _DENSE_GRAD = struct.Struct("=10q")
 assert _DENSE.size == ctypes.sizeof(_Dense) and _DENSE_GRAD.size == ctypes.sizeof(_DenseGrad)
 _CHOICES = struct.Struct("=Q4I4q")
-_CHOICE_LOSS = struct.Struct("=4q4dq")
+_CHOICE_LOSS = struct.Struct("=4q4d2q")
 assert _CHOICES.size == ctypes.sizeof(_Choices) and _CHOICE_LOSS.size == ctypes.sizeof(_ChoiceLoss)
 _NONE = (0, 0)
 
@@ -261,17 +261,18 @@ class _LossCall(_ChoiceCall):
                 raise TypeError("%s is %s: float32 is taken" % (name, t.dtype))
         self.rows = [None if t is None else t.contiguous() for t in rows]
         self.l = _ChoiceLoss.from_buffer_copy(_CHOICE_LOSS.pack(*(_address(t) or 0 for t in self.rows), low, high, kl_coef,
-                                                                entropy_coef, 0))
+                                                                entropy_coef, 0, 0))
 
     def forward(self):
         L = _library()
         keep, work = ctypes.c_uint64(), ctypes.c_uint64()
         check(L.mdn_op_choices_loss_sizes(ctypes.byref(self.c), ctypes.byref(keep), ctypes.byref(work)))
-        kept, buffer, out = _buffer(keep.value, self.device), _buffer(work.value, self.device), self.results(6)
-        self.l.loss = out.data_ptr()
+        kept, buffer = _buffer(keep.value, self.device), _buffer(work.value, self.device)
+        loss, metrics = self.results(), self.results(5)
+        self.l.loss, self.l.metrics = loss.data_ptr(), metrics.data_ptr()
         check(L.mdn_op_choices_loss_forward(ctypes.byref(self.c), ctypes.byref(self.l), _address(kept), keep.value,
                                             _address(buffer), work.value, _stream(self.device)))
-        return out, kept
+        return loss, metrics, kept
 
     def backward(self, kept, d_loss, shape):
         made = torch.empty(shape, dtype=self.logits.dtype, device=self.device)
@@ -285,10 +286,9 @@ class _LossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, old_log_prob, advantages, ref_log_prob, mask, *numbers):
         call = _LossCall(logits, actions, old_log_prob, advantages, ref_log_prob, mask, *numbers)
-        out, kept = _on(call.device, call.forward)
+        loss, metrics, kept = _on(call.device, call.forward)
         ctx.numbers = numbers
         ctx.save_for_backward(logits, actions, old_log_prob, advantages, ref_log_prob, mask, kept)
-        loss, metrics = out[0].clone(), out[1:]
         ctx.mark_non_differentiable(metrics)
         ctx.set_materialize_grads(False)
         return loss, metrics
@@ -344,8 +344,7 @@ def clipped_loss(logits, actions, old_log_prob, advantages, ref_log_prob=None, m
     if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return _LossFunction.apply(logits, actions, *rows, *numbers)
     call = _LossCall(logits, actions, *rows, *numbers)
-    out, _ = _on(call.device, call.forward)
-    return out[0], out[1:]
+    return _on(call.device, call.forward)[:2]
 
 
 def log_prob(logits, actions):
