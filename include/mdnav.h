@@ -553,8 +553,8 @@ int mdn_op_dense_forward(const MdnDense* dense, void* workspace, uint64_t worksp
 /* The gradients, from the same inputs and the gradient of y, which is also
  * the residual's.  Those whose data is NULL are not wanted; `residual` and
  * `y` of `dense` are not read.  What the activation had as its argument is
- * made again, bit for bit; its gradient enters the products that follow
- * rounded to dtype, and the biases' unrounded. */
+ * made again; its gradient enters the products that follow rounded to dtype,
+ * and the biases' unrounded. */
 typedef struct MdnDenseGrad {
     MdnMatrix d_y, d_x, d_w, d_w_up;
     void *d_b, *d_b_up;

@@ -1,9 +1,3 @@
-#ifndef MIDK
-#define MIDK 128
-#define MIDS 2
-#define MIDP false
-#define MIDW 2
-#endif
 // dense.hip — the linear layer y = residual + act(x W^T + b) and the gated
 // feed-forward block y = act(x Wg^T + bg) * (x Wu^T + bu), with gradients.
 //
@@ -12,7 +6,7 @@
 // the other at the same place; bias, activation and product or residual are
 // made from the fp32 sums, which are rounded once.
 //
-// Backward: z is made again by the same product, bit for bit, with
+// Backward: z is made again by the same product with
 //     dz = dy act'(z)        or  dzg = dy zu act'(zg),  dzu = dy act(zg)
 // in its epilogue, rounded once to the rows' type (the matrix cores' operand),
 // and the column sums that are the biases' gradients, from the unrounded
@@ -117,7 +111,7 @@ template <class T, bool N2> constexpr int piece_tiles(int tiles, uint32_t room) 
 // PIPED: one wavefront on each SIMD, whose loads and LDS reads go out between
 // its own products (there is no other to fill the gaps).
 template <class T, int BM, int BN, int WM, int WN, int KB, int STAGES, bool PIPED, bool MC, bool NC, int RESULT>
-__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(BM == 256 ? 1 : MIDW))) product_kernel(Job a) {
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(BM == 256 ? 1 : KB == 64 ? 3 : 2))) product_kernel(Job a) {
     constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr bool N2 = two_weights(RESULT);
     constexpr int OUT = N2 ? BN / 2 : BN, TO = N2 ? TN / 2 : TN;  // columns of the result, and a wavefront's tiles of them
@@ -524,9 +518,9 @@ struct Cost { uint32_t m, n; float alone, beside, rest; };
 // of: bfloat16 or not, projections of a gated block beside each other or one
 Cost cost_of(Tile t, bool bf, bool two) {
     switch (t) {
-        case SMALL: return {64, 64, (bf ? 0.38f : 0.55f) * (two ? 1.6f : 1.0f), (bf ? 0.48f : 1.02f) * (two ? 1.8f : 1.0f), two ? 2.2f : 1.8f};
-        case MIDDLE: return {128, two ? 64u : 128u, bf ? 0.72f : 2.1f, bf ? (two ? 1.05f : 1.25f) : 4.1f, two ? 3.4f : 4.6f};
-        default: return {256, two ? 128u : 256u, bf ? 1.77f : 8.2f, bf ? 3.54f : 16.4f, two ? 9.0f : 16.0f};
+        case SMALL: return {64, 64, (bf ? 0.38f : 0.55f) * (two ? 1.6f : 1.0f), (bf ? 0.48f : 1.02f) * (two ? 1.8f : 1.0f), bf ? (two ? 2.2f : 1.8f) : 6.0f};
+        case MIDDLE: return {128, two ? 64u : 128u, bf ? 0.72f : 2.1f, bf ? (two ? 1.05f : 1.25f) : 4.1f, bf ? (two ? 3.4f : 4.6f) : (two ? 3.0f : 9.0f)};
+        default: return {256, two ? 128u : 256u, bf ? 1.77f : 8.2f, bf ? 3.54f : 16.4f, bf ? (two ? 9.0f : 16.0f) : (two ? 9.0f : 25.0f)};
     }
 }
 float time_of(Tile t, bool bf, bool two, uint64_t m, uint64_t n, uint64_t k, uint64_t times) {
@@ -545,7 +539,15 @@ Tile tile_of(bool bf, bool two, uint64_t m, uint64_t n, uint64_t k) {
 template <class T, bool MC, bool NC, int RESULT>
 hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
     if (tile == LARGE) return launch<T, 256, 256, 2, 2, 128, 2, true, MC, NC, RESULT>(a, batches, st);
-    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, MIDK, MIDS, MIDP, MC, NC, RESULT>(a, batches, st);
+    if constexpr (!MC && !NC) {
+        // Where there are more than two middle tiles a compute unit, three at once with
+        // half the LDS: 262,144 rows of 256 to 1,024, gated: 424 us, and 478 with two;
+        // of 64: 220 and 267; but 1,024 of 5,120 to 5,120: 97 and 73.
+        const uint64_t out = two_weights(RESULT) ? 64 : 128;
+        if (tile == MIDDLE && (a.m.count + 127ull) / 128 * ((a.n.count + out - 1) / out) > 2 * UNITS)
+            return launch<T, 128, 128, 2, 2, 64, 2, false, MC, NC, RESULT>(a, batches, st);
+    }
+    if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 128, 2, false, MC, NC, RESULT>(a, batches, st);
     if constexpr (two_weights(RESULT))
         return launch<T, 64, 128, 2, 2, 128, 3, false, MC, NC, RESULT>(a, batches, st);
     else

@@ -22,12 +22,31 @@ template <class T> __device__ __forceinline__ float tanh_of(float z) {
 }
 constexpr float C_TANH = 1.5957691216f;  // 2 sqrt(2 / pi)
 
+// Phi(z) of the normal distribution, and exp(-z^2 / 2).  For bfloat16 the
+// approximation 7.1.26 of Abramowitz and Stegun's handbook, whose tail is good to
+// 2^-9 of its value down to z = -5 (and 2^-7 to -7), in place of erfc: 32,768 x 2,560
+// to 5,120 then takes as long as with silu, and 15 % longer with erfc.
+template <class T> __device__ __forceinline__ float normal(float z, float& e) {
+    e = exp_of<T>(-0.5f * z * z);
+    if (sizeof(T) == 4) return 0.5f * erfcf(-0.70710678f * z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.0f));
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    q *= 0.5f * t * e;
+    return z < 0.0f ? q : 1.0f - q;
+}
+
 template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z) {
     if (ACT == MDN_ACT_RELU) return z > 0.0f ? z : z == z ? 0.0f : z;
     if (ACT == MDN_ACT_TANH) return tanh_of<T>(z);
     if (ACT == MDN_ACT_SIGMOID) return sigmoid<T>(z);
     if (ACT == MDN_ACT_SILU) return z * sigmoid<T>(z);
-    if (ACT == MDN_ACT_GELU) return 0.5f * z * erfcf(-0.70710678f * z);
+    if (ACT == MDN_ACT_GELU) {
+        float e;
+        return z * normal<T>(z, e);
+    }
     if (ACT == MDN_ACT_GELU_TANH) return z * sigmoid<T>(C_TANH * z * fmaf(0.044715f * z, z, 1.0f));
     return z;
 }
@@ -57,8 +76,9 @@ template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z
         return z * s;
     }
     if (ACT == MDN_ACT_GELU) {
-        const float s = 0.5f * erfcf(-0.70710678f * z);
-        slope = fmaf(z * 0.39894228f, exp_of<T>(-0.5f * z * z), s);
+        float e;
+        const float s = normal<T>(z, e);
+        slope = fmaf(z * 0.39894228f, e, s);
         return z * s;
     }
     if (ACT == MDN_ACT_GELU_TANH) {

@@ -1,10 +1,11 @@
 // dense_rows.hip — the forward call of few rows: a tick of a few vehicles, whose
 // cost is reading the weights once.
 //
-// A workgroup makes 16 columns of the result for up to 16 MT rows.  Its W
-// wavefronts take turns along k, 128 bytes of each of the 16 weight rows at a
-// time (whole lines, straight to registers, UNROLL of them on their way), as
-// operands of 16 x 16 tiles; their sums meet in LDS.
+// A workgroup makes up to 16 columns of the result for up to 16 MT rows.  Its W
+// wavefronts take turns along k, 128 bytes of each of the weight rows at a time
+// (whole lines, straight to registers, UNROLL of them on their way), as operands
+// of 16 x 16 tiles; their sums meet in LDS.  Bound by memory: one row of 5,120 to
+// 65,536 in bfloat16 reads its weights at 5.4 TB/s.
 #include "dense.h"
 
 #include "dense_tiles.h"
@@ -43,13 +44,14 @@ template <class T, bool WORDS> __device__ __forceinline__ typename Word<T>::type
 }
 
 template <class T, int MT, int W, bool G, bool WORDS>
-__global__ void __launch_bounds__(64 * W) rows_kernel(Args a) {
+__global__ void __launch_bounds__(64 * W) rows_kernel(Args a, uint32_t columns) {
     constexpr int N = G ? 2 : 1, UNROLL = WORDS ? (MT * N <= 2 ? 4 : 2) : 1;
     __shared__ f32x4 part[W][N * MT][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT, rows = uint32_t(a.rows);
+    const uint32_t n0 = blockIdx.x * columns, m0 = blockIdx.y * 16 * MT, rows = uint32_t(a.rows);
+    const uint32_t n_end = n0 + columns < a.out ? n0 + columns : a.out;
     const T *w[N], *x[MT];
-    const uint32_t n = n0 + (lane & 15) < a.out ? n0 + (lane & 15) : a.out - 1;
+    const uint32_t n = n0 + (lane & 15) < n_end ? n0 + (lane & 15) : n_end - 1;
 #pragma unroll
     for (int i = 0; i < N; i++) w[i] = reinterpret_cast<const T*>(a.w[i].p) + int64_t(n) * a.w[i].ld;
 #pragma unroll
@@ -66,7 +68,7 @@ __global__ void __launch_bounds__(64 * W) rows_kernel(Args a) {
     for (uint32_t k = wave * step; k < a.in; k += W * step * UNROLL) {
         typename Word<T>::type fw[UNROLL][2][N], fx[UNROLL][2][MT];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++)
+        for (int u = 0; u < UNROLL; u++) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t c = k + u * W * step + h * (step / 2) + at;
@@ -75,6 +77,7 @@ __global__ void __launch_bounds__(64 * W) rows_kernel(Args a) {
 #pragma unroll
                 for (int j = 0; j < MT; j++) fx[u][h][j] = word_at<T, WORDS>(x[j], c, a.in);
             }
+        }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++)
 #pragma unroll
@@ -99,25 +102,37 @@ __global__ void __launch_bounds__(64 * W) rows_kernel(Args a) {
             for (int s = 1; s < W; s++) z[i] += part[s][i * MT + j][lane];
         }
         const uint32_t m = m0 + 16 * j + (lane & 15), c = n0 + 4 * (lane >> 4);
-        if (m >= rows || c >= a.out) continue;
+        if (m >= rows || c >= n_end) continue;
 #pragma unroll
         for (int i = 0; i < N; i++)
-            if (a.b[i]) z[i] += load4<T>(a.b[i], c, a.out);
+            if (a.b[i]) z[i] += load4<T>(a.b[i], c, n_end);
         float act[4] = {z[0][0], z[0][1], z[0][2], z[0][3]};
         act_of<T>(a.activation, act);
         f32x4 v = {act[0], act[1], act[2], act[3]};
         if constexpr (G) v = v * z[1];
-        if (!G && a.residual.p) v = load4<T>(row_of<T>(a.residual, m), c, a.out) + v;
-        store4<T>(row_of<T>(a.y, m), c, a.out, v);
+        if (!G && a.residual.p) v = load4<T>(row_of<T>(a.residual, m), c, n_end) + v;
+        store4<T>(row_of<T>(a.y, m), c, n_end, v);
     }
 }
 
+// Columns of a workgroup, so that the compute units have the same to read: a
+// weight's row each, and the rows of x, which come from the L2, at a third.  (1 row of
+// 5,120 to 5,120 in bfloat16: 13.6 us with 10, and 17 with 16, which is 320
+// workgroups on 256 units; 24 rows of 5,120 to 1,280: 13.3 with 5 and 17.5 with 16.)
+uint32_t columns_of(const Args& a) {
+    uint32_t best = 16;
+    const auto cost = [&](uint32_t c) { return ((a.out + c - 1) / c + 255) / 256 * (float(c) + 0.33f * float(a.rows)); };
+    for (uint32_t c = 15; c >= 1; c--)
+        if (cost(c) < 0.95f * cost(best)) best = c;
+    return best;
+}
 template <class T, int MT, int W, bool G> hipError_t launch(const Args& a, bool words, hipStream_t st) {
-    const dim3 grid((a.out + 15) / 16, uint32_t((a.rows + 16 * MT - 1) / (16 * MT)));
+    const uint32_t columns = columns_of(a);
+    const dim3 grid((a.out + columns - 1) / columns, uint32_t((a.rows + 16 * MT - 1) / (16 * MT)));
     if (words)
-        rows_kernel<T, MT, W, G, true><<<grid, dim3(64 * W), 0, st>>>(a);
+        rows_kernel<T, MT, W, G, true><<<grid, dim3(64 * W), 0, st>>>(a, columns);
     else
-        rows_kernel<T, MT, W, G, false><<<grid, dim3(64 * W), 0, st>>>(a);
+        rows_kernel<T, MT, W, G, false><<<grid, dim3(64 * W), 0, st>>>(a, columns);
     return hipGetLastError();
 }
 template <class T, int MT, bool G> hipError_t by_waves(const Args& a, bool words, hipStream_t st) {
@@ -133,7 +148,14 @@ template <class T, bool G> hipError_t by_rows(const Args& a, bool words, hipStre
 
 }  // namespace
 
-bool few_rows(const Args& a) { return a.rows <= 32; }
+// Up to where this is faster than tiles: 64 rows in bfloat16 and 128 in fp32, more
+// where the weights are small. In bfloat16, 64 rows of 1,024 to 1,024: 6.9 us here and 7.2
+// on tiles, 128: 11.3 and 7.2; of 184 to 256, 256 rows: 3.0 and 3.5, 512: 3.7 and 3.6. In fp32, 128
+// rows of 1,024 to 1,024: 24 and 33, 256: 41 and 34; of 181 to 333, 512 rows: 11.8 and 12.4.
+bool few_rows(const Args& a) {
+    const bool small = uint64_t(a.in) * a.out * (a.gated ? 2 : 1) <= 1u << 16;
+    return a.rows <= (a.bf ? (small ? 256u : 64u) : (small ? 512u : 128u));
+}
 
 hipError_t forward_few(const Args& a, hipStream_t st) {
     const uint32_t size = a.bf ? 2 : 4, per = 16 / size;
