@@ -14,6 +14,12 @@ namespace dense {
 // faster exponential, whose relative error is |z| 2^-24.
 template <class T> __device__ __forceinline__ float exp_of(float x) { return sizeof(T) == 2 ? __expf(x) : expf(x); }
 template <class T> __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_of<T>(-z)); }
+// sigmoid(z) and sigmoid(-z), neither by a difference from 1.
+template <class T> __device__ __forceinline__ float sigmoids(float z, float& other) {
+    const float e = exp_of<T>(-fabsf(z)), big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+    other = z < 0.0f ? big : small;
+    return z < 0.0f ? small : big;
+}
 template <class T> __device__ __forceinline__ float tanh_of(float z) {
     if (sizeof(T) == 4) return tanhf(z);
     // 1 - 2 / (e^2z + 1) cancels near 0, where the series' next term is below 2^-17 of the value
@@ -66,13 +72,15 @@ template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z
         return t;
     }
     if (ACT == MDN_ACT_SIGMOID) {
-        const float s = sigmoid<T>(z);
-        slope = s * sigmoid<T>(-z);
+        float other;
+        const float s = sigmoids<T>(z, other);
+        slope = s * other;
         return s;
     }
     if (ACT == MDN_ACT_SILU) {
-        const float s = sigmoid<T>(z);
-        slope = s * fmaf(z, 1.0f - s, 1.0f);
+        float other;
+        const float s = sigmoids<T>(z, other);
+        slope = s * fmaf(z, other, 1.0f);
         return z * s;
     }
     if (ACT == MDN_ACT_GELU) {
@@ -84,8 +92,9 @@ template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z
     if (ACT == MDN_ACT_GELU_TANH) {
         // beyond 30 the slope is 0 or 1; the polynomial would overflow
         const float c = fminf(fmaxf(z, -30.0f), 30.0f), u = C_TANH * c * fmaf(0.044715f * c, c, 1.0f);
-        const float s = sigmoid<T>(u);
-        slope = fmaf(c * s * (1.0f - s), C_TANH * fmaf(0.134145f * c, c, 1.0f), s) + 0.0f * z;
+        float other;
+        const float s = sigmoids<T>(u, other);
+        slope = fmaf(c * s * other, C_TANH * fmaf(0.134145f * c, c, 1.0f), s) + 0.0f * z;
         return z * s;
     }
     slope = 1.0f;

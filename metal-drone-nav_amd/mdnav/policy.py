@@ -179,6 +179,12 @@ _LINEAR = ("x", "weight", "weight", "bias", "bias", "residual")
 _GATED = ("x", "w_gate", "w_up", "b_gate", "b_up", "residual")
 
 
+def _tensors(**args):
+    for name, t in args.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s is no tensor" % name)
+
+
 def linear(x, weight, bias=None, activation=None, residual=None):
     """residual + act(x weight^T + bias), rounded once.
 
@@ -190,6 +196,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     activation's argument is made again for them and not kept, and its gradient
     enters the products that follow with the rows' type.
     """
+    _tensors(x=x, weight=weight)
     return _dense(_LINEAR, activation, x, weight, None, bias, None, residual)
 
 
@@ -199,8 +206,7 @@ def gated_feed_forward(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu
     x: [..., in], w_gate, w_up: [out, in], b_gate, b_up: [out]; types,
     activations, strides and gradients as in ``linear``.
     """
-    if not isinstance(w_up, torch.Tensor):
-        raise TypeError("w_up is no tensor")
+    _tensors(x=x, w_gate=w_gate, w_up=w_up)
     return _dense(_GATED, activation, x, w_gate, w_up, b_gate, b_up, None)
 
 
@@ -330,6 +336,7 @@ def clipped_loss(logits, actions, old_log_prob, advantages, ref_log_prob=None, m
     gives NaN.  The gradient reaches the logits alone.
     """
     rows = (old_log_prob, advantages, ref_log_prob, mask)
+    _tensors(logits=logits, actions=actions, old_log_prob=old_log_prob, advantages=advantages)
     _no_tangents(logits, *rows)
     for name, t in zip(_LossCall.NAMES, rows):
         _data(name, t)
@@ -353,6 +360,7 @@ def log_prob(logits, actions):
     logits and actions as in ``clipped_loss``.  No gradients: logits that want
     one are refused.
     """
+    _tensors(logits=logits, actions=actions)
     _no_tangents(logits)
     _data("logits", logits)
     call = _ChoiceCall(logits, actions)
