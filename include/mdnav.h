@@ -569,7 +569,7 @@ int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void*
  *     l = sum of log softmax(logits)[action],  H = sum of the heads' entropies
  *     r = exp(l - old_log_prob)
  *     L = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef K - entropy_coef H
- *     K = exp(ref_log_prob - l) - (ref_log_prob - l) - 1   (0 without ref_log_prob)
+ *     K = exp(ref_log_prob - l) - (ref_log_prob - l) - 1   (0 without ref_log_prob; out of L where kl_coef is 0)
  * and the loss is the mean of L over the steps whose mask is not 0 (all, if
  * mask is NULL); if none counts, it and its gradient are 0, and nothing of a
  * step that does not count is looked at.  A logit of -inf rules a choice out.

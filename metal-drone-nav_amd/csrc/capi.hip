@@ -2514,7 +2514,7 @@ int choice_loss_args(const char* name, const MdnChoices* c, const MdnChoiceLoss*
     if (!l) return fail(MDN_E_ARG, who + "null");
     if (a.steps && (!l->old_log_prob || !l->advantages)) return fail(MDN_E_ARG, who + "null rows");
     if (!(l->clip_low >= 0.0) || !(l->clip_high >= 0.0)) return fail(MDN_E_ARG, who + "clip_low and clip_high must be at least 0");
-    if (l->kl_coef != 0.0 && !l->ref_log_prob) return fail(MDN_E_ARG, who + "kl_coef needs ref_log_prob");
+    if (a.steps && l->kl_coef != 0.0 && !l->ref_log_prob) return fail(MDN_E_ARG, who + "kl_coef needs ref_log_prob");
     if (keep_bytes < choices::keep_floats(a) * sizeof(float) || !keep) return fail(MDN_E_ARG, who + "keep is too small");
     a.old_log_prob = l->old_log_prob; a.advantages = l->advantages; a.ref_log_prob = l->ref_log_prob; a.mask = l->mask;
     a.low = l->clip_low; a.high = l->clip_high; a.kl_coef = l->kl_coef; a.entropy_coef = l->entropy_coef;

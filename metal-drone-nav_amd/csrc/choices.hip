@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) steps_kernel(Args a) {
             if (a.ref_log_prob) {
                 const double far = double(a.ref_log_prob[step]) - l, e = expm1(far);
                 total[1] += e - far;
-                slope -= a.kl_coef * e;
+                if (a.kl_coef != 0.0) slope -= a.kl_coef * e;  // (0 leaves the term out, infinite or not)
             }
             total[2] += entropy;
             total[3] += r;
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(384) finish_kernel(Args a, uint32_t count) {
     __syncthreads();
     if (threadIdx.x == 0) {
         const double by = sums[5] > 0.0 ? 1.0 / sums[5] : 0.0;  // no step counts: all is 0
-        a.loss[0] = float((sums[0] + a.kl_coef * sums[1] - a.entropy_coef * sums[2]) * by);
+        a.loss[0] = float((sums[0] + (a.kl_coef != 0.0 ? a.kl_coef * sums[1] : 0.0) - a.entropy_coef * sums[2]) * by);
 #pragma unroll
         for (int i = 0; i < 5; i++) a.metrics[i] = float(sums[i] * by);
         a.one_over[0] = float(by);

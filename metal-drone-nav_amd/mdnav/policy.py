@@ -325,7 +325,8 @@ def clipped_loss(logits, actions, old_log_prob, advantages, ref_log_prob=None, m
     ref_log_prob: [...] float32, mask: [...] bool or uint8.  With l the sum of
     the heads' log-probabilities, H that of their entropies,
     r = exp(l - old_log_prob) and K = exp(ref_log_prob - l) -
-    (ref_log_prob - l) - 1 (0 without ref_log_prob), the loss is the mean of
+    (ref_log_prob - l) - 1 (0 without ref_log_prob, and left out of the loss
+    where kl_coef is 0), the loss is the mean of
 
         -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef K - entropy_coef H
 
