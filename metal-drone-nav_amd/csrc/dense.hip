@@ -241,12 +241,15 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     if constexpr (PIPED) {
         // A step's last place is read while the one before is multiplied, so its
         // stage is free from the barrier before the last place's products on, where
-        // the next step has landed too. From there to the same point of the next step
-        // the step STAGES later is loaded, evenly: its loads take half of that time in
-        // the memory pipe. Past the sum's end these are loads of zeros that no one
-        // reads, as the last step's reads of a next one are of what was there.
+        // the next step has landed too. The step STAGES later is loaded behind the
+        // products of half a step from there, where its loads keep the memory pipe
+        // busy, and has the other half to arrive in. (8,192 x 4,096 x 8,192 of zeros, which
+        // draw little power: a step takes 0.98 us of which the products are 0.85; with
+        // loads over a quarter of it 1.14, over three quarters 1.06.) Past the sum's end
+        // these are loads of zeros that no one reads, as the last step's reads of a
+        // next one are of what was there.
         landed<LOADS*(STAGES - 2)>();
-        constexpr int SLOTS = (KK > 2 ? KK - 1 : KK) * MULS;  // products that loads go out behind
+        constexpr int SLOTS = KK / 2 * MULS;  // products that loads go out behind
         const auto load_at = [&](auto whole_steps, int slot) {
 #pragma unroll
             for (int l = slot * LOADS / SLOTS; l < (slot + 1) * LOADS / SLOTS; l++) whole_steps() ? load(l) : load_end(l);
@@ -314,6 +317,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     // What is beside a piece, the residual or the gradient of y, is loaded while
     // the piece before it is worked on, and waits in LDS.
     const bool beside = SLOPES || (RESULT == LINEAR && a.residual.p);
+    const bool as_is = RESULT == STORE || RESULT == PART || (RESULT == LINEAR && a.act == MDN_ACT_NONE && !beside);
     const Matrix side = RESULT == LINEAR ? a.residual : a.dy;
     typename Out::LdsWord words[Out::TURNS];
     const auto load_beside = [&](int i0, int j) {
@@ -347,18 +351,37 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
                     load_beside(i0 + PT, 0);
             }
             Out::order();
+            if (as_is) {
+                float z[Out::TURNS][N];
+#pragma unroll
+                for (uint32_t t = 0; t < Out::TURNS; t++) Out::get(own, Out::row(lane, t), lane, z[t]);
+#pragma unroll
+                for (uint32_t t = 0; t < Out::TURNS; t++)
+                    if (m0 + 32 * j + Out::row(lane, t) < mc) Out::store(y, m0 + 32 * j + Out::row(lane, t), n, nc, z[t]);
+                continue;
+            }
+            // (not unrolled, the activations would fill the instruction cache; the next turn's values are read ahead)
+            float z_next[N], up_next[N];
+            Out::get(own, Out::row(lane, 0), lane, z_next);
+            if constexpr (N2) Out::get(own + Out::BYTES, Out::row(lane, 0), lane, up_next);
 #pragma unroll 1
             for (uint32_t t = 0; t < Out::TURNS; t++) {
                 const uint32_t m = m0 + 32 * j + Out::row(lane, t);
-                if (m >= mc) break;
                 float z[N], up[N], with[N];
-                Out::get(own, Out::row(lane, t), lane, z);
-                if constexpr (N2) Out::get(own + Out::BYTES, Out::row(lane, t), lane, up);
+#pragma unroll
+                for (uint32_t e = 0; e < N; e++) {
+                    z[e] = z_next[e];
+                    if constexpr (N2) up[e] = up_next[e];
+                }
+                const uint32_t ahead = t + 1 < Out::TURNS ? t + 1 : t;
+                Out::get(own, Out::row(lane, ahead), lane, z_next);
+                if constexpr (N2) Out::get(own + Out::BYTES, Out::row(lane, ahead), lane, up_next);
                 if (beside) {
                     const auto word = *reinterpret_cast<const typename Out::LdsWord*>(own + BESIDE + t * 1024 + lane * 16);
 #pragma unroll
                     for (uint32_t e = 0; e < N; e++) with[e] = float(word[e]);
                 }
+                if (m >= mc) continue;
                 if constexpr (RESULT == LINEAR) {
                     act_of<T>(a.act, z);
                     if (beside)
@@ -409,22 +432,25 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 
 // ---------------------------------------------------------------- what is left
 // Rows with words of their own: row r of `to` (ld elements, a multiple of a
-// word's) is row r of `from`, zeros behind it.
-template <class T>
-__global__ void __launch_bounds__(256) lay_out_kernel(Matrix from, Matrix to, uint64_t rows, uint32_t width) {
-    const uint32_t words = uint32_t(to.ld) / per_word<T>();
-    const uint64_t all = rows * words;
-    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += uint64_t(gridDim.x) * 256) {
-        const uint64_t row = i / words;
-        const uint32_t c = uint32_t(i - row * words) * per_word<T>();
+// word's) is row r of `from`, zeros behind it.  I: an index that all words fit.
+template <class T, class I>
+__global__ void __launch_bounds__(256) lay_out_kernel(Matrix from, Matrix to, I all, uint32_t width) {
+    constexpr uint32_t N = per_word<T>();
+    typedef T Word __attribute__((ext_vector_type(N)));
+    typedef T AnyWord __attribute__((ext_vector_type(N), aligned(sizeof(T))));  // at any multiple of an element
+    const I words = I(to.ld) / N, step = I(gridDim.x) * 256;
+    for (I i = I(blockIdx.x) * 256 + threadIdx.x; i < all; i += step) {
+        const I row = i / words;
+        const uint32_t c = uint32_t(i - row * words) * N;
         const T* src = reinterpret_cast<const T*>(from.p) + int64_t(row) * from.ld + c;
-        T v[per_word<T>()];
+        Word v;
+        if (c + N <= width) {
+            v = *reinterpret_cast<const AnyWord*>(src);
+        } else {
 #pragma unroll
-        for (uint32_t e = 0; e < per_word<T>(); e++) v[e] = c + e < width ? src[e] : T(0.0f);
-        T* dst = reinterpret_cast<T*>(to.p) + row * to.ld + c;
-#pragma unroll
-        for (uint32_t e = 0; e < per_word<T>(); e += 4)
-            *reinterpret_cast<typename Four<T>::type*>(dst + e) = typename Four<T>::type{v[e], v[e + 1], v[e + 2], v[e + 3]};
+            for (uint32_t e = 0; e < N; e++) v[e] = c + e < width ? src[e] : T(0.0f);
+        }
+        *reinterpret_cast<Word*>(reinterpret_cast<T*>(to.p) + int64_t(row) * to.ld + c) = v;
     }
 }
 
@@ -634,7 +660,11 @@ BackPlan back_plan_of(const Args& a, const GradArgs& d) {
 
 template <class T> hipError_t lay_out(const Matrix& from, const Matrix& to, uint64_t rows, uint32_t width, hipStream_t st) {
     const uint64_t words = rows * (to.ld / per_word<T>());
-    lay_out_kernel<T><<<dim3(blocks_for(words, 256, 8192)), dim3(256), 0, st>>>(from, to, rows, width);
+    const dim3 grid(blocks_for(words, 256, 16384));
+    if (words < (1ull << 31))
+        lay_out_kernel<T, uint32_t><<<grid, dim3(256), 0, st>>>(from, to, uint32_t(words), width);
+    else
+        lay_out_kernel<T, uint64_t><<<grid, dim3(256), 0, st>>>(from, to, words, width);
     return hipGetLastError();
 }
 // x and the weights in words; copies go to `work`, which is advanced.
