@@ -535,30 +535,31 @@ hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
 // The tile of a product: the one of the least estimated time.  A compute unit
 // takes one large tile at a time and two of the others; measured, in us: a step
 // of 128 bytes of k alone on a compute unit and beside another tile, and what a
-// tile takes besides (512 x 2,048 x 2,048 in bfloat16: 15, 26 and 48 us on small,
-// middle and large tiles; 32,768 x 5,120 to 1,280: 775, 506 and 405; 262,144 x 184
-// to 256: 103, 65 and 93).
+// tile takes besides (1,024 x 2,048 x 2,048 in bfloat16: 18, 27 and 51 us on small,
+// middle and large tiles; 4,096 x 2,048 x 2,048: 58, 42 and 53; 32,768 x 5,120 to 1,280:
+// 775, 506 and 404; 262,144 x 256 to 1,024 with silu: 511, 316 and 360).
 enum Tile { SMALL, MIDDLE, LARGE };
 constexpr uint32_t UNITS = 256;
 struct Cost { uint32_t m, n; float alone, beside, rest; };
-// of: bfloat16 or not, projections of a gated block beside each other or one
-Cost cost_of(Tile t, bool bf, bool two) {
+enum Kind { PLAIN, SHAPED, TWO };  // sums alone, with an epilogue, of both projections of a gated block
+Cost cost_of(Tile t, bool bf, Kind kind) {
+    const bool two = kind == TWO, plain = kind == PLAIN;
     switch (t) {
-        case SMALL: return {64, 64, (bf ? 0.38f : 0.55f) * (two ? 1.6f : 1.0f), (bf ? 0.48f : 1.02f) * (two ? 1.8f : 1.0f), bf ? (two ? 2.2f : 1.8f) : 6.0f};
-        case MIDDLE: return {128, two ? 64u : 128u, bf ? 0.72f : 2.1f, bf ? (two ? 1.05f : 1.25f) : 4.1f, bf ? (two ? 3.4f : 4.6f) : (two ? 3.0f : 9.0f)};
-        default: return {256, two ? 128u : 256u, bf ? 1.77f : 8.2f, bf ? 3.54f : 16.4f, bf ? (two ? 9.0f : 16.0f) : (two ? 9.0f : 25.0f)};
+        case SMALL: return {64, 64, (bf ? 0.40f : 0.55f) * (two ? 1.6f : 1.0f), (bf ? 0.48f : 1.02f) * (two ? 1.8f : 1.0f), bf ? (two ? 2.2f : 1.8f) : 5.0f};
+        case MIDDLE: return {128, two ? 64u : 128u, bf ? 0.72f : 2.1f, bf ? (two ? 1.05f : 1.15f) : 4.1f, bf ? (two ? 3.4f : plain ? 3.0f : 4.4f) : (two ? 2.0f : 6.0f)};
+        default: return {256, two ? 128u : 256u, bf ? 1.55f : 8.2f, bf ? 3.1f : 16.4f, bf ? (plain || two ? 9.0f : 15.0f) : (two ? 9.0f : 20.0f)};
     }
 }
-float time_of(Tile t, bool bf, bool two, uint64_t m, uint64_t n, uint64_t k, uint64_t times) {
-    const Cost c = cost_of(t, bf, two);
+float time_of(Tile t, bool bf, Kind kind, uint64_t m, uint64_t n, uint64_t k, uint64_t times) {
+    const Cost c = cost_of(t, bf, kind);
     const uint64_t tiles = (m + c.m - 1) / c.m * ((n + c.n - 1) / c.n) * times, each = (tiles + UNITS - 1) / UNITS;
     const float steps = float((k * (bf ? 2 : 4) + 127) / 128), rest = t == LARGE ? 2.0f * c.rest : c.rest;
     return float(each / 2) * (steps * c.beside + rest) + (each & 1 ? steps * c.alone + c.rest : 0.0f);
 }
-Tile tile_of(bool bf, bool two, uint64_t m, uint64_t n, uint64_t k) {
+Tile tile_of(bool bf, Kind kind, uint64_t m, uint64_t n, uint64_t k) {
     Tile best = SMALL;
     for (Tile t : {MIDDLE, LARGE})
-        if (time_of(t, bf, two, m, n, k, 1) < time_of(best, bf, two, m, n, k, 1)) best = t;
+        if (time_of(t, bf, kind, m, n, k, 1) < time_of(best, bf, kind, m, n, k, 1)) best = t;
     return best;
 }
 
@@ -566,11 +567,11 @@ template <class T, bool MC, bool NC, int RESULT>
 hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
     if (tile == LARGE) return launch<T, 256, 256, 2, 2, 128, 2, true, MC, NC, RESULT>(a, batches, st);
     if constexpr (!MC && !NC) {
-        // Where there are more than two middle tiles a compute unit, three at once with
-        // half the LDS: 262,144 rows of 256 to 1,024, gated: 424 us, and 478 with two;
-        // of 64: 220 and 267; but 1,024 of 5,120 to 5,120: 97 and 73.
+        // Where there are more than two middle tiles a compute unit and few steps, three
+        // tiles at once with half the LDS: 262,144 rows of 256 to 1,024, gated: 424 us, and
+        // 478 with two; of 64: 220 and 267; but 32,768 of 2,560 to 5,120: 2,207 and 1,743.
         const uint64_t out = two_weights(RESULT) ? 64 : 128;
-        if (tile == MIDDLE && (a.m.count + 127ull) / 128 * ((a.n.count + out - 1) / out) > 2 * UNITS)
+        if (tile == MIDDLE && a.k * sizeof(T) <= 1024 && (a.m.count + 127ull) / 128 * ((a.n.count + out - 1) / out) > 2 * UNITS)
             return launch<T, 128, 128, 2, 2, 64, 2, false, MC, NC, RESULT>(a, batches, st);
     }
     if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 128, 2, false, MC, NC, RESULT>(a, batches, st);
@@ -608,7 +609,7 @@ Plan plan_of(const Args& a) {
     p.w_copy = !in_words(a.w[0], a.in, p.size) || (a.gated && (!in_words(a.w[1], a.in, p.size) || a.w[1].ld != a.w[0].ld));
     p.x_bytes = p.x_copy ? aligned(a.rows * p.in_ld * p.size) : 0;
     p.w_bytes = p.w_copy ? aligned(uint64_t(a.out) * p.in_ld * p.size) : 0;
-    p.forward_tile = tile_of(a.bf, a.gated, a.rows, a.out, a.in);
+    p.forward_tile = tile_of(a.bf, a.gated ? TWO : SHAPED, a.rows, a.out, a.in);
     return p;
 }
 // Of the backward pass.
@@ -637,7 +638,7 @@ BackPlan back_plan_of(const Args& a, const GradArgs& d) {
     } else
         p.sum_rows = uint32_t(a.rows < 16 * SHARES ? (a.rows + 15) / 16 : SHARES);
     p.sums_bytes = db ? aligned(uint64_t(p.sum_rows) * 2 * a.out * 4) : 0;
-    p.dx_tile = tile_of(a.bf, false, a.rows, a.in, uint64_t(a.out) * pieces);
+    p.dx_tile = tile_of(a.bf, PLAIN, a.rows, a.in, uint64_t(a.out) * pieces);
     // dW has few results and a long sum, which is cut into pieces of at least 256
     // rows: as many as are worth the 4.5 TB/s at which their fp32 results are
     // written and added up.
@@ -648,7 +649,7 @@ BackPlan back_plan_of(const Args& a, const GradArgs& d) {
         const uint32_t k = uint32_t((a.rows + splits - 1) / splits + 63) / 64 * 64;
         const float parts = splits == 1 ? 0.0f : 5.0f + float(splits) * float(a.out) * float(a.in) * float(pieces) * 8.0f / 4.5e6f;
         for (Tile t : {SMALL, MIDDLE, LARGE}) {
-            const float time = time_of(t, a.bf, false, a.out, a.in, k, uint64_t(pieces) * splits) + parts;
+            const float time = time_of(t, a.bf, PLAIN, a.out, a.in, k, uint64_t(pieces) * splits) + parts;
             if (rows == 0 || time < least) least = time, rows = k, p.dw_tile = t;
         }
     }
