@@ -74,24 +74,28 @@ template <class T, int PW> struct Piece {
         }
     }
     // One word of a row, columns c .. c + N - 1 of `count`; 0 outside.
-    static __device__ __forceinline__ LdsWord load(const Matrix& from, uint32_t m, uint32_t c, uint32_t count) {
+    // ONCE: past the caches, which large tiles fill with operands.
+    template <bool ONCE> static __device__ __forceinline__ LdsWord load(const Matrix& from, uint32_t m, uint32_t c, uint32_t count) {
         const T* p = reinterpret_cast<const T*>(from.p) + int64_t(m) * from.ld + c;
         LdsWord v;
         if (c + N <= count) {
-            v = *reinterpret_cast<const Word*>(p);
+            v = ONCE ? __builtin_nontemporal_load(reinterpret_cast<const Word*>(p)) : *reinterpret_cast<const Word*>(p);
         } else {
 #pragma unroll
             for (uint32_t e = 0; e < N; e++) v[e] = c + e < count ? p[e] : T(0.0f);
         }
         return v;
     }
-    static __device__ __forceinline__ void store(const Matrix& to, uint32_t m, uint32_t c, uint32_t count, const float (&z)[N]) {
+    template <bool ONCE> static __device__ __forceinline__ void store(const Matrix& to, uint32_t m, uint32_t c, uint32_t count, const float (&z)[N]) {
         T* p = reinterpret_cast<T*>(to.p) + int64_t(m) * to.ld + c;
         if (c + N <= count) {
             Word v;
 #pragma unroll
             for (uint32_t e = 0; e < N; e++) v[e] = T(z[e]);
-            *reinterpret_cast<Word*>(p) = v;
+            if (ONCE)
+                __builtin_nontemporal_store(v, reinterpret_cast<Word*>(p));
+            else
+                *reinterpret_cast<Word*>(p) = v;
         } else {
 #pragma unroll
             for (uint32_t e = 0; e < N; e++)
@@ -308,6 +312,9 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     typedef Piece<TR, PW> Out;
     constexpr uint32_t N = Out::N;
     constexpr bool SLOPES = RESULT == SLOPE || RESULT == GATED_SLOPE;
+    // (32,768 x 2,560 to 5,120, gated: 1,387 us, and 1,458 with y by way of the caches; its
+    // slopes 1,512, and 1,635 with dy and dz by way of them.)
+    constexpr bool ONCE = BM == 256 && RESULT != STORE && RESULT != PART;
     constexpr uint32_t BESIDE = (N2 ? 2 : 1) * Out::BYTES;
     char* own = shared + wave * REGION;
     Matrix y = (RESULT == STORE || RESULT == PART) && batch ? a.y2 : a.y;
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
         for (uint32_t t = 0; t < Out::TURNS; t++) {
             const uint32_t m = m0 + 32 * j + Out::row(lane, t);
-            if (m < mc) words[t] = Out::load(side, m, n, nc);
+            if (m < mc) words[t] = Out::template load<BM == 256>(side, m, n, nc);
         }
     };
     if (beside) load_beside(0, 0);
@@ -333,6 +340,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     for (int i0 = 0; i0 < TO; i0 += PT) {
         const uint32_t n = n0 + 32 * i0 + Out::column(lane);
         float sum[SLOPES ? 2 : 1][N] = {};
+        const bool whole = n0 + 32 * i0 + PW <= nc;
 #pragma unroll
         for (int j = 0; j < TM; j++) {
             Out::order();
@@ -357,7 +365,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
                 for (uint32_t t = 0; t < Out::TURNS; t++) Out::get(own, Out::row(lane, t), lane, z[t]);
 #pragma unroll
                 for (uint32_t t = 0; t < Out::TURNS; t++)
-                    if (m0 + 32 * j + Out::row(lane, t) < mc) Out::store(y, m0 + 32 * j + Out::row(lane, t), n, nc, z[t]);
+                    if (m0 + 32 * j + Out::row(lane, t) < mc) Out::template store<ONCE>(y, m0 + 32 * j + Out::row(lane, t), n, nc, z[t]);
                 continue;
             }
             // (not unrolled, the activations would fill the instruction cache; the next turn's values are read ahead)
@@ -394,23 +402,34 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
                     for (uint32_t e = 0; e < N; e++) z[e] *= up[e];
                 }
                 if constexpr (SLOPES) {
-                    // zeros past the last column, also where z is none: the next products read whole words
                     float slope[N];
                     act_of<T>(a.act, z, slope);
 #pragma unroll
                     for (uint32_t e = 0; e < N; e++) {
                         if constexpr (N2) {
                             slope[e] *= up[e];
-                            up[e] = n + e < nc ? with[e] * z[e] : 0.0f;
-                            sum[1][e] += up[e];
+                            up[e] = with[e] * z[e];
                         }
-                        z[e] = n + e < nc ? with[e] * slope[e] : 0.0f;
-                        sum[0][e] += z[e];
+                        z[e] = with[e] * slope[e];
                     }
-                    Out::store(a.dz, m, n, a.dz_half, z);
-                    if constexpr (N2) Out::store(dz2, m, n, a.dz_half, up);
+                    if (!whole) {  // zeros past the last column, also where z is none: the next products read whole words
+#pragma unroll
+                        for (uint32_t e = 0; e < N; e++) {
+                            z[e] = n + e < nc ? z[e] : 0.0f;
+                            if constexpr (N2) up[e] = n + e < nc ? up[e] : 0.0f;
+                        }
+                    }
+                    if (a.sums) {
+#pragma unroll
+                        for (uint32_t e = 0; e < N; e++) {
+                            sum[0][e] += z[e];
+                            if constexpr (N2) sum[1][e] += up[e];
+                        }
+                    }
+                    Out::template store<ONCE>(a.dz, m, n, a.dz_half, z);
+                    if constexpr (N2) Out::template store<ONCE>(dz2, m, n, a.dz_half, up);
                 } else
-                    Out::store(y, m, n, nc, z);
+                    Out::template store<ONCE>(y, m, n, nc, z);
             }
         }
         if constexpr (SLOPES) {

@@ -78,9 +78,9 @@ template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z
         return s;
     }
     if (ACT == MDN_ACT_SILU) {
-        float other;
-        const float s = sigmoids<T>(z, other);
-        slope = s * fmaf(z, other, 1.0f);
+        // (below -80 the value and the slope are under 1e-32; z brings a NaN back)
+        const float e = exp_of<T>(fminf(-z, 80.0f)), s = __builtin_amdgcn_rcpf(1.0f + e);
+        slope = s * fmaf(z, e * s, 1.0f);
         return z * s;
     }
     if (ACT == MDN_ACT_GELU) {
