@@ -546,7 +546,7 @@ typedef struct MdnDense {
 } MdnDense;
 /* The workspace depends on sizes, strides and addresses (operands that do not
  * lie in 16-byte words are copied there): it is asked for with the struct of
- * the call. */
+ * the call.  It is 16-byte aligned. */
 int mdn_op_dense_forward_bytes(const MdnDense* dense, uint64_t* bytes);
 int mdn_op_dense_forward(const MdnDense* dense, void* workspace, uint64_t workspace_bytes, void* stream);
 
@@ -597,7 +597,8 @@ typedef struct MdnChoiceLoss {
     double clip_low, clip_high, kl_coef, entropy_coef;
     float *loss, *metrics; /* [1], and [5]: the means of -min(..), K, H, r and of r outside the clip's borders */
 } MdnChoiceLoss;
-/* Bytes of `keep`, 16-byte aligned, which the backward pass reads, and of the workspace. */
+/* Bytes of `keep`, 16-byte aligned, which the backward pass reads, and of the
+ * workspace, 8-byte aligned. */
 int mdn_op_choices_loss_sizes(const MdnChoices* choices, uint64_t* keep, uint64_t* workspace);
 int mdn_op_choices_loss_forward(const MdnChoices* choices, const MdnChoiceLoss* loss, void* keep, uint64_t keep_bytes,
                                 void* workspace, uint64_t workspace_bytes, void* stream);

@@ -2462,6 +2462,7 @@ int mdn_op_dense_forward(const MdnDense* dense, void* workspace, uint64_t worksp
     if (!a.y.p) return fail(MDN_E_ARG, "mdn_op_dense_forward: null rows");
     const uint64_t need = dense::forward_bytes(a);
     if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_dense_forward: workspace is too small");
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(MDN_E_ARG, "mdn_op_dense_forward: workspace must be 16-byte aligned");
     HIP_TRY(dense::forward(a, static_cast<char*>(workspace), static_cast<hipStream_t>(stream)));
     return MDN_OK;
 }
@@ -2482,6 +2483,7 @@ int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void*
     if (int rc = dense_grad_args("mdn_op_dense_backward", dense, grad, &a, &d)) return rc;
     const uint64_t need = a.rows ? dense::backward_bytes(a, d) : 0;
     if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_dense_backward: workspace is too small");
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(MDN_E_ARG, "mdn_op_dense_backward: workspace must be 16-byte aligned");
     HIP_TRY(dense::backward(a, d, static_cast<char*>(workspace), static_cast<hipStream_t>(stream)));
     return MDN_OK;
 }
@@ -2559,6 +2561,7 @@ int mdn_op_choices_loss_forward(const MdnChoices* choices, const MdnChoiceLoss* 
     if (!a.loss || !a.metrics) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: null results");
     const uint64_t need = uint64_t(choices::parts_of(a)) * 6 * sizeof(double);
     if (workspace_bytes < need || (need && !workspace)) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: workspace is too small");
+    if (reinterpret_cast<uintptr_t>(workspace) % 8) return fail(MDN_E_ARG, "mdn_op_choices_loss_forward: workspace must be 8-byte aligned");
     a.parts = static_cast<double*>(workspace);
     HIP_TRY(choices::launch_loss(a, static_cast<hipStream_t>(stream)));
     return MDN_OK;

@@ -280,9 +280,12 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
                 }
             }
         };
-        // as long as this step's loads and the next one's are whole
+        // the steps whose loads, of the two steps after them, are whole
+        static_assert(STAGES == 2, "");
+        const uint32_t full = (k_end - k_first) / STEP, ahead = full == steps ? total : full;
+        const uint32_t fast = ahead > 2 ? ahead - 2 : 0;
         uint32_t s = 0;
-        for (; next + 1 < total && next_k + 2 * STEP <= k_end; s++) step(std::true_type());
+        for (; s < fast; s++) step(std::true_type());
         for (; s < total; s++) step(std::false_type());
         landed<0>();
     } else {
@@ -473,6 +476,14 @@ __global__ void __launch_bounds__(256) lay_out_kernel(Matrix from, Matrix to, I 
     }
 }
 
+// Zeros in a matrix of `width` columns.
+template <class T>
+__global__ void __launch_bounds__(256) clear_kernel(Matrix to, uint64_t rows, uint32_t width) {
+    const uint64_t all = rows * width;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += uint64_t(gridDim.x) * 256)
+        reinterpret_cast<T*>(to.p)[int64_t(i / width) * to.ld + int64_t(i % width)] = T(0.0f);
+}
+
 // Adds up the parts of a product, in order: to[r][c] = sum of from[s][r][c].
 template <class T>
 __global__ void __launch_bounds__(256) add_parts_kernel(const float* from, uint32_t parts, Matrix to, uint32_t rows, uint32_t width) {
@@ -543,6 +554,7 @@ hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
     static_assert(bytes <= 160 * 1024, "");
     a.m_tiles = (a.m.count + BM - 1) / BM;
     a.n_tiles = (a.n.count + OUT - 1) / OUT;
+    if (uint64_t(a.m_tiles) * a.n_tiles > 0x7fffffffull) return hipErrorInvalidConfiguration;
     const auto kernel = product_kernel<T, BM, BN, WM, WN, KB, STAGES, PIPED, MC, NC, RESULT>;
     if (bytes > 64 * 1024)
         if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
@@ -734,7 +746,18 @@ template <class T> hipError_t add_sums(const float* sums, uint32_t count, uint64
     return hipGetLastError();
 }
 
+// The gradients of no rows.
+template <class T> hipError_t clear(const Args& a, const GradArgs& d, hipStream_t st) {
+    for (uint32_t i = 0; i < pieces_of(a); i++) {
+        if (d.d_w[i].p)
+            clear_kernel<T><<<dim3(blocks_for(uint64_t(a.out) * a.in, 256, 4096)), dim3(256), 0, st>>>(d.d_w[i], a.out, a.in);
+        if (d.d_b[i]) clear_kernel<T><<<dim3(blocks_for(a.out, 256, 4096)), dim3(256), 0, st>>>(Matrix{d.d_b[i], a.out}, 1, a.out);
+    }
+    return hipGetLastError();
+}
+
 template <class T> hipError_t backward_of(Args a, const GradArgs& d, char* work, hipStream_t st) {
+    if (a.rows == 0) return clear<T>(a, d, st);
     const BackPlan p = back_plan_of(a, d);
     const uint32_t pieces = pieces_of(a);
     if (hipError_t e = operands<T>(a, p, work, st)) return e;

@@ -302,6 +302,30 @@ def test_no_rows():
 
 
 @gpu
+def test_no_rows_through_the_c_entries():
+    """The weights' and biases' gradients are zeros, between which nothing is written."""
+    from mdnav import native, policy
+    L = native.lib()
+    v = inputs(0, 40, 30, BF16, True, seed=12)
+    c = policy._Dense.from_buffer_copy(policy._DENSE.pack(
+        0, 40, 30, 1, policy.ACTIVATIONS["silu"], 1, 0, 40, v["w"].data_ptr(), 40, v["w_up"].data_ptr(), 40, 0, 0, 0, 30, 0, 0))
+    d_w, d_up = (torch.full((31, 44), 7.0, dtype=BF16, device="cuda") for _ in range(2))
+    d_b, d_b_up = (torch.full((31,), 7.0, dtype=BF16, device="cuda") for _ in range(2))
+    d = policy._DenseGrad.from_buffer_copy(policy._DENSE_GRAD.pack(0, 30, 0, 40, d_w.data_ptr(), 44, d_up.data_ptr(), 44,
+                                                                   d_b.data_ptr(), d_b_up.data_ptr()))
+    size = ctypes.c_uint64(9)
+    stream = torch.cuda.current_stream().cuda_stream
+    native.check(L.mdn_op_dense_forward(ctypes.byref(c), None, 0, stream))
+    native.check(L.mdn_op_dense_backward_bytes(ctypes.byref(c), ctypes.byref(d), ctypes.byref(size)))
+    assert size.value == 0
+    native.check(L.mdn_op_dense_backward(ctypes.byref(c), ctypes.byref(d), None, 0, stream))
+    for t in (d_w, d_up):
+        assert not t[:30, :40].any() and (t[30:] == 7).all() and (t[:, 40:] == 7).all()
+    for t in (d_b, d_b_up):
+        assert not t[:30].any() and t[30] == 7
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_the_same_bits_every_time(dtype):
     v = inputs(20011, 200, 136, dtype, True, seed=8)
@@ -496,6 +520,7 @@ def test_the_c_entries_refuse_before_anything_runs():
     c = dense(rows=1000, in_=7)
     assert L.mdn_op_dense_forward_bytes(ctypes.byref(c), ctypes.byref(size)) == 0 and size.value >= 1000 * 8 * 4
     assert L.mdn_op_dense_forward(ctypes.byref(c), None, 0, None) == -1 and b"workspace" in L.mdn_last_error()
+    assert L.mdn_op_dense_forward(ctypes.byref(c), 4100, size.value, None) == -1 and b"aligned" in L.mdn_last_error()
     d = policy._DenseGrad()
     c = dense(rows=1000)
     assert L.mdn_op_dense_backward(ctypes.byref(c), None, None, 0, None) == -1
@@ -505,3 +530,4 @@ def test_the_c_entries_refuse_before_anything_runs():
     d.d_w_up.data, d.d_b = None, 4096
     assert L.mdn_op_dense_backward_bytes(ctypes.byref(c), ctypes.byref(d), ctypes.byref(size)) == 0 and size.value > 0
     assert L.mdn_op_dense_backward(ctypes.byref(c), ctypes.byref(d), None, 0, None) == -1 and b"workspace" in L.mdn_last_error()
+    assert L.mdn_op_dense_backward(ctypes.byref(c), ctypes.byref(d), 4100, size.value, None) == -1 and b"aligned" in L.mdn_last_error()

@@ -391,7 +391,7 @@ def test_the_c_entries_refuse_before_anything_runs():
                        ((loss(clip_low=-1.0),), b"clip"), ((loss(clip_high=float("nan")),), b"clip"), ((loss(kl_coef=0.1),), b"ref_log_prob"),
                        ((loss(), None), b"keep"), ((loss(), 4096, keep.value - 1), b"keep"), ((loss(), 4100), b"aligned"),
                        ((loss(), 4096, keep.value, None), b"workspace"), ((loss(), 4096, keep.value, 4096, work.value - 1), b"workspace"),
-                       ((loss(loss=None),), b"null results"), ((loss(metrics=None),), b"null results")]:
+                       ((loss(), 4096, keep.value, 4100, work.value), b"aligned"), ((loss(loss=None),), b"null results"), ((loss(metrics=None),), b"null results")]:
         assert forward(*args) == -1 and text in L.mdn_last_error(), (args, L.mdn_last_error())
     l = loss()
     for d_loss, d_logits in ((None, 4096), (4096, None)):
