@@ -484,10 +484,12 @@ __global__ void __launch_bounds__(256) clear_kernel(Matrix to, uint64_t rows, ui
         reinterpret_cast<T*>(to.p)[int64_t(i / width) * to.ld + int64_t(i % width)] = T(0.0f);
 }
 
-// Adds up the parts of a product, in order: to[r][c] = sum of from[s][r][c].
+// Adds up the parts of a product, in order: to[r][c] = sum of from[s][r][c]; blockIdx.y: of which of two products.
 template <class T>
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* from, uint32_t parts, Matrix to, uint32_t rows, uint32_t width) {
+__global__ void __launch_bounds__(256) add_parts_kernel(const float* from, uint32_t parts, Matrix to0, Matrix to1, uint32_t rows, uint32_t width) {
+    const Matrix to = blockIdx.y ? to1 : to0;
     const uint64_t all = uint64_t(rows) * width;
+    from += blockIdx.y * parts * all;
     for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += uint64_t(gridDim.x) * 256) {
         float v = 0.0f;
         for (uint32_t s = 0; s < parts; s++) v += from[s * all + i];
@@ -517,10 +519,14 @@ __global__ void __launch_bounds__(256) column_sums_kernel(Matrix from, uint64_t 
     if (slice == 0 && c < width)
         sums[uint64_t(blockIdx.y) * width + c] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
 }
-// Rows of sums, `pitch` apart, to a vector: 64 columns a workgroup, a sixteenth of the rows a wavefront.
+// Rows of sums, `pitch` apart, to one vector or two (blockIdx.y; null: none): 64 columns a workgroup, a sixteenth of the
+// rows a wavefront.
 template <class T>
-__global__ void __launch_bounds__(1024) add_sums_kernel(const float* sums, uint32_t count, uint64_t pitch, uint32_t width, char* to) {
+__global__ void __launch_bounds__(1024) add_sums_kernel(const float* sums, uint32_t count, uint64_t pitch, uint32_t width, char* to0, char* to1) {
     __shared__ float part[16][64];
+    char* to = blockIdx.y ? to1 : to0;
+    if (!to) return;
+    sums += blockIdx.y * width;
     const uint32_t c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (c < width) {
@@ -741,8 +747,8 @@ template <class T> hipError_t forward_of(Args a, char* work, hipStream_t st) {
     return a.gated ? product<T, false, false, GATED>(j, p.forward_tile, 1, st) : product<T, false, false, LINEAR>(j, p.forward_tile, 1, st);
 }
 
-template <class T> hipError_t add_sums(const float* sums, uint32_t count, uint64_t pitch, uint32_t width, char* to, hipStream_t st) {
-    add_sums_kernel<T><<<dim3((width + 63) / 64), dim3(1024), 0, st>>>(sums, count, pitch, width, to);
+template <class T> hipError_t add_sums(const float* sums, uint32_t count, uint64_t pitch, uint32_t width, char* const (&to)[2], hipStream_t st) {
+    add_sums_kernel<T><<<dim3((width + 63) / 64, to[1] ? 2 : 1), dim3(1024), 0, st>>>(sums, count, pitch, width, to[0], to[1]);
     return hipGetLastError();
 }
 
@@ -777,9 +783,8 @@ template <class T> hipError_t backward_of(Args a, const GradArgs& d, char* work,
         if (hipError_t e = a.gated ? product<T, false, false, GATED_SLOPE>(j, p.forward_tile, 1, st)
                                    : product<T, false, false, SLOPE>(j, p.forward_tile, 1, st))
             return e;
-        for (uint32_t i = 0; i < pieces; i++)
-            if (d.d_b[i])
-                if (hipError_t e = add_sums<T>(sums + i * a.out, p.sum_rows, 2 * uint64_t(a.out), a.out, d.d_b[i], st)) return e;
+        if (sums)
+            if (hipError_t e = add_sums<T>(sums, p.sum_rows, 2 * uint64_t(a.out), a.out, d.d_b, st)) return e;
     } else {
         if (p.dz_copy)
             if (hipError_t e = lay_out<T>(d.d_y, dz, a.rows, a.out, st)) return e;
@@ -787,7 +792,7 @@ template <class T> hipError_t backward_of(Args a, const GradArgs& d, char* work,
             const uint64_t share = (a.rows + p.sum_rows - 1) / p.sum_rows;
             column_sums_kernel<T><<<dim3((a.out + 63) / 64, p.sum_rows), dim3(256), 0, st>>>(d.d_y, a.rows, a.out, share, sums);
             if (hipError_t e = hipGetLastError()) return e;
-            if (hipError_t e = add_sums<T>(sums, p.sum_rows, a.out, a.out, d.d_b[0], st)) return e;
+            if (hipError_t e = add_sums<T>(sums, p.sum_rows, a.out, a.out, d.d_b, st)) return e;
         }
     }
     const char* dz2 = dz.p + uint64_t(p.out_ld) * p.size;
@@ -820,11 +825,9 @@ template <class T> hipError_t backward_of(Args a, const GradArgs& d, char* work,
         j.y = Matrix{reinterpret_cast<char*>(parts), a.in};
         j.y2 = Matrix{reinterpret_cast<char*>(parts + p.splits * all), a.in};
         if (hipError_t e = product<T, true, true, PART>(j, p.dw_tile, both ? 2 : 1, st)) return e;
-        for (uint32_t i = 0; i < (both ? 2u : 1u); i++) {
-            add_parts_kernel<T><<<dim3(blocks_for(all, 256, 4096)), dim3(256), 0, st>>>(parts + i * p.splits * all, p.splits,
-                                                                                        d.d_w[first + i], a.out, a.in);
-            if (hipError_t e = hipGetLastError()) return e;
-        }
+        add_parts_kernel<T><<<dim3(blocks_for(all, 256, 4096), both ? 2 : 1), dim3(256), 0, st>>>(parts, p.splits, d.d_w[first], d.d_w[1],
+                                                                                                  a.out, a.in);
+        return hipGetLastError();
     }
     return hipSuccess;
 }
