@@ -526,7 +526,7 @@ int mdn_op_block_norm_workspace_bytes(const MdnBlockNorm* norm, uint64_t* bytes)
  * with weights [out][in].  Every array has dtype; sums are fp32 and a result
  * is rounded once (fp32 rows are multiplied in fp32).  An MdnMatrix names rows
  * `row` elements apart (0 broadcasts an input) with contiguous columns.
- * in and out are 1..65,536, rows below 2^31 and may be 0. */
+ * in and out are 1..65,536, rows 0..0x7fffff00. */
 typedef struct MdnMatrix {
     void* data;
     int64_t row;

@@ -17,7 +17,6 @@
 
 #include "dense_act.h"
 #include "dense_tiles.h"
-#include "lane_sums.h"
 
 #include <type_traits>
 
@@ -551,6 +550,8 @@ uint32_t blocks_for(uint64_t items, uint32_t per, uint32_t most) {
     return uint32_t(n < most ? (n ? n : 1) : most);
 }
 
+constexpr uint64_t MOST_TILES = 0xffffffffull / 256;  // a launch has below 2^32 threads
+
 template <class T, int BM, int BN, int WM, int WN, int KB, int STAGES, bool PIPED, bool MC, bool NC, int RESULT>
 hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
     constexpr bool N2 = two_weights(RESULT);
@@ -560,7 +561,7 @@ hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
     static_assert(bytes <= 160 * 1024, "");
     a.m_tiles = (a.m.count + BM - 1) / BM;
     a.n_tiles = (a.n.count + OUT - 1) / OUT;
-    if (uint64_t(a.m_tiles) * a.n_tiles > 0x7fffffffull) return hipErrorInvalidConfiguration;
+    if (uint64_t(a.m_tiles) * a.n_tiles > MOST_TILES) return hipErrorInvalidConfiguration;
     const auto kernel = product_kernel<T, BM, BN, WM, WN, KB, STAGES, PIPED, MC, NC, RESULT>;
     if (bytes > 64 * 1024)
         if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
@@ -590,6 +591,7 @@ Cost cost_of(Tile t, bool bf, Kind kind) {
 float time_of(Tile t, bool bf, Kind kind, uint64_t m, uint64_t n, uint64_t k, uint64_t times) {
     const Cost c = cost_of(t, bf, kind);
     const uint64_t tiles = (m + c.m - 1) / c.m * ((n + c.n - 1) / c.n) * times, each = (tiles + UNITS - 1) / UNITS;
+    if (tiles > MOST_TILES) return 1e30f;
     const float steps = float((k * (bf ? 2 : 4) + 127) / 128), rest = t == LARGE ? 2.0f * c.rest : c.rest;
     return float(each / 2) * (steps * c.beside + rest) + (each & 1 ? steps * c.alone + c.rest : 0.0f);
 }
@@ -624,8 +626,8 @@ uint64_t aligned(uint64_t bytes) { return (bytes + ALIGN - 1) / ALIGN * ALIGN; }
 
 // A matrix whose rows move in 16-byte words as they are.
 bool in_words(const Matrix& m, uint32_t width, uint32_t size) {
-    return width % (16 / size) == 0 && (m.ld * size) % 16 == 0 && reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld >= 0 &&
-           m.ld * size <= (1 << 22);
+    return width % (16 / size) == 0 && m.ld >= 0 && m.ld <= int64_t((1u << 22) / size) && (m.ld * size) % 16 == 0 &&
+           reinterpret_cast<uintptr_t>(m.p) % 16 == 0;
 }
 uint32_t pieces_of(const Args& a) { return a.gated ? 2 : 1; }
 uint32_t words_of(uint32_t width, uint32_t size) { return (width + 16 / size - 1) / (16 / size) * (16 / size); }

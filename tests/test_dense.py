@@ -358,6 +358,18 @@ def test_rows_past_four_gigabytes():
 
 
 @gpu
+def test_more_rows_than_a_launch_has_small_tiles():
+    """2^30 rows, all the same one: 2^24 tiles of 64 rows would be 2^32 threads."""
+    from mdnav import policy
+    v = inputs(64, 8, 64, BF16, False, seed=14)
+    y = policy.linear(v["x"][:1].expand(1 << 30, 8), v["w"], v["b"], "silu")
+    want = policy.linear(v["x"], v["w"], v["b"], "silu")[:1]
+    for at in (0, (1 << 29) - 500, (1 << 30) - 1000):
+        # sums of 8 in another order, at most one step of the result
+        torch.testing.assert_close(y[at:at + 1000].float(), want.expand(1000, 64).float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+@gpu
 @pytest.mark.parametrize("rows", [20, 500])
 def test_only_the_results_are_written(rows):
     """Results with rows apart, through the C entries: what lies between stays."""

@@ -324,6 +324,21 @@ def test_rows_past_four_gigabytes():
         assert torch.equal(a, b)
 
 
+@gpu
+def test_a_long_row_of_equal_shares():
+    """Equal terms round alike in a long sum: 2^-24 for each of a lane's 16 additions, 245 times one of these sums and 10
+    joins, 5 more for the exponential and its argument, and half a step of the result, at 15."""
+    z = torch.zeros(2, 1, 2000003, device="cuda")
+    z[:, 0, 1234567] = 0.2
+    actions = torch.tensor([[1234567], [2000002]], device="cuda")
+    from mdnav import policy
+    l, entropy = policy.log_prob(z, actions)
+    want = torch.log_softmax(z.double(), -1)
+    room = 276 * U + 2.0 ** -21
+    assert (l - want.gather(-1, actions[..., None])[:, 0, 0]).abs().max() < room
+    assert (entropy + (want.exp() * want).sum(-1)[:, 0]).abs().max() < 2 * room
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals(monkeypatch):
     import torch.autograd.forward_ad as forward_ad
