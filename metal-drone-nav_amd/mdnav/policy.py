@@ -80,6 +80,25 @@ def _matrix(t):
     return t, (t.data_ptr(), t.shape[-1] if row is None else row)
 
 
+class _Kept:
+    """A call for its gradient: the structs with the addresses of what autograd saves, and none of the tensors.  (Checking
+    them anew takes 15 of the 120 us that a small loss and its gradient do.)"""
+
+    def __init__(self, call, saved):
+        self.call = call if all([t is None or t.is_contiguous() for t in saved]) else None
+        self.at = [None if t is None else (t.data_ptr(), t.shape) for t in saved]
+        call.drop()
+
+    def again(self, saved):
+        """The call, if what was saved is as it was, or None: a hook or an assignment to .data may have changed it."""
+        if self.call is None:
+            return None
+        for t, at in zip(saved, self.at):
+            if t is not None and (t.data_ptr() != at[0] or t.shape != at[1] or not t.is_contiguous()):
+                return None
+        return self.call
+
+
 class _DenseCall:
     """Checked arguments of one call of a linear layer or a gated block: the C struct and what it points to."""
 
@@ -129,12 +148,14 @@ class _DenseCall:
         check(L.mdn_op_dense_forward(ctypes.byref(c), _address(work), size.value, _stream(self.device)))
         return y
 
-    def backward(self, d_y, want):
+    def drop(self):
+        self.x = self.w = self.w_up = self.b = self.b_up = self.residual = None
+
+    def backward(self, d_y, inputs, want):
         """(d_x, d_w, d_w_up, d_b, d_b_up), None where `want` is false"""
         L = _library()
         d_y, my = _matrix(d_y)
-        made = [_like(t) if wanted and t is not None else None
-                for wanted, t in zip(want, (self.x, self.w, self.w_up, self.b, self.b_up))]
+        made = [_like(t) if wanted and t is not None else None for wanted, t in zip(want, inputs)]
         if self.rows == 0:
             return [None if t is None else t.zero_() for t in made]
         at = [(0 if t is None else t.data_ptr(), 0 if t is None else t.shape[-1]) for t in made]
@@ -151,9 +172,11 @@ class _DenseFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, names, activation, x, w, w_up, b, b_up, residual):
         call = _DenseCall(names, x, w, w_up, b, b_up, residual, activation)
-        ctx.names, ctx.activation, ctx.like = names, activation, residual is not None
-        ctx.save_for_backward(x, w, w_up, b, b_up)
-        return _on(call.device, call.forward)
+        y = _on(call.device, call.forward)
+        saved = (x, w, w_up, b, b_up)
+        ctx.names, ctx.activation, ctx.like, ctx.kept = names, activation, residual is not None, _Kept(call, saved)
+        ctx.save_for_backward(*saved)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -162,8 +185,9 @@ class _DenseFunction(torch.autograd.Function):
         d_residual = d_y if ctx.like and want[7] else None
         if not any(want[2:7]):
             return (*[None] * 7, d_residual)
-        call = _DenseCall(ctx.names, *ctx.saved_tensors, None, ctx.activation)
-        grads = _on(call.device, call.backward, d_y, want[2:7])
+        saved = ctx.saved_tensors
+        call = ctx.kept.again(saved) or _DenseCall(ctx.names, *saved, None, ctx.activation)
+        grads = _on(call.device, call.backward, d_y, saved, want[2:7])
         return (None, None, *grads, d_residual)
 
 
@@ -228,15 +252,19 @@ class _ChoiceCall:
         if actions.dtype not in (torch.int64, torch.int32):
             raise TypeError("actions are %s: int64 or int32 are taken" % actions.dtype)
         self.steps = logits.numel() // (heads * choices)
-        rows = _wide(logits)
-        try:
-            rows = rows.view(self.steps, heads, choices)
-        except RuntimeError:
-            rows = rows.contiguous().view(self.steps, heads, choices)
+        if logits.is_contiguous():
+            rows, strides = logits, (heads * choices, choices)
+        else:
+            rows = _wide(logits)
+            try:
+                rows = rows.view(self.steps, heads, choices)
+            except RuntimeError:
+                rows = rows.contiguous().view(self.steps, heads, choices)
+            strides = rows.stride()[:2]
         self.logits, self.actions = rows, actions.contiguous()
         self.c = _Choices.from_buffer_copy(_CHOICES.pack(
-            self.steps, heads, choices, _DTYPES[logits.dtype], self.actions.element_size(), rows.data_ptr(),
-            rows.stride(0), rows.stride(1), self.actions.data_ptr()))
+            self.steps, heads, choices, _DTYPES[logits.dtype], self.actions.element_size(), rows.data_ptr(), *strides,
+            self.actions.data_ptr()))
 
     def results(self, *shape):
         return torch.empty(shape, dtype=torch.float32, device=self.device)
@@ -280,8 +308,11 @@ class _LossCall(_ChoiceCall):
                                             _address(buffer), work.value, _stream(self.device)))
         return loss, metrics, kept
 
-    def backward(self, kept, d_loss, shape):
-        made = torch.empty(shape, dtype=self.logits.dtype, device=self.device)
+    def drop(self):
+        self.logits = self.actions = self.rows = None
+
+    def backward(self, kept, d_loss, logits):
+        made = _like(logits)
         check(_library().mdn_op_choices_loss_backward(
             ctypes.byref(self.c), ctypes.byref(self.l), _address(kept), kept.numel(), d_loss.data_ptr(), made.data_ptr(),
             _stream(self.device)))
@@ -293,8 +324,9 @@ class _LossFunction(torch.autograd.Function):
     def forward(ctx, logits, actions, old_log_prob, advantages, ref_log_prob, mask, *numbers):
         call = _LossCall(logits, actions, old_log_prob, advantages, ref_log_prob, mask, *numbers)
         loss, metrics, kept = _on(call.device, call.forward)
-        ctx.numbers = numbers
-        ctx.save_for_backward(logits, actions, old_log_prob, advantages, ref_log_prob, mask, kept)
+        saved = (logits, actions, old_log_prob, advantages, ref_log_prob, mask)
+        ctx.numbers, ctx.kept = numbers, _Kept(call, saved)
+        ctx.save_for_backward(*saved, kept)
         ctx.mark_non_differentiable(metrics)
         ctx.set_materialize_grads(False)
         return loss, metrics
@@ -305,8 +337,8 @@ class _LossFunction(torch.autograd.Function):
         if d_loss is None:
             return (None,) * 10
         *rows, kept = ctx.saved_tensors
-        call = _LossCall(*rows, *ctx.numbers)
-        return (_on(call.device, call.backward, kept, d_loss.contiguous(), rows[0].shape), *[None] * 9)
+        call = ctx.kept.again(rows) or _LossCall(*rows, *ctx.numbers)
+        return (_on(call.device, call.backward, kept, d_loss.contiguous(), rows[0]), *[None] * 9)
 
 
 def _data(name, x):

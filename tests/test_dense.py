@@ -358,6 +358,28 @@ def test_rows_past_four_gigabytes():
 
 
 @gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_what_was_saved_may_move(gated):
+    """Saved tensors that a hook brings back elsewhere, or as a view of more, give the same gradients; so does a weight
+    whose memory is another by then."""
+    v = inputs(300, 40, 48, BF16, gated, seed=15)
+    names = [n for n in LEAVES if v[n] is not None]
+    leaves = {n: v[n].clone().requires_grad_() for n in names}
+    want = torch.autograd.grad(call(dict(v, **leaves), "silu"), list(leaves.values()), v["d_y"])
+    for back in (lambda t: t.clone(), lambda t: torch.cat((t, t), -1)[..., :t.shape[-1]]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: back(t.cuda())):
+            y = call(dict(v, **leaves), "silu")
+        for a, b in zip(torch.autograd.grad(y, list(leaves.values()), v["d_y"]), want):
+            assert torch.equal(a, b)
+    y = call(dict(v, **leaves), "silu")
+    old = leaves["w"].data
+    leaves["w"].data = old.clone()
+    old.fill_(math.nan)
+    for a, b in zip(torch.autograd.grad(y, list(leaves.values()), v["d_y"]), want):
+        assert torch.equal(a, b)
+
+
+@gpu
 def test_more_rows_than_a_launch_has_small_tiles():
     """2^30 rows, all the same one: 2^24 tiles of 64 rows would be 2^32 threads."""
     from mdnav import policy

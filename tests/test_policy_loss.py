@@ -325,6 +325,20 @@ def test_rows_past_four_gigabytes():
 
 
 @gpu
+def test_what_was_saved_may_move():
+    """Saved tensors that a hook brings back elsewhere, or as a view of more, give the same gradient."""
+    x = inputs(300, 2, 40, BF16, seed=15)
+    loss, want = run(x, **NUMBERS)[0], run(x, **NUMBERS)[-1]
+    from mdnav import policy
+    for back in (lambda t: t.clone(), lambda t: torch.cat((t, t), -1)[..., :t.shape[-1]]):
+        z = x["logits"].clone().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: back(t.cuda())):
+            got = policy.clipped_loss(**dict(x, logits=z), **NUMBERS)[0]
+        (g,) = torch.autograd.grad(got, z)
+        assert torch.equal(got, loss) and torch.equal(g, want)
+
+
+@gpu
 def test_a_long_row_of_equal_shares():
     """Equal terms round alike in a long sum: 2^-24 for each of a lane's 16 additions, 245 times one of these sums and 10
     joins, 5 more for the exponential and its argument, and half a step of the result, at 15."""
