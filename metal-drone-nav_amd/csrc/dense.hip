@@ -15,11 +15,12 @@
 // kernel adds up in order: no atomics, the same bits every time.
 //
 // Bound: long sums by the matrix cores and the power that they may draw (8,192^3 in
-// bfloat16 runs at 1,180 to 1,370 TFLOP/s on the cards seen, 0.93 of a plain
+// bfloat16 runs at 1,180 to 1,370 TFLOP/s on the cards seen, 0.92 of a plain
 // library product beside it; 4,096^3 in fp32 at 128 to 144, 0.96 of it). Short ones
-// by LDS, which a 128 x 128 tile's reads keep as busy as the matrix cores, and by
-// what leaves: 262,144 rows of 256 to 1,024, gated, take 400 us and 215 with 64 in
-// place of 256; a copy writes those results in 105.
+// by what a tile does besides its products: 262,144 rows of 256 to 1,024, gated, take
+// 400 us, and 215 with 64 in place of 256, whose results a copy writes in 105. (Results
+// straight from registers, twice as long pieces of rows and four workgroups a compute
+// unit in place of three each took at most 4 % off, or added as much.)
 #include "dense.h"
 
 #include "dense_act.h"
