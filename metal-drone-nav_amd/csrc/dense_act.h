@@ -78,10 +78,11 @@ template <class T, uint32_t ACT> __device__ __forceinline__ float act_of(float z
         return s;
     }
     if (ACT == MDN_ACT_SILU) {
-        // (below -80 the value and the slope are under 1e-32; z brings a NaN back)
-        const float e = exp_of<T>(fminf(-z, 80.0f)), s = __builtin_amdgcn_rcpf(1.0f + e);
-        slope = s * fmaf(z, e * s, 1.0f);
-        return z * s;
+        // e s must not be inf times 0: below -87, where 1 / e^87 is still a normal number, value and slope stay those of
+        // -87, under 1.5e-36 and next to the 0 that they go to (the comparison lets a NaN through)
+        const float c = z < -87.0f ? -87.0f : z, e = exp_of<T>(-c), s = __builtin_amdgcn_rcpf(1.0f + e);
+        slope = s * fmaf(c, e * s, 1.0f);
+        return c * s;
     }
     if (ACT == MDN_ACT_GELU) {
         float e;
