@@ -6,8 +6,9 @@ log-probabilities that acting stores for that loss (``log_prob``).
 
 They go with ``sequence``, whose ``block_norm`` has the norms around such a
 block, and follow its rules: device tensors as they are, on torch's current
-stream; a lazily negated view is to be resolved before; torch is imported
-before the library is first used.
+stream; an argument that is a lazily negated view is to be resolved before (a
+gradient that arrives as one is resolved here); torch is imported before the
+library is first used.
 """
 import ctypes
 import struct
@@ -154,7 +155,7 @@ class _DenseCall:
     def backward(self, d_y, inputs, want):
         """(d_x, d_w, d_w_up, d_b, d_b_up), None where `want` is false"""
         L = _library()
-        d_y, my = _matrix(d_y)
+        d_y, my = _matrix(d_y.resolve_neg())
         made = [_like(t) if wanted and t is not None else None for wanted, t in zip(want, inputs)]
         if self.rows == 0:
             return [None if t is None else t.zero_() for t in made]
@@ -338,7 +339,7 @@ class _LossFunction(torch.autograd.Function):
             return (None,) * 10
         *rows, kept = ctx.saved_tensors
         call = ctx.kept.again(rows) or _LossCall(*rows, *ctx.numbers)
-        return (_on(call.device, call.backward, kept, d_loss.contiguous(), rows[0]), *[None] * 9)
+        return (_on(call.device, call.backward, kept, d_loss.resolve_neg().contiguous(), rows[0]), *[None] * 9)
 
 
 def _data(name, x):
