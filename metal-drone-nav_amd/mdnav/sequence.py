@@ -7,8 +7,9 @@ Unlike ``ops``, which copies numpy arrays to the device and back, these take
 device tensors as they are, run on torch's current stream and return device
 tensors.  Rows are time-major, [ticks][envs][heads][width], as the rollout
 buffers are; any strides go as long as the width is contiguous, so
-``x.transpose(0, 1)`` of batch-first rows needs no copy.  A lazily negated view
-(``is_neg()``, of a conjugate's imaginary part) is to be resolved before.
+``x.transpose(0, 1)`` of batch-first rows needs no copy.  An argument that is a
+lazily negated view (``is_neg()``, of a conjugate's imaginary part) is to be
+resolved before; a gradient that arrives as one is resolved here.
 
 torch is imported here and nowhere else in the package, and it has to be
 imported before the library is first used: both need the same HIP runtime in
@@ -281,8 +282,8 @@ class _DeltaRuleFunction(torch.autograd.Function):
         if d_o is None and d_last is None:
             return (None,) * 9
         q, k, v, g, beta, state, reset, kept = ctx.saved_tensors
-        d_o = torch.zeros_like(v) if d_o is None else _wide(d_o)
-        d_last = None if d_last is None else d_last.contiguous()
+        d_o = torch.zeros_like(v) if d_o is None else _wide(d_o.resolve_neg())
+        d_last = None if d_last is None else d_last.resolve_neg().contiguous()
         want_state = state is not None and ctx.needs_input_grad[5]
         if q.shape[0] == 0:  # nothing happens to the state
             d_state = None if not want_state else torch.zeros_like(state) if d_last is None else d_last
@@ -474,6 +475,7 @@ class _BlockNormFunction(torch.autograd.Function):
     def backward(ctx, d_s, d_h):
         if d_s is None and d_h is None:
             return (None,) * 7
+        d_s, d_h = (None if d is None else d.resolve_neg() for d in (d_s, d_h))
         x, y, w_post, w_pre, gate, residual_scale, stats = ctx.saved_tensors
         call = _NormCall(x, y, w_post, w_pre, gate, residual_scale, ctx.eps)
         return (*_on(call.device, call.backward, stats, d_s, d_h), None)

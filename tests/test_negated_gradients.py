@@ -97,3 +97,60 @@ def test_policy_gradients():
     for d_loss in (negated(torch.tensor(3.0, device="cuda")), torch.tensor(3.0, device="cuda")):
         grads.append(torch.autograd.grad(policy.clipped_loss(logits, *data)[0], logits, d_loss)[0])
     assert grads[0].any() and torch.equal(*grads)
+
+
+class _Sequence(_Library):
+    def mdn_op_delta_rule_sizes(self, rule, sizes):
+        sizes._obj.keep = 16
+        return 0
+
+    def mdn_op_delta_rule_backward(self, rule, grad, *_):
+        r, d_o = rule._obj, grad._obj.d_o
+        self.seen.append([[floats(d_o.data + 4 * (t * d_o.tick + n * d_o.env), r.v_dim) for n in range(r.envs)] for t in range(r.ticks)])
+        self.seen.append(floats(grad._obj.d_state_out, r.envs * r.k_dim * r.v_dim))
+        return 0
+
+    def mdn_op_block_norm_backward(self, norm, grad, *_):
+        for m in (grad._obj.d_s, grad._obj.d_h):
+            self.seen.append([floats(m.data + 4 * m.inner * i, norm._obj.width) for i in range(norm._obj.rows)])
+        return 0
+
+
+@pytest.mark.parametrize("width", [1, 4])
+def test_a_memory_and_norms_see_the_values(monkeypatch, width):
+    from mdnav import sequence
+    library = _Sequence()
+    monkeypatch.setattr(sequence, "_device", lambda names, tensors: torch.device("cpu"))
+    monkeypatch.setattr(sequence, "_on", lambda device, f, *args: f(*args))
+    monkeypatch.setattr(sequence, "_stream", lambda device: None)
+    monkeypatch.setattr(sequence, "_library", library)
+    q, k, gate = torch.randn(3, 2, 1, 5), torch.randn(3, 2, 1, 5), torch.rand(3, 2, 1)
+    v = torch.randn(3, 2, 1, width, requires_grad=True)
+    d_o, d_last = torch.randn(3, 2, 1, width), torch.randn(2, 1, 5, width)
+    out = sequence.delta_rule(q, k, v, -gate, gate, final_state=True)
+    torch.autograd.grad(out, v, [negated(d_o), negated(d_last)])
+    assert library.seen == [d_o[:, :, 0].tolist(), d_last.flatten().tolist()]
+    library.seen.clear()
+    x, w, d_s, d_h = torch.randn(6, width, requires_grad=True), torch.ones(width), torch.randn(6, width), torch.randn(6, width)
+    torch.autograd.grad(sequence.block_norm(x, torch.randn(6, width), w, w), x, [negated(d_s), negated(d_h)])
+    assert library.seen == [d_s.tolist(), d_h.tolist()]
+
+
+@gpu
+@pytest.mark.parametrize("width", [1, 16])
+def test_sequence_gradients(width):
+    """The bits of gradients without the flag."""
+    from mdnav import sequence
+    gen = torch.Generator().manual_seed(2)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=gen).cuda()
+
+    q, k, gate = 0.3 * randn(40, 3, 1, 16), 0.3 * randn(40, 3, 1, 16), torch.sigmoid(randn(40, 3, 1))
+    v, d_o, d_last = randn(40, 3, 1, width).requires_grad_(), randn(40, 3, 1, width), randn(3, 1, 16, width)
+    grads = [torch.autograd.grad(sequence.delta_rule(q, k, v, -gate, gate, final_state=True), v, d)[0]
+             for d in ([negated(d_o), negated(d_last)], [d_o, d_last])]
+    assert grads[0].any() and torch.equal(*grads)
+    x, y, w, d_s, d_h = randn(30, width).requires_grad_(), randn(30, width).requires_grad_(), randn(width), randn(30, width), randn(30, width)
+    for a, b in zip(*[torch.autograd.grad(sequence.block_norm(x, y, w, w), [x, y], d) for d in ([negated(d_s), negated(d_h)], [d_s, d_h])]):
+        assert torch.equal(a, b)
