@@ -28,19 +28,20 @@ template <class T> __device__ __forceinline__ float tanh_of(float z) {
 }
 constexpr float C_TANH = 1.5957691216f;  // 2 sqrt(2 / pi)
 
-// Phi(z) of the normal distribution, and exp(-z^2 / 2).  For bfloat16 the
-// approximation 7.1.26 of Abramowitz and Stegun's handbook, whose tail is good to
-// 2^-9 of its value down to z = -5 (and 2^-7 to -7), in place of erfc: 262,144 x 1,024
-// to 1,024 takes 1,103 us, and 1,445 with erfc; silu takes 4 to 5 % less.
+// Phi(z) of the normal distribution, and exp(-z^2 / 2).  For bfloat16 exp(z^2 / 2) Phi(-|z|) is a polynomial in
+// t = 1 / (1 + 0.29 |z|), fitted for the least error that is at most 2^-13 of its value to z = -13, where the numbers end,
+// and of Phi 2e-7, in place of erfc: 262,144 x 1,024 to 1,024 takes 688 us, and 1,029 with erfc (gated: 1,132 and 1,356);
+// silu takes 11 % less (8).
 template <class T> __device__ __forceinline__ float normal(float z, float& e) {
     e = exp_of<T>(-0.5f * z * z);
     if (sizeof(T) == 4) return 0.5f * erfcf(-0.70710678f * z);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.0f));
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    q *= 0.5f * t * e;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.28991377f, fabsf(z), 1.0f));
+    float q = fmaf(-0.08933758f, t, 0.28708297f);
+    q = fmaf(q, t, -0.09619254f);
+    q = fmaf(q, t, 0.1814572f);
+    q = fmaf(q, t, 0.10008496f);
+    q = fmaf(q, t, 0.116905004f);
+    q *= t * e;
     return z < 0.0f ? q : 1.0f - q;
 }
 

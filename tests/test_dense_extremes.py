@@ -41,3 +41,25 @@ def test_far_from_zero(act, rows, dtype):
         err = (got.detach().double() - want).abs()
         print("  %s: %s" % (name, (err / allowed(want, dtype)).max().item()), flush=True)
         assert (err <= allowed(want, dtype)).all(), (name, got, want)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [30, 480])
+def test_the_tail_of_gelu(rows):
+    """Every bfloat16 number from -1 to -13, where z Phi(z) ends: half a step of the result, 2^-8, 2^-13 for the
+    approximation of Phi / exp(-z^2 / 2), and 4 u 90 for the exponential's argument and the rest.  The slope
+    Phi + z phi passes 0: the same of its parts."""
+    z = torch.arange(0xBF80, 0xBF80 + 467).to(torch.int16).view(BF16)
+    z = torch.cat((z, torch.full((13,), -2.0, dtype=BF16))).reshape(30, 16).repeat(rows // 30, 1)
+    assert z.min() < -13 and z.max() == -1 and (z == -1).any()
+    print("case: gelu's tail", rows, flush=True)
+    x = z.cuda().requires_grad_()
+    y = call(dict(x=x, w=torch.eye(16, dtype=BF16).cuda()), "gelu")
+    slope, = torch.autograd.grad(y, x, torch.ones_like(y))
+    at = x.detach().double()
+    share, density = 0.5 * torch.erfc(-at / 2 ** 0.5), torch.exp(-at * at / 2) / (2 * torch.pi) ** 0.5
+    room = 2.0 ** -8 + 2.0 ** -13 + 4 * 90 * U
+    for name, got, want, size in (("value", y, at * share, (at * share).abs()), ("slope", slope, share + at * density, share + (at * density).abs())):
+        err = (got.detach().double() - want).abs() / size
+        print("  %s: %.2e of %.2e" % (name, err.max(), room), flush=True)
+        assert (err <= room).all(), name
