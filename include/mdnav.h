@@ -563,6 +563,17 @@ int mdn_op_dense_backward_bytes(const MdnDense* dense, const MdnDenseGrad* grad,
 int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void* workspace, uint64_t workspace_bytes,
                           void* stream);
 
+/* Test support: how a call's products are cut, decided on the host from its
+ * sizes: tiles[0] of the forward pass, [1] of the gradient of the activation's
+ * argument, [2] of d_x and [3] of the weights' gradients (grad NULL: the first
+ * alone).  rows: 64, 128 or 256, those of a tile of the result; 0 where no such
+ * product is made, and in the forward pass where few rows have a kernel of
+ * their own.  step: the bytes of k that a step takes; parts: pieces of the sum. */
+typedef struct MdnDenseTile {
+    uint32_t rows, step, parts;
+} MdnDenseTile;
+int mdn_op_dense_tiles(const MdnDense* dense, const MdnDenseGrad* grad, MdnDenseTile* tiles);
+
 /* The clipped loss of a policy over discrete choices.  A step has `heads`
  * independent choices among `choices` each (four commands of so many levels, or
  * one of many manoeuvres); over its heads

@@ -2488,6 +2488,17 @@ int mdn_op_dense_backward(const MdnDense* dense, const MdnDenseGrad* grad, void*
     return MDN_OK;
 }
 
+int mdn_op_dense_tiles(const MdnDense* dense, const MdnDenseGrad* grad, MdnDenseTile* tiles) {
+    dense::Args a;
+    dense::GradArgs d;
+    if (int rc = grad ? dense_grad_args("mdn_op_dense_tiles", dense, grad, &a, &d) : dense_args("mdn_op_dense_tiles", dense, &a)) return rc;
+    if (!tiles) return fail(MDN_E_ARG, "mdn_op_dense_tiles: null");
+    dense::Choice made[4];
+    dense::choices(a, grad ? &d : nullptr, made);
+    for (int i = 0; i < 4; i++) tiles[i] = MdnDenseTile{made[i].rows, made[i].step, made[i].parts};
+    return MDN_OK;
+}
+
 }  // extern "C"
 
 namespace {

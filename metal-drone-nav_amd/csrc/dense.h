@@ -27,6 +27,10 @@ struct GradArgs {
 // Bytes of workspace, by sizes, strides and addresses.
 uint64_t forward_bytes(const Args& a);
 uint64_t backward_bytes(const Args& a, const GradArgs& d);  // (which gradients are wanted, and d_y)
+// The tiles of the forward product, the arguments' gradients, d_x and the weights' gradients: their rows (0: no such
+// product, or the kernel of few rows), bytes of a step, pieces of the sum.
+struct Choice { uint32_t rows, step, parts; };
+void choices(const Args& a, const GradArgs* d, Choice (&to)[4]);
 hipError_t forward(const Args& a, char* work, hipStream_t st);
 hipError_t backward(const Args& a, const GradArgs& d, char* work, hipStream_t st);
 

@@ -610,17 +610,20 @@ Tile tile_of(bool bf, Kind kind, uint64_t m, uint64_t n, uint64_t k) {
     return best;
 }
 
+// Of products of rows by rows. Where there are more than two middle tiles a compute unit and few
+// steps, three tiles at once with half the LDS: 262,144 rows of 256 to 1,024, gated: 424 us, and
+// 478 with two; of 64: 220 and 267; but 32,768 of 2,560 to 5,120: 2,207 and 1,743.
+bool short_sum(uint64_t m, uint64_t n, uint64_t bytes, bool two) {
+    const uint64_t out = two ? 64 : 128;
+    return bytes <= 1024 && (m + 127) / 128 * ((n + out - 1) / out) > 2 * UNITS;
+}
+
 template <class T, bool MC, bool NC, int RESULT>
 hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
     if (tile == LARGE) return launch<T, 256, 256, 2, 2, 128, 2, true, MC, NC, RESULT>(a, batches, st);
-    if constexpr (!MC && !NC) {
-        // Where there are more than two middle tiles a compute unit and few steps, three
-        // tiles at once with half the LDS: 262,144 rows of 256 to 1,024, gated: 424 us, and
-        // 478 with two; of 64: 220 and 267; but 32,768 of 2,560 to 5,120: 2,207 and 1,743.
-        const uint64_t out = two_weights(RESULT) ? 64 : 128;
-        if (tile == MIDDLE && a.k * sizeof(T) <= 1024 && (a.m.count + 127ull) / 128 * ((a.n.count + out - 1) / out) > 2 * UNITS)
+    if constexpr (!MC && !NC)
+        if (tile == MIDDLE && short_sum(a.m.count, a.n.count, a.k * sizeof(T), two_weights(RESULT)))
             return launch<T, 128, 128, 2, 2, 64, 2, false, MC, NC, RESULT>(a, batches, st);
-    }
     if (tile == MIDDLE) return launch<T, 128, 128, 2, 2, 128, 2, false, MC, NC, RESULT>(a, batches, st);
     if constexpr (two_weights(RESULT))
         return launch<T, 64, 128, 2, 2, 128, 3, false, MC, NC, RESULT>(a, batches, st);
@@ -852,6 +855,22 @@ uint64_t forward_bytes(const Args& a) {
 uint64_t backward_bytes(const Args& a, const GradArgs& d) {
     const BackPlan p = back_plan_of(a, d);
     return p.x_bytes + pieces_of(a) * p.w_bytes + p.dz_bytes + p.sums_bytes + p.parts_bytes;
+}
+void choices(const Args& a, const GradArgs* d, Choice (&to)[4]) {
+    for (Choice& c : to) c = Choice{0, 0, 0};
+    if (a.rows == 0) return;
+    const auto choice = [](Tile t, uint32_t parts) { return Choice{t == LARGE ? 256u : t == MIDDLE ? 128u : 64u, 128, parts}; };
+    const auto forward = [&](const Plan& p) {
+        Choice c = choice(p.forward_tile, 1);
+        if (p.forward_tile == MIDDLE && short_sum(a.rows, a.out, uint64_t(p.in_ld) * p.size, a.gated)) c.step = 64;
+        return c;
+    };
+    if (!few_rows(a)) to[0] = forward(plan_of(a));
+    if (!d) return;
+    const BackPlan p = back_plan_of(a, *d);
+    if (p.slope) to[1] = forward(p);
+    if (d->d_x.p) to[2] = choice(p.dx_tile, 1);
+    if (d->d_w[0].p || d->d_w[1].p) to[3] = choice(p.dw_tile, p.splits);
 }
 hipError_t forward(const Args& a, char* work, hipStream_t st) {
     if (few_rows(a)) return forward_few(a, st);

@@ -32,8 +32,8 @@ EXPORTS = [
     "mdn_sim_get_camera", "mdn_ppo_grad_norm_summary", "mdn_lppo_grad_norm_summary", "mdn_op_delta_rule_forward",
     "mdn_op_delta_rule_backward", "mdn_op_delta_rule_sizes", "mdn_op_block_norm_forward", "mdn_op_block_norm_backward",
     "mdn_op_block_norm_workspace_bytes", "mdn_op_dense_forward_bytes", "mdn_op_dense_forward",
-    "mdn_op_dense_backward_bytes", "mdn_op_dense_backward", "mdn_op_choices_log_prob", "mdn_op_choices_loss_sizes",
-    "mdn_op_choices_loss_forward", "mdn_op_choices_loss_backward",
+    "mdn_op_dense_backward_bytes", "mdn_op_dense_backward", "mdn_op_dense_tiles", "mdn_op_choices_log_prob",
+    "mdn_op_choices_loss_sizes", "mdn_op_choices_loss_forward", "mdn_op_choices_loss_backward",
 ]
 
 P = ctypes.c_void_p
@@ -145,6 +145,7 @@ def lib():
         _sig(L, "mdn_op_dense_forward", I32, P, P, U64, P)
         _sig(L, "mdn_op_dense_backward_bytes", I32, P, P, ctypes.POINTER(U64))
         _sig(L, "mdn_op_dense_backward", I32, P, P, P, U64, P)
+        _sig(L, "mdn_op_dense_tiles", I32, P, P, P)
         _sig(L, "mdn_op_choices_log_prob", I32, P, P, P, P)
         _sig(L, "mdn_op_choices_loss_sizes", I32, P, ctypes.POINTER(U64), ctypes.POINTER(U64))
         _sig(L, "mdn_op_choices_loss_forward", I32, P, P, P, U64, P, U64, P)
