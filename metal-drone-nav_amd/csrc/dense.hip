@@ -583,7 +583,9 @@ hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
 // of 128 bytes of k alone on a compute unit and beside another tile, and what a
 // tile takes besides (1,024 x 2,048 x 2,048 in bfloat16: 18, 27 and 51 us on small,
 // middle and large tiles; 4,096 x 2,048 x 2,048: 58, 42 and 53; 32,768 x 5,120 to 1,280:
-// 775, 506 and 404; 262,144 x 256 to 1,024 with silu: 511, 316 and 360).
+// 775, 506 and 404; 262,144 x 256 to 1,024 with silu: 511, 316 and 360).  Large ones are
+// for bfloat16: in fp32 a step took 8.2 us, as the four middle tiles in its place do, and
+// the rest 20 where theirs is 12, so by this no size gains by them.
 enum Tile { SMALL, MIDDLE, LARGE };
 constexpr uint32_t UNITS = 256;
 struct Cost { uint32_t m, n; float alone, beside, rest; };
@@ -593,13 +595,13 @@ Cost cost_of(Tile t, bool bf, Kind kind) {
     switch (t) {
         case SMALL: return {64, 64, (bf ? 0.40f : 0.55f) * (two ? 1.6f : 1.0f), (bf ? 0.48f : 1.02f) * (two ? 1.8f : 1.0f), bf ? (two ? 2.2f : 1.8f) : 5.0f};
         case MIDDLE: return {128, two ? 64u : 128u, bf ? 0.72f : 2.1f, bf ? (two ? 1.05f : 1.15f) : 4.1f, bf ? (two ? 3.4f : plain ? 3.0f : 4.4f) : (two ? 2.0f : 6.0f)};
-        default: return {256, two ? 128u : 256u, bf ? 1.55f : 8.2f, bf ? 3.1f : 16.4f, bf ? (plain || two ? 9.0f : 15.0f) : (two ? 9.0f : 20.0f)};
+        default: return {256, two ? 128u : 256u, 1.55f, 3.1f, plain || two ? 9.0f : 15.0f};
     }
 }
 float time_of(Tile t, bool bf, Kind kind, uint64_t m, uint64_t n, uint64_t k, uint64_t times) {
     const Cost c = cost_of(t, bf, kind);
     const uint64_t tiles = (m + c.m - 1) / c.m * ((n + c.n - 1) / c.n) * times, each = (tiles + UNITS - 1) / UNITS;
-    if (tiles > MOST_TILES) return 1e30f;
+    if (tiles > MOST_TILES || (t == LARGE && !bf)) return 1e30f;
     const float steps = float((k * (bf ? 2 : 4) + 127) / 128), rest = t == LARGE ? 2.0f * c.rest : c.rest;
     return float(each / 2) * (steps * c.beside + rest) + (each & 1 ? steps * c.alone + c.rest : 0.0f);
 }
@@ -620,7 +622,8 @@ bool short_sum(uint64_t m, uint64_t n, uint64_t bytes, bool two) {
 
 template <class T, bool MC, bool NC, int RESULT>
 hipError_t product(const Job& a, Tile tile, uint32_t batches, hipStream_t st) {
-    if (tile == LARGE) return launch<T, 256, 256, 2, 2, 128, 2, true, MC, NC, RESULT>(a, batches, st);
+    if constexpr (sizeof(T) == 2)
+        if (tile == LARGE) return launch<T, 256, 256, 2, 2, 128, 2, true, MC, NC, RESULT>(a, batches, st);
     if constexpr (!MC && !NC)
         if (tile == MIDDLE && short_sum(a.m.count, a.n.count, a.k * sizeof(T), two_weights(RESULT)))
             return launch<T, 128, 128, 2, 2, 64, 2, false, MC, NC, RESULT>(a, batches, st);

@@ -4,10 +4,11 @@ Which tile a product gets is decided on the host, from sizes (mdn_op_dense_tiles
 gets; a change of the estimates behind that choice shows in a test that needs no GPU, so that no tile loses its tests
 unseen.  Tolerances are those of test_dense.py, whose formulas and inputs these are."""
 import ctypes
+import re
 
 import pytest
 import torch  # before the library: one HIP runtime in the process
-from test_dense import ACTS, BF16, F32, LEAVES, call, check, inputs
+from test_dense import ACTS, BF16, F32, LEAVES, SHAPES, call, check, inputs
 
 gpu = pytest.mark.gpu
 FORWARD, SLOPES, D_X, D_W = range(4)
@@ -214,3 +215,25 @@ def test_captured():
         torch.cuda.synchronize()
         for a, b in zip(captured, want):
             assert torch.equal(a, b)
+
+
+def test_every_kernel_is_reached():
+    """The product kernels in the library are those that the calls of this file and of test_dense.py launch: none is
+    built that no call reaches, and none is untested."""
+    from mdnav import native
+    LINEAR, GATED, SLOPE, GATED_SLOPE, STORE, PART = range(6)
+    calls = [(shape, dtype, gated, slope) for shape, dtype, gated, _ in TILES for slope in ([True] if gated else [True, False])]
+    for shape in SHAPES:
+        for dtype in (F32, BF16):
+            for i, gated in enumerate((False, True, False)):  # the activations that test_dense.py gives them
+                calls.append((shape, dtype, gated, gated or (i != 2 and list(ACTS)[(sum(shape) + 3 * i) % len(ACTS)] != "none")))
+    reached = set()
+    for shape, dtype, gated, slope in calls:
+        for i, (rows, step, parts) in enumerate(tiles(*shape, dtype, gated, slope)):
+            if rows:
+                result = [GATED if gated else LINEAR, GATED_SLOPE if gated else SLOPE, STORE, PART if parts > 1 else STORE][i]
+                reached.add((dtype, rows, step, i == D_W, i >= D_X, result))
+    with open(native.LIB_PATH, "rb") as f:
+        names = re.findall(rb"14product_kernelI(f|DF16b)Li(\d+)ELi\d+ELi\d+ELi\d+ELi(\d+)ELi\d+ELb[01]ELb([01])ELb([01])ELi(\d)E", f.read())
+    built = {(F32 if t == b"f" else BF16, int(rows), int(step), m == b"1", n == b"1", int(result)) for t, rows, step, m, n, result in names}
+    assert len(built) > 30 and built == reached, (built - reached, reached - built)
