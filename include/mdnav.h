@@ -590,8 +590,8 @@ int mdn_op_dense_tiles(const MdnDense* dense, const MdnDenseGrad* grad, MdnDense
  * Logits are fp32 or bfloat16, [steps][heads][choices] with strides of elements
  * and contiguous choices; exponentials and their sums are fp32, everything a
  * step makes of them is 64 bits, and so is the sum where r is so near to the
- * clip's border that 32 bits could not tell its side.  heads and choices are
- * at least 1, choices below 2^24, steps heads choices below 2^48. */
+ * clip's border that 32 bits could not tell its side.  heads are 1..65,536,
+ * choices 1..2^24 - 1, steps heads choices at most 2^48. */
 typedef struct MdnChoices {
     uint64_t steps;
     uint32_t heads, choices, dtype, action_bytes; /* action_bytes: 4 or 8 (int32_t, int64_t) */

@@ -322,8 +322,9 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     typedef Piece<TR, PW> Out;
     constexpr uint32_t N = Out::N;
     constexpr bool SLOPES = RESULT == SLOPE || RESULT == GATED_SLOPE;
-    // (32,768 x 2,560 to 5,120, gated: 1,387 us, and 1,458 with y by way of the caches; its
-    // slopes 1,512, and 1,635 with dy and dz by way of them.)
+    // (With gelu 32,768 x 2,560 to 5,120, gated: 1,387 us, and 1,458 with y by way of the caches; its slopes 1,512, and
+    // 1,635 with dy and dz by way of them.  With silu 1,345 and 1,442; a quarter of the rows 346 and 355, with all
+    // gradients 1,564 and 1,547; 14,374 x 203 to 3,935 123 and 127; 49,596 x 304 to 66 22 either way.)
     constexpr bool ONCE = BM == 256 && RESULT != STORE && RESULT != PART;
     constexpr uint32_t BESIDE = (N2 ? 2 : 1) * Out::BYTES;
     char* own = shared + wave * REGION;
@@ -585,7 +586,8 @@ hipError_t launch(Job a, uint32_t batches, hipStream_t st) {
 // middle and large tiles; 4,096 x 2,048 x 2,048: 58, 42 and 53; 32,768 x 5,120 to 1,280:
 // 775, 506 and 404; 262,144 x 256 to 1,024 with silu: 511, 316 and 360).  Large ones are
 // for bfloat16: in fp32 a step took 8.2 us, as the four middle tiles in its place do, and
-// the rest 20 where theirs is 12, so by this no size gains by them.
+// the rest 20 where theirs is 12, so by this no size gains by them.  Middle ones have one
+// set of numbers for both of their kernels (short_sum).
 enum Tile { SMALL, MIDDLE, LARGE };
 constexpr uint32_t UNITS = 256;
 struct Cost { uint32_t m, n; float alone, beside, rest; };
@@ -613,8 +615,10 @@ Tile tile_of(bool bf, Kind kind, uint64_t m, uint64_t n, uint64_t k) {
 }
 
 // Of products of rows by rows. Where there are more than two middle tiles a compute unit and few
-// steps, three tiles at once with half the LDS: 262,144 rows of 256 to 1,024, gated: 424 us, and
-// 478 with two; of 64: 220 and 267; but 32,768 of 2,560 to 5,120: 2,207 and 1,743.
+// steps, three tiles at once with half the LDS. In bfloat16, 131,072 rows to 1,024, gated: of 64
+// 109 us, and 130 with two; of 256 211 and 245; of 512 334 and 333; not gated: 114 and 100, 166 and 168,
+// 221 and 236. In fp32, 65,536 rows to 512: of 64 66 and 72, of 256 153 and 161, of 512, past the limit, 271
+// and 281. Long sums are slower: 32,768 of 2,560 to 5,120, gated, in bfloat16: 2,207 and 1,743.
 bool short_sum(uint64_t m, uint64_t n, uint64_t bytes, bool two) {
     const uint64_t out = two ? 64 : 128;
     return bytes <= 1024 && (m + 127) / 128 * ((n + out - 1) / out) > 2 * UNITS;

@@ -1,11 +1,12 @@
 // dense_rows.hip — the forward call of few rows: a tick of a few vehicles, whose
-// cost is reading the weights once.
+// cost is reading the weights.
 //
 // A workgroup makes up to 16 columns of the result for up to 16 MT rows.  Its W
 // wavefronts take turns along k, 128 bytes of each of the weight rows at a time
 // (whole lines, straight to registers, UNROLL of them on their way), as operands
-// of 16 x 16 tiles; their sums meet in LDS.  Bound by memory: one row of 5,120 to
-// 65,536 in bfloat16 reads its weights at 5.4 TB/s.
+// of 16 x 16 tiles; their sums meet in LDS.  The weights are read once for every 32
+// rows.  Bound by memory: one row of 5,120 to 65,536 in bfloat16 reads its weights at
+// 5.4 TB/s.
 #include "dense.h"
 
 #include "dense_tiles.h"
@@ -148,10 +149,13 @@ template <class T, bool G> hipError_t by_rows(const Args& a, bool words, hipStre
 
 }  // namespace
 
-// Up to where this is faster than tiles: 64 rows in bfloat16 and 128 in fp32, more
-// where the weights are small. In bfloat16, 64 rows of 1,024 to 1,024: 6.9 us here and 7.2
-// on tiles, 128: 11.3 and 7.2; of 184 to 256, 256 rows: 3.0 and 3.5, 512: 3.7 and 3.6. In fp32, 128
-// rows of 1,024 to 1,024: 24 and 33, 256: 41 and 34; of 181 to 333, 512 rows: 11.8 and 12.4.
+// Up to about where this is faster than tiles: 64 rows in bfloat16 and 128 in fp32, more
+// where the weights are small. In bfloat16, 64 rows of 1,024 to 1,024: 7.1 us here and 7.5
+// on tiles, 96: 9.5 and 7.5; of 256 to 1,024: 3.7 and 4.0, 4.4 and 4.1; of 5,120 to 1,280, 48 rows: 22.2 and
+// 25.0, 64: 25.5 and 25.0; of 184 to 256, 256 rows: 3.0 and 3.5, 512: 3.7 and 3.6. In fp32, 128 rows of
+// 1,024 to 1,024: 25 and 34, 192: 36 and 34; of 2,048 to 2,048, 128 rows: 51 and 65, 192: 78 and 65; of 181 to
+// 333, 512 rows: 12.3 and 12.9.  Where there are as many columns as tiles need, in bfloat16, tiles are faster
+// from fewer rows on, and the rule does not know it: of 5,120 to 5,120, 32 rows: 34 and 27, 64: 58 and 30.
 bool few_rows(const Args& a) {
     const bool small = uint64_t(a.in) * a.out * (a.gated ? 2 : 1) <= 1u << 16;
     return a.rows <= (a.bf ? (small ? 256u : 64u) : (small ? 512u : 128u));

@@ -353,7 +353,8 @@ def clipped_loss(logits, actions, old_log_prob, advantages, ref_log_prob=None, m
     """The clipped loss of a policy over discrete choices: (loss, metrics).
 
     logits: [..., heads, choices], float32 or bfloat16: the independent choices
-    of a step, four commands of so many levels or one of many manoeuvres.
+    of a step, four commands of so many levels or one of many manoeuvres, 1 to
+    65,536 heads of below 2^24 choices.
     actions: [..., heads] int64 or int32.  old_log_prob, advantages,
     ref_log_prob: [...] float32, mask: [...] bool or uint8.  With l the sum of
     the heads' log-probabilities, H that of their entropies,
